@@ -7,7 +7,8 @@ framework's entry points.  Seven kinds:
 
   embed_fwd   out[r] = scale * table[ids[r]]                       (an id outside the table: a row of zeros)
   embed_bwd   d_table[v] = scale * sum over r with ids[r] = v of d_out[r]
-  logp        of each row of logits / temperature: log sum exp, log p(target), entropy, the k most likely tokens
+  logp        of each row of logits / temperature: log sum exp in two parts (largest, log of the sum above it), log p(target),
+              entropy, the k most likely tokens
   logp_bwd    gradient of the logits from those of log p(target) and of the entropy
   scan        u = sigmoid(-f), h_t = h_{t-1} + u_t (x_t - h_{t-1}), y_t = h_t * SiLU(z_t)
   scan_bwd    gradients of x, f, z and of the state that entered, from those of y and of the state that left
@@ -139,9 +140,12 @@ def prepare(case, seed):
         s.update(logits=logits, targets=targets, temperature=c["temperature"], top=c.get("top", 0))
         if kind == "logp_bwd":  # what the forward left, and the gradients of its results
             l = logits.float() / c["temperature"]
-            s["lse"] = torch.logsumexp(l, 1)
-            p = torch.exp(l - torch.where(torch.isinf(s["lse"]), 0.0, s["lse"])[:, None])
-            s["entropy"] = torch.where(torch.isinf(s["lse"]), 0.0, s["lse"]) - (p * torch.where(p > 0, l, 0.0)).sum(1)
+            m = l.amax(1)
+            d = l - torch.where(torch.isinf(m), 0.0, m)[:, None]
+            e = torch.exp(d)
+            S = torch.where(torch.isinf(m), 1.0, e.sum(1))
+            s["lse"] = torch.stack([m, torch.log(S)])
+            s["entropy"] = torch.log(S) - (e * torch.where(e > 0, d, 0.0)).sum(1) / S
             s.update(d_logprob=rn(c["rows"]).div_(c["rows"]), d_entropy=torch.full((c["rows"],), 0.01 / c["rows"], device=dev))
     else:
         B, T, D, w = c["B"], c["T"], c["D"], 3 if c["z"] else 2
@@ -224,17 +228,18 @@ def _run_plain(s):
             m = l.amax(1, keepdim=True)
             d = l - torch.where(torch.isinf(m), 0.0, m)  # (a row with nothing left is -inf throughout)
             e = torch.exp(d)
-            S = e.sum(1, keepdim=True)
-            lse = m + torch.log(torch.where(S > 0, S, 1.0))
-            H = torch.where(S > 0, torch.log(S) - (e * torch.where(e > 0, d, 0.0)).sum(1, keepdim=True) / S, 0.0)
-            logp = l.gather(1, t) - torch.where(S > 0, lse, 0.0)
-            out = dict(lse=lse[:, 0], entropy=H[:, 0], logprob=torch.where(ok, logp[:, 0], 0.0))
+            S = torch.where(torch.isinf(m), 1.0, e.sum(1, keepdim=True))
+            log_s = torch.log(S)
+            H = log_s - (e * torch.where(e > 0, d, 0.0)).sum(1, keepdim=True) / S
+            out = dict(lse=torch.stack([m[:, 0], log_s[:, 0]]), entropy=H[:, 0],
+                       logprob=torch.where(ok, (d.gather(1, t) - log_s)[:, 0], 0.0))
             if s["top"]:
-                v, i = torch.sort(s["logits"].float(), dim=1, descending=True, stable=True)
-                out.update(top_ids=i[:, :s["top"]].int(), top_logprobs=v[:, :s["top"]] / s["temperature"] - torch.where(S > 0, lse, 0.0))
+                i = torch.sort(s["logits"].float(), dim=1, descending=True, stable=True)[1]
+                out.update(top_ids=i[:, :s["top"]].int(), top_logprobs=d.gather(1, i[:, :s["top"]]) - log_s)
             return out
-        some = ~torch.isinf(s["lse"])
-        logp = torch.where(some[:, None], l - s["lse"][:, None], -math.inf)
+        m, log_s = s["lse"]
+        some = ~torch.isinf(m)
+        logp = torch.where(some[:, None], l - m[:, None] - log_s[:, None], -math.inf)
         p = torch.exp(logp)
         g = torch.where(ok & some, s["d_logprob"], 0.0)[:, None]
         d = -p * (g + s["d_entropy"][:, None] * torch.where(p > 0, logp + s["entropy"][:, None], 0.0))
@@ -287,7 +292,8 @@ def exact(case, seed):
         parts = [_exact_rows(case, s, r, min(r + 256, case["rows"])) for r in range(0, case["rows"], 256)]
         if kind == "logp_bwd":
             return torch.cat(parts)
-        return {k: torch.cat([p[k] for p in parts]) for k in parts[0]}
+        out = {k: torch.cat([p[k] for p in parts]) for k in parts[0]}
+        return {**out, "lse": out["lse"].T.contiguous()}
     # step by step
     B, T, D = case["B"], case["T"], case["D"]
     rows = lambda t: None if t is None else t.double().reshape(B, T, D)  # noqa: E731
@@ -321,7 +327,7 @@ def _exact_rows(case, s, r0, r1):
     l, t = s["logits"][r0:r1].double() / case["temperature"], s["targets"][r0:r1].long()
     counted = (t >= 0) & (t < case["vocab"])
     lse = torch.logsumexp(l, 1)
-    empty = torch.isinf(lse)
+    empty, m = torch.isinf(lse), l.amax(1)
     p = torch.softmax(l, 1).nan_to_num(0.0)
     logp = (l - lse[:, None]).masked_fill(empty[:, None], -math.inf)
     H = -(p * logp.masked_fill(p == 0, 0.0)).sum(1)
@@ -329,7 +335,7 @@ def _exact_rows(case, s, r0, r1):
     hot[counted, t[counted]] = 1.0
     if case["kind"] == "logp":
         own_logp = logp.gather(1, t.clamp(min=0)[:, None])[:, 0].masked_fill(~counted, 0.0)
-        out = dict(lse=lse, entropy=H, logprob=own_logp)
+        out = dict(lse=torch.stack([m, (lse - m).masked_fill(empty, 0.0)], 1), entropy=H, logprob=own_logp)
         if case["top"]:
             order = torch.argsort(-l, dim=1, stable=True)[:, :case["top"]]
             out.update(top_ids=order.int(), top_logprobs=logp.gather(1, order))
@@ -363,8 +369,8 @@ def work(case):
     if kind in ("logp", "logp_bwd"):
         n = c["rows"] * c["vocab"]
         if kind == "logp":
-            return {"bytes": e * n + c["rows"] * (16.0 + 8.0 * c["top"]), "flops": 6.0 * n}
-        return {"bytes": 2.0 * e * n + c["rows"] * 20.0, "flops": 8.0 * n}
+            return {"bytes": e * n + c["rows"] * (20.0 + 8.0 * c["top"]), "flops": 6.0 * n}
+        return {"bytes": 2.0 * e * n + c["rows"] * 24.0, "flops": 8.0 * n}
     n, b = c["B"] * c["T"] * c["D"], c["B"] * c["D"]
     gates = 3 if c["z"] else 2
     if kind != "scan_bwd":
