@@ -7,8 +7,8 @@ framework's entry points.  Seven kinds:
 
   embed_fwd   out[r] = scale * table[ids[r]]                       (an id outside the table: a row of zeros)
   embed_bwd   d_table[v] = scale * sum over r with ids[r] = v of d_out[r]
-  logp        of each row of logits / temperature: log sum exp in two parts (largest, log of the sum above it), log p(target),
-              entropy, the k most likely tokens
+  logp        of each row of logits / temperature: log sum exp in two parts (largest logit, log of the sum of exponentials
+              beside it), log p(target), entropy, the k most likely tokens
   logp_bwd    gradient of the logits from those of log p(target) and of the entropy
   scan        u = sigmoid(-f), h_t = h_{t-1} + u_t (x_t - h_{t-1}), y_t = h_t * SiLU(z_t)
   scan_bwd    gradients of x, f, z and of the state that entered, from those of y and of the state that left
@@ -139,9 +139,9 @@ def prepare(case, seed):
         logits, targets = _logits(c, dev, g)
         s.update(logits=logits, targets=targets, temperature=c["temperature"], top=c.get("top", 0))
         if kind == "logp_bwd":  # what the forward left, and the gradients of its results
-            l = logits.float() / c["temperature"]
+            l = logits.float()
             m = l.amax(1)
-            d = l - torch.where(torch.isinf(m), 0.0, m)[:, None]
+            d = (l - torch.where(torch.isinf(m), 0.0, m)[:, None]) / c["temperature"]
             e = torch.exp(d)
             S = torch.where(torch.isinf(m), 1.0, e.sum(1))
             s["lse"] = torch.stack([m, torch.log(S)])
@@ -220,13 +220,13 @@ def _run_plain(s):
         rows = torch.where(ok[:, None], s["d_out"].float() * s["scale"], 0.0)
         return torch.zeros(s["vocab"], rows.shape[1], device=rows.device).index_add_(0, torch.where(ok, ids, 0), rows)
     if kind in ("logp", "logp_bwd"):
-        l = s["logits"].float() / s["temperature"]
+        l = s["logits"].float()
         V, t = l.shape[1], s["targets"].long()
         ok = (t >= 0) & (t < V)
         t = torch.where(ok, t, 0)[:, None]
         if kind == "logp":
             m = l.amax(1, keepdim=True)
-            d = l - torch.where(torch.isinf(m), 0.0, m)  # (a row with nothing left is -inf throughout)
+            d = (l - torch.where(torch.isinf(m), 0.0, m)) / s["temperature"]  # (a row with nothing left is -inf throughout)
             e = torch.exp(d)
             S = torch.where(torch.isinf(m), 1.0, e.sum(1, keepdim=True))
             log_s = torch.log(S)
@@ -234,12 +234,12 @@ def _run_plain(s):
             out = dict(lse=torch.stack([m[:, 0], log_s[:, 0]]), entropy=H[:, 0],
                        logprob=torch.where(ok, (d.gather(1, t) - log_s)[:, 0], 0.0))
             if s["top"]:
-                i = torch.sort(s["logits"].float(), dim=1, descending=True, stable=True)[1]
+                i = torch.sort(l, dim=1, descending=True, stable=True)[1]
                 out.update(top_ids=i[:, :s["top"]].int(), top_logprobs=d.gather(1, i[:, :s["top"]]) - log_s)
             return out
         m, log_s = s["lse"]
         some = ~torch.isinf(m)
-        logp = torch.where(some[:, None], l - m[:, None] - log_s[:, None], -math.inf)
+        logp = torch.where(some[:, None], (l - m[:, None]) / s["temperature"] - log_s[:, None], -math.inf)
         p = torch.exp(logp)
         g = torch.where(ok & some, s["d_logprob"], 0.0)[:, None]
         d = -p * (g + s["d_entropy"][:, None] * torch.where(p > 0, logp + s["entropy"][:, None], 0.0))
@@ -335,7 +335,7 @@ def _exact_rows(case, s, r0, r1):
     hot[counted, t[counted]] = 1.0
     if case["kind"] == "logp":
         own_logp = logp.gather(1, t.clamp(min=0)[:, None])[:, 0].masked_fill(~counted, 0.0)
-        out = dict(lse=torch.stack([m, (lse - m).masked_fill(empty, 0.0)], 1), entropy=H, logprob=own_logp)
+        out = dict(lse=torch.stack([m * case["temperature"], (lse - m).masked_fill(empty, 0.0)], 1), entropy=H, logprob=own_logp)
         if case["top"]:
             order = torch.argsort(-l, dim=1, stable=True)[:, :case["top"]]
             out.update(top_ids=order.int(), top_logprobs=logp.gather(1, order))
