@@ -563,6 +563,89 @@ typedef struct mamba_b200_decode_args {
 MAMBA_B200_API long long mamba_b200_decode_workspace_bytes(void* handle, const mamba_b200_decode_args* args);
 MAMBA_B200_API int mamba_b200_decode_step(void* handle, void* stream, const mamba_b200_decode_args* args);
 
+/*
+ * The token table with scaling, and its gradient (no kernel counterpart in the reference, whose embedding and tied head
+ * are one [vocab, d_model] table, src/module/gpu_lm.rs:560-679).
+ *   fwd: out[r, :] = scale * table[ids[r], :], one rounding; table [vocab, ld_table] in `dtype`, out [rows, ld_out] f32 or
+ *        `dtype`.  An id outside [0, vocab) gives a row of zeros.
+ *   bwd: d_table[v, :] = scale * (sum over the rows r with ids[r] = v of d_out[r, :]), added to what d_table holds when
+ *        accumulate is not 0, else written, zeros included.  d_out [rows, ld_dout] in `dtype`, d_table [vocab, dim] f32
+ *        contiguous.  Sums run in f32 in an order that depends on the sizes and ids alone (no atomics on values): the same
+ *        inputs give the same bits.  An id outside [0, vocab) counts nowhere.  workspace: 256-byte aligned,
+ *        mamba_b200_embedding_bwd_workspace_bytes(...) bytes (may be 0); nothing in it is kept between calls.
+ */
+MAMBA_B200_API int mamba_b200_embedding_fwd(void* handle, void* stream, int dtype, const void* table, long long ld_table,
+                                            const int* ids, int out_dtype, void* out, long long ld_out, long long rows, int dim,
+                                            int vocab, float scale);
+MAMBA_B200_API long long mamba_b200_embedding_bwd_workspace_bytes(long long rows, int dim, int vocab);
+MAMBA_B200_API int mamba_b200_embedding_bwd(void* handle, void* stream, int dtype, const void* d_out, long long ld_dout,
+                                            const int* ids, float* d_table, int accumulate, long long rows, int dim, int vocab,
+                                            float scale, void* workspace, long long workspace_bytes);
+
+/*
+ * Log probabilities of given tokens, entropy and the most likely alternatives, per row of logits [rows, ld] (V used columns,
+ * storage dtype); l = logits / temperature, all sums f32.
+ *   lse [2, rows]: a row's largest logit M, and log sum exp(l - M / temperature): log sum exp l is M / temperature + the second
+ *   logprob[r] = l[targets[r]] - log sum exp l (0 where the target is outside [0, V))
+ *   entropy[r] = log sum exp l - sum p l
+ *   top_ids / top_logprobs [rows, top]: by falling logit, equal ones by rising index
+ * lse, entropy, logprob and targets may be NULL (logprob needs targets); 0 <= top <= 32, top <= V.
+ * A logit of minus infinity is a token that is ruled out.  Where a whole row is: lse is minus infinity and 0, the log
+ * probabilities are minus infinity, the entropy is 0, the alternatives are the lowest indices.  A NaN or plus infinity makes its row's values NaN;
+ * among the alternatives NaN ranks as minus infinity.
+ * bwd: dlogits[v] = (d_logprob (1[v = target] - p_v) - d_entropy p_v (log p_v + entropy)) / temperature from lse and entropy
+ * as the forward left them; d_logprob or d_entropy may be NULL (no such part), dlogits may be the logits themselves.  The
+ * log probabilities of the alternatives have no gradient here.
+ */
+MAMBA_B200_API int mamba_b200_token_logprobs(void* handle, void* stream, int dtype, const void* logits, long long ld,
+                                             const int* targets, float temperature, float* lse, float* entropy, float* logprob,
+                                             int top, int* top_ids, float* top_logprobs, long long rows, int V);
+MAMBA_B200_API int mamba_b200_token_logprobs_bwd(void* handle, void* stream, int dtype, const void* logits, long long ld,
+                                                 const int* targets, float temperature, const float* lse, const float* entropy,
+                                                 const float* d_logprob, const float* d_entropy, void* dlogits, long long ld_d,
+                                                 long long rows, int V);
+
+/*
+ * Gated linear recurrence over [B, T, D], elementwise over channels, forward and backward:
+ *   u_t = sigmoid(-f_t)     h_t = h_{t-1} + u_t (x_t - h_{t-1})     y_t = h_t * SiLU(z_t)   (z NULL: y = h)
+ * x, f, z, y and the gradients in the storage dtype with row strides (x, f, z may be columns of one projection); states
+ * [B, D] f32.  T = 1 is the decode step.  T = 0 hands the state on.
+ *   forward : h0 (NULL: zeros) enters, h_last (NULL: not written; may be h0) leaves.  chunk_states (NULL: not kept)
+ *             [B, ceil(T / MAMBA_B200_GATED_SCAN_SAVE), D] f32: the state that enters each block of that many steps, which is
+ *             what the backward needs.
+ *   backward: by recomputation from chunk_states.  d_last (NULL: zeros) is the gradient of the state that left, d_h0
+ *             (NULL: not written; may be d_last) that of the state that entered; d_x, d_f and, with z, d_z are overwritten.
+ */
+#define MAMBA_B200_GATED_SCAN_SAVE 64
+typedef struct mamba_b200_gated_scan_args {
+    int dtype;
+    int B, T, D;
+    const void* x;       /* [B*T, ld_x] */
+    long long ld_x;
+    const void* f;       /* [B*T, ld_f]: forget gate before its sigmoid */
+    long long ld_f;
+    const void* z;       /* [B*T, ld_z] or NULL */
+    long long ld_z;
+    const float* h0;
+    float* h_last;
+    void* y;             /* forward [B*T, ld_y] */
+    long long ld_y;
+    float* chunk_states;
+    const void* dy;      /* backward from here */
+    long long ld_dy;
+    const float* d_last;
+    float* d_h0;
+    void* d_x;
+    long long ld_dx;
+    void* d_f;
+    long long ld_df;
+    void* d_z;
+    long long ld_dz;
+} mamba_b200_gated_scan_args;
+
+MAMBA_B200_API int mamba_b200_gated_scan_fwd(void* handle, void* stream, const mamba_b200_gated_scan_args* args);
+MAMBA_B200_API int mamba_b200_gated_scan_bwd(void* handle, void* stream, const mamba_b200_gated_scan_args* args);
+
 #ifdef __cplusplus
 }
 #endif

@@ -122,6 +122,20 @@ class DecodeArgs(C.Structure):
     ]
 
 
+class GatedScanArgs(C.Structure):
+    _fields_ = [
+        ("dtype", C.c_int), ("B", C.c_int), ("T", C.c_int), ("D", C.c_int),
+        ("x", C.c_void_p), ("ld_x", C.c_longlong), ("f", C.c_void_p), ("ld_f", C.c_longlong),
+        ("z", C.c_void_p), ("ld_z", C.c_longlong),
+        ("h0", C.c_void_p), ("h_last", C.c_void_p), ("y", C.c_void_p), ("ld_y", C.c_longlong), ("chunk_states", C.c_void_p),
+        ("dy", C.c_void_p), ("ld_dy", C.c_longlong), ("d_last", C.c_void_p), ("d_h0", C.c_void_p),
+        ("d_x", C.c_void_p), ("ld_dx", C.c_longlong), ("d_f", C.c_void_p), ("ld_df", C.c_longlong),
+        ("d_z", C.c_void_p), ("ld_dz", C.c_longlong),
+    ]
+
+
+GATED_SCAN_SAVE = 64  # MAMBA_B200_GATED_SCAN_SAVE
+
 _lib = None
 
 
@@ -175,6 +189,13 @@ def lib() -> C.CDLL:
         bind("mamba_b200_embedding_gather", [vp, vp, it, vp, vp, vp, ll, it, it])
         bind("mamba_b200_softmax_xent", [vp, vp, it, vp, vp, vp, vp, fl, ll, it, ll])
         bind("mamba_b200_adamw_step", [vp, vp, vp, vp, vp, vp, fl, fl, fl, fl, fl, vp, vp, it, ll])
+        bind("mamba_b200_embedding_fwd", [vp, vp, it, vp, ll, vp, it, vp, ll, ll, it, it, fl])
+        bind("mamba_b200_embedding_bwd_workspace_bytes", [ll, it, it], ll)
+        bind("mamba_b200_embedding_bwd", [vp, vp, it, vp, ll, vp, vp, it, ll, it, it, fl, vp, ll])
+        bind("mamba_b200_token_logprobs", [vp, vp, it, vp, ll, vp, fl, vp, vp, vp, it, vp, vp, ll, it])
+        bind("mamba_b200_token_logprobs_bwd", [vp, vp, it, vp, ll, vp, fl, vp, vp, vp, vp, vp, ll, ll, it])
+        bind("mamba_b200_gated_scan_fwd", [vp, vp, C.POINTER(GatedScanArgs)])
+        bind("mamba_b200_gated_scan_bwd", [vp, vp, C.POINTER(GatedScanArgs)])
         bind("mamba_b200_decode_workspace_bytes", [vp, C.POINTER(DecodeArgs)], ll)
         bind("mamba_b200_decode_step", [vp, vp, C.POINTER(DecodeArgs)])
         bind("mamba_b200_m3_ssd_fwd", [vp, vp, C.POINTER(M3SsdArgs)])

@@ -18,7 +18,9 @@ from . import ffi
 __all__ = ["selective_scan_fwd", "selective_scan_fwd_workspace_bytes", "selective_scan_bwd",
            "selective_scan_bwd_workspace_bytes",
            "residual_rmsnorm_fwd", "residual_rmsnorm_bwd", "embedding_gather", "softmax_xent", "adamw_step",
-           "ssm_parallel_scan_fwd_nosave", "ssm_scan_fwd_save", "ssm_scan_bwd", "conv1d_fwd_nosave", "selective_scan_step", "conv1d_fwd", "conv1d_bwd", "m3_ssd_fwd", "m3_ssd_fwd_fused_kq", "m3_ssd_bwd", "dtype_code"]
+           "ssm_parallel_scan_fwd_nosave", "ssm_scan_fwd_save", "ssm_scan_bwd", "conv1d_fwd_nosave", "selective_scan_step", "conv1d_fwd", "conv1d_bwd", "m3_ssd_fwd", "m3_ssd_fwd_fused_kq", "m3_ssd_bwd", "dtype_code",
+           "embedding_fwd", "embedding_bwd", "embedding_bwd_workspace_bytes", "token_logprobs", "token_logprobs_bwd",
+           "gated_scan_fwd", "gated_scan_bwd", "gated_scan_step", "gated_scan_states"]
 
 
 _DTYPES = {torch.float32: ffi.F32, torch.float16: ffi.F16, torch.bfloat16: ffi.BF16}
@@ -568,3 +570,222 @@ def adamw_step(param, grad, m, v, bias_factors, *, lr, beta1=0.9, beta2=0.999, e
                                              param.numel())
     h.check(rc, "mamba_b200_adamw_step")
     return param
+
+
+def _same_device(dev, *named):
+    for t, nm in named:
+        if t is not None and t.device != dev:
+            raise ValueError(f"{nm} is on {t.device}, not on {dev}")
+
+
+def embedding_fwd(table, ids, *, scale=1.0, out=None, out_dtype=torch.float32, handle=None):
+    """out [rows, dim] = scale * table[ids]: table [vocab, dim] in the storage dtype (any row stride), ids int32 of any
+    shape; out in float32 (the residual stream) or the table's dtype.  An id outside the table gives a row of zeros."""
+    _require_cuda(table, ids, out)
+    dev = table.device
+    if table.dim() != 2 or table.stride(1) != 1 or ids.dtype != torch.int32 or not ids.is_contiguous():
+        raise TypeError("the table is [vocab, dim] with contiguous rows, ids are contiguous int32")
+    vocab, dim = table.shape
+    rows = ids.numel()
+    if out is None:
+        out = torch.empty((rows, dim), dtype=out_dtype, device=dev)
+    elif tuple(out.shape) != (rows, dim) or out.stride(1) != 1:
+        raise ValueError(f"out is [{rows}, {dim}] with contiguous rows")
+    _same_device(dev, (ids, "ids"), (out, "out"))
+    h = handle or ffi.default_handle(dev.index or 0)
+    with _on(dev):
+        rc = ffi.lib().mamba_b200_embedding_fwd(h.ptr, _stream(dev), dtype_code(table.dtype), table.data_ptr(),
+                                                max(table.stride(0), dim), ids.data_ptr(), dtype_code(out.dtype), out.data_ptr(),
+                                                max(out.stride(0), dim), rows, dim, vocab, scale)
+    h.check(rc, "mamba_b200_embedding_fwd")
+    return out
+
+
+def embedding_bwd_workspace_bytes(rows, dim, vocab) -> int:
+    """Bytes of scratch the table's gradient needs (rows sorted by token, sums of rows that go on)."""
+    return int(ffi.lib().mamba_b200_embedding_bwd_workspace_bytes(rows, dim, vocab))
+
+
+def embedding_bwd(ids, d_out, vocab=None, *, d_table=None, scale=1.0, workspace=None, handle=None):
+    """Gradient of embedding_fwd's table: scale * the sums of d_out's rows by token, f32 [vocab, dim].  Accumulated into
+    d_table when it is given, else a fresh tensor.  ids int32 of any shape, d_out [ids.numel(), dim] in a storage dtype (any
+    row stride).  The order of the sums is fixed: the same inputs give the same bits."""
+    _require_cuda(ids, d_out, d_table, workspace)
+    dev = d_out.device
+    rows = ids.numel()
+    if ids.dtype != torch.int32 or not ids.is_contiguous():
+        raise TypeError("ids are contiguous int32")
+    if d_out.dim() != 2 or d_out.shape[0] != rows or d_out.stride(1) != 1:
+        raise ValueError(f"d_out is [{rows}, dim] with contiguous rows")
+    dim = d_out.shape[1]
+    accumulate = d_table is not None
+    if accumulate:
+        if d_table.dtype != torch.float32 or not d_table.is_contiguous():
+            raise TypeError("d_table is contiguous float32")
+        if d_table.dim() != 2 or d_table.shape[1] != dim or (vocab is not None and vocab != d_table.shape[0]):
+            raise ValueError(f"d_table is [vocab, {dim}], not {list(d_table.shape)}")
+        vocab = d_table.shape[0]
+    elif vocab is None:
+        raise ValueError("the vocabulary's size or a table to accumulate into is needed")
+    else:
+        d_table = torch.empty((vocab, dim), dtype=torch.float32, device=dev)
+    lib = ffi.lib()
+    if workspace is None:
+        workspace = torch.empty(lib.mamba_b200_embedding_bwd_workspace_bytes(rows, dim, vocab), dtype=torch.uint8, device=dev)
+    _same_device(dev, (ids, "ids"), (d_table, "d_table"), (workspace, "workspace"))
+    h = handle or ffi.default_handle(dev.index or 0)
+    with _on(dev):
+        rc = lib.mamba_b200_embedding_bwd(h.ptr, _stream(dev), dtype_code(d_out.dtype), d_out.data_ptr(), max(d_out.stride(0), dim),
+                                          ids.data_ptr(), d_table.data_ptr(), accumulate, rows, dim, vocab, scale,
+                                          workspace.data_ptr(), workspace.numel() * workspace.element_size())
+    h.check(rc, "mamba_b200_embedding_bwd")
+    return d_table
+
+
+def _logit_rows(logits, targets):
+    if logits.dim() != 2 or logits.stride(1) != 1:
+        raise TypeError("logits are [rows, V] with contiguous rows")
+    if targets is not None and (targets.dtype != torch.int32 or not targets.is_contiguous() or targets.numel() != logits.shape[0]):
+        raise TypeError(f"targets are {logits.shape[0]} contiguous int32")
+
+
+def token_logprobs(logits, targets=None, *, top=0, temperature=1.0, handle=None):
+    """Per row of logits [rows, V] / temperature: dict(entropy [rows], lse [2, rows]), with targets (int32 [rows]; outside
+    the vocabulary: not counted, 0) also logprob [rows], all f32; with top > 0 (at most 32) also top_ids int32 and
+    top_logprobs f32 [rows, top], by falling probability, equal ones by rising index.  lse holds the largest
+    logit M and the log of the sum of exp((logits - M) / temperature): the log-sum-exp is M / temperature plus that.  Logits of -inf are tokens that are ruled out."""
+    _require_cuda(logits, targets)
+    _logit_rows(logits, targets)
+    rows, V = logits.shape
+    dev = logits.device
+    _same_device(dev, (targets, "targets"))
+    h = handle or ffi.default_handle(dev.index or 0)
+    if not 0 <= top <= min(32, V):
+        raise ValueError(f"{top} alternatives of {V} tokens (at most 32)")
+    res = torch.empty((3 if targets is None else 4, rows), dtype=torch.float32, device=dev)
+    base = res.data_ptr()
+    out = dict(lse=res[:2], entropy=res[2])
+    if targets is not None:
+        out["logprob"] = res[3]
+    ip = vp = None
+    if top:
+        ids, val = torch.empty((rows, top), dtype=torch.int32, device=dev), torch.empty((rows, top), dtype=torch.float32, device=dev)
+        ip, vp = ids.data_ptr(), val.data_ptr()
+        out["top_ids"], out["top_logprobs"] = ids, val
+    with _on(dev):
+        rc = ffi.lib().mamba_b200_token_logprobs(h.ptr, _stream(dev), dtype_code(logits.dtype), logits.data_ptr(),
+                                                 max(logits.stride(0), V), _ptr(targets), temperature, base, base + 8 * rows,
+                                                 None if targets is None else base + 12 * rows, top, ip, vp, rows, V)
+    h.check(rc, "mamba_b200_token_logprobs")
+    return out
+
+
+def token_logprobs_bwd(logits, targets, lse, entropy, d_logprob=None, d_entropy=None, *, temperature=1.0, dlogits=None,
+                       handle=None):
+    """Gradient of the logits from those of logprob and entropy (f32 [rows], either may be None), with lse and entropy as
+    token_logprobs returned them.  dlogits in the logits' dtype; it may be the logits themselves."""
+    _require_cuda(logits, targets, lse, entropy, d_logprob, d_entropy, dlogits)
+    _logit_rows(logits, targets)
+    rows, V = logits.shape
+    dev = logits.device
+    for t, nm, n in ((lse, "lse", 2), (entropy, "entropy", 1), (d_logprob, "d_logprob", 1), (d_entropy, "d_entropy", 1)):
+        if t is not None and (t.dtype != torch.float32 or not t.is_contiguous() or t.numel() != n * rows):
+            raise TypeError(f"{nm} is contiguous float32, {n} x {rows}")
+    if dlogits is None:
+        dlogits = torch.empty((rows, V), dtype=logits.dtype, device=dev)
+    elif dlogits.dtype != logits.dtype or dlogits.shape != logits.shape or dlogits.stride(1) != 1:
+        raise TypeError("dlogits has the logits' dtype and shape and contiguous rows")
+    _same_device(dev, (targets, "targets"), (lse, "lse"), (entropy, "entropy"), (d_logprob, "d_logprob"), (d_entropy, "d_entropy"),
+                 (dlogits, "dlogits"))
+    h = handle or ffi.default_handle(dev.index or 0)
+    with _on(dev):
+        rc = ffi.lib().mamba_b200_token_logprobs_bwd(h.ptr, _stream(dev), dtype_code(logits.dtype), logits.data_ptr(),
+                                                     max(logits.stride(0), V), _ptr(targets), temperature, lse.data_ptr(),
+                                                     _ptr(entropy), _ptr(d_logprob), _ptr(d_entropy), dlogits.data_ptr(),
+                                                     max(dlogits.stride(0), V), rows, V)
+    h.check(rc, "mamba_b200_token_logprobs_bwd")
+    return dlogits
+
+
+def gated_scan_states(B, T, D):
+    """Shape of the chunk_states that gated_scan_fwd keeps for gated_scan_bwd."""
+    return (B, -(-T // ffi.GATED_SCAN_SAVE), D)
+
+
+def _gated_rows(t, name, like):
+    """Row stride of a [B, T, D] view whose rows are one after another: any stride where there is but one row."""
+    if t.dtype != like.dtype or t.shape != like.shape or t.device != like.device:
+        raise TypeError(f"{name} has x's dtype, shape and device: {list(like.shape)} {like.dtype}")
+    B, T, D = t.shape
+    s0, s1, s2 = t.stride()
+    if s2 != 1 and D > 1:
+        raise ValueError(f"{name}: last dimension must be contiguous")
+    if T <= 1:
+        s1 = s0 if B > 1 and T else D
+    elif B > 1 and s0 != T * s1:
+        raise ValueError(f"{name}: batch stride must equal T * row stride")
+    return s1
+
+
+def _gated_state(t, name, x, shape=None):
+    shape = shape or (x.shape[0], x.shape[2])
+    if t is not None and (t.dtype != torch.float32 or tuple(t.shape) != shape or not t.is_contiguous() or t.device != x.device):
+        raise TypeError(f"{name} is contiguous float32 {list(shape)} on x's device")
+    return _ptr(t)
+
+
+def gated_scan_fwd(x, f, z=None, *, h0=None, h_last=None, y=None, chunk_states=None, handle=None):
+    """Gated linear recurrence: u = sigmoid(-f), h_t = h_{t-1} + u_t (x_t - h_{t-1}), y = h * SiLU(z) (y = h without z).
+    x, f, z, y [B,T,D] in a storage dtype, any row stride; h0 (zeros if None) and h_last (written if given, may be h0)
+    [B,D] f32; chunk_states f32 of gated_scan_states(B,T,D) receives what gated_scan_bwd needs.  Returns y."""
+    _require_cuda(x, f, z, h0, h_last, y, chunk_states)
+    if y is None:
+        y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    B, T, D = x.shape
+    dev = x.device
+    h = handle or ffi.default_handle(dev.index or 0)
+    a = ffi.GatedScanArgs(dtype_code(x.dtype), B, T, D, x.data_ptr(), _gated_rows(x, "x", x), f.data_ptr(), _gated_rows(f, "f", x),
+                          _ptr(z), 0 if z is None else _gated_rows(z, "z", x), _gated_state(h0, "h0", x),
+                          _gated_state(h_last, "h_last", x), y.data_ptr(), _gated_rows(y, "y", x),
+                          _gated_state(chunk_states, "chunk_states", x, gated_scan_states(B, T, D)))
+    with _on(dev):
+        rc = ffi.lib().mamba_b200_gated_scan_fwd(h.ptr, _stream(dev), C.byref(a))
+    h.check(rc, "mamba_b200_gated_scan_fwd")
+    return y
+
+
+def gated_scan_step(x, f, h0, z=None, *, h_last=None, y=None, handle=None):
+    """One token per sequence: x, f, z, y [B,D]; the state h0 [B,D] f32 is updated in place, or h_last receives it."""
+    row = lambda t: None if t is None else t.unsqueeze(1)  # noqa: E731
+    if y is None:
+        y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    gated_scan_fwd(x.unsqueeze(1), f.unsqueeze(1), row(z), h0=h0, h_last=h0 if h_last is None else h_last, y=y.unsqueeze(1),
+                   handle=handle)
+    return y
+
+
+def gated_scan_bwd(x, f, dy, chunk_states, z=None, *, d_last=None, d_h0=None, d_x=None, d_f=None, d_z=None, handle=None):
+    """Backward of gated_scan_fwd from its chunk_states.  d_last [B,D] f32: gradient of the state that left (None: zeros).
+    Returns dict(d_x, d_f, d_z (with z), d_h0 f32); the outputs may be given (columns of one projection's gradient, say)."""
+    _require_cuda(x, f, z, dy, chunk_states, d_last, d_h0, d_x, d_f, d_z)
+    B, T, D = x.shape
+    dev = x.device
+    h = handle or ffi.default_handle(dev.index or 0)
+    new = lambda t: torch.empty(x.shape, dtype=x.dtype, device=dev) if t is None else t  # noqa: E731
+    d_x, d_f = new(d_x), new(d_f)
+    d_z = new(d_z) if z is not None else None
+    if d_h0 is None:
+        d_h0 = torch.empty((B, D), dtype=torch.float32, device=dev)
+    a = ffi.GatedScanArgs(dtype_code(x.dtype), B, T, D, x.data_ptr(), _gated_rows(x, "x", x), f.data_ptr(), _gated_rows(f, "f", x),
+                          _ptr(z), 0 if z is None else _gated_rows(z, "z", x), None, None, None, 0,
+                          _gated_state(chunk_states, "chunk_states", x, gated_scan_states(B, T, D)),
+                          dy.data_ptr(), _gated_rows(dy, "dy", x), _gated_state(d_last, "d_last", x), _gated_state(d_h0, "d_h0", x),
+                          d_x.data_ptr(), _gated_rows(d_x, "d_x", x), d_f.data_ptr(), _gated_rows(d_f, "d_f", x),
+                          _ptr(d_z), 0 if d_z is None else _gated_rows(d_z, "d_z", x))
+    with _on(dev):
+        rc = ffi.lib().mamba_b200_gated_scan_bwd(h.ptr, _stream(dev), C.byref(a))
+    h.check(rc, "mamba_b200_gated_scan_bwd")
+    out = dict(d_x=d_x, d_f=d_f, d_h0=d_h0)
+    if d_z is not None:
+        out["d_z"] = d_z
+    return out
