@@ -88,6 +88,7 @@ int m3_bwd_configure(Ctx* c);   // m3_ssd_bwd.cu
 int norm_configure(Ctx* c);     // norm.cu
 int train_ops_configure(Ctx* c);  // train_ops.cu
 int decode_configure(Ctx* c);     // decode.cu
+int gated_scan_configure(Ctx* c);  // gated_scan.cu
 
 }  // namespace mb200
 
@@ -130,6 +131,8 @@ extern "C" MAMBA_B200_API int mamba_b200_init(int device, void** handle) {
     rc = train_ops_configure(c);
     if (rc) return rc;
     rc = decode_configure(c);
+    if (rc) return rc;
+    rc = gated_scan_configure(c);
     if (rc) return rc;
     return MAMBA_B200_OK;
 }
