@@ -641,7 +641,13 @@ typedef struct mamba_b200_gated_scan_args {
     long long ld_df;
     void* d_z;
     long long ld_dz;
+    void* workspace;     /* optional caller-owned scratch, 16-byte aligned, or NULL: with
+                            mamba_b200_gated_scan_workspace_bytes(B,T,D) bytes (may be 0) a long axis of few channels is cut
+                            into segments that run side by side; nothing in it is kept between calls */
+    long long workspace_bytes;
 } mamba_b200_gated_scan_args;
+
+MAMBA_B200_API long long mamba_b200_gated_scan_workspace_bytes(int B, int T, int D);
 
 MAMBA_B200_API int mamba_b200_gated_scan_fwd(void* handle, void* stream, const mamba_b200_gated_scan_args* args);
 MAMBA_B200_API int mamba_b200_gated_scan_bwd(void* handle, void* stream, const mamba_b200_gated_scan_args* args);

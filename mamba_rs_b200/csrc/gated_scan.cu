@@ -61,20 +61,11 @@ __device__ __forceinline__ void put(float* row, int c, int D, Ch<2> v) {
     if (c < D) row[c] = v.a.x;
     if (c + 1 < D) row[c + 1] = v.a.y;
 }
-template <int V> __device__ __forceinline__ Ch<V> ld_remote(uint32_t at) {
-    if constexpr (V == 1) {
-        return {ld_cluster1(at)};
-    } else {
-        float2 v;
-        asm volatile("ld.shared::cluster.v2.f32 {%0,%1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(at));
-        return {v};
-    }
-}
-
 struct Params {
     mamba_b200_gated_scan_args a;
     int* status;
-    int tiles, ranks, tma_in, tma_out;
+    float* sums;  // [B, segments, 2, D]: what each segment does to the state (or gradient) that enters it
+    int tiles, segments, per_segment, tma_in, tma_out;
 };
 
 // ---------------------------------------------------------------------------------------------------
@@ -82,7 +73,7 @@ struct Params {
 // to a state, the four warps join their spans in order, and each walks its steps again from the state that is really there.
 // Gates and inputs stay in registers between the two walks, so everything is read once; results take the place of the inputs
 // in shared memory and leave by TMA, which also clips what lies outside the tensor.  Where there are few strips of channels,
-// the CTAs of a cluster take consecutive tiles of one strip and join their spans through distributed shared memory.
+// time is cut into segments: a first kernel finds what each does to a state, and a CTA starts from what the earlier ones leave.
 // ---------------------------------------------------------------------------------------------------
 constexpr int kWarps = 4, L = kTile / kWarps;
 
@@ -90,11 +81,9 @@ template <typename T, int V, int NIN>
 struct Layout {
     static constexpr int CH = 32 * V;
     static constexpr uint32_t kIn = kTile * CH * sizeof(T);  // one input's tile
-    // two stages of inputs | the warps' sums (three each, the forward uses two) | barriers | (clusters) two buffers of the CTA's
-    // two sums
-    static constexpr uint32_t oPart = 2 * NIN * kIn, oBar = oPart + 3 * kWarps * CH * sizeof(float), oTot = oBar + 16;
-    static constexpr uint32_t kBytes = oTot + 128;
-    static constexpr uint32_t kMore = 4 * CH * sizeof(float);
+    // two stages of inputs | the warps' sums (three each, the forward uses two) | barriers
+    static constexpr uint32_t oPart = 2 * NIN * kIn, oBar = oPart + 3 * kWarps * CH * sizeof(float);
+    static constexpr uint32_t kBytes = oBar + 16 + 128;
 };
 
 template <typename T, int V, int NIN>
@@ -106,13 +95,12 @@ struct Tiles {
     int b, c0, warp, lane;
     bool alive;
 
-    __device__ __forceinline__ bool exists(int k) const { return k >= 0 && k < p.tiles; }
     __device__ __forceinline__ T* at(int s, int i) const { return reinterpret_cast<T*>(sm + (s * NIN + i) * Lay::kIn); }
     // The warp's first row, this lane's first channel.
     __device__ __forceinline__ T* mine(int s, int i) const { return at(s, i) + warp * L * Lay::CH + lane * V; }
     // Asks for tile k in stage s, once what was written from that stage has been read.
     __device__ __forceinline__ void ask(int s, int k, const CUtensorMap* const* map) {
-        if (threadIdx.x != 0 || !exists(k)) return;
+        if (threadIdx.x != 0) return;
         if (p.tma_out) tma_wait_read0();
         if (!p.tma_in) return;
         mbar_expect_tx(&bars[s], NIN * Lay::kIn);
@@ -145,19 +133,35 @@ struct Tiles {
     }
 };
 
-// The CTA's two sums, joined over the cluster: what was there before this CTA's tile, and behind the last one's.
+// What segments from, from + step, ... up to (not including) to make of v, the warps sharing them.
 template <int V>
-__device__ __forceinline__ Ch<V> join_cluster(float* tot, int it, int rank, int R, int lane, Ch<V>& carry) {
+__device__ __forceinline__ Ch<V> enter(const Params& p, float* part, int b, int c, int from, int to, int step, Ch<V> v) {
+    using C = Ch<V>;
     constexpr int CH = 32 * V;
-    Ch<V> h = carry;
-    const uint32_t base = smem_u32(tot + (it & 1) * (2 * CH) + lane * V);
-    for (int r = 0; r < R; ++r) {
-        const uint32_t far = cluster_addr(base, r);
-        const Ch<V> n = ld_remote<V>(far), a = ld_remote<V>(far + CH * 4);
-        if (r == rank) h = carry;
-        carry = over(n, a, carry);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, n = (to - from) * step, per = (n + kWarps - 1) / kWarps;
+    C N = C::splat(0.0f), A = C::splat(0.0f);
+    for (int i0 = warp * per; i0 < min(n, (warp + 1) * per); i0 += 8) {
+        C m[8], a[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const bool ok = i0 + i < min(n, (warp + 1) * per);
+            const float* row = p.sums + (static_cast<long long>(b) * p.segments + (ok ? from + (i0 + i) * step : 0)) * 2 * p.a.D;
+            m[i] = get<V>(row, ok ? c : p.a.D, p.a.D);
+            a[i] = get<V>(row + p.a.D, ok ? c : p.a.D, p.a.D);
+        }
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            A = over(m[i], a[i], A);
+            N = both(N, m[i]);
+        }
     }
-    return h;
+    N.store(part + warp * CH + lane * V);
+    A.store(part + (kWarps + warp) * CH + lane * V);
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) v = over(C::load(part + w * CH + lane * V), C::load(part + (kWarps + w) * CH + lane * V), v);
+    __syncthreads();
+    return v;
 }
 
 template <typename T, int V, bool GATE>
@@ -170,10 +174,10 @@ __global__ void __launch_bounds__(kWarps * 32, 3)
     constexpr int CH = Lay::CH;
     extern __shared__ unsigned char raw[];
     unsigned char* sm = raw + (128 - (smem_u32(raw) & 127)) % 128;
-    float *part = reinterpret_cast<float*>(sm + Lay::oPart), *tot = reinterpret_cast<float*>(sm + Lay::oTot);
+    float* part = reinterpret_cast<float*>(sm + Lay::oPart);
     uint64_t* bars = reinterpret_cast<uint64_t*>(sm + Lay::oBar);
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, R = p.ranks, rank = R == 1 ? 0 : static_cast<int>(blockIdx.x) % R;
-    const int strip = static_cast<int>(blockIdx.x) / R, per_b = (p.a.D + CH - 1) / CH, b = strip / per_b;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, seg = static_cast<int>(blockIdx.x) % p.segments;
+    const int strip = static_cast<int>(blockIdx.x) / p.segments, per_b = (p.a.D + CH - 1) / CH, b = strip / per_b;
     const int c0 = (strip - b * per_b) * CH, c = c0 + lane * V, D = p.a.D;
     if (threadIdx.x == 0) {
         mbar_init(&bars[0], 1);
@@ -185,80 +189,59 @@ __global__ void __launch_bounds__(kWarps * 32, 3)
     const CUtensorMap* maps[3] = {&mf, &mx, &mz};
     const void* src[3] = {p.a.f, p.a.x, p.a.z};
     const long long ld[3] = {p.a.ld_f, p.a.ld_x, p.a.ld_z};
-    in.ask(0, rank, maps);
+    const int first = seg * p.per_segment, rounds = min(p.per_segment, p.tiles - first);
+    in.ask(0, first, maps);
     C carry = p.a.h0 ? get<V>(p.a.h0 + static_cast<long long>(b) * D, c, D) : C::splat(0.0f);
-    const int rounds = (p.tiles + R - 1) / R;
+    if (seg > 0) carry = enter<V>(p, part, b, c, 0, seg, 1, carry);
     for (int it = 0; it < rounds; ++it) {
-        const int k = it * R + rank, s = it & 1;
-        const bool here = in.exists(k);
+        const int k = first + it, s = it & 1;
         C n[L], x[L], N = C::splat(0.0f), A = C::splat(0.0f);
-        if (here) {
-            in.wait(s, k, (it >> 1) & 1, src, ld);
-            const T *sf = in.mine(s, 0), *sx = in.mine(s, 1);
+        in.wait(s, k, (it >> 1) & 1, src, ld);
+        const T* sf = in.mine(s, 0);
+        T* sx = in.mine(s, 1);
 #pragma unroll
-            for (int j = 0; j < L; ++j) {
-                n[j] = neg_gate(C::load(sf + j * CH), kLog2e);
-                x[j] = C::load(sx + j * CH);
-                A = fma(n[j], sub(A, x[j]), A);
-                N = both(N, n[j]);
-            }
+        for (int j = 0; j < L; ++j) {
+            n[j] = neg_gate(C::load(sf + j * CH), kLog2e);
+            x[j] = C::load(sx + j * CH);
+            A = fma(n[j], sub(A, x[j]), A);
+            N = both(N, n[j]);
         }
         N.store(part + warp * CH + lane * V);
         A.store(part + (kWarps + warp) * CH + lane * V);
         __syncthreads();
-        in.ask(s ^ 1, k + R, maps);
-        C h = carry, start = carry;
-        if (R > 1) {
-            if (warp == 0) {
-                N = C::splat(0.0f), A = C::splat(0.0f);
-#pragma unroll
-                for (int w = 0; w < kWarps; ++w) {
-                    const C m = C::load(part + w * CH + lane * V);
-                    A = over(m, C::load(part + (kWarps + w) * CH + lane * V), A);
-                    N = both(N, m);
-                }
-                N.store(tot + (it & 1) * (2 * CH) + lane * V);
-                A.store(tot + (it & 1) * (2 * CH) + CH + lane * V);
-            }
-            cluster_sync();
-            h = join_cluster<V>(tot, it, rank, R, lane, carry);
-        }
+        if (it + 1 < rounds) in.ask(s ^ 1, k + 1, maps);
+        C h = carry;
 #pragma unroll
         for (int w = 0; w < kWarps; ++w) {
-            if (w == warp) start = h;
+            if (w == warp) carry = h;  // (what enters this warp's span)
             h = over(C::load(part + w * CH + lane * V), C::load(part + (kWarps + w) * CH + lane * V), h);
         }
-        if (R == 1) carry = h;
-        if (here) {
-            if (p.a.chunk_states && warp == 0) put(p.a.chunk_states + (static_cast<long long>(b) * p.tiles + k) * D, c, D, start);
-            h = start;
-            T* sy = in.mine(s, 1);
-            const T* sz = in.mine(s, NIN - 1);
+        if (p.a.chunk_states && warp == 0) put(p.a.chunk_states + (static_cast<long long>(b) * p.tiles + k) * D, c, D, carry);
+        const T* sz = in.mine(s, NIN - 1);
 #pragma unroll
-            for (int j = 0; j < L; ++j) {
-                h = fma(n[j], sub(h, x[j]), h);
-                if constexpr (GATE) {
-                    const C z = C::load(sz + j * CH);
-                    mul(mul(h, z), mul(neg_gate(z, -kLog2e), C::splat(-1.0f))).store(sy + j * CH);
-                } else {
-                    h.store(sy + j * CH);
-                }
-            }
-            fence_proxy_async();
-            if (!p.tma_out) {
-                __syncwarp();
-                in.plain_out(s, 1, k, p.a.y, p.a.ld_y);
+        for (int j = 0; j < L; ++j) {
+            carry = fma(n[j], sub(carry, x[j]), carry);
+            if constexpr (GATE) {
+                const C z = C::load(sz + j * CH);
+                mul(mul(carry, z), mul(neg_gate(z, -kLog2e), C::splat(-1.0f))).store(sx + j * CH);
+            } else {
+                carry.store(sx + j * CH);
             }
         }
+        carry = h;
+        fence_proxy_async();
+        if (!p.tma_out) {
+            __syncwarp();
+            in.plain_out(s, 1, k, p.a.y, p.a.ld_y);
+        }
         __syncthreads();
-        if (p.tma_out && threadIdx.x == 0 && here) {
+        if (p.tma_out && threadIdx.x == 0) {
             tma_store_3d(&my, in.at(s, 1), c0, k * kTile, b);
             tma_commit();
         }
     }
-    if (p.a.h_last && rank == 0 && warp == 0) put(p.a.h_last + static_cast<long long>(b) * D, c, D, carry);
+    if (p.a.h_last && seg == p.segments - 1 && warp == 0) put(p.a.h_last + static_cast<long long>(b) * D, c, D, carry);
     if (p.tma_out && threadIdx.x == 0) tma_wait_read0();
-    if (R > 1) cluster_sync();  // the others may still read this CTA's sums
 }
 
 // The gradient walks the tiles from the last to the first.  The states inside a tile come from the saved one that enters it, by
@@ -275,10 +258,10 @@ __global__ void __launch_bounds__(kWarps * 32, 3)
     constexpr int CH = Lay::CH;
     extern __shared__ unsigned char raw[];
     unsigned char* sm = raw + (128 - (smem_u32(raw) & 127)) % 128;
-    float *part = reinterpret_cast<float*>(sm + Lay::oPart), *tot = reinterpret_cast<float*>(sm + Lay::oTot);
+    float* part = reinterpret_cast<float*>(sm + Lay::oPart);
     uint64_t* bars = reinterpret_cast<uint64_t*>(sm + Lay::oBar);
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, R = p.ranks, rank = R == 1 ? 0 : static_cast<int>(blockIdx.x) % R;
-    const int strip = static_cast<int>(blockIdx.x) / R, per_b = (p.a.D + CH - 1) / CH, b = strip / per_b;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, seg = static_cast<int>(blockIdx.x) % p.segments;
+    const int strip = static_cast<int>(blockIdx.x) / p.segments, per_b = (p.a.D + CH - 1) / CH, b = strip / per_b;
     const int c0 = (strip - b * per_b) * CH, c = c0 + lane * V, D = p.a.D;
     if (threadIdx.x == 0) {
         mbar_init(&bars[0], 1);
@@ -290,65 +273,47 @@ __global__ void __launch_bounds__(kWarps * 32, 3)
     const CUtensorMap* maps[4] = {&mf, &mx, &me, &mz};
     const void* src[4] = {p.a.f, p.a.x, p.a.dy, p.a.z};
     const long long ld[4] = {p.a.ld_f, p.a.ld_x, p.a.ld_dy, p.a.ld_z};
-    const int last = p.tiles - 1 - rank;
+    const int first = min((seg + 1) * p.per_segment, p.tiles) - 1, rounds = first + 1 - seg * p.per_segment;
     const C minus = C::splat(-1.0f);
-    in.ask(0, last, maps);
+    if (rounds > 0) in.ask(0, first, maps);
     C carry = p.a.d_last ? mul(get<V>(p.a.d_last + static_cast<long long>(b) * D, c, D), minus) : C::splat(0.0f);
     const float* states = p.a.chunk_states + static_cast<long long>(b) * p.tiles * D;
     auto state = [&](int k) { return k >= 0 ? get<V>(states + static_cast<long long>(k) * D, c, D) : C::splat(0.0f); };
-    C next = state(last);
-    const int rounds = (p.tiles + R - 1) / R;
+    C next = state(first);
+    if (seg + 1 < p.segments) carry = enter<V>(p, part, b, c, p.segments - 1, seg, -1, carry);
     for (int it = 0; it < rounds; ++it) {
-        const int k = last - it * R, s = it & 1;
-        const bool here = k >= 0;
+        const int k = first - it, s = it & 1;
         C h = next;
-        next = state(k - R);
+        next = state(k - 1);
         C n[L], x[L], e[L], q[L], N = C::splat(0.0f), A = C::splat(0.0f), G = C::splat(0.0f);
-        if (here) {
-            in.wait(s, k, (it >> 1) & 1, src, ld);
-            const T *sf = in.mine(s, 0), *sx = in.mine(s, 1), *se = in.mine(s, 2), *sz = in.mine(s, NIN - 1);
+        in.wait(s, k, (it >> 1) & 1, src, ld);
+        const T *sf = in.mine(s, 0), *sx = in.mine(s, 1), *se = in.mine(s, 2), *sz = in.mine(s, NIN - 1);
 #pragma unroll
-            for (int j = 0; j < L; ++j) {
-                n[j] = neg_gate(C::load(sf + j * CH), kLog2e);
-                x[j] = C::load(sx + j * CH);
-                const C dy = C::load(se + j * CH);
-                if constexpr (GATE) {
-                    const C z = C::load(sz + j * CH), m = neg_gate(z, -kLog2e);  // -sigmoid(z)
-                    q[j] = mul(dy, mul(m, fma(z, fma(m, minus, minus), minus)));  // dy SiLU'(z) = dy sigmoid (1 + z (1 - sigmoid))
-                    e[j] = mul(dy, mul(z, m));                                    // -dy SiLU(z)
-                } else {
-                    e[j] = mul(dy, minus);
-                }
-                A = fma(n[j], sub(A, x[j]), A);
-                N = both(N, n[j]);
+        for (int j = 0; j < L; ++j) {
+            n[j] = neg_gate(C::load(sf + j * CH), kLog2e);
+            x[j] = C::load(sx + j * CH);
+            const C dy = C::load(se + j * CH);
+            if constexpr (GATE) {
+                const C z = C::load(sz + j * CH), m = neg_gate(z, -kLog2e);  // -sigmoid(z)
+                q[j] = mul(dy, mul(m, fma(z, fma(m, minus, minus), minus)));  // dy SiLU'(z) = dy sigmoid (1 + z (1 - sigmoid))
+                e[j] = mul(dy, mul(z, m));                                    // -dy SiLU(z)
+            } else {
+                e[j] = mul(dy, minus);
             }
+            A = fma(n[j], sub(A, x[j]), A);
+            N = both(N, n[j]);
+        }
 #pragma unroll
-            for (int j = L - 1; j >= 0; --j) {
-                const C g = add(e[j], G);
-                G = fma(n[j], g, g);
-            }
+        for (int j = L - 1; j >= 0; --j) {
+            const C g = add(e[j], G);
+            G = fma(n[j], g, g);
         }
         N.store(part + warp * CH + lane * V);
         A.store(part + (kWarps + warp) * CH + lane * V);
         G.store(part + (2 * kWarps + warp) * CH + lane * V);
         __syncthreads();
-        in.ask(s ^ 1, k - R, maps);
+        if (it + 1 < rounds) in.ask(s ^ 1, k - 1, maps);
         C g = carry, start = carry;
-        if (R > 1) {
-            if (warp == 0) {
-                N = C::splat(0.0f), G = C::splat(0.0f);
-#pragma unroll
-                for (int w = kWarps - 1; w >= 0; --w) {
-                    const C m = C::load(part + w * CH + lane * V);
-                    G = over(m, C::load(part + (2 * kWarps + w) * CH + lane * V), G);
-                    N = both(N, m);
-                }
-                N.store(tot + (it & 1) * (2 * CH) + lane * V);
-                G.store(tot + (it & 1) * (2 * CH) + CH + lane * V);
-            }
-            cluster_sync();
-            g = join_cluster<V>(tot, it, rank, R, lane, carry);
-        }
 #pragma unroll
         for (int w = 0; w < kWarps - 1; ++w)
             if (w < warp) h = over(C::load(part + w * CH + lane * V), C::load(part + (kWarps + w) * CH + lane * V), h);
@@ -357,42 +322,112 @@ __global__ void __launch_bounds__(kWarps * 32, 3)
             if (w == warp) start = g;
             g = over(C::load(part + w * CH + lane * V), C::load(part + (2 * kWarps + w) * CH + lane * V), g);
         }
-        if (R == 1) carry = g;
-        if (here) {
-            T *df = in.mine(s, 0), *dx = in.mine(s, 1), *dz = in.mine(s, NIN - 1);
+        carry = g;
+        T *df = in.mine(s, 0), *dx = in.mine(s, 1), *dz = in.mine(s, NIN - 1);
 #pragma unroll
-            for (int j = 0; j < L; ++j) {
-                x[j] = sub(h, x[j]);  // h_{t-1} - x_t
-                h = fma(n[j], x[j], h);
-                if constexpr (GATE) mul(q[j], h).store(dz + j * CH);
-            }
-            g = start;
+        for (int j = 0; j < L; ++j) {
+            x[j] = sub(h, x[j]);  // h_{t-1} - x_t
+            h = fma(n[j], x[j], h);
+            if constexpr (GATE) mul(q[j], h).store(dz + j * CH);
+        }
+        g = start;
 #pragma unroll
-            for (int j = L - 1; j >= 0; --j) {
-                g = add(g, e[j]);
-                mul(g, n[j]).store(dx + j * CH);
-                g = fma(n[j], g, g);
-                mul(x[j], mul(n[j], g)).store(df + j * CH);
-            }
-            fence_proxy_async();
-            if (!p.tma_out) {
-                __syncwarp();
-                in.plain_out(s, 0, k, p.a.d_f, p.a.ld_df);
-                in.plain_out(s, 1, k, p.a.d_x, p.a.ld_dx);
-                if constexpr (GATE) in.plain_out(s, 3, k, p.a.d_z, p.a.ld_dz);
-            }
+        for (int j = L - 1; j >= 0; --j) {
+            g = add(g, e[j]);
+            mul(g, n[j]).store(dx + j * CH);
+            g = fma(n[j], g, g);
+            mul(x[j], mul(n[j], g)).store(df + j * CH);
+        }
+        fence_proxy_async();
+        if (!p.tma_out) {
+            __syncwarp();
+            in.plain_out(s, 0, k, p.a.d_f, p.a.ld_df);
+            in.plain_out(s, 1, k, p.a.d_x, p.a.ld_dx);
+            if constexpr (GATE) in.plain_out(s, 3, k, p.a.d_z, p.a.ld_dz);
         }
         __syncthreads();
-        if (p.tma_out && threadIdx.x == 0 && here) {
+        if (p.tma_out && threadIdx.x == 0) {
             tma_store_3d(&mdf, in.at(s, 0), c0, k * kTile, b);
             tma_store_3d(&mdx, in.at(s, 1), c0, k * kTile, b);
             if constexpr (GATE) tma_store_3d(&mdz, in.at(s, 3), c0, k * kTile, b);
             tma_commit();
         }
     }
-    if (p.a.d_h0 && rank == 0 && warp == 0) put(p.a.d_h0 + static_cast<long long>(b) * D, c, D, mul(carry, minus));
+    if (p.a.d_h0 && seg == 0 && warp == 0) put(p.a.d_h0 + static_cast<long long>(b) * D, c, D, mul(carry, minus));
     if (p.tma_out && threadIdx.x == 0) tma_wait_read0();
-    if (R > 1) cluster_sync();
+}
+
+// What each segment of time does to a state (forward) or to the gradient that comes from behind it, without results: f and x
+// (dy and z) are read once more than the floor.  A warp has a quarter of the segment, 16 steps at a time, all their loads in
+// flight; it ends where the kernel above begins, so that what it read last is still in L2 then.
+template <typename T, int V, bool GATE, bool BWD>
+__global__ void __launch_bounds__(kWarps * 32) gated_scan_sums_kernel(const __grid_constant__ Params p) {
+    using C = Ch<V>;
+    constexpr int CH = 32 * V, M = kTile / L;
+    __shared__ __align__(8) float part[2 * kWarps * CH];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, parts = p.segments - 1;
+    const int seg = static_cast<int>(blockIdx.x) % parts + (BWD ? 1 : 0), strip = static_cast<int>(blockIdx.x) / parts;
+    const int D = p.a.D, per_b = (D + CH - 1) / CH, b = strip / per_b, c = (strip - b * per_b) * CH + lane * V;
+    const int first = seg * p.per_segment * M, n = min(p.per_segment, p.tiles - seg * p.per_segment) * M, per = (n + kWarps - 1) / kWarps;
+    const int lo = first + min(n, warp * per), hi = first + min(n, (warp + 1) * per);  // pieces of L steps
+    const bool inside = (strip - b * per_b + 1) * CH <= D;
+    struct __align__(sizeof(T) * V) Word { T v[V]; };
+    // L steps from t0; behind the end, and beside the last channel, `none`.
+    auto fetch = [&](Word* to, const void* src, long long ld, int t0, float none) {
+        const T* row = static_cast<const T*>(src) + (static_cast<long long>(b) * p.a.T + t0) * ld + c;
+        if (inside && t0 + L <= p.a.T) {
+#pragma unroll
+            for (int j = 0; j < L; ++j) to[j] = *reinterpret_cast<const Word*>(row + j * ld);
+        } else {
+#pragma unroll
+            for (int j = 0; j < L; ++j)
+#pragma unroll
+                for (int e = 0; e < V; ++e) to[j].v[e] = t0 + j < p.a.T && c + e < D ? row[j * ld + e] : from_f<T>(none);
+        }
+    };
+    C N = C::splat(0.0f), A = C::splat(0.0f);
+    for (int i = 0; i < hi - lo; ++i) {
+        const int t0 = (BWD ? lo + i : hi - 1 - i) * L;
+        Word fw[L], xw[L], zw[L];
+        fetch(fw, p.a.f, p.a.ld_f, t0, INFINITY);
+        fetch(xw, BWD ? p.a.dy : p.a.x, BWD ? p.a.ld_dy : p.a.ld_x, t0, 0.0f);
+        if constexpr (BWD && GATE) fetch(zw, p.a.z, p.a.ld_z, t0, 0.0f);
+        C n1 = C::splat(0.0f), a1 = C::splat(0.0f);
+#pragma unroll
+        for (int jj = 0; jj < L; ++jj) {
+            const int j = BWD ? L - 1 - jj : jj;
+            const C m = neg_gate(C::load(fw[j].v), kLog2e), x = C::load(xw[j].v);
+            if constexpr (BWD) {
+                C e = mul(x, C::splat(-1.0f));
+                if constexpr (GATE) {
+                    const C z = C::load(zw[j].v);
+                    e = mul(x, mul(z, neg_gate(z, -kLog2e)));
+                }
+                const C g = add(e, a1);
+                a1 = fma(m, g, g);
+            } else {
+                a1 = fma(m, sub(a1, x), a1);
+            }
+            n1 = both(n1, m);
+        }
+        A = over(N, A, a1);  // this piece is met before those that are there
+        N = both(n1, N);
+    }
+    N.store(part + warp * CH + lane * V);
+    A.store(part + (kWarps + warp) * CH + lane * V);
+    __syncthreads();
+    if (warp != 0) return;
+    N = C::splat(0.0f), A = C::splat(0.0f);
+#pragma unroll
+    for (int i = 0; i < kWarps; ++i) {
+        const int w = BWD ? kWarps - 1 - i : i;
+        const C m = C::load(part + w * CH + lane * V);
+        A = over(m, C::load(part + (kWarps + w) * CH + lane * V), A);
+        N = both(N, m);
+    }
+    float* row = p.sums + (static_cast<long long>(b) * p.segments + seg) * 2 * D;
+    put(row, c, D, N);
+    put(row + D, c, D, A);
 }
 
 // Windows of a few steps (decoding: one): a thread has one channel and walks it, its loads in flight together.
@@ -444,11 +479,12 @@ static int check(Ctx* c, const mamba_b200_gated_scan_args* a, bool bwd) {
 }
 
 
-// How many CTAs of a cluster share a strip: as many as keep every CTA resident, up to 16, when strips are few.
-static int pick_ranks(int strips, int tiles, int slots) {
-    int r = 1;
-    while (r < 16 && 2 * r <= tiles && strips * 2 * r <= slots) r *= 2;
-    return r;
+// Segments of time: as many as give every SM its three CTAs, none where half of that is there without.
+constexpr int kMaxSegments = 128;
+static int pick_segments(int sms, long long strips, int tiles) {
+    const long long want = strips * 2 > 3ll * sms ? 1 : 3ll * sms / strips;
+    const int most = static_cast<int>(want < kMaxSegments ? want : kMaxSegments);
+    return most < tiles ? most : (tiles > 0 ? tiles : 1);
 }
 
 template <typename T, int V, bool GATE, bool BWD>
@@ -463,19 +499,27 @@ static int launch_tiled(Ctx* c, const mamba_b200_gated_scan_args& a, cudaStream_
     const void* fn = kernel<T, V, GATE, BWD>();
     Params p{a, c->d_status};
     const long long strips = static_cast<long long>(a.B) * ((a.D + Lay::CH - 1) / Lay::CH);
-    if (strips > 2147483647ll / 16) return fail(c, MAMBA_B200_ERR_SHAPE, "gated_scan: too many channels");
+    if (strips > 2147483647ll) return fail(c, MAMBA_B200_ERR_SHAPE, "gated_scan: too many channels");
     p.tiles = (a.T + kTile - 1) / kTile;
-    p.ranks = pick_ranks(static_cast<int>(strips), p.tiles, c->sm_count * 3);
+    int segments = pick_segments(c->sm_count, strips, p.tiles);
+    if (reinterpret_cast<uintptr_t>(a.workspace) % 16 != 0) return fail(c, MAMBA_B200_ERR_ARG, "gated_scan: the workspace is 16-byte aligned");
+    const long long row = static_cast<long long>(a.B) * a.D * 2 * sizeof(float);  // a segment's sums
+    if (!a.workspace || a.workspace_bytes < 0) segments = 1;
+    else if (segments * row > a.workspace_bytes) segments = a.workspace_bytes / row > 1 ? static_cast<int>(a.workspace_bytes / row) : 1;
+    p.per_segment = (p.tiles + segments - 1) / segments;
+    p.segments = p.tiles ? (p.tiles + p.per_segment - 1) / p.per_segment : 1;
+    p.sums = static_cast<float*>(a.workspace);
     CUtensorMap mf{}, mx{}, me{}, mz{}, o0{}, o1{}, o2{};
     auto map = [&](CUtensorMap* m, const void* base, long long ld) { return make_tmap_3d(c, m, a.dtype, base, ld, a.D, a.T, a.B, Lay::CH, kTile); };
     p.tma_in = map(&mf, a.f, a.ld_f) && map(&mx, a.x, a.ld_x) && (!BWD || map(&me, a.dy, a.ld_dy)) && (!GATE || map(&mz, a.z, a.ld_z));
     p.tma_out = BWD ? map(&o0, a.d_f, a.ld_df) && map(&o1, a.d_x, a.ld_dx) && (!GATE || map(&o2, a.d_z, a.ld_dz)) : map(&o0, a.y, a.ld_y);
     void* fwd_args[] = {&mf, &mx, &mz, &o0, &p};
     void* bwd_args[] = {&mf, &mx, &me, &mz, &o0, &o1, &o2, &p};
-    const dim3 grid(static_cast<unsigned>(strips * p.ranks)), block(kWarps * 32);
-    void** args = BWD ? bwd_args : fwd_args;
-    if (p.ranks == 1) MB200_CUDA_CHECK(c, cudaLaunchKernel(fn, grid, block, args, Lay::kBytes, st));
-    else MB200_CUDA_CHECK(c, launch_cluster(fn, grid, block, Lay::kBytes + Lay::kMore, st, p.ranks, args));
+    if (p.segments > 1)
+        gated_scan_sums_kernel<T, V, GATE, BWD><<<static_cast<unsigned>(strips * (p.segments - 1)), kWarps * 32, 0, st>>>(p);
+    MB200_CUDA_CHECK(c, cudaLaunchKernel(fn, dim3(static_cast<unsigned>(strips * p.segments)), dim3(kWarps * 32), BWD ? bwd_args : fwd_args,
+                                         Lay::kBytes, st));
+    MB200_CUDA_CHECK(c, cudaGetLastError());
     return MAMBA_B200_OK;
 }
 
@@ -483,18 +527,19 @@ template <typename T, int V, bool GATE, bool BWD>
 static int configure(Ctx* c) {
     using Lay = Layout<T, V, (GATE ? 3 : 2) + (BWD ? 1 : 0)>;
     const void* fn = kernel<T, V, GATE, BWD>();
-    MB200_CUDA_CHECK(c, cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, Lay::kBytes + Lay::kMore));
-    MB200_CUDA_CHECK(c, cudaFuncSetAttribute(fn, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
+    MB200_CUDA_CHECK(c, cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, Lay::kBytes));
     return MAMBA_B200_OK;
 }
 
-// f32 rows of 32 channels and 16-bit rows of 64 are both 128 bytes; where 16-bit strips are few, they are halved.
+// A lane has two channels in 16 bits and one in f32: rows of 128 bytes.  Pairs are fetched as one word by the sums' kernel, so
+// rows that start on odd elements have one channel a lane.
 template <bool GATE, bool BWD>
 static int launch_typed(Ctx* c, const mamba_b200_gated_scan_args& a, cudaStream_t st) {
-    const bool few = static_cast<long long>(a.B) * ((a.D + 63) / 64) * 16 < 2 * c->sm_count;
     if (a.dtype == MAMBA_B200_F32) return launch_tiled<float, 1, GATE, BWD>(c, a, st);
-    if (a.dtype == MAMBA_B200_F16) return few ? launch_tiled<__half, 1, GATE, BWD>(c, a, st) : launch_tiled<__half, 2, GATE, BWD>(c, a, st);
-    return few ? launch_tiled<__nv_bfloat16, 1, GATE, BWD>(c, a, st) : launch_tiled<__nv_bfloat16, 2, GATE, BWD>(c, a, st);
+    auto words = [](const void* q, long long ld) { return reinterpret_cast<uintptr_t>(q) % 4 == 0 && ld % 2 == 0; };
+    const bool two = words(a.f, a.ld_f) && (BWD ? words(a.dy, a.ld_dy) : words(a.x, a.ld_x)) && (!(GATE && BWD) || words(a.z, a.ld_z));
+    if (a.dtype == MAMBA_B200_F16) return two ? launch_tiled<__half, 2, GATE, BWD>(c, a, st) : launch_tiled<__half, 1, GATE, BWD>(c, a, st);
+    return two ? launch_tiled<__nv_bfloat16, 2, GATE, BWD>(c, a, st) : launch_tiled<__nv_bfloat16, 1, GATE, BWD>(c, a, st);
 }
 
 }  // namespace gs
@@ -514,6 +559,13 @@ int gated_scan_configure(Ctx* c) {
 }  // namespace mb200
 
 using namespace mb200;
+
+extern "C" MAMBA_B200_API long long mamba_b200_gated_scan_workspace_bytes(int B, int T, int D) {
+    if (B <= 0 || T <= gs::kShort || D <= 0) return 0;
+    // (strips of 64 channels, or of 32: the more segments of the two; sized for 148 SMs, which a launch on fewer only halves further)
+    const int segments = gs::pick_segments(148, static_cast<long long>(B) * ((D + 63) / 64), (T + gs::kTile - 1) / gs::kTile);
+    return segments > 1 ? static_cast<long long>(segments) * B * D * 2 * sizeof(float) : 0;
+}
 
 extern "C" MAMBA_B200_API int mamba_b200_gated_scan_fwd(void* handle, void* stream, const mamba_b200_gated_scan_args* args) {
     Ctx* c = static_cast<Ctx*>(handle);

@@ -130,7 +130,7 @@ class GatedScanArgs(C.Structure):
         ("h0", C.c_void_p), ("h_last", C.c_void_p), ("y", C.c_void_p), ("ld_y", C.c_longlong), ("chunk_states", C.c_void_p),
         ("dy", C.c_void_p), ("ld_dy", C.c_longlong), ("d_last", C.c_void_p), ("d_h0", C.c_void_p),
         ("d_x", C.c_void_p), ("ld_dx", C.c_longlong), ("d_f", C.c_void_p), ("ld_df", C.c_longlong),
-        ("d_z", C.c_void_p), ("ld_dz", C.c_longlong),
+        ("d_z", C.c_void_p), ("ld_dz", C.c_longlong), ("workspace", C.c_void_p), ("workspace_bytes", C.c_longlong),
     ]
 
 
@@ -194,6 +194,7 @@ def lib() -> C.CDLL:
         bind("mamba_b200_embedding_bwd", [vp, vp, it, vp, ll, vp, vp, it, ll, it, it, fl, vp, ll])
         bind("mamba_b200_token_logprobs", [vp, vp, it, vp, ll, vp, fl, vp, vp, vp, it, vp, vp, ll, it])
         bind("mamba_b200_token_logprobs_bwd", [vp, vp, it, vp, ll, vp, fl, vp, vp, vp, vp, vp, ll, ll, it])
+        bind("mamba_b200_gated_scan_workspace_bytes", [it, it, it], ll)
         bind("mamba_b200_gated_scan_fwd", [vp, vp, C.POINTER(GatedScanArgs)])
         bind("mamba_b200_gated_scan_bwd", [vp, vp, C.POINTER(GatedScanArgs)])
         bind("mamba_b200_decode_workspace_bytes", [vp, C.POINTER(DecodeArgs)], ll)

@@ -20,7 +20,8 @@ __all__ = ["selective_scan_fwd", "selective_scan_fwd_workspace_bytes", "selectiv
            "residual_rmsnorm_fwd", "residual_rmsnorm_bwd", "embedding_gather", "softmax_xent", "adamw_step",
            "ssm_parallel_scan_fwd_nosave", "ssm_scan_fwd_save", "ssm_scan_bwd", "conv1d_fwd_nosave", "selective_scan_step", "conv1d_fwd", "conv1d_bwd", "m3_ssd_fwd", "m3_ssd_fwd_fused_kq", "m3_ssd_bwd", "dtype_code",
            "embedding_fwd", "embedding_bwd", "embedding_bwd_workspace_bytes", "token_logprobs", "token_logprobs_bwd",
-           "gated_scan_fwd", "gated_scan_bwd", "gated_scan_step", "gated_scan_states"]
+           "gated_scan_fwd", "gated_scan_bwd", "gated_scan_step", "gated_scan_states",
+           "gated_scan_workspace_bytes"]
 
 
 _DTYPES = {torch.float32: ffi.F32, torch.float16: ffi.F16, torch.bfloat16: ffi.BF16}
@@ -712,6 +713,23 @@ def gated_scan_states(B, T, D):
     return (B, -(-T // ffi.GATED_SCAN_SAVE), D)
 
 
+def gated_scan_workspace_bytes(B, T, D) -> int:
+    """Bytes of the scratch that lets a long axis of few channels run as segments side by side (0: it is not cut)."""
+    return int(ffi.lib().mamba_b200_gated_scan_workspace_bytes(B, T, D))
+
+
+def _gated_workspace(workspace, x):
+    """(tensor, address, bytes) of the scratch for x: the caller's, or one of its own where it is needed."""
+    if workspace is None:
+        need = ffi.lib().mamba_b200_gated_scan_workspace_bytes(*x.shape)
+        if not need:
+            return None, None, 0
+        workspace = torch.empty(need, dtype=torch.uint8, device=x.device)
+    elif workspace.device != x.device or not workspace.is_contiguous():
+        raise ValueError("the workspace is contiguous, on x's device")
+    return workspace, workspace.data_ptr(), workspace.numel() * workspace.element_size()
+
+
 def _gated_rows(t, name, like):
     """Row stride of a [B, T, D] view whose rows are one after another: any stride where there is but one row."""
     if t.dtype != like.dtype or t.shape != like.shape or t.device != like.device:
@@ -734,11 +752,12 @@ def _gated_state(t, name, x, shape=None):
     return _ptr(t)
 
 
-def gated_scan_fwd(x, f, z=None, *, h0=None, h_last=None, y=None, chunk_states=None, handle=None):
+def gated_scan_fwd(x, f, z=None, *, h0=None, h_last=None, y=None, chunk_states=None, workspace=None, handle=None):
     """Gated linear recurrence: u = sigmoid(-f), h_t = h_{t-1} + u_t (x_t - h_{t-1}), y = h * SiLU(z) (y = h without z).
     x, f, z, y [B,T,D] in a storage dtype, any row stride; h0 (zeros if None) and h_last (written if given, may be h0)
-    [B,D] f32; chunk_states f32 of gated_scan_states(B,T,D) receives what gated_scan_bwd needs.  Returns y."""
-    _require_cuda(x, f, z, h0, h_last, y, chunk_states)
+    [B,D] f32; chunk_states f32 of gated_scan_states(B,T,D) receives what gated_scan_bwd needs.  workspace: scratch of
+    gated_scan_workspace_bytes(B,T,D) bytes (made here if None).  Returns y."""
+    _require_cuda(x, f, z, h0, h_last, y, chunk_states, workspace)
     if y is None:
         y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
     B, T, D = x.shape
@@ -748,6 +767,8 @@ def gated_scan_fwd(x, f, z=None, *, h0=None, h_last=None, y=None, chunk_states=N
                           _ptr(z), 0 if z is None else _gated_rows(z, "z", x), _gated_state(h0, "h0", x),
                           _gated_state(h_last, "h_last", x), y.data_ptr(), _gated_rows(y, "y", x),
                           _gated_state(chunk_states, "chunk_states", x, gated_scan_states(B, T, D)))
+    if T > 8:
+        workspace, a.workspace, a.workspace_bytes = _gated_workspace(workspace, x)
     with _on(dev):
         rc = ffi.lib().mamba_b200_gated_scan_fwd(h.ptr, _stream(dev), C.byref(a))
     h.check(rc, "mamba_b200_gated_scan_fwd")
@@ -764,10 +785,11 @@ def gated_scan_step(x, f, h0, z=None, *, h_last=None, y=None, handle=None):
     return y
 
 
-def gated_scan_bwd(x, f, dy, chunk_states, z=None, *, d_last=None, d_h0=None, d_x=None, d_f=None, d_z=None, handle=None):
+def gated_scan_bwd(x, f, dy, chunk_states, z=None, *, d_last=None, d_h0=None, d_x=None, d_f=None, d_z=None, workspace=None,
+                   handle=None):
     """Backward of gated_scan_fwd from its chunk_states.  d_last [B,D] f32: gradient of the state that left (None: zeros).
     Returns dict(d_x, d_f, d_z (with z), d_h0 f32); the outputs may be given (columns of one projection's gradient, say)."""
-    _require_cuda(x, f, z, dy, chunk_states, d_last, d_h0, d_x, d_f, d_z)
+    _require_cuda(x, f, z, dy, chunk_states, d_last, d_h0, d_x, d_f, d_z, workspace)
     B, T, D = x.shape
     dev = x.device
     h = handle or ffi.default_handle(dev.index or 0)
@@ -782,6 +804,7 @@ def gated_scan_bwd(x, f, dy, chunk_states, z=None, *, d_last=None, d_h0=None, d_
                           dy.data_ptr(), _gated_rows(dy, "dy", x), _gated_state(d_last, "d_last", x), _gated_state(d_h0, "d_h0", x),
                           d_x.data_ptr(), _gated_rows(d_x, "d_x", x), d_f.data_ptr(), _gated_rows(d_f, "d_f", x),
                           _ptr(d_z), 0 if d_z is None else _gated_rows(d_z, "d_z", x))
+    workspace, a.workspace, a.workspace_bytes = _gated_workspace(workspace, x)
     with _on(dev):
         rc = ffi.lib().mamba_b200_gated_scan_bwd(h.ptr, _stream(dev), C.byref(a))
     h.check(rc, "mamba_b200_gated_scan_bwd")
