@@ -77,18 +77,19 @@ struct Params {
 // ---------------------------------------------------------------------------------------------------
 constexpr int kWarps = 4, L = kTile / kWarps;
 
-template <typename T, int V, int NIN>
+template <typename T, int V, int NIN, bool BWD>
 struct Layout {
-    static constexpr int CH = 32 * V;
+    static constexpr int CH = 32 * V, kStages = BWD ? 2 : 3, kSums = BWD ? 3 : 2;
     static constexpr uint32_t kIn = kTile * CH * sizeof(T);  // one input's tile
-    // two stages of inputs | the warps' sums (three each, the forward uses two) | barriers
-    static constexpr uint32_t oPart = 2 * NIN * kIn, oBar = oPart + 3 * kWarps * CH * sizeof(float);
-    static constexpr uint32_t kBytes = oBar + 16 + 128;
+    // stages of inputs | the warps' sums | barriers
+    static constexpr uint32_t oPart = kStages * NIN * kIn, oBar = oPart + kSums * kWarps * CH * sizeof(float);
+    static constexpr uint32_t kBytes = oBar + 8 * kStages + 128;
+    static_assert(3 * (kBytes + 1024) <= 228 * 1024, "three CTAs on an SM");
 };
 
-template <typename T, int V, int NIN>
+template <typename T, int V, int NIN, bool BWD>
 struct Tiles {
-    using Lay = Layout<T, V, NIN>;
+    using Lay = Layout<T, V, NIN, BWD>;
     const Params& p;
     unsigned char* sm;
     uint64_t* bars;
@@ -169,9 +170,9 @@ __global__ void __launch_bounds__(kWarps * 32, 3)
     gated_scan_fwd_kernel(const __grid_constant__ CUtensorMap mf, const __grid_constant__ CUtensorMap mx,
                           const __grid_constant__ CUtensorMap mz, const __grid_constant__ CUtensorMap my, const __grid_constant__ Params p) {
     constexpr int NIN = GATE ? 3 : 2;
-    using Lay = Layout<T, V, NIN>;
+    using Lay = Layout<T, V, NIN, false>;
     using C = Ch<V>;
-    constexpr int CH = Lay::CH;
+    constexpr int CH = Lay::CH, S = Lay::kStages;
     extern __shared__ unsigned char raw[];
     unsigned char* sm = raw + (128 - (smem_u32(raw) & 127)) % 128;
     float* part = reinterpret_cast<float*>(sm + Lay::oPart);
@@ -180,23 +181,26 @@ __global__ void __launch_bounds__(kWarps * 32, 3)
     const int strip = static_cast<int>(blockIdx.x) / p.segments, per_b = (p.a.D + CH - 1) / CH, b = strip / per_b;
     const int c0 = (strip - b * per_b) * CH, c = c0 + lane * V, D = p.a.D;
     if (threadIdx.x == 0) {
-        mbar_init(&bars[0], 1);
-        mbar_init(&bars[1], 1);
+        for (int i = 0; i < S; ++i) mbar_init(&bars[i], 1);
         fence_barrier_init();
     }
     __syncthreads();
-    Tiles<T, V, NIN> in{p, sm, bars, b, c0, warp, lane, true};
+    Tiles<T, V, NIN, false> in{p, sm, bars, b, c0, warp, lane, true};
     const CUtensorMap* maps[3] = {&mf, &mx, &mz};
     const void* src[3] = {p.a.f, p.a.x, p.a.z};
     const long long ld[3] = {p.a.ld_f, p.a.ld_x, p.a.ld_z};
     const int first = seg * p.per_segment, rounds = min(p.per_segment, p.tiles - first);
-    in.ask(0, first, maps);
+#pragma unroll
+    for (int i = 0; i < S - 1; ++i)
+        if (i < rounds) in.ask(i, first + i, maps);
     C carry = p.a.h0 ? get<V>(p.a.h0 + static_cast<long long>(b) * D, c, D) : C::splat(0.0f);
     if (seg > 0) carry = enter<V>(p, part, b, c, 0, seg, 1, carry);
+    int s = 0;
+    uint32_t parity = 0;
     for (int it = 0; it < rounds; ++it) {
-        const int k = first + it, s = it & 1;
+        const int k = first + it;
         C n[L], x[L], N = C::splat(0.0f), A = C::splat(0.0f);
-        in.wait(s, k, (it >> 1) & 1, src, ld);
+        in.wait(s, k, parity, src, ld);
         const T* sf = in.mine(s, 0);
         T* sx = in.mine(s, 1);
 #pragma unroll
@@ -209,7 +213,7 @@ __global__ void __launch_bounds__(kWarps * 32, 3)
         N.store(part + warp * CH + lane * V);
         A.store(part + (kWarps + warp) * CH + lane * V);
         __syncthreads();
-        if (it + 1 < rounds) in.ask(s ^ 1, k + 1, maps);
+        if (it + S - 1 < rounds) in.ask(s == 0 ? S - 1 : s - 1, k + S - 1, maps);
         C h = carry;
 #pragma unroll
         for (int w = 0; w < kWarps; ++w) {
@@ -239,6 +243,7 @@ __global__ void __launch_bounds__(kWarps * 32, 3)
             tma_store_3d(&my, in.at(s, 1), c0, k * kTile, b);
             tma_commit();
         }
+        if (++s == S) s = 0, parity ^= 1;
     }
     if (p.a.h_last && seg == p.segments - 1 && warp == 0) put(p.a.h_last + static_cast<long long>(b) * D, c, D, carry);
     if (p.tma_out && threadIdx.x == 0) tma_wait_read0();
@@ -253,9 +258,9 @@ __global__ void __launch_bounds__(kWarps * 32, 3)
                           const __grid_constant__ CUtensorMap mz, const __grid_constant__ CUtensorMap mdf, const __grid_constant__ CUtensorMap mdx,
                           const __grid_constant__ CUtensorMap mdz, const __grid_constant__ Params p) {
     constexpr int NIN = GATE ? 4 : 3;
-    using Lay = Layout<T, V, NIN>;
+    using Lay = Layout<T, V, NIN, true>;
     using C = Ch<V>;
-    constexpr int CH = Lay::CH;
+    constexpr int CH = Lay::CH, S = Lay::kStages;
     extern __shared__ unsigned char raw[];
     unsigned char* sm = raw + (128 - (smem_u32(raw) & 127)) % 128;
     float* part = reinterpret_cast<float*>(sm + Lay::oPart);
@@ -264,29 +269,32 @@ __global__ void __launch_bounds__(kWarps * 32, 3)
     const int strip = static_cast<int>(blockIdx.x) / p.segments, per_b = (p.a.D + CH - 1) / CH, b = strip / per_b;
     const int c0 = (strip - b * per_b) * CH, c = c0 + lane * V, D = p.a.D;
     if (threadIdx.x == 0) {
-        mbar_init(&bars[0], 1);
-        mbar_init(&bars[1], 1);
+        for (int i = 0; i < S; ++i) mbar_init(&bars[i], 1);
         fence_barrier_init();
     }
     __syncthreads();
-    Tiles<T, V, NIN> in{p, sm, bars, b, c0, warp, lane, true};
+    Tiles<T, V, NIN, true> in{p, sm, bars, b, c0, warp, lane, true};
     const CUtensorMap* maps[4] = {&mf, &mx, &me, &mz};
     const void* src[4] = {p.a.f, p.a.x, p.a.dy, p.a.z};
     const long long ld[4] = {p.a.ld_f, p.a.ld_x, p.a.ld_dy, p.a.ld_z};
     const int first = min((seg + 1) * p.per_segment, p.tiles) - 1, rounds = first + 1 - seg * p.per_segment;
     const C minus = C::splat(-1.0f);
-    if (rounds > 0) in.ask(0, first, maps);
+#pragma unroll
+    for (int i = 0; i < S - 1; ++i)
+        if (i < rounds) in.ask(i, first - i, maps);
     C carry = p.a.d_last ? mul(get<V>(p.a.d_last + static_cast<long long>(b) * D, c, D), minus) : C::splat(0.0f);
     const float* states = p.a.chunk_states + static_cast<long long>(b) * p.tiles * D;
     auto state = [&](int k) { return k >= 0 ? get<V>(states + static_cast<long long>(k) * D, c, D) : C::splat(0.0f); };
     C next = state(first);
     if (seg + 1 < p.segments) carry = enter<V>(p, part, b, c, p.segments - 1, seg, -1, carry);
+    int s = 0;
+    uint32_t parity = 0;
     for (int it = 0; it < rounds; ++it) {
-        const int k = first - it, s = it & 1;
+        const int k = first - it;
         C h = next;
         next = state(k - 1);
         C n[L], x[L], e[L], q[L], N = C::splat(0.0f), A = C::splat(0.0f), G = C::splat(0.0f);
-        in.wait(s, k, (it >> 1) & 1, src, ld);
+        in.wait(s, k, parity, src, ld);
         const T *sf = in.mine(s, 0), *sx = in.mine(s, 1), *se = in.mine(s, 2), *sz = in.mine(s, NIN - 1);
 #pragma unroll
         for (int j = 0; j < L; ++j) {
@@ -312,7 +320,7 @@ __global__ void __launch_bounds__(kWarps * 32, 3)
         A.store(part + (kWarps + warp) * CH + lane * V);
         G.store(part + (2 * kWarps + warp) * CH + lane * V);
         __syncthreads();
-        if (it + 1 < rounds) in.ask(s ^ 1, k - 1, maps);
+        if (it + S - 1 < rounds) in.ask(s == 0 ? S - 1 : s - 1, k - (S - 1), maps);
         C g = carry, start = carry;
 #pragma unroll
         for (int w = 0; w < kWarps - 1; ++w)
@@ -352,6 +360,7 @@ __global__ void __launch_bounds__(kWarps * 32, 3)
             if constexpr (GATE) tma_store_3d(&mdz, in.at(s, 3), c0, k * kTile, b);
             tma_commit();
         }
+        if (++s == S) s = 0, parity ^= 1;
     }
     if (p.a.d_h0 && seg == 0 && warp == 0) put(p.a.d_h0 + static_cast<long long>(b) * D, c, D, mul(carry, minus));
     if (p.tma_out && threadIdx.x == 0) tma_wait_read0();
@@ -495,7 +504,7 @@ static const void* kernel() {
 
 template <typename T, int V, bool GATE, bool BWD>
 static int launch_tiled(Ctx* c, const mamba_b200_gated_scan_args& a, cudaStream_t st) {
-    using Lay = Layout<T, V, (GATE ? 3 : 2) + (BWD ? 1 : 0)>;
+    using Lay = Layout<T, V, (GATE ? 3 : 2) + (BWD ? 1 : 0), BWD>;
     const void* fn = kernel<T, V, GATE, BWD>();
     Params p{a, c->d_status};
     const long long strips = static_cast<long long>(a.B) * ((a.D + Lay::CH - 1) / Lay::CH);
@@ -525,7 +534,7 @@ static int launch_tiled(Ctx* c, const mamba_b200_gated_scan_args& a, cudaStream_
 
 template <typename T, int V, bool GATE, bool BWD>
 static int configure(Ctx* c) {
-    using Lay = Layout<T, V, (GATE ? 3 : 2) + (BWD ? 1 : 0)>;
+    using Lay = Layout<T, V, (GATE ? 3 : 2) + (BWD ? 1 : 0), BWD>;
     const void* fn = kernel<T, V, GATE, BWD>();
     MB200_CUDA_CHECK(c, cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, Lay::kBytes));
     return MAMBA_B200_OK;
