@@ -75,16 +75,18 @@ struct Params {
 // in shared memory and leave by TMA, which also clips what lies outside the tensor.  Where there are few strips of channels,
 // time is cut into segments: a first kernel finds what each does to a state, and a CTA starts from what the earlier ones leave.
 // ---------------------------------------------------------------------------------------------------
-constexpr int kWarps = 4, L = kTile / kWarps;
+constexpr int kFwdWarps = 4, kBwdWarps = 4;
+constexpr int kFwdCtas = 3, kFwdStages = 3;
 
 template <typename T, int V, int NIN, bool BWD>
 struct Layout {
-    static constexpr int CH = 32 * V, kStages = BWD ? 2 : 3, kSums = BWD ? 3 : 2;
+    static constexpr int CH = 32 * V, kStages = BWD ? 2 : kFwdStages, kWarps = BWD ? kBwdWarps : kFwdWarps, L = kTile / kWarps;
     static constexpr uint32_t kIn = kTile * CH * sizeof(T);  // one input's tile
-    // stages of inputs | the warps' sums | barriers
-    static constexpr uint32_t oPart = kStages * NIN * kIn, oBar = oPart + kSums * kWarps * CH * sizeof(float);
+    // stages of inputs | backward: the warps' three sums (the forward's two lie in the place of f, which is done with) | barriers
+    static constexpr uint32_t oPart = kStages * NIN * kIn, oBar = oPart + (BWD ? 3 * kWarps * CH * sizeof(float) : 0);
     static constexpr uint32_t kBytes = oBar + 8 * kStages + 128;
-    static_assert(3 * (kBytes + 1024) <= 228 * 1024, "three CTAs on an SM");
+    static_assert((BWD ? 3 : kFwdCtas) * (kBytes + 1024) <= 228 * 1024, "CTAs on an SM");
+    static_assert(L * CH * sizeof(T) >= 2 * CH * sizeof(float), "two sums in a warp's rows of f");
 };
 
 template <typename T, int V, int NIN, bool BWD>
@@ -95,6 +97,7 @@ struct Tiles {
     uint64_t* bars;
     int b, c0, warp, lane;
     bool alive;
+    static constexpr int L = Lay::L;
 
     __device__ __forceinline__ T* at(int s, int i) const { return reinterpret_cast<T*>(sm + (s * NIN + i) * Lay::kIn); }
     // The warp's first row, this lane's first channel.
@@ -134,12 +137,15 @@ struct Tiles {
     }
 };
 
-// What segments from, from + step, ... up to (not including) to make of v, the warps sharing them.
-template <int V>
-__device__ __forceinline__ Ch<V> enter(const Params& p, float* part, int b, int c, int from, int to, int step, Ch<V> v) {
+// What enters a segment: the state (or gradient) that enters the call, of which the first kernel kept a copy in the place of the
+// sums that nobody needs (`copy`; the call may write its result over the original), through segments from, from + step, ...
+// before `to`, which the warps share.
+template <int V, int kWarps>
+__device__ __forceinline__ Ch<V> enter(const Params& p, float* part, int b, int c, int copy, int from, int to, int step) {
     using C = Ch<V>;
     constexpr int CH = 32 * V;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, n = (to - from) * step, per = (n + kWarps - 1) / kWarps;
+    asm volatile("griddepcontrol.wait;" ::: "memory");
     C N = C::splat(0.0f), A = C::splat(0.0f);
     for (int i0 = warp * per; i0 < min(n, (warp + 1) * per); i0 += 8) {
         C m[8], a[8];
@@ -158,24 +164,25 @@ __device__ __forceinline__ Ch<V> enter(const Params& p, float* part, int b, int 
     }
     N.store(part + warp * CH + lane * V);
     A.store(part + (kWarps + warp) * CH + lane * V);
+    C v = get<V>(p.sums + (static_cast<long long>(b) * p.segments + copy) * 2 * p.a.D, c, p.a.D);
     __syncthreads();
 #pragma unroll
     for (int w = 0; w < kWarps; ++w) v = over(C::load(part + w * CH + lane * V), C::load(part + (kWarps + w) * CH + lane * V), v);
+    fence_proxy_async();  // (a tile may come here)
     __syncthreads();
     return v;
 }
 
 template <typename T, int V, bool GATE>
-__global__ void __launch_bounds__(kWarps * 32, 3)
+__global__ void __launch_bounds__(kFwdWarps * 32, kFwdCtas)
     gated_scan_fwd_kernel(const __grid_constant__ CUtensorMap mf, const __grid_constant__ CUtensorMap mx,
                           const __grid_constant__ CUtensorMap mz, const __grid_constant__ CUtensorMap my, const __grid_constant__ Params p) {
     constexpr int NIN = GATE ? 3 : 2;
     using Lay = Layout<T, V, NIN, false>;
     using C = Ch<V>;
-    constexpr int CH = Lay::CH, S = Lay::kStages;
+    constexpr int CH = Lay::CH, S = Lay::kStages, W = Lay::kWarps, L = Lay::L;
     extern __shared__ unsigned char raw[];
     unsigned char* sm = raw + (128 - (smem_u32(raw) & 127)) % 128;
-    float* part = reinterpret_cast<float*>(sm + Lay::oPart);
     uint64_t* bars = reinterpret_cast<uint64_t*>(sm + Lay::oBar);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, seg = static_cast<int>(blockIdx.x) % p.segments;
     const int strip = static_cast<int>(blockIdx.x) / p.segments, per_b = (p.a.D + CH - 1) / CH, b = strip / per_b;
@@ -193,44 +200,48 @@ __global__ void __launch_bounds__(kWarps * 32, 3)
 #pragma unroll
     for (int i = 0; i < S - 1; ++i)
         if (i < rounds) in.ask(i, first + i, maps);
-    C carry = p.a.h0 ? get<V>(p.a.h0 + static_cast<long long>(b) * D, c, D) : C::splat(0.0f);
-    if (seg > 0) carry = enter<V>(p, part, b, c, 0, seg, 1, carry);
+    C carry = C::splat(0.0f);
+    if (p.segments > 1) carry = enter<V, W>(p, reinterpret_cast<float*>(in.at(S - 1, 0)), b, c, p.segments - 1, 0, seg, 1);
+    else if (p.a.h0) carry = get<V>(p.a.h0 + static_cast<long long>(b) * D, c, D);
     int s = 0;
     uint32_t parity = 0;
     for (int it = 0; it < rounds; ++it) {
         const int k = first + it;
-        C n[L], x[L], N = C::splat(0.0f), A = C::splat(0.0f);
+        // what the steps up to each one do to the state that enters the span, and the output gates
+        C n[L], a[L], q[GATE ? L : 1], N = C::splat(0.0f), A = C::splat(0.0f);
         in.wait(s, k, parity, src, ld);
-        const T* sf = in.mine(s, 0);
-        T* sx = in.mine(s, 1);
+        const T *sf = in.mine(s, 0), *sx = in.mine(s, 1), *sz = in.mine(s, NIN - 1);
 #pragma unroll
         for (int j = 0; j < L; ++j) {
-            n[j] = neg_gate(C::load(sf + j * CH), kLog2e);
-            x[j] = C::load(sx + j * CH);
-            A = fma(n[j], sub(A, x[j]), A);
-            N = both(N, n[j]);
-        }
-        N.store(part + warp * CH + lane * V);
-        A.store(part + (kWarps + warp) * CH + lane * V);
-        __syncthreads();
-        if (it + S - 1 < rounds) in.ask(s == 0 ? S - 1 : s - 1, k + S - 1, maps);
-        C h = carry;
-#pragma unroll
-        for (int w = 0; w < kWarps; ++w) {
-            if (w == warp) carry = h;  // (what enters this warp's span)
-            h = over(C::load(part + w * CH + lane * V), C::load(part + (kWarps + w) * CH + lane * V), h);
-        }
-        if (p.a.chunk_states && warp == 0) put(p.a.chunk_states + (static_cast<long long>(b) * p.tiles + k) * D, c, D, carry);
-        const T* sz = in.mine(s, NIN - 1);
-#pragma unroll
-        for (int j = 0; j < L; ++j) {
-            carry = fma(n[j], sub(carry, x[j]), carry);
+            const C u = neg_gate(C::load(sf + j * CH), kLog2e);
+            a[j] = A = fma(u, sub(A, C::load(sx + j * CH)), A);
+            n[j] = N = both(N, u);
             if constexpr (GATE) {
                 const C z = C::load(sz + j * CH);
-                mul(mul(carry, z), mul(neg_gate(z, -kLog2e), C::splat(-1.0f))).store(sx + j * CH);
-            } else {
-                carry.store(sx + j * CH);
+                q[j] = mul(z, neg_gate(z, -kLog2e));  // -SiLU(z)
             }
+        }
+        // the sums go where the warp's rows of f were: two rows of 4-byte channels
+        float* part = reinterpret_cast<float*>(in.at(s, 0));
+        constexpr int kStep = L * CH * sizeof(T) / sizeof(float);
+        __syncwarp();
+        N.store(part + warp * kStep + lane * V);
+        A.store(part + warp * kStep + CH + lane * V);
+        __syncthreads();
+        C h = carry;
+#pragma unroll
+        for (int w = 0; w < W; ++w) {
+            if (w == warp) carry = h;  // (what enters this warp's span)
+            h = over(C::load(part + w * kStep + lane * V), C::load(part + w * kStep + CH + lane * V), h);
+        }
+        if (p.a.chunk_states && warp == 0) put(p.a.chunk_states + (static_cast<long long>(b) * p.tiles + k) * D, c, D, carry);
+        T* sy = in.mine(s, 1);
+        const C minus = C::splat(-1.0f);
+#pragma unroll
+        for (int j = 0; j < L; ++j) {
+            const C o = over(n[j], a[j], carry);
+            if constexpr (GATE) mul(o, mul(q[j], minus)).store(sy + j * CH);
+            else o.store(sy + j * CH);
         }
         carry = h;
         fence_proxy_async();
@@ -239,6 +250,8 @@ __global__ void __launch_bounds__(kWarps * 32, 3)
             in.plain_out(s, 1, k, p.a.y, p.a.ld_y);
         }
         __syncthreads();
+        // the stage of the tile before: what was written from it has long been read
+        if (it + S - 1 < rounds) in.ask(s == 0 ? S - 1 : s - 1, k + S - 1, maps);
         if (p.tma_out && threadIdx.x == 0) {
             tma_store_3d(&my, in.at(s, 1), c0, k * kTile, b);
             tma_commit();
@@ -253,14 +266,14 @@ __global__ void __launch_bounds__(kWarps * 32, 3)
 // the same two walks; g is joined over the warps (and the cluster) the same way in the other direction: over a span of steps
 // (1 - u) g at its first step = g_behind - U g_behind + G, with the forward's U.  g runs with its sign turned, like the gates.
 template <typename T, int V, bool GATE>
-__global__ void __launch_bounds__(kWarps * 32, 3)
+__global__ void __launch_bounds__(kBwdWarps * 32, 3)
     gated_scan_bwd_kernel(const __grid_constant__ CUtensorMap mf, const __grid_constant__ CUtensorMap mx, const __grid_constant__ CUtensorMap me,
                           const __grid_constant__ CUtensorMap mz, const __grid_constant__ CUtensorMap mdf, const __grid_constant__ CUtensorMap mdx,
                           const __grid_constant__ CUtensorMap mdz, const __grid_constant__ Params p) {
     constexpr int NIN = GATE ? 4 : 3;
     using Lay = Layout<T, V, NIN, true>;
     using C = Ch<V>;
-    constexpr int CH = Lay::CH, S = Lay::kStages;
+    constexpr int CH = Lay::CH, S = Lay::kStages, W = Lay::kWarps, L = Lay::L;
     extern __shared__ unsigned char raw[];
     unsigned char* sm = raw + (128 - (smem_u32(raw) & 127)) % 128;
     float* part = reinterpret_cast<float*>(sm + Lay::oPart);
@@ -282,11 +295,12 @@ __global__ void __launch_bounds__(kWarps * 32, 3)
 #pragma unroll
     for (int i = 0; i < S - 1; ++i)
         if (i < rounds) in.ask(i, first - i, maps);
-    C carry = p.a.d_last ? mul(get<V>(p.a.d_last + static_cast<long long>(b) * D, c, D), minus) : C::splat(0.0f);
+    C carry = C::splat(0.0f);
+    if (p.segments > 1) carry = enter<V, W>(p, part, b, c, 0, p.segments - 1, seg, -1);
+    else if (p.a.d_last) carry = mul(get<V>(p.a.d_last + static_cast<long long>(b) * D, c, D), minus);
     const float* states = p.a.chunk_states + static_cast<long long>(b) * p.tiles * D;
     auto state = [&](int k) { return k >= 0 ? get<V>(states + static_cast<long long>(k) * D, c, D) : C::splat(0.0f); };
     C next = state(first);
-    if (seg + 1 < p.segments) carry = enter<V>(p, part, b, c, p.segments - 1, seg, -1, carry);
     int s = 0;
     uint32_t parity = 0;
     for (int it = 0; it < rounds; ++it) {
@@ -317,18 +331,18 @@ __global__ void __launch_bounds__(kWarps * 32, 3)
             G = fma(n[j], g, g);
         }
         N.store(part + warp * CH + lane * V);
-        A.store(part + (kWarps + warp) * CH + lane * V);
-        G.store(part + (2 * kWarps + warp) * CH + lane * V);
+        A.store(part + (W + warp) * CH + lane * V);
+        G.store(part + (2 * W + warp) * CH + lane * V);
         __syncthreads();
         if (it + S - 1 < rounds) in.ask(s == 0 ? S - 1 : s - 1, k - (S - 1), maps);
         C g = carry, start = carry;
 #pragma unroll
-        for (int w = 0; w < kWarps - 1; ++w)
-            if (w < warp) h = over(C::load(part + w * CH + lane * V), C::load(part + (kWarps + w) * CH + lane * V), h);
+        for (int w = 0; w < W - 1; ++w)
+            if (w < warp) h = over(C::load(part + w * CH + lane * V), C::load(part + (W + w) * CH + lane * V), h);
 #pragma unroll
-        for (int w = kWarps - 1; w >= 0; --w) {
+        for (int w = W - 1; w >= 0; --w) {
             if (w == warp) start = g;
-            g = over(C::load(part + w * CH + lane * V), C::load(part + (2 * kWarps + w) * CH + lane * V), g);
+            g = over(C::load(part + w * CH + lane * V), C::load(part + (2 * W + w) * CH + lane * V), g);
         }
         carry = g;
         T *df = in.mine(s, 0), *dx = in.mine(s, 1), *dz = in.mine(s, NIN - 1);
@@ -369,10 +383,11 @@ __global__ void __launch_bounds__(kWarps * 32, 3)
 // What each segment of time does to a state (forward) or to the gradient that comes from behind it, without results: f and x
 // (dy and z) are read once more than the floor.  A warp has a quarter of the segment, 16 steps at a time, all their loads in
 // flight; it ends where the kernel above begins, so that what it read last is still in L2 then.
+constexpr int kSumWarps = 8;  // (4: 61.5 us for one sequence of 32749 x 768, 8: 57.8, 16: 63.0)
 template <typename T, int V, bool GATE, bool BWD>
-__global__ void __launch_bounds__(kWarps * 32) gated_scan_sums_kernel(const __grid_constant__ Params p) {
+__global__ void __launch_bounds__(kSumWarps * 32) gated_scan_sums_kernel(const __grid_constant__ Params p) {
     using C = Ch<V>;
-    constexpr int CH = 32 * V, M = kTile / L;
+    constexpr int CH = 32 * V, kWarps = kSumWarps, L = 16, M = kTile / L;
     __shared__ __align__(8) float part[2 * kWarps * CH];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, parts = p.segments - 1;
     const int seg = static_cast<int>(blockIdx.x) % parts + (BWD ? 1 : 0), strip = static_cast<int>(blockIdx.x) / parts;
@@ -434,9 +449,17 @@ __global__ void __launch_bounds__(kWarps * 32) gated_scan_sums_kernel(const __gr
         A = over(m, C::load(part + (kWarps + w) * CH + lane * V), A);
         N = both(N, m);
     }
+    // From here on the other kernel's CTAs may start; they wait for this one's end before they read the sums.  (Let in at the
+    // beginning they took the room of CTAs that were still to come: 48 strips, 6 segments 80 us, 69 like this, 70 without.)
+    asm volatile("griddepcontrol.launch_dependents;");
     float* row = p.sums + (static_cast<long long>(b) * p.segments + seg) * 2 * D;
     put(row, c, D, N);
     put(row + D, c, D, A);
+    if (seg == (BWD ? 1 : 0)) {
+        const float* from = BWD ? p.a.d_last : p.a.h0;
+        const C v = from ? get<V>(from + static_cast<long long>(b) * D, c, D) : C::splat(0.0f);
+        put(p.sums + (static_cast<long long>(b) * p.segments + (BWD ? 0 : p.segments - 1)) * 2 * D, c, D, BWD ? mul(v, C::splat(-1.0f)) : v);
+    }
 }
 
 // Windows of a few steps (decoding: one): a thread has one channel and walks it, its loads in flight together.
@@ -488,12 +511,15 @@ static int check(Ctx* c, const mamba_b200_gated_scan_args* a, bool bwd) {
 }
 
 
-// Segments of time: as many as give every SM its three CTAs, none where half of that is there without.
+// Segments of time, so that every SM has its three CTAs.  Cut, f and x (dy and z) are read twice; whole, a CTA's tiles follow one
+// another at 1.1 us (backward 1.7).  us, whole and cut: 168 strips x 64 tiles 96 and 100 (backward 156 and 172), 120 x 64 74 and 72
+// (137 and 123), 80 x 128 144 and 103 (249 and 161), 12 x 128 140 and 20; 12 x 4 tiles are 5 whole and 6 cut.
 constexpr int kMaxSegments = 128;
 static int pick_segments(int sms, long long strips, int tiles) {
-    const long long want = strips * 2 > 3ll * sms ? 1 : 3ll * sms / strips;
+    if (strips * 10 > 9ll * sms || tiles <= 4) return 1;
+    const long long want = 3ll * sms / (strips > 0 ? strips : 1);
     const int most = static_cast<int>(want < kMaxSegments ? want : kMaxSegments);
-    return most < tiles ? most : (tiles > 0 ? tiles : 1);
+    return most < tiles ? most : tiles;
 }
 
 template <typename T, int V, bool GATE, bool BWD>
@@ -524,11 +550,23 @@ static int launch_tiled(Ctx* c, const mamba_b200_gated_scan_args& a, cudaStream_
     p.tma_out = BWD ? map(&o0, a.d_f, a.ld_df) && map(&o1, a.d_x, a.ld_dx) && (!GATE || map(&o2, a.d_z, a.ld_dz)) : map(&o0, a.y, a.ld_y);
     void* fwd_args[] = {&mf, &mx, &mz, &o0, &p};
     void* bwd_args[] = {&mf, &mx, &me, &mz, &o0, &o1, &o2, &p};
-    if (p.segments > 1)
-        gated_scan_sums_kernel<T, V, GATE, BWD><<<static_cast<unsigned>(strips * (p.segments - 1)), kWarps * 32, 0, st>>>(p);
-    MB200_CUDA_CHECK(c, cudaLaunchKernel(fn, dim3(static_cast<unsigned>(strips * p.segments)), dim3(kWarps * 32), BWD ? bwd_args : fwd_args,
-                                         Lay::kBytes, st));
-    MB200_CUDA_CHECK(c, cudaGetLastError());
+    cudaLaunchConfig_t cfg;
+    memset(&cfg, 0, sizeof(cfg));
+    cfg.gridDim = dim3(static_cast<unsigned>(strips * p.segments));
+    cfg.blockDim = dim3(Lay::kWarps * 32);
+    cfg.dynamicSmemBytes = Lay::kBytes;
+    cfg.stream = st;
+    cudaLaunchAttribute early;
+    memset(&early, 0, sizeof(early));
+    early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    early.val.programmaticStreamSerializationAllowed = 1;
+    if (p.segments > 1) {  // the second kernel asks for its first tiles while the first one ends
+        gated_scan_sums_kernel<T, V, GATE, BWD><<<static_cast<unsigned>(strips * (p.segments - 1)), kSumWarps * 32, 0, st>>>(p);
+        MB200_CUDA_CHECK(c, cudaGetLastError());
+        cfg.attrs = &early;
+        cfg.numAttrs = 1;
+    }
+    MB200_CUDA_CHECK(c, cudaLaunchKernelExC(&cfg, fn, BWD ? bwd_args : fwd_args));
     return MAMBA_B200_OK;
 }
 
