@@ -89,6 +89,7 @@ int norm_configure(Ctx* c);     // norm.cu
 int train_ops_configure(Ctx* c);  // train_ops.cu
 int decode_configure(Ctx* c);     // decode.cu
 int gated_scan_configure(Ctx* c);  // gated_scan.cu
+int logprobs_configure(Ctx* c);    // logprobs.cu
 
 }  // namespace mb200
 
@@ -133,6 +134,8 @@ extern "C" MAMBA_B200_API int mamba_b200_init(int device, void** handle) {
     rc = decode_configure(c);
     if (rc) return rc;
     rc = gated_scan_configure(c);
+    if (rc) return rc;
+    rc = logprobs_configure(c);
     if (rc) return rc;
     return MAMBA_B200_OK;
 }

@@ -118,6 +118,27 @@ def test_alternatives_among_many_equals(cuda_dev, dt):
 
 
 @pytest.mark.parametrize("dt", DT)
+@pytest.mark.parametrize("V", [20011, 50280])
+def test_alternatives_where_more_stand_out_than_there_is_room_for(cuda_dev, dt, V):
+    """Large logits that gather in a few columns of the row's layout, distinct and in runs of equals, at its start or its end."""
+    import torch
+
+    import mamba_rs_b200 as mb
+    i = torch.arange(V, device=cuda_dev)
+    rows = []
+    for span in (2048, 1024):  # (256 threads x 16 bytes, in 16 and 32 bits)
+        for few in (24, 160, 400):
+            top = i % span < few
+            rows += [torch.where(top, 100.0 + i * 0.5, 0.0), torch.where(top, 3.0, 0.0), torch.where(top, 3.0 + (i % 5), -math.inf),
+                     torch.where(top & (i > V // 2), 3.0, -1.0), torch.where(top, 2000.0 - (i // 7), -i * 0.01)]
+    l = torch.stack(rows).to(_dt(dt))
+    order = torch.sort(l.float(), dim=1, descending=True, stable=True)[1]
+    for top in (1, 20, 32):
+        for many in (1, 25):
+            assert torch.equal(mb.token_logprobs(l.repeat(many, 1), top=top)["top_ids"].long(), order[:, :top].repeat(many, 1))
+
+
+@pytest.mark.parametrize("dt", DT)
 def test_what_is_not_a_number_shows(cuda_dev, dt):
     import torch
 
