@@ -15,7 +15,7 @@
 namespace mb200 {
 namespace lp {
 
-constexpr int kThreads = 256, kWarps = kThreads / 32, kMaxTop = 32, kGroups = 128, kRoom = 1024, kUnroll = 4;
+constexpr int kThreads = 256, kWarps = kThreads / 32, kMaxTop = 32, kRoom = 1024, kUnroll = 4;
 constexpr float kNothing = -256.0f;  // 2^-256 is 0 in f32
 
 // max that a NaN passes through.
@@ -39,16 +39,48 @@ struct Piece {
             return j == 0 ? make_float2(__uint_as_float(q.x), __uint_as_float(q.y)) : make_float2(__uint_as_float(q.z), __uint_as_float(q.w));
         }
     }
-    // The largest (NaN aside).
-    __device__ __forceinline__ float top() const {
+    __device__ __forceinline__ void put(int i, T v) {  // (i known to the compiler)
         if constexpr (sizeof(T) == 4) {
-            return fmaxf(fmaxf(__uint_as_float(q.x), __uint_as_float(q.y)), fmaxf(__uint_as_float(q.z), __uint_as_float(q.w)));
-        } else if constexpr (std::is_same<T, __half>::value) {
-            const __half2 *h = reinterpret_cast<const __half2*>(&q), m = __hmax2(__hmax2(h[0], h[1]), __hmax2(h[2], h[3]));
-            return fmaxf(__low2float(m), __high2float(m));
+            (i == 0 ? q.x : q.y) = *reinterpret_cast<uint32_t*>(&v);
         } else {
-            const __nv_bfloat162 *h = reinterpret_cast<const __nv_bfloat162*>(&q), m = __hmax2(__hmax2(h[0], h[1]), __hmax2(h[2], h[3]));
+            const uint32_t w = *reinterpret_cast<unsigned short*>(&v);
+            q.x = i == 0 ? (q.x & 0xffff0000u) | w : (q.x & 0xffffu) | (w << 16);
+        }
+    }
+    // The largest of kUnroll pieces (NaN aside).
+    __device__ __forceinline__ static float top(const Piece* q) {
+        if constexpr (sizeof(T) == 4) {
+            float m = -INFINITY;
+#pragma unroll
+            for (int u = 0; u < kUnroll; ++u)
+#pragma unroll
+                for (int k = 0; k < 2; ++k) {
+                    const float2 v = q[u].pair(k);
+                    m = fmaxf(m, fmaxf(v.x, v.y));
+                }
+            return m;
+        } else {
+            using H2 = typename std::conditional<std::is_same<T, __half>::value, __half2, __nv_bfloat162>::type;
+            H2 m = *reinterpret_cast<const H2*>(&q[0].q.x);
+#pragma unroll
+            for (int u = 0; u < kUnroll; ++u) {
+                const H2* h = reinterpret_cast<const H2*>(&q[u].q);
+#pragma unroll
+                for (int k = 0; k < 4; ++k) m = __hmax2(m, h[k]);
+            }
             return fmaxf(__low2float(m), __high2float(m));
+        }
+    }
+    // No value below `lowest` (NaN stays).
+    __device__ __forceinline__ static void floor(Piece* q, float lowest) {
+        using H2 = typename std::conditional<std::is_same<T, __half>::value, __half2, __nv_bfloat162>::type;
+        const uint32_t w = pack2<T>(lowest, lowest);
+        const H2 lo = *reinterpret_cast<const H2*>(&w);
+#pragma unroll
+        for (int u = 0; u < kUnroll; ++u) {
+            H2* h = reinterpret_cast<H2*>(&q[u].q);
+#pragma unroll
+            for (int k = 0; k < 4; ++k) h[k] = __hmax2_nan(h[k], lo);
         }
     }
 };
@@ -81,62 +113,115 @@ struct FwdParams {
     float inv_temp;
 };
 
-// m: largest logit; s = sum of 2^d, s1 = sum of 2^d d with d = (logit - m) c.  Nothing yet: m is the lowest finite value, s 0
-// (so a row has something left if and only if its s is not 0).
+// top: largest logit.  With rho a reference near top c (c = log2 e / temperature; the product is rounded, but the same rho meets
+// every term): s = sum of 2^t, s1 = sum of 2^t t, t = logit c - rho in one rounding.  Then log2 S = log2 s - (top c - rho) and, in
+// base 2, the entropy = log2 s - s1 / s whatever rho is.
 struct Sums {
-    float m, s, s1;
-    __device__ __forceinline__ void raise(float to, float c) {
-        const float d = max_nan((m - to) * c, kNothing), e = ex2(d);
+    float top, rho, s, s1;
+    __device__ __forceinline__ void raise(float to) {
+        const float d = max_nan(rho - to, kNothing), e = ex2(d);
         s1 = e * fmaf(s, d, s1);
         s *= e;
-        m = to;
-    }
-    __device__ __forceinline__ void add(float v, float c) {
-        const float d = max_nan((v - m) * c, kNothing), e = ex2(d);
-        s += e;
-        s1 = fmaf(e, d, s1);
+        rho = to;
     }
 };
-constexpr float kLowest = -3.402823466e38f;
+constexpr float kFarDown = -1e37f;  // below any reference
+__device__ __forceinline__ Sums no_sums() { return {-INFINITY, kFarDown, 0.0f, 0.0f}; }
+// Where rho cannot follow the largest logit (a row of the type's lowest value: the product with c overflows, or 16-bit logits of
+// minus infinity cannot be told from it), the pass shows it by these and the row is summed again.
+__device__ __forceinline__ bool in_doubt(const Sums& a) { return a.top > -INFINITY && (a.s == 0.0f || (a.s == a.s && a.s1 != a.s1)); }
 
-__device__ __forceinline__ bool before(float v, int i, float v2, int i2) { return v > v2 || (v == v2 && i < i2); }
-__device__ __forceinline__ float ranked(float v) { return v == v ? v : -INFINITY; }
+// Sums over the lanes that differ in the bits below `lanes`, the same in each of them.
+__device__ __forceinline__ void join_lanes(Sums& a, int lanes) {
+    float rho = a.rho;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1)
+        if (o < lanes) {
+            a.top = fmaxf(a.top, __shfl_xor_sync(0xffffffffu, a.top, o));
+            rho = fmaxf(rho, __shfl_xor_sync(0xffffffffu, rho, o));
+        }
+    a.raise(rho);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1)
+        if (o < lanes) {
+            a.s += __shfl_xor_sync(0xffffffffu, a.s, o);
+            a.s1 += __shfl_xor_sync(0xffffffffu, a.s1, o);
+        }
+}
+__device__ __forceinline__ void join_block(Sums& a, Sums* part) {
+    join_lanes(a, 32);
+    if (threadIdx.x % 32 == 0) part[threadIdx.x / 32] = a;
+    __syncthreads();
+    a = part[threadIdx.x % kWarps];
+    join_lanes(a, kWarps);
+}
 
-// The alternatives of [lo, hi) pieces (and the ends) of a row, in order, in sel_v / sel_i[0 .. top); beyond what is there, index
-// 0x7fffffff.  Two threads' elements form a group.  tau, the top-th largest of the groups' maxima, is a lower bound of the
-// top-th largest element, so only groups that reach it are read again (from L2); what reaches it in them is ranked by counting.
-struct TopRoom {
-    float group[kGroups], v[kRoom], sel_v[kMaxTop];
-    int i[kRoom], sel_i[kMaxTop], n, best_i[kWarps];
-    float tau, best_v[kWarps];
-};
-
+// The sums of a whole row relative to its largest logit, term by term.
 template <typename T>
-__device__ __noinline__ void pick_top(TopRoom& t, const Row<T>& row, int lo, int hi, bool first, bool last, int top) {
+__device__ __noinline__ Sums sum_again(const Row<T>& row, float top, float c, Sums* part) {
+    Sums a{top, 0.0f, 0.0f, 0.0f};
+    for (int i = threadIdx.x; i < row.V; i += kThreads) {
+        const float t = max_nan((to_f(row.p[i]) - top) * c, kNothing), e = ex2(t);
+        a.s += e;
+        a.s1 = fmaf(e, t, a.s1);
+    }
+    __syncthreads();
+    join_block(a, part);
+    return a;
+}
+
+// Order of the alternatives: by falling logit (NaN as minus infinity), equal ones by rising index, as one number; 0 is none.
+__device__ __forceinline__ uint64_t key_of(float v, int i) {
+    const uint32_t b = __float_as_uint((v == v ? v : -INFINITY) + 0.0f);  // (-0 is 0)
+    return (static_cast<uint64_t>(b & 0x80000000u ? ~b : b | 0x80000000u) << 32) | (0xffffffffu - static_cast<uint32_t>(i));
+}
+__device__ __forceinline__ int key_index(uint64_t k) { return static_cast<int>(0xffffffffu - static_cast<uint32_t>(k)); }
+__device__ __forceinline__ float key_value(uint64_t k) {
+    const uint32_t b = static_cast<uint32_t>(k >> 32);
+    return __uint_as_float(b & 0x80000000u ? b & 0x7fffffffu : ~b);
+}
+
+struct TopRoom {
+    float group[32];
+    uint64_t key[kRoom], sel[kMaxTop], best[kWarps];
+    int n;
+};
+
+// The alternatives of [lo, hi) pieces (and the ends) of a row, in order, in sel[0 .. top).  Eight threads' elements form a group.
+// tau, the top-th largest of the 32 groups' maxima, is a lower bound of the top-th largest element: only what threads whose own
+// maximum reaches it have seen is read again (from L2), and what reaches it there is ranked by counting.
+template <typename T>
+__device__ __noinline__ void pick_top(TopRoom& t, const Row<T>& row, int lo, int hi, bool first, bool last, int top, float own_top) {
     constexpr int W = Piece<T>::W;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-    // (the groups' maxima are there; a barrier lies behind them)
-    if (tid < kGroups) {
-        const float mine = t.group[tid];
-        int rank = 0;
-        for (int j = 0; j < kGroups; ++j) rank += before(t.group[j], j, mine, tid);
-        if (rank == top - 1) t.tau = mine;
-    }
-    if (tid == 0) t.n = 0;
-    if (tid < kMaxTop) t.sel_v[tid] = -INFINITY, t.sel_i[tid] = 0x7fffffff;
-    __syncthreads();
-    const float tau = t.tau;
+    // (the groups' maxima and n = 0 are there; a barrier lies behind them)
+    float tau = t.group[lane];
+#pragma unroll
+    for (int size = 2; size <= 32; size <<= 1)
+#pragma unroll
+        for (int o = size >> 1; o > 0; o >>= 1) {
+            const float other = __shfl_xor_sync(0xffffffffu, tau, o);
+            tau = ((lane & o) == 0) == ((lane & size) == 0) ? fmaxf(tau, other) : fminf(tau, other);
+        }
+    tau = __shfl_sync(0xffffffffu, tau, top - 1);
+    if (tid < kMaxTop) t.sel[tid] = 0;
     auto offer = [&](float v, int i) {
-        v = ranked(v);
-        if (v > -INFINITY && v >= tau) {
+        if (v >= tau && v > -INFINITY) {
             const int at = atomicAdd(&t.n, 1);
-            if (at < kRoom) t.v[at] = v, t.i[at] = i;
+            if (at < kRoom) t.key[at] = key_of(v, i);
         }
     };
-    for (int g = warp; g < kGroups; g += kWarps) {
-        if (!(t.group[g] >= tau) || t.group[g] == -INFINITY) continue;
-        // the pieces of threads 2 g and 2 g + 1: lane l has every 16th of one of them
-        for (int j = lo + 2 * g + (lane & 1) + (lane >> 1) * kThreads; j < hi; j += 16 * kThreads) {
+    // half a warp for each such thread: a lane has every 16th of its pieces
+    unsigned reach = __ballot_sync(0xffffffffu, own_top >= tau && own_top > -INFINITY);
+    while (reach) {
+        const int one = __ffs(reach) - 1;
+        reach &= reach - 1;
+        const int two = reach ? __ffs(reach) - 1 : -1;
+        reach &= reach - 1;
+        const int who = lane < 16 ? one : two;
+        if (who < 0) continue;
+        const int x = warp * 32 + who;
+        for (int j = lo + x + (lane & 15) * kThreads; j < hi; j += 16 * kThreads) {
             Piece<T> q;
             q.load(row.p + row.head + j * W);
 #pragma unroll
@@ -146,174 +231,177 @@ __device__ __noinline__ void pick_top(TopRoom& t, const Row<T>& row, int lo, int
                 offer(v.y, row.head + j * W + e + 1);
             }
         }
-        if (lane < 2) {
-            const int i = 2 * g + lane;
-            if (first && i < row.head) offer(to_f(row.p[i]), i);
-            if (last && row.tail() + i < row.V) offer(to_f(row.p[row.tail() + i]), row.tail() + i);
-        }
+        if ((lane & 15) == 0 && first && x < row.head) offer(to_f(row.p[x]), x);
+        if ((lane & 15) == 1 && last && row.tail() + x < row.V) offer(to_f(row.p[row.tail() + x]), row.tail() + x);
     }
     __syncthreads();
     int n = t.n;
+    const bool crowded = n > kRoom;
     const int begin = first ? 0 : row.head + lo * W, end = last ? row.V : row.head + hi * W;
-    if (n > kRoom) {
+    if (crowded) {
         // More reach tau than there is room for: those above it one after the other, until tau itself is met.
         __syncthreads();
-        float last_v = INFINITY;
-        int last_i = -1, k = 0;
-        for (; k < top; ++k) {
-            float v = -INFINITY;
-            int at = 0x7fffffff;
+        uint64_t below = ~0ull;
+        for (n = 0; n < top; ++n) {
+            uint64_t k = 0;
             for (int i = begin + tid; i < end; i += kThreads) {
-                const float l = ranked(to_f(row.p[i]));
-                if (before(last_v, last_i, l, i) && before(l, i, v, at)) v = l, at = i;
+                const uint64_t k2 = key_of(to_f(row.p[i]), i);
+                if (k2 < below && k2 > k) k = k2;
             }
 #pragma unroll
             for (int o = 16; o > 0; o >>= 1) {
-                const float v2 = __shfl_xor_sync(0xffffffffu, v, o);
-                const int at2 = __shfl_xor_sync(0xffffffffu, at, o);
-                if (before(v2, at2, v, at)) v = v2, at = at2;
+                const uint64_t k2 = __shfl_xor_sync(0xffffffffu, k, o);
+                if (k2 > k) k = k2;
             }
-            if (lane == 0) t.best_v[warp] = v, t.best_i[warp] = at;
+            if (lane == 0) t.best[warp] = k;
             __syncthreads();
-            v = t.best_v[0], at = t.best_i[0];
-            for (int w = 1; w < kWarps; ++w)
-                if (before(t.best_v[w], t.best_i[w], v, at)) v = t.best_v[w], at = t.best_i[w];
+            for (int w = 0; w < kWarps; ++w)
+                if (t.best[w] > k) k = t.best[w];
             __syncthreads();
-            if (v <= tau) break;
-            last_v = v, last_i = at;
-            if (tid == 0) t.v[k] = v, t.i[k] = at;
+            if (key_value(k) <= tau) break;
+            below = k;
+            if (tid == 0) t.key[n] = k;
         }
-        n = k;
         __syncthreads();
     }
-    // in order by counting who comes before; each warp's lanes share a candidate's count
-    const int kept = n < top ? n : top;
-    for (int a = warp; a < n; a += kWarps) {
+    for (int a = tid; a < n; a += kThreads) {
+        const uint64_t mine = t.key[a];
         int rank = 0;
-        for (int b = lane; b < n; b += 32) rank += before(t.v[b], t.i[b], t.v[a], t.i[a]);
-        rank = __reduce_add_sync(0xffffffffu, rank);
-        if (lane == 0 && rank < top) t.sel_v[rank] = t.v[a], t.sel_i[rank] = t.i[a];
+        for (int b = 0; b < n; ++b) rank += t.key[b] > mine;
+        if (rank < top) t.sel[rank] = mine;
     }
-    if (kept < top) {
+    if (n < top && warp == 0) {
         // what is left are equals: tau where there was no room, else tokens that are ruled out.  The lowest indices.
-        const float equal = t.n > kRoom ? tau : -INFINITY;
-        if (warp == 0) {
-            int found = kept;
-            for (int i0 = begin; i0 < end && found < top; i0 += 8 * 32) {
-                bool hit[8];
+        const float equal = crowded ? tau : -INFINITY;
+        int found = n;
+        for (int i0 = begin; i0 < end && found < top; i0 += 8 * 32) {
+            bool hit[8];
 #pragma unroll
-                for (int u = 0; u < 8; ++u) {
-                    const int i = i0 + 32 * u + lane;
-                    hit[u] = i < end && ranked(to_f(row.p[i])) == equal;
-                }
+            for (int u = 0; u < 8; ++u) {
+                const int i = i0 + 32 * u + lane;
+                const float v = i < end ? to_f(row.p[i]) : 0.0f;
+                hit[u] = i < end && (v == v ? v : -INFINITY) == equal;
+            }
 #pragma unroll
-                for (int u = 0; u < 8; ++u) {
-                    const unsigned hits = __ballot_sync(0xffffffffu, hit[u]);
-                    const int at = found + __popc(hits & ((1u << lane) - 1));
-                    if (hit[u] && at < top) t.sel_v[at] = equal, t.sel_i[at] = i0 + 32 * u + lane;
-                    found += __popc(hits);
-                }
+            for (int u = 0; u < 8; ++u) {
+                const unsigned hits = __ballot_sync(0xffffffffu, hit[u]);
+                const int at = found + __popc(hits & ((1u << lane) - 1));
+                if (hit[u] && at < top) t.sel[at] = key_of(equal, i0 + 32 * u + lane);
+                found += __popc(hits);
             }
         }
     }
     __syncthreads();
 }
 
-// A CTA has a row, or with SPLIT the CTAs of a cluster have a piece of one each and the first joins what they found.
+// A CTA has a row, or with SPLIT the CTAs of a cluster have a part of one each and the first joins what they found.
 template <typename T, bool TOP, bool SPLIT>
 __global__ void __launch_bounds__(kThreads, 4) token_logprobs_kernel(const FwdParams p) {
     constexpr int W = Piece<T>::W;
-    __shared__ Sums part[kWarps], mine;
+    __shared__ Sums part[kWarps];
+    __shared__ __align__(16) Sums mine;
     __shared__ TopRoom room;
-    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int tid = threadIdx.x, lane = tid & 31;
     const float c = p.inv_temp * kLog2e;
     const int R = SPLIT ? p.split : 1, rank = SPLIT ? static_cast<int>(blockIdx.x) % R : 0;
     const long long r = SPLIT ? blockIdx.x / R : blockIdx.x;
     const Row<T> row(static_cast<const T*>(p.logits) + r * p.ld, p.V);
     const int lo = static_cast<int>(static_cast<long long>(row.pieces) * rank / R), hi = static_cast<int>(static_cast<long long>(row.pieces) * (rank + 1) / R);
     const bool first = rank == 0, last = rank == R - 1;
-    Sums a{kLowest, 0.0f, 0.0f};
-    float top_v = -INFINITY;
+    Sums a = no_sums();
     float2 s2 = splat2(0.0f), s12 = splat2(0.0f);
     const float2 cc = splat2(c);
-    for (int j0 = lo + tid; j0 < hi; j0 += kThreads * kUnroll) {
-        Piece<T> q[kUnroll];
+    const float margin = 200.0f / c;
+    auto take = [&](Piece<T>* q) {
+        a.top = fmaxf(a.top, Piece<T>::top(q));
+        if constexpr (sizeof(T) == 2) {
+            if (a.top == -INFINITY) {  // nothing but ruled out tokens (or NaN) yet
 #pragma unroll
-        for (int u = 0; u < kUnroll; ++u) {
-            const int j = j0 + u * kThreads;
-            if (j < hi) q[u].load(row.p + row.head + j * W);
-            else q[u].fill(minus_inf<T>());
+                for (int u = 0; u < kUnroll; ++u)
+#pragma unroll
+                    for (int k = 0; k < W / 2; ++k) {
+                        const float2 v = q[u].pair(k);
+                        if (v.x != v.x || v.y != v.y) s2.x = NAN;
+                    }
+                return;
+            }
         }
-        float m = q[0].top();
-#pragma unroll
-        for (int u = 1; u < kUnroll; ++u) m = fmaxf(m, q[u].top());
-        top_v = fmaxf(top_v, m);
-        const float to = fmaxf(a.m, m), d = fmaxf((a.m - to) * c, kNothing), e = ex2(d);
-        a.m = to;
+        const float to = fmaxf(a.rho, a.top * c), d = fmaxf(a.rho - to, kNothing), e = ex2(d);
+        a.rho = to;
         s12 = mul2(splat2(e), fma2(s2, splat2(d), s12));
         s2 = mul2(s2, splat2(e));
         const float2 neg = splat2(-to);
+        // 16-bit logits far below are brought to a finite one whose exponential is still 0, two at a time; f32 ones after the product
+        if constexpr (sizeof(T) == 2) Piece<T>::floor(q, a.top - margin - fabsf(a.top) * 0.015625f);
 #pragma unroll
         for (int u = 0; u < kUnroll; ++u)
 #pragma unroll
             for (int k = 0; k < W / 2; ++k) {
-                float2 t = mul2(add2(q[u].pair(k), neg), cc);
-                t.x = max_nan(t.x, kNothing), t.y = max_nan(t.y, kNothing);
+                float2 t = fma2(q[u].pair(k), cc, neg);
+                if constexpr (sizeof(T) == 4) t.x = max_nan(t.x, kNothing), t.y = max_nan(t.y, kNothing);
                 const float2 x = make_float2(ex2(t.x), ex2(t.y));
                 s2 = add2(s2, x);
                 s12 = fma2(x, t, s12);
             }
+    };
+    const T* base = row.p + row.head;
+    int j0 = lo + tid;
+    Piece<T> q[kUnroll], next[kUnroll];
+    const int whole = j0 < hi ? (hi - j0 + kThreads * kUnroll - 1 - (kUnroll - 1) * kThreads) / (kThreads * kUnroll) : 0;  // full rounds
+    if (whole > 0) {
+#pragma unroll
+        for (int u = 0; u < kUnroll; ++u) next[u].load(base + static_cast<long long>(j0 + u * kThreads) * W);
+    }
+    for (int k = 0; k < whole; ++k) {
+#pragma unroll
+        for (int u = 0; u < kUnroll; ++u) q[u] = next[u];
+        j0 += kThreads * kUnroll;
+        if (k + 1 < whole) {
+#pragma unroll
+            for (int u = 0; u < kUnroll; ++u) next[u].load(base + static_cast<long long>(j0 + u * kThreads) * W);
+        }
+        take(q);
+    }
+    // what is left of the thread's pieces, and the ends
+    const bool head = first && tid < row.head, tail = last && row.tail() + tid < p.V;
+    if (j0 < hi || head || tail) {
+#pragma unroll
+        for (int u = 0; u < kUnroll; ++u) {
+            q[u].fill(minus_inf<T>());
+            if (u < kUnroll - 1 && j0 + u * kThreads < hi) q[u].load(base + static_cast<long long>(j0 + u * kThreads) * W);
+        }
+        if (head) q[kUnroll - 1].put(0, row.p[tid]);
+        if (tail) q[kUnroll - 1].put(1, row.p[row.tail() + tid]);
+        take(q);
     }
     a.s = s2.x + s2.y, a.s1 = s12.x + s12.y;
-    // the ends
-    auto end = [&](int i) {
-        const float v = to_f(row.p[i]);
-        top_v = fmaxf(top_v, v);
-        a.raise(fmaxf(a.m, v), c);
-        a.add(v, c);
-    };
-    if (first && tid < row.head) end(tid);
-    if (last && row.tail() + tid < p.V) end(row.tail() + tid);
+    const float own_top = a.top;
     if (TOP) {
-        const float other = fmaxf(top_v, __shfl_xor_sync(0xffffffffu, top_v, 1));
-        if ((lane & 1) == 0) room.group[tid >> 1] = other;
+        float g = own_top;
+#pragma unroll
+        for (int o = 4; o > 0; o >>= 1) g = fmaxf(g, __shfl_xor_sync(0xffffffffu, g, o));
+        if (lane % 8 == 0) room.group[tid / 8] = g;
+        if (tid == 0) room.n = 0;
     }
-    auto join_lanes = [&](int from) {
-        float m = a.m;
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1)
-            if (o <= from) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-        a.raise(m, c);
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1)
-            if (o <= from) {
-                a.s += __shfl_xor_sync(0xffffffffu, a.s, o);
-                a.s1 += __shfl_xor_sync(0xffffffffu, a.s1, o);
-            }
-    };
-    join_lanes(16);
-    if (lane == 0) part[warp] = a;
-    __syncthreads();
-    a = part[lane % kWarps];
-    join_lanes(kWarps / 2);
-    if (TOP) pick_top<T>(room, row, lo, hi, first, last, p.top);
+    join_block(a, part);
+    if (TOP) pick_top<T>(room, row, lo, hi, first, last, p.top, own_top);
     if (SPLIT) {
         if (tid == 0) mine = a;
         cluster_sync();
         if (rank == 0) {
             const uint32_t at = smem_u32(&mine);
-            a = Sums{kLowest, 0.0f, 0.0f};
+            a = no_sums();
             if (lane < R) {
-                const uint32_t far = cluster_addr(at, lane);
-                a = Sums{ld_cluster1(far), ld_cluster1(far + 4), ld_cluster1(far + 8)};
+                const float4 v = ld_cluster4(cluster_addr(at, lane));
+                a = Sums{v.x, v.y, v.z, v.w};
             }
-            join_lanes(16);
-            if (TOP) {  // every piece's alternatives, in order by counting
-                const int n = R * p.top;
-                for (int i = tid; i < n; i += kThreads) {
+            join_lanes(a, 32);
+            if (TOP) {
+                for (int i = tid; i < R * p.top; i += kThreads) {
                     const int from = i / p.top, k = i - from * p.top;
-                    room.v[i] = ld_cluster1(cluster_addr(smem_u32(room.sel_v + k), from));
-                    room.i[i] = __float_as_int(ld_cluster1(cluster_addr(smem_u32(room.sel_i + k), from)));
+                    uint64_t v;
+                    asm volatile("ld.shared::cluster.u64 %0, [%1];" : "=l"(v) : "r"(cluster_addr(smem_u32(room.sel + k), from)));
+                    room.key[i] = v;
                 }
                 __syncthreads();
             }
@@ -321,33 +409,43 @@ __global__ void __launch_bounds__(kThreads, 4) token_logprobs_kernel(const FwdPa
         cluster_sync();
         if (rank != 0) return;
         if (TOP) {
-            const int n = R * p.top;
-            for (int i = warp; i < n; i += kWarps) {
-                int k = 0;
-                for (int b = lane; b < n; b += 32) k += before(room.v[b], room.i[b], room.v[i], room.i[i]);
-                k = __reduce_add_sync(0xffffffffu, k);
-                if (lane == 0 && k < p.top && room.i[i] != 0x7fffffff) room.sel_v[k] = room.v[i], room.sel_i[k] = room.i[i];
+            // each part's alternatives are in order: a token's place is the sum of its places in the parts
+            for (int i = tid; i < R * p.top; i += kThreads) {
+                const uint64_t v = room.key[i];
+                int place = 0;
+                for (int f = 0; f < R; ++f) {
+                    const uint64_t* list = room.key + f * p.top;
+                    int at = 0;
+#pragma unroll
+                    for (int step = 32; step > 0; step >>= 1)
+                        if (at + step <= p.top && list[at + step - 1] > v) at += step;
+                    place += at;
+                }
+                if (v != 0 && place < p.top) room.sel[place] = v;
             }
             __syncthreads();
         }
     }
-    const float log_s = lg2(a.s) * kLn2;
+    if (in_doubt(a)) a = sum_again(row, a.top, c, part);  // (alike in all threads)
+    else a.rho = fmaf(a.top, c, -a.rho);                  // top c - rho
+    const float log_s = (lg2(a.s) - a.rho) * kLn2;
     const bool none = a.s == 0.0f;
     if (tid == 0) {
         if (p.lse) {
-            p.lse[r] = none ? -INFINITY : a.s == a.s ? a.m : a.s;
+            p.lse[r] = a.s == a.s ? a.top : a.s;
             p.lse[p.rows + r] = none ? 0.0f : log_s;
         }
-        if (p.entropy) p.entropy[r] = none ? 0.0f : log_s - a.s1 / a.s * kLn2;
+        if (p.entropy) p.entropy[r] = none ? 0.0f : (lg2(a.s) - a.s1 / a.s) * kLn2;
     }
     if (tid == 32 && p.targets && p.logprob) {
         const int t = p.targets[r];
         const bool ok = t >= 0 && t < p.V;
-        p.logprob[r] = !ok ? 0.0f : none ? -INFINITY : (to_f(row.p[t]) - a.m) * p.inv_temp - log_s;
+        p.logprob[r] = !ok ? 0.0f : none ? -INFINITY : (to_f(row.p[t]) - a.top) * p.inv_temp - log_s;
     }
     if (TOP && tid < p.top) {
-        p.top_ids[r * p.top + tid] = room.sel_i[tid];
-        p.top_logprobs[r * p.top + tid] = none ? -INFINITY : (room.sel_v[tid] - a.m) * p.inv_temp - log_s;
+        const uint64_t k = room.sel[tid];
+        p.top_ids[r * p.top + tid] = key_index(k);
+        p.top_logprobs[r * p.top + tid] = none ? -INFINITY : (key_value(k) - a.top) * p.inv_temp - log_s;
     }
 }
 
