@@ -11,11 +11,12 @@
 
 #include "common.cuh"
 #include "internal.h"
+#include "m3_tc.cuh"
 
 namespace mb200 {
 namespace lp {
 
-constexpr int kThreads = 256, kWarps = kThreads / 32, kMaxTop = 32, kRoom = 1024, kUnroll = 4;
+constexpr int kThreads = 256, kWarps = kThreads / 32, kMaxTop = 32, kRoom = 512, kUnroll = 4, kCtas = 4;
 constexpr float kNothing = -256.0f;  // 2^-256 is 0 in f32
 
 // max that a NaN passes through.
@@ -31,7 +32,6 @@ struct Piece {
     static constexpr int W = 16 / sizeof(T);
     uint4 q;
     __device__ __forceinline__ void load(const T* p) { q = *reinterpret_cast<const uint4*>(p); }
-    __device__ __forceinline__ void fill(uint32_t w) { q = make_uint4(w, w, w, w); }
     __device__ __forceinline__ float2 pair(int j) const {
         if constexpr (sizeof(T) == 2) {
             return unpack2<T>(j == 0 ? q.x : j == 1 ? q.y : j == 2 ? q.z : q.w);
@@ -39,20 +39,12 @@ struct Piece {
             return j == 0 ? make_float2(__uint_as_float(q.x), __uint_as_float(q.y)) : make_float2(__uint_as_float(q.z), __uint_as_float(q.w));
         }
     }
-    __device__ __forceinline__ void put(int i, T v) {  // (i known to the compiler)
-        if constexpr (sizeof(T) == 4) {
-            (i == 0 ? q.x : q.y) = *reinterpret_cast<uint32_t*>(&v);
-        } else {
-            const uint32_t w = *reinterpret_cast<unsigned short*>(&v);
-            q.x = i == 0 ? (q.x & 0xffff0000u) | w : (q.x & 0xffffu) | (w << 16);
-        }
-    }
-    // The largest of kUnroll pieces (NaN aside).
-    __device__ __forceinline__ static float top(const Piece* q) {
+    // The largest of N pieces (NaN aside).
+    template <int N> __device__ __forceinline__ static float top(const Piece* q) {
         if constexpr (sizeof(T) == 4) {
             float m = -INFINITY;
 #pragma unroll
-            for (int u = 0; u < kUnroll; ++u)
+            for (int u = 0; u < N; ++u)
 #pragma unroll
                 for (int k = 0; k < 2; ++k) {
                     const float2 v = q[u].pair(k);
@@ -63,7 +55,7 @@ struct Piece {
             using H2 = typename std::conditional<std::is_same<T, __half>::value, __half2, __nv_bfloat162>::type;
             H2 m = *reinterpret_cast<const H2*>(&q[0].q.x);
 #pragma unroll
-            for (int u = 0; u < kUnroll; ++u) {
+            for (int u = 0; u < N; ++u) {
                 const H2* h = reinterpret_cast<const H2*>(&q[u].q);
 #pragma unroll
                 for (int k = 0; k < 4; ++k) m = __hmax2(m, h[k]);
@@ -71,24 +63,7 @@ struct Piece {
             return fmaxf(__low2float(m), __high2float(m));
         }
     }
-    // No value below `lowest` (NaN stays).
-    __device__ __forceinline__ static void floor(Piece* q, float lowest) {
-        using H2 = typename std::conditional<std::is_same<T, __half>::value, __half2, __nv_bfloat162>::type;
-        const uint32_t w = pack2<T>(lowest, lowest);
-        const H2 lo = *reinterpret_cast<const H2*>(&w);
-#pragma unroll
-        for (int u = 0; u < kUnroll; ++u) {
-            H2* h = reinterpret_cast<H2*>(&q[u].q);
-#pragma unroll
-            for (int k = 0; k < 4; ++k) h[k] = __hmax2_nan(h[k], lo);
-        }
-    }
 };
-template <typename T> __device__ __forceinline__ uint32_t minus_inf();
-template <> __device__ __forceinline__ uint32_t minus_inf<float>() { return 0xff800000u; }
-template <> __device__ __forceinline__ uint32_t minus_inf<__half>() { return 0xfc00fc00u; }
-template <> __device__ __forceinline__ uint32_t minus_inf<__nv_bfloat16>() { return 0xff80ff80u; }
-
 // A row in 16-byte pieces: `head` elements before the first aligned one, `pieces`, and a tail of less than one.
 template <typename T>
 struct Row {
@@ -113,8 +88,8 @@ struct FwdParams {
     float inv_temp;
 };
 
-// top: largest logit.  With rho a reference near top c (c = log2 e / temperature; the product is rounded, but the same rho meets
-// every term): s = sum of 2^t, s1 = sum of 2^t t, t = logit c - rho in one rounding.  Then log2 S = log2 s - (top c - rho) and, in
+// top: largest logit.  With rho a reference near top c (c = log2 e / temperature; the product is rounded, and rho may lie up to
+// kSlack below, but the same rho meets every term): s = sum of 2^t, s1 = sum of 2^t t, t = logit c - rho in one rounding.  Then log2 S = log2 s - (top c - rho) and, in
 // base 2, the entropy = log2 s - s1 / s whatever rho is.
 struct Sums {
     float top, rho, s, s1;
@@ -126,10 +101,70 @@ struct Sums {
     }
 };
 constexpr float kFarDown = -1e37f;  // below any reference
+constexpr float kSlack = 60.0f;     // a term may be 2^60: f32 sums have room for that
 __device__ __forceinline__ Sums no_sums() { return {-INFINITY, kFarDown, 0.0f, 0.0f}; }
 // Where rho cannot follow the largest logit (a row of the type's lowest value: the product with c overflows, or 16-bit logits of
 // minus infinity cannot be told from it), the pass shows it by these and the row is summed again.
 __device__ __forceinline__ bool in_doubt(const Sums& a) { return a.top > -INFINITY && (a.s == 0.0f || (a.s == a.s && a.s1 != a.s1)); }
+
+// A thread's running sums over pieces of a row, two chains.
+template <typename T>
+struct Running {
+    float top, rho;
+    float2 s, s1;
+    __device__ __forceinline__ Running() : top(-INFINITY), rho(kFarDown), s(splat2(0.0f)), s1(splat2(0.0f)) {}
+    __device__ __forceinline__ Sums sums() const { return {top, rho, s.x + s.y, s1.x + s1.y}; }
+
+    // N pieces, kThreads apart, from `at`.
+    template <int N>
+    __device__ __forceinline__ void take(const T* at, float c) {
+        constexpr int W = Piece<T>::W;
+        Piece<T> q[N];
+#pragma unroll
+        for (int u = 0; u < N; ++u) q[u].load(at + u * kThreads * W);
+        top = fmaxf(top, Piece<T>::template top<N>(q));
+        if (top * c > rho + kSlack) raise(top * c);  // (the first time, and where a row rises steeply)
+        const float2 cc = splat2(c), neg = splat2(-rho), was = s1;
+#pragma unroll
+        for (int u = 0; u < N; ++u)
+#pragma unroll
+            for (int k = 0; k < W / 2; ++k) {
+                const float2 t = fma2(q[u].pair(k), cc, neg), x = make_float2(ex2(t.x), ex2(t.y));
+                s = add2(s, x);
+                s1 = fma2(x, t, s1);
+            }
+        // A logit of minus infinity has made 0 times minus infinity of its term (unless the sum is NaN already, and stays so).
+        if (!(s1.x + s1.y == s1.x + s1.y)) s1 = again<N>(at, c, was);
+    }
+    template <int N>
+    __device__ __noinline__ float2 again(const T* at, float c, float2 sum) const {
+#pragma unroll 1
+        for (int u = 0; u < N; ++u) {
+            Piece<T> q;
+            q.load(at + u * kThreads * Piece<T>::W);
+#pragma unroll
+            for (int k = 0; k < Piece<T>::W / 2; ++k) {
+                float2 t = fma2(q.pair(k), splat2(c), splat2(-rho));
+                t.x = max_nan(t.x, kNothing), t.y = max_nan(t.y, kNothing);
+                sum = fma2(make_float2(ex2(t.x), ex2(t.y)), t, sum);
+            }
+        }
+        return sum;
+    }
+    __device__ __forceinline__ void raise(float to) {
+        const float d = fmaxf(rho - to, kNothing), e = ex2(d);
+        rho = to;
+        s1 = mul2(splat2(e), fma2(s, splat2(d), s1));
+        s = mul2(s, splat2(e));
+    }
+    __device__ __forceinline__ void end(float v, float c) {
+        top = fmaxf(top, v);
+        if (top * c > rho + kSlack) raise(top * c);
+        const float t = max_nan(fmaf(v, c, -rho), kNothing), x = ex2(t);
+        s.x += x;
+        s1.x = fmaf(x, t, s1.x);
+    }
+};
 
 // Sums over the lanes that differ in the bits below `lanes`, the same in each of them.
 __device__ __forceinline__ void join_lanes(Sums& a, int lanes) {
@@ -148,25 +183,22 @@ __device__ __forceinline__ void join_lanes(Sums& a, int lanes) {
             a.s1 += __shfl_xor_sync(0xffffffffu, a.s1, o);
         }
 }
-__device__ __forceinline__ void join_block(Sums& a, Sums* part) {
-    join_lanes(a, 32);
-    if (threadIdx.x % 32 == 0) part[threadIdx.x / 32] = a;
-    __syncthreads();
-    a = part[threadIdx.x % kWarps];
-    join_lanes(a, kWarps);
-}
-
-// The sums of a whole row relative to its largest logit, term by term.
+// The sums of a whole row relative to its largest logit, term by term, by one warp.
 template <typename T>
-__device__ __noinline__ Sums sum_again(const Row<T>& row, float top, float c, Sums* part) {
+__device__ __noinline__ Sums sum_again(const Row<T>& row, float top, float c) {
     Sums a{top, 0.0f, 0.0f, 0.0f};
-    for (int i = threadIdx.x; i < row.V; i += kThreads) {
-        const float t = max_nan((to_f(row.p[i]) - top) * c, kNothing), e = ex2(t);
-        a.s += e;
-        a.s1 = fmaf(e, t, a.s1);
+    for (int i0 = threadIdx.x % 32; i0 < row.V; i0 += 8 * 32) {
+        float v[8];
+#pragma unroll
+        for (int u = 0; u < 8; ++u) v[u] = i0 + 32 * u < row.V ? to_f(row.p[i0 + 32 * u]) : -INFINITY;
+#pragma unroll
+        for (int u = 0; u < 8; ++u) {
+            const float t = max_nan((v[u] - top) * c, kNothing), e = ex2(t);
+            a.s += e;
+            a.s1 = fmaf(e, t, a.s1);
+        }
     }
-    __syncthreads();
-    join_block(a, part);
+    join_lanes(a, 32);
     return a;
 }
 
@@ -181,20 +213,29 @@ __device__ __forceinline__ float key_value(uint64_t k) {
     return __uint_as_float(b & 0x80000000u ? b & 0x7fffffffu : ~b);
 }
 
+constexpr int kGroup = kThreads / 32;  // threads of a group
 struct TopRoom {
     float group[32];
     uint64_t key[kRoom], sel[kMaxTop], best[kWarps];
     int n;
 };
+__device__ __forceinline__ void group_max(TopRoom& t, float own_top) {
+#pragma unroll
+    for (int o = kGroup / 2; o > 0; o >>= 1) own_top = fmaxf(own_top, __shfl_xor_sync(0xffffffffu, own_top, o));
+    if (threadIdx.x % kGroup == 0) t.group[threadIdx.x / kGroup] = own_top;
+}
+__device__ __forceinline__ void sync_consumers() { asm volatile("bar.sync 1, %0;" ::"n"(kThreads) : "memory"); }
 
-// The alternatives of [lo, hi) pieces (and the ends) of a row, in order, in sel[0 .. top).  Eight threads' elements form a group.
-// tau, the top-th largest of the 32 groups' maxima, is a lower bound of the top-th largest element: only what threads whose own
-// maximum reaches it have seen is read again (from L2), and what reaches it there is ranked by counting.
+// The alternatives of [lo, hi) pieces (and the ends) of a row.  Eight threads' elements form a group.  tau, the top-th largest of
+// the 32 groups' maxima, is a lower bound of the top-th largest element: only what threads whose own maximum reaches it have seen
+// is read again (from L2), and what reaches it there goes to key[0 .. n) in any order.  Called by kThreads threads behind a
+// barrier that the groups' maxima and n = 0 have passed; a barrier ends it.  Returns how many keys there are: all that reach tau,
+// or where there was no room the largest (what is left equals tau then); or kInOrder, when sel is complete.
+constexpr int kInOrder = -1;
 template <typename T>
-__device__ __noinline__ void pick_top(TopRoom& t, const Row<T>& row, int lo, int hi, bool first, bool last, int top, float own_top) {
+__device__ __noinline__ int reach(TopRoom& t, const Row<T>& row, int lo, int hi, bool first, bool last, int top, float own_top, float* equals) {
     constexpr int W = Piece<T>::W;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-    // (the groups' maxima and n = 0 are there; a barrier lies behind them)
     float tau = t.group[lane];
 #pragma unroll
     for (int size = 2; size <= 32; size <<= 1)
@@ -204,7 +245,6 @@ __device__ __noinline__ void pick_top(TopRoom& t, const Row<T>& row, int lo, int
             tau = ((lane & o) == 0) == ((lane & size) == 0) ? fmaxf(tau, other) : fminf(tau, other);
         }
     tau = __shfl_sync(0xffffffffu, tau, top - 1);
-    if (tid < kMaxTop) t.sel[tid] = 0;
     auto offer = [&](float v, int i) {
         if (v >= tau && v > -INFINITY) {
             const int at = atomicAdd(&t.n, 1);
@@ -212,18 +252,19 @@ __device__ __noinline__ void pick_top(TopRoom& t, const Row<T>& row, int lo, int
         }
     };
     // half a warp for each such thread: a lane has every 16th of its pieces
-    unsigned reach = __ballot_sync(0xffffffffu, own_top >= tau && own_top > -INFINITY);
-    while (reach) {
-        const int one = __ffs(reach) - 1;
-        reach &= reach - 1;
-        const int two = reach ? __ffs(reach) - 1 : -1;
-        reach &= reach - 1;
-        const int who = lane < 16 ? one : two;
-        if (who < 0) continue;
-        const int x = warp * 32 + who;
-        for (int j = lo + x + (lane & 15) * kThreads; j < hi; j += 16 * kThreads) {
+    unsigned who = __ballot_sync(0xffffffffu, own_top >= tau && own_top > -INFINITY);
+    while (who) {
+        const int one = __ffs(who) - 1;
+        who &= who - 1;
+        const int two = who ? __ffs(who) - 1 : -1;
+        who &= who - 1;
+        const int x = lane < 16 ? one : two;
+        if (x < 0) continue;
+        const int y = warp * 32 + x;
+        for (int j = lo + y + (lane & 15) * kThreads; j < hi; j += 16 * kThreads) {
             Piece<T> q;
-            q.load(row.p + row.head + j * W);
+            q.load(row.p + row.head + static_cast<long long>(j) * W);
+            if (Piece<T>::template top<1>(&q) < tau) continue;
 #pragma unroll
             for (int e = 0; e < W; e += 2) {
                 const float2 v = q.pair(e / 2);
@@ -231,222 +272,400 @@ __device__ __noinline__ void pick_top(TopRoom& t, const Row<T>& row, int lo, int
                 offer(v.y, row.head + j * W + e + 1);
             }
         }
-        if ((lane & 15) == 0 && first && x < row.head) offer(to_f(row.p[x]), x);
-        if ((lane & 15) == 1 && last && row.tail() + x < row.V) offer(to_f(row.p[row.tail() + x]), row.tail() + x);
+        if ((lane & 15) == 0 && first && y < row.head) offer(to_f(row.p[y]), y);
+        if ((lane & 15) == 1 && last && row.tail() + y < row.V) offer(to_f(row.p[row.tail() + y]), row.tail() + y);
     }
-    __syncthreads();
-    int n = t.n;
-    const bool crowded = n > kRoom;
+    sync_consumers();
+    const int n = t.n;
+    *equals = -INFINITY;
+    if (n <= 64) return n;
+    if (n <= kRoom) {  // (many equals: one warp alone would take long)
+        for (int a = tid; a < n; a += kThreads) {
+            const uint64_t mine = t.key[a];
+            int rank = 0;
+            for (int b = 0; b < n; ++b) rank += t.key[b] > mine;
+            if (rank < top) t.sel[rank] = mine;
+        }
+        sync_consumers();
+        return kInOrder;
+    }
+    // More reach tau than there is room for: those above it one after the other, until tau itself is met.
+    sync_consumers();
+    *equals = tau;
     const int begin = first ? 0 : row.head + lo * W, end = last ? row.V : row.head + hi * W;
-    if (crowded) {
-        // More reach tau than there is room for: those above it one after the other, until tau itself is met.
-        __syncthreads();
-        uint64_t below = ~0ull;
-        for (n = 0; n < top; ++n) {
-            uint64_t k = 0;
-            for (int i = begin + tid; i < end; i += kThreads) {
-                const uint64_t k2 = key_of(to_f(row.p[i]), i);
-                if (k2 < below && k2 > k) k = k2;
-            }
-#pragma unroll
-            for (int o = 16; o > 0; o >>= 1) {
-                const uint64_t k2 = __shfl_xor_sync(0xffffffffu, k, o);
-                if (k2 > k) k = k2;
-            }
-            if (lane == 0) t.best[warp] = k;
-            __syncthreads();
-            for (int w = 0; w < kWarps; ++w)
-                if (t.best[w] > k) k = t.best[w];
-            __syncthreads();
-            if (key_value(k) <= tau) break;
-            below = k;
-            if (tid == 0) t.key[n] = k;
+    uint64_t below = ~0ull;
+    int k = 0;
+    for (; k < top; ++k) {
+        uint64_t best = 0;
+        for (int i = begin + tid; i < end; i += kThreads) {
+            const uint64_t k2 = key_of(to_f(row.p[i]), i);
+            if (k2 < below && k2 > best) best = k2;
         }
-        __syncthreads();
-    }
-    for (int a = tid; a < n; a += kThreads) {
-        const uint64_t mine = t.key[a];
-        int rank = 0;
-        for (int b = 0; b < n; ++b) rank += t.key[b] > mine;
-        if (rank < top) t.sel[rank] = mine;
-    }
-    if (n < top && warp == 0) {
-        // what is left are equals: tau where there was no room, else tokens that are ruled out.  The lowest indices.
-        const float equal = crowded ? tau : -INFINITY;
-        int found = n;
-        for (int i0 = begin; i0 < end && found < top; i0 += 8 * 32) {
-            bool hit[8];
 #pragma unroll
-            for (int u = 0; u < 8; ++u) {
-                const int i = i0 + 32 * u + lane;
-                const float v = i < end ? to_f(row.p[i]) : 0.0f;
-                hit[u] = i < end && (v == v ? v : -INFINITY) == equal;
-            }
-#pragma unroll
-            for (int u = 0; u < 8; ++u) {
-                const unsigned hits = __ballot_sync(0xffffffffu, hit[u]);
-                const int at = found + __popc(hits & ((1u << lane) - 1));
-                if (hit[u] && at < top) t.sel[at] = key_of(equal, i0 + 32 * u + lane);
-                found += __popc(hits);
-            }
+        for (int o = 16; o > 0; o >>= 1) {
+            const uint64_t k2 = __shfl_xor_sync(0xffffffffu, best, o);
+            if (k2 > best) best = k2;
         }
+        if (lane == 0) t.best[warp] = best;
+        sync_consumers();
+        for (int w = 0; w < kWarps; ++w)
+            if (t.best[w] > best) best = t.best[w];
+        sync_consumers();
+        if (key_value(best) <= tau) break;
+        below = best;
+        if (tid == 0) t.key[k] = best;
     }
-    __syncthreads();
+    sync_consumers();
+    return k;
 }
 
-// A CTA has a row, or with SPLIT the CTAs of a cluster have a part of one each and the first joins what they found.
-template <typename T, bool TOP, bool SPLIT>
-__global__ void __launch_bounds__(kThreads, 4) token_logprobs_kernel(const FwdParams p) {
-    constexpr int W = Piece<T>::W;
-    __shared__ Sums part[kWarps];
-    __shared__ __align__(16) Sums mine;
-    __shared__ TopRoom room;
-    const int tid = threadIdx.x, lane = tid & 31;
-    const float c = p.inv_temp * kLog2e;
-    const int R = SPLIT ? p.split : 1, rank = SPLIT ? static_cast<int>(blockIdx.x) % R : 0;
-    const long long r = SPLIT ? blockIdx.x / R : blockIdx.x;
-    const Row<T> row(static_cast<const T*>(p.logits) + r * p.ld, p.V);
-    const int lo = static_cast<int>(static_cast<long long>(row.pieces) * rank / R), hi = static_cast<int>(static_cast<long long>(row.pieces) * (rank + 1) / R);
-    const bool first = rank == 0, last = rank == R - 1;
-    Sums a = no_sums();
-    float2 s2 = splat2(0.0f), s12 = splat2(0.0f);
-    const float2 cc = splat2(c);
-    const float margin = 200.0f / c;
-    auto take = [&](Piece<T>* q) {
-        a.top = fmaxf(a.top, Piece<T>::top(q));
-        if constexpr (sizeof(T) == 2) {
-            if (a.top == -INFINITY) {  // nothing but ruled out tokens (or NaN) yet
-#pragma unroll
-                for (int u = 0; u < kUnroll; ++u)
-#pragma unroll
-                    for (int k = 0; k < W / 2; ++k) {
-                        const float2 v = q[u].pair(k);
-                        if (v.x != v.x || v.y != v.y) s2.x = NAN;
-                    }
-                return;
-            }
-        }
-        const float to = fmaxf(a.rho, a.top * c), d = fmaxf(a.rho - to, kNothing), e = ex2(d);
-        a.rho = to;
-        s12 = mul2(splat2(e), fma2(s2, splat2(d), s12));
-        s2 = mul2(s2, splat2(e));
-        const float2 neg = splat2(-to);
-        // 16-bit logits far below are brought to a finite one whose exponential is still 0, two at a time; f32 ones after the product
-        if constexpr (sizeof(T) == 2) Piece<T>::floor(q, a.top - margin - fabsf(a.top) * 0.015625f);
-#pragma unroll
-        for (int u = 0; u < kUnroll; ++u)
-#pragma unroll
-            for (int k = 0; k < W / 2; ++k) {
-                float2 t = fma2(q[u].pair(k), cc, neg);
-                if constexpr (sizeof(T) == 4) t.x = max_nan(t.x, kNothing), t.y = max_nan(t.y, kNothing);
-                const float2 x = make_float2(ex2(t.x), ex2(t.y));
-                s2 = add2(s2, x);
-                s12 = fma2(x, t, s12);
-            }
-    };
-    const T* base = row.p + row.head;
-    int j0 = lo + tid;
-    Piece<T> q[kUnroll], next[kUnroll];
-    const int whole = j0 < hi ? (hi - j0 + kThreads * kUnroll - 1 - (kUnroll - 1) * kThreads) / (kThreads * kUnroll) : 0;  // full rounds
-    if (whole > 0) {
-#pragma unroll
-        for (int u = 0; u < kUnroll; ++u) next[u].load(base + static_cast<long long>(j0 + u * kThreads) * W);
+// One warp puts the n keys in order into sel[0 .. top) and fills up with the lowest indices of what equals `equals`.
+template <typename T>
+__device__ __forceinline__ void rank_keys(const uint64_t* key, uint64_t* sel, int n, float equals, const Row<T>& row, int begin, int end, int top) {
+    const int lane = threadIdx.x % 32;
+    if (n == kInOrder) return;
+    sel[lane] = 0;
+    __syncwarp();
+    for (int a = lane; a < n; a += 32) {
+        const uint64_t mine = key[a];
+        int rank = 0;
+        for (int b = 0; b < n; ++b) rank += key[b] > mine;
+        if (rank < top) sel[rank] = mine;
     }
-    for (int k = 0; k < whole; ++k) {
+    int found = n;
+    for (int i0 = begin; i0 < end && found < top; i0 += 8 * 32) {
+        bool hit[8];
 #pragma unroll
-        for (int u = 0; u < kUnroll; ++u) q[u] = next[u];
-        j0 += kThreads * kUnroll;
-        if (k + 1 < whole) {
-#pragma unroll
-            for (int u = 0; u < kUnroll; ++u) next[u].load(base + static_cast<long long>(j0 + u * kThreads) * W);
+        for (int u = 0; u < 8; ++u) {
+            const int i = i0 + 32 * u + lane;
+            const float v = i < end ? to_f(row.p[i]) : 0.0f;
+            hit[u] = i < end && (v == v ? v : -INFINITY) == equals;
         }
-        take(q);
-    }
-    // what is left of the thread's pieces, and the ends
-    const bool head = first && tid < row.head, tail = last && row.tail() + tid < p.V;
-    if (j0 < hi || head || tail) {
 #pragma unroll
-        for (int u = 0; u < kUnroll; ++u) {
-            q[u].fill(minus_inf<T>());
-            if (u < kUnroll - 1 && j0 + u * kThreads < hi) q[u].load(base + static_cast<long long>(j0 + u * kThreads) * W);
-        }
-        if (head) q[kUnroll - 1].put(0, row.p[tid]);
-        if (tail) q[kUnroll - 1].put(1, row.p[row.tail() + tid]);
-        take(q);
-    }
-    a.s = s2.x + s2.y, a.s1 = s12.x + s12.y;
-    const float own_top = a.top;
-    if (TOP) {
-        float g = own_top;
-#pragma unroll
-        for (int o = 4; o > 0; o >>= 1) g = fmaxf(g, __shfl_xor_sync(0xffffffffu, g, o));
-        if (lane % 8 == 0) room.group[tid / 8] = g;
-        if (tid == 0) room.n = 0;
-    }
-    join_block(a, part);
-    if (TOP) pick_top<T>(room, row, lo, hi, first, last, p.top, own_top);
-    if (SPLIT) {
-        if (tid == 0) mine = a;
-        cluster_sync();
-        if (rank == 0) {
-            const uint32_t at = smem_u32(&mine);
-            a = no_sums();
-            if (lane < R) {
-                const float4 v = ld_cluster4(cluster_addr(at, lane));
-                a = Sums{v.x, v.y, v.z, v.w};
-            }
-            join_lanes(a, 32);
-            if (TOP) {
-                for (int i = tid; i < R * p.top; i += kThreads) {
-                    const int from = i / p.top, k = i - from * p.top;
-                    uint64_t v;
-                    asm volatile("ld.shared::cluster.u64 %0, [%1];" : "=l"(v) : "r"(cluster_addr(smem_u32(room.sel + k), from)));
-                    room.key[i] = v;
-                }
-                __syncthreads();
-            }
-        }
-        cluster_sync();
-        if (rank != 0) return;
-        if (TOP) {
-            // each part's alternatives are in order: a token's place is the sum of its places in the parts
-            for (int i = tid; i < R * p.top; i += kThreads) {
-                const uint64_t v = room.key[i];
-                int place = 0;
-                for (int f = 0; f < R; ++f) {
-                    const uint64_t* list = room.key + f * p.top;
-                    int at = 0;
-#pragma unroll
-                    for (int step = 32; step > 0; step >>= 1)
-                        if (at + step <= p.top && list[at + step - 1] > v) at += step;
-                    place += at;
-                }
-                if (v != 0 && place < p.top) room.sel[place] = v;
-            }
-            __syncthreads();
+        for (int u = 0; u < 8; ++u) {
+            const unsigned hits = __ballot_sync(0xffffffffu, hit[u]);
+            const int at = found + __popc(hits & ((1u << lane) - 1));
+            if (hit[u] && at < top) sel[at] = key_of(equals, i0 + 32 * u + lane);
+            found += __popc(hits);
         }
     }
-    if (in_doubt(a)) a = sum_again(row, a.top, c, part);  // (alike in all threads)
-    else a.rho = fmaf(a.top, c, -a.rho);                  // top c - rho
+    __syncwarp();
+}
+
+// One warp writes a row's results from its sums (alike in all lanes), the target's logit and the alternatives in order.
+template <typename T>
+__device__ __forceinline__ void write_row(const FwdParams& p, long long r, const Row<T>& row, Sums a, float c, int target, float logit, const uint64_t* sel) {
+    const int lane = threadIdx.x % 32;
+    if (in_doubt(a)) a = sum_again(row, a.top, c);
+    else a.rho = fmaf(a.top, c, -a.rho);  // top c - rho
     const float log_s = (lg2(a.s) - a.rho) * kLn2;
     const bool none = a.s == 0.0f;
-    if (tid == 0) {
+    if (lane == 0) {
         if (p.lse) {
             p.lse[r] = a.s == a.s ? a.top : a.s;
             p.lse[p.rows + r] = none ? 0.0f : log_s;
         }
         if (p.entropy) p.entropy[r] = none ? 0.0f : (lg2(a.s) - a.s1 / a.s) * kLn2;
+        if (p.logprob) {
+            const bool ok = target >= 0 && target < p.V;
+            p.logprob[r] = !ok ? 0.0f : none ? -INFINITY : (logit - a.top) * p.inv_temp - log_s;
+        }
     }
-    if (tid == 32 && p.targets && p.logprob) {
-        const int t = p.targets[r];
-        const bool ok = t >= 0 && t < p.V;
-        p.logprob[r] = !ok ? 0.0f : none ? -INFINITY : (to_f(row.p[t]) - a.top) * p.inv_temp - log_s;
+    if (sel && lane < p.top) {
+        const uint64_t k = sel[lane];
+        p.top_ids[r * p.top + lane] = key_index(k);
+        p.top_logprobs[r * p.top + lane] = none ? -INFINITY : (key_value(k) - a.top) * p.inv_temp - log_s;
     }
-    if (TOP && tid < p.top) {
-        const uint64_t k = room.sel[tid];
-        p.top_ids[r * p.top + tid] = key_index(k);
-        p.top_logprobs[r * p.top + tid] = none ? -INFINITY : (key_value(k) - a.top) * p.inv_temp - log_s;
+}
+__device__ __forceinline__ int target_of(const FwdParams& p, long long r) { return p.targets && p.logprob ? p.targets[r] : -1; }
+
+// Rows one after another, by eight warps that do nothing but read: a ninth brings the rows to shared memory by bulk copies of
+// 16 KB, a tenth makes the results of a row while the next is read, so the memory is never idle.  HBM would be 12 logits a cycle
+// and SM in 16 bits: with 16 exponentials a cycle and some 5 instructions a logit (of 128) the arithmetic is close behind, so the
+// pass has one fma and one exponential a logit, no clamp, and no test but two in 32 logits.
+constexpr int kRound = kThreads * kUnroll, kStages = 3;
+struct RowsRoom {
+    float thread_top[2][kThreads];  // (a row's, while the next row's are found)
+    Sums part[2][kWarps];
+    uint64_t key[kRoom], sel[kMaxTop];
+    uint64_t full[kStages], empty[kStages], row_full[2], row_empty[2];
+    int threads[kThreads], n;
+};
+constexpr int kRowsSmem = kStages * kRound * 16 + static_cast<int>(sizeof(RowsRoom)) + 128;
+static_assert(kCtas * (kRowsSmem + 1024) <= 228 * 1024, "CTAs on an SM");
+
+// The alternatives of a row in order into sel, by one warp.  Eight threads' elements form a group.  tau, the top-th largest of
+// the 32 groups' maxima, is a lower bound of the top-th largest element: only what threads whose own maximum reaches it have seen
+// is read again (from L2), and what reaches it there is ranked by counting.
+template <typename T>
+__device__ __noinline__ void find_top(RowsRoom& t, const float* thread_top, const Row<T>& row, float row_top, int top, uint64_t* release) {
+    constexpr int W = Piece<T>::W, kEach = kThreads / 32, kAtOnce = 4;
+    const int lane = threadIdx.x % 32;
+    float mine[kEach], tau = -INFINITY;
+#pragma unroll
+    for (int i = 0; i < kEach; i += 4) {
+        const float4 v = *reinterpret_cast<const float4*>(thread_top + lane * kEach + i);
+        mine[i] = v.x, mine[i + 1] = v.y, mine[i + 2] = v.z, mine[i + 3] = v.w;
+        tau = fmaxf(tau, fmaxf(fmaxf(v.x, v.y), fmaxf(v.z, v.w)));
     }
+    __syncwarp();
+    if (lane == 0) tc::mbar_arrive(release);
+#pragma unroll
+    for (int size = 2; size <= 32; size <<= 1)
+#pragma unroll
+        for (int o = size >> 1; o > 0; o >>= 1) {
+            const float other = __shfl_xor_sync(0xffffffffu, tau, o);
+            tau = ((lane & o) == 0) == ((lane & size) == 0) ? fmaxf(tau, other) : fminf(tau, other);
+        }
+    tau = __shfl_sync(0xffffffffu, tau, top - 1);
+    int threads = 0;
+#pragma unroll
+    for (int i = 0; i < kEach; ++i) {
+        const bool hit = mine[i] >= tau && mine[i] > -INFINITY;
+        const unsigned hits = __ballot_sync(0xffffffffu, hit);
+        if (hit) t.threads[threads + __popc(hits & ((1u << lane) - 1))] = lane * kEach + i;
+        threads += __popc(hits);
+    }
+    if (lane == 0) t.n = 0;
+    __syncwarp();
+    auto offer = [&](float v, int i) {
+        if (v >= tau && v > -INFINITY) {
+            const int at = atomicAdd(&t.n, 1);
+            if (at < kRoom) t.key[at] = key_of(v, i);
+        }
+    };
+    for (int x = 0; x < threads; x += kAtOnce)
+        for (int j0 = 0; j0 < row.pieces; j0 += 32 * kThreads) {
+            Piece<T> q[kAtOnce];
+            int j[kAtOnce];
+#pragma unroll
+            for (int u = 0; u < kAtOnce; ++u) {
+                j[u] = x + u < threads ? j0 + lane * kThreads + t.threads[x + u] : row.pieces;
+                if (j[u] < row.pieces) q[u].load(row.p + row.head + static_cast<long long>(j[u]) * W);
+            }
+#pragma unroll
+            for (int u = 0; u < kAtOnce; ++u) {
+                if (j[u] >= row.pieces || Piece<T>::template top<1>(q + u) < tau) continue;
+#pragma unroll
+                for (int e = 0; e < W; e += 2) {
+                    const float2 v = q[u].pair(e / 2);
+                    offer(v.x, row.head + j[u] * W + e);
+                    offer(v.y, row.head + j[u] * W + e + 1);
+                }
+            }
+        }
+    if (lane < row.head) offer(to_f(row.p[lane]), lane);
+    if (row.tail() + lane < row.V) offer(to_f(row.p[row.tail() + lane]), row.tail() + lane);
+    __syncwarp();
+    int n = t.n;
+    float equals = -INFINITY;
+    if (n > kRoom) {
+        // More reach tau than there is room for: those above it one after the other, until tau itself is met.
+        equals = tau;
+        n = 0;
+        uint64_t below = ~0ull;
+        if (row_top > tau)
+            for (; n < top; ++n) {
+                uint64_t best = 0;
+                for (int i0 = lane; i0 < row.V; i0 += 8 * 32) {
+                    float v[8];
+#pragma unroll
+                    for (int u = 0; u < 8; ++u) v[u] = i0 + 32 * u < row.V ? to_f(row.p[i0 + 32 * u]) : -INFINITY;
+#pragma unroll
+                    for (int u = 0; u < 8; ++u) {
+                        const uint64_t k = key_of(v[u], i0 + 32 * u);
+                        if (k < below && k > best) best = k;
+                    }
+                }
+#pragma unroll
+                for (int o = 16; o > 0; o >>= 1) {
+                    const uint64_t k = __shfl_xor_sync(0xffffffffu, best, o);
+                    if (k > best) best = k;
+                }
+                if (key_value(best) <= tau) break;
+                below = best;
+                if (lane == 0) t.key[n] = best;
+            }
+        __syncwarp();
+    }
+    rank_keys<T>(t.key, t.sel, n, equals, row, 0, row.V, top);
+}
+
+template <typename T, bool TOP>
+__global__ void __launch_bounds__(kThreads + 64, kCtas) token_logprobs_rows_kernel(const FwdParams p, int* status) {
+    constexpr int W = Piece<T>::W;
+    extern __shared__ unsigned char raw[];
+    unsigned char* sm = raw + (128 - (smem_u32(raw) & 127)) % 128;
+    RowsRoom& room = *reinterpret_cast<RowsRoom*>(sm + kStages * kRound * 16);
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    if (tid == 0) {
+        for (int s = 0; s < kStages; ++s) {
+            mbar_init(&room.full[s], 1);
+            mbar_init(&room.empty[s], kWarps);
+        }
+        for (int b = 0; b < 2; ++b) {
+            mbar_init(&room.row_full[b], kWarps);
+            mbar_init(&room.row_empty[b], 1);
+        }
+        fence_barrier_init();
+    }
+    __syncthreads();
+    const float c = p.inv_temp * kLog2e;
+    bool alive = true;
+    if (warp == kWarps) {  // brings the rows
+        if (lane != 0) return;
+        int s = 0;
+        uint32_t parity = 1;  // (the first round of the ring waits for nobody)
+        for (long long r = blockIdx.x; r < p.rows; r += gridDim.x) {
+            const Row<T> row(static_cast<const T*>(p.logits) + r * p.ld, p.V);
+            for (int j = 0; j < row.pieces; j += kRound) {
+                alive = alive && mbar_wait(&room.empty[s], parity, status);
+                const uint32_t bytes = 16u * min(kRound, row.pieces - j);
+                mbar_expect_tx(&room.full[s], bytes);
+                bulk_load(sm + s * kRound * 16, row.p + row.head + static_cast<long long>(j) * W, bytes, &room.full[s]);
+                if (++s == kStages) s = 0, parity ^= 1;
+            }
+        }
+        return;
+    }
+    int buffer = 0;
+    uint32_t flips = 0;
+    if (warp == kWarps + 1) {  // makes the results
+        for (long long r = blockIdx.x; r < p.rows; r += gridDim.x) {
+            const Row<T> row(static_cast<const T*>(p.logits) + r * p.ld, p.V);
+            const int target = target_of(p, r);
+            const float logit = target >= 0 && target < p.V ? to_f(row.p[target]) : 0.0f;
+            alive = alive && mbar_wait(&room.row_full[buffer], flips, status);
+            Sums a = room.part[buffer][lane % kWarps];
+            join_lanes(a, kWarps);
+            if (TOP) {
+                find_top<T>(room, room.thread_top[buffer], row, a.top, p.top, &room.row_empty[buffer]);
+            } else {
+                __syncwarp();
+                if (lane == 0) tc::mbar_arrive(&room.row_empty[buffer]);
+            }
+            write_row<T>(p, r, row, a, c, target, logit, TOP ? room.sel : nullptr);
+            buffer ^= 1;
+            if (buffer == 0) flips ^= 1;
+        }
+        return;
+    }
+    int s = 0;
+    uint32_t parity = 0;
+    for (long long r = blockIdx.x; r < p.rows; r += gridDim.x) {
+        const Row<T> row(static_cast<const T*>(p.logits) + r * p.ld, p.V);
+        const bool head = tid < row.head, tail = row.tail() + tid < p.V;
+        const T head_v = head ? row.p[tid] : from_f<T>(0.0f), tail_v = tail ? row.p[row.tail() + tid] : from_f<T>(0.0f);
+        Running<T> run;
+        for (int j = 0; j < row.pieces; j += kRound) {
+            alive = alive && mbar_wait(&room.full[s], parity, status);
+            const T* stage = reinterpret_cast<const T*>(sm + s * kRound * 16) + tid * W;
+            if (j + kRound <= row.pieces) {
+                run.template take<kUnroll>(stage, c);
+            } else {
+#pragma unroll 1
+                for (int u = 0; j + u * kThreads + tid < row.pieces; ++u) run.template take<1>(stage + u * kThreads * W, c);
+            }
+            __syncwarp();
+            if (lane == 0) tc::mbar_arrive(&room.empty[s]);
+            if (++s == kStages) s = 0, parity ^= 1;
+        }
+        if (head) run.end(to_f(head_v), c);
+        if (tail) run.end(to_f(tail_v), c);
+        const float own_top = run.top;
+        Sums a = run.sums();
+        join_lanes(a, 32);
+        alive = alive && mbar_wait(&room.row_empty[buffer], flips ^ 1, status);  // (the row before the last is done with)
+        if (TOP) room.thread_top[buffer][tid] = own_top;
+        if (lane == 0) room.part[buffer][warp] = a;
+        __syncwarp();
+        if (lane == 0) tc::mbar_arrive(&room.row_full[buffer]);
+        buffer ^= 1;
+        if (buffer == 0) flips ^= 1;
+    }
+}
+
+// Few rows: the CTAs of a cluster have a part of one each, and the first joins what they found.
+template <typename T, bool TOP>
+__global__ void __launch_bounds__(kThreads, 4) token_logprobs_split_kernel(const FwdParams p) {
+    constexpr int W = Piece<T>::W;
+    __shared__ Sums part[kWarps];
+    __shared__ __align__(16) Sums mine;
+    __shared__ TopRoom room;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const float c = p.inv_temp * kLog2e;
+    const int R = p.split, rank = static_cast<int>(blockIdx.x) % R;
+    const long long r = blockIdx.x / R;
+    const Row<T> row(static_cast<const T*>(p.logits) + r * p.ld, p.V);
+    const int lo = static_cast<int>(static_cast<long long>(row.pieces) * rank / R), hi = static_cast<int>(static_cast<long long>(row.pieces) * (rank + 1) / R);
+    const bool first = rank == 0, last = rank == R - 1;
+    const T* base = row.p + row.head;
+    int target = -1;
+    float logit = 0.0f;
+    if (first && tid == 0) {
+        target = target_of(p, r);
+        if (target >= 0 && target < p.V) logit = to_f(row.p[target]);
+        room.n = 0;
+    }
+    if (!first && tid == 0) room.n = 0;
+    Running<T> run;
+    int j = lo + tid;
+    for (; j + (kUnroll - 1) * kThreads < hi; j += kRound) run.template take<kUnroll>(base + static_cast<long long>(j) * W, c);
+    for (; j < hi; j += kThreads) run.template take<1>(base + static_cast<long long>(j) * W, c);
+    if (first && tid < row.head) run.end(to_f(row.p[tid]), c);
+    if (last && row.tail() + tid < p.V) run.end(to_f(row.p[row.tail() + tid]), c);
+    if (TOP) group_max(room, run.top);
+    Sums a = run.sums();
+    join_lanes(a, 32);
+    if (lane == 0) part[warp] = a;
+    sync_consumers();
+    int n = 0;
+    float equals = 0.0f;
+    if (TOP) n = reach<T>(room, row, lo, hi, first, last, p.top, run.top, &equals);
+    if (warp == 0) {
+        a = part[lane % kWarps];
+        join_lanes(a, kWarps);
+        if (lane == 0) mine = a;
+        if (TOP) rank_keys<T>(room.key, room.sel, n, equals, row, first ? 0 : row.head + lo * W, last ? p.V : row.head + hi * W, p.top);
+    }
+    cluster_sync();
+    if (first) {
+        if (warp == 0) {
+            a = no_sums();
+            if (lane < R) {
+                const float4 v = ld_cluster4(cluster_addr(smem_u32(&mine), lane));
+                a = Sums{v.x, v.y, v.z, v.w};
+            }
+            join_lanes(a, 32);
+        }
+        if (TOP)
+            for (int i = tid; i < R * p.top; i += kThreads) {
+                const int from = i / p.top, k = i - from * p.top;
+                uint64_t v;
+                asm volatile("ld.shared::cluster.u64 %0, [%1];" : "=l"(v) : "r"(cluster_addr(smem_u32(room.sel + k), from)));
+                room.key[i] = v;
+            }
+    }
+    cluster_sync();
+    if (!first) return;
+    if (TOP) {
+        // each part's alternatives are in order: a token's place is the sum of its places in the parts
+        for (int i = tid; i < R * p.top; i += kThreads) {
+            const uint64_t v = room.key[i];
+            int place = 0;
+            for (int f = 0; f < R; ++f) {
+                const uint64_t* list = room.key + f * p.top;
+                int at = 0;
+#pragma unroll
+                for (int step = 32; step > 0; step >>= 1)
+                    if (at + step <= p.top && list[at + step - 1] > v) at += step;
+                place += at;
+            }
+            if (v != 0 && place < p.top) room.sel[place] = v;
+        }
+        sync_consumers();
+    }
+    if (warp == 0) write_row<T>(p, r, row, a, c, target, logit, TOP ? room.sel : nullptr);
 }
 
 struct BwdParams {
@@ -461,8 +680,9 @@ struct BwdParams {
 
 // With t = log2 p: d_logits = -p (k0 + k1 t), plus the target's share.  One read and one write; ALIGNED: rows of both tensors
 // start at the same place of 16 bytes.
+constexpr int kBwdThreads = 256, kBwdUnroll = 4;
 template <typename T, bool ALIGNED>
-__global__ void __launch_bounds__(kThreads, 4) token_logprobs_bwd_kernel(const BwdParams p) {
+__global__ void __launch_bounds__(kBwdThreads, 4) token_logprobs_bwd_kernel(const BwdParams p) {
     constexpr int W = Piece<T>::W;
     const int tid = threadIdx.x;
     const long long r = blockIdx.x;
@@ -480,19 +700,19 @@ __global__ void __launch_bounds__(kThreads, 4) token_logprobs_bwd_kernel(const B
         return i == tgt ? d + g : d;
     };
     if (!ALIGNED) {
-        for (int i = tid; i < p.V; i += kThreads) out[i] = from_f<T>(one(to_f(row.p[i]), i));
+        for (int i = tid; i < p.V; i += kBwdThreads) out[i] = from_f<T>(one(to_f(row.p[i]), i));
         return;
     }
     const float2 neg = splat2(none ? 0.0f : -m), cc = splat2(c), ls = splat2(-log2_s), kk0 = splat2(k0), kk1 = splat2(k1);
-    for (int j0 = tid; j0 < row.pieces; j0 += kThreads * kUnroll) {
-        Piece<T> q[kUnroll];
+    for (int j0 = tid; j0 < row.pieces; j0 += kBwdThreads * kBwdUnroll) {
+        Piece<T> q[kBwdUnroll];
 #pragma unroll
-        for (int u = 0; u < kUnroll; ++u)
-            if (j0 + u * kThreads < row.pieces) q[u].load(row.p + row.head + (j0 + u * kThreads) * W);
+        for (int u = 0; u < kBwdUnroll; ++u)
+            if (j0 + u * kBwdThreads < row.pieces) q[u].load(row.p + row.head + (j0 + u * kBwdThreads) * W);
 #pragma unroll
-        for (int u = 0; u < kUnroll; ++u) {
-            const int i = row.head + (j0 + u * kThreads) * W;
-            if (j0 + u * kThreads >= row.pieces) break;
+        for (int u = 0; u < kBwdUnroll; ++u) {
+            const int i = row.head + (j0 + u * kBwdThreads) * W;
+            if (j0 + u * kBwdThreads >= row.pieces) break;
             float2 d[W / 2];
 #pragma unroll
             for (int k = 0; k < W / 2; ++k) {
@@ -532,14 +752,21 @@ static int pick_split(int sms, long long rows, int V) {
 template <typename T, bool TOP>
 static int launch_fwd(Ctx* c, FwdParams& p, cudaStream_t st) {
     p.split = pick_split(c->sm_count, p.rows, p.V);
-    const dim3 grid(static_cast<unsigned>(p.rows * p.split));
     if (p.split == 1) {
-        token_logprobs_kernel<T, TOP, false><<<grid, kThreads, 0, st>>>(p);
+        const long long most = static_cast<long long>(kCtas) * c->sm_count;
+        token_logprobs_rows_kernel<T, TOP><<<static_cast<unsigned>(p.rows < most ? p.rows : most), kThreads + 64, kRowsSmem, st>>>(p, c->d_status);
     } else {
         void* args[] = {&p};
-        MB200_CUDA_CHECK(c, launch_cluster(reinterpret_cast<const void*>(token_logprobs_kernel<T, TOP, true>), grid, dim3(kThreads), 0, st, p.split, args));
+        MB200_CUDA_CHECK(c, launch_cluster(reinterpret_cast<const void*>(token_logprobs_split_kernel<T, TOP>), dim3(static_cast<unsigned>(p.rows * p.split)),
+                                           dim3(kThreads), 0, st, p.split, args));
     }
     MB200_CUDA_CHECK(c, cudaGetLastError());
+    return MAMBA_B200_OK;
+}
+template <typename T, bool TOP>
+static int configure(Ctx* c) {
+    MB200_CUDA_CHECK(c, cudaFuncSetAttribute(token_logprobs_rows_kernel<T, TOP>, cudaFuncAttributeMaxDynamicSharedMemorySize, kRowsSmem));
+    MB200_CUDA_CHECK(c, cudaFuncSetAttribute(token_logprobs_split_kernel<T, TOP>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
     return MAMBA_B200_OK;
 }
 template <typename T>
@@ -552,8 +779,8 @@ static int launch_bwd(Ctx* c, const BwdParams& p, cudaStream_t st) {
     const uintptr_t x = reinterpret_cast<uintptr_t>(p.logits), y = reinterpret_cast<uintptr_t>(p.dlogits);
     const bool aligned = (x - y) % 16 == 0 && (p.rows == 1 || (p.ld - p.ld_d) * static_cast<long long>(sizeof(T)) % 16 == 0);
     const unsigned grid = static_cast<unsigned>(p.rows);
-    if (aligned) token_logprobs_bwd_kernel<T, true><<<grid, kThreads, 0, st>>>(p);
-    else token_logprobs_bwd_kernel<T, false><<<grid, kThreads, 0, st>>>(p);
+    if (aligned) token_logprobs_bwd_kernel<T, true><<<grid, kBwdThreads, 0, st>>>(p);
+    else token_logprobs_bwd_kernel<T, false><<<grid, kBwdThreads, 0, st>>>(p);
     MB200_CUDA_CHECK(c, cudaGetLastError());
     return MAMBA_B200_OK;
 }
@@ -561,14 +788,13 @@ static int launch_bwd(Ctx* c, const BwdParams& p, cudaStream_t st) {
 }  // namespace lp
 
 int logprobs_configure(Ctx* c) {
-    const void* fns[] = {reinterpret_cast<const void*>(lp::token_logprobs_kernel<float, true, true>),
-                         reinterpret_cast<const void*>(lp::token_logprobs_kernel<float, false, true>),
-                         reinterpret_cast<const void*>(lp::token_logprobs_kernel<__half, true, true>),
-                         reinterpret_cast<const void*>(lp::token_logprobs_kernel<__half, false, true>),
-                         reinterpret_cast<const void*>(lp::token_logprobs_kernel<__nv_bfloat16, true, true>),
-                         reinterpret_cast<const void*>(lp::token_logprobs_kernel<__nv_bfloat16, false, true>)};
-    for (const void* fn : fns) MB200_CUDA_CHECK(c, cudaFuncSetAttribute(fn, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
-    return MAMBA_B200_OK;
+    int rc = lp::configure<float, true>(c);
+    if (!rc) rc = lp::configure<float, false>(c);
+    if (!rc) rc = lp::configure<__half, true>(c);
+    if (!rc) rc = lp::configure<__half, false>(c);
+    if (!rc) rc = lp::configure<__nv_bfloat16, true>(c);
+    if (!rc) rc = lp::configure<__nv_bfloat16, false>(c);
+    return rc;
 }
 
 }  // namespace mb200
