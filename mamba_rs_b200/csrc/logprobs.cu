@@ -16,7 +16,7 @@
 namespace mb200 {
 namespace lp {
 
-constexpr int kThreads = 256, kWarps = kThreads / 32, kMaxTop = 32, kRoom = 512, kUnroll = 4, kCtas = 4;
+constexpr int kThreads = 256, kWarps = kThreads / 32, kMaxTop = 32, kRoom = 512, kUnroll = 4, kCtas = 3;
 constexpr float kNothing = -256.0f;  // 2^-256 is 0 in f32
 
 // max that a NaN passes through.
@@ -214,6 +214,8 @@ __device__ __forceinline__ float key_value(uint64_t k) {
 }
 
 constexpr int kGroup = kThreads / 32;  // threads of a group
+constexpr int kMaxSplit = 16;
+static_assert(kRoom >= kMaxSplit * kMaxTop, "the parts' alternatives are joined in key");
 struct TopRoom {
     float group[32];
     uint64_t key[kRoom], sel[kMaxTop], best[kWarps];
@@ -384,13 +386,19 @@ __device__ __forceinline__ int target_of(const FwdParams& p, long long r) { retu
 // and SM in 16 bits: with 16 exponentials a cycle and some 5 instructions a logit (of 128) the arithmetic is close behind, so the
 // pass has one fma and one exponential a logit, no clamp, and no test but two in 32 logits.
 constexpr int kRound = kThreads * kUnroll, kStages = 3;
-struct RowsRoom {
-    float thread_top[2][kThreads];  // (a row's, while the next row's are found)
-    Sums part[2][kWarps];
-    uint64_t key[kRoom], sel[kMaxTop];
-    uint64_t full[kStages], empty[kStages], row_full[2], row_empty[2];
-    int threads[kThreads], n;
+constexpr int kMakers = 2;  // warps that make results
+struct __align__(16) Maker {  // a row's, while the next rows' are found
+    float thread_top[kThreads];
+    Sums part[kWarps];
+    uint64_t key[kRoom], sel[kMaxTop], full, empty;
+    int n;
+    unsigned char threads[kThreads];
 };
+struct RowsRoom {
+    Maker maker[kMakers];
+    uint64_t full[kStages], empty[kStages];
+};
+static_assert(sizeof(Maker) % 16 == 0 && kThreads <= 256, "float4 reads of thread_top; threads are bytes");
 constexpr int kRowsSmem = kStages * kRound * 16 + static_cast<int>(sizeof(RowsRoom)) + 128;
 static_assert(kCtas * (kRowsSmem + 1024) <= 228 * 1024, "CTAs on an SM");
 
@@ -398,18 +406,18 @@ static_assert(kCtas * (kRowsSmem + 1024) <= 228 * 1024, "CTAs on an SM");
 // the 32 groups' maxima, is a lower bound of the top-th largest element: only what threads whose own maximum reaches it have seen
 // is read again (from L2), and what reaches it there is ranked by counting.
 template <typename T>
-__device__ __noinline__ void find_top(RowsRoom& t, const float* thread_top, const Row<T>& row, float row_top, int top, uint64_t* release) {
+__device__ __noinline__ void find_top(Maker& t, const Row<T>& row, float row_top, int top) {
     constexpr int W = Piece<T>::W, kEach = kThreads / 32, kAtOnce = 4;
     const int lane = threadIdx.x % 32;
     float mine[kEach], tau = -INFINITY;
 #pragma unroll
     for (int i = 0; i < kEach; i += 4) {
-        const float4 v = *reinterpret_cast<const float4*>(thread_top + lane * kEach + i);
+        const float4 v = *reinterpret_cast<const float4*>(t.thread_top + lane * kEach + i);
         mine[i] = v.x, mine[i + 1] = v.y, mine[i + 2] = v.z, mine[i + 3] = v.w;
         tau = fmaxf(tau, fmaxf(fmaxf(v.x, v.y), fmaxf(v.z, v.w)));
     }
     __syncwarp();
-    if (lane == 0) tc::mbar_arrive(release);
+    if (lane == 0) tc::mbar_arrive(&t.empty);
 #pragma unroll
     for (int size = 2; size <= 32; size <<= 1)
 #pragma unroll
@@ -492,7 +500,7 @@ __device__ __noinline__ void find_top(RowsRoom& t, const float* thread_top, cons
 }
 
 template <typename T, bool TOP>
-__global__ void __launch_bounds__(kThreads + 64, kCtas) token_logprobs_rows_kernel(const FwdParams p, int* status) {
+__global__ void __launch_bounds__(kThreads + 32 + 32 * kMakers, kCtas) token_logprobs_rows_kernel(const FwdParams p, int* status) {
     constexpr int W = Piece<T>::W;
     extern __shared__ unsigned char raw[];
     unsigned char* sm = raw + (128 - (smem_u32(raw) & 127)) % 128;
@@ -503,9 +511,9 @@ __global__ void __launch_bounds__(kThreads + 64, kCtas) token_logprobs_rows_kern
             mbar_init(&room.full[s], 1);
             mbar_init(&room.empty[s], kWarps);
         }
-        for (int b = 0; b < 2; ++b) {
-            mbar_init(&room.row_full[b], kWarps);
-            mbar_init(&room.row_empty[b], 1);
+        for (int m = 0; m < kMakers; ++m) {
+            mbar_init(&room.maker[m].full, kWarps);
+            mbar_init(&room.maker[m].empty, 1);
         }
         fence_barrier_init();
     }
@@ -528,28 +536,28 @@ __global__ void __launch_bounds__(kThreads + 64, kCtas) token_logprobs_rows_kern
         }
         return;
     }
-    int buffer = 0;
-    uint32_t flips = 0;
-    if (warp == kWarps + 1) {  // makes the results
-        for (long long r = blockIdx.x; r < p.rows; r += gridDim.x) {
+    if (warp > kWarps) {  // makes the results of every kMakers-th row
+        Maker& t = room.maker[warp - kWarps - 1];
+        uint32_t flips = 0;
+        for (long long r = blockIdx.x + static_cast<long long>(warp - kWarps - 1) * gridDim.x; r < p.rows; r += static_cast<long long>(kMakers) * gridDim.x, flips ^= 1) {
             const Row<T> row(static_cast<const T*>(p.logits) + r * p.ld, p.V);
             const int target = target_of(p, r);
             const float logit = target >= 0 && target < p.V ? to_f(row.p[target]) : 0.0f;
-            alive = alive && mbar_wait(&room.row_full[buffer], flips, status);
-            Sums a = room.part[buffer][lane % kWarps];
+            alive = alive && mbar_wait(&t.full, flips, status);
+            Sums a = t.part[lane % kWarps];
             join_lanes(a, kWarps);
             if (TOP) {
-                find_top<T>(room, room.thread_top[buffer], row, a.top, p.top, &room.row_empty[buffer]);
+                find_top<T>(t, row, a.top, p.top);
             } else {
                 __syncwarp();
-                if (lane == 0) tc::mbar_arrive(&room.row_empty[buffer]);
+                if (lane == 0) tc::mbar_arrive(&t.empty);
             }
-            write_row<T>(p, r, row, a, c, target, logit, TOP ? room.sel : nullptr);
-            buffer ^= 1;
-            if (buffer == 0) flips ^= 1;
+            write_row<T>(p, r, row, a, c, target, logit, TOP ? t.sel : nullptr);
         }
         return;
     }
+    int maker = 0;
+    uint32_t flips = 1;
     int s = 0;
     uint32_t parity = 0;
     for (long long r = blockIdx.x; r < p.rows; r += gridDim.x) {
@@ -575,13 +583,13 @@ __global__ void __launch_bounds__(kThreads + 64, kCtas) token_logprobs_rows_kern
         const float own_top = run.top;
         Sums a = run.sums();
         join_lanes(a, 32);
-        alive = alive && mbar_wait(&room.row_empty[buffer], flips ^ 1, status);  // (the row before the last is done with)
-        if (TOP) room.thread_top[buffer][tid] = own_top;
-        if (lane == 0) room.part[buffer][warp] = a;
+        Maker& t = room.maker[maker];
+        alive = alive && mbar_wait(&t.empty, flips, status);  // (its last row is done with)
+        if (TOP) t.thread_top[tid] = own_top;
+        if (lane == 0) t.part[warp] = a;
         __syncwarp();
-        if (lane == 0) tc::mbar_arrive(&room.row_full[buffer]);
-        buffer ^= 1;
-        if (buffer == 0) flips ^= 1;
+        if (lane == 0) tc::mbar_arrive(&t.full);
+        if (++maker == kMakers) maker = 0, flips ^= 1;
     }
 }
 
@@ -745,7 +753,7 @@ __global__ void __launch_bounds__(kBwdThreads, 4) token_logprobs_bwd_kernel(cons
 // How many CTAs share a row: as many as find room beside one another (four on an SM), each with 2048 logits or more.
 static int pick_split(int sms, long long rows, int V) {
     int s = 1;
-    while (s < 16 && rows * 2 * s <= 4ll * sms && V >= 2 * s * 2048) s *= 2;
+    while (s < kMaxSplit && rows * 2 * s <= 4ll * sms && V >= 2 * s * 2048) s *= 2;
     return s;
 }
 
@@ -754,7 +762,7 @@ static int launch_fwd(Ctx* c, FwdParams& p, cudaStream_t st) {
     p.split = pick_split(c->sm_count, p.rows, p.V);
     if (p.split == 1) {
         const long long most = static_cast<long long>(kCtas) * c->sm_count;
-        token_logprobs_rows_kernel<T, TOP><<<static_cast<unsigned>(p.rows < most ? p.rows : most), kThreads + 64, kRowsSmem, st>>>(p, c->d_status);
+        token_logprobs_rows_kernel<T, TOP><<<static_cast<unsigned>(p.rows < most ? p.rows : most), kThreads + 32 + 32 * kMakers, kRowsSmem, st>>>(p, c->d_status);
     } else {
         void* args[] = {&p};
         MB200_CUDA_CHECK(c, launch_cluster(reinterpret_cast<const void*>(token_logprobs_split_kernel<T, TOP>), dim3(static_cast<unsigned>(p.rows * p.split)),
