@@ -90,6 +90,7 @@ int train_ops_configure(Ctx* c);  // train_ops.cu
 int decode_configure(Ctx* c);     // decode.cu
 int gated_scan_configure(Ctx* c);  // gated_scan.cu
 int logprobs_configure(Ctx* c);    // logprobs.cu
+int embedding_configure(Ctx* c);   // embedding.cu
 
 }  // namespace mb200
 
@@ -136,6 +137,8 @@ extern "C" MAMBA_B200_API int mamba_b200_init(int device, void** handle) {
     rc = gated_scan_configure(c);
     if (rc) return rc;
     rc = logprobs_configure(c);
+    if (rc) return rc;
+    rc = embedding_configure(c);
     if (rc) return rc;
     return MAMBA_B200_OK;
 }
