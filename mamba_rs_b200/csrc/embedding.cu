@@ -44,40 +44,32 @@ struct FwdParams {
     float scale;
 };
 
-// Rows of the output, N elements a thread (16 bytes of the wider type), U pieces in flight: a piece is a row's next kThreads * N
-// columns or the next row's.  HBM-bound: a table row read, an f32 row written.
-constexpr int kThreads = 256;
-template <typename Tin, typename Tout, int N, int U>
-__global__ void __launch_bounds__(kThreads) embedding_fwd_kernel(const FwdParams p) {
-    const Tin* table = static_cast<const Tin*>(p.table);
-    Tout* out = static_cast<Tout*>(p.out);
-    const int per_row = (p.dim + N - 1) / N;
-    const long long total = p.rows * per_row, i0 = blockIdx.x * static_cast<long long>(kThreads * U) + threadIdx.x;
-    Vec<Tin, N> q[U];
-    long long r[U];
-    int c[U];
-    bool ok[U];
+// A warp has up to 8 pieces a lane of one row, N elements each (4: 16 bytes of f32), their loads in flight together.  HBM-bound: a
+// table row is read, an f32 row written.
+constexpr int kThreads = 256, kPieces = 8;
+template <typename Tin, typename Tout, int N>
+__global__ void __launch_bounds__(kThreads) embedding_fwd_kernel(const FwdParams p, int parts) {
+    const int lane = threadIdx.x & 31;
+    const long long task = blockIdx.x * static_cast<long long>(kThreads / 32) + threadIdx.x / 32, r = parts == 1 ? task : task / parts;
+    if (r >= p.rows) return;
+    const int id = p.ids[r], c0 = (static_cast<int>(task - r * parts) * kPieces * 32 + lane) * N;
+    const bool ok = id >= 0 && id < p.vocab;
+    const Tin* from = static_cast<const Tin*>(p.table) + (ok ? id : 0) * p.ld_table + c0;
+    Tout* to = static_cast<Tout*>(p.out) + r * p.ld_out + c0;
+    Vec<Tin, N> q[kPieces];
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-        const long long i = i0 + u * kThreads;
-        r[u] = total <= 0x7fffffff ? static_cast<unsigned>(i) / static_cast<unsigned>(per_row) : i / per_row;
-        c[u] = static_cast<int>(i - r[u] * per_row) * N;
-        ok[u] = false;
-        if (i >= total) continue;
-        const int id = p.ids[r[u]];
-        ok[u] = id >= 0 && id < p.vocab;
-        if (ok[u]) q[u] = *reinterpret_cast<const Vec<Tin, N>*>(table + id * p.ld_table + c[u]);
-    }
+    for (int u = 0; u < kPieces; ++u)
+        if (c0 + u * 32 * N < p.dim) q[u] = *reinterpret_cast<const Vec<Tin, N>*>(from + u * 32 * N);
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-        if (i0 + u * kThreads >= total) break;
+    for (int u = 0; u < kPieces; ++u) {
+        if (c0 + u * 32 * N >= p.dim) break;
         float f[N];
         q[u].widen(f);
 #pragma unroll
-        for (int k = 0; k < N; ++k) f[k] = ok[u] ? f[k] * p.scale : 0.0f;
+        for (int k = 0; k < N; ++k) f[k] = ok ? f[k] * p.scale : 0.0f;
         Vec<Tout, N> o;
         o.narrow(f);
-        *reinterpret_cast<Vec<Tout, N>*>(out + r[u] * p.ld_out + c[u]) = o;
+        *reinterpret_cast<Vec<Tout, N>*>(to + u * 32 * N) = o;
     }
 }
 
@@ -88,10 +80,12 @@ static void launch_fwd(const FwdParams& p, cudaStream_t st) {
         return p.dim % n == 0 && p.ld_table % n == 0 && p.ld_out % n == 0 && reinterpret_cast<uintptr_t>(p.table) % (n * sizeof(Tin)) == 0 &&
                reinterpret_cast<uintptr_t>(p.out) % (n * sizeof(Tout)) == 0;
     };
-    constexpr int U = 4;
-    auto blocks = [&](int n) { return static_cast<unsigned>((p.rows * ((p.dim + n - 1) / n) + kThreads * U - 1) / (kThreads * U)); };
-    if (fits(4)) embedding_fwd_kernel<Tin, Tout, 4, U><<<blocks(4), kThreads, 0, st>>>(p);
-    else embedding_fwd_kernel<Tin, Tout, 1, U><<<blocks(1), kThreads, 0, st>>>(p);
+    auto run = [&](auto kernel, int n) {
+        const int parts = (p.dim + 32 * n * kPieces - 1) / (32 * n * kPieces);
+        kernel<<<static_cast<unsigned>((p.rows * parts + kThreads / 32 - 1) / (kThreads / 32)), kThreads, 0, st>>>(p, parts);
+    };
+    if (fits(4)) run(embedding_fwd_kernel<Tin, Tout, 4>, 4);
+    else run(embedding_fwd_kernel<Tin, Tout, 1>, 1);
 }
 
 // ---------------------------------------------------------------------------------------------------
@@ -100,23 +94,26 @@ static void launch_fwd(const FwdParams& p, cudaStream_t st) {
 // Few rows, one kernel: a CTA whose row is the first of its token finds the others among the ids and adds them; further CTAs clear
 // the rows of tokens that do not occur.
 //
-// More rows are sorted by token first.  A CTA of the sort has a range of tokens and reads ALL ids: it counts those below its range
-// (where its rows begin in the sorted order) and, for each warp's part of the rows, those of each token of the range.  Prefix sums
-// of that table are every row's place, a token's rows in rising order, without exchange between CTAs and without atomics whose
-// order shows.  Then a warp adds a run of kRun sorted rows over 32 N columns.  A token whose rows all lie in the run is written at
-// once; the sum of one that goes on beyond an end of the run (padding, a frequent token) goes to the workspace, and a third kernel
-// adds such a token's sums in the order of the runs.
+// More rows are sorted by token first, by one cluster of 16 CTAs: 8 bits of the token at a time, rows of equal bits in rising
+// order, counts of each warp's contiguous rows in shared memory, the CTAs' counts joined through distributed shared memory.  The
+// other SMs clear rows of the table meanwhile.  (A sort by 148 CTAs with a range of tokens each, without exchange, read all ids
+// 148 times: 23 us for 32768 rows.)  Then a warp adds a run of up to 32 sorted rows over 32 N columns.  A token whose rows all lie
+// in the run is written at once; the sum of one that goes on beyond an end of the run (padding, a frequent token) goes to the
+// workspace, and a third kernel adds such a token's sums in the order of the runs.
 // ---------------------------------------------------------------------------------------------------
-constexpr int kFewRows = 512, kRun = 32, kSortThreads = 1024, kSortWarps = kSortThreads / 32, kMaxRange = 1024, kJoinRuns = 8;
+constexpr int kFewRows = 512, kMaxRun = 32, kSortThreads = 1024, kSortWarps = kSortThreads / 32, kSorters = 16, kDigits = 256;
 
 struct BwdParams {
     const void* d_out;
     const int* ids;
     float* d_table;
     long long ld_dout;
-    int rows, dim, vocab, accumulate, range, slices, runs;
+    int rows, dim, vocab, accumulate, slices, run, runs;
+    int cleared;             // rows from here on are cleared beside the sort, whether their token occurs or not
+    int passes;              // of the sort
     float scale;
     int2* sorted;            // row, token
+    int2* other;             // of the sort's passes before the last
     int* counted;            // rows whose token lies in the table
     unsigned char* present;  // [vocab]
     float* part;             // [runs, 2, dim]: a run's sum of the token that came from before, and of the one that goes on
@@ -144,17 +141,13 @@ template <int N, int WARPS> __device__ __forceinline__ void add_warps(float* acc
         for (int w = 0; w < WARPS; ++w) acc[k] += room[w][k * 32 + lane];
     }
 }
-// A warp clears rows lo .. hi of the table (where `absent` says so).
-template <int N, typename F> __device__ __forceinline__ void clear_rows(float* table, int lo, int hi, int dim, F absent) {
-    const int lane = threadIdx.x & 31;
+// A warp clears a row of the table.
+template <int N> __device__ __forceinline__ void clear_row(float* row, int dim) {
     Vec<float, N> zero;
 #pragma unroll
     for (int k = 0; k < N; ++k) zero.v[k] = 0.0f;
-    for (int v = lo; v < hi; ++v) {
-        if (!absent(v)) continue;
-        float* row = table + static_cast<long long>(v) * dim;
-        for (int c = lane * N; c < dim; c += 32 * N) *reinterpret_cast<Vec<float, N>*>(row + c) = zero;
-    }
+#pragma unroll 4
+    for (int c = (threadIdx.x & 31) * N; c < dim; c += 32 * N) *reinterpret_cast<Vec<float, N>*>(row + c) = zero;
 }
 
 template <typename T, int N>
@@ -172,7 +165,7 @@ __global__ void __launch_bounds__(kThreads) embedding_bwd_few_kernel(const BwdPa
         bool any = false;
         for (int i = lane; i < R; i += 32) any |= ids[i] == v;
         any = __any_sync(0xffffffffu, any);
-        clear_rows<NF>(p.d_table, v, v + 1, p.dim, [any](int) { return !any; });
+        if (!any) clear_row<NF>(p.d_table + static_cast<long long>(v) * p.dim, p.dim);
         return;
     }
     const int r = static_cast<int>(blockIdx.x) / p.slices, c = (static_cast<int>(blockIdx.x) - r * p.slices) * 32 * N + lane * N, id = ids[r];
@@ -225,78 +218,111 @@ __global__ void __launch_bounds__(kThreads) embedding_bwd_few_kernel(const BwdPa
     }
 }
 
+template <int N>
 __global__ void __launch_bounds__(kSortThreads) embedding_sort_kernel(const BwdParams p) {
-    extern __shared__ int table[];  // [kSortWarps][range]: how many, then the next place
-    __shared__ int sums[kSortWarps], base;
-    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, W = p.range, lo = static_cast<int>(blockIdx.x) * W, hi = min(p.vocab, lo + W);
-    for (int i = tid; i < kSortWarps * W; i += kSortThreads) table[i] = 0;
-    if (tid == 0) base = 0;
-    __syncthreads();
-    int* mine = table + warp * W;
-    const int per = (((p.rows + kSortWarps - 1) / kSortWarps) + 31) / 32 * 32;
-    const long long first = static_cast<long long>(warp) * per;
-    const int begin = static_cast<int>(first < p.rows ? first : p.rows), end = min(p.rows - begin, per) + begin;
-    constexpr int U = 8;
-    int below = 0;
-    for (int i = begin + lane; i < end; i += 32 * U) {
-        int id[U];
-#pragma unroll
-        for (int u = 0; u < U; ++u) id[u] = i + 32 * u < end ? p.ids[i + 32 * u] : -1;
-#pragma unroll
-        for (int u = 0; u < U; ++u) {
-            below += id[u] >= 0 && id[u] < lo;
-            if (id[u] >= lo && id[u] < hi) atomicAdd(&mine[id[u] - lo], 1);
-        }
+    __shared__ int table[kSortWarps][kDigits], digit[kDigits], sums[kSortWarps];
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, rank = blockIdx.x;
+    if (rank >= kSorters) {  // the sort waits for its loads and counters: HBM is free to clear rows meanwhile
+        for (int v = p.cleared + (rank - kSorters) * kSortWarps + warp; v < p.vocab; v += (gridDim.x - kSorters) * kSortWarps)
+            clear_row<N>(p.d_table + static_cast<long long>(v) * p.dim, p.dim);
+        return;
     }
-    below = __reduce_add_sync(0xffffffffu, below);
-    if (lane == 0 && below) atomicAdd(&base, below);
-    __syncthreads();
-    // places: tokens in order, within a token the warps in order
-    int total = 0;
-    if (tid < W)
-        for (int w = 0; w < kSortWarps; ++w) total += table[w * W + tid];
-    int sum = total;
+    for (int v = rank * kSortThreads + tid; v < p.vocab; v += kSorters * kSortThreads) p.present[v] = 0;
+    int n = p.rows;
+    constexpr int U = 4;
+    for (int pass = 0; pass < p.passes; ++pass) {
+        const bool first = pass == 0, last = pass + 1 == p.passes;
+        const int2* from = (p.passes - pass) % 2 ? p.other : p.sorted;
+        int2* to = (p.passes - pass) % 2 ? p.sorted : p.other;
+        // this warp's elements
+        const int per = ((n + kSorters * kSortWarps - 1) / (kSorters * kSortWarps) + 31) / 32 * 32;
+        const long long lo = static_cast<long long>(rank * kSortWarps + warp) * per;
+        const int begin = static_cast<int>(lo < n ? lo : n), end = min(n - begin, per) + begin, shift = 8 * pass;
+        auto element = [&](int i) -> int2 {
+            if (i >= end) return make_int2(0, -1);
+            if (!first) return from[i];
+            const int id = p.ids[i];
+            return make_int2(i, id < p.vocab ? id : -1);
+        };
+        for (int i = tid; i < kSortWarps * kDigits; i += kSortThreads) (&table[0][0])[i] = 0;
+        __syncthreads();
+        for (int i0 = begin; i0 < end; i0 += 32 * U) {
+            int2 e[U];
 #pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-        const int up = __shfl_up_sync(0xffffffffu, sum, o);
-        if (lane >= o) sum += up;
-    }
-    if (lane == 31) sums[warp] = sum;
-    __syncthreads();
-    int before = base;
-    for (int w = 0; w < warp; ++w) before += sums[w];
-    int at = before + sum - total;
-    if (tid < W) {
-        for (int w = 0; w < kSortWarps; ++w) {
-            const int n = table[w * W + tid];
-            table[w * W + tid] = at;
-            at += n;
-        }
-        if (lo + tid < hi) {
-            p.present[lo + tid] = total != 0;
-            if (lo + tid == p.vocab - 1) *p.counted = at;
-        }
-    }
-    __syncthreads();
-    for (int i0 = begin; i0 < end; i0 += 32 * U) {
-        int id[U];
+            for (int u = 0; u < U; ++u) e[u] = element(i0 + 32 * u + lane);
 #pragma unroll
-        for (int u = 0; u < U; ++u) id[u] = i0 + lane + 32 * u < end ? p.ids[i0 + lane + 32 * u] : -1;
-#pragma unroll
-        for (int u = 0; u < U; ++u) {
-            const bool in = id[u] >= lo && id[u] < hi;
-            const unsigned any = __ballot_sync(0xffffffffu, in);
-            if (any == 0) continue;
-            if (in) {
-                const unsigned same = __match_any_sync(any, id[u]);
-                const int place = mine[id[u] - lo] + __popc(same & ((1u << lane) - 1));
-                p.sorted[place] = make_int2(i0 + lane + 32 * u, id[u]);
-                __syncwarp(any);
-                if ((same >> lane) == 1) mine[id[u] - lo] = place + 1;  // (the last of them)
-                __syncwarp(any);
+            for (int u = 0; u < U; ++u) {
+                const int d = e[u].y < 0 ? kDigits : (e[u].y >> shift) & (kDigits - 1);
+                const unsigned same = __match_any_sync(0xffffffffu, d);
+                if (d < kDigits && (same & ((1u << lane) - 1)) == 0) atomicAdd(&table[warp][d], __popc(same));
             }
         }
+        __syncthreads();
+        int mine = 0;
+        if (tid < kDigits) {
+#pragma unroll
+            for (int w = 0; w < kSortWarps; ++w) mine += table[w][tid];
+            digit[tid] = mine;
+        }
+        cluster_sync();
+        int before = 0, all = 0;
+        if (tid < kDigits) {
+            int of[kSorters];
+#pragma unroll
+            for (int k = 0; k < kSorters; ++k) of[k] = __float_as_int(ld_cluster1(cluster_addr(smem_u32(digit + tid), k)));
+#pragma unroll
+            for (int k = 0; k < kSorters; ++k) {
+                if (k < rank) before += of[k];
+                all += of[k];
+            }
+            int sum = all;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const int up = __shfl_up_sync(0xffffffffu, sum, o);
+                if (lane >= o) sum += up;
+            }
+            if (lane == 31) sums[warp] = sum;
+            before += sum - all;
+        }
+        __syncthreads();
+        if (tid < kDigits) {
+            for (int w = 0; w < warp; ++w) before += sums[w];
+#pragma unroll
+            for (int w0 = 0; w0 < kSortWarps; w0 += 8) {
+                int c[8];
+#pragma unroll
+                for (int w = 0; w < 8; ++w) c[w] = table[w0 + w][tid];
+#pragma unroll
+                for (int w = 0; w < 8; ++w) {
+                    table[w0 + w][tid] = before;
+                    before += c[w];
+                }
+            }
+        }
+        __syncthreads();
+        n = 0;
+        for (int w = 0; w < kDigits / 32; ++w) n += sums[w];
+        for (int i0 = begin; i0 < end; i0 += 32 * U) {
+            int2 e[U];
+#pragma unroll
+            for (int u = 0; u < U; ++u) e[u] = element(i0 + 32 * u + lane);
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                const int d = e[u].y < 0 ? kDigits : (e[u].y >> shift) & (kDigits - 1);
+                const unsigned same = __match_any_sync(0xffffffffu, d);
+                const int place = d < kDigits ? table[warp][d] + __popc(same & ((1u << lane) - 1)) : 0;
+                __syncwarp();
+                if (d < kDigits) {
+                    to[place] = e[u];
+                    if (last) p.present[e[u].y] = 1;
+                    if ((same >> lane) == 1) table[warp][d] = place + 1;  // (the last of them)
+                }
+                __syncwarp();
+            }
+        }
+        cluster_sync();  // the elements are there, and nobody reads this CTA's counts any more
     }
+    if (rank == 0 && tid == 0) *p.counted = n;
 }
 
 template <typename T, int N>
@@ -304,17 +330,20 @@ __global__ void __launch_bounds__(kThreads) embedding_sums_kernel(const BwdParam
     constexpr int NF = N == 8 ? 4 : N;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     asm volatile("griddepcontrol.wait;" ::: "memory");
-    if (static_cast<int>(blockIdx.x) >= sum_blocks) {  // 64 rows of the table
-        const int lo = ((static_cast<int>(blockIdx.x) - sum_blocks) * (kThreads / 32) + warp) * 8;
-        clear_rows<NF>(p.d_table, lo, min(p.vocab, lo + 8), p.dim, [&p](int v) { return !p.present[v]; });
+    // blocks that clear lie evenly between those that add: the ones write, the others read
+    const int clears = gridDim.x - sum_blocks, cleared = static_cast<int>(static_cast<long long>(blockIdx.x) * clears / gridDim.x);
+    if (static_cast<int>((blockIdx.x + 1ll) * clears / gridDim.x) != cleared) {  // 64 rows of the table
+        const int v0 = (cleared * (kThreads / 32) + warp) * 8;
+        const unsigned absent = __ballot_sync(0xffffffffu, lane < 8 && v0 + lane < p.cleared && !p.present[v0 + lane]);
+        for (unsigned m = absent; m; m &= m - 1) clear_row<NF>(p.d_table + static_cast<long long>(v0 + __ffs(m) - 1) * p.dim, p.dim);
         return;
     }
-    const long long task = blockIdx.x * static_cast<long long>(kThreads / 32) + warp;
+    const long long task = (static_cast<int>(blockIdx.x) - cleared) * static_cast<long long>(kThreads / 32) + warp;
     const int run = static_cast<int>(task / p.slices), c = (static_cast<int>(task - static_cast<long long>(run) * p.slices) * 32 + lane) * N;
-    const int first = run * kRun, total = *p.counted, n = min(kRun, total - first);
+    const int first = run * p.run, total = *p.counted, n = min(p.run, total - first);
     if (n <= 0) return;
     const int2 own = lane < n ? p.sorted[first + lane] : make_int2(0, -1);
-    const int before = first > 0 ? p.sorted[first - 1].y : -1, behind = first + kRun < total ? p.sorted[first + kRun].y : -1;
+    const int before = first > 0 ? p.sorted[first - 1].y : -1, behind = first + p.run < total ? p.sorted[first + p.run].y : -1;
     float acc[N];
 #pragma unroll
     for (int k = 0; k < N; ++k) acc[k] = 0.0f;
@@ -356,60 +385,84 @@ __global__ void __launch_bounds__(kThreads) embedding_sums_kernel(const BwdParam
     }
 }
 
-// Tokens that go on beyond a run, by the CTA of the run that they begin in.
+// Tokens that go on beyond a run.  A warp looks after the one that begins in its run and adds its runs' sums, if they are few; the
+// CTA does so for one that reaches far.
 template <int N>
 __global__ void __launch_bounds__(kThreads) embedding_join_kernel(const BwdParams p) {
     constexpr int WARPS = kThreads / 32;
     __shared__ float room[WARPS][32 * N];
+    __shared__ int far[WARPS];
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, c = (blockIdx.y * 32 + lane) * N;
     asm volatile("griddepcontrol.wait;" ::: "memory");
-    const int total = *p.counted, runs = (total + kRun - 1) / kRun;
-    for (int run = blockIdx.x * kJoinRuns; run < min(runs - 1, (static_cast<int>(blockIdx.x) + 1) * kJoinRuns); ++run) {
-        const int token = p.sorted[run * kRun + kRun - 1].y;
-        if (p.sorted[(run + 1) * kRun].y != token) continue;                      // it ends here
-        if (run > 0 && p.sorted[run * kRun - 1].y == token) continue;             // it began before
+    const int total = *p.counted, runs = (total + p.run - 1) / p.run;
+    if (static_cast<int>(blockIdx.x) * WARPS >= runs - 1) return;
+    auto add = [&](float* acc, int run, int begin, int end) {  // sums begin .. end of the token that begins in the run
+        if (c >= p.dim) return;
+        for (int i0 = begin; i0 < end; i0 += 8) {
+            Vec<float, N> q[8];
+#pragma unroll
+            for (int u = 0; u < 8; ++u)
+                if (i0 + u < end) q[u] = *reinterpret_cast<const Vec<float, N>*>(p.part + (2ll * (run + i0 + u) + (i0 + u == 0 ? 1 : 0)) * p.dim + c);
+#pragma unroll
+            for (int u = 0; u < 8; ++u)
+                if (i0 + u < end)
+#pragma unroll
+                    for (int k = 0; k < N; ++k) acc[k] += q[u].v[k];
+        }
+    };
+    float acc[N];
+#pragma unroll
+    for (int k = 0; k < N; ++k) acc[k] = 0.0f;
+    const int run = blockIdx.x * WARPS + warp;
+    // lane l: the token at the start of run run + 1 + l; and those before this run and at its end
+    const int ahead = run + 1 + lane < runs ? p.sorted[(run + 1 + lane) * p.run].y : -1;
+    const int before = run > 0 && run < runs ? p.sorted[run * p.run - 1].y : -1, token = run + 1 < runs ? p.sorted[run * p.run + p.run - 1].y : -2;
+    const unsigned same = __ballot_sync(0xffffffffu, ahead == token);
+    const bool begins = (same & 1) && before != token;
+    if (lane == 0) far[warp] = begins && same == 0xffffffffu;
+    if (begins && same != 0xffffffffu) {
+        add(acc, run, 0, __ffs(~same));
+        if (c < p.dim) write_sum<N>(p.d_table + static_cast<long long>(token) * p.dim + c, acc, p.scale, p.accumulate);
+    }
+    __syncthreads();
+    for (int w = 0; w < WARPS; ++w) {
+        if (!far[w]) continue;
+        const int from = blockIdx.x * WARPS + w, its = p.sorted[from * p.run + p.run - 1].y;
         int n = 0;  // runs behind this one that it reaches
-        for (int i0 = run + 1;; i0 += kThreads) {
-            const int here = __syncthreads_count(i0 + tid < runs && p.sorted[(i0 + tid) * kRun].y == token);
+        for (int i0 = from + 1;; i0 += kThreads) {
+            const int here = __syncthreads_count(i0 + tid < runs && p.sorted[(i0 + tid) * p.run].y == its);
             n += here;
             if (here < kThreads) break;
         }
-        float acc[N];
 #pragma unroll
         for (int k = 0; k < N; ++k) acc[k] = 0.0f;
-        const int each = (n + 1 + WARPS - 1) / WARPS, end = min(n + 1, (warp + 1) * each);
-        if (c < p.dim)
-            for (int i0 = warp * each; i0 < end; i0 += 8) {
-                Vec<float, N> q[8];
-#pragma unroll
-                for (int u = 0; u < 8; ++u)
-                    if (i0 + u < end) q[u] = *reinterpret_cast<const Vec<float, N>*>(p.part + (2ll * (run + i0 + u) + (i0 + u == 0 ? 1 : 0)) * p.dim + c);
-#pragma unroll
-                for (int u = 0; u < 8; ++u)
-                    if (i0 + u < end)
-#pragma unroll
-                        for (int k = 0; k < N; ++k) acc[k] += q[u].v[k];
-            }
+        const int each = (n + 1 + WARPS - 1) / WARPS;
+        add(acc, from, warp * each, min(n + 1, (warp + 1) * each));
         add_warps<N, WARPS>(acc, room);
-        if (warp == 0 && c < p.dim) write_sum<N>(p.d_table + static_cast<long long>(token) * p.dim + c, acc, p.scale, p.accumulate);
+        if (warp == 0 && c < p.dim) write_sum<N>(p.d_table + static_cast<long long>(its) * p.dim + c, acc, p.scale, p.accumulate);
     }
 }
 
-static int range_of(int vocab) {
-    const int w = (vocab + 147) / 148;
-    return w < 8 ? 8 : w > kMaxRange ? kMaxRange : w;
+constexpr long long kClearBeside = 48 << 20;
+// Rows of a run: fewer where that gives more warps something to do.
+static int run_of(long long rows, int dim) {
+    int run = kMaxRun;
+    while (run > 8 && rows / run * ((dim + 127) / 128) < 148 * 32) run /= 2;
+    return run;
 }
 struct Room {
-    long long sorted, counted, present, part, bytes;
+    long long sorted, other, counted, present, part, bytes;
 };
 static Room room_of(long long rows, int dim, int vocab) {
     auto up = [](long long n) { return (n + 255) / 256 * 256; };
     Room r{};
     if (rows <= kFewRows) return r;
-    r.counted = up(rows * 8);
+    r.other = up(rows * 8);
+    r.counted = 2 * r.other;
     r.present = r.counted + 256;
     r.part = r.present + up(vocab);
-    r.bytes = r.part + (rows + kRun - 1) / kRun * 2 * dim * 4;
+    const int run = run_of(rows, dim);
+    r.bytes = r.part + (rows + run - 1) / run * 2 * dim * 4;
     return r;
 }
 
@@ -438,15 +491,22 @@ static int launch_bwd(Ctx* c, BwdParams& p, cudaStream_t st) {
         MB200_CUDA_CHECK(c, cudaGetLastError());
         return MAMBA_B200_OK;
     }
-    p.range = range_of(p.vocab);
-    p.runs = (p.rows + kRun - 1) / kRun;
-    const long long sums = (static_cast<long long>(p.runs) * p.slices + kThreads / 32 - 1) / (kThreads / 32), clears = p.accumulate ? 0 : (p.vocab + 63) / 64;
+    p.run = run_of(p.rows, p.dim);
+    p.runs = (p.rows + p.run - 1) / p.run;
+    for (p.passes = 1; p.passes < 4 && (p.vocab - 1) >> (8 * p.passes); ++p.passes) {}
+    // what HBM can clear while the sort runs (some 8 us), of the last tokens: the rare ones where tokens are in order of frequency
+    const long long beside = p.accumulate ? 0 : kClearBeside / (4ll * p.dim);
+    p.cleared = p.vocab - static_cast<int>(beside < p.vocab ? beside : p.vocab);
+    const int clearers = p.cleared == p.vocab ? 0 : (c->sm_count - kSorters) / kSorters * kSorters;
+    const long long sums = (static_cast<long long>(p.runs) * p.slices + kThreads / 32 - 1) / (kThreads / 32), clears = p.accumulate ? 0 : (p.cleared + 63) / 64;
     if (sums + clears > 2147483647ll) return fail(c, MAMBA_B200_ERR_SHAPE, "embedding_bwd: too many rows");
-    embedding_sort_kernel<<<(p.vocab + p.range - 1) / p.range, kSortThreads, kSortWarps * p.range * sizeof(int), st>>>(p);
-    MB200_CUDA_CHECK(c, cudaGetLastError());
-    MB200_CUDA_CHECK(c, launch_early(embedding_sums_kernel<T, N>, dim3(static_cast<unsigned>(sums + clears)), kThreads, st, p, static_cast<int>(sums)));
     constexpr int NJ = N == 8 ? 4 : N;
-    MB200_CUDA_CHECK(c, launch_early(embedding_join_kernel<NJ>, dim3((p.runs + kJoinRuns - 1) / kJoinRuns, (p.dim + 32 * NJ - 1) / (32 * NJ)), kThreads, st, p));
+    void* args[] = {&p};
+    MB200_CUDA_CHECK(c, launch_cluster(reinterpret_cast<const void*>(embedding_sort_kernel<NJ>), dim3(kSorters + clearers), dim3(kSortThreads), 0, st,
+                                       kSorters, args));
+    MB200_CUDA_CHECK(c, launch_early(embedding_sums_kernel<T, N>, dim3(static_cast<unsigned>(sums + clears)), kThreads, st, p, static_cast<int>(sums)));
+    MB200_CUDA_CHECK(c, launch_early(embedding_join_kernel<NJ>, dim3((p.runs + kThreads / 32 - 1) / (kThreads / 32), (p.dim + 32 * NJ - 1) / (32 * NJ)),
+                                     kThreads, st, p));
     return MAMBA_B200_OK;
 }
 template <typename T>
@@ -464,8 +524,8 @@ static int launch_bwd(Ctx* c, BwdParams& p, cudaStream_t st) {
 }  // namespace emb
 
 int embedding_configure(Ctx* c) {
-    MB200_CUDA_CHECK(c, cudaFuncSetAttribute(emb::embedding_sort_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                             emb::kSortWarps * emb::kMaxRange * static_cast<int>(sizeof(int))));
+    MB200_CUDA_CHECK(c, cudaFuncSetAttribute(emb::embedding_sort_kernel<1>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
+    MB200_CUDA_CHECK(c, cudaFuncSetAttribute(emb::embedding_sort_kernel<4>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
     return MAMBA_B200_OK;
 }
 
@@ -483,7 +543,7 @@ extern "C" MAMBA_B200_API int mamba_b200_embedding_fwd(void* handle, void* strea
         return fail(c, MAMBA_B200_ERR_ARG, "embedding_fwd: rows come out as f32 or in the table's dtype, not %d", out_dtype);
     if (rows < 0 || dim <= 0 || vocab <= 0 || ld_table < dim || ld_out < dim) return fail(c, MAMBA_B200_ERR_ARG, "embedding_fwd: bad dims");
     if (rows == 0) return MAMBA_B200_OK;
-    if (rows * ((dim + 3) / 4) > 2147483647ll * 256) return fail(c, MAMBA_B200_ERR_SHAPE, "embedding_fwd: too many rows");
+    if (rows > 2147483647ll * 8 / ((dim + 255) / 256)) return fail(c, MAMBA_B200_ERR_SHAPE, "embedding_fwd: too many rows");
     if (!table || !ids || !out) return fail(c, MAMBA_B200_ERR_ARG, "embedding_fwd: null pointer");
     const emb::FwdParams p{table, ids, out, ld_table, ld_out, rows, dim, vocab, scale};
     cudaStream_t st = static_cast<cudaStream_t>(stream);
@@ -514,9 +574,11 @@ extern "C" MAMBA_B200_API int mamba_b200_embedding_bwd(void* handle, void* strea
     const emb::Room r = emb::room_of(rows, dim, vocab);
     if (workspace_bytes < r.bytes || (r.bytes && (!workspace || reinterpret_cast<uintptr_t>(workspace) % 256)))
         return fail(c, MAMBA_B200_ERR_ARG, "embedding_bwd: the workspace is %lld bytes, 256-byte aligned", r.bytes);
-    emb::BwdParams p{d_out, ids, d_table, ld_dout, static_cast<int>(rows), dim, vocab, accumulate, 0, 0, 0, scale};
+    emb::BwdParams p{d_out, ids, d_table, ld_dout, static_cast<int>(rows), dim, vocab, accumulate};
+    p.scale = scale;
     unsigned char* ws = static_cast<unsigned char*>(workspace);
     p.sorted = reinterpret_cast<int2*>(ws + r.sorted);
+    p.other = reinterpret_cast<int2*>(ws + r.other);
     p.counted = reinterpret_cast<int*>(ws + r.counted);
     p.present = ws + r.present;
     p.part = reinterpret_cast<float*>(ws + r.part);
