@@ -112,9 +112,8 @@ struct BwdParams {
     int cleared;             // rows from here on are cleared beside the sort, whether their token occurs or not
     int passes;              // of the sort
     float scale;
-    int2* sorted;            // row, token
+    int2* sorted;            // [(runs + 1) * run] row, token; behind the last one token -1
     int2* other;             // of the sort's passes before the last
-    int* counted;            // rows whose token lies in the table
     unsigned char* present;  // [vocab]
     float* part;             // [runs, 2, dim]: a run's sum of the token that came from before, and of the one that goes on
 };
@@ -218,15 +217,17 @@ __global__ void __launch_bounds__(kThreads) embedding_bwd_few_kernel(const BwdPa
     }
 }
 
+// Clears the rows from p.cleared on.  The sort starts while this runs, and ends after it.
 template <int N>
+__global__ void __launch_bounds__(kThreads) embedding_clear_kernel(const BwdParams p) {
+    asm volatile("griddepcontrol.launch_dependents;");
+    for (int v = p.cleared + static_cast<int>(blockIdx.x) * (kThreads / 32) + static_cast<int>(threadIdx.x) / 32; v < p.vocab; v += gridDim.x * (kThreads / 32))
+        clear_row<N>(p.d_table + static_cast<long long>(v) * p.dim, p.dim);
+}
+
 __global__ void __launch_bounds__(kSortThreads) embedding_sort_kernel(const BwdParams p) {
     __shared__ int table[kSortWarps][kDigits], digit[kDigits], sums[kSortWarps];
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, rank = blockIdx.x;
-    if (rank >= kSorters) {  // the sort waits for its loads and counters: HBM is free to clear rows meanwhile
-        for (int v = p.cleared + (rank - kSorters) * kSortWarps + warp; v < p.vocab; v += (gridDim.x - kSorters) * kSortWarps)
-            clear_row<N>(p.d_table + static_cast<long long>(v) * p.dim, p.dim);
-        return;
-    }
     for (int v = rank * kSortThreads + tid; v < p.vocab; v += kSorters * kSortThreads) p.present[v] = 0;
     int n = p.rows;
     constexpr int U = 4;
@@ -244,12 +245,16 @@ __global__ void __launch_bounds__(kSortThreads) embedding_sort_kernel(const BwdP
             const int id = p.ids[i];
             return make_int2(i, id < p.vocab ? id : -1);
         };
+        int2 e[U];  // (all that a warp has, most often: it is fetched once)
+#pragma unroll
+        for (int u = 0; u < U; ++u) e[u] = element(begin + 32 * u + lane);
         for (int i = tid; i < kSortWarps * kDigits; i += kSortThreads) (&table[0][0])[i] = 0;
         __syncthreads();
         for (int i0 = begin; i0 < end; i0 += 32 * U) {
-            int2 e[U];
+            if (i0 > begin) {
 #pragma unroll
-            for (int u = 0; u < U; ++u) e[u] = element(i0 + 32 * u + lane);
+                for (int u = 0; u < U; ++u) e[u] = element(i0 + 32 * u + lane);
+            }
 #pragma unroll
             for (int u = 0; u < U; ++u) {
                 const int d = e[u].y < 0 ? kDigits : (e[u].y >> shift) & (kDigits - 1);
@@ -303,9 +308,10 @@ __global__ void __launch_bounds__(kSortThreads) embedding_sort_kernel(const BwdP
         n = 0;
         for (int w = 0; w < kDigits / 32; ++w) n += sums[w];
         for (int i0 = begin; i0 < end; i0 += 32 * U) {
-            int2 e[U];
+            if (end - begin > 32 * U) {
 #pragma unroll
-            for (int u = 0; u < U; ++u) e[u] = element(i0 + 32 * u + lane);
+                for (int u = 0; u < U; ++u) e[u] = element(i0 + 32 * u + lane);
+            }
 #pragma unroll
             for (int u = 0; u < U; ++u) {
                 const int d = e[u].y < 0 ? kDigits : (e[u].y >> shift) & (kDigits - 1);
@@ -322,12 +328,15 @@ __global__ void __launch_bounds__(kSortThreads) embedding_sort_kernel(const BwdP
         }
         cluster_sync();  // the elements are there, and nobody reads this CTA's counts any more
     }
-    if (rank == 0 && tid == 0) *p.counted = n;
+    for (int i = n + rank * kSortThreads + tid; i < (p.runs + 1) * p.run; i += kSorters * kSortThreads) p.sorted[i] = make_int2(0, -1);
+    asm volatile("griddepcontrol.wait;" ::: "memory");  // (what comes next relies on the cleared rows too)
 }
 
-template <typename T, int N>
-__global__ void __launch_bounds__(kThreads) embedding_sums_kernel(const BwdParams p, int sum_blocks) {
-    constexpr int NF = N == 8 ? 4 : N;
+// A warp has M vectors of N columns a lane, 32 N apart: what a row costs beside its loads and additions is shared by more columns
+// (one vector: 56 instructions a row and vector, the kernel was bound by them).
+template <typename T, int N, int M>
+__global__ void __launch_bounds__(kThreads, 3) embedding_sums_kernel(const BwdParams p, int sum_blocks) {
+    constexpr int NF = N == 8 ? 4 : N, U = 8 / M;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     asm volatile("griddepcontrol.wait;" ::: "memory");
     // blocks that clear lie evenly between those that add: the ones write, the others read
@@ -339,48 +348,62 @@ __global__ void __launch_bounds__(kThreads) embedding_sums_kernel(const BwdParam
         return;
     }
     const long long task = (static_cast<int>(blockIdx.x) - cleared) * static_cast<long long>(kThreads / 32) + warp;
-    const int run = static_cast<int>(task / p.slices), c = (static_cast<int>(task - static_cast<long long>(run) * p.slices) * 32 + lane) * N;
-    const int first = run * p.run, total = *p.counted, n = min(p.run, total - first);
-    if (n <= 0) return;
-    const int2 own = lane < n ? p.sorted[first + lane] : make_int2(0, -1);
-    const int before = first > 0 ? p.sorted[first - 1].y : -1, behind = first + p.run < total ? p.sorted[first + p.run].y : -1;
-    float acc[N];
+    const int run = static_cast<int>(task / p.slices), c = (static_cast<int>(task - static_cast<long long>(run) * p.slices) * M * 32 + lane) * N;
+    if (run >= p.runs) return;
+    const int first = run * p.run;
+    const int2 own = lane < p.run ? p.sorted[first + lane] : make_int2(0, -1);
+    const int before = first > 0 ? p.sorted[first - 1].y : -1, behind = p.sorted[first + p.run].y;
+    const int n = __popc(__ballot_sync(0xffffffffu, own.y >= 0));
+    if (n == 0) return;
+    const int next = __shfl_down_sync(0xffffffffu, own.y, 1);
+    const unsigned ends = __ballot_sync(0xffffffffu, lane + 1 < n && next != own.y) | 1u << (n - 1);  // last rows of a token in this run
+    bool from_before = before == __shfl_sync(0xffffffffu, own.y, 0);
+    const bool goes_on = behind == __shfl_sync(0xffffffffu, own.y, n - 1);
+    const T* columns = static_cast<const T*>(p.d_out) + c;
+    bool in[M];
+    float acc[M][N];
 #pragma unroll
-    for (int k = 0; k < N; ++k) acc[k] = 0.0f;
-    int start = 0;
-    constexpr int U = 8;
+    for (int m = 0; m < M; ++m) {
+        in[m] = c + m * 32 * N < p.dim;
+#pragma unroll
+        for (int k = 0; k < N; ++k) acc[m][k] = 0.0f;
+    }
     for (int i0 = 0; i0 < n; i0 += U) {
-        Vec<T, N> q[U];
+        Vec<T, N> q[U][M];
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-            const long long row = __shfl_sync(0xffffffffu, own.x, (i0 + u) & 31);
-            if (i0 + u < n && c < p.dim) q[u] = *reinterpret_cast<const Vec<T, N>*>(static_cast<const T*>(p.d_out) + row * p.ld_dout + c);
+            const T* row = columns + __shfl_sync(0xffffffffu, own.x, (i0 + u) & 31) * p.ld_dout;
+            if (i0 + u < n)
+#pragma unroll
+                for (int m = 0; m < M; ++m)
+                    if (in[m]) q[u][m] = *reinterpret_cast<const Vec<T, N>*>(row + m * 32 * N);
         }
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-            const int i = i0 + u, token = __shfl_sync(0xffffffffu, own.y, i & 31), next = __shfl_sync(0xffffffffu, own.y, (i + 1) & 31);
+            const int i = i0 + u;
             if (i >= n) break;
-            float f[N];
-            q[u].widen(f);
 #pragma unroll
-            for (int k = 0; k < N; ++k) acc[k] += f[k];
-            const bool last = i + 1 == n;
-            if (!last && next == token) continue;
-            const bool begins = start > 0 || before != token, ends = !last || behind != token;
-            if (c < p.dim) {
-                if (begins && ends) {
-                    float* to = p.d_table + static_cast<long long>(token) * p.dim + c;
-                    write_sum<NF>(to, acc, p.scale, p.accumulate);
-                    if constexpr (N == 8) write_sum<NF>(to + 4, acc + 4, p.scale, p.accumulate);
-                } else {
-                    float* to = p.part + (2ll * run + (begins ? 1 : 0)) * p.dim + c;
-                    write_sum<NF>(to, acc, 1.0f, false);
-                    if constexpr (N == 8) write_sum<NF>(to + 4, acc + 4, 1.0f, false);
-                }
+            for (int m = 0; m < M; ++m) {
+                float f[N];
+                q[u][m].widen(f);
+#pragma unroll
+                for (int k = 0; k < N; ++k) acc[m][k] += f[k];
             }
+            if (!(ends >> i & 1)) continue;
+            // the run's part of a token that goes on, or the token's row
+            const bool whole = !from_before && !(goes_on && i + 1 == n);
+            float* to = whole ? p.d_table + static_cast<long long>(__shfl_sync(0xffffffffu, own.y, i)) * p.dim + c
+                              : p.part + (2ll * run + (from_before ? 0 : 1)) * p.dim + c;
 #pragma unroll
-            for (int k = 0; k < N; ++k) acc[k] = 0.0f;
-            start = i + 1;
+            for (int m = 0; m < M; ++m) {
+                if (in[m])
+#pragma unroll
+                    for (int k = 0; k < N; k += NF)
+                        write_sum<NF>(to + m * 32 * N + k, acc[m] + k, whole ? p.scale : 1.0f, whole && p.accumulate);
+#pragma unroll
+                for (int k = 0; k < N; ++k) acc[m][k] = 0.0f;
+            }
+            from_before = false;
         }
     }
 }
@@ -394,17 +417,17 @@ __global__ void __launch_bounds__(kThreads) embedding_join_kernel(const BwdParam
     __shared__ int far[WARPS];
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, c = (blockIdx.y * 32 + lane) * N;
     asm volatile("griddepcontrol.wait;" ::: "memory");
-    const int total = *p.counted, runs = (total + p.run - 1) / p.run;
-    if (static_cast<int>(blockIdx.x) * WARPS >= runs - 1) return;
+    const int runs = p.runs;
     auto add = [&](float* acc, int run, int begin, int end) {  // sums begin .. end of the token that begins in the run
         if (c >= p.dim) return;
-        for (int i0 = begin; i0 < end; i0 += 8) {
-            Vec<float, N> q[8];
+        constexpr int U = 8;
+        for (int i0 = begin; i0 < end; i0 += U) {
+            Vec<float, N> q[U];
 #pragma unroll
-            for (int u = 0; u < 8; ++u)
+            for (int u = 0; u < U; ++u)
                 if (i0 + u < end) q[u] = *reinterpret_cast<const Vec<float, N>*>(p.part + (2ll * (run + i0 + u) + (i0 + u == 0 ? 1 : 0)) * p.dim + c);
 #pragma unroll
-            for (int u = 0; u < 8; ++u)
+            for (int u = 0; u < U; ++u)
                 if (i0 + u < end)
 #pragma unroll
                     for (int k = 0; k < N; ++k) acc[k] += q[u].v[k];
@@ -416,7 +439,8 @@ __global__ void __launch_bounds__(kThreads) embedding_join_kernel(const BwdParam
     const int run = blockIdx.x * WARPS + warp;
     // lane l: the token at the start of run run + 1 + l; and those before this run and at its end
     const int ahead = run + 1 + lane < runs ? p.sorted[(run + 1 + lane) * p.run].y : -1;
-    const int before = run > 0 && run < runs ? p.sorted[run * p.run - 1].y : -1, token = run + 1 < runs ? p.sorted[run * p.run + p.run - 1].y : -2;
+    const int before = run > 0 && run < runs ? p.sorted[run * p.run - 1].y : -1, end = run + 1 < runs ? p.sorted[run * p.run + p.run - 1].y : -1;
+    const int token = end >= 0 ? end : -2;  // (-2: none goes on from here)
     const unsigned same = __ballot_sync(0xffffffffu, ahead == token);
     const bool begins = (same & 1) && before != token;
     if (lane == 0) far[warp] = begins && same == 0xffffffffu;
@@ -443,7 +467,7 @@ __global__ void __launch_bounds__(kThreads) embedding_join_kernel(const BwdParam
     }
 }
 
-constexpr long long kClearBeside = 48 << 20;
+constexpr long long kClearBeside = 128 << 20;
 // Rows of a run: fewer where that gives more warps something to do.
 static int run_of(long long rows, int dim) {
     int run = kMaxRun;
@@ -451,62 +475,72 @@ static int run_of(long long rows, int dim) {
     return run;
 }
 struct Room {
-    long long sorted, other, counted, present, part, bytes;
+    long long sorted, other, present, part, bytes;
 };
 static Room room_of(long long rows, int dim, int vocab) {
     auto up = [](long long n) { return (n + 255) / 256 * 256; };
     Room r{};
     if (rows <= kFewRows) return r;
-    r.other = up(rows * 8);
-    r.counted = 2 * r.other;
-    r.present = r.counted + 256;
-    r.part = r.present + up(vocab);
     const int run = run_of(rows, dim);
+    r.other = up(((rows + run - 1) / run + 1) * run * 8);
+    r.present = r.other + up(rows * 8);
+    r.part = r.present + up(vocab);
     r.bytes = r.part + (rows + run - 1) / run * 2 * dim * 4;
     return r;
 }
 
+// With `early` the kernel may start before the one ahead of it in the stream has ended, and waits for it itself.
 template <typename Kernel, typename... Args>
-static cudaError_t launch_early(Kernel fn, dim3 grid, int threads, cudaStream_t st, Args... args) {
+static cudaError_t launch_early(Kernel fn, dim3 grid, int threads, cudaStream_t st, int cluster, bool early, Args... args) {
     cudaLaunchConfig_t cfg;
     memset(&cfg, 0, sizeof(cfg));
     cfg.gridDim = grid;
     cfg.blockDim = dim3(threads);
     cfg.stream = st;
-    cudaLaunchAttribute at;
-    memset(&at, 0, sizeof(at));
-    at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    at.val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs = &at;
-    cfg.numAttrs = 1;
+    cudaLaunchAttribute at[2];
+    memset(at, 0, sizeof(at));
+    if (early) {
+        at[cfg.numAttrs].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        at[cfg.numAttrs++].val.programmaticStreamSerializationAllowed = 1;
+    }
+    if (cluster > 1) {
+        at[cfg.numAttrs].id = cudaLaunchAttributeClusterDimension;
+        at[cfg.numAttrs].val.clusterDim.x = cluster;
+        at[cfg.numAttrs].val.clusterDim.y = at[cfg.numAttrs].val.clusterDim.z = 1;
+        ++cfg.numAttrs;
+    }
+    cfg.attrs = at;
     return cudaLaunchKernelEx(&cfg, fn, args...);
 }
 
-template <typename T, int N>
+template <typename T, int N, int M>
 static int launch_bwd(Ctx* c, BwdParams& p, cudaStream_t st) {
-    p.slices = (p.dim + 32 * N - 1) / (32 * N);
     if (p.rows <= kFewRows) {
+        p.slices = (p.dim + 32 * N - 1) / (32 * N);
         const long long blocks = static_cast<long long>(p.rows) * p.slices + (p.accumulate ? 0 : (p.vocab + 7) / 8);
         embedding_bwd_few_kernel<T, N><<<static_cast<unsigned>(blocks), kThreads, 0, st>>>(p);
         MB200_CUDA_CHECK(c, cudaGetLastError());
         return MAMBA_B200_OK;
     }
+    p.slices = (p.dim + 32 * N * M - 1) / (32 * N * M);
     p.run = run_of(p.rows, p.dim);
     p.runs = (p.rows + p.run - 1) / p.run;
     for (p.passes = 1; p.passes < 4 && (p.vocab - 1) >> (8 * p.passes); ++p.passes) {}
     // what HBM can clear while the sort runs (some 8 us), of the last tokens: the rare ones where tokens are in order of frequency
     const long long beside = p.accumulate ? 0 : kClearBeside / (4ll * p.dim);
     p.cleared = p.vocab - static_cast<int>(beside < p.vocab ? beside : p.vocab);
-    const int clearers = p.cleared == p.vocab ? 0 : (c->sm_count - kSorters) / kSorters * kSorters;
     const long long sums = (static_cast<long long>(p.runs) * p.slices + kThreads / 32 - 1) / (kThreads / 32), clears = p.accumulate ? 0 : (p.cleared + 63) / 64;
     if (sums + clears > 2147483647ll) return fail(c, MAMBA_B200_ERR_SHAPE, "embedding_bwd: too many rows");
     constexpr int NJ = N == 8 ? 4 : N;
-    void* args[] = {&p};
-    MB200_CUDA_CHECK(c, launch_cluster(reinterpret_cast<const void*>(embedding_sort_kernel<NJ>), dim3(kSorters + clearers), dim3(kSortThreads), 0, st,
-                                       kSorters, args));
-    MB200_CUDA_CHECK(c, launch_early(embedding_sums_kernel<T, N>, dim3(static_cast<unsigned>(sums + clears)), kThreads, st, p, static_cast<int>(sums)));
+    const bool beside_sort = p.cleared < p.vocab;
+    if (beside_sort) {
+        embedding_clear_kernel<NJ><<<2 * c->sm_count, kThreads, 0, st>>>(p);
+        MB200_CUDA_CHECK(c, cudaGetLastError());
+    }
+    MB200_CUDA_CHECK(c, launch_early(embedding_sort_kernel, dim3(kSorters), kSortThreads, st, kSorters, beside_sort, p));
+    MB200_CUDA_CHECK(c, launch_early(embedding_sums_kernel<T, N, M>, dim3(static_cast<unsigned>(sums + clears)), kThreads, st, 1, true, p, static_cast<int>(sums)));
     MB200_CUDA_CHECK(c, launch_early(embedding_join_kernel<NJ>, dim3((p.runs + kThreads / 32 - 1) / (kThreads / 32), (p.dim + 32 * NJ - 1) / (32 * NJ)),
-                                     kThreads, st, p));
+                                     kThreads, st, 1, true, p));
     return MAMBA_B200_OK;
 }
 template <typename T>
@@ -516,16 +550,15 @@ static int launch_bwd(Ctx* c, BwdParams& p, cudaStream_t st) {
                reinterpret_cast<uintptr_t>(p.d_table) % 16 == 0;
     };
     if constexpr (sizeof(T) == 2) {
-        if (fits(8)) return launch_bwd<T, 8>(c, p, st);
+        if (fits(8)) return launch_bwd<T, 8, 1>(c, p, st);
     }
-    return fits(4) ? launch_bwd<T, 4>(c, p, st) : launch_bwd<T, 1>(c, p, st);
+    return fits(4) ? launch_bwd<T, 4, 2>(c, p, st) : launch_bwd<T, 1, 4>(c, p, st);
 }
 
 }  // namespace emb
 
 int embedding_configure(Ctx* c) {
-    MB200_CUDA_CHECK(c, cudaFuncSetAttribute(emb::embedding_sort_kernel<1>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
-    MB200_CUDA_CHECK(c, cudaFuncSetAttribute(emb::embedding_sort_kernel<4>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
+    MB200_CUDA_CHECK(c, cudaFuncSetAttribute(emb::embedding_sort_kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
     return MAMBA_B200_OK;
 }
 
@@ -579,7 +612,6 @@ extern "C" MAMBA_B200_API int mamba_b200_embedding_bwd(void* handle, void* strea
     unsigned char* ws = static_cast<unsigned char*>(workspace);
     p.sorted = reinterpret_cast<int2*>(ws + r.sorted);
     p.other = reinterpret_cast<int2*>(ws + r.other);
-    p.counted = reinterpret_cast<int*>(ws + r.counted);
     p.present = ws + r.present;
     p.part = reinterpret_cast<float*>(ws + r.part);
     cudaStream_t st = static_cast<cudaStream_t>(stream);
