@@ -32,6 +32,10 @@ struct Piece {
     static constexpr int W = 16 / sizeof(T);
     uint4 q;
     __device__ __forceinline__ void load(const T* p) { q = *reinterpret_cast<const uint4*>(p); }
+    __device__ __forceinline__ void ruled_out() {
+        const uint32_t w = sizeof(T) == 4 ? 0xff800000u : std::is_same<T, __half>::value ? 0xfc00fc00u : 0xff80ff80u;
+        q = make_uint4(w, w, w, w);
+    }
     __device__ __forceinline__ float2 pair(int j) const {
         if constexpr (sizeof(T) == 2) {
             return unpack2<T>(j == 0 ? q.x : j == 1 ? q.y : j == 2 ? q.z : q.w);
@@ -112,7 +116,8 @@ template <typename T>
 struct Running {
     float top, rho;
     float2 s, s1;
-    __device__ __forceinline__ Running() : top(-INFINITY), rho(kFarDown), s(splat2(0.0f)), s1(splat2(0.0f)) {}
+    bool masked;  // logits of minus infinity have been met
+    __device__ __forceinline__ Running() : top(-INFINITY), rho(kFarDown), s(splat2(0.0f)), s1(splat2(0.0f)), masked(false) {}
     __device__ __forceinline__ Sums sums() const { return {top, rho, s.x + s.y, s1.x + s1.y}; }
 
     // N pieces, kThreads apart, from `at`.
@@ -125,6 +130,19 @@ struct Running {
         top = fmaxf(top, Piece<T>::template top<N>(q));
         if (top * c > rho + kSlack) raise(top * c);  // (the first time, and where a row rises steeply)
         const float2 cc = splat2(c), neg = splat2(-rho), was = s1;
+        if (masked) {
+#pragma unroll
+            for (int u = 0; u < N; ++u)
+#pragma unroll
+                for (int k = 0; k < W / 2; ++k) {
+                    float2 t = fma2(q[u].pair(k), cc, neg);
+                    t.x = max_nan(t.x, kNothing), t.y = max_nan(t.y, kNothing);
+                    const float2 x = make_float2(ex2(t.x), ex2(t.y));
+                    s = add2(s, x);
+                    s1 = fma2(x, t, s1);
+                }
+            return;
+        }
 #pragma unroll
         for (int u = 0; u < N; ++u)
 #pragma unroll
@@ -134,7 +152,10 @@ struct Running {
                 s1 = fma2(x, t, s1);
             }
         // A logit of minus infinity has made 0 times minus infinity of its term (unless the sum is NaN already, and stays so).
-        if (!(s1.x + s1.y == s1.x + s1.y)) s1 = again<N>(at, c, was);
+        if (!(s1.x + s1.y == s1.x + s1.y)) {
+            s1 = again<N>(at, c, was);
+            masked = true;
+        }
     }
     template <int N>
     __device__ __noinline__ float2 again(const T* at, float c, float2 sum) const {
@@ -228,6 +249,33 @@ __device__ __forceinline__ void group_max(TopRoom& t, float own_top) {
 }
 __device__ __forceinline__ void sync_consumers() { asm volatile("bar.sync 1, %0;" ::"n"(kThreads) : "memory"); }
 
+// The n-th largest of the lanes' values (of their two values), in every lane.
+__device__ __forceinline__ float ordered(float v, int o, bool falling) {
+    const float other = __shfl_xor_sync(0xffffffffu, v, o);
+    return ((threadIdx.x & o) == 0) == falling ? fmaxf(v, other) : fminf(v, other);
+}
+__device__ __forceinline__ float nth_of_32(float v, int n) {
+#pragma unroll
+    for (int size = 2; size <= 32; size <<= 1)
+#pragma unroll
+        for (int o = size >> 1; o > 0; o >>= 1) v = ordered(v, o, (threadIdx.x % 32 & size) == 0);
+    return __shfl_sync(0xffffffffu, v, n - 1);
+}
+__device__ __forceinline__ float nth_of_64(float a, float b, int n) {  // n <= 32
+#pragma unroll
+    for (int size = 2; size <= 32; size <<= 1)
+#pragma unroll
+        for (int o = size >> 1; o > 0; o >>= 1) {
+            const bool falling = (threadIdx.x % 32 & size) == 0;
+            a = ordered(a, o, falling);
+            b = ordered(b, o, size == 32 ? false : falling);
+        }
+    a = fmaxf(a, b);  // the larger half; it falls and rises, one more pass puts it in order
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) a = ordered(a, o, true);
+    return __shfl_sync(0xffffffffu, a, n - 1);
+}
+
 // The alternatives of [lo, hi) pieces (and the ends) of a row.  Eight threads' elements form a group.  tau, the top-th largest of
 // the 32 groups' maxima, is a lower bound of the top-th largest element: only what threads whose own maximum reaches it have seen
 // is read again (from L2), and what reaches it there goes to key[0 .. n) in any order.  Called by kThreads threads behind a
@@ -238,15 +286,7 @@ template <typename T>
 __device__ __noinline__ int reach(TopRoom& t, const Row<T>& row, int lo, int hi, bool first, bool last, int top, float own_top, float* equals) {
     constexpr int W = Piece<T>::W;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-    float tau = t.group[lane];
-#pragma unroll
-    for (int size = 2; size <= 32; size <<= 1)
-#pragma unroll
-        for (int o = size >> 1; o > 0; o >>= 1) {
-            const float other = __shfl_xor_sync(0xffffffffu, tau, o);
-            tau = ((lane & o) == 0) == ((lane & size) == 0) ? fmaxf(tau, other) : fminf(tau, other);
-        }
-    tau = __shfl_sync(0xffffffffu, tau, top - 1);
+    const float tau = nth_of_32(t.group[lane], top);
     auto offer = [&](float v, int i) {
         if (v >= tau && v > -INFINITY) {
             const int at = atomicAdd(&t.n, 1);
@@ -354,12 +394,17 @@ __device__ __forceinline__ void rank_keys(const uint64_t* key, uint64_t* sel, in
     __syncwarp();
 }
 
-// One warp writes a row's results from its sums (alike in all lanes), the target's logit and the alternatives in order.
+// Sums relative to a row's largest logit from those relative to rho: rho is 0 then.
 template <typename T>
-__device__ __forceinline__ void write_row(const FwdParams& p, long long r, const Row<T>& row, Sums a, float c, int target, float logit, const uint64_t* sel) {
-    const int lane = threadIdx.x % 32;
+__device__ __forceinline__ void settle(Sums& a, const Row<T>& row, float c) {
     if (in_doubt(a)) a = sum_again(row, a.top, c);
     else a.rho = fmaf(a.top, c, -a.rho);  // top c - rho
+}
+// One warp writes a row's results from its sums (alike in all lanes; 2^rho more than those relative to the largest logit), the
+// target's logit and the alternatives in order.
+template <typename T>
+__device__ __forceinline__ void write_row(const FwdParams& p, long long r, const Sums& a, int target, float logit, const uint64_t* sel) {
+    const int lane = threadIdx.x % 32;
     const float log_s = (lg2(a.s) - a.rho) * kLn2;
     const bool none = a.s == 0.0f;
     if (lane == 0) {
@@ -386,12 +431,12 @@ __device__ __forceinline__ int target_of(const FwdParams& p, long long r) { retu
 // and SM in 16 bits: with 16 exponentials a cycle and some 5 instructions a logit (of 128) the arithmetic is close behind, so the
 // pass has one fma and one exponential a logit, no clamp, and no test but two in 32 logits.
 constexpr int kRound = kThreads * kUnroll, kStages = 3;
-constexpr int kMakers = 2;  // warps that make results
+constexpr int kMakers = 2, kMakerRoom = 256;  // warps that make results
 struct __align__(16) Maker {  // a row's, while the next rows' are found
     float thread_top[kThreads];
     Sums part[kWarps];
-    uint64_t key[kRoom], sel[kMaxTop], full, empty;
-    int n;
+    uint64_t key[kMakerRoom], sel[kMaxTop], full, empty;
+    int piece[kMakerRoom], n;
     unsigned char threads[kThreads];
 };
 struct RowsRoom {
@@ -408,40 +453,30 @@ static_assert(kCtas * (kRowsSmem + 1024) <= 228 * 1024, "CTAs on an SM");
 template <typename T>
 __device__ __noinline__ void find_top(Maker& t, const Row<T>& row, float row_top, int top) {
     constexpr int W = Piece<T>::W, kEach = kThreads / 32, kAtOnce = 4;
+    static_assert(kEach == 8, "two groups of four threads a lane");
     const int lane = threadIdx.x % 32;
-    float mine[kEach], tau = -INFINITY;
+    float mine[kEach];
 #pragma unroll
     for (int i = 0; i < kEach; i += 4) {
         const float4 v = *reinterpret_cast<const float4*>(t.thread_top + lane * kEach + i);
         mine[i] = v.x, mine[i + 1] = v.y, mine[i + 2] = v.z, mine[i + 3] = v.w;
-        tau = fmaxf(tau, fmaxf(fmaxf(v.x, v.y), fmaxf(v.z, v.w)));
     }
     __syncwarp();
     if (lane == 0) tc::mbar_arrive(&t.empty);
-#pragma unroll
-    for (int size = 2; size <= 32; size <<= 1)
-#pragma unroll
-        for (int o = size >> 1; o > 0; o >>= 1) {
-            const float other = __shfl_xor_sync(0xffffffffu, tau, o);
-            tau = ((lane & o) == 0) == ((lane & size) == 0) ? fmaxf(tau, other) : fminf(tau, other);
-        }
-    tau = __shfl_sync(0xffffffffu, tau, top - 1);
+    const float a = fmaxf(fmaxf(mine[0], mine[1]), fmaxf(mine[2], mine[3])), b = fmaxf(fmaxf(mine[4], mine[5]), fmaxf(mine[6], mine[7]));
+    const float tau = top <= 8 ? nth_of_32(fmaxf(a, b), top) : nth_of_64(a, b, top);
     int threads = 0;
 #pragma unroll
     for (int i = 0; i < kEach; ++i) {
         const bool hit = mine[i] >= tau && mine[i] > -INFINITY;
         const unsigned hits = __ballot_sync(0xffffffffu, hit);
-        if (hit) t.threads[threads + __popc(hits & ((1u << lane) - 1))] = lane * kEach + i;
+        if (hit) t.threads[threads + __popc(hits & ((1u << lane) - 1))] = static_cast<unsigned char>(lane * kEach + i);
         threads += __popc(hits);
     }
     if (lane == 0) t.n = 0;
     __syncwarp();
-    auto offer = [&](float v, int i) {
-        if (v >= tau && v > -INFINITY) {
-            const int at = atomicAdd(&t.n, 1);
-            if (at < kRoom) t.key[at] = key_of(v, i);
-        }
-    };
+    // their pieces that reach tau
+    int pieces = 0;
     for (int x = 0; x < threads; x += kAtOnce)
         for (int j0 = 0; j0 < row.pieces; j0 += 32 * kThreads) {
             Piece<T> q[kAtOnce];
@@ -453,21 +488,39 @@ __device__ __noinline__ void find_top(Maker& t, const Row<T>& row, float row_top
             }
 #pragma unroll
             for (int u = 0; u < kAtOnce; ++u) {
-                if (j[u] >= row.pieces || Piece<T>::template top<1>(q + u) < tau) continue;
-#pragma unroll
-                for (int e = 0; e < W; e += 2) {
-                    const float2 v = q[u].pair(e / 2);
-                    offer(v.x, row.head + j[u] * W + e);
-                    offer(v.y, row.head + j[u] * W + e + 1);
-                }
+                const float best = j[u] < row.pieces ? Piece<T>::template top<1>(q + u) : -INFINITY;
+                const bool hit = best >= tau && best > -INFINITY;
+                const unsigned hits = __ballot_sync(0xffffffffu, hit);
+                const int at = pieces + __popc(hits & ((1u << lane) - 1));
+                if (hit && at < kMakerRoom) t.piece[at] = j[u];
+                pieces += __popc(hits);
             }
         }
+    __syncwarp();
+    auto offer = [&](float v, int i) {
+        if (v >= tau && v > -INFINITY) {
+            const int at = atomicAdd(&t.n, 1);
+            if (at < kMakerRoom) t.key[at] = key_of(v, i);
+        }
+    };
+    for (int x = lane; x < min(pieces, kMakerRoom); x += 32) {
+        Piece<T> q;
+        const int j = t.piece[x];
+        q.load(row.p + row.head + static_cast<long long>(j) * W);
+#pragma unroll
+        for (int e = 0; e < W; e += 2) {
+            const float2 v = q.pair(e / 2);
+            offer(v.x, row.head + j * W + e);
+            offer(v.y, row.head + j * W + e + 1);
+        }
+    }
     if (lane < row.head) offer(to_f(row.p[lane]), lane);
     if (row.tail() + lane < row.V) offer(to_f(row.p[row.tail() + lane]), row.tail() + lane);
     __syncwarp();
-    int n = t.n;
+    int n = max(t.n, pieces);
+    if (n <= kMakerRoom) n = t.n;
     float equals = -INFINITY;
-    if (n > kRoom) {
+    if (n > kMakerRoom) {
         // More reach tau than there is room for: those above it one after the other, until tau itself is met.
         equals = tau;
         n = 0;
@@ -552,7 +605,8 @@ __global__ void __launch_bounds__(kThreads + 32 + 32 * kMakers, kCtas) token_log
                 __syncwarp();
                 if (lane == 0) tc::mbar_arrive(&t.empty);
             }
-            write_row<T>(p, r, row, a, c, target, logit, TOP ? t.sel : nullptr);
+            settle(a, row, c);
+            write_row<T>(p, r, a, target, logit, TOP ? t.sel : nullptr);
         }
         return;
     }
@@ -591,6 +645,106 @@ __global__ void __launch_bounds__(kThreads + 32 + 32 * kMakers, kCtas) token_log
         if (lane == 0) tc::mbar_arrive(&t.full);
         if (++maker == kMakers) maker = 0, flips ^= 1;
     }
+}
+
+// Short rows: a warp has one in registers, so the largest logit is known before the sums and nothing is read twice.  Up to
+// 32 P pieces; kShortPieces 32 are 8192 logits in 16 bits.
+constexpr int kShortPieces = 32, kShortWarps = 4, kShortRoom = 128;
+template <typename T, bool TOP, int P>
+__global__ void __launch_bounds__(kShortWarps * 32) token_logprobs_short_kernel(const FwdParams p) {
+    constexpr int W = Piece<T>::W;
+    __shared__ uint64_t keys[TOP ? kShortWarps : 1][kShortRoom], sels[TOP ? kShortWarps : 1][kMaxTop];
+    __shared__ int counts[kShortWarps];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const long long r = blockIdx.x * static_cast<long long>(kShortWarps) + warp;
+    if (r >= p.rows) return;
+    const Row<T> row(static_cast<const T*>(p.logits) + r * p.ld, p.V);
+    Piece<T> q[P];
+#pragma unroll
+    for (int u = 0; u < P; ++u) {
+        if (u * 32 + lane < row.pieces) q[u].load(row.p + row.head + (u * 32 + lane) * W);
+        else q[u].ruled_out();
+    }
+    const float head = lane < row.head ? to_f(row.p[lane]) : -INFINITY, tail = row.tail() + lane < p.V ? to_f(row.p[row.tail() + lane]) : -INFINITY;
+    const int target = target_of(p, r);
+    const float logit = target >= 0 && target < p.V ? to_f(row.p[target]) : 0.0f;
+    const float c = p.inv_temp * kLog2e, own_top = fmaxf(fmaxf(head, tail), Piece<T>::template top<P>(q));
+    Sums a{own_top, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) a.top = fmaxf(a.top, __shfl_xor_sync(0xffffffffu, a.top, o));
+    const float from = a.top == -INFINITY ? 0.0f : a.top;  // (nothing left: every term is 0, but for NaN)
+    const float2 cc = splat2(c), neg = splat2(-from);
+    float2 s = splat2(0.0f), s1 = splat2(0.0f);
+    auto term = [&](float2 v) {
+        float2 t = mul2(add2(v, neg), cc);
+        t.x = max_nan(t.x, kNothing), t.y = max_nan(t.y, kNothing);
+        const float2 x = make_float2(ex2(t.x), ex2(t.y));
+        s = add2(s, x);
+        s1 = fma2(x, t, s1);
+    };
+#pragma unroll
+    for (int u = 0; u < P; ++u)
+        if (u * 32 < row.pieces)
+#pragma unroll
+            for (int k = 0; k < W / 2; ++k) term(q[u].pair(k));
+    term(make_float2(head, tail));
+    a.s = s.x + s.y, a.s1 = s1.x + s1.y;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+        a.s += __shfl_xor_sync(0xffffffffu, a.s, o);
+        a.s1 += __shfl_xor_sync(0xffffffffu, a.s1, o);
+    }
+    uint64_t* sel = sels[TOP ? warp : 0];
+    if (TOP) {
+        uint64_t* key = keys[TOP ? warp : 0];
+        const float tau = nth_of_32(own_top, p.top);
+        if (lane == 0) counts[warp] = 0;
+        __syncwarp();
+        auto offer = [&](float v, int i) {
+            if (v >= tau && v > -INFINITY) {
+                const int at = atomicAdd(&counts[warp], 1);
+                if (at < kShortRoom) key[at] = key_of(v, i);
+            }
+        };
+        if (own_top >= tau && own_top > -INFINITY) {
+#pragma unroll
+            for (int u = 0; u < P; ++u)
+                if (Piece<T>::template top<1>(q + u) >= tau)
+#pragma unroll
+                    for (int e = 0; e < W; e += 2) {
+                        const float2 v = q[u].pair(e / 2);
+                        const int i = row.head + (u * 32 + lane) * W + e;
+                        offer(v.x, i);
+                        offer(v.y, i + 1);
+                    }
+            offer(head, lane);
+            offer(tail, row.tail() + lane);
+        }
+        __syncwarp();
+        const int n = counts[warp];
+        if (n >= p.top && n <= kShortRoom) {
+            rank_keys<T>(key, sel, n, 0.0f, row, 0, 0, p.top);
+        } else {
+            // crowded by equals, or fewer are left than asked for: one after the other
+            uint64_t below = ~0ull;
+            for (int k = 0; k < p.top; ++k) {
+                uint64_t best = 0;
+                for (int i = lane; i < p.V; i += 32) {
+                    const uint64_t k2 = key_of(to_f(row.p[i]), i);
+                    if (k2 < below && k2 > best) best = k2;
+                }
+#pragma unroll
+                for (int o = 16; o > 0; o >>= 1) {
+                    const uint64_t k2 = __shfl_xor_sync(0xffffffffu, best, o);
+                    if (k2 > best) best = k2;
+                }
+                below = best;
+                if (lane == 0) sel[k] = best;
+            }
+            __syncwarp();
+        }
+    }
+    write_row<T>(p, r, a, target, logit, TOP ? sel : nullptr);
 }
 
 // Few rows: the CTAs of a cluster have a part of one each, and the first joins what they found.
@@ -673,7 +827,10 @@ __global__ void __launch_bounds__(kThreads, 4) token_logprobs_split_kernel(const
         }
         sync_consumers();
     }
-    if (warp == 0) write_row<T>(p, r, row, a, c, target, logit, TOP ? room.sel : nullptr);
+    if (warp == 0) {
+        settle(a, row, c);
+        write_row<T>(p, r, a, target, logit, TOP ? room.sel : nullptr);
+    }
 }
 
 struct BwdParams {
@@ -759,6 +916,15 @@ static int pick_split(int sms, long long rows, int V) {
 
 template <typename T, bool TOP>
 static int launch_fwd(Ctx* c, FwdParams& p, cudaStream_t st) {
+    constexpr int W = Piece<T>::W;
+    if (p.V <= 32 * W * kShortPieces) {
+        const unsigned blocks = static_cast<unsigned>((p.rows + kShortWarps - 1) / kShortWarps);
+        if (p.V <= 32 * W * 4) token_logprobs_short_kernel<T, TOP, 4><<<blocks, kShortWarps * 32, 0, st>>>(p);
+        else if (p.V <= 32 * W * 16) token_logprobs_short_kernel<T, TOP, 16><<<blocks, kShortWarps * 32, 0, st>>>(p);
+        else token_logprobs_short_kernel<T, TOP, kShortPieces><<<blocks, kShortWarps * 32, 0, st>>>(p);
+        MB200_CUDA_CHECK(c, cudaGetLastError());
+        return MAMBA_B200_OK;
+    }
     p.split = pick_split(c->sm_count, p.rows, p.V);
     if (p.split == 1) {
         const long long most = static_cast<long long>(kCtas) * c->sm_count;
