@@ -431,7 +431,7 @@ __device__ __forceinline__ int target_of(const FwdParams& p, long long r) { retu
 // and SM in 16 bits: with 16 exponentials a cycle and some 5 instructions a logit (of 128) the arithmetic is close behind, so the
 // pass has one fma and one exponential a logit, no clamp, and no test but two in 32 logits.
 constexpr int kRound = kThreads * kUnroll, kStages = 3;
-constexpr int kMakers = 2, kMakerRoom = 256;  // warps that make results
+constexpr int kMakers = 3, kMakerRoom = 256;  // warps that make results
 struct __align__(16) Maker {  // a row's, while the next rows' are found
     float thread_top[kThreads];
     Sums part[kWarps];
@@ -907,25 +907,28 @@ __global__ void __launch_bounds__(kBwdThreads, 4) token_logprobs_bwd_kernel(cons
     if (i < p.V) out[i] = from_f<T>(one(to_f(row.p[i]), i));
 }
 
-// How many CTAs share a row: as many as find room beside one another (four on an SM), each with 2048 logits or more.
-static int pick_split(int sms, long long rows, int V) {
+// How many CTAs share a row: as many as find room beside one another (four on an SM), each with 2048 logits or more.  Joining the
+// parts' alternatives costs more than reading them faster gains: 8 rows of 50280 with 20 alternatives 15.6 us over 16 CTAs, 10.6 over
+// 8, 9.9 over 4; without alternatives 4.1, 4.8 and 4.8.
+static int pick_split(int sms, long long rows, int V, bool top) {
     int s = 1;
-    while (s < kMaxSplit && rows * 2 * s <= 4ll * sms && V >= 2 * s * 2048) s *= 2;
+    while (s < (top ? 4 : kMaxSplit) && rows * 2 * s <= 4ll * sms && V >= 2 * s * 2048) s *= 2;
     return s;
 }
 
 template <typename T, bool TOP>
 static int launch_fwd(Ctx* c, FwdParams& p, cudaStream_t st) {
     constexpr int W = Piece<T>::W;
-    if (p.V <= 32 * W * kShortPieces) {
+    if (p.V <= 32 * W * (TOP ? kShortPieces / 2 : kShortPieces)) {
         const unsigned blocks = static_cast<unsigned>((p.rows + kShortWarps - 1) / kShortWarps);
         if (p.V <= 32 * W * 4) token_logprobs_short_kernel<T, TOP, 4><<<blocks, kShortWarps * 32, 0, st>>>(p);
+        else if (p.V <= 32 * W * 8) token_logprobs_short_kernel<T, TOP, 8><<<blocks, kShortWarps * 32, 0, st>>>(p);
         else if (p.V <= 32 * W * 16) token_logprobs_short_kernel<T, TOP, 16><<<blocks, kShortWarps * 32, 0, st>>>(p);
         else token_logprobs_short_kernel<T, TOP, kShortPieces><<<blocks, kShortWarps * 32, 0, st>>>(p);
         MB200_CUDA_CHECK(c, cudaGetLastError());
         return MAMBA_B200_OK;
     }
-    p.split = pick_split(c->sm_count, p.rows, p.V);
+    p.split = pick_split(c->sm_count, p.rows, p.V, TOP);
     if (p.split == 1) {
         const long long most = static_cast<long long>(kCtas) * c->sm_count;
         token_logprobs_rows_kernel<T, TOP><<<static_cast<unsigned>(p.rows < most ? p.rows : most), kThreads + 32 + 32 * kMakers, kRowsSmem, st>>>(p, c->d_status);

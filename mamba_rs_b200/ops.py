@@ -579,6 +579,24 @@ def _same_device(dev, *named):
             raise ValueError(f"{nm} is on {t.device}, not on {dev}")
 
 
+def _row(t, width):
+    """Row stride of a matrix (of one row: any that is no narrower than the row)."""
+    return t.stride(0) if t.shape[0] > 1 else max(t.stride(0), width)
+
+
+def _launch(fn, dev, handle, *args):
+    """fn(handle, current stream of dev, *args) with dev current; failures as the library words them."""
+    index = dev.index or 0
+    h = handle or ffi.default_handle(index)
+    if torch._C._cuda_getDevice() == index:
+        rc = fn(h.ptr, torch._C._cuda_getCurrentRawStream(index), *args)
+    else:
+        with torch.cuda.device(dev):
+            rc = fn(h.ptr, torch._C._cuda_getCurrentRawStream(index), *args)
+    if rc:
+        h.check(rc, fn.__name__)
+
+
 def embedding_fwd(table, ids, *, scale=1.0, out=None, out_dtype=torch.float32, handle=None):
     """out [rows, dim] = scale * table[ids]: table [vocab, dim] in the storage dtype (any row stride), ids int32 of any
     shape; out in float32 (the residual stream) or the table's dtype.  An id outside the table gives a row of zeros."""
@@ -593,12 +611,8 @@ def embedding_fwd(table, ids, *, scale=1.0, out=None, out_dtype=torch.float32, h
     elif tuple(out.shape) != (rows, dim) or out.stride(1) != 1:
         raise ValueError(f"out is [{rows}, {dim}] with contiguous rows")
     _same_device(dev, (ids, "ids"), (out, "out"))
-    h = handle or ffi.default_handle(dev.index or 0)
-    with _on(dev):
-        rc = ffi.lib().mamba_b200_embedding_fwd(h.ptr, _stream(dev), dtype_code(table.dtype), table.data_ptr(),
-                                                max(table.stride(0), dim), ids.data_ptr(), dtype_code(out.dtype), out.data_ptr(),
-                                                max(out.stride(0), dim), rows, dim, vocab, scale)
-    h.check(rc, "mamba_b200_embedding_fwd")
+    _launch(ffi.lib().mamba_b200_embedding_fwd, dev, handle, dtype_code(table.dtype), table.data_ptr(), _row(table, dim), ids.data_ptr(),
+            dtype_code(out.dtype), out.data_ptr(), _row(out, dim), rows, dim, vocab, scale)
     return out
 
 
@@ -632,14 +646,12 @@ def embedding_bwd(ids, d_out, vocab=None, *, d_table=None, scale=1.0, workspace=
         d_table = torch.empty((vocab, dim), dtype=torch.float32, device=dev)
     lib = ffi.lib()
     if workspace is None:
-        workspace = torch.empty(lib.mamba_b200_embedding_bwd_workspace_bytes(rows, dim, vocab), dtype=torch.uint8, device=dev)
+        need = lib.mamba_b200_embedding_bwd_workspace_bytes(rows, dim, vocab)
+        workspace = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
     _same_device(dev, (ids, "ids"), (d_table, "d_table"), (workspace, "workspace"))
-    h = handle or ffi.default_handle(dev.index or 0)
-    with _on(dev):
-        rc = lib.mamba_b200_embedding_bwd(h.ptr, _stream(dev), dtype_code(d_out.dtype), d_out.data_ptr(), max(d_out.stride(0), dim),
-                                          ids.data_ptr(), d_table.data_ptr(), accumulate, rows, dim, vocab, scale,
-                                          workspace.data_ptr(), workspace.numel() * workspace.element_size())
-    h.check(rc, "mamba_b200_embedding_bwd")
+    _launch(lib.mamba_b200_embedding_bwd, dev, handle, dtype_code(d_out.dtype), d_out.data_ptr(), _row(d_out, dim), ids.data_ptr(),
+            d_table.data_ptr(), accumulate, rows, dim, vocab, scale, _ptr(workspace),
+            0 if workspace is None else workspace.numel() * workspace.element_size())
     return d_table
 
 
@@ -660,7 +672,6 @@ def token_logprobs(logits, targets=None, *, top=0, temperature=1.0, handle=None)
     rows, V = logits.shape
     dev = logits.device
     _same_device(dev, (targets, "targets"))
-    h = handle or ffi.default_handle(dev.index or 0)
     if not 0 <= top <= min(32, V):
         raise ValueError(f"{top} alternatives of {V} tokens (at most 32)")
     res = torch.empty((3 if targets is None else 4, rows), dtype=torch.float32, device=dev)
@@ -673,11 +684,8 @@ def token_logprobs(logits, targets=None, *, top=0, temperature=1.0, handle=None)
         ids, val = torch.empty((rows, top), dtype=torch.int32, device=dev), torch.empty((rows, top), dtype=torch.float32, device=dev)
         ip, vp = ids.data_ptr(), val.data_ptr()
         out["top_ids"], out["top_logprobs"] = ids, val
-    with _on(dev):
-        rc = ffi.lib().mamba_b200_token_logprobs(h.ptr, _stream(dev), dtype_code(logits.dtype), logits.data_ptr(),
-                                                 max(logits.stride(0), V), _ptr(targets), temperature, base, base + 8 * rows,
-                                                 None if targets is None else base + 12 * rows, top, ip, vp, rows, V)
-    h.check(rc, "mamba_b200_token_logprobs")
+    _launch(ffi.lib().mamba_b200_token_logprobs, dev, handle, dtype_code(logits.dtype), logits.data_ptr(), _row(logits, V), _ptr(targets),
+            temperature, base, base + 8 * rows, None if targets is None else base + 12 * rows, top, ip, vp, rows, V)
     return out
 
 
@@ -698,13 +706,9 @@ def token_logprobs_bwd(logits, targets, lse, entropy, d_logprob=None, d_entropy=
         raise TypeError("dlogits has the logits' dtype and shape and contiguous rows")
     _same_device(dev, (targets, "targets"), (lse, "lse"), (entropy, "entropy"), (d_logprob, "d_logprob"), (d_entropy, "d_entropy"),
                  (dlogits, "dlogits"))
-    h = handle or ffi.default_handle(dev.index or 0)
-    with _on(dev):
-        rc = ffi.lib().mamba_b200_token_logprobs_bwd(h.ptr, _stream(dev), dtype_code(logits.dtype), logits.data_ptr(),
-                                                     max(logits.stride(0), V), _ptr(targets), temperature, lse.data_ptr(),
-                                                     _ptr(entropy), _ptr(d_logprob), _ptr(d_entropy), dlogits.data_ptr(),
-                                                     max(dlogits.stride(0), V), rows, V)
-    h.check(rc, "mamba_b200_token_logprobs_bwd")
+    _launch(ffi.lib().mamba_b200_token_logprobs_bwd, dev, handle, dtype_code(logits.dtype), logits.data_ptr(), _row(logits, V),
+            _ptr(targets), temperature, lse.data_ptr(), _ptr(entropy), _ptr(d_logprob), _ptr(d_entropy), dlogits.data_ptr(),
+            _row(dlogits, V), rows, V)
     return dlogits
 
 
@@ -762,26 +766,38 @@ def gated_scan_fwd(x, f, z=None, *, h0=None, h_last=None, y=None, chunk_states=N
         y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
     B, T, D = x.shape
     dev = x.device
-    h = handle or ffi.default_handle(dev.index or 0)
     a = ffi.GatedScanArgs(dtype_code(x.dtype), B, T, D, x.data_ptr(), _gated_rows(x, "x", x), f.data_ptr(), _gated_rows(f, "f", x),
                           _ptr(z), 0 if z is None else _gated_rows(z, "z", x), _gated_state(h0, "h0", x),
                           _gated_state(h_last, "h_last", x), y.data_ptr(), _gated_rows(y, "y", x),
                           _gated_state(chunk_states, "chunk_states", x, gated_scan_states(B, T, D)))
     if T > 8:
         workspace, a.workspace, a.workspace_bytes = _gated_workspace(workspace, x)
-    with _on(dev):
-        rc = ffi.lib().mamba_b200_gated_scan_fwd(h.ptr, _stream(dev), C.byref(a))
-    h.check(rc, "mamba_b200_gated_scan_fwd")
+    _launch(ffi.lib().mamba_b200_gated_scan_fwd, dev, handle, C.byref(a))
     return y
 
 
 def gated_scan_step(x, f, h0, z=None, *, h_last=None, y=None, handle=None):
     """One token per sequence: x, f, z, y [B,D]; the state h0 [B,D] f32 is updated in place, or h_last receives it."""
-    row = lambda t: None if t is None else t.unsqueeze(1)  # noqa: E731
+    _require_cuda(x, f, z, h0, h_last, y)
     if y is None:
         y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    gated_scan_fwd(x.unsqueeze(1), f.unsqueeze(1), row(z), h0=h0, h_last=h0 if h_last is None else h_last, y=y.unsqueeze(1),
-                   handle=handle)
+    B, D = shape = x.shape
+
+    def row(t, name):
+        if t.dtype != x.dtype or t.shape != shape or t.device != x.device:
+            raise TypeError(f"{name} has x's dtype, shape and device: {list(shape)} {x.dtype}")
+        ld, one = t.stride()
+        if one != 1 and D > 1:
+            raise ValueError(f"{name}: last dimension must be contiguous")
+        return ld if B > 1 else D
+
+    for t, name in ((h0, "h0"), (h_last, "h_last")):
+        if t is not None and (t.dtype != torch.float32 or t.shape != shape or not t.is_contiguous() or t.device != x.device):
+            raise TypeError(f"{name} is contiguous float32 {list(shape)} on x's device")
+    h = h0.data_ptr()
+    a = ffi.GatedScanArgs(dtype_code(x.dtype), B, 1, D, x.data_ptr(), row(x, "x"), f.data_ptr(), row(f, "f"), _ptr(z),
+                          0 if z is None else row(z, "z"), h, h if h_last is None else h_last.data_ptr(), y.data_ptr(), row(y, "y"))
+    _launch(ffi.lib().mamba_b200_gated_scan_fwd, x.device, handle, C.byref(a))
     return y
 
 
@@ -792,7 +808,6 @@ def gated_scan_bwd(x, f, dy, chunk_states, z=None, *, d_last=None, d_h0=None, d_
     _require_cuda(x, f, z, dy, chunk_states, d_last, d_h0, d_x, d_f, d_z, workspace)
     B, T, D = x.shape
     dev = x.device
-    h = handle or ffi.default_handle(dev.index or 0)
     new = lambda t: torch.empty(x.shape, dtype=x.dtype, device=dev) if t is None else t  # noqa: E731
     d_x, d_f = new(d_x), new(d_f)
     d_z = new(d_z) if z is not None else None
@@ -805,9 +820,7 @@ def gated_scan_bwd(x, f, dy, chunk_states, z=None, *, d_last=None, d_h0=None, d_
                           d_x.data_ptr(), _gated_rows(d_x, "d_x", x), d_f.data_ptr(), _gated_rows(d_f, "d_f", x),
                           _ptr(d_z), 0 if d_z is None else _gated_rows(d_z, "d_z", x))
     workspace, a.workspace, a.workspace_bytes = _gated_workspace(workspace, x)
-    with _on(dev):
-        rc = ffi.lib().mamba_b200_gated_scan_bwd(h.ptr, _stream(dev), C.byref(a))
-    h.check(rc, "mamba_b200_gated_scan_bwd")
+    _launch(ffi.lib().mamba_b200_gated_scan_bwd, dev, handle, C.byref(a))
     out = dict(d_x=d_x, d_f=d_f, d_h0=d_h0)
     if d_z is not None:
         out["d_z"] = d_z

@@ -165,3 +165,14 @@ def test_no_rows_and_refusals(cuda_dev):
         with pytest.raises(RuntimeError, match="workspace"):
             mb.embedding_bwd(torch.zeros(9000, dtype=torch.int32, device=cuda_dev), torch.ones(9000, 8, device=cuda_dev), 5,
                              workspace=torch.empty(0, dtype=torch.uint8, device=cuda_dev))
+
+
+def test_rows_that_are_one_in_memory_are_refused(cuda_dev):
+    """An expanded tensor has a row stride of 0: it is no matrix of that many rows for the kernels."""
+    import torch
+
+    import mamba_rs_b200 as mb
+    one, ids = torch.ones(1, 8, device=cuda_dev), torch.zeros(4, dtype=torch.int32, device=cuda_dev)
+    for bad in (lambda: mb.embedding_fwd(one.expand(5, 8), ids), lambda: mb.embedding_bwd(ids, one.expand(4, 8), 5)):
+        with pytest.raises(RuntimeError, match="bad dims"):
+            bad()

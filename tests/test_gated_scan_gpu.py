@@ -268,3 +268,40 @@ def test_empty_windows_and_refusals(cuda_dev):
         mb.gated_scan_fwd(c[0], c[1][:1, :1].expand(2, 6, 8))
     with pytest.raises(RuntimeError, match="CUDA tensors only"):
         mb.gated_scan_fwd(c[0].cpu(), c[1])
+
+
+def test_step_refusals_and_strides(cuda_dev):
+    import torch
+
+    import mamba_rs_b200 as mb
+    x, f, z, h0 = _inputs(3, 1, 9, "bf16", cuda_dev, pad=2)
+    x, f, z = x[:, 0], f[:, 0], z[:, 0]
+    out = torch.empty_like(h0)
+    want = mb.gated_scan_step(x.contiguous(), f.contiguous(), h0, z.contiguous(), h_last=out)
+    assert torch.equal(mb.gated_scan_step(x, f, h0, z, h_last=out), want)
+    for bad in (lambda: mb.gated_scan_step(x, f[:2], h0), lambda: mb.gated_scan_step(x, f.float(), h0), lambda: mb.gated_scan_step(x, f, h0.half()),
+                lambda: mb.gated_scan_step(x, f, h0, h_last=h0[:2])):
+        with pytest.raises(TypeError):
+            bad()
+    with pytest.raises(ValueError):
+        mb.gated_scan_step(x, torch.zeros(9, 3, device=cuda_dev, dtype=x.dtype).t(), h0)
+    with pytest.raises(RuntimeError, match="row stride"):
+        mb.gated_scan_step(x, f[:1].expand(3, 9), h0)
+
+
+@pytest.mark.parametrize("dt", DT)
+@pytest.mark.parametrize("B,T,D", [(1, 1300, 40), (1, 700, 130), (2, 5000, 33)])
+def test_any_workspace_gives_the_same_up_to_rounding(cuda_dev, dt, B, T, D):
+    """None, too little for every segment, and more than enough."""
+    import torch
+
+    import mamba_rs_b200 as mb
+    x, f, z, h0 = _inputs(B, T, D, dt, cuda_dev, seed=9)
+    hs, y, last = _plain(x, f, z, h0)
+    tol, gz = _state_tol(x, f, h0), (z.double() * torch.sigmoid(z.double())).abs()
+    need = mb.gated_scan_workspace_bytes(B, T, D)
+    for size in (0, 8 * B * D, 8 * B * D * 3, need, need + 4096):
+        h = h0.clone()
+        got = mb.gated_scan_fwd(x, f, z, h0=h, h_last=h, workspace=torch.full((size,), 255, dtype=torch.uint8, device=cuda_dev))
+        assert ((got.double() - y).abs() <= tol * gz + (HALF[dt] * 1.01 + 2.0 ** -20) * y.abs() + TINY[dt]).all()
+        assert ((h.double() - last).abs() <= tol).all()

@@ -274,3 +274,16 @@ def test_no_rows_and_refusals(cuda_dev):
         mb.token_logprobs_bwd(l, None, v2, v, v)  # a gradient of log probabilities of no tokens
     with pytest.raises(RuntimeError, match="CUDA tensors only"):
         mb.token_logprobs(l.cpu())
+
+
+def test_rows_that_are_one_in_memory_are_refused(cuda_dev):
+    """An expanded tensor has a row stride of 0: it is no matrix of that many rows for the kernels."""
+    import torch
+
+    import mamba_rs_b200 as mb
+    l, t = _case(1, 40, "f32", cuda_dev)
+    v = torch.zeros(3, device=cuda_dev)
+    with pytest.raises(RuntimeError, match="bad dims"):
+        mb.token_logprobs(l.expand(3, 40))
+    with pytest.raises(RuntimeError, match="bad dims"):
+        mb.token_logprobs_bwd(l.expand(3, 40), None, torch.zeros(2, 3, device=cuda_dev), v, None, v)
