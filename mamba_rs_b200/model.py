@@ -671,6 +671,24 @@ class GpuMambaLM:
         torch.matmul(hidden, emb.t(), out=self.logits)
         self.next_ids.copy_(self.logits.argmax(dim=1))
 
+    def score(self, ids: torch.Tensor, top: int = 0, temperature: float = 1.0, rows: int = 4096) -> dict:
+        """ids [B, T] int32, T > 1: of each token behind the first its log probability given those before it, the entropy of its
+        distribution and the `top` most likely tokens (dict of logprob, entropy [B, T-1], with top > 0 top_ids, top_logprobs
+        [B, T-1, top]).  Starts from the engine's state and leaves it behind the last token but one (``backbone.reset`` for a new
+        text).  The logits of at most `rows` positions exist at a time."""
+        if ids.dtype != torch.int32 or ids.dim() != 2:
+            raise TypeError("ids are int32 [B, T]")
+        B, T = ids.shape
+        if T < 2 or rows < 1:
+            raise ValueError("a text has two tokens or more, and a part of it at least one row")
+        emb = self.w.tail()["embedding"]
+        temporal = ops.embedding_gather(emb, ids[:, :-1].contiguous()).view(B, T - 1, -1)
+        hidden = self.backbone.prefill_sequence(temporal).view(B * (T - 1), -1)
+        targets = ids[:, 1:].reshape(-1)
+        parts = [ops.token_logprobs(hidden[r:r + rows] @ emb.t(), targets[r:r + rows], top=top, temperature=temperature)
+                 for r in range(0, hidden.shape[0], rows)]
+        return {k: torch.cat([p[k] for p in parts]).view(B, T - 1, *parts[0][k].shape[1:]) for k in parts[0] if k != "lse"}
+
     def _decode_once(self, operators=False):
         emb = self.w.tail()["embedding"]
         temporal = ops.embedding_gather(emb, self.next_ids)
