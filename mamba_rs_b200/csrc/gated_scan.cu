@@ -65,7 +65,7 @@ struct Params {
     mamba_b200_gated_scan_args a;
     int* status;
     float* sums;  // [B, segments, 2, D]: what each segment does to the state (or gradient) that enters it
-    int tiles, segments, per_segment, tma_in, tma_out;
+    int tiles, segments, per_segment, tma_out;
 };
 
 // ---------------------------------------------------------------------------------------------------
@@ -89,7 +89,7 @@ struct Layout {
     static_assert(L * CH * sizeof(T) >= 2 * CH * sizeof(float), "two sums in a warp's rows of f");
 };
 
-template <typename T, int V, int NIN, bool BWD>
+template <typename T, int V, int NIN, bool BWD, bool PLAIN>
 struct Tiles {
     using Lay = Layout<T, V, NIN, BWD>;
     const Params& p;
@@ -106,23 +106,41 @@ struct Tiles {
     __device__ __forceinline__ void ask(int s, int k, const CUtensorMap* const* map) {
         if (threadIdx.x != 0) return;
         if (p.tma_out) tma_wait_read0();
-        if (!p.tma_in) return;
+        if (PLAIN) return;
         mbar_expect_tx(&bars[s], NIN * Lay::kIn);
 #pragma unroll
         for (int i = 0; i < NIN; ++i) tma_load_3d(sm + (s * NIN + i) * Lay::kIn, map[i], &bars[s], c0, k * kTile, b);
     }
     // The warp's rows of tile k are in stage s from here on; steps behind the end have gates that change nothing.
-    __device__ __forceinline__ void wait(int s, int k, uint32_t parity, const void* const* src, const long long* ld) {
-        if (p.tma_in) {
-            alive = alive && mbar_wait(&bars[s], parity, p.status);
-        } else {
-#pragma unroll 1
-            for (int i = 0; i < NIN; ++i)
-                plain_channels<Lay::CH>(at(s, i) + warp * L * Lay::CH, static_cast<const T*>(src[i]), ld[i],
-                                        static_cast<long long>(b) * p.a.T, k * kTile + warp * L, L, p.a.T, c0, p.a.D, lane);
-            __syncwarp();
-        }
+    __device__ __forceinline__ void wait(int s, int k, uint32_t parity) {
+        alive = alive && mbar_wait(&bars[s], parity, p.status);
         for (int j = max(0, p.a.T - k * kTile - warp * L); j < L; ++j) Ch<V>::splat(INFINITY).store(mine(s, 0) + j * Lay::CH);
+    }
+    // Rows that TMA cannot describe: a lane fetches its own channels of the warp's rows, a tile ahead, and hands them over in shared
+    // memory.  (Fetched when they were needed, a tile took 4 us.)
+    struct __align__(sizeof(T) * V) Word { T v[V]; };
+    __device__ __forceinline__ void fetch(Word (*to)[L], int k, const void* const* src, const long long* ld) const {
+        const int c = c0 + lane * V, t0 = k * kTile + warp * L;
+        const bool inside = c0 + Lay::CH <= p.a.D && t0 + L <= p.a.T;
+#pragma unroll
+        for (int i = 0; i < NIN; ++i) {
+            const T* row = static_cast<const T*>(src[i]) + (static_cast<long long>(b) * p.a.T + t0) * ld[i] + c;
+            if (inside) {
+#pragma unroll
+                for (int j = 0; j < L; ++j) to[i][j] = *reinterpret_cast<const Word*>(row + j * ld[i]);
+            } else {
+#pragma unroll
+                for (int j = 0; j < L; ++j)
+#pragma unroll
+                    for (int e = 0; e < V; ++e) to[i][j].v[e] = t0 + j < p.a.T && c + e < p.a.D ? row[j * ld[i] + e] : from_f<T>(i == 0 ? INFINITY : 0.0f);
+            }
+        }
+    }
+    __device__ __forceinline__ void hand_over(const Word (*from)[L], int s) {
+#pragma unroll
+        for (int i = 0; i < NIN; ++i)
+#pragma unroll
+            for (int j = 0; j < L; ++j) *reinterpret_cast<Word*>(mine(s, i) + j * Lay::CH) = from[i][j];
     }
     // Writes input i's place in stage s to a tensor, row by row, where TMA cannot.
     __device__ __forceinline__ void plain_out(int s, int i, int k, void* dst, long long ld) const {
@@ -173,8 +191,8 @@ __device__ __forceinline__ Ch<V> enter(const Params& p, float* part, int b, int 
     return v;
 }
 
-template <typename T, int V, bool GATE>
-__global__ void __launch_bounds__(kFwdWarps * 32, kFwdCtas)
+template <typename T, int V, bool GATE, bool PLAIN>
+__global__ void __launch_bounds__(kFwdWarps * 32, PLAIN ? 2 : kFwdCtas)
     gated_scan_fwd_kernel(const __grid_constant__ CUtensorMap mf, const __grid_constant__ CUtensorMap mx,
                           const __grid_constant__ CUtensorMap mz, const __grid_constant__ CUtensorMap my, const __grid_constant__ Params p) {
     constexpr int NIN = GATE ? 3 : 2;
@@ -192,7 +210,8 @@ __global__ void __launch_bounds__(kFwdWarps * 32, kFwdCtas)
         fence_barrier_init();
     }
     __syncthreads();
-    Tiles<T, V, NIN, false> in{p, sm, bars, b, c0, warp, lane, true};
+    using In = Tiles<T, V, NIN, false, PLAIN>;
+    In in{p, sm, bars, b, c0, warp, lane, true};
     const CUtensorMap* maps[3] = {&mf, &mx, &mz};
     const void* src[3] = {p.a.f, p.a.x, p.a.z};
     const long long ld[3] = {p.a.ld_f, p.a.ld_x, p.a.ld_z};
@@ -200,6 +219,8 @@ __global__ void __launch_bounds__(kFwdWarps * 32, kFwdCtas)
 #pragma unroll
     for (int i = 0; i < S - 1; ++i)
         if (i < rounds) in.ask(i, first + i, maps);
+    typename In::Word next_rows[PLAIN ? NIN : 1][L];
+    if (PLAIN && rounds > 0) in.fetch(next_rows, first, src, ld);
     C carry = C::splat(0.0f);
     if (p.segments > 1) carry = enter<V, W>(p, reinterpret_cast<float*>(in.at(S - 1, 0)), b, c, p.segments - 1, 0, seg, 1);
     else if (p.a.h0) carry = get<V>(p.a.h0 + static_cast<long long>(b) * D, c, D);
@@ -209,7 +230,12 @@ __global__ void __launch_bounds__(kFwdWarps * 32, kFwdCtas)
         const int k = first + it;
         // what the steps up to each one do to the state that enters the span, and the output gates
         C n[L], a[L], q[GATE ? L : 1], N = C::splat(0.0f), A = C::splat(0.0f);
-        in.wait(s, k, parity, src, ld);
+        if constexpr (PLAIN) {
+            in.hand_over(next_rows, s);
+            if (it + 1 < rounds) in.fetch(next_rows, k + 1, src, ld);
+        } else {
+            in.wait(s, k, parity);
+        }
         const T *sf = in.mine(s, 0), *sx = in.mine(s, 1), *sz = in.mine(s, NIN - 1);
 #pragma unroll
         for (int j = 0; j < L; ++j) {
@@ -265,8 +291,8 @@ __global__ void __launch_bounds__(kFwdWarps * 32, kFwdCtas)
 // The gradient walks the tiles from the last to the first.  The states inside a tile come from the saved one that enters it, by
 // the same two walks; g is joined over the warps (and the cluster) the same way in the other direction: over a span of steps
 // (1 - u) g at its first step = g_behind - U g_behind + G, with the forward's U.  g runs with its sign turned, like the gates.
-template <typename T, int V, bool GATE>
-__global__ void __launch_bounds__(kBwdWarps * 32, 3)
+template <typename T, int V, bool GATE, bool PLAIN>
+__global__ void __launch_bounds__(kBwdWarps * 32, PLAIN ? 2 : 3)
     gated_scan_bwd_kernel(const __grid_constant__ CUtensorMap mf, const __grid_constant__ CUtensorMap mx, const __grid_constant__ CUtensorMap me,
                           const __grid_constant__ CUtensorMap mz, const __grid_constant__ CUtensorMap mdf, const __grid_constant__ CUtensorMap mdx,
                           const __grid_constant__ CUtensorMap mdz, const __grid_constant__ Params p) {
@@ -286,7 +312,8 @@ __global__ void __launch_bounds__(kBwdWarps * 32, 3)
         fence_barrier_init();
     }
     __syncthreads();
-    Tiles<T, V, NIN, true> in{p, sm, bars, b, c0, warp, lane, true};
+    using In = Tiles<T, V, NIN, true, PLAIN>;
+    In in{p, sm, bars, b, c0, warp, lane, true};
     const CUtensorMap* maps[4] = {&mf, &mx, &me, &mz};
     const void* src[4] = {p.a.f, p.a.x, p.a.dy, p.a.z};
     const long long ld[4] = {p.a.ld_f, p.a.ld_x, p.a.ld_dy, p.a.ld_z};
@@ -295,6 +322,8 @@ __global__ void __launch_bounds__(kBwdWarps * 32, 3)
 #pragma unroll
     for (int i = 0; i < S - 1; ++i)
         if (i < rounds) in.ask(i, first - i, maps);
+    typename In::Word next_rows[PLAIN ? NIN : 1][L];
+    if (PLAIN && rounds > 0) in.fetch(next_rows, first, src, ld);
     C carry = C::splat(0.0f);
     if (p.segments > 1) carry = enter<V, W>(p, part, b, c, 0, p.segments - 1, seg, -1);
     else if (p.a.d_last) carry = mul(get<V>(p.a.d_last + static_cast<long long>(b) * D, c, D), minus);
@@ -308,7 +337,12 @@ __global__ void __launch_bounds__(kBwdWarps * 32, 3)
         C h = next;
         next = state(k - 1);
         C n[L], x[L], e[L], q[L], N = C::splat(0.0f), A = C::splat(0.0f), G = C::splat(0.0f);
-        in.wait(s, k, parity, src, ld);
+        if constexpr (PLAIN) {
+            in.hand_over(next_rows, s);
+            if (it + 1 < rounds) in.fetch(next_rows, k - 1, src, ld);
+        } else {
+            in.wait(s, k, parity);
+        }
         const T *sf = in.mine(s, 0), *sx = in.mine(s, 1), *se = in.mine(s, 2), *sz = in.mine(s, NIN - 1);
 #pragma unroll
         for (int j = 0; j < L; ++j) {
@@ -522,16 +556,15 @@ static int pick_segments(int sms, long long strips, int tiles) {
     return most < tiles ? most : tiles;
 }
 
-template <typename T, int V, bool GATE, bool BWD>
+template <typename T, int V, bool GATE, bool BWD, bool PLAIN>
 static const void* kernel() {
-    if constexpr (BWD) return reinterpret_cast<const void*>(gated_scan_bwd_kernel<T, V, GATE>);
-    else return reinterpret_cast<const void*>(gated_scan_fwd_kernel<T, V, GATE>);
+    if constexpr (BWD) return reinterpret_cast<const void*>(gated_scan_bwd_kernel<T, V, GATE, PLAIN>);
+    else return reinterpret_cast<const void*>(gated_scan_fwd_kernel<T, V, GATE, PLAIN>);
 }
 
 template <typename T, int V, bool GATE, bool BWD>
 static int launch_tiled(Ctx* c, const mamba_b200_gated_scan_args& a, cudaStream_t st) {
     using Lay = Layout<T, V, (GATE ? 3 : 2) + (BWD ? 1 : 0), BWD>;
-    const void* fn = kernel<T, V, GATE, BWD>();
     Params p{a, c->d_status};
     const long long strips = static_cast<long long>(a.B) * ((a.D + Lay::CH - 1) / Lay::CH);
     if (strips > 2147483647ll) return fail(c, MAMBA_B200_ERR_SHAPE, "gated_scan: too many channels");
@@ -546,7 +579,11 @@ static int launch_tiled(Ctx* c, const mamba_b200_gated_scan_args& a, cudaStream_
     p.sums = static_cast<float*>(a.workspace);
     CUtensorMap mf{}, mx{}, me{}, mz{}, o0{}, o1{}, o2{};
     auto map = [&](CUtensorMap* m, const void* base, long long ld) { return make_tmap_3d(c, m, a.dtype, base, ld, a.D, a.T, a.B, Lay::CH, kTile); };
-    p.tma_in = map(&mf, a.f, a.ld_f) && map(&mx, a.x, a.ld_x) && (!BWD || map(&me, a.dy, a.ld_dy)) && (!GATE || map(&mz, a.z, a.ld_z));
+    const bool tma_in = map(&mf, a.f, a.ld_f) && map(&mx, a.x, a.ld_x) && (!BWD || map(&me, a.dy, a.ld_dy)) && (!GATE || map(&mz, a.z, a.ld_z));
+    const void* fn = kernel<T, V, GATE, BWD, true>();
+    if constexpr (V * sizeof(T) == 4) {  // (rows that start on odd elements of 16 bits are none that TMA takes)
+        if (tma_in) fn = kernel<T, V, GATE, BWD, false>();
+    }
     p.tma_out = BWD ? map(&o0, a.d_f, a.ld_df) && map(&o1, a.d_x, a.ld_dx) && (!GATE || map(&o2, a.d_z, a.ld_dz)) : map(&o0, a.y, a.ld_y);
     void* fwd_args[] = {&mf, &mx, &mz, &o0, &p};
     void* bwd_args[] = {&mf, &mx, &me, &mz, &o0, &o1, &o2, &p};
@@ -573,18 +610,19 @@ static int launch_tiled(Ctx* c, const mamba_b200_gated_scan_args& a, cudaStream_
 template <typename T, int V, bool GATE, bool BWD>
 static int configure(Ctx* c) {
     using Lay = Layout<T, V, (GATE ? 3 : 2) + (BWD ? 1 : 0), BWD>;
-    const void* fn = kernel<T, V, GATE, BWD>();
-    MB200_CUDA_CHECK(c, cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, Lay::kBytes));
+    MB200_CUDA_CHECK(c, cudaFuncSetAttribute(kernel<T, V, GATE, BWD, true>(), cudaFuncAttributeMaxDynamicSharedMemorySize, Lay::kBytes));
+    if constexpr (V * sizeof(T) == 4)
+        MB200_CUDA_CHECK(c, cudaFuncSetAttribute(kernel<T, V, GATE, BWD, false>(), cudaFuncAttributeMaxDynamicSharedMemorySize, Lay::kBytes));
     return MAMBA_B200_OK;
 }
 
-// A lane has two channels in 16 bits and one in f32: rows of 128 bytes.  Pairs are fetched as one word by the sums' kernel, so
-// rows that start on odd elements have one channel a lane.
+// A lane has two channels in 16 bits and one in f32: rows of 128 bytes.  Pairs are fetched as one word where TMA does not bring them,
+// so with rows that start on odd elements a lane has one channel.
 template <bool GATE, bool BWD>
 static int launch_typed(Ctx* c, const mamba_b200_gated_scan_args& a, cudaStream_t st) {
     if (a.dtype == MAMBA_B200_F32) return launch_tiled<float, 1, GATE, BWD>(c, a, st);
     auto words = [](const void* q, long long ld) { return reinterpret_cast<uintptr_t>(q) % 4 == 0 && ld % 2 == 0; };
-    const bool two = words(a.f, a.ld_f) && (BWD ? words(a.dy, a.ld_dy) : words(a.x, a.ld_x)) && (!(GATE && BWD) || words(a.z, a.ld_z));
+    const bool two = words(a.f, a.ld_f) && words(a.x, a.ld_x) && (!BWD || words(a.dy, a.ld_dy)) && (!GATE || words(a.z, a.ld_z));
     if (a.dtype == MAMBA_B200_F16) return two ? launch_tiled<__half, 2, GATE, BWD>(c, a, st) : launch_tiled<__half, 1, GATE, BWD>(c, a, st);
     return two ? launch_tiled<__nv_bfloat16, 2, GATE, BWD>(c, a, st) : launch_tiled<__nv_bfloat16, 1, GATE, BWD>(c, a, st);
 }
