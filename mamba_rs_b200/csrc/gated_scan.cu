@@ -144,14 +144,14 @@ struct Tiles {
     }
     // Writes input i's place in stage s to a tensor, row by row, where TMA cannot.
     __device__ __forceinline__ void plain_out(int s, int i, int k, void* dst, long long ld) const {
-        const T* from = at(s, i) + warp * L * Lay::CH;
-        const int t0 = k * kTile + warp * L;
-        for (int j = 0; j < L && t0 + j < p.a.T; ++j)
+        const T* from = mine(s, i);
+        const int t0 = k * kTile + warp * L, c = c0 + lane * V, n = p.a.T - t0;
+        T* to = static_cast<T*>(dst) + (static_cast<long long>(b) * p.a.T + t0) * ld + c;
 #pragma unroll
-            for (int e = 0; e < V; ++e) {
-                const int c = e * 32 + lane;
-                if (c0 + c < p.a.D) static_cast<T*>(dst)[(static_cast<long long>(b) * p.a.T + t0 + j) * ld + c0 + c] = from[j * Lay::CH + c];
-            }
+        for (int j = 0; j < L; ++j)
+#pragma unroll
+            for (int e = 0; e < V; ++e)
+                if (j < n && c + e < p.a.D) to[j * ld + e] = from[j * Lay::CH + e];
     }
 };
 
@@ -192,7 +192,7 @@ __device__ __forceinline__ Ch<V> enter(const Params& p, float* part, int b, int 
 }
 
 template <typename T, int V, bool GATE, bool PLAIN>
-__global__ void __launch_bounds__(kFwdWarps * 32, PLAIN ? 2 : kFwdCtas)
+__global__ void __launch_bounds__(kFwdWarps * 32, kFwdCtas)
     gated_scan_fwd_kernel(const __grid_constant__ CUtensorMap mf, const __grid_constant__ CUtensorMap mx,
                           const __grid_constant__ CUtensorMap mz, const __grid_constant__ CUtensorMap my, const __grid_constant__ Params p) {
     constexpr int NIN = GATE ? 3 : 2;
@@ -271,10 +271,7 @@ __global__ void __launch_bounds__(kFwdWarps * 32, PLAIN ? 2 : kFwdCtas)
         }
         carry = h;
         fence_proxy_async();
-        if (!p.tma_out) {
-            __syncwarp();
-            in.plain_out(s, 1, k, p.a.y, p.a.ld_y);
-        }
+        if (!p.tma_out) in.plain_out(s, 1, k, p.a.y, p.a.ld_y);
         __syncthreads();
         // the stage of the tile before: what was written from it has long been read
         if (it + S - 1 < rounds) in.ask(s == 0 ? S - 1 : s - 1, k + S - 1, maps);
@@ -292,7 +289,7 @@ __global__ void __launch_bounds__(kFwdWarps * 32, PLAIN ? 2 : kFwdCtas)
 // the same two walks; g is joined over the warps (and the cluster) the same way in the other direction: over a span of steps
 // (1 - u) g at its first step = g_behind - U g_behind + G, with the forward's U.  g runs with its sign turned, like the gates.
 template <typename T, int V, bool GATE, bool PLAIN>
-__global__ void __launch_bounds__(kBwdWarps * 32, PLAIN ? 2 : 3)
+__global__ void __launch_bounds__(kBwdWarps * 32, 3)
     gated_scan_bwd_kernel(const __grid_constant__ CUtensorMap mf, const __grid_constant__ CUtensorMap mx, const __grid_constant__ CUtensorMap me,
                           const __grid_constant__ CUtensorMap mz, const __grid_constant__ CUtensorMap mdf, const __grid_constant__ CUtensorMap mdx,
                           const __grid_constant__ CUtensorMap mdz, const __grid_constant__ Params p) {
@@ -396,7 +393,6 @@ __global__ void __launch_bounds__(kBwdWarps * 32, PLAIN ? 2 : 3)
         }
         fence_proxy_async();
         if (!p.tma_out) {
-            __syncwarp();
             in.plain_out(s, 0, k, p.a.d_f, p.a.ld_df);
             in.plain_out(s, 1, k, p.a.d_x, p.a.ld_dx);
             if constexpr (GATE) in.plain_out(s, 3, k, p.a.d_z, p.a.ld_dz);
@@ -562,7 +558,7 @@ static const void* kernel() {
     else return reinterpret_cast<const void*>(gated_scan_fwd_kernel<T, V, GATE, PLAIN>);
 }
 
-template <typename T, int V, bool GATE, bool BWD>
+template <typename T, int V, bool GATE, bool BWD, bool PLAIN>
 static int launch_tiled(Ctx* c, const mamba_b200_gated_scan_args& a, cudaStream_t st) {
     using Lay = Layout<T, V, (GATE ? 3 : 2) + (BWD ? 1 : 0), BWD>;
     Params p{a, c->d_status};
@@ -579,11 +575,9 @@ static int launch_tiled(Ctx* c, const mamba_b200_gated_scan_args& a, cudaStream_
     p.sums = static_cast<float*>(a.workspace);
     CUtensorMap mf{}, mx{}, me{}, mz{}, o0{}, o1{}, o2{};
     auto map = [&](CUtensorMap* m, const void* base, long long ld) { return make_tmap_3d(c, m, a.dtype, base, ld, a.D, a.T, a.B, Lay::CH, kTile); };
-    const bool tma_in = map(&mf, a.f, a.ld_f) && map(&mx, a.x, a.ld_x) && (!BWD || map(&me, a.dy, a.ld_dy)) && (!GATE || map(&mz, a.z, a.ld_z));
-    const void* fn = kernel<T, V, GATE, BWD, true>();
-    if constexpr (V * sizeof(T) == 4) {  // (rows that start on odd elements of 16 bits are none that TMA takes)
-        if (tma_in) fn = kernel<T, V, GATE, BWD, false>();
-    }
+    const void* fn = kernel<T, V, GATE, BWD, PLAIN>();
+    if (!PLAIN && !(map(&mf, a.f, a.ld_f) && map(&mx, a.x, a.ld_x) && (!BWD || map(&me, a.dy, a.ld_dy)) && (!GATE || map(&mz, a.z, a.ld_z))))
+        return fail(c, MAMBA_B200_ERR_CUDA, "gated_scan: a tensor map was refused");
     p.tma_out = BWD ? map(&o0, a.d_f, a.ld_df) && map(&o1, a.d_x, a.ld_dx) && (!GATE || map(&o2, a.d_z, a.ld_dz)) : map(&o0, a.y, a.ld_y);
     void* fwd_args[] = {&mf, &mx, &mz, &o0, &p};
     void* bwd_args[] = {&mf, &mx, &me, &mz, &o0, &o1, &o2, &p};
@@ -607,36 +601,37 @@ static int launch_tiled(Ctx* c, const mamba_b200_gated_scan_args& a, cudaStream_
     return MAMBA_B200_OK;
 }
 
-template <typename T, int V, bool GATE, bool BWD>
+template <typename T, int V, bool GATE, bool BWD, bool PLAIN>
 static int configure(Ctx* c) {
     using Lay = Layout<T, V, (GATE ? 3 : 2) + (BWD ? 1 : 0), BWD>;
-    MB200_CUDA_CHECK(c, cudaFuncSetAttribute(kernel<T, V, GATE, BWD, true>(), cudaFuncAttributeMaxDynamicSharedMemorySize, Lay::kBytes));
-    if constexpr (V * sizeof(T) == 4)
-        MB200_CUDA_CHECK(c, cudaFuncSetAttribute(kernel<T, V, GATE, BWD, false>(), cudaFuncAttributeMaxDynamicSharedMemorySize, Lay::kBytes));
+    MB200_CUDA_CHECK(c, cudaFuncSetAttribute(kernel<T, V, GATE, BWD, PLAIN>(), cudaFuncAttributeMaxDynamicSharedMemorySize, Lay::kBytes));
     return MAMBA_B200_OK;
 }
 
-// A lane has two channels in 16 bits and one in f32: rows of 128 bytes.  Pairs are fetched as one word where TMA does not bring them,
-// so with rows that start on odd elements a lane has one channel.
+// A lane has two channels in 16 bits and one in f32: rows of 128 bytes, brought by TMA.  Rows that it cannot describe (odd channel
+// counts or starts) take one channel a lane: two of their 2-byte columns a lane were slower, 140 us for 16 x 2048 x 770 against 110 (770
+// and 769 channels), the gradient 414 against 2 x 112.
 template <bool GATE, bool BWD>
 static int launch_typed(Ctx* c, const mamba_b200_gated_scan_args& a, cudaStream_t st) {
-    if (a.dtype == MAMBA_B200_F32) return launch_tiled<float, 1, GATE, BWD>(c, a, st);
-    auto words = [](const void* q, long long ld) { return reinterpret_cast<uintptr_t>(q) % 4 == 0 && ld % 2 == 0; };
-    const bool two = words(a.f, a.ld_f) && words(a.x, a.ld_x) && (!BWD || words(a.dy, a.ld_dy)) && (!GATE || words(a.z, a.ld_z));
-    if (a.dtype == MAMBA_B200_F16) return two ? launch_tiled<__half, 2, GATE, BWD>(c, a, st) : launch_tiled<__half, 1, GATE, BWD>(c, a, st);
-    return two ? launch_tiled<__nv_bfloat16, 2, GATE, BWD>(c, a, st) : launch_tiled<__nv_bfloat16, 1, GATE, BWD>(c, a, st);
+    const int cols = a.dtype == MAMBA_B200_F32 ? 32 : 64;
+    auto fits = [&](const void* q, long long ld) { return tmap_3d_fits(c, a.dtype, q, ld, a.D, a.T, cols, kTile); };
+    const bool tma = a.T > 0 && fits(a.f, a.ld_f) && fits(a.x, a.ld_x) && (!BWD || fits(a.dy, a.ld_dy)) && (!GATE || fits(a.z, a.ld_z));
+    if (a.dtype == MAMBA_B200_F32) return tma ? launch_tiled<float, 1, GATE, BWD, false>(c, a, st) : launch_tiled<float, 1, GATE, BWD, true>(c, a, st);
+    if (a.dtype == MAMBA_B200_F16) return tma ? launch_tiled<__half, 2, GATE, BWD, false>(c, a, st) : launch_tiled<__half, 1, GATE, BWD, true>(c, a, st);
+    return tma ? launch_tiled<__nv_bfloat16, 2, GATE, BWD, false>(c, a, st) : launch_tiled<__nv_bfloat16, 1, GATE, BWD, true>(c, a, st);
 }
 
 }  // namespace gs
 
 int gated_scan_configure(Ctx* c) {
     int rc = MAMBA_B200_OK;
-#define MB200_GS(T, V)                                                    \
-    if (!rc) rc = gs::configure<T, V, true, true>(c);                  \
-    if (!rc) rc = gs::configure<T, V, false, true>(c);                 \
-    if (!rc) rc = gs::configure<T, V, true, false>(c);                 \
-    if (!rc) rc = gs::configure<T, V, false, false>(c);
-    MB200_GS(float, 1) MB200_GS(__half, 1) MB200_GS(__half, 2) MB200_GS(__nv_bfloat16, 1) MB200_GS(__nv_bfloat16, 2)
+#define MB200_GS(T, V, PLAIN)                                             \
+    if (!rc) rc = gs::configure<T, V, true, true, PLAIN>(c);              \
+    if (!rc) rc = gs::configure<T, V, false, true, PLAIN>(c);             \
+    if (!rc) rc = gs::configure<T, V, true, false, PLAIN>(c);             \
+    if (!rc) rc = gs::configure<T, V, false, false, PLAIN>(c);
+    MB200_GS(float, 1, false) MB200_GS(float, 1, true) MB200_GS(__half, 2, false) MB200_GS(__half, 1, true)
+    MB200_GS(__nv_bfloat16, 2, false) MB200_GS(__nv_bfloat16, 1, true)
 #undef MB200_GS
     return rc;
 }
