@@ -332,34 +332,74 @@ __global__ void __launch_bounds__(kSortThreads) embedding_sort_kernel(const BwdP
     asm volatile("griddepcontrol.wait;" ::: "memory");  // (what comes next relies on the cleared rows too)
 }
 
-// A warp has M vectors of N columns a lane, 32 N apart: what a row costs beside its loads and additions is shared by more columns
-// (one vector: 56 instructions a row and vector, the kernel was bound by them).
-template <typename T, int N, int M>
-__global__ void __launch_bounds__(kThreads, 3) embedding_sums_kernel(const BwdParams p, int sum_blocks) {
-    constexpr int NF = N == 8 ? 4 : N, U = 8 / M;
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    asm volatile("griddepcontrol.wait;" ::: "memory");
-    // blocks that clear lie evenly between those that add: the ones write, the others read
-    const int clears = gridDim.x - sum_blocks, cleared = static_cast<int>(static_cast<long long>(blockIdx.x) * clears / gridDim.x);
-    if (static_cast<int>((blockIdx.x + 1ll) * clears / gridDim.x) != cleared) {  // 64 rows of the table
-        const int v0 = (cleared * (kThreads / 32) + warp) * 8;
-        const unsigned absent = __ballot_sync(0xffffffffu, lane < 8 && v0 + lane < p.cleared && !p.present[v0 + lane]);
+// What a warp of the sums has: a run of sorted rows and a part of the columns, or rows of the table to clear (kClear of them).  Those
+// that clear lie evenly between those that add: the ones write, the others read.
+constexpr int kClear = 32;
+struct Task {
+    int run, slice;  // run < 0: done
+    int2 own;        // lane l: the run's l-th row and its token
+    int n;
+    unsigned ends;   // last rows of a token in this run
+    bool from_before, goes_on;
+};
+template <int NF>
+__device__ __forceinline__ Task next_task(const BwdParams& p, long long index, long long sums, long long clears) {
+    const int lane = threadIdx.x & 31;
+    Task t;
+    t.run = -1;
+    const long long total = sums + clears, cleared = index * clears / total;
+    if (index >= total) return t;
+    if ((index + 1) * clears / total != cleared) {
+        const int v0 = static_cast<int>(cleared) * kClear;
+        const unsigned absent = __ballot_sync(0xffffffffu, v0 + lane < p.cleared && !p.present[v0 + lane]);
         for (unsigned m = absent; m; m &= m - 1) clear_row<NF>(p.d_table + static_cast<long long>(v0 + __ffs(m) - 1) * p.dim, p.dim);
-        return;
+        return t;
     }
-    const long long task = (static_cast<int>(blockIdx.x) - cleared) * static_cast<long long>(kThreads / 32) + warp;
-    const int run = static_cast<int>(task / p.slices), c = (static_cast<int>(task - static_cast<long long>(run) * p.slices) * M * 32 + lane) * N;
-    if (run >= p.runs) return;
-    const int first = run * p.run;
-    const int2 own = lane < p.run ? p.sorted[first + lane] : make_int2(0, -1);
+    const long long task = index - cleared;
+    const int run = static_cast<int>(task / p.slices), first = run * p.run;
+    t.slice = static_cast<int>(task - static_cast<long long>(run) * p.slices);
+    t.own = lane < p.run ? p.sorted[first + lane] : make_int2(0, -1);
     const int before = first > 0 ? p.sorted[first - 1].y : -1, behind = p.sorted[first + p.run].y;
-    const int n = __popc(__ballot_sync(0xffffffffu, own.y >= 0));
-    if (n == 0) return;
-    const int next = __shfl_down_sync(0xffffffffu, own.y, 1);
-    const unsigned ends = __ballot_sync(0xffffffffu, lane + 1 < n && next != own.y) | 1u << (n - 1);  // last rows of a token in this run
-    bool from_before = before == __shfl_sync(0xffffffffu, own.y, 0);
-    const bool goes_on = behind == __shfl_sync(0xffffffffu, own.y, n - 1);
-    const T* columns = static_cast<const T*>(p.d_out) + c;
+    t.n = __popc(__ballot_sync(0xffffffffu, t.own.y >= 0));
+    if (t.n == 0) return t;
+    const int next = __shfl_down_sync(0xffffffffu, t.own.y, 1);
+    t.ends = __ballot_sync(0xffffffffu, lane + 1 < t.n && next != t.own.y) | 1u << (t.n - 1);
+    t.from_before = before == __shfl_sync(0xffffffffu, t.own.y, 0);
+    t.goes_on = behind == __shfl_sync(0xffffffffu, t.own.y, t.n - 1);
+    t.run = run;
+    return t;
+}
+// Where the sum of the token that ends with row i of the run goes: the token's row, or the run's part of a token that goes on.
+__device__ __forceinline__ float* sum_place(const BwdParams& p, const Task& t, int i, int c, bool& whole) {
+    whole = !t.from_before && !(t.goes_on && i + 1 == t.n);
+    return whole ? p.d_table + static_cast<long long>(__shfl_sync(0xffffffffu, t.own.y, i)) * p.dim + c
+                 : p.part + (2ll * t.run + (t.from_before ? 0 : 1)) * p.dim + c;
+}
+
+// Rows whose parts are 16-byte aligned come to shared memory by bulk copies, a lane asking for one row's part: a run's 16 or 32 KB are
+// in flight at once.  Parts of 512 bytes in f32, 1 KB in 16 bits: 32768 x 768 f32 73 us (with 1 KB 75), 16384 x 2560 bf16 130 (with 512
+// bytes 135).  Some 30 us of the first are this kernel, whose 155 MB (rows read, rows of tokens written, what is left to clear) are 24.
+template <typename T> constexpr int part_bytes() { return sizeof(T) == 2 ? 1024 : 512; }
+template <typename T>
+__global__ void __launch_bounds__(32) embedding_sums_kernel(const BwdParams p, long long sums, long long clears, int* status) {
+    constexpr int N = 16 / sizeof(T), NF = 4, kPart = part_bytes<T>(), M = kPart / 512;
+    extern __shared__ unsigned char raw[];
+    unsigned char* sm = raw + (128 - (smem_u32(raw) & 127)) % 128;
+    uint64_t* bar = reinterpret_cast<uint64_t*>(sm + p.run * kPart);
+    const int lane = threadIdx.x;
+    if (lane == 0) {
+        mbar_init(bar, 1);
+        fence_barrier_init();
+    }
+    __syncwarp();
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    Task t = next_task<NF>(p, blockIdx.x, sums, clears);
+    if (t.run < 0) return;
+    const int c0 = t.slice * (kPart / static_cast<int>(sizeof(T))), c = c0 + lane * N;
+    const uint32_t bytes = static_cast<uint32_t>(min(kPart, (p.dim - c0) * static_cast<int>(sizeof(T))));
+    if (lane == 0) mbar_expect_tx(bar, bytes * t.n);
+    __syncwarp();
+    if (lane < t.n) bulk_load(sm + lane * kPart, static_cast<const T*>(p.d_out) + t.own.x * p.ld_dout + c0, bytes, bar);
     bool in[M];
     float acc[M][N];
 #pragma unroll
@@ -368,51 +408,79 @@ __global__ void __launch_bounds__(kThreads, 3) embedding_sums_kernel(const BwdPa
 #pragma unroll
         for (int k = 0; k < N; ++k) acc[m][k] = 0.0f;
     }
-    for (int i0 = 0; i0 < n; i0 += U) {
-        Vec<T, N> q[U][M];
+    if (!mbar_wait(bar, 0, status)) return;
+#pragma unroll 4
+    for (int i = 0; i < t.n; ++i) {
+#pragma unroll
+        for (int m = 0; m < M; ++m) {
+            float f[N];
+            reinterpret_cast<const Vec<T, N>*>(sm + i * kPart + m * 512 + lane * 16)->widen(f);
+#pragma unroll
+            for (int k = 0; k < N; ++k) acc[m][k] += f[k];
+        }
+        if (!(t.ends >> i & 1)) continue;
+        bool whole;
+        float* to = sum_place(p, t, i, c, whole);
+#pragma unroll
+        for (int m = 0; m < M; ++m) {
+            if (in[m])
+#pragma unroll
+                for (int k = 0; k < N; k += NF)
+                    write_sum<NF>(to + m * 32 * N + k, acc[m] + k, whole ? p.scale : 1.0f, whole && p.accumulate);
+#pragma unroll
+            for (int k = 0; k < N; ++k) acc[m][k] = 0.0f;
+        }
+        t.from_before = false;
+    }
+}
+
+// Other rows: M columns a lane, 32 apart.  (Two rows' loads at once 98 us for 32768 x 769, one 84: the warps of an SM suffice.)
+template <typename T>
+__global__ void __launch_bounds__(kThreads) embedding_sums_plain_kernel(const BwdParams p, long long sums, long long clears) {
+    constexpr int M = 4, U = 1;
+    const int lane = threadIdx.x & 31;
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    Task t = next_task<1>(p, blockIdx.x * static_cast<long long>(kThreads / 32) + threadIdx.x / 32, sums, clears);
+    if (t.run < 0) return;
+    const int c = t.slice * 32 * M + lane;
+    const T* columns = static_cast<const T*>(p.d_out) + c;
+    float acc[M];
+#pragma unroll
+    for (int m = 0; m < M; ++m) acc[m] = 0.0f;
+    for (int i0 = 0; i0 < t.n; i0 += U) {
+        T q[U][M];
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-            const T* row = columns + __shfl_sync(0xffffffffu, own.x, (i0 + u) & 31) * p.ld_dout;
-            if (i0 + u < n)
+            const T* row = columns + __shfl_sync(0xffffffffu, t.own.x, (i0 + u) & 31) * p.ld_dout;
 #pragma unroll
-                for (int m = 0; m < M; ++m)
-                    if (in[m]) q[u][m] = *reinterpret_cast<const Vec<T, N>*>(row + m * 32 * N);
+            for (int m = 0; m < M; ++m)
+                if (i0 + u < t.n && c + 32 * m < p.dim) q[u][m] = row[32 * m];
         }
 #pragma unroll
         for (int u = 0; u < U; ++u) {
             const int i = i0 + u;
-            if (i >= n) break;
+            if (i >= t.n) break;
+#pragma unroll
+            for (int m = 0; m < M; ++m) acc[m] += to_f(q[u][m]);
+            if (!(t.ends >> i & 1)) continue;
+            bool whole;
+            float* to = sum_place(p, t, i, c, whole);
 #pragma unroll
             for (int m = 0; m < M; ++m) {
-                float f[N];
-                q[u][m].widen(f);
-#pragma unroll
-                for (int k = 0; k < N; ++k) acc[m][k] += f[k];
+                if (c + 32 * m < p.dim) write_sum<1>(to + 32 * m, acc + m, whole ? p.scale : 1.0f, whole && p.accumulate);
+                acc[m] = 0.0f;
             }
-            if (!(ends >> i & 1)) continue;
-            // the run's part of a token that goes on, or the token's row
-            const bool whole = !from_before && !(goes_on && i + 1 == n);
-            float* to = whole ? p.d_table + static_cast<long long>(__shfl_sync(0xffffffffu, own.y, i)) * p.dim + c
-                              : p.part + (2ll * run + (from_before ? 0 : 1)) * p.dim + c;
-#pragma unroll
-            for (int m = 0; m < M; ++m) {
-                if (in[m])
-#pragma unroll
-                    for (int k = 0; k < N; k += NF)
-                        write_sum<NF>(to + m * 32 * N + k, acc[m] + k, whole ? p.scale : 1.0f, whole && p.accumulate);
-#pragma unroll
-                for (int k = 0; k < N; ++k) acc[m][k] = 0.0f;
-            }
-            from_before = false;
+            t.from_before = false;
         }
     }
 }
 
 // Tokens that go on beyond a run.  A warp looks after the one that begins in its run and adds its runs' sums, if they are few; the
 // CTA does so for one that reaches far.
+constexpr int kJoinThreads = 256;
 template <int N>
-__global__ void __launch_bounds__(kThreads) embedding_join_kernel(const BwdParams p) {
-    constexpr int WARPS = kThreads / 32;
+__global__ void __launch_bounds__(kJoinThreads) embedding_join_kernel(const BwdParams p) {
+    constexpr int WARPS = kJoinThreads / 32;
     __shared__ float room[WARPS][32 * N];
     __shared__ int far[WARPS];
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, c = (blockIdx.y * 32 + lane) * N;
@@ -453,10 +521,10 @@ __global__ void __launch_bounds__(kThreads) embedding_join_kernel(const BwdParam
         if (!far[w]) continue;
         const int from = blockIdx.x * WARPS + w, its = p.sorted[from * p.run + p.run - 1].y;
         int n = 0;  // runs behind this one that it reaches
-        for (int i0 = from + 1;; i0 += kThreads) {
+        for (int i0 = from + 1;; i0 += kJoinThreads) {
             const int here = __syncthreads_count(i0 + tid < runs && p.sorted[(i0 + tid) * p.run].y == its);
             n += here;
-            if (here < kThreads) break;
+            if (here < kJoinThreads) break;
         }
 #pragma unroll
         for (int k = 0; k < N; ++k) acc[k] = 0.0f;
@@ -471,7 +539,7 @@ constexpr long long kClearBeside = 128 << 20;
 // Rows of a run: fewer where that gives more warps something to do.
 static int run_of(long long rows, int dim) {
     int run = kMaxRun;
-    while (run > 8 && rows / run * ((dim + 127) / 128) < 148 * 32) run /= 2;
+    while (run > 8 && rows / run * ((dim + 255) / 256) < 148 * 12) run /= 2;
     return run;
 }
 struct Room {
@@ -491,11 +559,12 @@ static Room room_of(long long rows, int dim, int vocab) {
 
 // With `early` the kernel may start before the one ahead of it in the stream has ended, and waits for it itself.
 template <typename Kernel, typename... Args>
-static cudaError_t launch_early(Kernel fn, dim3 grid, int threads, cudaStream_t st, int cluster, bool early, Args... args) {
+static cudaError_t launch_early(Kernel fn, dim3 grid, int threads, size_t smem, cudaStream_t st, int cluster, bool early, Args... args) {
     cudaLaunchConfig_t cfg;
     memset(&cfg, 0, sizeof(cfg));
     cfg.gridDim = grid;
     cfg.blockDim = dim3(threads);
+    cfg.dynamicSmemBytes = smem;
     cfg.stream = st;
     cudaLaunchAttribute at[2];
     memset(at, 0, sizeof(at));
@@ -513,7 +582,7 @@ static cudaError_t launch_early(Kernel fn, dim3 grid, int threads, cudaStream_t 
     return cudaLaunchKernelEx(&cfg, fn, args...);
 }
 
-template <typename T, int N, int M>
+template <typename T, int N>
 static int launch_bwd(Ctx* c, BwdParams& p, cudaStream_t st) {
     if (p.rows <= kFewRows) {
         p.slices = (p.dim + 32 * N - 1) / (32 * N);
@@ -522,37 +591,36 @@ static int launch_bwd(Ctx* c, BwdParams& p, cudaStream_t st) {
         MB200_CUDA_CHECK(c, cudaGetLastError());
         return MAMBA_B200_OK;
     }
-    p.slices = (p.dim + 32 * N * M - 1) / (32 * N * M);
+    constexpr int NF = N == 1 ? 1 : 4, kColumns = N == 1 ? 128 : part_bytes<T>() / static_cast<int>(sizeof(T));
+    p.slices = (p.dim + kColumns - 1) / kColumns;
     p.run = run_of(p.rows, p.dim);
     p.runs = (p.rows + p.run - 1) / p.run;
     for (p.passes = 1; p.passes < 4 && (p.vocab - 1) >> (8 * p.passes); ++p.passes) {}
-    // what HBM can clear while the sort runs (some 8 us), of the last tokens: the rare ones where tokens are in order of frequency
+    // what HBM can clear while the sort runs (some 20 us), of the last tokens: the rare ones where tokens are in order of frequency
     const long long beside = p.accumulate ? 0 : kClearBeside / (4ll * p.dim);
     p.cleared = p.vocab - static_cast<int>(beside < p.vocab ? beside : p.vocab);
-    const long long sums = (static_cast<long long>(p.runs) * p.slices + kThreads / 32 - 1) / (kThreads / 32), clears = p.accumulate ? 0 : (p.cleared + 63) / 64;
+    const long long sums = static_cast<long long>(p.runs) * p.slices, clears = p.accumulate ? 0 : (p.cleared + kClear - 1) / kClear;
     if (sums + clears > 2147483647ll) return fail(c, MAMBA_B200_ERR_SHAPE, "embedding_bwd: too many rows");
-    constexpr int NJ = N == 8 ? 4 : N;
     const bool beside_sort = p.cleared < p.vocab;
     if (beside_sort) {
-        embedding_clear_kernel<NJ><<<2 * c->sm_count, kThreads, 0, st>>>(p);
+        embedding_clear_kernel<NF><<<2 * c->sm_count, kThreads, 0, st>>>(p);
         MB200_CUDA_CHECK(c, cudaGetLastError());
     }
-    MB200_CUDA_CHECK(c, launch_early(embedding_sort_kernel, dim3(kSorters), kSortThreads, st, kSorters, beside_sort, p));
-    MB200_CUDA_CHECK(c, launch_early(embedding_sums_kernel<T, N, M>, dim3(static_cast<unsigned>(sums + clears)), kThreads, st, 1, true, p, static_cast<int>(sums)));
-    MB200_CUDA_CHECK(c, launch_early(embedding_join_kernel<NJ>, dim3((p.runs + kThreads / 32 - 1) / (kThreads / 32), (p.dim + 32 * NJ - 1) / (32 * NJ)),
-                                     kThreads, st, 1, true, p));
+    MB200_CUDA_CHECK(c, launch_early(embedding_sort_kernel, dim3(kSorters), kSortThreads, 0, st, kSorters, beside_sort, p));
+    const unsigned tasks = static_cast<unsigned>(sums + clears);
+    if constexpr (N == 1)
+        MB200_CUDA_CHECK(c, launch_early(embedding_sums_plain_kernel<T>, dim3((tasks + kThreads / 32 - 1) / (kThreads / 32)), kThreads, 0, st, 1, true, p, sums, clears));
+    else
+        MB200_CUDA_CHECK(c, launch_early(embedding_sums_kernel<T>, dim3(tasks), 32, p.run * part_bytes<T>() + 16 + 128, st, 1, true, p, sums, clears, c->d_status));
+    MB200_CUDA_CHECK(c, launch_early(embedding_join_kernel<NF>, dim3((p.runs + kJoinThreads / 32 - 1) / (kJoinThreads / 32), (p.dim + 32 * NF - 1) / (32 * NF)),
+                                     kJoinThreads, 0, st, 1, true, p));
     return MAMBA_B200_OK;
 }
 template <typename T>
 static int launch_bwd(Ctx* c, BwdParams& p, cudaStream_t st) {
-    auto fits = [&](int n) {
-        return p.dim % n == 0 && p.ld_dout % n == 0 && reinterpret_cast<uintptr_t>(p.d_out) % (n * sizeof(T)) == 0 &&
-               reinterpret_cast<uintptr_t>(p.d_table) % 16 == 0;
-    };
-    if constexpr (sizeof(T) == 2) {
-        if (fits(8)) return launch_bwd<T, 8, 1>(c, p, st);
-    }
-    return fits(4) ? launch_bwd<T, 4, 2>(c, p, st) : launch_bwd<T, 1, 4>(c, p, st);
+    constexpr int N = 16 / sizeof(T);
+    const bool wide = p.dim % N == 0 && p.ld_dout % N == 0 && reinterpret_cast<uintptr_t>(p.d_out) % 16 == 0 && reinterpret_cast<uintptr_t>(p.d_table) % 16 == 0;
+    return wide ? launch_bwd<T, N>(c, p, st) : launch_bwd<T, 1>(c, p, st);
 }
 
 }  // namespace emb
