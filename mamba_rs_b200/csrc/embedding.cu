@@ -379,10 +379,10 @@ __device__ __forceinline__ float* sum_place(const BwdParams& p, const Task& t, i
 // Rows whose parts are 16-byte aligned come to shared memory by bulk copies, a lane asking for one row's part: a run's 16 or 32 KB are
 // in flight at once.  Parts of 512 bytes in f32, 1 KB in 16 bits: 32768 x 768 f32 73 us (with 1 KB 75), 16384 x 2560 bf16 130 (with 512
 // bytes 135).  Some 30 us of the first are this kernel, whose 155 MB (rows read, rows of tokens written, what is left to clear) are 24.
-template <typename T> constexpr int part_bytes() { return sizeof(T) == 2 ? 1024 : 512; }
+template <typename T> constexpr int kPartBytes = sizeof(T) == 2 ? 1024 : 512;
 template <typename T>
 __global__ void __launch_bounds__(32) embedding_sums_kernel(const BwdParams p, long long sums, long long clears, int* status) {
-    constexpr int N = 16 / sizeof(T), NF = 4, kPart = part_bytes<T>(), M = kPart / 512;
+    constexpr int N = 16 / sizeof(T), NF = 4, kPart = kPartBytes<T>, M = kPart / 512;
     extern __shared__ unsigned char raw[];
     unsigned char* sm = raw + (128 - (smem_u32(raw) & 127)) % 128;
     uint64_t* bar = reinterpret_cast<uint64_t*>(sm + p.run * kPart);
@@ -591,7 +591,7 @@ static int launch_bwd(Ctx* c, BwdParams& p, cudaStream_t st) {
         MB200_CUDA_CHECK(c, cudaGetLastError());
         return MAMBA_B200_OK;
     }
-    constexpr int NF = N == 1 ? 1 : 4, kColumns = N == 1 ? 128 : part_bytes<T>() / static_cast<int>(sizeof(T));
+    constexpr int NF = N == 1 ? 1 : 4, kColumns = N == 1 ? 128 : kPartBytes<T> / static_cast<int>(sizeof(T));
     p.slices = (p.dim + kColumns - 1) / kColumns;
     p.run = run_of(p.rows, p.dim);
     p.runs = (p.rows + p.run - 1) / p.run;
@@ -611,7 +611,7 @@ static int launch_bwd(Ctx* c, BwdParams& p, cudaStream_t st) {
     if constexpr (N == 1)
         MB200_CUDA_CHECK(c, launch_early(embedding_sums_plain_kernel<T>, dim3((tasks + kThreads / 32 - 1) / (kThreads / 32)), kThreads, 0, st, 1, true, p, sums, clears));
     else
-        MB200_CUDA_CHECK(c, launch_early(embedding_sums_kernel<T>, dim3(tasks), 32, p.run * part_bytes<T>() + 16 + 128, st, 1, true, p, sums, clears, c->d_status));
+        MB200_CUDA_CHECK(c, launch_early(embedding_sums_kernel<T>, dim3(tasks), 32, p.run * kPartBytes<T> + 16 + 128, st, 1, true, p, sums, clears, c->d_status));
     MB200_CUDA_CHECK(c, launch_early(embedding_join_kernel<NF>, dim3((p.runs + kJoinThreads / 32 - 1) / (kJoinThreads / 32), (p.dim + 32 * NF - 1) / (32 * NF)),
                                      kJoinThreads, 0, st, 1, true, p));
     return MAMBA_B200_OK;
