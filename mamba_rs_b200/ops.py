@@ -674,18 +674,20 @@ def token_logprobs(logits, targets=None, *, top=0, temperature=1.0, handle=None)
     _same_device(dev, (targets, "targets"))
     if not 0 <= top <= min(32, V):
         raise ValueError(f"{top} alternatives of {V} tokens (at most 32)")
-    res = torch.empty((3 if targets is None else 4, rows), dtype=torch.float32, device=dev)
-    base = res.data_ptr()
-    out = dict(lse=res[:2], entropy=res[2])
+    # (a tensor of its own costs the host half of what a slice does)
+    lse = torch.empty((2, rows), dtype=torch.float32, device=dev)
+    entropy = lse.new_empty(rows)
+    out = dict(lse=lse, entropy=entropy)
+    tp = lp = ip = vp = None
     if targets is not None:
-        out["logprob"] = res[3]
-    ip = vp = None
+        out["logprob"] = logprob = lse.new_empty(rows)
+        tp, lp = targets.data_ptr(), logprob.data_ptr()
     if top:
-        ids, val = torch.empty((rows, top), dtype=torch.int32, device=dev), torch.empty((rows, top), dtype=torch.float32, device=dev)
+        out["top_ids"] = ids = torch.empty((rows, top), dtype=torch.int32, device=dev) if targets is None else targets.new_empty((rows, top))
+        out["top_logprobs"] = val = lse.new_empty((rows, top))
         ip, vp = ids.data_ptr(), val.data_ptr()
-        out["top_ids"], out["top_logprobs"] = ids, val
-    _launch(ffi.lib().mamba_b200_token_logprobs, dev, handle, dtype_code(logits.dtype), logits.data_ptr(), _row(logits, V), _ptr(targets),
-            temperature, base, base + 8 * rows, None if targets is None else base + 12 * rows, top, ip, vp, rows, V)
+    _launch(ffi.lib().mamba_b200_token_logprobs, dev, handle, dtype_code(logits.dtype), logits.data_ptr(), _row(logits, V), tp,
+            temperature, lse.data_ptr(), entropy.data_ptr(), lp, top, ip, vp, rows, V)
     return out
 
 
@@ -763,7 +765,7 @@ def gated_scan_fwd(x, f, z=None, *, h0=None, h_last=None, y=None, chunk_states=N
     gated_scan_workspace_bytes(B,T,D) bytes (made here if None).  Returns y."""
     _require_cuda(x, f, z, h0, h_last, y, chunk_states, workspace)
     if y is None:
-        y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+        y = x.new_empty(x.shape)
     B, T, D = x.shape
     dev = x.device
     a = ffi.GatedScanArgs(dtype_code(x.dtype), B, T, D, x.data_ptr(), _gated_rows(x, "x", x), f.data_ptr(), _gated_rows(f, "f", x),
@@ -779,9 +781,9 @@ def gated_scan_fwd(x, f, z=None, *, h0=None, h_last=None, y=None, chunk_states=N
 def gated_scan_step(x, f, h0, z=None, *, h_last=None, y=None, handle=None):
     """One token per sequence: x, f, z, y [B,D]; the state h0 [B,D] f32 is updated in place, or h_last receives it."""
     _require_cuda(x, f, z, h0, h_last, y)
-    if y is None:
-        y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
     B, D = shape = x.shape
+    if y is None:
+        y = x.new_empty(shape)
 
     def row(t, name):
         if t.dtype != x.dtype or t.shape != shape or t.device != x.device:
