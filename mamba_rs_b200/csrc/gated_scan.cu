@@ -65,7 +65,7 @@ struct Params {
     mamba_b200_gated_scan_args a;
     int* status;
     float* sums;  // [B, segments, 2, D]: what each segment does to the state (or gradient) that enters it
-    int tiles, segments, per_segment, tma_out;
+    int tiles, segments, per_segment, tma_out, stages;
 };
 
 // ---------------------------------------------------------------------------------------------------
@@ -77,15 +77,22 @@ struct Params {
 // ---------------------------------------------------------------------------------------------------
 constexpr int kFwdWarps = 4, kBwdWarps = 4;
 constexpr int kFwdCtas = 3, kFwdStages = 3;
+// The gradient writes over its inputs, so a stage is asked for again only when its results have been read: with two CTAs or one on an
+// SM two stages leave the memory idle meanwhile, and three are used.  us with two and three: 135 strips x 49 tiles 116 and 82, 144 x 64
+// 139 and 106, 168 x 64 158 and 139, 192 x 32 84 and 73; but 288 x 32 98 and 105, and three CTAs with two stages are 384 x 32 120, two
+// with three 142.  (The forward gains 2 % from a fourth.)
+constexpr int kFewStages = 3;
+static bool few_ctas(int sms, long long ctas) { return 2 * ctas <= 3ll * sms; }
 
 template <typename T, int V, int NIN, bool BWD>
 struct Layout {
     static constexpr int CH = 32 * V, kStages = BWD ? 2 : kFwdStages, kWarps = BWD ? kBwdWarps : kFwdWarps, L = kTile / kWarps;
     static constexpr uint32_t kIn = kTile * CH * sizeof(T);  // one input's tile
-    // stages of inputs | backward: the warps' three sums (the forward's two lie in the place of f, which is done with) | barriers
-    static constexpr uint32_t oPart = kStages * NIN * kIn, oBar = oPart + (BWD ? 3 * kWarps * CH * sizeof(float) : 0);
-    static constexpr uint32_t kBytes = oBar + 8 * kStages + 128;
-    static_assert((BWD ? 3 : kFwdCtas) * (kBytes + 1024) <= 228 * 1024, "CTAs on an SM");
+    // backward: the warps' three sums (the forward's two lie in the place of f, which is done with) | barriers | stages of inputs
+    static constexpr uint32_t oBar = BWD ? 3 * kWarps * CH * sizeof(float) : 0, oIn = oBar + 128;
+    static constexpr uint32_t bytes(int stages) { return oIn + stages * NIN * kIn + 128; }
+    static_assert((BWD ? 3 : kFwdCtas) * (bytes(kStages) + 1024) <= 228 * 1024, "CTAs on an SM");
+    static_assert(!BWD || 2 * (bytes(kFewStages) + 1024) <= 228 * 1024, "two CTAs on an SM");
     static_assert(L * CH * sizeof(T) >= 2 * CH * sizeof(float), "two sums in a warp's rows of f");
 };
 
@@ -99,7 +106,7 @@ struct Tiles {
     bool alive;
     static constexpr int L = Lay::L;
 
-    __device__ __forceinline__ T* at(int s, int i) const { return reinterpret_cast<T*>(sm + (s * NIN + i) * Lay::kIn); }
+    __device__ __forceinline__ T* at(int s, int i) const { return reinterpret_cast<T*>(sm + Lay::oIn + (s * NIN + i) * Lay::kIn); }
     // The warp's first row, this lane's first channel.
     __device__ __forceinline__ T* mine(int s, int i) const { return at(s, i) + warp * L * Lay::CH + lane * V; }
     // Asks for tile k in stage s, once what was written from that stage has been read.
@@ -109,7 +116,7 @@ struct Tiles {
         if (PLAIN) return;
         mbar_expect_tx(&bars[s], NIN * Lay::kIn);
 #pragma unroll
-        for (int i = 0; i < NIN; ++i) tma_load_3d(sm + (s * NIN + i) * Lay::kIn, map[i], &bars[s], c0, k * kTile, b);
+        for (int i = 0; i < NIN; ++i) tma_load_3d(at(s, i), map[i], &bars[s], c0, k * kTile, b);
     }
     // The warp's rows of tile k are in stage s from here on; steps behind the end have gates that change nothing.
     __device__ __forceinline__ void wait(int s, int k, uint32_t parity) {
@@ -296,10 +303,11 @@ __global__ void __launch_bounds__(kBwdWarps * 32, 3)
     constexpr int NIN = GATE ? 4 : 3;
     using Lay = Layout<T, V, NIN, true>;
     using C = Ch<V>;
-    constexpr int CH = Lay::CH, S = Lay::kStages, W = Lay::kWarps, L = Lay::L;
+    constexpr int CH = Lay::CH, W = Lay::kWarps, L = Lay::L;
+    const int S = p.stages;
     extern __shared__ unsigned char raw[];
     unsigned char* sm = raw + (128 - (smem_u32(raw) & 127)) % 128;
-    float* part = reinterpret_cast<float*>(sm + Lay::oPart);
+    float* part = reinterpret_cast<float*>(sm);
     uint64_t* bars = reinterpret_cast<uint64_t*>(sm + Lay::oBar);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, seg = static_cast<int>(blockIdx.x) % p.segments;
     const int strip = static_cast<int>(blockIdx.x) / p.segments, per_b = (p.a.D + CH - 1) / CH, b = strip / per_b;
@@ -316,9 +324,7 @@ __global__ void __launch_bounds__(kBwdWarps * 32, 3)
     const long long ld[4] = {p.a.ld_f, p.a.ld_x, p.a.ld_dy, p.a.ld_z};
     const int first = min((seg + 1) * p.per_segment, p.tiles) - 1, rounds = first + 1 - seg * p.per_segment;
     const C minus = C::splat(-1.0f);
-#pragma unroll
-    for (int i = 0; i < S - 1; ++i)
-        if (i < rounds) in.ask(i, first - i, maps);
+    for (int i = 0; i < min(S - 1, rounds); ++i) in.ask(i, first - i, maps);
     typename In::Word next_rows[PLAIN ? NIN : 1][L];
     if (PLAIN && rounds > 0) in.fetch(next_rows, first, src, ld);
     C carry = C::splat(0.0f);
@@ -542,11 +548,11 @@ static int check(Ctx* c, const mamba_b200_gated_scan_args* a, bool bwd) {
 
 
 // Segments of time, so that every SM has its three CTAs.  Cut, f and x (dy and z) are read twice; whole, a CTA's tiles follow one
-// another at 1.1 us (backward 1.7).  us, whole and cut: 168 strips x 64 tiles 96 and 100 (backward 156 and 172), 120 x 64 74 and 72
-// (137 and 123), 80 x 128 144 and 103 (249 and 161), 12 x 128 140 and 20; 12 x 4 tiles are 5 whole and 6 cut.
+// another at 1.1 us (backward 1.6).  us, whole and cut: 168 strips x 64 tiles 94 and 100 (backward 140 and 172), 120 x 64 74 and 72
+// (104 and 123), 96 x 64 69 and 55 (104 and 90), 72 x 64 69 and 44 (105 and 70), 12 x 128 140 and 20; 12 x 4 tiles are 5 whole and 6 cut.
 constexpr int kMaxSegments = 128;
-static int pick_segments(int sms, long long strips, int tiles) {
-    if (strips * 10 > 9ll * sms || tiles <= 4) return 1;
+static int pick_segments(int sms, long long strips, int tiles, bool bwd) {
+    if (strips * 20 > (bwd ? 15ll : 18ll) * sms || tiles <= 4) return 1;
     const long long want = 3ll * sms / (strips > 0 ? strips : 1);
     const int most = static_cast<int>(want < kMaxSegments ? want : kMaxSegments);
     return most < tiles ? most : tiles;
@@ -565,7 +571,7 @@ static int launch_tiled(Ctx* c, const mamba_b200_gated_scan_args& a, cudaStream_
     const long long strips = static_cast<long long>(a.B) * ((a.D + Lay::CH - 1) / Lay::CH);
     if (strips > 2147483647ll) return fail(c, MAMBA_B200_ERR_SHAPE, "gated_scan: too many channels");
     p.tiles = (a.T + kTile - 1) / kTile;
-    int segments = pick_segments(c->sm_count, strips, p.tiles);
+    int segments = pick_segments(c->sm_count, strips, p.tiles, BWD);
     if (reinterpret_cast<uintptr_t>(a.workspace) % 16 != 0) return fail(c, MAMBA_B200_ERR_ARG, "gated_scan: the workspace is 16-byte aligned");
     const long long row = static_cast<long long>(a.B) * a.D * 2 * sizeof(float);  // a segment's sums
     if (!a.workspace || a.workspace_bytes < 0) segments = 1;
@@ -583,9 +589,11 @@ static int launch_tiled(Ctx* c, const mamba_b200_gated_scan_args& a, cudaStream_
     void* bwd_args[] = {&mf, &mx, &me, &mz, &o0, &o1, &o2, &p};
     cudaLaunchConfig_t cfg;
     memset(&cfg, 0, sizeof(cfg));
-    cfg.gridDim = dim3(static_cast<unsigned>(strips * p.segments));
+    const long long ctas = strips * p.segments;
+    p.stages = BWD && few_ctas(c->sm_count, ctas) ? kFewStages : Lay::kStages;
+    cfg.gridDim = dim3(static_cast<unsigned>(ctas));
     cfg.blockDim = dim3(Lay::kWarps * 32);
-    cfg.dynamicSmemBytes = Lay::kBytes;
+    cfg.dynamicSmemBytes = Lay::bytes(p.stages);
     cfg.stream = st;
     cudaLaunchAttribute early;
     memset(&early, 0, sizeof(early));
@@ -604,7 +612,7 @@ static int launch_tiled(Ctx* c, const mamba_b200_gated_scan_args& a, cudaStream_
 template <typename T, int V, bool GATE, bool BWD, bool PLAIN>
 static int configure(Ctx* c) {
     using Lay = Layout<T, V, (GATE ? 3 : 2) + (BWD ? 1 : 0), BWD>;
-    MB200_CUDA_CHECK(c, cudaFuncSetAttribute(kernel<T, V, GATE, BWD, PLAIN>(), cudaFuncAttributeMaxDynamicSharedMemorySize, Lay::kBytes));
+    MB200_CUDA_CHECK(c, cudaFuncSetAttribute(kernel<T, V, GATE, BWD, PLAIN>(), cudaFuncAttributeMaxDynamicSharedMemorySize, Lay::bytes(BWD ? kFewStages : Lay::kStages)));
     return MAMBA_B200_OK;
 }
 
@@ -643,7 +651,7 @@ using namespace mb200;
 extern "C" MAMBA_B200_API long long mamba_b200_gated_scan_workspace_bytes(int B, int T, int D) {
     if (B <= 0 || T <= gs::kShort || D <= 0) return 0;
     // (strips of 64 channels, or of 32: the more segments of the two; sized for 148 SMs, which a launch on fewer only halves further)
-    const int segments = gs::pick_segments(148, static_cast<long long>(B) * ((D + 63) / 64), (T + gs::kTile - 1) / gs::kTile);
+    const int segments = gs::pick_segments(148, static_cast<long long>(B) * ((D + 63) / 64), (T + gs::kTile - 1) / gs::kTile, false);
     return segments > 1 ? static_cast<long long>(segments) * B * D * 2 * sizeof(float) : 0;
 }
 
