@@ -476,19 +476,29 @@ __global__ void __launch_bounds__(kThreads) embedding_sums_plain_kernel(const Bw
 }
 
 // Tokens that go on beyond a run.  A warp looks after the one that begins in its run and adds its runs' sums, if they are few; the
-// CTA does so for one that reaches far.
-constexpr int kJoinThreads = 256;
+// CTAs of a cluster share one that reaches 32 runs or more.  What counts for the many short ones is how many CTAs an SM has: with 8
+// loads in flight a warp and four CTAs 8192 x 768 f32 took 47.4 us, with 16 and two 53, with 4 and six 46.6.
+constexpr int kJoinThreads = 256, kJoinCtas = 4;
 template <int N>
-__global__ void __launch_bounds__(kJoinThreads) embedding_join_kernel(const BwdParams p) {
-    constexpr int WARPS = kJoinThreads / 32;
-    __shared__ float room[WARPS][32 * N];
-    __shared__ int far[WARPS];
-    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, c = (blockIdx.y * 32 + lane) * N;
+__global__ void __launch_bounds__(kJoinThreads, 6) embedding_join_kernel(const BwdParams p) {
+    constexpr int WARPS = kJoinThreads / 32, RUNS = kJoinCtas * WARPS, kCount = 8;
+    static_assert(RUNS % 32 == 0 && RUNS <= kJoinThreads, "a thread for each of the cluster's runs");
+    __shared__ float room[WARPS][32 * N], joined[32 * N];
+    __shared__ unsigned far[RUNS / 32];
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, c = (blockIdx.y * 32 + lane) * N, rank = blockIdx.x % kJoinCtas;
     asm volatile("griddepcontrol.wait;" ::: "memory");
-    const int runs = p.runs;
+    const int runs = p.runs, first = (static_cast<int>(blockIdx.x) - rank) * WARPS;
+    auto starts_with = [&](int run) { return p.sorted[run * p.run].y; };
+    auto ends_with = [&](int run) { return p.sorted[run * p.run + p.run - 1].y; };
+    if (warp < RUNS / 32) {  // the same in all CTAs of the cluster
+        const int run = first + tid;
+        const int token = run + 32 < runs ? ends_with(run) : -1;
+        const unsigned mask = __ballot_sync(0xffffffffu, token >= 0 && starts_with(run + 32) == token && (run == 0 || ends_with(run - 1) != token));
+        if (lane == 0) far[warp] = mask;
+    }
     auto add = [&](float* acc, int run, int begin, int end) {  // sums begin .. end of the token that begins in the run
         if (c >= p.dim) return;
-        constexpr int U = 8;
+        constexpr int U = 4;
         for (int i0 = begin; i0 < end; i0 += U) {
             Vec<float, N> q[U];
 #pragma unroll
@@ -504,35 +514,53 @@ __global__ void __launch_bounds__(kJoinThreads) embedding_join_kernel(const BwdP
     float acc[N];
 #pragma unroll
     for (int k = 0; k < N; ++k) acc[k] = 0.0f;
-    const int run = blockIdx.x * WARPS + warp;
+    const int run = first + rank * WARPS + warp;
     // lane l: the token at the start of run run + 1 + l; and those before this run and at its end
-    const int ahead = run + 1 + lane < runs ? p.sorted[(run + 1 + lane) * p.run].y : -1;
-    const int before = run > 0 && run < runs ? p.sorted[run * p.run - 1].y : -1, end = run + 1 < runs ? p.sorted[run * p.run + p.run - 1].y : -1;
+    const int ahead = run + 1 + lane < runs ? starts_with(run + 1 + lane) : -1;
+    const int before = run > 0 && run < runs ? ends_with(run - 1) : -1, end = run + 1 < runs ? ends_with(run) : -1;
     const int token = end >= 0 ? end : -2;  // (-2: none goes on from here)
     const unsigned same = __ballot_sync(0xffffffffu, ahead == token);
-    const bool begins = (same & 1) && before != token;
-    if (lane == 0) far[warp] = begins && same == 0xffffffffu;
-    if (begins && same != 0xffffffffu) {
+    if ((same & 1) && before != token && same != 0xffffffffu) {
         add(acc, run, 0, __ffs(~same));
         if (c < p.dim) write_sum<N>(p.d_table + static_cast<long long>(token) * p.dim + c, acc, p.scale, p.accumulate);
     }
     __syncthreads();
-    for (int w = 0; w < WARPS; ++w) {
-        if (!far[w]) continue;
-        const int from = blockIdx.x * WARPS + w, its = p.sorted[from * p.run + p.run - 1].y;
-        int n = 0;  // runs behind this one that it reaches
-        for (int i0 = from + 1;; i0 += kJoinThreads) {
-            const int here = __syncthreads_count(i0 + tid < runs && p.sorted[(i0 + tid) * p.run].y == its);
-            n += here;
-            if (here < kJoinThreads) break;
-        }
+#pragma unroll 1
+    for (int w = 0; w < RUNS / 32; ++w)
+#pragma unroll 1
+        for (unsigned m = far[w]; m; m &= m - 1) {
+            const int from = first + 32 * w + __ffs(m) - 1, its = ends_with(from);
+            int n = 0, here = 1;  // runs behind this one that it reaches
+            for (int i0 = from + 1 + tid; here; i0 += kCount * kJoinThreads) {
+                int starts[kCount];
 #pragma unroll
-        for (int k = 0; k < N; ++k) acc[k] = 0.0f;
-        const int each = (n + 1 + WARPS - 1) / WARPS;
-        add(acc, from, warp * each, min(n + 1, (warp + 1) * each));
-        add_warps<N, WARPS>(acc, room);
-        if (warp == 0 && c < p.dim) write_sum<N>(p.d_table + static_cast<long long>(its) * p.dim + c, acc, p.scale, p.accumulate);
-    }
+                for (int u = 0; u < kCount; ++u) starts[u] = i0 + u * kJoinThreads < runs ? starts_with(i0 + u * kJoinThreads) : -1;
+                here = 0;
+#pragma unroll
+                for (int u = 0; u < kCount; ++u) here += __syncthreads_count(starts[u] == its);
+                n += here;
+            }
+#pragma unroll
+            for (int k = 0; k < N; ++k) acc[k] = 0.0f;
+            const int each = (n + 1 + RUNS - 1) / RUNS, at = (rank * WARPS + warp) * each;
+            add(acc, from, at, min(n + 1, at + each));
+            add_warps<N, WARPS>(acc, room);
+            if (warp == 0) {
+#pragma unroll
+                for (int k = 0; k < N; ++k) joined[k * 32 + lane] = acc[k];
+            }
+            __syncwarp();
+            cluster_sync();
+            if (rank == 0 && warp == 0) {
+#pragma unroll
+                for (int i = 1; i < kJoinCtas; ++i)
+#pragma unroll
+                    for (int k = 0; k < N; ++k) acc[k] += ld_cluster1(cluster_addr(smem_u32(joined + k * 32 + lane), i));
+                if (c < p.dim) write_sum<N>(p.d_table + static_cast<long long>(its) * p.dim + c, acc, p.scale, p.accumulate);
+            }
+            __syncwarp();
+            cluster_sync();
+        }
 }
 
 constexpr long long kClearBeside = 128 << 20;
@@ -591,7 +619,7 @@ static int launch_bwd(Ctx* c, BwdParams& p, cudaStream_t st) {
         MB200_CUDA_CHECK(c, cudaGetLastError());
         return MAMBA_B200_OK;
     }
-    constexpr int NF = N == 1 ? 1 : 4, kColumns = N == 1 ? 128 : kPartBytes<T> / static_cast<int>(sizeof(T));
+    constexpr int NF = N == 1 ? 1 : 4, kJoinRuns = kJoinCtas * (kJoinThreads / 32), kColumns = N == 1 ? 128 : kPartBytes<T> / static_cast<int>(sizeof(T));
     p.slices = (p.dim + kColumns - 1) / kColumns;
     p.run = run_of(p.rows, p.dim);
     p.runs = (p.rows + p.run - 1) / p.run;
@@ -612,8 +640,8 @@ static int launch_bwd(Ctx* c, BwdParams& p, cudaStream_t st) {
         MB200_CUDA_CHECK(c, launch_early(embedding_sums_plain_kernel<T>, dim3((tasks + kThreads / 32 - 1) / (kThreads / 32)), kThreads, 0, st, 1, true, p, sums, clears));
     else
         MB200_CUDA_CHECK(c, launch_early(embedding_sums_kernel<T>, dim3(tasks), 32, p.run * kPartBytes<T> + 16 + 128, st, 1, true, p, sums, clears, c->d_status));
-    MB200_CUDA_CHECK(c, launch_early(embedding_join_kernel<NF>, dim3((p.runs + kJoinThreads / 32 - 1) / (kJoinThreads / 32), (p.dim + 32 * NF - 1) / (32 * NF)),
-                                     kJoinThreads, 0, st, 1, true, p));
+    MB200_CUDA_CHECK(c, launch_early(embedding_join_kernel<NF>, dim3((p.runs + kJoinRuns - 1) / kJoinRuns * kJoinCtas, (p.dim + 32 * NF - 1) / (32 * NF)),
+                                     kJoinThreads, 0, st, kJoinCtas, true, p));
     return MAMBA_B200_OK;
 }
 template <typename T>
