@@ -16,7 +16,7 @@
 namespace mb200 {
 namespace lp {
 
-constexpr int kThreads = 256, kWarps = kThreads / 32, kMaxTop = 32, kRoom = 512, kUnroll = 4, kCtas = 3;
+constexpr int kThreads = 256, kWarps = kThreads / 32, kMaxTop = 32, kRoom = 1024, kUnroll = 4, kCtas = 3;
 constexpr float kNothing = -256.0f;  // 2^-256 is 0 in f32
 
 // max that a NaN passes through.
@@ -43,16 +43,16 @@ struct Piece {
             return j == 0 ? make_float2(__uint_as_float(q.x), __uint_as_float(q.y)) : make_float2(__uint_as_float(q.z), __uint_as_float(q.w));
         }
     }
-    // The largest of N pieces (NaN aside).
-    template <int N> __device__ __forceinline__ static float top(const Piece* q) {
+    // The largest of N pieces' even elements and of their odd ones (NaN aside).
+    template <int N> __device__ __forceinline__ static float2 tops(const Piece* q) {
         if constexpr (sizeof(T) == 4) {
-            float m = -INFINITY;
+            float2 m = make_float2(-INFINITY, -INFINITY);
 #pragma unroll
             for (int u = 0; u < N; ++u)
 #pragma unroll
                 for (int k = 0; k < 2; ++k) {
                     const float2 v = q[u].pair(k);
-                    m = fmaxf(m, fmaxf(v.x, v.y));
+                    m.x = fmaxf(m.x, v.x), m.y = fmaxf(m.y, v.y);
                 }
             return m;
         } else {
@@ -64,8 +64,12 @@ struct Piece {
 #pragma unroll
                 for (int k = 0; k < 4; ++k) m = __hmax2(m, h[k]);
             }
-            return fmaxf(__low2float(m), __high2float(m));
+            return make_float2(__low2float(m), __high2float(m));
         }
+    }
+    template <int N> __device__ __forceinline__ static float top(const Piece* q) {
+        const float2 m = tops<N>(q);
+        return fmaxf(m.x, m.y);
     }
 };
 // A row in 16-byte pieces: `head` elements before the first aligned one, `pieces`, and a tail of less than one.
@@ -234,11 +238,12 @@ __device__ __forceinline__ float key_value(uint64_t k) {
     return __uint_as_float(b & 0x80000000u ? b & 0x7fffffffu : ~b);
 }
 
-constexpr int kGroup = kThreads / 32;  // threads of a group
+constexpr int kGroup = kThreads / 64;  // threads of a group
 constexpr int kMaxSplit = 16;
 static_assert(kRoom >= kMaxSplit * kMaxTop, "the parts' alternatives are joined in key");
+static_assert(kRoom >= kMaxTop * 4 * 8, "neighbouring tokens that are fewer than the groups they would need fit");
 struct TopRoom {
-    float group[32];
+    float group[64];
     uint64_t key[kRoom], sel[kMaxTop], best[kWarps];
     int n;
 };
@@ -261,7 +266,7 @@ __device__ __forceinline__ float nth_of_32(float v, int n) {
         for (int o = size >> 1; o > 0; o >>= 1) v = ordered(v, o, (threadIdx.x % 32 & size) == 0);
     return __shfl_sync(0xffffffffu, v, n - 1);
 }
-__device__ __forceinline__ float nth_of_64(float a, float b, int n) {  // n <= 32
+__device__ __forceinline__ float first_of_64(float a, float b) {  // the 32 largest in falling order
 #pragma unroll
     for (int size = 2; size <= 32; size <<= 1)
 #pragma unroll
@@ -273,11 +278,12 @@ __device__ __forceinline__ float nth_of_64(float a, float b, int n) {  // n <= 3
     a = fmaxf(a, b);  // the larger half; it falls and rises, one more pass puts it in order
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) a = ordered(a, o, true);
-    return __shfl_sync(0xffffffffu, a, n - 1);
+    return a;
 }
+__device__ __forceinline__ float nth_of_64(float a, float b, int n) { return __shfl_sync(0xffffffffu, first_of_64(a, b), n - 1); }  // n <= 32
 
-// The alternatives of [lo, hi) pieces (and the ends) of a row.  Eight threads' elements form a group.  tau, the top-th largest of
-// the 32 groups' maxima, is a lower bound of the top-th largest element: only what threads whose own maximum reaches it have seen
+// The alternatives of [lo, hi) pieces (and the ends) of a row.  Four threads' elements form a group.  tau, the top-th largest of
+// the 64 groups' maxima (of 32 groups': 32 alternatives of 8 rows 16.8 us instead of 10.6, 20 alternatives 10.1 instead of 9.0), is a lower bound of the top-th largest element: only what threads whose own maximum reaches it have seen
 // is read again (from L2), and what reaches it there goes to key[0 .. n) in any order.  Called by kThreads threads behind a
 // barrier that the groups' maxima and n = 0 have passed; a barrier ends it.  Returns how many keys there are: all that reach tau,
 // or where there was no room the largest (what is left equals tau then); or kInOrder, when sel is complete.
@@ -286,7 +292,7 @@ template <typename T>
 __device__ __noinline__ int reach(TopRoom& t, const Row<T>& row, int lo, int hi, bool first, bool last, int top, float own_top, float* equals) {
     constexpr int W = Piece<T>::W;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-    const float tau = nth_of_32(t.group[lane], top);
+    const float tau = nth_of_64(t.group[lane], t.group[lane + 32], top);
     auto offer = [&](float v, int i) {
         if (v >= tau && v > -INFINITY) {
             const int at = atomicAdd(&t.n, 1);
@@ -427,7 +433,7 @@ __device__ __forceinline__ void write_row(const FwdParams& p, long long r, const
 __device__ __forceinline__ int target_of(const FwdParams& p, long long r) { return p.targets && p.logprob ? p.targets[r] : -1; }
 
 // Rows one after another, by eight warps that do nothing but read: a ninth brings the rows to shared memory by bulk copies of
-// 16 KB, a tenth makes the results of a row while the next is read, so the memory is never idle.  HBM would be 12 logits a cycle
+// 16 KB, three more make the results of rows while the next ones are read, so the memory is never idle.  HBM would be 12 logits a cycle
 // and SM in 16 bits: with 16 exponentials a cycle and some 5 instructions a logit (of 128) the arithmetic is close behind, so the
 // pass has one fma and one exponential a logit, no clamp, and no test but two in 32 logits.
 constexpr int kRound = kThreads * kUnroll, kStages = 3;
@@ -447,8 +453,8 @@ static_assert(sizeof(Maker) % 16 == 0 && kThreads <= 256, "float4 reads of threa
 constexpr int kRowsSmem = kStages * kRound * 16 + static_cast<int>(sizeof(RowsRoom)) + 128;
 static_assert(kCtas * (kRowsSmem + 1024) <= 228 * 1024, "CTAs on an SM");
 
-// The alternatives of a row in order into sel, by one warp.  Eight threads' elements form a group.  tau, the top-th largest of
-// the 32 groups' maxima, is a lower bound of the top-th largest element: only what threads whose own maximum reaches it have seen
+// The alternatives of a row in order into sel, by one warp.  Four threads' elements form a group.  tau, the top-th largest of
+// the 64 groups' maxima, is a lower bound of the top-th largest element: only what threads whose own maximum reaches it have seen
 // is read again (from L2), and what reaches it there is ranked by counting.
 template <typename T>
 __device__ __noinline__ void find_top(Maker& t, const Row<T>& row, float row_top, int top) {
@@ -464,7 +470,7 @@ __device__ __noinline__ void find_top(Maker& t, const Row<T>& row, float row_top
     __syncwarp();
     if (lane == 0) tc::mbar_arrive(&t.empty);
     const float a = fmaxf(fmaxf(mine[0], mine[1]), fmaxf(mine[2], mine[3])), b = fmaxf(fmaxf(mine[4], mine[5]), fmaxf(mine[6], mine[7]));
-    const float tau = top <= 8 ? nth_of_32(fmaxf(a, b), top) : nth_of_64(a, b, top);
+    float tau = top <= 8 ? nth_of_32(fmaxf(a, b), top) : nth_of_64(a, b, top);
     int threads = 0;
 #pragma unroll
     for (int i = 0; i < kEach; ++i) {
@@ -475,9 +481,10 @@ __device__ __noinline__ void find_top(Maker& t, const Row<T>& row, float row_top
     }
     if (lane == 0) t.n = 0;
     __syncwarp();
-    // their pieces that reach tau
-    int pieces = 0;
-    for (int x = 0; x < threads; x += kAtOnce)
+    // their pieces that reach tau (where tau is the largest logit and many threads have it, the first of its equals are enough)
+    const bool level = tau == row_top && threads > 64;
+    int pieces = level ? kMakerRoom + 1 : 0;
+    for (int x = 0; x < threads && !level; x += kAtOnce)
         for (int j0 = 0; j0 < row.pieces; j0 += 32 * kThreads) {
             Piece<T> q[kAtOnce];
             int j[kAtOnce];
@@ -503,20 +510,45 @@ __device__ __noinline__ void find_top(Maker& t, const Row<T>& row, float row_top
             if (at < kMakerRoom) t.key[at] = key_of(v, i);
         }
     };
-    for (int x = lane; x < min(pieces, kMakerRoom); x += 32) {
+    auto piece = [&](int x) {
         Piece<T> q;
-        const int j = t.piece[x];
-        q.load(row.p + row.head + static_cast<long long>(j) * W);
+        q.load(row.p + row.head + static_cast<long long>(t.piece[x]) * W);
+        return q;
+    };
+    auto offer_all = [&]() {
+        for (int x = lane; x < pieces; x += 32) {
+            const Piece<T> q = piece(x);
+            const int i = row.head + t.piece[x] * W;
 #pragma unroll
-        for (int e = 0; e < W; e += 2) {
-            const float2 v = q.pair(e / 2);
-            offer(v.x, row.head + j * W + e);
-            offer(v.y, row.head + j * W + e + 1);
+            for (int e = 0; e < W; e += 2) {
+                const float2 v = q.pair(e / 2);
+                offer(v.x, i + e);
+                offer(v.y, i + e + 1);
+            }
         }
+        if (lane < row.head) offer(to_f(row.p[lane]), lane);
+        if (row.tail() + lane < row.V) offer(to_f(row.p[row.tail() + lane]), row.tail() + lane);
+        __syncwarp();
+    };
+    if (pieces <= kMakerRoom) offer_all();
+    if (t.n > kMakerRoom) {
+        // Many in few threads' places (neighbouring tokens, when all others are ruled out): the top-th largest of the pieces' own
+        // largest is a closer bound.
+        float first = -INFINITY;
+        for (int x = lane; x - lane < pieces; x += 32) {
+            float best = -INFINITY;
+            if (x < pieces) {
+                const Piece<T> q = piece(x);
+                best = Piece<T>::template top<1>(&q);
+            }
+            first = first_of_64(first, best);
+        }
+        tau = fmaxf(tau, __shfl_sync(0xffffffffu, first, top - 1));
+        __syncwarp();
+        if (lane == 0) t.n = 0;
+        __syncwarp();
+        offer_all();
     }
-    if (lane < row.head) offer(to_f(row.p[lane]), lane);
-    if (row.tail() + lane < row.V) offer(to_f(row.p[row.tail() + lane]), row.tail() + lane);
-    __syncwarp();
     int n = max(t.n, pieces);
     if (n <= kMakerRoom) n = t.n;
     float equals = -INFINITY;
@@ -648,7 +680,9 @@ __global__ void __launch_bounds__(kThreads + 32 + 32 * kMakers, kCtas) token_log
 }
 
 // Short rows: a warp has one in registers, so the largest logit is known before the sums and nothing is read twice.  Up to
-// 32 P pieces; kShortPieces 32 are 8192 logits in 16 bits.
+// 32 P pieces; kShortPieces 32 are 8192 logits in 16 bits.  tau, a lower bound of the top-th largest logit, comes from the largest
+// of each lane's even and odd elements (of each lane's alone, 32 alternatives of 4096 x 4000 were 374 us and not 26: the smallest of
+// 32 lanes lets too many through); up to 8 alternatives the lanes' suffice and cost less.
 constexpr int kShortPieces = 32, kShortWarps = 4, kShortRoom = 128;
 template <typename T, bool TOP, int P>
 __global__ void __launch_bounds__(kShortWarps * 32) token_logprobs_short_kernel(const FwdParams p) {
@@ -668,7 +702,9 @@ __global__ void __launch_bounds__(kShortWarps * 32) token_logprobs_short_kernel(
     const float head = lane < row.head ? to_f(row.p[lane]) : -INFINITY, tail = row.tail() + lane < p.V ? to_f(row.p[row.tail() + lane]) : -INFINITY;
     const int target = target_of(p, r);
     const float logit = target >= 0 && target < p.V ? to_f(row.p[target]) : 0.0f;
-    const float c = p.inv_temp * kLog2e, own_top = fmaxf(fmaxf(head, tail), Piece<T>::template top<P>(q));
+    float2 own = Piece<T>::template tops<P>(q);
+    own.x = fmaxf(own.x, head), own.y = fmaxf(own.y, tail);
+    const float c = p.inv_temp * kLog2e, own_top = fmaxf(own.x, own.y);
     Sums a{own_top, 0.0f, 0.0f, 0.0f};
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) a.top = fmaxf(a.top, __shfl_xor_sync(0xffffffffu, a.top, o));
@@ -697,7 +733,7 @@ __global__ void __launch_bounds__(kShortWarps * 32) token_logprobs_short_kernel(
     uint64_t* sel = sels[TOP ? warp : 0];
     if (TOP) {
         uint64_t* key = keys[TOP ? warp : 0];
-        const float tau = nth_of_32(own_top, p.top);
+        const float tau = p.top <= 8 ? nth_of_32(own_top, p.top) : nth_of_64(own.x, own.y, p.top);
         if (lane == 0) counts[warp] = 0;
         __syncwarp();
         auto offer = [&](float v, int i) {
@@ -722,26 +758,30 @@ __global__ void __launch_bounds__(kShortWarps * 32) token_logprobs_short_kernel(
         }
         __syncwarp();
         const int n = counts[warp];
-        if (n >= p.top && n <= kShortRoom) {
-            rank_keys<T>(key, sel, n, 0.0f, row, 0, 0, p.top);
+        if (n <= kShortRoom) {
+            rank_keys<T>(key, sel, n, -INFINITY, row, 0, p.V, p.top);
         } else {
-            // crowded by equals, or fewer are left than asked for: one after the other
+            // crowded by what equals tau: those above it one after the other
             uint64_t below = ~0ull;
-            for (int k = 0; k < p.top; ++k) {
-                uint64_t best = 0;
-                for (int i = lane; i < p.V; i += 32) {
-                    const uint64_t k2 = key_of(to_f(row.p[i]), i);
-                    if (k2 < below && k2 > best) best = k2;
-                }
+            int k = 0;
+            if (a.top > tau)
+                for (; k < p.top; ++k) {
+                    uint64_t best = 0;
+                    for (int i = lane; i < p.V; i += 32) {
+                        const uint64_t k2 = key_of(to_f(row.p[i]), i);
+                        if (k2 < below && k2 > best) best = k2;
+                    }
 #pragma unroll
-                for (int o = 16; o > 0; o >>= 1) {
-                    const uint64_t k2 = __shfl_xor_sync(0xffffffffu, best, o);
-                    if (k2 > best) best = k2;
+                    for (int o = 16; o > 0; o >>= 1) {
+                        const uint64_t k2 = __shfl_xor_sync(0xffffffffu, best, o);
+                        if (k2 > best) best = k2;
+                    }
+                    if (key_value(best) <= tau) break;
+                    below = best;
+                    if (lane == 0) key[k] = best;
                 }
-                below = best;
-                if (lane == 0) sel[k] = best;
-            }
             __syncwarp();
+            rank_keys<T>(key, sel, k, tau, row, 0, p.V, p.top);
         }
     }
     write_row<T>(p, r, a, target, logit, TOP ? sel : nullptr);

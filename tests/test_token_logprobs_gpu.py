@@ -139,6 +139,34 @@ def test_alternatives_where_more_stand_out_than_there_is_room_for(cuda_dev, dt, 
 
 
 @pytest.mark.parametrize("dt", DT)
+@pytest.mark.parametrize("rows", [3, 700])
+@pytest.mark.parametrize("V", [637, 4001, 20011, 50280])
+def test_alternatives_where_neighbours_are_left_or_many_are_equal(cuda_dev, dt, V, rows):
+    """A run of tokens is left and all others are ruled out, or the logits have few distinct values."""
+    import torch
+
+    import mamba_rs_b200 as mb
+    g = torch.Generator(cuda_dev).manual_seed(V + rows)
+    l = torch.randn(8, V, device=cuda_dev, generator=g) * 3
+    for i, n in enumerate((5, 100, 300, 600, 1000)):
+        at = (137 * i + 1) % V
+        l[i, :at] = -math.inf
+        l[i, at + n:] = -math.inf
+    l[5] = torch.round(l[5])
+    l[6] = torch.round(l[6] * 8) / 8
+    l[7] = -1.5
+    l = l.to(_dt(dt))
+    order = torch.sort(l.float(), dim=1, descending=True, stable=True)[1]
+    many = (rows + 7) // 8
+    for top in (1, 8, 9, 20, 32):
+        got = mb.token_logprobs(l.repeat(many, 1)[:rows], top=top)["top_ids"]
+        assert torch.equal(got.long(), order[:, :top].repeat(many, 1)[:rows])
+        if rows < 8:
+            got = mb.token_logprobs(l[8 - rows:], top=top)["top_ids"]
+            assert torch.equal(got.long(), order[8 - rows:, :top])
+
+
+@pytest.mark.parametrize("dt", DT)
 def test_what_is_not_a_number_shows(cuda_dev, dt):
     import torch
 
