@@ -377,8 +377,9 @@ __device__ __forceinline__ float* sum_place(const BwdParams& p, const Task& t, i
 }
 
 // Rows whose parts are 16-byte aligned come to shared memory by bulk copies, a lane asking for one row's part: a run's 16 or 32 KB are
-// in flight at once.  Parts of 512 bytes in f32, 1 KB in 16 bits: 32768 x 768 f32 73 us (with 1 KB 75), 16384 x 2560 bf16 130 (with 512
-// bytes 135).  Some 30 us of the first are this kernel, whose 155 MB (rows read, rows of tokens written, what is left to clear) are 24.
+// in flight at once.  Parts of 512 bytes in f32, 1 KB in 16 bits: 32768 x 768 f32 takes 71 us (with 1 KB 2 more), 16384 x 2560 bf16 123
+// (with 512 bytes 5 more).  Some 30 us of the first are this kernel, whose 155 MB (rows read, rows of tokens written, what is left to
+// clear) are 24.
 template <typename T> constexpr int kPartBytes = sizeof(T) == 2 ? 1024 : 512;
 template <typename T>
 __global__ void __launch_bounds__(32) embedding_sums_kernel(const BwdParams p, long long sums, long long clears, int* status) {
