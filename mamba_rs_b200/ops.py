@@ -573,10 +573,22 @@ def adamw_step(param, grad, m, v, bias_factors, *, lr, beta1=0.9, beta2=0.999, e
     return param
 
 
-def _same_device(dev, *named):
-    for t, nm in named:
-        if t is not None and t.device != dev:
-            raise ValueError(f"{nm} is on {t.device}, not on {dev}")
+def _device_index(*ts):
+    """The index of the CUDA device that all the tensors (None aside) are on."""
+    index = ts[0].get_device()
+    for t in ts:
+        if t is not None and t.get_device() != index:
+            index = -1
+            break
+    if index < 0:
+        _require_cuda(*ts)
+        raise ValueError(f"tensors on several devices: {', '.join(sorted({str(t.device) for t in ts if t is not None}))}")
+    return index
+
+
+def _new(like, dtype, rows, width):
+    """An empty [rows, width] on like's device (half the host time of torch.empty)."""
+    return torch.empty_strided((rows, width), (width, 1), dtype=dtype, device=like.device)
 
 
 def _row(t, width):
@@ -584,14 +596,13 @@ def _row(t, width):
     return t.stride(0) if t.shape[0] > 1 else max(t.stride(0), width)
 
 
-def _launch(fn, dev, handle, *args):
-    """fn(handle, current stream of dev, *args) with dev current; failures as the library words them."""
-    index = dev.index or 0
+def _launch(fn, index, handle, *args):
+    """fn(handle, current stream of the device, *args) with the device current; failures as the library words them."""
     h = handle or ffi.default_handle(index)
     if torch._C._cuda_getDevice() == index:
         rc = fn(h.ptr, torch._C._cuda_getCurrentRawStream(index), *args)
     else:
-        with torch.cuda.device(dev):
+        with torch.cuda.device(index):
             rc = fn(h.ptr, torch._C._cuda_getCurrentRawStream(index), *args)
     if rc:
         h.check(rc, fn.__name__)
@@ -600,19 +611,19 @@ def _launch(fn, dev, handle, *args):
 def embedding_fwd(table, ids, *, scale=1.0, out=None, out_dtype=torch.float32, handle=None):
     """out [rows, dim] = scale * table[ids]: table [vocab, dim] in the storage dtype (any row stride), ids int32 of any
     shape; out in float32 (the residual stream) or the table's dtype.  An id outside the table gives a row of zeros."""
-    _require_cuda(table, ids, out)
-    dev = table.device
+    dev = _device_index(table, ids, out)
     if table.dim() != 2 or table.stride(1) != 1 or ids.dtype != torch.int32 or not ids.is_contiguous():
         raise TypeError("the table is [vocab, dim] with contiguous rows, ids are contiguous int32")
     vocab, dim = table.shape
     rows = ids.numel()
     if out is None:
-        out = torch.empty((rows, dim), dtype=out_dtype, device=dev)
+        out, ld_out = _new(table, out_dtype, rows, dim), dim
     elif tuple(out.shape) != (rows, dim) or out.stride(1) != 1:
         raise ValueError(f"out is [{rows}, {dim}] with contiguous rows")
-    _same_device(dev, (ids, "ids"), (out, "out"))
+    else:
+        out_dtype, ld_out = out.dtype, _row(out, dim)
     _launch(ffi.lib().mamba_b200_embedding_fwd, dev, handle, dtype_code(table.dtype), table.data_ptr(), _row(table, dim), ids.data_ptr(),
-            dtype_code(out.dtype), out.data_ptr(), _row(out, dim), rows, dim, vocab, scale)
+            dtype_code(out_dtype), out.data_ptr(), ld_out, rows, dim, vocab, scale)
     return out
 
 
@@ -625,8 +636,7 @@ def embedding_bwd(ids, d_out, vocab=None, *, d_table=None, scale=1.0, workspace=
     """Gradient of embedding_fwd's table: scale * the sums of d_out's rows by token, f32 [vocab, dim].  Accumulated into
     d_table when it is given, else a fresh tensor.  ids int32 of any shape, d_out [ids.numel(), dim] in a storage dtype (any
     row stride).  The order of the sums is fixed: the same inputs give the same bits."""
-    _require_cuda(ids, d_out, d_table, workspace)
-    dev = d_out.device
+    dev = _device_index(ids, d_out, d_table, workspace)
     rows = ids.numel()
     if ids.dtype != torch.int32 or not ids.is_contiguous():
         raise TypeError("ids are contiguous int32")
@@ -643,12 +653,11 @@ def embedding_bwd(ids, d_out, vocab=None, *, d_table=None, scale=1.0, workspace=
     elif vocab is None:
         raise ValueError("the vocabulary's size or a table to accumulate into is needed")
     else:
-        d_table = torch.empty((vocab, dim), dtype=torch.float32, device=dev)
+        d_table = _new(d_out, torch.float32, vocab, dim)
     lib = ffi.lib()
     if workspace is None:
         need = lib.mamba_b200_embedding_bwd_workspace_bytes(rows, dim, vocab)
-        workspace = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
-    _same_device(dev, (ids, "ids"), (d_table, "d_table"), (workspace, "workspace"))
+        workspace = torch.empty(need, dtype=torch.uint8, device=d_out.device) if need else None
     _launch(lib.mamba_b200_embedding_bwd, dev, handle, dtype_code(d_out.dtype), d_out.data_ptr(), _row(d_out, dim), ids.data_ptr(),
             d_table.data_ptr(), accumulate, rows, dim, vocab, scale, _ptr(workspace),
             0 if workspace is None else workspace.numel() * workspace.element_size())
@@ -667,24 +676,22 @@ def token_logprobs(logits, targets=None, *, top=0, temperature=1.0, handle=None)
     the vocabulary: not counted, 0) also logprob [rows], all f32; with top > 0 (at most 32) also top_ids int32 and
     top_logprobs f32 [rows, top], by falling probability, equal ones by rising index.  lse holds the largest
     logit M and the log of the sum of exp((logits - M) / temperature): the log-sum-exp is M / temperature plus that.  Logits of -inf are tokens that are ruled out."""
-    _require_cuda(logits, targets)
+    dev = _device_index(logits, targets)
     _logit_rows(logits, targets)
     rows, V = logits.shape
-    dev = logits.device
-    _same_device(dev, (targets, "targets"))
     if not 0 <= top <= min(32, V):
         raise ValueError(f"{top} alternatives of {V} tokens (at most 32)")
     # (a tensor of its own costs the host half of what a slice does)
-    lse = torch.empty((2, rows), dtype=torch.float32, device=dev)
+    lse = _new(logits, torch.float32, 2, rows)
     entropy = lse.new_empty(rows)
     out = dict(lse=lse, entropy=entropy)
     tp = lp = ip = vp = None
     if targets is not None:
-        out["logprob"] = logprob = lse.new_empty(rows)
+        out["logprob"] = logprob = torch.empty_like(entropy)
         tp, lp = targets.data_ptr(), logprob.data_ptr()
     if top:
-        out["top_ids"] = ids = torch.empty((rows, top), dtype=torch.int32, device=dev) if targets is None else targets.new_empty((rows, top))
-        out["top_logprobs"] = val = lse.new_empty((rows, top))
+        out["top_logprobs"] = val = _new(logits, torch.float32, rows, top)
+        out["top_ids"] = ids = torch.empty_like(val, dtype=torch.int32)
         ip, vp = ids.data_ptr(), val.data_ptr()
     _launch(ffi.lib().mamba_b200_token_logprobs, dev, handle, dtype_code(logits.dtype), logits.data_ptr(), _row(logits, V), tp,
             temperature, lse.data_ptr(), entropy.data_ptr(), lp, top, ip, vp, rows, V)
@@ -695,19 +702,16 @@ def token_logprobs_bwd(logits, targets, lse, entropy, d_logprob=None, d_entropy=
                        handle=None):
     """Gradient of the logits from those of logprob and entropy (f32 [rows], either may be None), with lse and entropy as
     token_logprobs returned them.  dlogits in the logits' dtype; it may be the logits themselves."""
-    _require_cuda(logits, targets, lse, entropy, d_logprob, d_entropy, dlogits)
+    dev = _device_index(logits, targets, lse, entropy, d_logprob, d_entropy, dlogits)
     _logit_rows(logits, targets)
     rows, V = logits.shape
-    dev = logits.device
     for t, nm, n in ((lse, "lse", 2), (entropy, "entropy", 1), (d_logprob, "d_logprob", 1), (d_entropy, "d_entropy", 1)):
         if t is not None and (t.dtype != torch.float32 or not t.is_contiguous() or t.numel() != n * rows):
             raise TypeError(f"{nm} is contiguous float32, {n} x {rows}")
     if dlogits is None:
-        dlogits = torch.empty((rows, V), dtype=logits.dtype, device=dev)
+        dlogits = _new(logits, logits.dtype, rows, V)
     elif dlogits.dtype != logits.dtype or dlogits.shape != logits.shape or dlogits.stride(1) != 1:
         raise TypeError("dlogits has the logits' dtype and shape and contiguous rows")
-    _same_device(dev, (targets, "targets"), (lse, "lse"), (entropy, "entropy"), (d_logprob, "d_logprob"), (d_entropy, "d_entropy"),
-                 (dlogits, "dlogits"))
     _launch(ffi.lib().mamba_b200_token_logprobs_bwd, dev, handle, dtype_code(logits.dtype), logits.data_ptr(), _row(logits, V),
             _ptr(targets), temperature, lse.data_ptr(), _ptr(entropy), _ptr(d_logprob), _ptr(d_entropy), dlogits.data_ptr(),
             _row(dlogits, V), rows, V)
@@ -731,15 +735,15 @@ def _gated_workspace(workspace, x):
         if not need:
             return None, None, 0
         workspace = torch.empty(need, dtype=torch.uint8, device=x.device)
-    elif workspace.device != x.device or not workspace.is_contiguous():
-        raise ValueError("the workspace is contiguous, on x's device")
+    elif not workspace.is_contiguous():
+        raise ValueError("the workspace is contiguous")
     return workspace, workspace.data_ptr(), workspace.numel() * workspace.element_size()
 
 
 def _gated_rows(t, name, like):
     """Row stride of a [B, T, D] view whose rows are one after another: any stride where there is but one row."""
-    if t.dtype != like.dtype or t.shape != like.shape or t.device != like.device:
-        raise TypeError(f"{name} has x's dtype, shape and device: {list(like.shape)} {like.dtype}")
+    if t.dtype != like.dtype or t.shape != like.shape:
+        raise TypeError(f"{name} has x's dtype and shape: {list(like.shape)} {like.dtype}")
     B, T, D = t.shape
     s0, s1, s2 = t.stride()
     if s2 != 1 and D > 1:
@@ -753,8 +757,8 @@ def _gated_rows(t, name, like):
 
 def _gated_state(t, name, x, shape=None):
     shape = shape or (x.shape[0], x.shape[2])
-    if t is not None and (t.dtype != torch.float32 or tuple(t.shape) != shape or not t.is_contiguous() or t.device != x.device):
-        raise TypeError(f"{name} is contiguous float32 {list(shape)} on x's device")
+    if t is not None and (t.dtype != torch.float32 or tuple(t.shape) != shape or not t.is_contiguous()):
+        raise TypeError(f"{name} is contiguous float32 {list(shape)}")
     return _ptr(t)
 
 
@@ -763,11 +767,10 @@ def gated_scan_fwd(x, f, z=None, *, h0=None, h_last=None, y=None, chunk_states=N
     x, f, z, y [B,T,D] in a storage dtype, any row stride; h0 (zeros if None) and h_last (written if given, may be h0)
     [B,D] f32; chunk_states f32 of gated_scan_states(B,T,D) receives what gated_scan_bwd needs.  workspace: scratch of
     gated_scan_workspace_bytes(B,T,D) bytes (made here if None).  Returns y."""
-    _require_cuda(x, f, z, h0, h_last, y, chunk_states, workspace)
+    dev = _device_index(x, f, z, h0, h_last, y, chunk_states, workspace)
     if y is None:
-        y = x.new_empty(x.shape)
+        y = torch.empty_like(x, memory_format=torch.contiguous_format)
     B, T, D = x.shape
-    dev = x.device
     a = ffi.GatedScanArgs(dtype_code(x.dtype), B, T, D, x.data_ptr(), _gated_rows(x, "x", x), f.data_ptr(), _gated_rows(f, "f", x),
                           _ptr(z), 0 if z is None else _gated_rows(z, "z", x), _gated_state(h0, "h0", x),
                           _gated_state(h_last, "h_last", x), y.data_ptr(), _gated_rows(y, "y", x),
@@ -780,26 +783,27 @@ def gated_scan_fwd(x, f, z=None, *, h0=None, h_last=None, y=None, chunk_states=N
 
 def gated_scan_step(x, f, h0, z=None, *, h_last=None, y=None, handle=None):
     """One token per sequence: x, f, z, y [B,D]; the state h0 [B,D] f32 is updated in place, or h_last receives it."""
-    _require_cuda(x, f, z, h0, h_last, y)
+    dev = _device_index(x, f, h0, z, h_last, y)
+    dtype = x.dtype
     B, D = shape = x.shape
     if y is None:
-        y = x.new_empty(shape)
+        y = torch.empty_like(x, memory_format=torch.contiguous_format)
 
     def row(t, name):
-        if t.dtype != x.dtype or t.shape != shape or t.device != x.device:
-            raise TypeError(f"{name} has x's dtype, shape and device: {list(shape)} {x.dtype}")
+        if t.dtype != dtype or t.shape != shape:
+            raise TypeError(f"{name} has x's dtype and shape: {list(shape)} {dtype}")
         ld, one = t.stride()
         if one != 1 and D > 1:
             raise ValueError(f"{name}: last dimension must be contiguous")
         return ld if B > 1 else D
 
     for t, name in ((h0, "h0"), (h_last, "h_last")):
-        if t is not None and (t.dtype != torch.float32 or t.shape != shape or not t.is_contiguous() or t.device != x.device):
-            raise TypeError(f"{name} is contiguous float32 {list(shape)} on x's device")
+        if t is not None and (t.dtype != torch.float32 or t.shape != shape or not t.is_contiguous()):
+            raise TypeError(f"{name} is contiguous float32 {list(shape)}")
     h = h0.data_ptr()
-    a = ffi.GatedScanArgs(dtype_code(x.dtype), B, 1, D, x.data_ptr(), row(x, "x"), f.data_ptr(), row(f, "f"), _ptr(z),
+    a = ffi.GatedScanArgs(dtype_code(dtype), B, 1, D, x.data_ptr(), row(x, "x"), f.data_ptr(), row(f, "f"), _ptr(z),
                           0 if z is None else row(z, "z"), h, h if h_last is None else h_last.data_ptr(), y.data_ptr(), row(y, "y"))
-    _launch(ffi.lib().mamba_b200_gated_scan_fwd, x.device, handle, C.byref(a))
+    _launch(ffi.lib().mamba_b200_gated_scan_fwd, dev, handle, C.byref(a))
     return y
 
 
@@ -807,14 +811,13 @@ def gated_scan_bwd(x, f, dy, chunk_states, z=None, *, d_last=None, d_h0=None, d_
                    handle=None):
     """Backward of gated_scan_fwd from its chunk_states.  d_last [B,D] f32: gradient of the state that left (None: zeros).
     Returns dict(d_x, d_f, d_z (with z), d_h0 f32); the outputs may be given (columns of one projection's gradient, say)."""
-    _require_cuda(x, f, z, dy, chunk_states, d_last, d_h0, d_x, d_f, d_z, workspace)
+    dev = _device_index(x, f, z, dy, chunk_states, d_last, d_h0, d_x, d_f, d_z, workspace)
     B, T, D = x.shape
-    dev = x.device
-    new = lambda t: torch.empty(x.shape, dtype=x.dtype, device=dev) if t is None else t  # noqa: E731
+    new = lambda t: torch.empty_like(x, memory_format=torch.contiguous_format) if t is None else t  # noqa: E731
     d_x, d_f = new(d_x), new(d_f)
     d_z = new(d_z) if z is not None else None
     if d_h0 is None:
-        d_h0 = torch.empty((B, D), dtype=torch.float32, device=dev)
+        d_h0 = _new(x, torch.float32, B, D)
     a = ffi.GatedScanArgs(dtype_code(x.dtype), B, T, D, x.data_ptr(), _gated_rows(x, "x", x), f.data_ptr(), _gated_rows(f, "f", x),
                           _ptr(z), 0 if z is None else _gated_rows(z, "z", x), None, None, None, 0,
                           _gated_state(chunk_states, "chunk_states", x, gated_scan_states(B, T, D)),
