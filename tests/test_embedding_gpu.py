@@ -176,3 +176,23 @@ def test_rows_that_are_one_in_memory_are_refused(cuda_dev):
     for bad in (lambda: mb.embedding_fwd(one.expand(5, 8), ids), lambda: mb.embedding_bwd(ids, one.expand(4, 8), 5)):
         with pytest.raises(RuntimeError, match="bad dims"):
             bad()
+
+
+@pytest.mark.parametrize("dt", ["f32", "bf16"])
+@pytest.mark.parametrize("dim", [4, 129, 520])
+@pytest.mark.parametrize("lengths", [(9000,), (1, 1023, 1025, 31, 2048, 33), (700, 5000, 3, 1100, 1100, 64), (40000, 513, 30000)])
+def test_tokens_that_reach_over_many_runs(cuda_dev, dt, dim, lengths):
+    """Sums of small whole numbers are exact in f32 in any order: rows of one token in thousands, in order and shuffled."""
+    import torch
+
+    import mamba_rs_b200 as mb
+    g = torch.Generator(cuda_dev).manual_seed(dim + len(lengths))
+    tokens = torch.tensor([5, 17, 18, 400, 401, 650][: len(lengths)], device=cuda_dev)
+    ids = torch.repeat_interleave(tokens, torch.tensor(lengths, device=cuda_dev)).int()
+    d = torch.randint(-3, 4, (ids.numel(), dim), device=cuda_dev, generator=g).to({"f32": torch.float32, "bf16": torch.bfloat16}[dt])
+    for order in (torch.arange(ids.numel(), device=cuda_dev), torch.randperm(ids.numel(), device=cuda_dev, generator=g)):
+        i, x = ids[order].contiguous(), d[order].contiguous()
+        want = torch.zeros(700, dim, dtype=torch.float64, device=cuda_dev).index_add_(0, i.long(), x.double())
+        assert torch.equal(mb.embedding_bwd(i, x, 700).double(), want)
+        start = torch.ones(700, dim, device=cuda_dev)
+        assert torch.equal(mb.embedding_bwd(i, x, d_table=start).double(), want + 1)
