@@ -102,7 +102,7 @@ struct FwdParams {
 struct Sums {
     float top, rho, s, s1;
     __device__ __forceinline__ void raise(float to) {
-        const float d = max_nan(rho - to, kNothing), e = ex2(d);
+        const float d = rho == to ? 0.0f : max_nan(rho - to, kNothing), e = ex2(d);  // (both may be infinite)
         s1 = e * fmaf(s, d, s1);
         s *= e;
         rho = to;
@@ -110,10 +110,18 @@ struct Sums {
 };
 constexpr float kFarDown = -1e37f;  // below any reference
 constexpr float kSlack = 60.0f;     // a term may be 2^60: f32 sums have room for that
+// The reference of a largest logit.  The product is rounded up: a term's exponent, which is exact but for its own rounding, is then
+// never far above kSlack, however large the product.  (To nearest, a thread that had met nothing but a mask's -1e10 had terms of
+// 2^440, and made its row NaN.)
+__device__ __forceinline__ float reference(float top, float c) { return __fmul_ru(top, c); }
 __device__ __forceinline__ Sums no_sums() { return {-INFINITY, kFarDown, 0.0f, 0.0f}; }
-// Where rho cannot follow the largest logit (a row of the type's lowest value: the product with c overflows, or 16-bit logits of
-// minus infinity cannot be told from it), the pass shows it by these and the row is summed again.
-__device__ __forceinline__ bool in_doubt(const Sums& a) { return a.top > -INFINITY && (a.s == 0.0f || (a.s == a.s && a.s1 != a.s1)); }
+// Where rho cannot follow the largest logit (products beyond 2^27 are 8 or more apart, or overflow to either side: a row of a mask's
+// value, a logit of the type's largest, a tiny temperature; or 16-bit logits of minus infinity cannot be told from it), the row is
+// summed again.  A logit of plus infinity is not in doubt: its own term is NaN.
+constexpr float kFarProduct = 134217728.0f;
+__device__ __forceinline__ bool in_doubt(const Sums& a, float c) {
+    return a.top > -INFINITY && a.top < INFINITY && (fabsf(a.top * c) >= kFarProduct || a.s == 0.0f || (a.s == a.s && a.s1 != a.s1));
+}
 
 // A thread's running sums over pieces of a row, two chains.
 template <typename T>
@@ -132,7 +140,7 @@ struct Running {
 #pragma unroll
         for (int u = 0; u < N; ++u) q[u].load(at + u * kThreads * W);
         top = fmaxf(top, Piece<T>::template top<N>(q));
-        if (top * c > rho + kSlack) raise(top * c);  // (the first time, and where a row rises steeply)
+        if (const float at_top = reference(top, c); at_top > rho + kSlack) raise(at_top);  // (the first time, and where a row rises steeply)
         const float2 cc = splat2(c), neg = splat2(-rho), was = s1;
         if (masked) {
 #pragma unroll
@@ -184,7 +192,7 @@ struct Running {
     }
     __device__ __forceinline__ void end(float v, float c) {
         top = fmaxf(top, v);
-        if (top * c > rho + kSlack) raise(top * c);
+        if (const float at_top = reference(top, c); at_top > rho + kSlack) raise(at_top);
         const float t = max_nan(fmaf(v, c, -rho), kNothing), x = ex2(t);
         s.x += x;
         s1.x = fmaf(x, t, s1.x);
@@ -403,7 +411,7 @@ __device__ __forceinline__ void rank_keys(const uint64_t* key, uint64_t* sel, in
 // Sums relative to a row's largest logit from those relative to rho: rho is 0 then.
 template <typename T>
 __device__ __forceinline__ void settle(Sums& a, const Row<T>& row, float c) {
-    if (in_doubt(a)) a = sum_again(row, a.top, c);
+    if (in_doubt(a, c)) a = sum_again(row, a.top, c);
     else a.rho = fmaf(a.top, c, -a.rho);  // top c - rho
 }
 // One warp writes a row's results from its sums (alike in all lanes; 2^rho more than those relative to the largest logit), the

@@ -1,0 +1,114 @@
+"""Token log probabilities where a row is hard on the arithmetic: very large and very low logits, tiny temperatures.  All against
+the definition in 64 bits.
+
+Tolerances.  As beside the ordinary rows: with E = 2^-21 (2 + log V) + 2^-24 (V / 256 + 16), log S is off by E, the entropy by
+E (2 + log V), a log probability by E and 2^-22 of its value."""
+import math
+
+import numpy as np
+import pytest
+
+pytestmark = pytest.mark.gpu
+DT = ["f32", "bf16", "f16"]
+# short rows, rows over a cluster's CTAs, rows one after another
+SIZES = [(5, 777), (3, 5003), (700, 5003), (3, 50280), (600, 50277)]
+
+
+def _dt(name):
+    import torch
+    return {"f32": torch.float32, "bf16": torch.bfloat16, "f16": torch.float16}[name]
+
+
+def _plain(l, t, temp):
+    """log S, entropy, log probabilities of all tokens (beyond f32's range: infinite) and of the targets."""
+    import torch
+    l = l.double() / float(np.float32(temp))
+    d = l - l.amax(1)[:, None]
+    e = torch.exp(d)
+    log_s = torch.log1p((e.sum(1) - 1.0).clamp(min=0.0))
+    logp = d - log_s[:, None]
+    H = log_s - (e * torch.where(e > 0, d, 0.0)).sum(1) / e.sum(1)
+    logp = torch.where(logp < -float(torch.finfo(torch.float32).max), -math.inf, logp)
+    return log_s, H, logp, logp.gather(1, t.long()[:, None])[:, 0]
+
+
+def _close(got, want, tol):
+    import torch
+    got, fin = got.double(), torch.isfinite(want)
+    assert torch.equal(got[~fin], want[~fin])
+    tol = tol.expand_as(want)[fin] if hasattr(tol, "expand_as") else tol
+    assert ((got - want).abs()[fin] <= tol).all(), (got - want)[fin].abs().max()
+
+
+def _check(l, t, temp, top=5):
+    import torch
+
+    import mamba_rs_b200 as mb
+    V = l.shape[1]
+    log_s, H, logp, lp = _plain(l, t, temp)
+    e, big = 2.0 ** -21 * (2 + math.log(V)) + 2.0 ** -24 * (V / 256 + 16), 2.0 ** -22
+    r = mb.token_logprobs(l, t, top=top, temperature=temp)
+    assert torch.equal(r["lse"][0], l.float().amax(1))
+    _close(r["lse"][1], log_s, e)
+    _close(r["entropy"], H, e * (2 + math.log(V)))
+    _close(r["logprob"], lp, e + big * lp.abs())
+    order = torch.sort(l.float(), dim=1, descending=True, stable=True)[1][:, :top]
+    assert torch.equal(r["top_ids"].long(), order)
+    want = logp.gather(1, order)
+    _close(r["top_logprobs"], want, e + big * want.abs())
+    plain = mb.token_logprobs(l, t, temperature=temp)  # (without alternatives: another kernel)
+    for k, tol in (("lse", e), ("entropy", e * (2 + math.log(V)))):
+        assert ((plain[k] - r[k]).abs() <= 2 * tol).all()
+    mb.ffi.default_handle(0).check_status()
+    return r
+
+
+@pytest.mark.parametrize("dt", DT)
+@pytest.mark.parametrize("rows,V", SIZES)
+@pytest.mark.parametrize("high", [1e6, 1e9, 1e10, 1e30, "max"])
+def test_tokens_that_are_forced(cuda_dev, dt, rows, V, high):
+    """A very large logit in one place, in some, in the whole row."""
+    import torch
+    g = torch.Generator(cuda_dev).manual_seed(V + rows)
+    l = torch.randn(rows, V, device=cuda_dev, generator=g) * 3
+    high = torch.finfo(_dt(dt)).max if high == "max" else min(high, torch.finfo(_dt(dt)).max)
+    at = torch.randint(0, V, (rows, 4), device=cuda_dev, generator=g)
+    l.scatter_(1, at[:, :1], high)
+    l[1::3] = l[1::3].scatter(1, at[1::3], high)
+    l[2::3] = high
+    t = torch.randint(0, V, (rows,), device=cuda_dev, dtype=torch.int32, generator=g)
+    t[::2] = at[::2, 0].int()
+    for temp in (1.0, 0.7):
+        _check(l.to(_dt(dt)), t, temp)
+
+
+@pytest.mark.parametrize("dt", DT)
+@pytest.mark.parametrize("rows,V", SIZES)
+@pytest.mark.parametrize("low", [-1e4, -1e9, -1e10, -1e20, -1e30])
+def test_masks_of_large_negative_values(cuda_dev, dt, rows, V, low):
+    """All but a few neighbouring tokens at one low value; whole rows of it."""
+    import torch
+    g = torch.Generator(cuda_dev).manual_seed(V + rows)
+    low = max(low, torch.finfo(_dt(dt)).min)
+    l = torch.full((rows, V), low, device=cuda_dev)
+    for r in range(rows):
+        if r % 3 != 1:
+            at = (977 * r + 31) % (V - 9)
+            l[r, at:at + 9] = torch.randn(9, device=cuda_dev, generator=g) * 3
+    t = torch.arange(rows, device=cuda_dev, dtype=torch.int32) * 977 + 33
+    t = (t % (V - 9)).int()
+    for temp in (1.0, 0.7):
+        _check(l.to(_dt(dt)), t, temp)
+
+
+@pytest.mark.parametrize("dt", DT)
+@pytest.mark.parametrize("rows,V", SIZES)
+@pytest.mark.parametrize("temp", [1e-4, 1e-6, 1e-8, 1e-12, 1e-30])
+def test_tiny_temperatures(cuda_dev, dt, rows, V, temp):
+    import torch
+    g = torch.Generator(cuda_dev).manual_seed(V + rows)
+    l = (torch.randn(rows, V, device=cuda_dev, generator=g) * 3).to(_dt(dt))
+    l[1::3] -= 40.0
+    t = torch.randint(0, V, (rows,), device=cuda_dev, dtype=torch.int32, generator=g)
+    t[::2] = l.float().argmax(1)[::2].int()
+    _check(l, t, temp)
