@@ -97,8 +97,9 @@ struct FwdParams {
 };
 
 // top: largest logit.  With rho a reference near top c (c = log2 e / temperature; the product is rounded, and rho may lie up to
-// kSlack below, but the same rho meets every term): s = sum of 2^t, s1 = sum of 2^t t, t = logit c - rho in one rounding.  Then log2 S = log2 s - (top c - rho) and, in
-// base 2, the entropy = log2 s - s1 / s whatever rho is.
+// kSlack below, but the same rho meets every term): s = sum of 2^t, s1 = sum of 2^t t, t = logit c - rho in one rounding.  With
+// r = top c - rho the sums relative to the largest logit are S = s 2^-r and S1 = (s1 - r s) 2^-r, the entropy is, in base 2,
+// log2 S - S1 / S.
 struct Sums {
     float top, rho, s, s1;
     __device__ __forceinline__ void raise(float to) {
@@ -109,7 +110,10 @@ struct Sums {
     }
 };
 constexpr float kFarDown = -1e37f;  // below any reference
-constexpr float kSlack = 60.0f;     // a term may be 2^60: f32 sums have room for that
+// A term may be 2^8.  The exponent of a token that is all but certain is rounded at that size (2^-21), and log S and the entropy, which
+// are near 0 then, are off by as much: with 60 they were off by 2.6e-6 and 5.1e-6 and came out below 0.  A raise is one thread's, in
+// rows with a logit that stands out; 4096 x 50280 takes no longer than with 60.
+constexpr float kSlack = 8.0f;
 // The reference of a largest logit.  The product is rounded up: a term's exponent, which is exact but for its own rounding, is then
 // never far above kSlack, however large the product.  (To nearest, a thread that had met nothing but a mask's -1e10 had terms of
 // 2^440, and made its row NaN.)
@@ -408,25 +412,30 @@ __device__ __forceinline__ void rank_keys(const uint64_t* key, uint64_t* sel, in
     __syncwarp();
 }
 
-// Sums relative to a row's largest logit from those relative to rho: rho is 0 then.
+// Sums relative to a row's largest logit from those relative to rho.
 template <typename T>
 __device__ __forceinline__ void settle(Sums& a, const Row<T>& row, float c) {
-    if (in_doubt(a, c)) a = sum_again(row, a.top, c);
-    else a.rho = fmaf(a.top, c, -a.rho);  // top c - rho
+    if (in_doubt(a, c)) {
+        a = sum_again(row, a.top, c);
+    } else if (a.top > -INFINITY) {
+        const float r = fmaf(a.top, c, -a.rho), e = exp2f(-r);
+        a.s1 = e * fmaf(-r, a.s, a.s1);
+        a.s *= e;
+    }
 }
-// One warp writes a row's results from its sums (alike in all lanes; 2^rho more than those relative to the largest logit), the
-// target's logit and the alternatives in order.
+// One warp writes a row's results from its sums (alike in all lanes, relative to the largest logit), the target's logit and the
+// alternatives in order.  The largest logit's own term is 1, so S is no less, a log probability no more than 0 and an entropy no less.
 template <typename T>
 __device__ __forceinline__ void write_row(const FwdParams& p, long long r, const Sums& a, int target, float logit, const uint64_t* sel) {
     const int lane = threadIdx.x % 32;
-    const float log_s = (lg2(a.s) - a.rho) * kLn2;
+    const float S = max_nan(a.s, 1.0f), log_s = logf(S);  // (lg2 near 1 is good to 2^-22 alone)
     const bool none = a.s == 0.0f;
     if (lane == 0) {
         if (p.lse) {
             p.lse[r] = a.s == a.s ? a.top : a.s;
             p.lse[p.rows + r] = none ? 0.0f : log_s;
         }
-        if (p.entropy) p.entropy[r] = none ? 0.0f : (lg2(a.s) - a.s1 / a.s) * kLn2;
+        if (p.entropy) p.entropy[r] = none ? 0.0f : max_nan(fmaf(-a.s1 / S, kLn2, log_s), 0.0f);
         if (p.logprob) {
             const bool ok = target >= 0 && target < p.V;
             p.logprob[r] = !ok ? 0.0f : none ? -INFINITY : (logit - a.top) * p.inv_temp - log_s;

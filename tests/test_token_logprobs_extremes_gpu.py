@@ -1,8 +1,12 @@
-"""Token log probabilities where a row is hard on the arithmetic: very large and very low logits, tiny temperatures.  All against
-the definition in 64 bits.
+"""Token log probabilities where a row is hard on the arithmetic: very large and very low logits, tiny temperatures, one token
+that is all but certain.  All against the definition in 64 bits.
 
 Tolerances.  As beside the ordinary rows: with E = 2^-21 (2 + log V) + 2^-24 (V / 256 + 16), log S is off by E, the entropy by
-E (2 + log V), a log probability by E and 2^-22 of its value."""
+E (2 + log V), a log probability by E and 2^-22 of its value.  For a token that is all but certain the bound is closer, since the
+others carry little weight: its exponent is rounded at no more than 8 or 9 in base 2 (2^-21), two exponentials (2^-22 each) scale it
+and a handful of roundings (2^-24 each) follow, below 2^-19 in all; the entropy's second sum is 8 or 9 times the first before the two
+are subtracted, which adds roundings of 2^-21 each, below 2^-18, and the rest have exponents of up to 100, whose relative error of 2^-17
+weighs as much as they do in the entropy."""
 import math
 
 import numpy as np
@@ -112,3 +116,28 @@ def test_tiny_temperatures(cuda_dev, dt, rows, V, temp):
     t = torch.randint(0, V, (rows,), device=cuda_dev, dtype=torch.int32, generator=g)
     t[::2] = l.float().argmax(1)[::2].int()
     _check(l, t, temp)
+
+
+@pytest.mark.parametrize("dt", DT)
+@pytest.mark.parametrize("rows,V", SIZES)
+@pytest.mark.parametrize("gap", [10, 12, 15, 20, 25, 30, 40])
+def test_one_token_that_is_all_but_certain(cuda_dev, dt, rows, V, gap):
+    """One logit stands above the rest, in the row's later half; no probability is above 1 and no entropy below 0."""
+    import torch
+
+    import mamba_rs_b200 as mb
+    g = torch.Generator(cuda_dev).manual_seed(V + rows + gap)
+    l = torch.randn(rows, V, device=cuda_dev, generator=g) * 2
+    at = torch.randint(V // 2, V, (rows, 1), device=cuda_dev, generator=g)
+    l.scatter_(1, at, l.amax(1, keepdim=True) + gap)
+    l = l.to(_dt(dt))
+    t = at[:, 0].int()
+    log_s, H, logp, lp = _plain(l, t, 1.0)
+    for top in (0, 3):
+        r = mb.token_logprobs(l, t, top=top)
+        assert (r["logprob"] <= 0).all() and (r["entropy"] >= 0).all() and (r["lse"][1] >= 0).all()
+        _close(r["lse"][1], log_s, 2.0 ** -19 * (1 + log_s))
+        _close(r["logprob"], lp, 2.0 ** -19 * (1 + lp.abs()))
+        _close(r["entropy"], H, 2.0 ** -18 + 2.0 ** -17 * H)
+        if top:
+            assert (r["top_logprobs"] <= 0).all() and torch.equal(r["top_ids"][:, 0], t)
