@@ -725,7 +725,9 @@ __global__ void __launch_bounds__(kShortWarps * 32) token_logprobs_short_kernel(
     const int target = target_of(p, r);
     const float logit = target >= 0 && target < p.V ? to_f(row.p[target]) : 0.0f;
     float2 own = Piece<T>::template tops<P>(q);
-    own.x = fmaxf(own.x, head), own.y = fmaxf(own.y, tail);
+    // (A lane that has met nothing but NaN: minus infinity.  As NaN it took the other lane's value in the search for the n-th largest,
+    // and the bound came out too high.)
+    own.x = fmaxf(fmaxf(own.x, head), -INFINITY), own.y = fmaxf(fmaxf(own.y, tail), -INFINITY);
     const float c = p.inv_temp * kLog2e, own_top = fmaxf(own.x, own.y);
     Sums a{own_top, 0.0f, 0.0f, 0.0f};
 #pragma unroll

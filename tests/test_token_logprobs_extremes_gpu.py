@@ -1,5 +1,5 @@
 """Token log probabilities where a row is hard on the arithmetic: very large and very low logits, tiny temperatures, one token
-that is all but certain.  All against the definition in 64 bits.
+that is all but certain, rows that are mostly no numbers.  All against the definition in 64 bits.
 
 Tolerances.  As beside the ordinary rows: with E = 2^-21 (2 + log V) + 2^-24 (V / 256 + 16), log S is off by E, the entropy by
 E (2 + log V), a log probability by E and 2^-22 of its value.  For a token that is all but certain the bound is closer, since the
@@ -141,3 +141,24 @@ def test_one_token_that_is_all_but_certain(cuda_dev, dt, rows, V, gap):
         _close(r["entropy"], H, 2.0 ** -18 + 2.0 ** -17 * H)
         if top:
             assert (r["top_logprobs"] <= 0).all() and torch.equal(r["top_ids"][:, 0], t)
+
+
+@pytest.mark.parametrize("dt", DT)
+def test_alternatives_of_rows_that_are_mostly_no_numbers(cuda_dev, dt):
+    """NaN ranks as minus infinity among the alternatives wherever it lies, in rows that start between 16-byte places too."""
+    import torch
+
+    import mamba_rs_b200 as mb
+    g = torch.Generator(cuda_dev).manual_seed(11)
+    for V, ld, off in ((1024, 1025, 1), (1024, 1031, 3), (512, 513, 1), (2048, 2049, 5), (4096, 4097, 1), (6000, 6001, 1)):
+        rows = 64
+        store = torch.full((rows * ld + off,), math.nan, device=cuda_dev, dtype=_dt(dt))
+        l = store[off:].view(rows, ld)[:, :V]
+        for r in range(rows):
+            n = 1 + r % 12
+            where = torch.randperm(V, device=cuda_dev, generator=g)[:n]
+            l[r, where] = torch.randn(n, device=cuda_dev, generator=g).to(_dt(dt))
+        ranked = torch.where(torch.isnan(l), -math.inf, l.float())
+        for top in (1, 5, 8, 20, 32):
+            order = torch.sort(ranked, dim=1, descending=True, stable=True)[1][:, :top]
+            assert torch.equal(mb.token_logprobs(l, top=top)["top_ids"].long(), order), (V, top)
