@@ -584,7 +584,7 @@ MAMBA_B200_API int mamba_b200_embedding_bwd(void* handle, void* stream, int dtyp
 
 /*
  * Log probabilities of given tokens, entropy and the most likely alternatives, per row of logits [rows, ld] (V used columns,
- * storage dtype); l = logits / temperature, all sums f32.
+ * storage dtype); l = logits / temperature (5e-39 to 3e38), all sums f32.
  *   lse [2, rows]: a row's largest logit M, and log sum exp(l - M / temperature): log sum exp l is M / temperature + the second
  *   logprob[r] = l[targets[r]] - log sum exp l (0 where the target is outside [0, V))
  *   entropy[r] = log sum exp l - sum p l

@@ -1071,6 +1071,9 @@ int logprobs_configure(Ctx* c) {
 
 using namespace mb200;
 
+// The kernels multiply by log2(e) / temperature.
+static bool temperature_ok(float temperature) { return temperature > 0.0f && temperature <= 3e38f && kLog2e / temperature <= 3e38f; }
+
 extern "C" MAMBA_B200_API int mamba_b200_token_logprobs(void* handle, void* stream, int dtype, const void* logits, long long ld,
                                                         const int* targets, float temperature, float* lse, float* entropy,
                                                         float* logprob, int top, int* top_ids, float* top_logprobs, long long rows,
@@ -1079,7 +1082,7 @@ extern "C" MAMBA_B200_API int mamba_b200_token_logprobs(void* handle, void* stre
     if (!c) return MAMBA_B200_ERR_ARG;
     if (!dtype_ok(dtype)) return fail(c, MAMBA_B200_ERR_ARG, "token_logprobs: bad dtype %d", dtype);
     if (rows < 0 || V <= 0 || ld < V) return fail(c, MAMBA_B200_ERR_ARG, "token_logprobs: bad dims");
-    if (!(temperature > 0.0f) || temperature > 3e38f || 1.0f / temperature > 3e38f) return fail(c, MAMBA_B200_ERR_ARG, "token_logprobs: temperature %g", temperature);
+    if (!temperature_ok(temperature)) return fail(c, MAMBA_B200_ERR_ARG, "token_logprobs: temperature %g", temperature);
     if (top < 0 || top > lp::kMaxTop || top > V)
         return fail(c, MAMBA_B200_ERR_SHAPE, "token_logprobs: %d alternatives of %d tokens (at most %d)", top, V, lp::kMaxTop);
     if (rows == 0) return MAMBA_B200_OK;
@@ -1102,7 +1105,7 @@ extern "C" MAMBA_B200_API int mamba_b200_token_logprobs_bwd(void* handle, void* 
     if (!c) return MAMBA_B200_ERR_ARG;
     if (!dtype_ok(dtype)) return fail(c, MAMBA_B200_ERR_ARG, "token_logprobs_bwd: bad dtype %d", dtype);
     if (rows < 0 || V <= 0 || ld < V || ld_d < V) return fail(c, MAMBA_B200_ERR_ARG, "token_logprobs_bwd: bad dims");
-    if (!(temperature > 0.0f) || temperature > 3e38f || 1.0f / temperature > 3e38f) return fail(c, MAMBA_B200_ERR_ARG, "token_logprobs_bwd: temperature %g", temperature);
+    if (!temperature_ok(temperature)) return fail(c, MAMBA_B200_ERR_ARG, "token_logprobs_bwd: temperature %g", temperature);
     if (rows == 0) return MAMBA_B200_OK;
     if (rows > 2147483647ll) return fail(c, MAMBA_B200_ERR_SHAPE, "token_logprobs_bwd: too many rows");
     if (!logits || !lse || !dlogits || (d_logprob && !targets) || (d_entropy && !entropy))

@@ -162,3 +162,19 @@ def test_alternatives_of_rows_that_are_mostly_no_numbers(cuda_dev, dt):
         for top in (1, 5, 8, 20, 32):
             order = torch.sort(ranked, dim=1, descending=True, stable=True)[1][:, :top]
             assert torch.equal(mb.token_logprobs(l, top=top)["top_ids"].long(), order), (V, top)
+
+
+def test_temperatures_whose_reciprocal_leaves_the_range_are_refused(cuda_dev):
+    """log2(e) / temperature has to be a number of 32 bits."""
+    import torch
+
+    import mamba_rs_b200 as mb
+    l, t = torch.zeros(2, 40, device=cuda_dev), torch.zeros(2, dtype=torch.int32, device=cuda_dev)
+    v, v2 = torch.zeros(2, device=cuda_dev), torch.zeros(2, 2, device=cuda_dev)
+    for temp in (4e-39, 3.5e-39, 1e-44):
+        with pytest.raises(RuntimeError, match="temperature"):
+            mb.token_logprobs(l, t, temperature=temp)
+        with pytest.raises(RuntimeError, match="temperature"):
+            mb.token_logprobs_bwd(l, t, v2, v, v, temperature=temp)
+    r = mb.token_logprobs(l, t, temperature=5e-39)
+    assert (r["lse"][1] - math.log(40)).abs().max() <= 2.0 ** -19
