@@ -1,9 +1,11 @@
 // Gated linear recurrence, elementwise over channels:
 //   u_t = sigmoid(-f_t)      h_t = h_{t-1} + u_t (x_t - h_{t-1})      y_t = h_t * SiLU(z_t)
-// that is h_t = a_t h_{t-1} + (1 - a_t) x_t with the forget gate a = sigmoid(f) = 1 - u.  Written with u, a channel that
-// forgets slowly (u near 0) keeps u's relative precision; a rounded to 1 - 2^-24 would not.
+// that is h_t = a_t h_{t-1} + (1 - a_t) x_t with the forget gate a = sigmoid(f) = 1 - u.
 //   backward  g_t = dy_t SiLU(z_t) + (1 - u_{t+1}) g_{t+1}
 //             d_x = u g      d_f = g (h_{t-1} - x) u (1 - u)      d_z = dy h SiLU'(z)
+// A channel that forgets slowly has u near 0, and 1 - u rounded would lose it; one that forgets fast has 1 - u near 0, and loses
+// that where only u is kept (6 % of it at f = -16, all at -17: a d_f of 0, and an error of 2^-25 of any earlier state in every
+// later one).  So both are made, and a gate in one number is the smaller one, with a sign that says which it is: c = -u or 1 - u.
 #include <string.h>
 
 #include "common.cuh"
@@ -39,20 +41,55 @@ __device__ __forceinline__ Ch<2> add(Ch<2> a, Ch<2> b) { return {add2(a.a, b.a)}
 // a - b; the packed instructions have no signs of their own, so it is a product with -1.
 template <int V> __device__ __forceinline__ Ch<V> sub(Ch<V> a, Ch<V> b) { return fma(b, Ch<V>::splat(-1.0f), a); }
 
-// -1 / (1 + 2^(v k)): with k = log2 e the negative of u = sigmoid(-v), with -log2 e that of sigmoid(v).  The negative, because
-// everything it meets is then one packed fma: h - u (h - x) = fma(-u, h - x, h).
-template <int V> __device__ __forceinline__ Ch<V> neg_gate(Ch<V> v, float k) {
-    const Ch<V> t = mul(v, Ch<V>::splat(k)).map(ex2), m = Ch<V>::splat(-1.0f);
-    return fma(t, m, m).map(rcp);
+template <int V> __device__ __forceinline__ Ch<V> sigmoid(Ch<V> v) {
+    return add(mul(v, Ch<V>::splat(-kLog2e)).map(ex2), Ch<V>::splat(1.0f)).map(rcp);
 }
-// A span of steps acts on a state as h -> h - U h + A.  span(h) with n = -U:
-template <int V> __device__ __forceinline__ Ch<V> over(Ch<V> n, Ch<V> a, Ch<V> h) { return add(fma(n, h, h), a); }
-// n of a span and one that follows it.
-template <int V> __device__ __forceinline__ Ch<V> both(Ch<V> n, Ch<V> m) { return fma(m, add(Ch<V>::splat(1.0f), n), n); }
+// By a sign (-0 has one).
+__device__ __forceinline__ float pick(float sign, float minus, float plus) { return __float_as_int(sign) < 0 ? minus : plus; }
+__device__ __forceinline__ Ch<1> pick(Ch<1> sign, Ch<1> minus, Ch<1> plus) { return {pick(sign.a, minus.a, plus.a)}; }
+__device__ __forceinline__ Ch<2> pick(Ch<2> sign, Ch<2> minus, Ch<2> plus) {
+    return {make_float2(pick(sign.a.x, minus.a.x, plus.a.x), pick(sign.a.y, minus.a.y, plus.a.y))};
+}
+// u and p = 1 - u, each to its own last places, from f (t = 2^(f log2 e), u = 1 / (1 + t), p = t u or, where t is above 1, 1 - u) or
+// from c.
+template <int V> struct Gate {
+    Ch<V> u, p;
+    __device__ __forceinline__ static Gate of(Ch<V> f) {
+        const Ch<V> one = Ch<V>::splat(1.0f), t = mul(f, Ch<V>::splat(kLog2e)).map(ex2), u = add(t, one).map(rcp);
+        return {u, pick(f, mul(t, u), sub(one, u))};
+    }
+    __device__ __forceinline__ static Gate from(Ch<V> c) {
+        const Ch<V> s = c.map([](float v) { return fabsf(v); }), rest = sub(Ch<V>::splat(1.0f), s);
+        return {pick(c, s, rest), pick(c, rest, s)};
+    }
+    // (A channel that keeps everything is -0.)
+    __device__ __forceinline__ Ch<V> small() const {
+        if constexpr (V == 1) return {u.a < 0.5f ? -u.a : p.a};
+        else return {make_float2(u.a.x < 0.5f ? -u.a.x : p.a.x, u.a.y < 0.5f ? -u.a.y : p.a.y)};
+    }
+    // The gate of this span of steps and one more, or another span, behind it: u is a sum of positive terms, so it keeps its relative
+    // precision as p does.
+    __device__ __forceinline__ void grow(const Gate& next) {
+        u = fma(next.u, p, u);
+        p = mul(p, next.p);
+    }
+};
+template <int V> __device__ __forceinline__ Gate<V> no_steps() { return {Ch<V>::splat(0.0f), Ch<V>::splat(1.0f)}; }
+// h + u (x - h) = x + p (h - x).  (p h + u x would round p, the same way at every step: a state that lives for a million steps
+// would drift by 3 %.  Over the 16 steps of a span that is 2^-21, and spans are joined by over.)
+template <int V> __device__ __forceinline__ Ch<V> step(Ch<V> c, Ch<V> h, Ch<V> x) { return fma(c, sub(h, x), pick(c, h, x)); }
+// A span of steps acts on a state as h -> p h + A; its gate is written by c too: h - u h or p h.
+template <int V> __device__ __forceinline__ Ch<V> over(Ch<V> c, Ch<V> a, Ch<V> h) { return add(fma(c, h, pick(c, h, Ch<V>::splat(0.0f))), a); }
+template <int V> __device__ __forceinline__ Ch<V> both(Ch<V> c, Ch<V> d) {
+    Gate<V> g = Gate<V>::from(c);
+    g.grow(Gate<V>::from(d));
+    return g.small();
+}
+constexpr float kKeeps = -0.0f;  // the gate of no steps
 
-template <int V> __device__ __forceinline__ Ch<V> get(const float* row, int c, int D) {
-    if constexpr (V == 1) return {c < D ? row[c] : 0.0f};
-    else return {make_float2(c < D ? row[c] : 0.0f, c + 1 < D ? row[c + 1] : 0.0f)};
+template <int V> __device__ __forceinline__ Ch<V> get(const float* row, int c, int D, float none = 0.0f) {
+    if constexpr (V == 1) return {c < D ? row[c] : none};
+    else return {make_float2(c < D ? row[c] : none, c + 1 < D ? row[c + 1] : none)};
 }
 __device__ __forceinline__ void put(float* row, int c, int D, Ch<1> v) {
     if (c < D) row[c] = v.a;
@@ -64,7 +101,7 @@ __device__ __forceinline__ void put(float* row, int c, int D, Ch<2> v) {
 struct Params {
     mamba_b200_gated_scan_args a;
     int* status;
-    float* sums;  // [B, segments, 2, D]: what each segment does to the state (or gradient) that enters it
+    float* sums;  // [B, segments, 2, D]: what each segment does to the state (or gradient) that enters it: its gate, and what it adds
     int tiles, segments, per_segment, tma_out, stages;
 };
 
@@ -171,14 +208,14 @@ __device__ __forceinline__ Ch<V> enter(const Params& p, float* part, int b, int 
     constexpr int CH = 32 * V;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, n = (to - from) * step, per = (n + kWarps - 1) / kWarps;
     asm volatile("griddepcontrol.wait;" ::: "memory");
-    C N = C::splat(0.0f), A = C::splat(0.0f);
+    C N = C::splat(kKeeps), A = C::splat(0.0f);
     for (int i0 = warp * per; i0 < min(n, (warp + 1) * per); i0 += 8) {
         C m[8], a[8];
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
             const bool ok = i0 + i < min(n, (warp + 1) * per);
             const float* row = p.sums + (static_cast<long long>(b) * p.segments + (ok ? from + (i0 + i) * step : 0)) * 2 * p.a.D;
-            m[i] = get<V>(row, ok ? c : p.a.D, p.a.D);
+            m[i] = get<V>(row, ok ? c : p.a.D, p.a.D, kKeeps);
             a[i] = get<V>(row + p.a.D, ok ? c : p.a.D, p.a.D);
         }
 #pragma unroll
@@ -235,8 +272,9 @@ __global__ void __launch_bounds__(kFwdWarps * 32, kFwdCtas)
     uint32_t parity = 0;
     for (int it = 0; it < rounds; ++it) {
         const int k = first + it;
-        // what the steps up to each one do to the state that enters the span, and the output gates
-        C n[L], a[L], q[GATE ? L : 1], N = C::splat(0.0f), A = C::splat(0.0f);
+        // what each step keeps and adds, the output gates, and what the span does to the state that enters it
+        C kept[L], added[L], q[GATE ? L : 1], A = C::splat(0.0f);
+        Gate<V> span = no_steps<V>();
         if constexpr (PLAIN) {
             in.hand_over(next_rows, s);
             if (it + 1 < rounds) in.fetch(next_rows, k + 1, src, ld);
@@ -246,19 +284,21 @@ __global__ void __launch_bounds__(kFwdWarps * 32, kFwdCtas)
         const T *sf = in.mine(s, 0), *sx = in.mine(s, 1), *sz = in.mine(s, NIN - 1);
 #pragma unroll
         for (int j = 0; j < L; ++j) {
-            const C u = neg_gate(C::load(sf + j * CH), kLog2e);
-            a[j] = A = fma(u, sub(A, C::load(sx + j * CH)), A);
-            n[j] = N = both(N, u);
+            const Gate<V> g = Gate<V>::of(C::load(sf + j * CH));
+            kept[j] = g.p;
+            added[j] = mul(g.u, C::load(sx + j * CH));
+            A = fma(g.p, A, added[j]);
+            span.grow(g);
             if constexpr (GATE) {
                 const C z = C::load(sz + j * CH);
-                q[j] = mul(z, neg_gate(z, -kLog2e));  // -SiLU(z)
+                q[j] = mul(z, sigmoid(z));  // SiLU(z)
             }
         }
         // the sums go where the warp's rows of f were: two rows of 4-byte channels
         float* part = reinterpret_cast<float*>(in.at(s, 0));
         constexpr int kStep = L * CH * sizeof(T) / sizeof(float);
         __syncwarp();
-        N.store(part + warp * kStep + lane * V);
+        span.small().store(part + warp * kStep + lane * V);
         A.store(part + warp * kStep + CH + lane * V);
         __syncthreads();
         C h = carry;
@@ -269,12 +309,11 @@ __global__ void __launch_bounds__(kFwdWarps * 32, kFwdCtas)
         }
         if (p.a.chunk_states && warp == 0) put(p.a.chunk_states + (static_cast<long long>(b) * p.tiles + k) * D, c, D, carry);
         T* sy = in.mine(s, 1);
-        const C minus = C::splat(-1.0f);
 #pragma unroll
         for (int j = 0; j < L; ++j) {
-            const C o = over(n[j], a[j], carry);
-            if constexpr (GATE) mul(o, mul(q[j], minus)).store(sy + j * CH);
-            else o.store(sy + j * CH);
+            carry = fma(kept[j], carry, added[j]);
+            if constexpr (GATE) mul(carry, q[j]).store(sy + j * CH);
+            else carry.store(sy + j * CH);
         }
         carry = h;
         fence_proxy_async();
@@ -293,8 +332,8 @@ __global__ void __launch_bounds__(kFwdWarps * 32, kFwdCtas)
 }
 
 // The gradient walks the tiles from the last to the first.  The states inside a tile come from the saved one that enters it, by
-// the same two walks; g is joined over the warps (and the cluster) the same way in the other direction: over a span of steps
-// (1 - u) g at its first step = g_behind - U g_behind + G, with the forward's U.  g runs with its sign turned, like the gates.
+// the same two walks; g is joined over the warps the same way in the other direction: over a span of steps (1 - u) g at its first
+// step = P g_behind + G, with the forward's P.
 template <typename T, int V, bool GATE, bool PLAIN>
 __global__ void __launch_bounds__(kBwdWarps * 32, 3)
     gated_scan_bwd_kernel(const __grid_constant__ CUtensorMap mf, const __grid_constant__ CUtensorMap mx, const __grid_constant__ CUtensorMap me,
@@ -323,13 +362,13 @@ __global__ void __launch_bounds__(kBwdWarps * 32, 3)
     const void* src[4] = {p.a.f, p.a.x, p.a.dy, p.a.z};
     const long long ld[4] = {p.a.ld_f, p.a.ld_x, p.a.ld_dy, p.a.ld_z};
     const int first = min((seg + 1) * p.per_segment, p.tiles) - 1, rounds = first + 1 - seg * p.per_segment;
-    const C minus = C::splat(-1.0f);
+    const C one = C::splat(1.0f), minus = C::splat(-1.0f);
     for (int i = 0; i < min(S - 1, rounds); ++i) in.ask(i, first - i, maps);
     typename In::Word next_rows[PLAIN ? NIN : 1][L];
     if (PLAIN && rounds > 0) in.fetch(next_rows, first, src, ld);
     C carry = C::splat(0.0f);
     if (p.segments > 1) carry = enter<V, W>(p, part, b, c, 0, p.segments - 1, seg, -1);
-    else if (p.a.d_last) carry = mul(get<V>(p.a.d_last + static_cast<long long>(b) * D, c, D), minus);
+    else if (p.a.d_last) carry = get<V>(p.a.d_last + static_cast<long long>(b) * D, c, D);
     const float* states = p.a.chunk_states + static_cast<long long>(b) * p.tiles * D;
     auto state = [&](int k) { return k >= 0 ? get<V>(states + static_cast<long long>(k) * D, c, D) : C::splat(0.0f); };
     C next = state(first);
@@ -339,7 +378,8 @@ __global__ void __launch_bounds__(kBwdWarps * 32, 3)
         const int k = first - it;
         C h = next;
         next = state(k - 1);
-        C n[L], x[L], e[L], q[L], N = C::splat(0.0f), A = C::splat(0.0f), G = C::splat(0.0f);
+        C n[L], x[L], e[L], q[L], A = C::splat(0.0f), G = C::splat(0.0f);
+        Gate<V> span = no_steps<V>();
         if constexpr (PLAIN) {
             in.hand_over(next_rows, s);
             if (it + 1 < rounds) in.fetch(next_rows, k - 1, src, ld);
@@ -349,25 +389,21 @@ __global__ void __launch_bounds__(kBwdWarps * 32, 3)
         const T *sf = in.mine(s, 0), *sx = in.mine(s, 1), *se = in.mine(s, 2), *sz = in.mine(s, NIN - 1);
 #pragma unroll
         for (int j = 0; j < L; ++j) {
-            n[j] = neg_gate(C::load(sf + j * CH), kLog2e);
+            const C f = C::load(sf + j * CH);
+            const Gate<V> gate = Gate<V>::of(f);
+            n[j] = pick(f, gate.p, mul(gate.u, minus));
             x[j] = C::load(sx + j * CH);
-            const C dy = C::load(se + j * CH);
+            e[j] = C::load(se + j * CH);
             if constexpr (GATE) {
-                const C z = C::load(sz + j * CH), m = neg_gate(z, -kLog2e);  // -sigmoid(z)
-                q[j] = mul(dy, mul(m, fma(z, fma(m, minus, minus), minus)));  // dy SiLU'(z) = dy sigmoid (1 + z (1 - sigmoid))
-                e[j] = mul(dy, mul(z, m));                                    // -dy SiLU(z)
-            } else {
-                e[j] = mul(dy, minus);
+                const C z = C::load(sz + j * CH), m = sigmoid(z), dm = mul(e[j], m);
+                q[j] = mul(dm, fma(z, fma(m, minus, one), one));  // dy SiLU'(z) = dy sigmoid (1 + z (1 - sigmoid))
+                e[j] = mul(dm, z);                                // dy SiLU(z)
             }
-            A = fma(n[j], sub(A, x[j]), A);
-            N = both(N, n[j]);
+            A = fma(gate.p, A, mul(gate.u, x[j]));
+            span.grow(gate);
+            G = fma(span.p, e[j], G);
         }
-#pragma unroll
-        for (int j = L - 1; j >= 0; --j) {
-            const C g = add(e[j], G);
-            G = fma(n[j], g, g);
-        }
-        N.store(part + warp * CH + lane * V);
+        span.small().store(part + warp * CH + lane * V);
         A.store(part + (W + warp) * CH + lane * V);
         G.store(part + (2 * W + warp) * CH + lane * V);
         __syncthreads();
@@ -385,17 +421,19 @@ __global__ void __launch_bounds__(kBwdWarps * 32, 3)
         T *df = in.mine(s, 0), *dx = in.mine(s, 1), *dz = in.mine(s, NIN - 1);
 #pragma unroll
         for (int j = 0; j < L; ++j) {
+            const C to = pick(n[j], h, x[j]);
             x[j] = sub(h, x[j]);  // h_{t-1} - x_t
-            h = fma(n[j], x[j], h);
+            h = fma(n[j], x[j], to);
             if constexpr (GATE) mul(q[j], h).store(dz + j * CH);
         }
         g = start;
 #pragma unroll
         for (int j = L - 1; j >= 0; --j) {
+            const Gate<V> gate = Gate<V>::from(n[j]);
             g = add(g, e[j]);
-            mul(g, n[j]).store(dx + j * CH);
-            g = fma(n[j], g, g);
-            mul(x[j], mul(n[j], g)).store(df + j * CH);
+            mul(gate.u, g).store(dx + j * CH);
+            g = mul(gate.p, g);
+            mul(x[j], mul(gate.u, g)).store(df + j * CH);
         }
         fence_proxy_async();
         if (!p.tma_out) {
@@ -412,7 +450,7 @@ __global__ void __launch_bounds__(kBwdWarps * 32, 3)
         }
         if (++s == S) s = 0, parity ^= 1;
     }
-    if (p.a.d_h0 && seg == 0 && warp == 0) put(p.a.d_h0 + static_cast<long long>(b) * D, c, D, mul(carry, minus));
+    if (p.a.d_h0 && seg == 0 && warp == 0) put(p.a.d_h0 + static_cast<long long>(b) * D, c, D, carry);
     if (p.tma_out && threadIdx.x == 0) tma_wait_read0();
 }
 
@@ -445,39 +483,39 @@ __global__ void __launch_bounds__(kSumWarps * 32) gated_scan_sums_kernel(const _
                 for (int e = 0; e < V; ++e) to[j].v[e] = t0 + j < p.a.T && c + e < D ? row[j * ld + e] : from_f<T>(none);
         }
     };
-    C N = C::splat(0.0f), A = C::splat(0.0f);
+    C N = C::splat(kKeeps), A = C::splat(0.0f);
     for (int i = 0; i < hi - lo; ++i) {
         const int t0 = (BWD ? lo + i : hi - 1 - i) * L;
         Word fw[L], xw[L], zw[L];
         fetch(fw, p.a.f, p.a.ld_f, t0, INFINITY);
         fetch(xw, BWD ? p.a.dy : p.a.x, BWD ? p.a.ld_dy : p.a.ld_x, t0, 0.0f);
         if constexpr (BWD && GATE) fetch(zw, p.a.z, p.a.ld_z, t0, 0.0f);
-        C n1 = C::splat(0.0f), a1 = C::splat(0.0f);
+        C a1 = C::splat(0.0f);
+        Gate<V> span = no_steps<V>();
 #pragma unroll
         for (int jj = 0; jj < L; ++jj) {
             const int j = BWD ? L - 1 - jj : jj;
-            const C m = neg_gate(C::load(fw[j].v), kLog2e), x = C::load(xw[j].v);
+            const Gate<V> gate = Gate<V>::of(C::load(fw[j].v));
+            C x = C::load(xw[j].v);
             if constexpr (BWD) {
-                C e = mul(x, C::splat(-1.0f));
                 if constexpr (GATE) {
                     const C z = C::load(zw[j].v);
-                    e = mul(x, mul(z, neg_gate(z, -kLog2e)));
+                    x = mul(x, mul(z, sigmoid(z)));
                 }
-                const C g = add(e, a1);
-                a1 = fma(m, g, g);
+                a1 = mul(gate.p, add(x, a1));
             } else {
-                a1 = fma(m, sub(a1, x), a1);
+                a1 = fma(gate.p, a1, mul(gate.u, x));
             }
-            n1 = both(n1, m);
+            span.grow(gate);
         }
         A = over(N, A, a1);  // this piece is met before those that are there
-        N = both(n1, N);
+        N = both(span.small(), N);
     }
     N.store(part + warp * CH + lane * V);
     A.store(part + (kWarps + warp) * CH + lane * V);
     __syncthreads();
     if (warp != 0) return;
-    N = C::splat(0.0f), A = C::splat(0.0f);
+    N = C::splat(kKeeps), A = C::splat(0.0f);
 #pragma unroll
     for (int i = 0; i < kWarps; ++i) {
         const int w = BWD ? kWarps - 1 - i : i;
@@ -494,7 +532,7 @@ __global__ void __launch_bounds__(kSumWarps * 32) gated_scan_sums_kernel(const _
     if (seg == (BWD ? 1 : 0)) {
         const float* from = BWD ? p.a.d_last : p.a.h0;
         const C v = from ? get<V>(from + static_cast<long long>(b) * D, c, D) : C::splat(0.0f);
-        put(p.sums + (static_cast<long long>(b) * p.segments + (BWD ? 0 : p.segments - 1)) * 2 * D, c, D, BWD ? mul(v, C::splat(-1.0f)) : v);
+        put(p.sums + (static_cast<long long>(b) * p.segments + (BWD ? 0 : p.segments - 1)) * 2 * D, c, D, v);
     }
 }
 
@@ -521,7 +559,7 @@ __global__ void __launch_bounds__(128) gated_scan_short_kernel(const mamba_b200_
 #pragma unroll
     for (int t = 0; t < kShort; ++t) {
         if (t >= p.T) break;
-        h = fmaf(rcp(1.0f + ex2(fv[t] * kLog2e)), xv[t] - h, h);
+        h = step(Gate<1>::of({fv[t]}).small(), {h}, {xv[t]}).a;
         y[t * p.ld_y] = from_f<T>(z ? h * siluf_fast(zv[t]) : h);
     }
     if (p.h_last) p.h_last[i] = h;
