@@ -673,7 +673,7 @@ extern "C" MAMBA_B200_API int mamba_b200_embedding_fwd(void* handle, void* strea
         return fail(c, MAMBA_B200_ERR_ARG, "embedding_fwd: rows come out as f32 or in the table's dtype, not %d", out_dtype);
     if (rows < 0 || dim <= 0 || vocab <= 0 || ld_table < dim || ld_out < dim) return fail(c, MAMBA_B200_ERR_ARG, "embedding_fwd: bad dims");
     if (rows == 0) return MAMBA_B200_OK;
-    if (rows > 2147483647ll * 8 / ((dim + 255) / 256)) return fail(c, MAMBA_B200_ERR_SHAPE, "embedding_fwd: too many rows");
+    if (dim > kMaxSize || rows > 2147483647ll * 8 / ((dim + 255) / 256)) return fail(c, MAMBA_B200_ERR_SHAPE, "embedding_fwd: too many rows or columns");
     if (!table || !ids || !out) return fail(c, MAMBA_B200_ERR_ARG, "embedding_fwd: null pointer");
     const emb::FwdParams p{table, ids, out, ld_table, ld_out, rows, dim, vocab, scale};
     cudaStream_t st = static_cast<cudaStream_t>(stream);
@@ -697,7 +697,7 @@ extern "C" MAMBA_B200_API int mamba_b200_embedding_bwd(void* handle, void* strea
     if (!c) return MAMBA_B200_ERR_ARG;
     if (!dtype_ok(dtype)) return fail(c, MAMBA_B200_ERR_ARG, "embedding_bwd: bad dtype %d", dtype);
     if (rows < 0 || dim <= 0 || vocab <= 0 || ld_dout < dim) return fail(c, MAMBA_B200_ERR_ARG, "embedding_bwd: bad dims");
-    if (rows > 2147483647ll - 1024 || dim > 32 * 65535 || vocab > 2147483647 - 1024)
+    if (rows > kMaxSize || dim > 32 * 65535 || vocab > kMaxSize)
         return fail(c, MAMBA_B200_ERR_SHAPE, "embedding_bwd: too many rows, columns or tokens");
     if (!d_table || (rows && (!d_out || !ids))) return fail(c, MAMBA_B200_ERR_ARG, "embedding_bwd: null pointer");
     if (rows == 0 && accumulate) return MAMBA_B200_OK;

@@ -569,6 +569,7 @@ static int check(Ctx* c, const mamba_b200_gated_scan_args* a, bool bwd) {
     const char* fn = bwd ? "gated_scan_bwd" : "gated_scan_fwd";
     if (!dtype_ok(a->dtype)) return fail(c, MAMBA_B200_ERR_ARG, "%s: bad dtype %d", fn, a->dtype);
     if (a->B < 0 || a->T < 0 || a->D <= 0) return fail(c, MAMBA_B200_ERR_ARG, "%s: bad dims", fn);
+    if (a->T > kMaxSize || a->D > kMaxSize) return fail(c, MAMBA_B200_ERR_SHAPE, "%s: too many steps or channels", fn);
     if (a->ld_x < a->D || a->ld_f < a->D || (a->z && a->ld_z < a->D)) return fail(c, MAMBA_B200_ERR_ARG, "%s: row stride below D", fn);
     if (a->B == 0) return MAMBA_B200_OK;
     if (a->T && (!a->x || !a->f)) return fail(c, MAMBA_B200_ERR_ARG, "%s: null pointer", fn);
@@ -687,7 +688,7 @@ int gated_scan_configure(Ctx* c) {
 using namespace mb200;
 
 extern "C" MAMBA_B200_API long long mamba_b200_gated_scan_workspace_bytes(int B, int T, int D) {
-    if (B <= 0 || T <= gs::kShort || D <= 0) return 0;
+    if (B <= 0 || T <= gs::kShort || D <= 0 || T > kMaxSize || D > kMaxSize) return 0;
     // (strips of 64 channels, or of 32: the more segments of the two; sized for 148 SMs, which a launch on fewer only halves further)
     const int segments = gs::pick_segments(148, static_cast<long long>(B) * ((D + 63) / 64), (T + gs::kTile - 1) / gs::kTile, false);
     return segments > 1 ? static_cast<long long>(segments) * B * D * 2 * sizeof(float) : 0;

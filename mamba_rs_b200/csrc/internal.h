@@ -29,6 +29,8 @@ inline int fail(Ctx* c, int code, const char* fmt, ...) {
     return code;
 }
 
+// Sizes that kernels step over in 32 bits end here: the largest step of a loop fits behind it.
+constexpr int kMaxSize = 2147483647 - 65536;
 inline size_t dtype_size(int dtype) { return dtype == MAMBA_B200_F32 ? 4 : 2; }
 inline bool dtype_ok(int dtype) {
     return dtype == MAMBA_B200_F32 || dtype == MAMBA_B200_F16 || dtype == MAMBA_B200_BF16;

@@ -1086,7 +1086,7 @@ extern "C" MAMBA_B200_API int mamba_b200_token_logprobs(void* handle, void* stre
     if (top < 0 || top > lp::kMaxTop || top > V)
         return fail(c, MAMBA_B200_ERR_SHAPE, "token_logprobs: %d alternatives of %d tokens (at most %d)", top, V, lp::kMaxTop);
     if (rows == 0) return MAMBA_B200_OK;
-    if (rows > 2147483647ll) return fail(c, MAMBA_B200_ERR_SHAPE, "token_logprobs: too many rows");
+    if (rows > 2147483647ll || V > kMaxSize) return fail(c, MAMBA_B200_ERR_SHAPE, "token_logprobs: too many rows or tokens");
     if (!logits || (logprob && !targets) || (top && (!top_ids || !top_logprobs)))
         return fail(c, MAMBA_B200_ERR_ARG, "token_logprobs: null pointer");
     if (reinterpret_cast<uintptr_t>(logits) % dtype_size(dtype)) return fail(c, MAMBA_B200_ERR_ARG, "token_logprobs: misaligned logits");
@@ -1107,7 +1107,7 @@ extern "C" MAMBA_B200_API int mamba_b200_token_logprobs_bwd(void* handle, void* 
     if (rows < 0 || V <= 0 || ld < V || ld_d < V) return fail(c, MAMBA_B200_ERR_ARG, "token_logprobs_bwd: bad dims");
     if (!temperature_ok(temperature)) return fail(c, MAMBA_B200_ERR_ARG, "token_logprobs_bwd: temperature %g", temperature);
     if (rows == 0) return MAMBA_B200_OK;
-    if (rows > 2147483647ll) return fail(c, MAMBA_B200_ERR_SHAPE, "token_logprobs_bwd: too many rows");
+    if (rows > 2147483647ll || V > kMaxSize) return fail(c, MAMBA_B200_ERR_SHAPE, "token_logprobs_bwd: too many rows or tokens");
     if (!logits || !lse || !dlogits || (d_logprob && !targets) || (d_entropy && !entropy))
         return fail(c, MAMBA_B200_ERR_ARG, "token_logprobs_bwd: null pointer");
     if ((reinterpret_cast<uintptr_t>(logits) | reinterpret_cast<uintptr_t>(dlogits)) % dtype_size(dtype))
