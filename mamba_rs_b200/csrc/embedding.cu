@@ -674,6 +674,8 @@ extern "C" MAMBA_B200_API int mamba_b200_embedding_fwd(void* handle, void* strea
     if (rows < 0 || dim <= 0 || vocab <= 0 || ld_table < dim || ld_out < dim) return fail(c, MAMBA_B200_ERR_ARG, "embedding_fwd: bad dims");
     if (rows == 0) return MAMBA_B200_OK;
     if (dim > kMaxSize || rows > 2147483647ll * 8 / ((dim + 255) / 256)) return fail(c, MAMBA_B200_ERR_SHAPE, "embedding_fwd: too many rows or columns");
+    if (!aligned_to(dtype_size(dtype), {table}) || !aligned_to(dtype_size(out_dtype), {out}) || !aligned_to(4, {ids}))
+        return fail(c, MAMBA_B200_ERR_ARG, "embedding_fwd: misaligned pointer");
     if (!table || !ids || !out) return fail(c, MAMBA_B200_ERR_ARG, "embedding_fwd: null pointer");
     const emb::FwdParams p{table, ids, out, ld_table, ld_out, rows, dim, vocab, scale};
     cudaStream_t st = static_cast<cudaStream_t>(stream);
@@ -699,6 +701,7 @@ extern "C" MAMBA_B200_API int mamba_b200_embedding_bwd(void* handle, void* strea
     if (rows < 0 || dim <= 0 || vocab <= 0 || ld_dout < dim) return fail(c, MAMBA_B200_ERR_ARG, "embedding_bwd: bad dims");
     if (rows > kMaxSize || dim > 32 * 65535 || vocab > kMaxSize)
         return fail(c, MAMBA_B200_ERR_SHAPE, "embedding_bwd: too many rows, columns or tokens");
+    if (!aligned_to(dtype_size(dtype), {d_out}) || !aligned_to(4, {ids, d_table})) return fail(c, MAMBA_B200_ERR_ARG, "embedding_bwd: misaligned pointer");
     if (!d_table || (rows && (!d_out || !ids))) return fail(c, MAMBA_B200_ERR_ARG, "embedding_bwd: null pointer");
     if (rows == 0 && accumulate) return MAMBA_B200_OK;
     const emb::Room r = emb::room_of(rows, dim, vocab);

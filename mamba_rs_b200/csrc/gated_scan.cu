@@ -572,6 +572,11 @@ static int check(Ctx* c, const mamba_b200_gated_scan_args* a, bool bwd) {
     if (a->T > kMaxSize || a->D > kMaxSize) return fail(c, MAMBA_B200_ERR_SHAPE, "%s: too many steps or channels", fn);
     if (a->ld_x < a->D || a->ld_f < a->D || (a->z && a->ld_z < a->D)) return fail(c, MAMBA_B200_ERR_ARG, "%s: row stride below D", fn);
     if (a->B == 0) return MAMBA_B200_OK;
+    const size_t n = dtype_size(a->dtype);
+    const bool aligned = aligned_to(n, {a->x, a->f, a->z}) && aligned_to(4, {a->chunk_states}) &&
+                         (bwd ? aligned_to(n, {a->dy, a->d_x, a->d_f, a->d_z}) && aligned_to(4, {a->d_last, a->d_h0})
+                              : aligned_to(n, {a->y}) && aligned_to(4, {a->h0, a->h_last}));
+    if (!aligned) return fail(c, MAMBA_B200_ERR_ARG, "%s: misaligned pointer", fn);
     if (a->T && (!a->x || !a->f)) return fail(c, MAMBA_B200_ERR_ARG, "%s: null pointer", fn);
     if (!bwd) {
         if (a->ld_y < a->D) return fail(c, MAMBA_B200_ERR_ARG, "%s: row stride below D", fn);

@@ -7,6 +7,8 @@
 #include <stdint.h>
 #include <stdio.h>
 
+#include <initializer_list>
+
 #include "../../include/mamba_b200.h"
 
 namespace mb200 {
@@ -32,6 +34,12 @@ inline int fail(Ctx* c, int code, const char* fmt, ...) {
 // Sizes that kernels step over in 32 bits end here: the largest step of a loop fits behind it.
 constexpr int kMaxSize = 2147483647 - 65536;
 inline size_t dtype_size(int dtype) { return dtype == MAMBA_B200_F32 ? 4 : 2; }
+// All at multiples of n bytes (null pointers are).
+inline bool aligned_to(size_t n, std::initializer_list<const void*> pointers) {
+    for (const void* p : pointers)
+        if (reinterpret_cast<uintptr_t>(p) % n) return false;
+    return true;
+}
 inline bool dtype_ok(int dtype) {
     return dtype == MAMBA_B200_F32 || dtype == MAMBA_B200_F16 || dtype == MAMBA_B200_BF16;
 }

@@ -1087,9 +1087,10 @@ extern "C" MAMBA_B200_API int mamba_b200_token_logprobs(void* handle, void* stre
         return fail(c, MAMBA_B200_ERR_SHAPE, "token_logprobs: %d alternatives of %d tokens (at most %d)", top, V, lp::kMaxTop);
     if (rows == 0) return MAMBA_B200_OK;
     if (rows > 2147483647ll || V > kMaxSize) return fail(c, MAMBA_B200_ERR_SHAPE, "token_logprobs: too many rows or tokens");
+    if (!aligned_to(dtype_size(dtype), {logits}) || !aligned_to(4, {targets, lse, entropy, logprob, top_ids, top_logprobs}))
+        return fail(c, MAMBA_B200_ERR_ARG, "token_logprobs: misaligned pointer");
     if (!logits || (logprob && !targets) || (top && (!top_ids || !top_logprobs)))
         return fail(c, MAMBA_B200_ERR_ARG, "token_logprobs: null pointer");
-    if (reinterpret_cast<uintptr_t>(logits) % dtype_size(dtype)) return fail(c, MAMBA_B200_ERR_ARG, "token_logprobs: misaligned logits");
     lp::FwdParams p{logits, targets, lse, entropy, logprob, top_ids, top_logprobs, ld, rows, V, top, 1, 1.0f / temperature};
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     if (dtype == MAMBA_B200_F32) return lp::launch_fwd<float>(c, p, st);
@@ -1108,10 +1109,10 @@ extern "C" MAMBA_B200_API int mamba_b200_token_logprobs_bwd(void* handle, void* 
     if (!temperature_ok(temperature)) return fail(c, MAMBA_B200_ERR_ARG, "token_logprobs_bwd: temperature %g", temperature);
     if (rows == 0) return MAMBA_B200_OK;
     if (rows > 2147483647ll || V > kMaxSize) return fail(c, MAMBA_B200_ERR_SHAPE, "token_logprobs_bwd: too many rows or tokens");
+    if (!aligned_to(dtype_size(dtype), {logits, dlogits}) || !aligned_to(4, {targets, lse, entropy, d_logprob, d_entropy}))
+        return fail(c, MAMBA_B200_ERR_ARG, "token_logprobs_bwd: misaligned pointer");
     if (!logits || !lse || !dlogits || (d_logprob && !targets) || (d_entropy && !entropy))
         return fail(c, MAMBA_B200_ERR_ARG, "token_logprobs_bwd: null pointer");
-    if ((reinterpret_cast<uintptr_t>(logits) | reinterpret_cast<uintptr_t>(dlogits)) % dtype_size(dtype))
-        return fail(c, MAMBA_B200_ERR_ARG, "token_logprobs_bwd: misaligned logits");
     const lp::BwdParams p{logits, targets, lse, entropy, d_logprob, d_entropy, dlogits, ld, ld_d, rows, V, 1.0f / temperature};
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     if (dtype == MAMBA_B200_F32) return lp::launch_bwd<float>(c, p, st);

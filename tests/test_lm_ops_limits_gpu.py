@@ -41,3 +41,30 @@ def test_sizes_beyond_32_bit_loops(refused):
     assert "null" in refused("token_logprobs_bwd", 0, None, ok, None, 1.0, None, None, None, None, None, ok, 1, ok)
     a = ffi.GatedScanArgs(dtype=0, B=1, T=ok, D=ok, ld_x=ok, ld_f=ok, ld_y=ok, ld_dy=ok, ld_dx=ok, ld_df=ok)
     assert "null" in refused("gated_scan_fwd", C.byref(a)) and "null" in refused("gated_scan_bwd", C.byref(a))
+
+
+def test_pointers_between_elements(refused):
+    """Each pointer alone, the others null."""
+    from mamba_rs_b200 import ffi
+    for dtype, odd in ((ffi.F32, 2), (ffi.BF16, 1)):
+        store, words = C.c_void_p(4096 + odd), C.c_void_p(4096 + 2)
+        for i, at in ((0, store), (1, words), (2, store)):
+            p = [at if k == i else None for k in range(3)]
+            assert "misaligned" in refused("embedding_fwd", dtype, p[0], 8, p[1], dtype, p[2], 8, 1, 8, 8, 1.0)
+            assert "misaligned" in refused("embedding_bwd", dtype, p[0], 8, p[1], words if i == 2 else None, 0, 1, 8, 8, 1.0, None, 0)
+        # an f32 result of a 16-bit table
+        assert "misaligned" in refused("embedding_fwd", dtype, None, 8, None, ffi.F32, words, 8, 1, 8, 8, 1.0)
+        for i in range(7):
+            p = [(store if k == 0 else words) if k == i else None for k in range(7)]
+            assert "misaligned" in refused("token_logprobs", dtype, p[0], 8, p[1], 1.0, p[2], p[3], p[4], 1, p[5], p[6], 1, 8)
+            p = [(store if k in (0, 6) else words) if k == i else None for k in range(7)]
+            assert "misaligned" in refused("token_logprobs_bwd", dtype, p[0], 8, p[1], 1.0, *p[2:6], p[6], 8, 1, 8)
+        sizes = dict(dtype=dtype, B=1, T=3, D=8, ld_x=8, ld_f=8, ld_z=8, ld_y=8, ld_dy=8, ld_dx=8, ld_df=8, ld_dz=8)
+        for names, at, fwd, bwd in ((("x", "f", "z"), store, True, True), (("y",), store, True, False), (("dy", "d_x", "d_f", "d_z"), store, False, True),
+                                    (("h0", "h_last"), words, True, False), (("d_last", "d_h0"), words, False, True), (("chunk_states",), words, True, True)):
+            for name in names:
+                a = ffi.GatedScanArgs(**sizes, **{name: at})
+                if fwd:
+                    assert "misaligned" in refused("gated_scan_fwd", C.byref(a)), name
+                if bwd:
+                    assert "misaligned" in refused("gated_scan_bwd", C.byref(a)), name
