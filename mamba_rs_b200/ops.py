@@ -658,6 +658,8 @@ def embedding_bwd(ids, d_out, vocab=None, *, d_table=None, scale=1.0, workspace=
     if workspace is None:
         need = lib.mamba_b200_embedding_bwd_workspace_bytes(rows, dim, vocab)
         workspace = torch.empty(need, dtype=torch.uint8, device=d_out.device) if need else None
+    elif not workspace.is_contiguous():
+        raise ValueError("the workspace is contiguous")
     _launch(lib.mamba_b200_embedding_bwd, dev, handle, dtype_code(d_out.dtype), d_out.data_ptr(), _row(d_out, dim), ids.data_ptr(),
             d_table.data_ptr(), accumulate, rows, dim, vocab, scale, _ptr(workspace),
             0 if workspace is None else workspace.numel() * workspace.element_size())

@@ -1,5 +1,5 @@
 """What the entry points of the token table, the token log probabilities and the gated scan refuse before anything is launched.
-Every call here lacks a pointer that it needs, so none of them could run."""
+The calls of the C entries here lack a pointer that they need, so none of them could run."""
 import ctypes as C
 
 import pytest
@@ -68,3 +68,20 @@ def test_pointers_between_elements(refused):
                     assert "misaligned" in refused("gated_scan_fwd", C.byref(a)), name
                 if bwd:
                     assert "misaligned" in refused("gated_scan_bwd", C.byref(a)), name
+
+
+def test_a_workspace_that_is_less_memory_than_it_has_elements(cuda_dev):
+    """An expanded or strided tensor's elements are not its memory."""
+    import torch
+
+    import mamba_rs_b200 as mb
+    ids, d = torch.zeros(600, dtype=torch.int32, device=cuda_dev), torch.ones(600, 8, device=cuda_dev)
+    need = mb.embedding_bwd_workspace_bytes(600, 8, 5)
+    assert need > 0
+    one = torch.zeros(1, dtype=torch.uint8, device=cuda_dev)
+    for ws in (one.expand(need), torch.zeros(2 * need, dtype=torch.uint8, device=cuda_dev)[::2]):
+        with pytest.raises(ValueError, match="contiguous"):
+            mb.embedding_bwd(ids, d, 5, workspace=ws)
+    x = torch.zeros(1, 1300, 40, device=cuda_dev)
+    with pytest.raises(ValueError, match="contiguous"):
+        mb.gated_scan_fwd(x, x, workspace=one.expand(mb.gated_scan_workspace_bytes(1, 1300, 40)))
