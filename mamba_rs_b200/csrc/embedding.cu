@@ -435,10 +435,10 @@ __global__ void __launch_bounds__(32) embedding_sums_kernel(const BwdParams p, l
     }
 }
 
-// Other rows: M columns a lane, 32 apart.  (Two rows' loads at once 98 us for 32768 x 769, one 84: the warps of an SM suffice.)
+// Other rows: M columns a lane, 32 apart.  (Two rows' loads at once took 98 us for 32768 x 769, one row's 84: the warps of an SM suffice.)
 template <typename T>
 __global__ void __launch_bounds__(kThreads) embedding_sums_plain_kernel(const BwdParams p, long long sums, long long clears) {
-    constexpr int M = 4, U = 1;
+    constexpr int M = 4;
     const int lane = threadIdx.x & 31;
     asm volatile("griddepcontrol.wait;" ::: "memory");
     Task t = next_task<1>(p, blockIdx.x * static_cast<long long>(kThreads / 32) + threadIdx.x / 32, sums, clears);
@@ -448,31 +448,22 @@ __global__ void __launch_bounds__(kThreads) embedding_sums_plain_kernel(const Bw
     float acc[M];
 #pragma unroll
     for (int m = 0; m < M; ++m) acc[m] = 0.0f;
-    for (int i0 = 0; i0 < t.n; i0 += U) {
-        T q[U][M];
+    for (int i = 0; i < t.n; ++i) {
+        const T* row = columns + __shfl_sync(0xffffffffu, t.own.x, i) * p.ld_dout;
+        T q[M];
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
-            const T* row = columns + __shfl_sync(0xffffffffu, t.own.x, (i0 + u) & 31) * p.ld_dout;
+        for (int m = 0; m < M; ++m) q[m] = c + 32 * m < p.dim ? row[32 * m] : from_f<T>(0.0f);
 #pragma unroll
-            for (int m = 0; m < M; ++m)
-                if (i0 + u < t.n && c + 32 * m < p.dim) q[u][m] = row[32 * m];
+        for (int m = 0; m < M; ++m) acc[m] += to_f(q[m]);
+        if (!(t.ends >> i & 1)) continue;
+        bool whole;
+        float* to = sum_place(p, t, i, c, whole);
+#pragma unroll
+        for (int m = 0; m < M; ++m) {
+            if (c + 32 * m < p.dim) write_sum<1>(to + 32 * m, acc + m, whole ? p.scale : 1.0f, whole && p.accumulate);
+            acc[m] = 0.0f;
         }
-#pragma unroll
-        for (int u = 0; u < U; ++u) {
-            const int i = i0 + u;
-            if (i >= t.n) break;
-#pragma unroll
-            for (int m = 0; m < M; ++m) acc[m] += to_f(q[u][m]);
-            if (!(t.ends >> i & 1)) continue;
-            bool whole;
-            float* to = sum_place(p, t, i, c, whole);
-#pragma unroll
-            for (int m = 0; m < M; ++m) {
-                if (c + 32 * m < p.dim) write_sum<1>(to + 32 * m, acc + m, whole ? p.scale : 1.0f, whole && p.accumulate);
-                acc[m] = 0.0f;
-            }
-            t.from_before = false;
-        }
+        t.from_before = false;
     }
 }
 

@@ -700,7 +700,7 @@ __global__ void __launch_bounds__(kThreads + 32 + 32 * kMakers, kCtas) token_log
 }
 
 // Short rows: a warp has one in registers, so the largest logit is known before the sums and nothing is read twice.  Up to
-// 32 P pieces; kShortPieces 32 are 8192 logits in 16 bits.  tau, a lower bound of the top-th largest logit, comes from the largest
+// 32 P pieces; kShortPieces 32 are 8192 logits in 16 bits, and half of that where there are alternatives.  tau, a lower bound of the top-th largest logit, comes from the largest
 // of each lane's even and odd elements (of each lane's alone, 32 alternatives of 4096 x 4000 were 374 us and not 26: the smallest of
 // 32 lanes lets too many through); up to 8 alternatives the lanes' suffice and cost less.
 constexpr int kShortPieces = 32, kShortWarps = 4, kShortRoom = 128;
@@ -1011,8 +1011,8 @@ static int launch_fwd(Ctx* c, FwdParams& p, cudaStream_t st) {
         const unsigned blocks = static_cast<unsigned>((p.rows + kShortWarps - 1) / kShortWarps);
         if (p.V <= 32 * W * 4) token_logprobs_short_kernel<T, TOP, 4><<<blocks, kShortWarps * 32, 0, st>>>(p);
         else if (p.V <= 32 * W * 8) token_logprobs_short_kernel<T, TOP, 8><<<blocks, kShortWarps * 32, 0, st>>>(p);
-        else if (p.V <= 32 * W * 16) token_logprobs_short_kernel<T, TOP, 16><<<blocks, kShortWarps * 32, 0, st>>>(p);
-        else token_logprobs_short_kernel<T, TOP, kShortPieces><<<blocks, kShortWarps * 32, 0, st>>>(p);
+        else if (TOP || p.V <= 32 * W * 16) token_logprobs_short_kernel<T, TOP, 16><<<blocks, kShortWarps * 32, 0, st>>>(p);
+        else if constexpr (!TOP) token_logprobs_short_kernel<T, TOP, kShortPieces><<<blocks, kShortWarps * 32, 0, st>>>(p);
         MB200_CUDA_CHECK(c, cudaGetLastError());
         return MAMBA_B200_OK;
     }
