@@ -592,11 +592,12 @@ static int check(Ctx* c, const mamba_b200_gated_scan_args* a, bool bwd) {
 
 
 // Segments of time, so that every SM has its three CTAs.  Cut, f and x (dy and z) are read twice; whole, a CTA's tiles follow one
-// another at 1.1 us (backward 1.6).  us, whole and cut: 168 strips x 64 tiles 94 and 100 (backward 140 and 172), 120 x 64 74 and 72
-// (104 and 123), 96 x 64 69 and 55 (104 and 90), 72 x 64 69 and 44 (105 and 70), 12 x 128 140 and 20; 12 x 4 tiles are 5 whole and 6 cut.
+// another at 1.1 us (backward 1.8).  Below 3/4 of a strip an SM there is room for four segments or more.  us, whole and cut: 168 strips
+// x 64 tiles 96 and 103 (backward 157 and 167), 120 x 64 70 and 75 (116 and 118), 112 x 64 71 and 80 (117 and 137), 108 x 64 70 and 62
+// (116 and 111), 96 x 64 70 and 57 (116 and 92), 72 x 64 69 and 46 (116 and 81), 12 x 128 132 and 21 (224 and 32); 12 x 4 5.9 and 5.9.
 constexpr int kMaxSegments = 128;
-static int pick_segments(int sms, long long strips, int tiles, bool bwd) {
-    if (strips * 20 > (bwd ? 15ll : 18ll) * sms || tiles <= 4) return 1;
+static int pick_segments(int sms, long long strips, int tiles) {
+    if (strips * 4 > 3ll * sms || tiles <= 4) return 1;
     const long long want = 3ll * sms / (strips > 0 ? strips : 1);
     const int most = static_cast<int>(want < kMaxSegments ? want : kMaxSegments);
     return most < tiles ? most : tiles;
@@ -615,7 +616,7 @@ static int launch_tiled(Ctx* c, const mamba_b200_gated_scan_args& a, cudaStream_
     const long long strips = static_cast<long long>(a.B) * ((a.D + Lay::CH - 1) / Lay::CH);
     if (strips > 2147483647ll) return fail(c, MAMBA_B200_ERR_SHAPE, "gated_scan: too many channels");
     p.tiles = (a.T + kTile - 1) / kTile;
-    int segments = pick_segments(c->sm_count, strips, p.tiles, BWD);
+    int segments = pick_segments(c->sm_count, strips, p.tiles);
     if (reinterpret_cast<uintptr_t>(a.workspace) % 16 != 0) return fail(c, MAMBA_B200_ERR_ARG, "gated_scan: the workspace is 16-byte aligned");
     const long long row = static_cast<long long>(a.B) * a.D * 2 * sizeof(float);  // a segment's sums
     if (!a.workspace || a.workspace_bytes < 0) segments = 1;
@@ -695,7 +696,7 @@ using namespace mb200;
 extern "C" MAMBA_B200_API long long mamba_b200_gated_scan_workspace_bytes(int B, int T, int D) {
     if (B <= 0 || T <= gs::kShort || D <= 0 || T > kMaxSize || D > kMaxSize) return 0;
     // (strips of 64 channels, or of 32: the more segments of the two; sized for 148 SMs, which a launch on fewer only halves further)
-    const int segments = gs::pick_segments(148, static_cast<long long>(B) * ((D + 63) / 64), (T + gs::kTile - 1) / gs::kTile, false);
+    const int segments = gs::pick_segments(148, static_cast<long long>(B) * ((D + 63) / 64), (T + gs::kTile - 1) / gs::kTile);
     return segments > 1 ? static_cast<long long>(segments) * B * D * 2 * sizeof(float) : 0;
 }
 
