@@ -220,21 +220,35 @@ __device__ __forceinline__ void join_lanes(Sums& a, int lanes) {
             a.s1 += __shfl_xor_sync(0xffffffffu, a.s1, o);
         }
 }
-// The sums of a whole row relative to its largest logit, term by term, by one warp.
+// The sums of a whole row relative to its largest logit, term by term, by one warp.  (4096 x 50280 bf16 with every row summed
+// again: 257 us; an element at a time 589.)
 template <typename T>
 __device__ __noinline__ Sums sum_again(const Row<T>& row, float top, float c) {
-    Sums a{top, 0.0f, 0.0f, 0.0f};
-    for (int i0 = threadIdx.x % 32; i0 < row.V; i0 += 8 * 32) {
-        float v[8];
+    constexpr int N = 4;
+    const int lane = threadIdx.x % 32;
+    const float2 neg = splat2(-top), cc = splat2(c);
+    float2 s = splat2(0.0f), s1 = splat2(0.0f);
+    auto term = [&](float2 v) {
+        float2 t = mul2(add2(v, neg), cc);
+        t.x = max_nan(t.x, kNothing), t.y = max_nan(t.y, kNothing);
+        const float2 e = make_float2(ex2(t.x), ex2(t.y));
+        s = add2(s, e);
+        s1 = fma2(e, t, s1);
+    };
+    for (int j0 = lane; j0 - lane < row.pieces; j0 += 32 * N) {
+        Piece<T> q[N];
 #pragma unroll
-        for (int u = 0; u < 8; ++u) v[u] = i0 + 32 * u < row.V ? to_f(row.p[i0 + 32 * u]) : -INFINITY;
-#pragma unroll
-        for (int u = 0; u < 8; ++u) {
-            const float t = max_nan((v[u] - top) * c, kNothing), e = ex2(t);
-            a.s += e;
-            a.s1 = fmaf(e, t, a.s1);
+        for (int u = 0; u < N; ++u) {
+            if (j0 + 32 * u < row.pieces) q[u].load(row.p + row.head + static_cast<long long>(j0 + 32 * u) * Piece<T>::W);
+            else q[u].ruled_out();
         }
+#pragma unroll
+        for (int u = 0; u < N; ++u)
+#pragma unroll
+            for (int k = 0; k < Piece<T>::W / 2; ++k) term(q[u].pair(k));
     }
+    term(make_float2(lane < row.head ? to_f(row.p[lane]) : -INFINITY, row.tail() + lane < row.V ? to_f(row.p[row.tail() + lane]) : -INFINITY));
+    Sums a{top, 0.0f, s.x + s.y, s1.x + s1.y};
     join_lanes(a, 32);
     return a;
 }
