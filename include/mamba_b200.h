@@ -571,7 +571,8 @@ MAMBA_B200_API int mamba_b200_decode_step(void* handle, void* stream, const mamb
  *   bwd: d_table[v, :] = scale * (sum over the rows r with ids[r] = v of d_out[r, :]), added to what d_table holds when
  *        accumulate is not 0, else written, zeros included.  d_out [rows, ld_dout] in `dtype`, d_table [vocab, dim] f32
  *        contiguous.  Sums run in f32 in an order that depends on the sizes and ids alone (no atomics on values): the same
- *        inputs give the same bits.  An id outside [0, vocab) counts nowhere.  workspace: 256-byte aligned,
+ *        inputs give the same bits.  An id outside [0, vocab) counts nowhere; rows and vocab are at most 2^31 - 65537 (as V, T and D are
+ *        in what follows).  workspace: 256-byte aligned,
  *        mamba_b200_embedding_bwd_workspace_bytes(...) bytes (may be 0); nothing in it is kept between calls.
  */
 MAMBA_B200_API int mamba_b200_embedding_fwd(void* handle, void* stream, int dtype, const void* table, long long ld_table,

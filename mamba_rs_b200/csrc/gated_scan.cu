@@ -115,9 +115,9 @@ struct Params {
 constexpr int kFwdWarps = 4, kBwdWarps = 4;
 constexpr int kFwdCtas = 3, kFwdStages = 3;
 // The gradient writes over its inputs, so a stage is asked for again only when its results have been read: with two CTAs or one on an
-// SM two stages leave the memory idle meanwhile, and three are used.  us with two and three: 135 strips x 49 tiles 116 and 82, 144 x 64
-// 139 and 106, 168 x 64 158 and 139, 192 x 32 84 and 73; but 288 x 32 98 and 105, and three CTAs with two stages are 384 x 32 120, two
-// with three 142.  (The forward gains 2 % from a fourth.)
+// SM two stages leave the memory idle meanwhile, and three are used.  us with two and three: 135 strips x 49 tiles 106 and 89, 144 x 64
+// 136 and 116, 168 x 64 165 and 157, 192 x 32 87 and 82, 288 x 32 99 and 96; but three CTAs with two stages are 384 x 32 121, two with
+// three 158.
 constexpr int kFewStages = 3;
 static bool few_ctas(int sms, long long ctas) { return 2 * ctas <= 3ll * sms; }
 
@@ -455,9 +455,9 @@ __global__ void __launch_bounds__(kBwdWarps * 32, 3)
 }
 
 // What each segment of time does to a state (forward) or to the gradient that comes from behind it, without results: f and x
-// (dy and z) are read once more than the floor.  A warp has a quarter of the segment, 16 steps at a time, all their loads in
+// (dy and z) are read once more than the floor.  A warp has an eighth of the segment, 16 steps at a time, all their loads in
 // flight; it ends where the kernel above begins, so that what it read last is still in L2 then.
-constexpr int kSumWarps = 8;  // (4: 61.5 us for one sequence of 32749 x 768, 8: 57.8, 16: 63.0)
+constexpr int kSumWarps = 8;  // (4: 62.0 us for one sequence of 32749 x 768, 8: 57.9, 16: 65.4)
 template <typename T, int V, bool GATE, bool BWD>
 __global__ void __launch_bounds__(kSumWarps * 32) gated_scan_sums_kernel(const __grid_constant__ Params p) {
     using C = Ch<V>;
@@ -524,7 +524,7 @@ __global__ void __launch_bounds__(kSumWarps * 32) gated_scan_sums_kernel(const _
         N = both(N, m);
     }
     // From here on the other kernel's CTAs may start; they wait for this one's end before they read the sums.  (Let in at the
-    // beginning they took the room of CTAs that were still to come: 48 strips, 6 segments 80 us, 69 like this, 70 without.)
+    // beginning they could take the room of CTAs that are still to come; 48 strips, 9 segments 58.6 us then, 59.5 like this, 59.8 without.)
     asm volatile("griddepcontrol.launch_dependents;");
     float* row = p.sums + (static_cast<long long>(b) * p.segments + seg) * 2 * D;
     put(row, c, D, N);
@@ -662,8 +662,8 @@ static int configure(Ctx* c) {
 }
 
 // A lane has two channels in 16 bits and one in f32: rows of 128 bytes, brought by TMA.  Rows that it cannot describe (odd channel
-// counts or starts) take one channel a lane: two of their 2-byte columns a lane were slower, 140 us for 16 x 2048 x 770 against 110 (770
-// and 769 channels), the gradient 414 against 2 x 112.
+// counts or starts) take one channel a lane: 16 x 2048 x 769 and x 770 are 109 us, the gradient 232.  Two of their 2-byte columns a lane
+// were slower, 140 and 414.
 template <bool GATE, bool BWD>
 static int launch_typed(Ctx* c, const mamba_b200_gated_scan_args& a, cudaStream_t st) {
     const int cols = a.dtype == MAMBA_B200_F32 ? 32 : 64;
@@ -695,7 +695,7 @@ using namespace mb200;
 
 extern "C" MAMBA_B200_API long long mamba_b200_gated_scan_workspace_bytes(int B, int T, int D) {
     if (B <= 0 || T <= gs::kShort || D <= 0 || T > kMaxSize || D > kMaxSize) return 0;
-    // (strips of 64 channels, or of 32: the more segments of the two; sized for 148 SMs, which a launch on fewer only halves further)
+    // (strips of 64 channels, or of 32: the more segments of the two; sized for 148 SMs, and a launch that would take more takes what fits)
     const int segments = gs::pick_segments(148, static_cast<long long>(B) * ((D + 63) / 64), (T + gs::kTile - 1) / gs::kTile);
     return segments > 1 ? static_cast<long long>(segments) * B * D * 2 * sizeof(float) : 0;
 }

@@ -703,7 +703,9 @@ def token_logprobs(logits, targets=None, *, top=0, temperature=1.0, handle=None)
 def token_logprobs_bwd(logits, targets, lse, entropy, d_logprob=None, d_entropy=None, *, temperature=1.0, dlogits=None,
                        handle=None):
     """Gradient of the logits from those of logprob and entropy (f32 [rows], either may be None), with lse and entropy as
-    token_logprobs returned them.  dlogits in the logits' dtype; it may be the logits themselves."""
+    token_logprobs returned them.  dlogits in the logits' dtype; it may be the logits themselves.  Where the row strides of the two
+    differ by no multiple of 16 bytes (a padded head's logits[:, :V] and a result that is made here), elements are moved one by one,
+    at a third of the speed: a dlogits with the logits' own stride avoids it."""
     dev = _device_index(logits, targets, lse, entropy, d_logprob, d_entropy, dlogits)
     _logit_rows(logits, targets)
     rows, V = logits.shape
