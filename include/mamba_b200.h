@@ -653,6 +653,135 @@ MAMBA_B200_API long long mamba_b200_gated_scan_workspace_bytes(int B, int T, int
 MAMBA_B200_API int mamba_b200_gated_scan_fwd(void* handle, void* stream, const mamba_b200_gated_scan_args* args);
 MAMBA_B200_API int mamba_b200_gated_scan_bwd(void* handle, void* stream, const mamba_b200_gated_scan_args* args);
 
+/*
+ * Linear attention with a decay for each head, forward, backward and decode step:
+ *   S_t = exp(decay[h]) S_{t-1} + k_t v_t^T      o_t = scale S_t^T q_t        S [K, V] per sequence and head
+ * (no kernel counterpart in the reference; its Mamba-3 scan, kernels/mamba3_chunked.cu:1-46, has data-dependent decays and a
+ * trapezoidal update.)  q [B, T, Hq, K], k [B, T, Hk, K], v [B, T, Hv, V] in the storage dtype, o and d_o [B, T, H, V]; each of Hq, Hk,
+ * Hv divides H, and head h reads head h / (H / Hx) of a tensor with fewer.  Strides of batch, step and head in elements, the last
+ * dimension contiguous (columns of one projection, say).  decay [H] f32, log of the factor a step (0: none, minus infinity: nothing is
+ * kept; above 0 the state grows as the formula says).  States [B, H, K, V] f32 contiguous.  K and V are at most 256.  T = 1 is the decode
+ * step; T = 0 hands the state on.  An infinite or NaN input may show in every output of the 128 steps (from a multiple of 128 on)
+ * that it lies in, the earlier ones among them, and in all that follow (T = 1: in its own alone).
+ *   forward : state (NULL: zeros) enters, state_out (NULL: not written; may be state) leaves.
+ *   backward: the states are made again.  d_state_out (NULL: zeros) is the gradient of the state that left, d_state (NULL: not
+ *             written; not d_state_out) that of the one that entered.  d_q, d_k, d_v have the heads of q, k, v (gradients of shared
+ *             heads are summed, in f32 and in the order of the heads) and are overwritten.  The decays have no gradient here.
+ * workspace: caller-owned scratch, 256-byte aligned, or NULL, of mamba_b200_linear_attention_workspace_bytes(args, backward) bytes (may
+ *   be 0; depends on the sizes alone).  A call with fewer does not cut its sequences; the backward of shared heads needs all of it.
+ *   Nothing in it is kept between calls; two calls that may run at once take one each.
+ */
+typedef struct mamba_b200_linear_attention_args {
+    int dtype;
+    int B, T, H, K, V;
+    int Hq, Hk, Hv;
+    float scale;
+    const float* decay; /* [H] */
+    const void* q;
+    long long q_b, q_t, q_h;
+    const void* k;
+    long long k_b, k_t, k_h;
+    const void* v;
+    long long v_b, v_t, v_h;
+    const float* state;
+    float* state_out;
+    void* o; /* forward */
+    long long o_b, o_t, o_h;
+    const void* d_o; /* backward from here */
+    long long do_b, do_t, do_h;
+    const float* d_state_out;
+    float* d_state;
+    void* d_q;
+    long long dq_b, dq_t, dq_h;
+    void* d_k;
+    long long dk_b, dk_t, dk_h;
+    void* d_v;
+    long long dv_b, dv_t, dv_h;
+    void* workspace;
+    long long workspace_bytes;
+} mamba_b200_linear_attention_args;
+
+MAMBA_B200_API long long mamba_b200_linear_attention_workspace_bytes(const mamba_b200_linear_attention_args* args, int backward);
+MAMBA_B200_API int mamba_b200_linear_attention_fwd(void* handle, void* stream, const mamba_b200_linear_attention_args* args);
+MAMBA_B200_API int mamba_b200_linear_attention_bwd(void* handle, void* stream, const mamba_b200_linear_attention_args* args);
+
+/*
+ * Rotation by position of queries and keys, one launch for both (the reference rotates inside kernels/mamba3_ops.cu:575-640, by an
+ * angle that its time steps carry):
+ *   (a, b) -> scale (a cos - b sin, b cos + a sin),  angle = positions[b, t] * inv_freq[i], in 64 bits before sine and cosine
+ * for pair i of the first R columns of each head: columns 2i and 2i + 1 (interleaved) or i and i + R / 2.  Columns from R on are handed
+ * on as they are.  inverse: the angle's sign is turned, which with the same scale is the gradient's way.  q [B, T, Hq, D],
+ * k [B, T, Hk, D] (NULL: none) in the storage dtype with strides of batch, step and head in elements, the last dimension contiguous;
+ * an output may be its input itself (same strides), else it overlaps none.  positions int32: [B, T] with pos_b = T, or [T] for every
+ * sequence with pos_b = 0.  inv_freq [R / 2] f32.  D is at most 1024.
+ */
+typedef struct mamba_b200_rotary_args {
+    int dtype;
+    int B, T, Hq, Hk, D, R;
+    int interleaved, inverse;
+    float scale;
+    const int* positions;
+    long long pos_b;
+    const float* inv_freq;
+    const void* q;
+    long long q_b, q_t, q_h;
+    void* q_out;
+    long long qo_b, qo_t, qo_h;
+    const void* k;
+    long long k_b, k_t, k_h;
+    void* k_out;
+    long long ko_b, ko_t, ko_h;
+} mamba_b200_rotary_args;
+
+MAMBA_B200_API int mamba_b200_rotary(void* handle, void* stream, const mamba_b200_rotary_args* args);
+
+/*
+ * Group norm over channels that lie last, with activation and gate, forward and backward (no kernel counterpart in the reference,
+ * which normalises whole rows, kernels/norms.cu:126-168):
+ *   y = act((x - mean) * rstd * weight + bias) * SiLU(z),   rstd = 1 / sqrt(var + eps)
+ * x, z, y, dy, d_x, d_z are N * S rows of C channels with a row stride (elements); mean and var are over the S rows of a sample and
+ * the C / G channels of a group (S = 1: each token by itself, a group for each head, say), in f32 around the mean.  weight, bias [C] f32
+ * (NULL: 1 and 0), z NULL: no gate.  stats [2, N, G] f32: mean and rstd, which the forward writes (NULL: not kept) and the backward
+ * reads.
+ *   backward: d_x and, with z, d_z are overwritten; d_weight and d_bias [C] f32 (NULL: not wanted) are added to what they hold when
+ *   accumulate is not 0, else written.  Sums run in an order that the sizes alone give: the same inputs give the same bits.
+ * workspace: 256-byte aligned, mamba_b200_group_norm_workspace_bytes(N, S, C, G, backward) bytes (may be 0); nothing in it is kept
+ *   between calls, and two calls that may run at once take one each.
+ */
+#define MAMBA_B200_ACT_NONE 0
+#define MAMBA_B200_ACT_SILU 1
+#define MAMBA_B200_ACT_GELU 2 /* v * (1 + erf(v / sqrt(2))) / 2 */
+typedef struct mamba_b200_group_norm_args {
+    int dtype;
+    int N, S, C, G;
+    int activation;
+    float eps;
+    const void* x;
+    long long ld_x;
+    const void* z;
+    long long ld_z;
+    const float* weight;
+    const float* bias;
+    float* stats;
+    void* y; /* forward */
+    long long ld_y;
+    const void* dy; /* backward from here */
+    long long ld_dy;
+    void* d_x;
+    long long ld_dx;
+    void* d_z;
+    long long ld_dz;
+    float* d_weight;
+    float* d_bias;
+    int accumulate;
+    void* workspace;
+    long long workspace_bytes;
+} mamba_b200_group_norm_args;
+
+MAMBA_B200_API long long mamba_b200_group_norm_workspace_bytes(int N, int S, int C, int G, int backward);
+MAMBA_B200_API int mamba_b200_group_norm_fwd(void* handle, void* stream, const mamba_b200_group_norm_args* args);
+MAMBA_B200_API int mamba_b200_group_norm_bwd(void* handle, void* stream, const mamba_b200_group_norm_args* args);
+
 #ifdef __cplusplus
 }
 #endif

@@ -91,6 +91,7 @@ int decode_configure(Ctx* c);     // decode.cu
 int gated_scan_configure(Ctx* c);  // gated_scan.cu
 int logprobs_configure(Ctx* c);    // logprobs.cu
 int embedding_configure(Ctx* c);   // embedding.cu
+int linear_attention_configure(Ctx* c);  // linear_attention.cu
 
 }  // namespace mb200
 
@@ -139,6 +140,8 @@ extern "C" MAMBA_B200_API int mamba_b200_init(int device, void** handle) {
     rc = logprobs_configure(c);
     if (rc) return rc;
     rc = embedding_configure(c);
+    if (rc) return rc;
+    rc = linear_attention_configure(c);
     if (rc) return rc;
     return MAMBA_B200_OK;
 }

@@ -1,0 +1,537 @@
+// Linear attention with a decay for each head: entry points, decode step, and the kernel for every size, type and stride.
+// The formulas and the roles are in linear_attention.cuh; 16-bit rows that TMA can describe go to linear_attention_tc.cu.
+#include <math.h>
+#include <string.h>
+
+#include "linear_attention.cuh"
+
+namespace mb200 {
+namespace la {
+
+// ---------------------------------------------------------------------------------------------------
+// One token for each sequence.  S is read and written once (K * V * 8 bytes a head, beside which nothing counts), so a thread has
+// four columns of it (one, where V is no multiple of four) and every row of its row group in flight; the groups' parts of o
+// are joined through shared memory in their order.  64 sequences x 32 heads of 128 x 64 bf16 take 25.6 us, 5.3 TB/s.
+// ---------------------------------------------------------------------------------------------------
+constexpr int kStepThreads = 256;
+
+template <typename T, int VEC>
+__global__ void __launch_bounds__(kStepThreads) step_kernel(const mamba_b200_linear_attention_args a) {
+    __shared__ float qs[kMaxDim], ks[kMaxDim];
+    __shared__ float part[kStepThreads * VEC];
+    const int h = blockIdx.x % a.H, b = blockIdx.x / a.H, tid = threadIdx.x;
+    const int K = a.K, V = a.V, lanes = (V + VEC - 1) / VEC, groups = kStepThreads / lanes;
+    const T* q = static_cast<const T*>(a.q) + b * a.q_b + (h / (a.H / a.Hq)) * a.q_h;
+    const T* k = static_cast<const T*>(a.k) + b * a.k_b + (h / (a.H / a.Hk)) * a.k_h;
+    const T* v = static_cast<const T*>(a.v) + b * a.v_b + (h / (a.H / a.Hv)) * a.v_h;
+    const long long at = static_cast<long long>(blockIdx.x) * K * V;
+    const int g = tid / lanes, c = (tid - g * lanes) * VEC;
+    const bool on = g < groups;
+    constexpr int U = 8;  // rows in flight
+    float s[U][VEC];
+    auto fetch = [&](int r0) {
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int r = r0 + u * groups;
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) s[u][e] = 0.0f;
+            if (on && r < K && a.state) {
+                const float* p = a.state + at + static_cast<long long>(r) * V + c;
+                if (VEC == 4) {
+                    const float4 f = *reinterpret_cast<const float4*>(p);
+                    s[u][0] = f.x; s[u][1 % VEC] = f.y; s[u][2 % VEC] = f.z; s[u][3 % VEC] = f.w;
+                } else {
+                    s[u][0] = *p;
+                }
+            }
+        }
+    };
+    fetch(g);  // (before q, k and v: the state is what takes time)
+    const float lam = expf(a.decay[h]);
+    if (tid < K) {
+        qs[tid] = to_f(q[tid]) * a.scale;
+        ks[tid] = to_f(k[tid]);
+    }
+    float vv[VEC], acc[VEC];
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) {
+        vv[e] = on ? to_f(v[c + e]) : 0.0f;
+        acc[e] = 0.0f;
+    }
+    __syncthreads();
+    for (int r0 = g; r0 < K; r0 += U * groups) {
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int r = r0 + u * groups;
+            if (on && r < K) {
+#pragma unroll
+                for (int e = 0; e < VEC; ++e) {
+                    s[u][e] = a.state ? fmaf(lam, s[u][e], ks[r] * vv[e]) : ks[r] * vv[e];
+                    acc[e] = fmaf(qs[r], s[u][e], acc[e]);
+                }
+                if (a.state_out) {
+                    float* p = a.state_out + at + static_cast<long long>(r) * V + c;
+                    if (VEC == 4) *reinterpret_cast<float4*>(p) = make_float4(s[u][0], s[u][1 % VEC], s[u][2 % VEC], s[u][3 % VEC]);
+                    else *p = s[u][0];
+                }
+            }
+        }
+        if (r0 + U * groups < K) fetch(r0 + U * groups);
+    }
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) part[tid * VEC + e] = acc[e];
+    __syncthreads();
+    T* o = static_cast<T*>(a.o) + b * a.o_b + h * a.o_h;
+    for (int j = tid; j < V; j += kStepThreads) {
+        float sum = 0.0f;
+        for (int i = 0; i < groups; ++i) sum += part[i * lanes * VEC + j];
+        o[j] = from_f<T>(sum);
+    }
+}
+
+// ---------------------------------------------------------------------------------------------------
+// Any size, type and stride: a block has 32 columns of one pair's state in shared memory and walks chunks of 32 steps,
+//   P = mask(X Y^T),  out = P Z + decayed X S,  S <- l^n S + Y^T (weights o Z),
+// all in f32 with tiles of registers.  Steps are numbered in the order they are walked, so the roles that run backwards
+// differ in what a step's address is alone.  Bound by the FP32 pipe and shared memory: 8 x 4096 x 32 heads of 128 x 64 bf16 7.1 ms.
+// With few pairs the sequence is cut into segments: STATE blocks find what each adds to a state from zero, and the full walk
+// starts from the sum of what was before.
+// ---------------------------------------------------------------------------------------------------
+constexpr int kSteps = 32, kCols = 32, kThreads = 256;
+
+inline size_t gen_smem(int A) { return sizeof(float) * (2 * kSteps * (A + 4) + 2 * kSteps * kCols + kSteps * (kSteps + 4) + A * kCols + 3 * kSteps); }
+
+template <typename T, bool STATE>
+__global__ void __launch_bounds__(kThreads) general_kernel(const Params p) {
+    extern __shared__ __align__(16) float sm[];
+    const Place w = place(p, blockIdx.x, STATE ? p.segments - 1 : p.segments);
+    const Role& r = p.role[w.role];
+    const int tid = threadIdx.x, A = r.A, Ar = (A + 3) & ~3, LD = Ar + 4, W = r.W;
+    const int b = static_cast<int>(w.pair / p.H), h = static_cast<int>(w.pair - static_cast<long long>(b) * p.H);
+    const int c0 = w.tile * kCols, nc = min(kCols, W - c0);
+    float* X = sm;
+    float* Y = X + kSteps * LD;
+    float* Z = Y + kSteps * LD;
+    float* Zw = Z + kSteps * kCols;
+    float* P = Zw + kSteps * kCols;
+    float* S = P + kSteps * (kSteps + 4);
+    float* pw = S + Ar * kCols;  // l^i, i <= kSteps
+    const float ld = p.decay[h], l2 = ld * kLog2e;
+    const int t_lo = w.seg * p.seg_len, t_hi = min(p.T, t_lo + p.seg_len);
+    const T* xg = static_cast<const T*>(r.x.p) + b * r.x.sb + (h / r.x.group) * r.x.sh;
+    const T* yg = static_cast<const T*>(r.y.p) + b * r.y.sb + (h / r.y.group) * r.y.sh;
+    const T* zg = static_cast<const T*>(r.z.p) + b * r.z.sb + (h / r.z.group) * r.z.sh + c0;
+    auto row = [&](int t) { return r.backwards ? p.T - 1 - t : t; };
+    if (tid <= kSteps) pw[tid] = decay_at(l2, tid);
+    // the state that enters this segment
+    const long long slot = static_cast<long long>(A) * W;
+    float* slots = r.slots ? r.slots + w.pair * p.segments * slot : nullptr;
+    const bool first = w.seg == 0;
+    const Pow per_seg = decay_pow(ld, p.seg_len);
+    bool entered = false;
+    if (first ? r.s_in != nullptr : !STATE) entered = true;
+    for (int i = tid; i < Ar * kCols; i += kThreads) {
+        const int a = i / kCols, c = i % kCols;
+        float s = 0.0f;
+        if (a < A && c < nc && entered) {
+            const long long e = static_cast<long long>(a) * W + c0 + c;
+            if (first && (STATE || p.segments == 1)) s = r.s_in[w.pair * slot + static_cast<long long>(a) * r.sa + static_cast<long long>(c0 + c) * r.sw];
+            else if (first) s = slots[e];
+            else {
+                for (int k = 1; k <= w.seg; ++k) s = (k > 1 ? times(per_seg, s) : 0.0f) + slots[k * slot + e];
+            }
+            if (STATE && first) slots[e] = s;
+        }
+        S[i] = s;
+    }
+    const int i4 = tid >> 3, j8 = tid & 7, w4 = j8 * 4;
+    for (int t0 = t_lo; t0 < t_hi; t0 += kSteps) {
+        const int n = min(kSteps, t_hi - t0);
+        const int late = r.late && first && t0 == t_lo ? 1 : 0;
+        __syncthreads();  // the last chunk's readers of X, Y, Z, Zw; the state is whole
+        for (int i = tid; i < kSteps * Ar; i += kThreads) {
+            const int s = i / Ar, a = i - s * Ar;
+            const bool ok = s < n && a < A;
+            if (!STATE) X[s * LD + a] = ok ? to_f(xg[row(t0 + s) * r.x.st + a]) : 0.0f;
+            Y[s * LD + a] = ok ? to_f(yg[row(t0 + s) * r.y.st + a]) : 0.0f;
+        }
+        for (int i = tid; i < kSteps * kCols; i += kThreads) {
+            const int s = i / kCols, c = i % kCols;
+            const float z = s < n && c < nc ? to_f(zg[row(t0 + s) * r.z.st + c]) : 0.0f;
+            Z[i] = z;
+            Zw[i] = s < n ? z * pw[n - 1 - s] * r.alpha_s : 0.0f;
+        }
+        __syncthreads();
+        if (!STATE) {
+            // P[i4][j8 + 8 m]
+            float g[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+            for (int a = 0; a < Ar; a += 4) {
+                const float4 x = *reinterpret_cast<const float4*>(X + i4 * LD + a);
+#pragma unroll
+                for (int m = 0; m < 4; ++m) {
+                    const float4 y = *reinterpret_cast<const float4*>(Y + (j8 + 8 * m) * LD + a);
+                    g[m] = fmaf(x.x, y.x, fmaf(x.y, y.y, fmaf(x.z, y.z, fmaf(x.w, y.w, g[m]))));
+                }
+            }
+#pragma unroll
+            for (int m = 0; m < 4; ++m) {
+                const int j = j8 + 8 * m;
+                P[i4 * (kSteps + 4) + j] = j <= i4 ? g[m] * (pw[max(i4 - j, 0)] * r.alpha_p) : 0.0f;
+            }
+            __syncthreads();
+            float o[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+            if (entered || t0 > t_lo) {
+                for (int a = 0; a < Ar; a += 4) {
+                    const float4 x = *reinterpret_cast<const float4*>(X + i4 * LD + a);
+                    const float xv[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+                    for (int u = 0; u < 4; ++u) {
+                        const float4 s = *reinterpret_cast<const float4*>(S + (a + u) * kCols + w4);
+                        o[0] = fmaf(xv[u], s.x, o[0]);
+                        o[1] = fmaf(xv[u], s.y, o[1]);
+                        o[2] = fmaf(xv[u], s.z, o[2]);
+                        o[3] = fmaf(xv[u], s.w, o[3]);
+                    }
+                }
+                const float f = pw[i4 + 1 - late] * r.alpha_x;
+#pragma unroll
+                for (int u = 0; u < 4; ++u) o[u] *= f;
+            }
+            for (int j = 0; j <= i4; ++j) {
+                const float q = P[i4 * (kSteps + 4) + j];
+                const float4 z = *reinterpret_cast<const float4*>(Z + j * kCols + w4);
+                o[0] = fmaf(q, z.x, o[0]);
+                o[1] = fmaf(q, z.y, o[1]);
+                o[2] = fmaf(q, z.z, o[2]);
+                o[3] = fmaf(q, z.w, o[3]);
+            }
+            if (i4 < n) {
+                const long long at = b * r.ob + row(t0 + i4) * r.ot + h * r.oh + c0 + w4;
+#pragma unroll
+                for (int u = 0; u < 4; ++u)
+                    if (w4 + u < nc) {
+                        if (r.out_f32) static_cast<float*>(r.out)[at + u] = o[u];
+                        else static_cast<T*>(r.out)[at + u] = from_f<T>(o[u]);
+                    }
+            }
+            __syncthreads();  // every reader of S
+        }
+        // S[a4 .. a4 + 3][w4 .. w4 + 3]
+        if (STATE || t0 + n < t_hi || (w.seg + 1 == p.segments && r.s_out)) {
+            const Pow f = decay_pow(ld, n - late);
+            for (int a4 = 4 * i4; a4 < Ar; a4 += 4 * (kThreads / 8)) {
+                float4 s[4];
+#pragma unroll
+                for (int u = 0; u < 4; ++u) {
+                    s[u] = *reinterpret_cast<const float4*>(S + (a4 + u) * kCols + w4);
+                    if (entered || t0 > t_lo) s[u] = make_float4(times(f, s[u].x), times(f, s[u].y), times(f, s[u].z), times(f, s[u].w));
+                }
+                for (int j = 0; j < n; ++j) {
+                    const float4 y = *reinterpret_cast<const float4*>(Y + j * LD + a4);
+                    const float4 z = *reinterpret_cast<const float4*>(Zw + j * kCols + w4);
+                    const float yv[4] = {y.x, y.y, y.z, y.w};
+#pragma unroll
+                    for (int u = 0; u < 4; ++u) {
+                        s[u].x = fmaf(yv[u], z.x, s[u].x);
+                        s[u].y = fmaf(yv[u], z.y, s[u].y);
+                        s[u].z = fmaf(yv[u], z.z, s[u].z);
+                        s[u].w = fmaf(yv[u], z.w, s[u].w);
+                    }
+                }
+#pragma unroll
+                for (int u = 0; u < 4; ++u) *reinterpret_cast<float4*>(S + (a4 + u) * kCols + w4) = s[u];
+            }
+        }
+    }
+    __syncthreads();
+    float* out = nullptr;
+    Pow f{1.0f, 0.0f};
+    if (STATE) out = slots + (w.seg + 1) * slot;
+    else if (w.seg + 1 == p.segments && r.s_out) {
+        out = r.s_out + w.pair * slot;
+        if (r.last_decay) f = decay_pow(ld, 1);
+    }
+    if (out)
+        for (int i = tid; i < A * kCols; i += kThreads) {
+            const int a = i / kCols, c = i % kCols;
+            if (c < nc) out[static_cast<long long>(a) * W + c0 + c] = times(f, S[i]);
+        }
+}
+
+// Gradients of shared heads: the heads' f32 parts [B, T, H, D], summed in their order.
+template <typename T>
+__global__ void __launch_bounds__(256) sum_heads_kernel(const float* __restrict__ part, T* out, long long ob, long long ot, long long oh,
+                                                        long long rows, int T_, int heads, int group, int D) {
+    const long long total = rows * heads * D;
+    for (long long i = blockIdx.x * 256ll + threadIdx.x; i < total; i += gridDim.x * 256ll) {
+        const int d = static_cast<int>(i % D);
+        const long long rh = i / D;
+        const int h = static_cast<int>(rh % heads);
+        const long long row = rh / heads;
+        const float* src = part + (row * heads + h) * group * D + d;
+        float s = 0.0f;
+        for (int g = 0; g < group; ++g) s += src[static_cast<long long>(g) * D];
+        out[(row / T_) * ob + (row % T_) * ot + h * oh + d] = from_f<T>(s);
+    }
+}
+
+// ---------------------------------------------------------------------------------------------------
+// host
+// ---------------------------------------------------------------------------------------------------
+inline long long up256(long long n) { return (n + 255) / 256 * 256; }
+
+// What a call's scratch holds: the states between segments of each role, and the f32 parts of shared heads' gradients.
+struct Room {
+    long long slots = 0, parts[3] = {0, 0, 0};
+    long long total() const { return slots + parts[0] + parts[1] + parts[2]; }
+};
+inline Room room(const mamba_b200_linear_attention_args& a, int backward) {
+    Room r;
+    const long long pairs = static_cast<long long>(a.B) * a.H, chunks = (a.T + kChunk - 1) / kChunk;
+    // more than 148 blocks of the narrowest tiles are not cut, so few pairs have many segments and many have few
+    const long long seg = chunks < 2 ? 0 : kMaxSegments < chunks ? kMaxSegments : chunks;
+    const long long most = pairs > 0 ? 2 * 148 / pairs + 1 : 0;
+    const long long n = seg < most ? seg : most;
+    if (n > 1) r.slots = up256(pairs * n * a.K * a.V * 4) * (backward ? 3 : 1);
+    if (backward) {
+        const long long rows = static_cast<long long>(a.B) * a.T * a.H * 4;
+        if (a.Hq < a.H) r.parts[0] = up256(rows * a.K);
+        if (a.Hk < a.H) r.parts[1] = up256(rows * a.K);
+        if (a.Hv < a.H) r.parts[2] = up256(rows * a.V);
+    }
+    return r;
+}
+
+// Segments of a launch of `blocks` blocks an uncut sequence: as many as fill the SMs once, each of at least four chunks
+// (the states of a segment cost about half a walk of it).
+int pick_segments(int sm_count, long long blocks, int T, long long pairs) {
+    const int chunks = (T + kChunk - 1) / kChunk;
+    long long n = blocks > 0 ? sm_count / blocks : 1;
+    if (n > chunks / 4) n = chunks / 4;
+    if (n > kMaxSegments) n = kMaxSegments;
+    if (pairs > 0 && n > 2 * 148 / pairs + 1) n = 2 * 148 / pairs + 1;  // (what room() has)
+    return n < 2 ? 1 : static_cast<int>(n);
+}
+
+template <typename T>
+int launch_general(Ctx* c, Params& p, bool may_cut, long long pairs, cudaStream_t st) {
+    long long blocks = 0;
+    int A = 0;
+    for (int i = 0; i < p.roles; ++i) {
+        p.role[i].tiles = (p.role[i].W + kCols - 1) / kCols;
+        p.role[i].block0 = blocks;
+        blocks += pairs * p.role[i].tiles;
+        if (p.role[i].A > A) A = p.role[i].A;
+    }
+    p.segments = may_cut ? pick_segments(c->sm_count, blocks, p.T, pairs) : 1;
+    const int chunks = (p.T + kChunk - 1) / kChunk, per = (chunks + p.segments - 1) / p.segments;
+    p.segments = per > 0 ? (chunks + per - 1) / per : 1;
+    p.seg_len = per * kChunk;
+    if (blocks * p.segments > 2147483647ll) return fail(c, MAMBA_B200_ERR_SHAPE, "linear_attention: too many heads");
+    const size_t smem = gen_smem((A + 3) & ~3);
+    if (p.segments > 1) {
+        general_kernel<T, true><<<static_cast<unsigned>(blocks * (p.segments - 1)), kThreads, smem, st>>>(p);
+        MB200_CUDA_CHECK(c, cudaGetLastError());
+    }
+    general_kernel<T, false><<<static_cast<unsigned>(blocks * p.segments), kThreads, smem, st>>>(p);
+    MB200_CUDA_CHECK(c, cudaGetLastError());
+    return MAMBA_B200_OK;
+}
+
+template <typename T>
+int launch_step(Ctx* c, const mamba_b200_linear_attention_args& a, cudaStream_t st) {
+    const unsigned grid = static_cast<unsigned>(a.B) * a.H;
+    if (a.V % 4 == 0 && aligned_to(16, {a.state, a.state_out})) step_kernel<T, 4><<<grid, kStepThreads, 0, st>>>(a);
+    else step_kernel<T, 1><<<grid, kStepThreads, 0, st>>>(a);
+    MB200_CUDA_CHECK(c, cudaGetLastError());
+    return MAMBA_B200_OK;
+}
+
+template <typename T>
+int sum_heads(Ctx* c, const float* part, void* out, long long ob, long long ot, long long oh, const mamba_b200_linear_attention_args& a, int heads,
+              int D, cudaStream_t st) {
+    const long long rows = static_cast<long long>(a.B) * a.T, blocks = (rows * heads * D + 255) / 256;
+    const long long most = 32ll * c->sm_count;
+    sum_heads_kernel<T><<<static_cast<unsigned>(blocks < most ? blocks : most), 256, 0, st>>>(part, static_cast<T*>(out), ob, ot, oh, rows, a.T, heads,
+                                                                                             a.H / heads, D);
+    MB200_CUDA_CHECK(c, cudaGetLastError());
+    return MAMBA_B200_OK;
+}
+
+// Rows of a tensor that a launch of this many steps, heads and sequences may touch, checked against the type's reach.
+int check(Ctx* c, const mamba_b200_linear_attention_args* a, bool backward) {
+    const char* what = backward ? "linear_attention_bwd" : "linear_attention_fwd";
+    int cur = -1;
+    MB200_CUDA_CHECK(c, cudaGetDevice(&cur));
+    if (cur != c->device)
+        return fail(c, MAMBA_B200_ERR_DEVICE, "%s: the handle belongs to device %d but device %d is current", what, c->device, cur);
+    if (!dtype_ok(a->dtype)) return fail(c, MAMBA_B200_ERR_ARG, "%s: unknown dtype %d", what, a->dtype);
+    if (a->B < 0 || a->T < 0 || a->H < 1 || a->K < 1 || a->V < 1)
+        return fail(c, MAMBA_B200_ERR_SHAPE, "%s: B %d T %d H %d K %d V %d", what, a->B, a->T, a->H, a->K, a->V);
+    if (a->K > kMaxDim || a->V > kMaxDim) return fail(c, MAMBA_B200_ERR_SHAPE, "%s: K %d and V %d are at most %d", what, a->K, a->V, kMaxDim);
+    if (a->T > kMaxSize) return fail(c, MAMBA_B200_ERR_SHAPE, "%s: too many steps (%d)", what, a->T);
+    if (static_cast<long long>(a->B) * a->H > 1000000) return fail(c, MAMBA_B200_ERR_SHAPE, "%s: too many sequences x heads (%d x %d)", what, a->B, a->H);
+    for (int h : {a->Hq, a->Hk, a->Hv})
+        if (h < 1 || a->H % h) return fail(c, MAMBA_B200_ERR_SHAPE, "%s: %d heads are not shared by %d evenly", what, h, a->H);
+    if (!isfinite(a->scale)) return fail(c, MAMBA_B200_ERR_ARG, "%s: the scale is not finite", what);
+    if (a->B == 0) return MAMBA_B200_OK;
+    const bool some = a->T > 0;
+    if (!a->decay || (some && (!a->q || !a->k || !a->v))) return fail(c, MAMBA_B200_ERR_ARG, "%s: null pointer", what);
+    if (some && !backward && !a->o) return fail(c, MAMBA_B200_ERR_ARG, "%s: null pointer", what);
+    if (some && backward && (!a->d_o || !a->d_q || !a->d_k || !a->d_v)) return fail(c, MAMBA_B200_ERR_ARG, "%s: null pointer", what);
+    if (backward && a->d_state && a->d_state == a->d_state_out)
+        return fail(c, MAMBA_B200_ERR_ARG, "%s: d_state and d_state_out are the same memory", what);
+    const size_t es = dtype_size(a->dtype);
+    if (!aligned_to(es, {a->q, a->k, a->v}) || !aligned_to(es, {backward ? a->d_o : a->o}) ||
+        (backward && !aligned_to(es, {a->d_q, a->d_k, a->d_v})) || !aligned_to(4, {a->decay, a->state}) ||
+        !aligned_to(4, {backward ? nullptr : a->state_out, backward ? a->d_state : nullptr, backward ? a->d_state_out : nullptr}))
+        return fail(c, MAMBA_B200_ERR_ARG, "%s: misaligned pointer", what);
+    if (a->workspace && reinterpret_cast<uintptr_t>(a->workspace) % 256) return fail(c, MAMBA_B200_ERR_ARG, "%s: misaligned workspace", what);
+    return MAMBA_B200_OK;
+}
+
+// T = 0: a state goes from `in` to `out`.
+int hand_on(Ctx* c, const float* in, float* out, const mamba_b200_linear_attention_args& a, cudaStream_t st) {
+    if (!out || in == out) return MAMBA_B200_OK;
+    const size_t bytes = sizeof(float) * static_cast<size_t>(a.B) * a.H * a.K * a.V;
+    if (in) MB200_CUDA_CHECK(c, cudaMemcpyAsync(out, in, bytes, cudaMemcpyDeviceToDevice, st));
+    else MB200_CUDA_CHECK(c, cudaMemsetAsync(out, 0, bytes, st));
+    return MAMBA_B200_OK;
+}
+
+int dispatch(Ctx* c, const mamba_b200_linear_attention_args& a, Params& p, bool may_cut, cudaStream_t st) {
+    const long long pairs = static_cast<long long>(a.B) * a.H;
+    if (a.dtype == MAMBA_B200_F32) return launch_general<float>(c, p, may_cut, pairs, st);
+    if (a.dtype == MAMBA_B200_F16) return launch_general<__half>(c, p, may_cut, pairs, st);
+    return launch_general<__nv_bfloat16>(c, p, may_cut, pairs, st);
+}
+
+}  // namespace la
+
+int linear_attention_configure(Ctx* c) {
+    const int most = static_cast<int>(la::gen_smem(la::kMaxDim));
+    const void* fns[] = {(const void*)la::general_kernel<float, false>,  (const void*)la::general_kernel<float, true>,
+                         (const void*)la::general_kernel<__half, false>, (const void*)la::general_kernel<__half, true>,
+                         (const void*)la::general_kernel<__nv_bfloat16, false>, (const void*)la::general_kernel<__nv_bfloat16, true>};
+    for (const void* f : fns) MB200_CUDA_CHECK(c, cudaFuncSetAttribute(f, cudaFuncAttributeMaxDynamicSharedMemorySize, most));
+    return MAMBA_B200_OK;
+}
+
+}  // namespace mb200
+
+using namespace mb200;
+
+extern "C" MAMBA_B200_API long long mamba_b200_linear_attention_workspace_bytes(const mamba_b200_linear_attention_args* a, int backward) {
+    if (!a || a->B < 1 || a->T < 1 || a->H < 1 || a->K < 1 || a->V < 1 || a->K > la::kMaxDim || a->V > la::kMaxDim || a->T > kMaxSize ||
+        static_cast<long long>(a->B) * a->H > 1000000)
+        return 0;
+    return la::room(*a, backward).total();
+}
+
+extern "C" MAMBA_B200_API int mamba_b200_linear_attention_fwd(void* handle, void* stream, const mamba_b200_linear_attention_args* args) {
+    Ctx* c = static_cast<Ctx*>(handle);
+    if (!c || !args) return MAMBA_B200_ERR_ARG;
+    const int rc = la::check(c, args, false);
+    if (rc || args->B == 0) return rc;
+    const mamba_b200_linear_attention_args& a = *args;
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    if (a.T == 0) return la::hand_on(c, a.state, a.state_out, a, st);
+    if (a.T == 1) {
+        if (a.dtype == MAMBA_B200_F32) return la::launch_step<float>(c, a, st);
+        if (a.dtype == MAMBA_B200_F16) return la::launch_step<__half>(c, a, st);
+        return la::launch_step<__nv_bfloat16>(c, a, st);
+    }
+    la::Params p;
+    memset(&p, 0, sizeof(p));
+    p.roles = 1;
+    p.B = a.B; p.T = a.T; p.H = a.H;
+    p.decay = a.decay;
+    p.status = c->d_status;
+    la::Role& r = p.role[0];
+    r.x = {a.q, a.q_b, a.q_t, a.q_h, a.H / a.Hq, a.K};
+    r.y = {a.k, a.k_b, a.k_t, a.k_h, a.H / a.Hk, a.K};
+    r.z = {a.v, a.v_b, a.v_t, a.v_h, a.H / a.Hv, a.V};
+    r.A = a.K; r.W = a.V;
+    r.out = a.o; r.ob = a.o_b; r.ot = a.o_t; r.oh = a.o_h;
+    r.s_in = a.state; r.sa = a.V; r.sw = 1;
+    r.s_out = a.state_out;
+    r.alpha_p = r.alpha_x = a.scale;
+    r.alpha_s = 1.0f;
+    const la::Room room = la::room(a, 0);
+    const bool may_cut = room.slots > 0 && a.workspace && a.workspace_bytes >= room.slots;
+    if (may_cut) r.slots = static_cast<float*>(a.workspace);
+    return la::dispatch(c, a, p, may_cut, st);
+}
+
+extern "C" MAMBA_B200_API int mamba_b200_linear_attention_bwd(void* handle, void* stream, const mamba_b200_linear_attention_args* args) {
+    Ctx* c = static_cast<Ctx*>(handle);
+    if (!c || !args) return MAMBA_B200_ERR_ARG;
+    int rc = la::check(c, args, true);
+    if (rc || args->B == 0) return rc;
+    const mamba_b200_linear_attention_args& a = *args;
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    if (a.T == 0) return la::hand_on(c, a.d_state_out, a.d_state, a, st);
+    const la::Room room = la::room(a, 1);
+    const long long parts = room.parts[0] + room.parts[1] + room.parts[2];
+    if (parts && (!a.workspace || a.workspace_bytes < room.total()))
+        return fail(c, MAMBA_B200_ERR_ARG, "linear_attention_bwd: shared heads need a workspace of %lld bytes (%lld given)", room.total(),
+                    a.workspace ? a.workspace_bytes : 0ll);
+    const bool may_cut = room.slots > 0 && a.workspace && a.workspace_bytes >= room.total();
+    char* ws = static_cast<char*>(a.workspace);
+    float* part[3] = {nullptr, nullptr, nullptr};
+    char* at = ws + room.slots;
+    for (int i = 0; i < 3; ++i)
+        if (room.parts[i]) {
+            part[i] = reinterpret_cast<float*>(at);
+            at += room.parts[i];
+        }
+    la::Params p;
+    memset(&p, 0, sizeof(p));
+    p.roles = 3;
+    p.B = a.B; p.T = a.T; p.H = a.H;
+    p.decay = a.decay;
+    p.status = c->d_status;
+    const la::Operand q = {a.q, a.q_b, a.q_t, a.q_h, a.H / a.Hq, a.K}, k = {a.k, a.k_b, a.k_t, a.k_h, a.H / a.Hk, a.K};
+    const la::Operand v = {a.v, a.v_b, a.v_t, a.v_h, a.H / a.Hv, a.V}, d = {a.d_o, a.do_b, a.do_t, a.do_h, 1, a.V};
+    void* outs[3] = {a.d_q, a.d_k, a.d_v};
+    const long long strides[3][3] = {{a.dq_b, a.dq_t, a.dq_h}, {a.dk_b, a.dk_t, a.dk_h}, {a.dv_b, a.dv_t, a.dv_h}};
+    const int heads[3] = {a.Hq, a.Hk, a.Hv};
+    for (int i = 0; i < 3; ++i) {
+        la::Role& r = p.role[i];
+        r.A = i == 2 ? a.K : a.V;
+        r.W = i == 2 ? a.V : a.K;
+        r.x = i == 0 ? d : i == 1 ? v : k;
+        r.y = i == 0 ? v : i == 1 ? d : q;
+        r.z = i == 0 ? k : i == 1 ? q : d;
+        if (part[i]) {
+            r.out = part[i];
+            r.out_f32 = 1;
+            r.oh = r.W;
+            r.ot = static_cast<long long>(a.H) * r.W;
+            r.ob = a.T * r.ot;
+        } else {
+            r.out = outs[i];
+            r.ob = strides[i][0]; r.ot = strides[i][1]; r.oh = strides[i][2];
+        }
+        r.s_in = i == 0 ? a.state : a.d_state_out;
+        r.sa = i == 2 ? a.V : 1;
+        r.sw = i == 2 ? 1 : a.V;
+        r.s_out = i == 2 ? a.d_state : nullptr;
+        r.backwards = i > 0;
+        r.late = i > 0;
+        r.last_decay = i == 2;
+        r.alpha_p = a.scale;
+        r.alpha_x = i == 0 ? a.scale : 1.0f;
+        r.alpha_s = i == 0 ? 1.0f : a.scale;
+        if (may_cut) r.slots = reinterpret_cast<float*>(ws + room.slots / 3 * i);
+    }
+    rc = la::dispatch(c, a, p, may_cut, st);
+    for (int i = 0; i < 3 && !rc; ++i)
+        if (part[i]) {
+            const int D = i == 2 ? a.V : a.K;
+            if (a.dtype == MAMBA_B200_F32) rc = la::sum_heads<float>(c, part[i], outs[i], strides[i][0], strides[i][1], strides[i][2], a, heads[i], D, st);
+            else if (a.dtype == MAMBA_B200_F16) rc = la::sum_heads<__half>(c, part[i], outs[i], strides[i][0], strides[i][1], strides[i][2], a, heads[i], D, st);
+            else rc = la::sum_heads<__nv_bfloat16>(c, part[i], outs[i], strides[i][0], strides[i][1], strides[i][2], a, heads[i], D, st);
+        }
+    return rc;
+}

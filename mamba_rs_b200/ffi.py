@@ -134,7 +134,43 @@ class GatedScanArgs(C.Structure):
     ]
 
 
+def _strided(name):
+    """A [B, T, heads, width] tensor of an argument struct: its pointer, and the strides of batch, step and head."""
+    short = {"q_out": "qo", "k_out": "ko", "d_o": "do", "d_q": "dq", "d_k": "dk", "d_v": "dv"}.get(name, name)
+    return [(name, C.c_void_p)] + [(f"{short}_{d}", C.c_longlong) for d in "bth"]
+
+
+class LinearAttentionArgs(C.Structure):
+    _fields_ = [
+        ("dtype", C.c_int), ("B", C.c_int), ("T", C.c_int), ("H", C.c_int), ("K", C.c_int), ("V", C.c_int),
+        ("Hq", C.c_int), ("Hk", C.c_int), ("Hv", C.c_int), ("scale", C.c_float), ("decay", C.c_void_p),
+        *_strided("q"), *_strided("k"), *_strided("v"), ("state", C.c_void_p), ("state_out", C.c_void_p), *_strided("o"),
+        *_strided("d_o"), ("d_state_out", C.c_void_p), ("d_state", C.c_void_p), *_strided("d_q"), *_strided("d_k"), *_strided("d_v"),
+        ("workspace", C.c_void_p), ("workspace_bytes", C.c_longlong),
+    ]
+
+
+class RotaryArgs(C.Structure):
+    _fields_ = [
+        ("dtype", C.c_int), ("B", C.c_int), ("T", C.c_int), ("Hq", C.c_int), ("Hk", C.c_int), ("D", C.c_int), ("R", C.c_int),
+        ("interleaved", C.c_int), ("inverse", C.c_int), ("scale", C.c_float), ("positions", C.c_void_p), ("pos_b", C.c_longlong),
+        ("inv_freq", C.c_void_p), *_strided("q"), *_strided("q_out"), *_strided("k"), *_strided("k_out"),
+    ]
+
+
+class GroupNormArgs(C.Structure):
+    _fields_ = [
+        ("dtype", C.c_int), ("N", C.c_int), ("S", C.c_int), ("C", C.c_int), ("G", C.c_int), ("activation", C.c_int), ("eps", C.c_float),
+        ("x", C.c_void_p), ("ld_x", C.c_longlong), ("z", C.c_void_p), ("ld_z", C.c_longlong),
+        ("weight", C.c_void_p), ("bias", C.c_void_p), ("stats", C.c_void_p), ("y", C.c_void_p), ("ld_y", C.c_longlong),
+        ("dy", C.c_void_p), ("ld_dy", C.c_longlong), ("d_x", C.c_void_p), ("ld_dx", C.c_longlong),
+        ("d_z", C.c_void_p), ("ld_dz", C.c_longlong), ("d_weight", C.c_void_p), ("d_bias", C.c_void_p), ("accumulate", C.c_int),
+        ("workspace", C.c_void_p), ("workspace_bytes", C.c_longlong),
+    ]
+
+
 GATED_SCAN_SAVE = 64  # MAMBA_B200_GATED_SCAN_SAVE
+ACTIVATIONS = {None: 0, "silu": 1, "gelu": 2}  # MAMBA_B200_ACT_*
 
 _lib = None
 
@@ -197,6 +233,13 @@ def lib() -> C.CDLL:
         bind("mamba_b200_gated_scan_workspace_bytes", [it, it, it], ll)
         bind("mamba_b200_gated_scan_fwd", [vp, vp, C.POINTER(GatedScanArgs)])
         bind("mamba_b200_gated_scan_bwd", [vp, vp, C.POINTER(GatedScanArgs)])
+        bind("mamba_b200_linear_attention_workspace_bytes", [C.POINTER(LinearAttentionArgs), it], ll)
+        bind("mamba_b200_linear_attention_fwd", [vp, vp, C.POINTER(LinearAttentionArgs)])
+        bind("mamba_b200_linear_attention_bwd", [vp, vp, C.POINTER(LinearAttentionArgs)])
+        bind("mamba_b200_rotary", [vp, vp, C.POINTER(RotaryArgs)])
+        bind("mamba_b200_group_norm_workspace_bytes", [it] * 5, ll)
+        bind("mamba_b200_group_norm_fwd", [vp, vp, C.POINTER(GroupNormArgs)])
+        bind("mamba_b200_group_norm_bwd", [vp, vp, C.POINTER(GroupNormArgs)])
         bind("mamba_b200_decode_workspace_bytes", [vp, C.POINTER(DecodeArgs)], ll)
         bind("mamba_b200_decode_step", [vp, vp, C.POINTER(DecodeArgs)])
         bind("mamba_b200_m3_ssd_fwd", [vp, vp, C.POINTER(M3SsdArgs)])

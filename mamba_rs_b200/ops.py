@@ -10,6 +10,7 @@ streams only; every compute call goes through ``libmamba_b200.so``.
 from __future__ import annotations
 
 import ctypes as C
+import math
 
 import torch
 
@@ -21,7 +22,9 @@ __all__ = ["selective_scan_fwd", "selective_scan_fwd_workspace_bytes", "selectiv
            "ssm_parallel_scan_fwd_nosave", "ssm_scan_fwd_save", "ssm_scan_bwd", "conv1d_fwd_nosave", "selective_scan_step", "conv1d_fwd", "conv1d_bwd", "m3_ssd_fwd", "m3_ssd_fwd_fused_kq", "m3_ssd_bwd", "dtype_code",
            "embedding_fwd", "embedding_bwd", "embedding_bwd_workspace_bytes", "token_logprobs", "token_logprobs_bwd",
            "gated_scan_fwd", "gated_scan_bwd", "gated_scan_step", "gated_scan_states",
-           "gated_scan_workspace_bytes"]
+           "gated_scan_workspace_bytes",
+           "linear_attention_fwd", "linear_attention_bwd", "linear_attention_step", "linear_attention_workspace_bytes",
+           "rotary_fwd", "rotary_bwd", "rotary_frequencies", "group_norm_fwd", "group_norm_bwd", "group_norm_workspace_bytes"]
 
 
 _DTYPES = {torch.float32: ffi.F32, torch.float16: ffi.F16, torch.bfloat16: ffi.BF16}
@@ -833,4 +836,320 @@ def gated_scan_bwd(x, f, dy, chunk_states, z=None, *, d_last=None, d_h0=None, d_
     out = dict(d_x=d_x, d_f=d_f, d_h0=d_h0)
     if d_z is not None:
         out["d_z"] = d_z
+    return out
+
+
+def _head_strides(t, name, shape, dtype):
+    """Strides of batch, step and head of a [B, T, heads, width] view with contiguous columns."""
+    if t.dtype != dtype or tuple(t.shape) != shape:
+        raise TypeError(f"{name} is {list(shape)} {dtype}, not {list(t.shape)} {t.dtype}")
+    if t.stride(3) != 1 and shape[3] > 1:
+        raise ValueError(f"{name}: last dimension must be contiguous")
+    return t.stride()[:3]
+
+
+def _written(t, name):
+    """Refuses an output whose elements share memory (an expanded view)."""
+    if any(s == 0 and n > 1 for s, n in zip(t.stride(), t.shape)):
+        raise ValueError(f"{name}: an expanded tensor cannot be written")
+
+
+def _attention_args(q, k, v, decay, scale, state):
+    """LinearAttentionArgs with what forward and backward share, and the shape of a state."""
+    if q.dim() != 4 or k.dim() != 4 or v.dim() != 4:
+        raise ValueError("q, k, v are [B, T, heads, width]")
+    B, T, Hq, K = q.shape
+    Hk, (Hv, V) = k.shape[2], v.shape[2:]
+    if decay.dtype != torch.float32 or decay.dim() != 1 or not decay.is_contiguous():
+        raise TypeError("decay is contiguous float32 [heads]")
+    H = decay.shape[0]
+    for n, h in (("q", Hq), ("k", Hk), ("v", Hv)):
+        if h < 1 or H % h:
+            raise ValueError(f"{n}: {h} heads are not shared by {H} evenly")
+    if not 1 <= K <= 256 or not 1 <= V <= 256:
+        raise ValueError(f"K {K} and V {V} are 1 to 256")
+    a = ffi.LinearAttentionArgs(dtype_code(q.dtype), B, T, H, K, V, Hq, Hk, Hv, K ** -0.5 if scale is None else scale, decay.data_ptr(),
+                                q.data_ptr(), *_head_strides(q, "q", (B, T, Hq, K), q.dtype), k.data_ptr(),
+                                *_head_strides(k, "k", (B, T, Hk, K), q.dtype), v.data_ptr(), *_head_strides(v, "v", (B, T, Hv, V), q.dtype))
+    shape = (B, H, K, V)
+    a.state = _attention_state(state, "state", shape)
+    return a, shape
+
+
+def _attention_state(t, name, shape):
+    if t is not None and (t.dtype != torch.float32 or tuple(t.shape) != shape or not t.is_contiguous()):
+        raise TypeError(f"{name} is contiguous float32 {list(shape)}")
+    return _ptr(t)
+
+
+def _scratch(a, need, workspace, like):
+    """Gives an argument struct its workspace (the caller's, or one made here); the tensor has to outlive the call."""
+    if workspace is None:
+        if not need:
+            return None
+        workspace = torch.empty(need, dtype=torch.uint8, device=like.device)
+    elif not workspace.is_contiguous():
+        raise ValueError("the workspace is contiguous")
+    a.workspace, a.workspace_bytes = workspace.data_ptr(), workspace.numel() * workspace.element_size()
+    return workspace
+
+
+def linear_attention_workspace_bytes(B, T, H, K, V, *, Hq=None, Hk=None, Hv=None, backward=False) -> int:
+    """Bytes of the scratch of linear_attention_fwd (backward: _bwd): states between the segments that a long text of few heads
+    is cut into, and the parts of shared heads' gradients.  0: none is needed."""
+    a = ffi.LinearAttentionArgs(B=B, T=T, H=H, K=K, V=V, Hq=Hq or H, Hk=Hk or H, Hv=Hv or H)
+    return int(ffi.lib().mamba_b200_linear_attention_workspace_bytes(C.byref(a), int(backward)))
+
+
+def linear_attention_fwd(q, k, v, decay, *, scale=None, state=None, state_out=None, o=None, workspace=None, handle=None):
+    """Linear attention with a decay for each head: S_t = exp(decay) S_{t-1} + k_t v_t^T, o_t = scale S_t^T q_t.
+    q [B,T,Hq,K], k [B,T,Hk,K], v [B,T,Hv,V] in a storage dtype with any strides of batch, step and head; decay [H] f32, the log of
+    each head's factor a token; Hq, Hk and Hv divide H (fewer heads are shared by consecutive ones); K, V <= 256; scale: K ** -0.5
+    if None.  state [B,H,K,V] f32 enters (zeros if None), state_out receives what leaves (may be state).  workspace: scratch of
+    linear_attention_workspace_bytes(...) bytes (made here if None).  Returns o [B,T,H,V] in q's dtype.  An infinite or NaN input
+    may show in all outputs of its block of 128 tokens, earlier ones too."""
+    dev = _device_index(q, k, v, decay, state, state_out, o, workspace)
+    a, shape = _attention_args(q, k, v, decay, scale, state)
+    B, H, _, V = shape
+    T = q.shape[1]
+    if o is None:
+        o = torch.empty((B, T, H, V), dtype=q.dtype, device=q.device)
+    a.o = o.data_ptr()
+    a.o_b, a.o_t, a.o_h = _head_strides(o, "o", (B, T, H, V), q.dtype)
+    _written(o, "o")
+    a.state_out = _attention_state(state_out, "state_out", shape)
+    lib = ffi.lib()
+    if T > 1:
+        workspace = _scratch(a, lib.mamba_b200_linear_attention_workspace_bytes(C.byref(a), 0), workspace, q)
+    _launch(lib.mamba_b200_linear_attention_fwd, dev, handle, C.byref(a))
+    return o
+
+
+def linear_attention_step(q, k, v, decay, state, *, scale=None, state_out=None, o=None, handle=None):
+    """One token for each sequence: q [B,Hq,K], k [B,Hk,K], v [B,Hv,V], o [B,H,V]; the state [B,H,K,V] f32 is updated in place, or
+    state_out receives it."""
+    dev = _device_index(q, k, v, decay, state, state_out, o)
+    dtype = q.dtype
+    B, Hq, K = q.shape
+    (_, Hk, K2), (_, Hv, V), H = k.shape, v.shape, decay.shape[0]
+    if k.dtype != dtype or v.dtype != dtype or k.shape[0] != B or v.shape[0] != B or K2 != K:
+        raise TypeError(f"k and v have q's dtype and sequences, k its width: {list(q.shape)} {dtype}")
+    if decay.dtype != torch.float32 or decay.dim() != 1 or not decay.is_contiguous():
+        raise TypeError("decay is contiguous float32 [heads]")
+    shape = (B, H, K, V)
+    for t, name in ((state, "state"), (state_out, "state_out")):
+        if t is not None and (t.dtype != torch.float32 or t.shape != shape or not t.is_contiguous()):
+            raise TypeError(f"{name} is contiguous float32 {list(shape)}")
+    if o is None:
+        o = torch.empty((B, H, V), dtype=dtype, device=q.device)
+    elif o.dtype != dtype or o.shape != (B, H, V):
+        raise TypeError(f"o is {[B, H, V]} {dtype}")
+    else:
+        _written(o, "o")
+
+    def at(t, name):
+        b, h, one = t.stride()
+        if one != 1 and t.shape[2] > 1:
+            raise ValueError(f"{name}: last dimension must be contiguous")
+        return t.data_ptr(), b, 0, h
+
+    s = state.data_ptr()
+    a = ffi.LinearAttentionArgs(dtype_code(dtype), B, 1, H, K, V, Hq, Hk, Hv, K ** -0.5 if scale is None else scale, decay.data_ptr(),
+                                *at(q, "q"), *at(k, "k"), *at(v, "v"), s, s if state_out is None else state_out.data_ptr(), *at(o, "o"))
+    _launch(ffi.lib().mamba_b200_linear_attention_fwd, dev, handle, C.byref(a))
+    return o
+
+
+def linear_attention_bwd(q, k, v, do, decay, *, scale=None, state=None, d_state_out=None, d_q=None, d_k=None, d_v=None, d_state=None,
+                         workspace=None, handle=None):
+    """Backward of linear_attention_fwd from its inputs alone.  do [B,T,H,V] in q's dtype, d_state_out [B,H,K,V] f32 the gradient of the
+    state that left (zeros if None).  Returns dict(d_q, d_k, d_v) in q's dtype (they may be given: columns of one projection's
+    gradient, say; those of shared heads are sums) and, with a state or a d_state to fill, d_state f32, the gradient of the state that
+    entered.  The decays have no gradient here."""
+    dev = _device_index(q, k, v, do, decay, state, d_state_out, d_q, d_k, d_v, d_state, workspace)
+    a, shape = _attention_args(q, k, v, decay, scale, state)
+    B, H, _, V = shape
+    new = lambda t, like: torch.empty(like.shape, dtype=like.dtype, device=like.device) if t is None else t  # noqa: E731
+    d_q, d_k, d_v = new(d_q, q), new(d_k, k), new(d_v, v)
+    if d_state is None and state is not None:
+        d_state = torch.empty(shape, dtype=torch.float32, device=q.device)
+    a.d_o = do.data_ptr()
+    a.do_b, a.do_t, a.do_h = _head_strides(do, "do", (B, q.shape[1], H, V), q.dtype)
+    a.d_state_out, a.d_state = _attention_state(d_state_out, "d_state_out", shape), _attention_state(d_state, "d_state", shape)
+    for n, t, like in (("q", d_q, q), ("k", d_k, k), ("v", d_v, v)):
+        setattr(a, f"d_{n}", t.data_ptr())
+        for d, s in zip("bth", _head_strides(t, f"d_{n}", tuple(like.shape), q.dtype)):
+            setattr(a, f"d{n}_{d}", s)
+        _written(t, f"d_{n}")
+    lib = ffi.lib()
+    workspace = _scratch(a, lib.mamba_b200_linear_attention_workspace_bytes(C.byref(a), 1), workspace, q)
+    _launch(lib.mamba_b200_linear_attention_bwd, dev, handle, C.byref(a))
+    out = dict(d_q=d_q, d_k=d_k, d_v=d_v)
+    if d_state is not None:
+        out["d_state"] = d_state
+    return out
+
+
+def rotary_frequencies(dim, base=10000.0, *, scaling=None, factor=1.0, trained=None, beta_fast=32.0, beta_slow=1.0, device=None):
+    """(inv_freq f32 [dim / 2], scale) for rotary_fwd: base ** (-2 i / dim) for pair i, for texts `factor` times as long as the `trained`
+    ones by scaling
+      "linear"  positions interpolated: every frequency divided by factor
+      "ntk"     a larger base, so that the slowest pair is divided by factor and the fastest stays (dim > 2)
+      "yarn"    pairs of more than beta_fast turns over `trained` positions stay, those of less than beta_slow are divided by factor, a
+                ramp between; scale = 0.1 ln(factor) + 1, once for q and once for k (Peng et al., YaRN, 2023, equations 17 to 22)
+    Computed in 64 bits on the host, rounded once."""
+    if dim < 2 or dim % 2:
+        raise ValueError(f"{dim} columns are no pairs")
+    if not (math.isfinite(base) and base > 0 and math.isfinite(factor) and factor > 0):
+        raise ValueError(f"base {base} and factor {factor} are positive")
+    if scaling not in (None, "linear", "ntk", "yarn"):
+        raise ValueError(f"unknown scaling {scaling!r}")
+    if scaling == "ntk":
+        if dim == 2:
+            raise ValueError("one pair has no slowest one beside its fastest")
+        base = base * factor ** (dim / (dim - 2))
+    pair = torch.arange(dim // 2, dtype=torch.float64)
+    freq, scale = base ** (-2.0 * pair / dim), 1.0
+    if scaling == "linear":
+        freq = freq / factor
+    elif scaling == "yarn":
+        if trained is None or trained < 1 or base <= 1 or not 0 < beta_slow < beta_fast:
+            raise ValueError("yarn needs the length trained on, a base above 1, and beta_slow below beta_fast")
+        # the pair that makes n turns over the trained length: trained * base ** (-2 i / dim) = 2 pi n
+        at = [dim * math.log(trained / (2 * math.pi * n)) / (2 * math.log(base)) for n in (beta_fast, beta_slow)]
+        low, high = max(math.floor(at[0]), 0), min(math.ceil(at[1]), dim - 1)
+        slow = ((pair - low) / max(high - low, 1e-3)).clamp(0, 1)
+        freq = freq / factor * slow + freq * (1 - slow)
+        scale = 0.1 * math.log(factor) + 1.0 if factor > 1 else 1.0
+    return freq.to(torch.float32).to(device or "cpu"), scale
+
+
+def _rotary(q, k, positions, inv_freq, interleaved, scale, inverse, q_out, k_out, handle):
+    dev = _device_index(q, k, positions, inv_freq, q_out, k_out)
+    if q.dim() != 4 or (k is not None and k.dim() != 4):
+        raise ValueError("q and k are [B, T, heads, width]")
+    B, T, Hq, D = q.shape
+    if inv_freq.dtype != torch.float32 or inv_freq.dim() != 1 or not inv_freq.is_contiguous() or 2 * inv_freq.shape[0] > D:
+        raise TypeError(f"inv_freq is contiguous float32 of at most {D // 2} pairs")
+    if positions.dtype != torch.int32 or not positions.is_contiguous() or tuple(positions.shape) not in ((T,), (B, T)):
+        raise TypeError(f"positions are contiguous int32 [{T}] or [{B}, {T}]")
+    if q_out is None:
+        q_out = torch.empty((B, T, Hq, D), dtype=q.dtype, device=q.device)
+    a = ffi.RotaryArgs(dtype_code(q.dtype), B, T, Hq, 0, D, 2 * inv_freq.shape[0], bool(interleaved), inverse, scale, positions.data_ptr(),
+                       T if positions.dim() == 2 else 0, inv_freq.data_ptr(), q.data_ptr(), *_head_strides(q, "q", (B, T, Hq, D), q.dtype),
+                       q_out.data_ptr(), *_head_strides(q_out, "q_out", (B, T, Hq, D), q.dtype))
+    _written(q_out, "q_out")
+    if k is not None:
+        shape = (B, T, k.shape[2], D)
+        if k_out is None:
+            k_out = torch.empty(shape, dtype=q.dtype, device=q.device)
+        a.Hk = shape[2]
+        a.k, (a.k_b, a.k_t, a.k_h) = k.data_ptr(), _head_strides(k, "k", shape, q.dtype)
+        a.k_out, (a.ko_b, a.ko_t, a.ko_h) = k_out.data_ptr(), _head_strides(k_out, "k_out", shape, q.dtype)
+        _written(k_out, "k_out")
+    _launch(ffi.lib().mamba_b200_rotary, dev, handle, C.byref(a))
+    return q_out, k_out
+
+
+def rotary_fwd(q, k, positions, inv_freq, *, interleaved=False, scale=1.0, q_out=None, k_out=None, handle=None):
+    """Rotation by position: pair i of each head's first 2 len(inv_freq) columns is turned by positions * inv_freq[i] (64 bits before
+    sine and cosine) and multiplied by scale; the columns behind are handed on.  Pairs are columns 2i, 2i + 1 (interleaved) or i and
+    i + len(inv_freq).  q [B,T,Hq,D], k [B,T,Hk,D] (or None) in a storage dtype with any strides of batch, step and head; positions int32
+    [T] or [B,T]; inv_freq f32 (rotary_frequencies makes one).  q_out / k_out may be q / k themselves.  Returns (q_out, k_out)."""
+    return _rotary(q, k, positions, inv_freq, interleaved, scale, False, q_out, k_out, handle)
+
+
+def rotary_bwd(d_q, d_k, positions, inv_freq, *, interleaved=False, scale=1.0, q_out=None, k_out=None, handle=None):
+    """Gradients of rotary_fwd's q and k from those of its results: the rotation the other way, with the same scale."""
+    return _rotary(d_q, d_k, positions, inv_freq, interleaved, scale, True, q_out, k_out, handle)
+
+
+def group_norm_workspace_bytes(N, S, C_, G, backward=False) -> int:
+    """Bytes of the scratch of group_norm_fwd (backward: _bwd): sums of blocks of rows."""
+    return int(ffi.lib().mamba_b200_group_norm_workspace_bytes(N, S, C_, G, int(backward)))
+
+
+def _norm_rows(t, name, like):
+    """Row stride of an [N, S, C] (or [N, C]) view whose rows are one after another."""
+    if t.dtype != like.dtype or t.shape != like.shape:
+        raise TypeError(f"{name} has x's dtype and shape: {list(like.shape)} {like.dtype}")
+    if t.stride(-1) != 1 and t.shape[-1] > 1:
+        raise ValueError(f"{name}: last dimension must be contiguous")
+    C_ = t.shape[-1]
+    if t.dim() == 2:
+        return t.stride(0) if t.shape[0] > 1 else C_
+    N, S = t.shape[:2]
+    if S <= 1:
+        return t.stride(0) if N > 1 and S else C_
+    if N > 1 and t.stride(0) != S * t.stride(1):
+        raise ValueError(f"{name}: sample stride must equal S * row stride")
+    return t.stride(1)
+
+
+def _norm_args(x, z, weight, bias, groups, activation, eps):
+    if x.dim() not in (2, 3):
+        raise ValueError("x is [N, S, C] or [N, C]")
+    N, C_ = x.shape[0], x.shape[-1]
+    if groups < 1 or C_ < 1 or C_ % groups:
+        raise ValueError(f"{C_} channels are no {groups} groups")
+    if activation not in ffi.ACTIVATIONS:
+        raise ValueError(f"unknown activation {activation!r}")
+    for t, n in ((weight, "weight"), (bias, "bias")):
+        if t is not None and (t.dtype != torch.float32 or tuple(t.shape) != (C_,) or not t.is_contiguous()):
+            raise TypeError(f"{n} is contiguous float32 [{C_}]")
+    return ffi.GroupNormArgs(dtype_code(x.dtype), N, 1 if x.dim() == 2 else x.shape[1], C_, groups, ffi.ACTIVATIONS[activation], eps,
+                             x.data_ptr(), _norm_rows(x, "x", x), _ptr(z), 0 if z is None else _norm_rows(z, "z", x), _ptr(weight), _ptr(bias))
+
+
+def group_norm_fwd(x, weight, bias, groups, *, eps=1e-5, activation=None, z=None, y=None, stats=None, workspace=None, handle=None):
+    """Group norm with channels last: y = act((x - mean) / sqrt(var + eps) * weight + bias) * SiLU(z).  x, z, y [N,S,C] in a storage dtype
+    (any row stride), mean and var over a sample's S rows and the C / groups channels of a group; [N,C] is S = 1, each row by itself
+    (a group for each head, say).  weight, bias [C] f32 or None; activation None, "silu" or "gelu" (by erf); z None: no gate.
+    Returns (y, stats): mean and rstd f32 [2,N,groups], which group_norm_bwd takes."""
+    dev = _device_index(x, weight, bias, z, y, stats, workspace)
+    a = _norm_args(x, z, weight, bias, groups, activation, eps)
+    if y is None:
+        y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    if stats is None:
+        stats = torch.empty((2, x.shape[0], groups), dtype=torch.float32, device=x.device)
+    elif stats.dtype != torch.float32 or tuple(stats.shape) != (2, x.shape[0], groups) or not stats.is_contiguous():
+        raise TypeError(f"stats is contiguous float32 {[2, x.shape[0], groups]}")
+    a.stats, a.y, a.ld_y = stats.data_ptr(), y.data_ptr(), _norm_rows(y, "y", x)
+    _written(y, "y")
+    lib = ffi.lib()
+    workspace = _scratch(a, lib.mamba_b200_group_norm_workspace_bytes(a.N, a.S, a.C, a.G, 0), workspace, x)
+    _launch(lib.mamba_b200_group_norm_fwd, dev, handle, C.byref(a))
+    return y, stats
+
+
+def group_norm_bwd(dy, x, stats, weight, bias, groups, *, activation=None, z=None, d_x=None, d_z=None, d_weight=None, d_bias=None,
+                   workspace=None, handle=None):
+    """Backward of group_norm_fwd from its inputs and stats.  Returns dict(d_x, d_weight, d_bias f32 [C], d_z (with z)).  d_x and d_z may
+    be given and are overwritten (d_x may be dy or x, d_z may be z); d_weight and d_bias, given both, are added to (a gradient arena),
+    else made."""
+    dev = _device_index(x, dy, stats, weight, bias, z, d_x, d_z, d_weight, d_bias, workspace)
+    a = _norm_args(x, z, weight, bias, groups, activation, 0.0)
+    if stats.dtype != torch.float32 or tuple(stats.shape) != (2, x.shape[0], groups) or not stats.is_contiguous():
+        raise TypeError(f"stats is contiguous float32 {[2, x.shape[0], groups]}")
+    if (d_weight is None) != (d_bias is None):
+        raise ValueError("d_weight and d_bias are given both or neither")
+    a.accumulate = d_weight is not None
+    if d_weight is None:
+        d_weight, d_bias = torch.empty((2, a.C), dtype=torch.float32, device=x.device)
+    for t, n in ((d_weight, "d_weight"), (d_bias, "d_bias")):
+        if t.dtype != torch.float32 or tuple(t.shape) != (a.C,) or not t.is_contiguous():
+            raise TypeError(f"{n} is contiguous float32 [{a.C}]")
+    new = lambda t: torch.empty(x.shape, dtype=x.dtype, device=x.device) if t is None else t  # noqa: E731
+    d_x = new(d_x)
+    a.stats, a.dy, a.ld_dy = stats.data_ptr(), dy.data_ptr(), _norm_rows(dy, "dy", x)
+    a.d_x, a.ld_dx, a.d_weight, a.d_bias = d_x.data_ptr(), _norm_rows(d_x, "d_x", x), d_weight.data_ptr(), d_bias.data_ptr()
+    _written(d_x, "d_x")
+    out = dict(d_x=d_x, d_weight=d_weight, d_bias=d_bias)
+    if z is not None:
+        out["d_z"] = d_z = new(d_z)
+        a.d_z, a.ld_dz = d_z.data_ptr(), _norm_rows(d_z, "d_z", x)
+        _written(d_z, "d_z")
+    lib = ffi.lib()
+    workspace = _scratch(a, lib.mamba_b200_group_norm_workspace_bytes(a.N, a.S, a.C, a.G, 1), workspace, x)
+    _launch(lib.mamba_b200_group_norm_bwd, dev, handle, C.byref(a))
     return out
