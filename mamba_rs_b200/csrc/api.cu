@@ -92,6 +92,7 @@ int gated_scan_configure(Ctx* c);  // gated_scan.cu
 int logprobs_configure(Ctx* c);    // logprobs.cu
 int embedding_configure(Ctx* c);   // embedding.cu
 int linear_attention_configure(Ctx* c);  // linear_attention.cu
+int linear_attention_tc_configure(Ctx* c);  // linear_attention_tc.cu
 
 }  // namespace mb200
 
@@ -142,6 +143,8 @@ extern "C" MAMBA_B200_API int mamba_b200_init(int device, void** handle) {
     rc = embedding_configure(c);
     if (rc) return rc;
     rc = linear_attention_configure(c);
+    if (rc) return rc;
+    rc = linear_attention_tc_configure(c);
     if (rc) return rc;
     return MAMBA_B200_OK;
 }

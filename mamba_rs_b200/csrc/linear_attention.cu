@@ -401,6 +401,9 @@ int hand_on(Ctx* c, const float* in, float* out, const mamba_b200_linear_attenti
 
 int dispatch(Ctx* c, const mamba_b200_linear_attention_args& a, Params& p, bool may_cut, cudaStream_t st) {
     const long long pairs = static_cast<long long>(a.B) * a.H;
+    bool taken = false;
+    const int rc = tc_launch(c, a.dtype, p, may_cut, pairs, st, &taken);
+    if (rc || taken) return rc;
     if (a.dtype == MAMBA_B200_F32) return launch_general<float>(c, p, may_cut, pairs, st);
     if (a.dtype == MAMBA_B200_F16) return launch_general<__half>(c, p, may_cut, pairs, st);
     return launch_general<__nv_bfloat16>(c, p, may_cut, pairs, st);

@@ -92,7 +92,8 @@ __device__ __forceinline__ float times(const Pow& f, float s) { return fmaf(f.hi
 // l^n, n >= 0, in 32 bits (n = 0: 1 for every decay, minus infinity among them)
 __device__ __forceinline__ float decay_at(float log2_decay, int n) { return n > 0 ? exp2f(log2_decay * n) : 1.0f; }
 
-int tc_launch(Ctx* c, const mamba_b200_linear_attention_args& a, Params& p, cudaStream_t st, bool* taken);
+// linear_attention_tc.cu: launches, if it takes such a call (`taken`).
+int tc_launch(Ctx* c, int dtype, Params& p, bool may_cut, long long pairs, cudaStream_t st, bool* taken);
 
 }  // namespace la
 }  // namespace mb200

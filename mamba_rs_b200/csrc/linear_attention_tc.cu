@@ -1,0 +1,813 @@
+// Linear attention with a decay for each head on the tensor cores: 16-bit rows that TMA can describe, K and V up to 128.
+//
+// A block has 64 columns of one pair's (sequence, head) state and walks chunks of 128 steps (roles and names: linear_attention.cuh):
+//   G = X Y^T,  P = G o l^{distance},  out = P Z + l^{row} o (X S),  S <- l^n S + Y^T (w o Z)
+// Beside HBM, which a chunk of 128 x 64 heads of 128 x 64 keeps busy for 4100 cycles an SM, its products take 1500 cycles of the
+// tensor pipe, so one block on an SM reaches HBM's rate if nothing waits for anything else: every part has warps of its own, and the
+// state, the only thing that is carried from chunk to chunk, stays in tensor memory,
+//   warp 0      asks for the tiles, as many chunks ahead as there are stages
+//   warp 1      issues X Y^T of the next chunk and P Z of this one
+//   warp 2      issues Y^T (w o Z) and X S, the chain from chunk to chunk
+//   warps 4-7   make P from G, of every other chunk; it goes back to tensor memory and is read there as an operand
+//   warps 8-11  leave a 16-bit copy of S for X S, and in its place what is left of it after the chunk
+//   warps 12-15 join P Z and X S and write rows
+//   warps 16-19 weigh Z
+//   warps 20-23 make P of the other chunks
+// and they meet on mbarriers alone; every wait gives up after a limit and takes the block to its end.
+//
+// Roundings to 16 bits: P (made from f32 scores) and the copy of S that is read, each once, as the result is.  The state itself is f32:
+// w o Z, which it is made of, is kept to f32 accuracy where a state is handed on: three bf16 terms of 8 bits each; where only out is
+// wanted one term is enough.  In f16 a second term of 2^-11 of the first gives 22 bits, P is scaled by a power of two a row and S by
+// one a tile, so that neither their size nor their smallness leaves the type.
+#include <math.h>
+#include <string.h>
+
+#include <type_traits>
+
+#include "linear_attention.cuh"
+#include "m3_tc.cuh"
+
+namespace mb200 {
+namespace la {
+namespace tcl {
+
+using namespace mb200::tc;
+
+constexpr int kThreads = 768, kTile = 64;
+constexpr uint32_t kSub = kSwSub;  // a [128 x 64] sub-tile
+// Tensor memory: two buffers of G, whose left half P takes and whose right half P Z; two of X S; S and, in f16, the sum of its second
+// terms.
+constexpr uint32_t cG = 0, cY1 = 64, cY2 = 256, cS = 384, cSlo = 448, kCols = 512;
+
+struct TcParams {
+    CUtensorMap x[3], y[3], z[3], out[3];
+    Params p;
+    int na, stages, z_stages;  // sub-tiles of X (and of Y) in a stage; stages of X and Y, of Z
+    int out_map[3];  // 1: out can be described too, and rows leave in tiles of 32
+};
+
+// Copies of S and stages of Z, in the room that two stages of X and Y (of two sub-tiles) and w o Z leave.
+template <int TERMS>
+constexpr int kCopies = TERMS == 1 ? 2 : 1;
+template <int TERMS>
+constexpr int kMostZ = TERMS == 3 ? 2 : 3;
+
+// behind the stages, the terms of w o Z and the copies of S
+struct Small {
+    float col[32];         // l^{31 - u} (back: l^u)
+    float diag[64];        // alpha_p l^{d} at 31 + d
+    float row_scale[2][128];
+    float tile_scale[4];  // (a copy's is read until its rows are out, which is known of the chunk three before)
+    float warp_max[2][4];
+    uint64_t full[4], empty[4], z_full[4], z_empty[4], g_full[2], p_full[2], y_full[2], x_full[2], y_empty[2], s_full[2], s_empty[2], w_full, d_full, max_full, drain[2];
+    uint32_t tmem;
+    int dead;
+};
+
+template <int TERMS>
+uint32_t smem_bytes(int na, int stages, int z_stages) {
+    return (stages * 2 * na + z_stages + TERMS + kCopies<TERMS>) * kSub + sizeof(Small);
+}
+
+__device__ __forceinline__ void mma_ta(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, bool accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
+        "r"(a), "l"(b), "r"(idesc), "r"(accumulate ? 1u : 0u)
+        : "memory");
+}
+__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t* w) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(taddr),
+        "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]), "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7]), "r"(w[8]), "r"(w[9]), "r"(w[10]), "r"(w[11]),
+        "r"(w[12]), "r"(w[13]), "r"(w[14]), "r"(w[15])
+        : "memory");
+}
+__device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+// A bounded wait that also ends when another role has given up.
+__device__ __forceinline__ bool look(uint64_t* bar, uint32_t parity) {
+    uint32_t ok;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(ok)
+        : "r"(smem_u32(bar)), "r"(parity)
+        : "memory");
+    return ok != 0;
+}
+__device__ __noinline__ bool wait_on(uint64_t* bar, uint32_t parity, Small* sm, int* status) {
+    for (int it = 0; it < kMbarMaxPolls; ++it) {
+        if (look(bar, parity)) return true;
+        if ((it & 15) == 15 && *reinterpret_cast<volatile int*>(&sm->dead)) return false;
+    }
+    *reinterpret_cast<volatile int*>(&sm->dead) = 1;
+    atomicCAS(status, kStatusOk, kStatusBarrierTimeout);
+    return false;
+}
+__device__ __forceinline__ bool wait(uint64_t* bar, uint32_t parity, Small* sm, int* status) {
+    return look(bar, parity) || wait_on(bar, parity, sm, status);
+}
+__device__ __forceinline__ bool wait_warp(uint64_t* bar, uint32_t parity, Small* sm, int* status) {
+    return __all_sync(0xffffffffu, wait(bar, parity, sm, status));
+}
+
+// One lane of a converged warp.  The products' warp goes through its loop as a whole and this lane issues them: descriptors then stay
+// in uniform registers (a branch on the lane's number had them moved there one by one, 130 cycles a product).
+__device__ __forceinline__ bool elect_one() {
+    uint32_t one;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(one));
+    return one != 0;
+}
+
+// 2^e that brings a magnitude to [2^13, 2^14), and back (0, infinities and NaN: as it is)
+__device__ __forceinline__ float scale_to(float m, float* back) {
+    const int e = static_cast<int>((__float_as_uint(m) >> 23) & 255);
+    if (e == 255 || m == 0.0f) {
+        *back = 1.0f;
+        return 1.0f;
+    }
+    const int d = min(max(e - 127 - 13, -110), 110);
+    *back = __uint_as_float(static_cast<uint32_t>(127 + d) << 23);
+    return __uint_as_float(static_cast<uint32_t>(127 - d) << 23);
+}
+
+template <typename Th, int TERMS, bool STATE>
+__global__ void __launch_bounds__(kThreads, 1) walk_kernel(const __grid_constant__ TcParams tp) {
+    constexpr bool F16 = std::is_same<Th, __half>::value;
+    constexpr int SB = kCopies<TERMS>;
+    constexpr uint32_t fmt = F16 ? 0u : 1u;
+    extern __shared__ __align__(1024) unsigned char smem[];
+    const Params& p = tp.p;
+    const Place w = place(p, blockIdx.x, STATE ? p.segments - 1 : p.segments);
+    const Role& r = p.role[w.role];
+    const int A = r.A, W = r.W, na = (A + 63) >> 6, c0 = w.tile * kTile, stages = tp.stages, zs = tp.z_stages;
+    const uint32_t stage = 2 * tp.na * kSub, oY = tp.na * kSub, kZ = stages * stage, kW = kZ + zs * kSub, kS = kW + TERMS * kSub;
+    Small* sm = reinterpret_cast<Small*>(smem + kS + SB * kSub);
+    const uint32_t sbase = smem_u32(smem);
+    const int b = static_cast<int>(w.pair / p.H), h = static_cast<int>(w.pair - static_cast<long long>(b) * p.H);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, role = warp >> 2, row = threadIdx.x & 127;
+    const bool back = r.backwards;
+    const float ld = p.decay[h], l2 = ld * kLog2e;
+    // chunks of this segment, numbered as they are walked
+    const int all = (p.T + kChunk - 1) / kChunk, per = p.seg_len / kChunk;
+    const int first = w.seg * per, n = min(all - first, per);
+    auto start = [&](int i) { return (back ? all - 1 - (first + i) : first + i) * kChunk; };
+    const bool enters = w.seg > 0 ? !STATE : r.s_in != nullptr;
+    const bool leaves = STATE || (w.seg + 1 == p.segments && r.s_out != nullptr);
+    const int late0 = r.late && w.seg == 0 ? 1 : 0;  // of chunk 0
+
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < 4; ++i) {
+            mbar_init(&sm->full[i], 1);
+            mbar_init(&sm->empty[i], STATE ? 1 : 2);
+            mbar_init(&sm->z_full[i], 1);
+            mbar_init(&sm->z_empty[i], STATE ? 1 : 4);
+        }
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(&sm->g_full[i], 1);
+            mbar_init(&sm->p_full[i], 128);
+            mbar_init(&sm->s_full[i], 128);
+            mbar_init(&sm->s_empty[i], 1);
+            mbar_init(&sm->x_full[i], 1);
+            mbar_init(&sm->y_full[i], 1);
+            mbar_init(&sm->y_empty[i], 128);
+            mbar_init(&sm->drain[i], 1);
+        }
+        mbar_init(&sm->w_full, 128);
+        mbar_init(&sm->d_full, 1);
+        mbar_init(&sm->max_full, 128);
+        sm->dead = 0;
+        fence_barrier_init();
+    }
+    if (threadIdx.x >= 32 && threadIdx.x < 64) {
+        sm->col[lane] = decay_at(l2, back ? lane : 31 - lane);
+        sm->diag[lane] = 0.0f;  // (31 is written below)
+        __syncwarp();
+        sm->diag[31 + lane] = decay_at(l2, lane) * r.alpha_p;
+    }
+    if (warp == 1) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&sm->tmem)), "r"(kCols) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    fence_before();
+    __syncthreads();
+    fence_after();
+    const uint32_t tmem = sm->tmem;
+    const uint32_t lanes = tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16);  // this warp's 32 rows
+
+    const uint32_t per_stage = stage >> 4;  // in descriptors
+    constexpr uint32_t kStep = 32 >> 4, mStep = 2048 >> 4, sub = kSub >> 4;
+
+    if (warp == 0 || warp == 3) {
+        if (lane == 0) {
+            // X and Y are free when the products of S are, Z only with the rows
+            const bool z = warp == 3;
+            const int hx = h / r.x.group, hy = h / r.y.group, hz = h / r.z.group, depth = z ? zs : stages;
+            uint64_t* full = z ? sm->z_full : sm->full;
+            uint64_t* empty = z ? sm->z_empty : sm->empty;
+            int asked = 0;
+            for (int i = 0, st = 0, turn = 0; i < n; ++i) {
+                const int t0 = start(i);
+                if (turn && !wait(&empty[st], (turn - 1) & 1, sm, p.status)) break;
+                if (z) {
+                    mbar_expect_tx(&full[st], kSub);
+                    tma_load_4d(smem + kZ + st * kSub, &tp.z[w.role], &full[st], c0, hz, t0, b);
+                } else {
+                    unsigned char* at = smem + st * stage;
+                    mbar_expect_tx(&full[st], (STATE ? 1 : 2) * na * kSub);
+                    for (int s = 0; s < na; ++s) {
+                        if (!STATE) tma_load_4d(at + s * kSub, &tp.x[w.role], &full[st], 64 * s, hx, t0, b);
+                        tma_load_4d(at + oY + s * kSub, &tp.y[w.role], &full[st], 64 * s, hy, t0, b);
+                    }
+                }
+                asked = i + 1;
+                if (++st == depth) {
+                    st = 0;
+                    ++turn;
+                }
+            }
+            // nothing may be in flight when the block ends (where all went well, it has long landed)
+            for (int i = max(0, asked - depth); i < asked; ++i) mbar_wait(&full[i % depth], (i / depth) & 1, p.status);
+        }
+    } else if (warp == 1) {
+        // ---- X Y^T and P Z ----
+        if (!STATE) {
+            const uint32_t idG = instr_desc(fmt, 0, 0, 128), idY = instr_desc(fmt, 0, 1, 64);
+            // descriptors of stage 0; a step along K is a constant more (m3_tc.cuh), a stage `per_stage`
+            const uint64_t xk = desc_sw_k(sbase, 0), yk = desc_sw_k(sbase + oY, 0), zm = desc_sw_mn(sbase + kZ, 0);
+            bool ok = true;
+            int st = 0, turn = 0, sz = 0, turn_z = 0;  // of the next G; of P Z
+            for (int i = -1; i < n; ++i) {
+                const uint32_t at = st * per_stage;
+                if (i + 1 < n) {
+                    // G of chunk i + 1; the rows of chunk i - 1 have left the buffer that it takes
+                    if (i > 0) ok = wait_warp(&sm->y_empty[(i - 1) & 1], ((i - 1) >> 1) & 1, sm, p.status);
+                    if (ok) ok = wait_warp(&sm->full[st], turn & 1, sm, p.status);
+                    if (!ok) break;
+                    fence_after();
+                    const uint32_t d = tmem + cG + ((i + 1) & 1) * 128;
+                    if (elect_one()) {
+#pragma unroll
+                        for (int k = 0; k < 4; ++k) mma(d, xk + at + k * kStep, yk + at + k * kStep, idG, k > 0);
+                        if (na == 2) {
+#pragma unroll
+                            for (int k = 0; k < 4; ++k) mma(d, xk + at + sub + k * kStep, yk + at + sub + k * kStep, idG, true);
+                        }
+                        commit(&sm->g_full[(i + 1) & 1]);
+                        commit(&sm->empty[st]);
+                    }
+                    __syncwarp();
+                }
+                if (i >= 0) {
+                    // P Z of chunk i
+                    ok = wait_warp(&sm->z_full[sz], turn_z & 1, sm, p.status);
+                    if (ok) ok = wait_warp(&sm->p_full[i & 1], (i >> 1) & 1, sm, p.status);
+                    if (!ok) break;
+                    fence_after();
+                    const uint32_t g = tmem + cG + (i & 1) * 128, z = sz * sub;
+                    if (elect_one()) {
+#pragma unroll
+                        for (int k = 0; k < kChunk / 16; ++k) mma_ta(g + cY1, g + k * 8, zm + z + k * mStep, idY, k > 0);
+                        commit(&sm->y_full[i & 1]);
+                    }
+                    __syncwarp();
+                    if (++sz == zs) {
+                        sz = 0;
+                        ++turn_z;
+                    }
+                }
+                if (++st == stages) {
+                    st = 0;
+                    ++turn;
+                }
+            }
+            if (!ok) {  // what was issued has to end before tensor memory is given back
+                if (elect_one()) commit(&sm->drain[0]);
+                __syncwarp();
+                mbar_wait(&sm->drain[0], 0, p.status);
+            }
+        }
+    } else if (warp == 2) {
+        // ---- Y^T (w o Z) and X S ----
+        const uint32_t idY = instr_desc(fmt, 0, 1, 64), idD = instr_desc(fmt, 1, 1, 64);
+        const uint64_t xk = desc_sw_k(sbase, 0), ym = desc_sw_mn(sbase + oY, 0);
+        const uint64_t wm = desc_sw_mn(sbase + kW, 0), sc = desc_sw_mn(sbase + kS, 0);
+        bool ok = true;
+        int st = 0, turn = 0;
+        for (int i = 0; i < n; ++i) {
+            const uint32_t at = st * per_stage;
+            const bool reads = i > 0 || enters;
+            const int u = enters ? i : i - 1;  // number of the copy of S
+            ok = wait_warp(&sm->full[st], turn & 1, sm, p.status);
+            // a copy of S, and what is left of S in its place
+            if (ok && reads) ok = wait_warp(&sm->s_full[STATE ? 0 : u % SB], (STATE ? u : u / SB) & 1, sm, p.status);
+            if (!ok) break;
+            if (leaves || i + 1 < n) {
+                ok = wait_warp(&sm->w_full, i & 1, sm, p.status);
+                if (!ok) break;
+                fence_after();
+                if (elect_one()) {
+#pragma unroll
+                    for (int t = 0; t < TERMS; ++t) {
+                        const bool own = F16 && t == 1;  // (the second f16 term is summed apart)
+#pragma unroll
+                        for (int k = 0; k < kChunk / 16; ++k)
+                            mma(tmem + (own ? cSlo : cS), ym + at + k * mStep, wm + t * sub + k * mStep, idD, reads || k > 0 || (t > 0 && !own));
+                    }
+                    commit(&sm->d_full);
+                }
+                __syncwarp();
+            }
+            if (!STATE) {
+                if (i > 1) ok = wait_warp(&sm->y_empty[i & 1], ((i >> 1) - 1) & 1, sm, p.status);
+                if (!ok) break;
+                fence_after();
+                const uint32_t d = tmem + cY2 + (i & 1) * 64, copy = (u % SB) * sub;
+                if (elect_one()) {
+                    if (reads) {
+#pragma unroll
+                        for (int k = 0; k < 4; ++k) mma(d, xk + at + k * kStep, sc + copy + k * mStep, idY, k > 0);
+                        if (na == 2) {
+#pragma unroll
+                            for (int k = 0; k < 4; ++k) mma(d, xk + at + sub + k * kStep, sc + copy + (4 + k) * mStep, idY, true);
+                        }
+                        commit(&sm->s_empty[u % SB]);
+                    }
+                    commit(&sm->x_full[i & 1]);
+                }
+                __syncwarp();
+            }
+            if (elect_one()) {
+                commit(&sm->empty[st]);
+                if (STATE) commit(&sm->z_empty[i % zs]);
+            }
+            __syncwarp();
+            if (++st == stages) {
+                st = 0;
+                ++turn;
+            }
+        }
+        if (!ok) {
+            if (elect_one()) commit(&sm->drain[1]);
+            __syncwarp();
+            mbar_wait(&sm->drain[1], 0, p.status);
+        }
+    } else if (role == 1 || role == 5) {
+        // ---- P ----
+        if (!STATE) {
+            const int q = warp & 3;  // the 32 columns that hold this warp's diagonal
+            // other blocks: l^{row - column} in two factors, col[u] = l^{31 - u} (back: l^u) and what is left, here of the blocks one, two and
+            // three away
+            float rf[3];
+#pragma unroll
+            for (int k = 0; k < 3; ++k) rf[k] = decay_at(l2, back ? 32 * (k + 1) - lane : lane + 32 * (k + 1) - 31) * r.alpha_p;
+            const float* diag = sm->diag + 31 + (back ? -lane : lane);
+            for (int i = role == 1 ? 0 : 1; i < n; i += 2) {
+                if (!wait_warp(&sm->g_full[i & 1], (i >> 1) & 1, sm, p.status)) break;
+                fence_after();
+                const uint32_t g0 = lanes + cG + (i & 1) * 128;
+                // weighted scores of block k
+                auto weigh = [&](int k, float* g) {
+                    tmem_ld32(g0 + 32 * k, g);
+                    if (k == q) {
+#pragma unroll
+                        for (int u = 0; u < 32; ++u) {
+                            // (a choice, not a product with 0: what lies behind the edge may be infinite)
+                            const bool in = back ? u >= lane : u <= lane;
+                            g[u] = in ? g[u] * diag[back ? u : -u] : 0.0f;
+                        }
+                    } else {
+                        const int away = back ? k - q : q - k;
+                        const float2 f = splat2(away == 1 ? rf[0] : away == 2 ? rf[1] : rf[2]);
+#pragma unroll
+                        for (int u = 0; u < 32; u += 4) {
+                            const float4 c = *reinterpret_cast<const float4*>(sm->col + u);
+                            const float2 a = mul2(mul2(make_float2(g[u], g[u + 1]), make_float2(c.x, c.y)), f);
+                            const float2 e = mul2(mul2(make_float2(g[u + 2], g[u + 3]), make_float2(c.z, c.w)), f);
+                            g[u] = a.x; g[u + 1] = a.y; g[u + 2] = e.x; g[u + 3] = e.y;
+                        }
+                    }
+                };
+                float scale = 1.0f;
+                if (F16) {
+                    float m = 0.0f;
+#pragma unroll 1
+                    for (int k = back ? q : 0; k <= (back ? 3 : q); ++k) {
+                        float g[32];
+                        weigh(k, g);
+#pragma unroll
+                        for (int u = 0; u < 32; ++u) m = fmaxf(m, fabsf(g[u]));
+                    }
+                    float undo;
+                    scale = scale_to(m, &undo);
+                    sm->row_scale[i & 1][row] = undo;
+                }
+                // (P takes the place of G's columns that have been read: from the left.  One block a turn: code unrolled over a chunk waits for
+                // instructions, 8000 cycles a chunk)
+#pragma unroll 1
+                for (int k = 0; k < 4; ++k) {
+                    uint32_t o[16];
+                    if (back ? k >= q : k <= q) {
+                        float g[32];
+                        weigh(k, g);
+#pragma unroll
+                        for (int u = 0; u < 16; ++u) o[u] = F16 ? pack2<Th>(g[2 * u] * scale, g[2 * u + 1] * scale) : pack2<Th>(g[2 * u], g[2 * u + 1]);
+                    } else {
+#pragma unroll
+                        for (int u = 0; u < 16; ++u) o[u] = 0;
+                    }
+                    tmem_st16(g0 + 16 * k, o);
+                }
+                tmem_st_wait();
+                fence_before();
+                mbar_arrive(&sm->p_full[i & 1]);
+            }
+        }
+    } else if (role == 2) {
+        // ---- S ----
+        const long long slot = static_cast<long long>(A) * W;
+        float* slots = r.slots ? r.slots + w.pair * p.segments * slot : nullptr;
+        const bool mine = row < A;
+        const int nc = min(kTile, W - c0);
+        if (enters) {
+            const long long e = static_cast<long long>(row) * W + c0;
+            const bool given = w.seg == 0 && (STATE || p.segments == 1);
+            const float* in = given ? r.s_in + w.pair * slot + static_cast<long long>(row) * r.sa + static_cast<long long>(c0) * r.sw : slots + e;
+            const int step = given ? r.sw : 1;
+            const Pow f = decay_pow(ld, p.seg_len);
+#pragma unroll 1
+            for (int s = 0; s < 2; ++s) {
+                float v[32];
+#pragma unroll
+                for (int c = 0; c < 32; ++c) {
+                    v[c] = 0.0f;
+                    if (mine && 32 * s + c < nc && w.seg == 0) v[c] = in[static_cast<long long>(32 * s + c) * step];
+                }
+#pragma unroll 1
+                for (int k = 1; k <= w.seg; ++k) {
+#pragma unroll
+                    for (int c = 0; c < 32; ++c)
+                        if (mine && 32 * s + c < nc) v[c] = (k > 1 ? times(f, v[c]) : 0.0f) + slots[k * slot + e + 32 * s + c];
+                }
+                if (STATE && mine) {
+#pragma unroll
+                    for (int c = 0; c < 32; ++c)
+                        if (32 * s + c < nc) slots[e + 32 * s + c] = v[c];
+                }
+                tmem_st32(lanes + cS + 32 * s, v);
+                if (F16) {
+#pragma unroll
+                    for (int c = 0; c < 32; ++c) v[c] = 0.0f;
+                    tmem_st32(lanes + cSlo + 32 * s, v);
+                }
+            }
+        }
+        const Pow whole = decay_pow(ld, kChunk);
+        // 32 columns of S
+        auto read = [&](int s, float* v, float* lo) {
+            if (F16) {
+                tmem_ld32x2(lanes + cS + 32 * s, v, lanes + cSlo + 32 * s, lo);
+            } else {
+                tmem_ld32(lanes + cS + 32 * s, v);
+            }
+        };
+        int u = 0;  // copies of S
+        bool ok = true;
+        for (int i = 0; i < n; ++i) {
+            const int rows = min(kChunk, p.T - start(i));
+            const bool adds = leaves || i + 1 < n;
+            if (i > 0) {
+                ok = wait_warp(&sm->d_full, (i - 1) & 1, sm, p.status);
+                if (!ok) break;
+                fence_after();
+            }
+            if (i > 0 || enters) {
+                // S enters chunk i: a copy for X S, and what is left of it when the chunk is over
+                float scale = 1.0f;
+                if (!STATE) {
+                    if (F16) {
+                        float m = 0.0f;
+#pragma unroll 1
+                        for (int s = 0; s < 2; ++s) {
+                            float v[32], lo[32];
+                            read(s, v, lo);
+                            if (mine) {
+#pragma unroll
+                                for (int c = 0; c < 32; ++c) m = fmaxf(m, fabsf(fmaf(lo[c], 1.0f / 2048, v[c])));
+                            }
+                        }
+                        m = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(m)));
+                        if (lane == 0) sm->warp_max[u & 1][warp & 3] = m;
+                        mbar_arrive(&sm->max_full);
+                        ok = wait_warp(&sm->max_full, u & 1, sm, p.status);
+                        if (!ok) break;
+                        const float* wm = sm->warp_max[u & 1];
+                        float undo;
+                        scale = scale_to(fmaxf(fmaxf(wm[0], wm[1]), fmaxf(wm[2], wm[3])), &undo);
+                        if (row == 0) sm->tile_scale[u & 3] = undo;
+                    }
+                    if (u >= SB) ok = wait_warp(&sm->s_empty[u % SB], (u / SB - 1) & 1, sm, p.status);
+                    if (!ok) break;
+                }
+                const bool odd = rows != kChunk || (i == 0 && late0);
+                const Pow f = odd ? decay_pow(ld, rows - (i == 0 ? late0 : 0)) : whole;
+                unsigned char* copy = smem + kS + (u % SB) * kSub;
+#pragma unroll 1
+                for (int s = 0; s < 2; ++s) {
+                    float v[32], lo[F16 ? 32 : 1];
+                    read(s, v, lo);
+                    if (!STATE) {
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) {
+                            uint32_t o[4];
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) {
+                                const int c = 8 * j + 2 * e;
+                                if (F16) o[e] = pack2<Th>(fmaf(lo[c % (F16 ? 32 : 1)], 1.0f / 2048, v[c]) * scale, fmaf(lo[(c + 1) % (F16 ? 32 : 1)], 1.0f / 2048, v[c + 1]) * scale);
+                                else o[e] = pack2<Th>(v[c], v[c + 1]);
+                            }
+                            *reinterpret_cast<uint4*>(copy + sw_chunk(row, 4 * s + j)) = make_uint4(o[0], o[1], o[2], o[3]);
+                        }
+                    }
+                    if (adds) {
+#pragma unroll
+                        for (int c = 0; c < 32; c += 2) {
+                            float2 x = make_float2(v[c], v[c + 1]);
+                            x = fma2(x, splat2(f.hi), mul2(x, splat2(f.lo)));
+                            v[c] = x.x;
+                            v[c + 1] = x.y;
+                        }
+                        tmem_st32(lanes + cS + 32 * s, v);
+                        if constexpr (F16) {
+#pragma unroll
+                            for (int c = 0; c < 32; ++c) lo[c] *= f.hi;
+                            tmem_st32(lanes + cSlo + 32 * s, lo);
+                        }
+                    }
+                }
+                if (!STATE) fence_proxy_async();
+                fence_before();
+                mbar_arrive(&sm->s_full[STATE ? 0 : u % SB]);
+                ++u;
+            }
+        }
+        if (ok && leaves && n > 0) {
+            ok = wait_warp(&sm->d_full, (n - 1) & 1, sm, p.status);
+            if (ok) {
+                fence_after();
+                float* out = (STATE ? slots + (w.seg + 1) * slot : r.s_out + w.pair * slot) + static_cast<long long>(row) * W + c0;
+                const Pow f = !STATE && r.last_decay ? decay_pow(ld, 1) : Pow{1.0f, 0.0f};
+#pragma unroll 1
+                for (int s = 0; s < 2; ++s) {
+                    float v[32], lo[32];
+                    read(s, v, lo);
+                    if (mine) {
+#pragma unroll
+                        for (int c = 0; c < 32; ++c)
+                            if (32 * s + c < nc) out[32 * s + c] = times(f, F16 ? fmaf(lo[c], 1.0f / 2048, v[c]) : v[c]);
+                    }
+                }
+            }
+        }
+    } else if (role == 3 && !STATE) {
+        // ---- out ----
+        const float x_whole = decay_at(l2, back ? kChunk - row : row + 1) * r.alpha_x;
+        const int nc = min(kTile, W - c0);
+        const bool tiles = tp.out_map[w.role];
+        for (int i = 0, sz = 0; i < n; ++i) {
+            if (!wait_warp(&sm->x_full[i & 1], (i >> 1) & 1, sm, p.status)) break;
+            if (!wait_warp(&sm->y_full[i & 1], (i >> 1) & 1, sm, p.status)) break;
+            fence_after();
+            const int t0 = start(i), rows = min(kChunk, p.T - t0);
+            const bool reads = i > 0 || enters;
+            const int late = i == 0 ? late0 : 0;
+            float f = x_whole, f1 = 1.0f;
+            if (late || (back && rows != kChunk)) f = decay_at(l2, back ? rows - row - late : row + 1 - late) * r.alpha_x;
+            if (F16) {
+                f1 = sm->row_scale[i & 1][row];
+                if (reads) f *= sm->tile_scale[(enters ? i : i - 1) & 3];
+            }
+            const uint32_t y1 = lanes + cG + (i & 1) * 128 + cY1, y2 = lanes + cY2 + (i & 1) * 64;
+            // 32 columns of out
+            auto read = [&](int s, float* y) {
+                float x[32];
+                if (reads) {
+                    tmem_ld32x2(y1 + 32 * s, y, y2 + 32 * s, x);
+#pragma unroll
+                    for (int c = 0; c < 32; c += 2) {
+                        float2 o = make_float2(y[c], y[c + 1]);
+                        if (F16) o = mul2(o, splat2(f1));
+                        o = fma2(make_float2(x[c], x[c + 1]), splat2(f), o);
+                        y[c] = o.x;
+                        y[c + 1] = o.y;
+                    }
+                } else {
+                    tmem_ld32(y1 + 32 * s, y);
+                    if (F16) {
+#pragma unroll
+                        for (int c = 0; c < 32; ++c) y[c] *= f1;
+                    }
+                }
+            };
+            if (tiles) {
+                // Rows go to Z's place, which the products have read, and leave from there in whole lines (a thread's own row in pieces of 32
+                // bytes took 2100 cycles a chunk).
+                unsigned char* at = smem + kZ + sz * kSub;
+#pragma unroll
+                for (int s = 0; s < 2; ++s) {
+                    float y[32];
+                    read(s, y);
+                    if (s == 1) {
+                        fence_before();
+                        mbar_arrive(&sm->y_empty[i & 1]);
+                    }
+#pragma unroll
+                    for (int j = 0; j < 4; ++j)
+                        *reinterpret_cast<uint4*>(at + sw_chunk(row, 4 * s + j)) =
+                            make_uint4(pack2<Th>(y[8 * j], y[8 * j + 1]), pack2<Th>(y[8 * j + 2], y[8 * j + 3]),
+                                       pack2<Th>(y[8 * j + 4], y[8 * j + 5]), pack2<Th>(y[8 * j + 6], y[8 * j + 7]));
+                }
+                fence_proxy_async();
+                __syncwarp();
+                if (lane == 0) {
+                    if (t0 + (row & ~31) < p.T) tma_store_4d(&tp.out[w.role], at + (row & ~31) * 128, c0, h, t0 + (row & ~31), b);
+                    tma_commit();
+                    tma_wait_read0();
+                }
+            } else {
+                const long long at = b * r.ob + static_cast<long long>(t0 + row) * r.ot + h * r.oh + c0;
+                const int left = row < rows ? nc : 0;
+#pragma unroll 1
+                for (int s = 0; s < 2; ++s) {
+                    float y[32];
+                    read(s, y);
+#pragma unroll
+                    for (int c = 0; c < 32; ++c)
+                        if (32 * s + c < left) {
+                            if (r.out_f32) static_cast<float*>(r.out)[at + 32 * s + c] = y[c];
+                            else static_cast<Th*>(r.out)[at + 32 * s + c] = from_f<Th>(y[c]);
+                        }
+                }
+                fence_before();
+                mbar_arrive(&sm->y_empty[i & 1]);
+            }
+            if (lane == 0) mbar_arrive(&sm->z_empty[sz]);
+            if (++sz == zs) sz = 0;
+        }
+    } else if (role == 4) {
+        // ---- w o Z ----
+        const float w_whole = decay_at(l2, back ? row : kChunk - 1 - row) * r.alpha_s;
+        for (int i = 0, st = 0, turn = 0; i < n - (leaves ? 0 : 1); ++i) {
+            const int rows = min(kChunk, p.T - start(i));
+            if (!wait_warp(&sm->z_full[st], turn & 1, sm, p.status)) break;
+            if (i > 0 && !wait_warp(&sm->d_full, (i - 1) & 1, sm, p.status)) break;
+            const float f = rows == kChunk ? w_whole : row < rows ? decay_at(l2, back ? row : rows - 1 - row) * r.alpha_s : 0.0f;
+            const unsigned char* z = smem + kZ + st * kSub;
+#pragma unroll 2
+            for (int j = 0; j < 8; ++j) {
+                const uint4 v = *reinterpret_cast<const uint4*>(z + sw_chunk(row, j));
+                const uint32_t in[4] = {v.x, v.y, v.z, v.w};
+                uint32_t o[TERMS][4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    float2 x = mul2(unpack2<Th>(in[e]), splat2(f));
+                    o[0][e] = pack2<Th>(x.x, x.y);
+#pragma unroll
+                    for (int t = 1; t < TERMS; ++t) {
+                        const float2 hi = unpack2<Th>(o[t - 1][e]);
+                        x = make_float2(x.x - hi.x, x.y - hi.y);
+                        if (F16) x = make_float2(x.x * 2048.0f, x.y * 2048.0f);
+                        o[t][e] = pack2<Th>(x.x, x.y);
+                    }
+                }
+#pragma unroll
+                for (int t = 0; t < TERMS; ++t)
+                    *reinterpret_cast<uint4*>(smem + kW + t * kSub + sw_chunk(row, j)) = make_uint4(o[t][0], o[t][1], o[t][2], o[t][3]);
+            }
+            fence_proxy_async();
+            mbar_arrive(&sm->w_full);
+            if (++st == zs) {
+                st = 0;
+                ++turn;
+            }
+        }
+    }
+    fence_before();
+    __syncthreads();
+    fence_after();
+    __syncwarp();
+    if (warp == 1) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kCols) : "memory");
+}
+
+typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*,
+                                  const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+// [rows x 64 columns] of one head, 128-byte swizzled; rows behind the last step and columns behind the last one are zeros.
+static bool make_map(Ctx* c, CUtensorMap* map, int dtype, const Operand& o, int H, int T, int B, int rows) {
+    const int heads = H / o.group;
+    if (!c->encode_tiled || reinterpret_cast<uintptr_t>(o.p) % 16) return false;
+    const long long st = T > 1 ? o.st : (o.cols + 7) & ~7, sh = heads > 1 ? o.sh : 8, sb = B > 1 ? o.sb : 8;
+    for (long long s : {st, sh, sb})
+        if (s <= 0 || s % 8 || s >= (1ll << 38)) return false;
+    cuuint64_t dims[4] = {static_cast<cuuint64_t>(o.cols), static_cast<cuuint64_t>(heads), static_cast<cuuint64_t>(T), static_cast<cuuint64_t>(B)};
+    cuuint64_t strides[3] = {static_cast<cuuint64_t>(sh) * 2, static_cast<cuuint64_t>(st) * 2, static_cast<cuuint64_t>(sb) * 2};
+    cuuint32_t box[4] = {64, 1, static_cast<cuuint32_t>(rows), 1}, each[4] = {1, 1, 1, 1};
+    return reinterpret_cast<EncodeTiledFn>(c->encode_tiled)(
+               map, dtype == MAMBA_B200_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, const_cast<void*>(o.p), dims,
+               strides, box, each, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B,
+               CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+template <typename Th, int TERMS>
+int launch(Ctx* c, TcParams& tp, long long pairs, cudaStream_t st) {
+    long long blocks = 0;
+    tp.na = 1;
+    for (int i = 0; i < tp.p.roles; ++i) {
+        tp.p.role[i].block0 = blocks;
+        blocks += pairs * tp.p.role[i].tiles;
+        if (tp.p.role[i].A > 64) tp.na = 2;
+    }
+    tp.stages = tp.na == 2 ? 2 : 3;
+    tp.z_stages = tp.na == 2 ? kMostZ<TERMS> : 4;
+    const uint32_t smem = smem_bytes<TERMS>(tp.na, tp.stages, tp.z_stages);
+    if (tp.p.segments > 1) {
+        walk_kernel<Th, TERMS, true><<<static_cast<unsigned>(blocks * (tp.p.segments - 1)), kThreads, smem, st>>>(tp);
+        MB200_CUDA_CHECK(c, cudaGetLastError());
+    }
+    walk_kernel<Th, TERMS, false><<<static_cast<unsigned>(blocks * tp.p.segments), kThreads, smem, st>>>(tp);
+    MB200_CUDA_CHECK(c, cudaGetLastError());
+    return MAMBA_B200_OK;
+}
+
+}  // namespace tcl
+
+int pick_segments(int sm_count, long long blocks, int T, long long pairs);
+
+// Takes the call where the tensor cores' kernel can: 16-bit types, both widths up to 128, tensors that TMA can describe, and more
+// steps than the general kernel's 32 (a tile has 128 rows whatever T is).
+int tc_launch(Ctx* c, int dtype, Params& p, bool may_cut, long long pairs, cudaStream_t st, bool* taken) {
+    using namespace tcl;
+    *taken = false;
+    if (dtype == MAMBA_B200_F32 || p.T <= 32) return MAMBA_B200_OK;
+    // (in f16 a weight above 1 could take Z out of the type)
+    if (dtype == MAMBA_B200_F16)
+        for (int i = 0; i < p.roles; ++i)
+            if (!(fabsf(p.role[i].alpha_s) <= 1.0f)) return MAMBA_B200_OK;
+    for (int i = 0; i < p.roles; ++i)
+        if (p.role[i].A > 128 || p.role[i].W > 128) return MAMBA_B200_OK;
+    TcParams tp[2];  // roles that leave no state, and roles that do
+    memset(tp, 0, sizeof(tp));
+    long long blocks = 0;
+    int roles[2] = {0, 0};
+    for (int i = 0; i < p.roles; ++i) {
+        Role& r = p.role[i];
+        TcParams& to = tp[r.s_out != nullptr];
+        int& k = roles[r.s_out != nullptr];
+        if (!make_map(c, &to.x[k], dtype, r.x, p.H, p.T, p.B, kChunk) || !make_map(c, &to.y[k], dtype, r.y, p.H, p.T, p.B, kChunk) ||
+            !make_map(c, &to.z[k], dtype, r.z, p.H, p.T, p.B, kChunk))
+            return MAMBA_B200_OK;
+        const Operand out = {r.out, r.ob, r.ot, r.oh, 1, r.W};
+        to.out_map[k] = !r.out_f32 && make_map(c, &to.out[k], dtype, out, p.H, p.T, p.B, 32);
+        r.tiles = (r.W + kTile - 1) / kTile;
+        blocks += pairs * r.tiles;
+        ++k;
+    }
+    if (blocks > 1000000000ll / kMaxSegments) return MAMBA_B200_OK;
+    p.segments = may_cut ? pick_segments(c->sm_count, blocks, p.T, pairs) : 1;
+    const int chunks = (p.T + kChunk - 1) / kChunk, per = (chunks + p.segments - 1) / p.segments;
+    p.segments = (chunks + per - 1) / per;
+    p.seg_len = per * kChunk;
+    *taken = true;
+    for (int state = 0; state < 2; ++state) {
+        if (!roles[state]) continue;
+        tp[state].p = p;
+        tp[state].p.roles = 0;
+        for (int i = 0; i < p.roles; ++i)
+            if ((p.role[i].s_out != nullptr) == (state == 1)) tp[state].p.role[tp[state].p.roles++] = p.role[i];
+        const int rc = dtype == MAMBA_B200_F16 ? launch<__half, 2>(c, tp[state], pairs, st)
+                       : state                 ? launch<__nv_bfloat16, 3>(c, tp[state], pairs, st)
+                                               : launch<__nv_bfloat16, 1>(c, tp[state], pairs, st);
+        if (rc) return rc;
+    }
+    return MAMBA_B200_OK;
+}
+
+}  // namespace la
+
+int linear_attention_tc_configure(Ctx* c) {
+    using namespace la::tcl;
+#define MB200_LA(Th, TERMS)                                                                                                              \
+    MB200_CUDA_CHECK(c, cudaFuncSetAttribute((const void*)walk_kernel<Th, TERMS, false>, cudaFuncAttributeMaxDynamicSharedMemorySize,     \
+                                             static_cast<int>(smem_bytes<TERMS>(2, 2, kMostZ<TERMS>))));                                                \
+    MB200_CUDA_CHECK(c, cudaFuncSetAttribute((const void*)walk_kernel<Th, TERMS, true>, cudaFuncAttributeMaxDynamicSharedMemorySize,      \
+                                             static_cast<int>(smem_bytes<TERMS>(2, 2, kMostZ<TERMS>))));
+    MB200_LA(__half, 2)
+    MB200_LA(__nv_bfloat16, 1)
+    MB200_LA(__nv_bfloat16, 3)
+#undef MB200_LA
+    return MAMBA_B200_OK;
+}
+
+}  // namespace mb200
