@@ -93,6 +93,7 @@ int logprobs_configure(Ctx* c);    // logprobs.cu
 int embedding_configure(Ctx* c);   // embedding.cu
 int linear_attention_configure(Ctx* c);  // linear_attention.cu
 int linear_attention_tc_configure(Ctx* c);  // linear_attention_tc.cu
+int group_norm_configure(Ctx* c);  // group_norm.cu
 
 }  // namespace mb200
 
@@ -145,6 +146,8 @@ extern "C" MAMBA_B200_API int mamba_b200_init(int device, void** handle) {
     rc = linear_attention_configure(c);
     if (rc) return rc;
     rc = linear_attention_tc_configure(c);
+    if (rc) return rc;
+    rc = group_norm_configure(c);
     if (rc) return rc;
     return MAMBA_B200_OK;
 }

@@ -34,6 +34,11 @@ __device__ __forceinline__ void load(const T* p, float* f) {
     for (int i = 0; i < VEC; ++i) f[i] = to_f(v.v[i]);
 }
 template <typename T, int VEC>
+__device__ __forceinline__ void widen(const Vec<T, VEC>& v, float* f) {
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) f[i] = to_f(v.v[i]);
+}
+template <typename T, int VEC>
 __device__ __forceinline__ void store(T* p, const float* f) {
     Vec<T, VEC> v;
 #pragma unroll
@@ -92,6 +97,10 @@ __device__ __forceinline__ float sum_lanes(float v, int lanes) {
     for (int m = lanes >> 1; m; m >>= 1) v += __shfl_xor_sync(0xffffffffu, v, m);
     return v;
 }
+// 16 bytes into this thread's own place in shared memory
+__device__ __forceinline__ void fetch16(void* dst, const void* src) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(dst)), "l"(src) : "memory");
+}
 // The same where a group may take several whole warps (every thread of the block calls it): `turn` alternates between two sets
 // of sums, so that one barrier a sum is enough.
 __device__ __forceinline__ float sum_group(float v, int lanes, float (*sums)[8], int& turn) {
@@ -121,138 +130,336 @@ __device__ __forceinline__ float through(int kind, float v, float dy, bool gate,
     return d * slope;
 }
 
+// The same for two values at a time, activation and gate known to the compiler (looked up for every value, they made up half of the
+// instructions of a kernel that is bound by them).
+template <typename T>
+__device__ __forceinline__ float2 sigmoid2(float2 v) {
+    if constexpr (sizeof(T) == 4) {
+        return make_float2(sigmoid<T>(v.x), sigmoid<T>(v.y));
+    } else {
+        const float2 e = mul2(v, splat2(-kLog2e)), d = add2(make_float2(ex2(e.x), ex2(e.y)), splat2(1.0f));
+        return make_float2(rcp(d.x), rcp(d.y));
+    }
+}
+template <typename T, int ACT>
+__device__ __forceinline__ float2 act2(float2 v) {
+    if constexpr (ACT == MAMBA_B200_ACT_NONE) return v;
+    if constexpr (ACT == MAMBA_B200_ACT_SILU) return mul2(v, sigmoid2<T>(v));
+    return make_float2(act<T>(ACT, v.x), act<T>(ACT, v.y));
+}
+// z^ = slope of z SiLU: q (1 + z (1 - q))
+__device__ __forceinline__ float2 silu_slope2(float2 z, float2 q) {
+    return mul2(q, fma2(z, fma2(q, splat2(-1.0f), splat2(1.0f)), splat2(1.0f)));
+}
+// dv of dy (and d_z, in z's place)
+template <typename T, int ACT, bool GATE>
+__device__ __forceinline__ float2 through2(float2 v, float2 dy, float2& z) {
+    float2 value = v, slope;
+    if constexpr (ACT == MAMBA_B200_ACT_SILU) {
+        const float2 q = sigmoid2<T>(v);
+        value = mul2(v, q);
+        slope = silu_slope2(v, q);
+    } else if constexpr (ACT == MAMBA_B200_ACT_GELU) {
+        slope = make_float2(act_slope<T>(ACT, v.x, &value.x), act_slope<T>(ACT, v.y, &value.y));
+    }
+    float2 d = dy;
+    if constexpr (GATE) {
+        const float2 q = sigmoid2<T>(z);
+        d = mul2(dy, mul2(z, q));
+        z = mul2(mul2(dy, value), silu_slope2(z, q));
+    }
+    if constexpr (ACT != MAMBA_B200_ACT_NONE) d = mul2(d, slope);
+    return d;
+}
+template <typename T, int VEC>
+__device__ __forceinline__ void widen2(const Vec<T, VEC>& v, float2* f) {
+#pragma unroll
+    for (int i = 0; i < VEC / 2; ++i) f[i] = ld_pair(v.v + 2 * i);
+}
+template <typename T, int VEC>
+__device__ __forceinline__ void store2(T* p, const float2* f) {
+    Vec<T, VEC> v;
+#pragma unroll
+    for (int i = 0; i < VEC / 2; ++i) st_pair(v.v + 2 * i, f[i]);
+    *reinterpret_cast<Vec<T, VEC>*>(p) = v;
+}
+
 // ---------------------------------------------------------------------------------------------------
 // rows
 // ---------------------------------------------------------------------------------------------------
-template <typename T, int VEC, int VPT, bool BWD>
-__global__ void __launch_bounds__(kThreads) rows_kernel(const Params p) {
-    constexpr int E = VEC * VPT;
+
+// Where a thread stands: its group, and the vectors of it that it has.
+template <int VEC, int VPT>
+struct Seat {
+    int wide, r, at, g, lane, col[VPT];
+    bool mine, have[VPT];
+    __device__ __forceinline__ Seat(const Params& p) {
+        wide = p.groups * p.lanes;  // threads of a row
+        r = threadIdx.x / wide;
+        at = threadIdx.x - r * wide;
+        const int g_in = at / p.lanes;
+        lane = at - g_in * p.lanes;
+        g = blockIdx.y * p.groups + g_in;
+        mine = r < p.rows && g < p.a.G;
+#pragma unroll
+        for (int i = 0; i < VPT; ++i) {
+            const int k = lane + i * p.lanes;
+            have[i] = mine && k < p.vecs;
+            col[i] = g * p.per + k * VEC;
+        }
+    }
+};
+
+// A block's d_w and d_b: its rows are joined in their order, a vector of each thread at a time.
+template <int VEC, int VPT>
+__device__ __forceinline__ void leave_sums(const Params& p, const Seat<VEC, VPT>& t, const float* dw, const float* db, float* sm) {
+    float* sw = sm;
+    float* sb = sm + VEC * kThreads;
+    float* out_w = p.sums + static_cast<long long>(blockIdx.x) * p.a.C;
+    float* out_b = out_w + static_cast<long long>(p.parts) * p.a.C;
+#pragma unroll
+    for (int i = 0; i < VPT; ++i) {
+        __syncthreads();
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) {
+            sw[e * kThreads + threadIdx.x] = dw[i * VEC + e];
+            sb[e * kThreads + threadIdx.x] = db[i * VEC + e];
+        }
+        __syncthreads();
+        if (t.r == 0 && t.have[i]) {
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) {
+                float tw = 0.0f, tb = 0.0f;
+                for (int k = 0; k < p.rows; ++k) {
+                    tw += sw[e * kThreads + k * t.wide + t.at];
+                    tb += sb[e * kThreads + k * t.wide + t.at];
+                }
+                out_w[t.col[i] + e] = tw;
+                out_b[t.col[i] + e] = tb;
+            }
+        }
+    }
+}
+
+// Vectors of 16 bytes.  A thread's vectors of the next rows are on their way to places of its own in shared memory (no barriers, no
+// registers): HBM's latency at its rate is 35 KB an SM.
+template <int VPT>
+constexpr int kRowsAhead = VPT == 1 ? 4 : 2;
+
+template <typename T, int VEC, int VPT, bool BWD, int ACT, bool GATE>
+__global__ void __launch_bounds__(kThreads, VPT > 1 ? 1 : BWD ? 2 : 4) rows_kernel(const Params p) {
+    constexpr int E = VEC * VPT, H = E / 2, D = kRowsAhead<VPT>, TENSORS = (BWD ? 2 : 1) + (GATE ? 1 : 0);
+    extern __shared__ __align__(16) unsigned char ring[];
     __shared__ float sums_sm[BWD ? 2 * VEC * kThreads : 1];
     __shared__ float warp_sums[2][8];
     int turn = 0;
     const mamba_b200_group_norm_args& a = p.a;
-    const int wide = p.groups * p.lanes;  // threads of a row
-    const int r = threadIdx.x / wide, at = threadIdx.x - r * wide, g_in = at / p.lanes, lane = at - g_in * p.lanes;
-    const int g = blockIdx.y * p.groups + g_in;
-    const bool mine = r < p.rows && g < a.G;
-    bool have[VPT];
-    int col[VPT];
-    float w[E], bias[E], dw[BWD ? E : 1], db[BWD ? E : 1];
+    const Seat<VEC, VPT> t(p);
+    float2 w[H], bias[H], dw[BWD ? H : 1], db[BWD ? H : 1];
 #pragma unroll
-    for (int i = 0; i < VPT; ++i) {
-        const int k = lane + i * p.lanes;
-        have[i] = mine && k < p.vecs;
-        col[i] = g * p.per + k * VEC;
+    for (int i = 0; i < VPT; ++i)
 #pragma unroll
-        for (int e = 0; e < VEC; ++e) {
-            w[i * VEC + e] = have[i] && a.weight ? a.weight[col[i] + e] : 1.0f;
-            bias[i * VEC + e] = have[i] && a.bias ? a.bias[col[i] + e] : 0.0f;
-            if (BWD) dw[i * VEC + e] = db[i * VEC + e] = 0.0f;
+        for (int e = 0; e < VEC / 2; ++e) {
+            const int c = t.col[i] + 2 * e, k = i * VEC / 2 + e;
+            w[k] = t.have[i] && a.weight ? make_float2(a.weight[c], a.weight[c + 1]) : splat2(1.0f);
+            bias[k] = t.have[i] && a.bias ? make_float2(a.bias[c], a.bias[c + 1]) : splat2(0.0f);
+            if (BWD) dw[k] = db[k] = splat2(0.0f);
         }
-    }
     const float inv = 1.0f / p.per;
-    const bool gate = a.z != nullptr;
     const long long NG = static_cast<long long>(a.N) * a.G;
+    Vec<T, VEC>* own = reinterpret_cast<Vec<T, VEC>*>(ring) + threadIdx.x;
+    auto in_ring = [&](int d, int tensor, int i) { return own + ((d * TENSORS + tensor) * VPT + i) * kThreads; };
+    auto ask = [&](long long n, int d) {
+#pragma unroll
+        for (int i = 0; i < VPT; ++i)
+            if (t.have[i] && n < a.N) {
+                fetch16(in_ring(d, 0, i), static_cast<const T*>(a.x) + n * a.ld_x + t.col[i]);
+                if (BWD) fetch16(in_ring(d, 1, i), static_cast<const T*>(a.dy) + n * a.ld_dy + t.col[i]);
+                if (GATE) fetch16(in_ring(d, TENSORS - 1, i), static_cast<const T*>(a.z) + n * a.ld_z + t.col[i]);
+            }
+        asm volatile("cp.async.commit_group;" ::: "memory");
+    };
+    const long long turn_rows = gridDim.x * static_cast<long long>(p.rows), first = blockIdx.x * static_cast<long long>(p.rows);
+    float mean_next = 0.0f, rstd_next = 0.0f;
+    auto ask_stats = [&](long long n) {
+        if (BWD && t.mine && n < a.N) {
+            mean_next = a.stats[n * a.G + t.g];
+            rstd_next = a.stats[NG + n * a.G + t.g];
+        }
+    };
+    ask_stats(first + t.r);
+#pragma unroll
+    for (int d = 0; d < D; ++d) ask(first + t.r + d * turn_rows, d);
+    int d = 0;
     // (every thread of a warp takes every turn: the sums are shuffles)
-    for (long long n0 = blockIdx.x * static_cast<long long>(p.rows); n0 < a.N; n0 += gridDim.x * static_cast<long long>(p.rows)) {
-        const long long n = n0 + r;
-        const bool on = mine && n < a.N;
-        float x[E], z[E], dy[E];
+    for (long long n0 = first; n0 < a.N; n0 += turn_rows) {
+        const long long n = n0 + t.r;
+        const bool on = t.mine && n < a.N;
+        asm volatile("cp.async.wait_group %0;" ::"n"(D - 1) : "memory");
+        float2 x[H], z[H], dy[H];
 #pragma unroll
         for (int i = 0; i < VPT; ++i) {
-            const bool ok = on && have[i];
+            // (what a thread has no row for is never looked at, but for the sums)
+            widen2(*in_ring(d, 0, i), x + i * VEC / 2);
+            if (BWD) widen2(*in_ring(d, 1, i), dy + i * VEC / 2);
+            if (GATE) widen2(*in_ring(d, TENSORS - 1, i), z + i * VEC / 2);
+            if (!(on && t.have[i])) {
 #pragma unroll
-            for (int e = 0; e < VEC; ++e) x[i * VEC + e] = z[i * VEC + e] = dy[i * VEC + e] = 0.0f;
-            if (ok) load<T, VEC>(static_cast<const T*>(a.x) + n * a.ld_x + col[i], x + i * VEC);
-            if (ok && gate) load<T, VEC>(static_cast<const T*>(a.z) + n * a.ld_z + col[i], z + i * VEC);
-            if (BWD && ok) load<T, VEC>(static_cast<const T*>(a.dy) + n * a.ld_dy + col[i], dy + i * VEC);
+                for (int e = 0; e < VEC / 2; ++e) {
+                    const int k = i * VEC / 2 + e;
+                    x[k] = splat2(0.0f);
+                    if (BWD) dy[k] = splat2(0.0f);
+                    if (GATE) z[k] = splat2(0.0f);
+                }
+            }
         }
+        const float mean_in = mean_next, rstd_in = rstd_next;
+        ask_stats(n + turn_rows);
+        ask(n + D * turn_rows, d);
+        d = d + 1 == D ? 0 : d + 1;
         if constexpr (!BWD) {
-            float s = 0.0f;
+            float2 s = x[0];
 #pragma unroll
-            for (int e = 0; e < E; ++e) s += x[e];
-            const float mean = sum_group(s, p.lanes, warp_sums, turn) * inv;
-            float q = 0.0f;
+            for (int k = 1; k < H; ++k) s = add2(s, x[k]);
+            const float mean = sum_group(s.x + s.y, p.lanes, warp_sums, turn) * inv;
+            float2 q = splat2(0.0f);
 #pragma unroll
             for (int i = 0; i < VPT; ++i)
 #pragma unroll
-                for (int e = 0; e < VEC; ++e) {
-                    float& d = x[i * VEC + e];
-                    d = have[i] ? d - mean : 0.0f;
-                    q = fmaf(d, d, q);
+                for (int e = 0; e < VEC / 2; ++e) {
+                    float2& v = x[i * VEC / 2 + e];
+                    v = add2(v, splat2(t.have[i] ? -mean : 0.0f));
+                    q = fma2(v, v, q);
                 }
-            const float rstd = 1.0f / sqrtf(sum_group(q, p.lanes, warp_sums, turn) * inv + a.eps);
-            if (on && lane == 0 && a.stats) {
-                a.stats[n * a.G + g] = mean;
-                a.stats[NG + n * a.G + g] = rstd;
+            const float rstd = 1.0f / sqrtf(sum_group(q.x + q.y, p.lanes, warp_sums, turn) * inv + a.eps);
+            if (on && t.lane == 0 && a.stats) {
+                a.stats[n * a.G + t.g] = mean;
+                a.stats[NG + n * a.G + t.g] = rstd;
             }
 #pragma unroll
-            for (int e = 0; e < E; ++e) {
-                x[e] = act<T>(a.activation, fmaf(x[e] * rstd, w[e], bias[e]));
-                if (gate) x[e] *= z[e] * sigmoid<T>(z[e]);
+            for (int k = 0; k < H; ++k) {
+                x[k] = act2<T, ACT>(fma2(mul2(x[k], splat2(rstd)), w[k], bias[k]));
+                if (GATE) x[k] = mul2(x[k], mul2(z[k], sigmoid2<T>(z[k])));
             }
 #pragma unroll
             for (int i = 0; i < VPT; ++i)
-                if (on && have[i]) store<T, VEC>(static_cast<T*>(a.y) + n * a.ld_y + col[i], x + i * VEC);
+                if (on && t.have[i]) store2<T, VEC>(static_cast<T*>(a.y) + n * a.ld_y + t.col[i], x + i * VEC / 2);
         } else {
-            const float mean = on ? a.stats[n * a.G + g] : 0.0f, rstd = on ? a.stats[NG + n * a.G + g] : 0.0f;
-            float s1 = 0.0f, s2 = 0.0f;
+            // (threads without a row: x and dy are 0, and so is all they add)
+            const float mean = on ? mean_in : 0.0f, rstd = on ? rstd_in : 0.0f;
+            float2 s1 = splat2(0.0f), s2 = splat2(0.0f);
+#pragma unroll
+            for (int k = 0; k < H; ++k) {
+                const float2 xh = mul2(add2(x[k], splat2(-mean)), splat2(rstd));
+                const float2 dv = through2<T, ACT, GATE>(fma2(xh, w[k], bias[k]), dy[k], z[k]);
+                dw[k] = fma2(dv, xh, dw[k]);
+                db[k] = add2(db[k], dv);
+                x[k] = xh;
+                dy[k] = mul2(dv, w[k]);
+                s1 = add2(s1, dy[k]);
+                s2 = fma2(dy[k], xh, s2);
+            }
+            const float m1 = sum_group(s1.x + s1.y, p.lanes, warp_sums, turn) * inv * rstd;
+            const float m2 = sum_group(s2.x + s2.y, p.lanes, warp_sums, turn) * inv * rstd;
+#pragma unroll
+            for (int k = 0; k < H; ++k) x[k] = fma2(x[k], splat2(-m2), fma2(dy[k], splat2(rstd), splat2(-m1)));
 #pragma unroll
             for (int i = 0; i < VPT; ++i)
-#pragma unroll
-                for (int e0 = 0; e0 < VEC; ++e0) {
-                    const int e = i * VEC + e0;
-                    if (!(on && have[i])) continue;
-                    const float xh = (x[e] - mean) * rstd;
-                    const float dv = through<T>(a.activation, fmaf(xh, w[e], bias[e]), dy[e], gate, z[e], &z[e]);
-                    dw[e] = fmaf(dv, xh, dw[e]);
-                    db[e] += dv;
-                    x[e] = xh;
-                    dy[e] = dv * w[e];
-                    s1 += dy[e];
-                    s2 = fmaf(dy[e], xh, s2);
-                }
-            s1 = sum_group(s1, p.lanes, warp_sums, turn) * inv;
-            s2 = sum_group(s2, p.lanes, warp_sums, turn) * inv;
-#pragma unroll
-            for (int e = 0; e < E; ++e) x[e] = rstd * (dy[e] - s1 - x[e] * s2);
-#pragma unroll
-            for (int i = 0; i < VPT; ++i)
-                if (on && have[i]) {
-                    store<T, VEC>(static_cast<T*>(a.d_x) + n * a.ld_dx + col[i], x + i * VEC);
-                    if (gate) store<T, VEC>(static_cast<T*>(a.d_z) + n * a.ld_dz + col[i], z + i * VEC);
+                if (on && t.have[i]) {
+                    store2<T, VEC>(static_cast<T*>(a.d_x) + n * a.ld_dx + t.col[i], x + i * VEC / 2);
+                    if (GATE) store2<T, VEC>(static_cast<T*>(a.d_z) + n * a.ld_dz + t.col[i], z + i * VEC / 2);
                 }
         }
     }
     if constexpr (BWD) {
-        // the block's rows are joined in their order, a vector of each thread at a time
-        float* sw = sums_sm;
-        float* sb = sums_sm + VEC * kThreads;
-        float* out_w = p.sums + static_cast<long long>(blockIdx.x) * a.C;
-        float* out_b = out_w + static_cast<long long>(p.parts) * a.C;
+        float fw[E], fb[E];
+#pragma unroll
+        for (int k = 0; k < H; ++k) {
+            fw[2 * k] = dw[k].x; fw[2 * k + 1] = dw[k].y;
+            fb[2 * k] = db[k].x; fb[2 * k + 1] = db[k].y;
+        }
+        leave_sums<VEC, VPT>(p, t, fw, fb, sums_sm);
+    }
+}
+
+// Rows that start or end between vectors: element by element.
+template <typename T, int VPT, bool BWD>
+__global__ void __launch_bounds__(kThreads) odd_rows_kernel(const Params p) {
+    constexpr int E = VPT;
+    __shared__ float sums_sm[BWD ? 2 * kThreads : 1];
+    __shared__ float warp_sums[2][8];
+    int turn = 0;
+    const mamba_b200_group_norm_args& a = p.a;
+    const Seat<1, VPT> t(p);
+    float w[E], bias[E], dw[E], db[E];
+#pragma unroll
+    for (int i = 0; i < VPT; ++i) {
+        w[i] = t.have[i] && a.weight ? a.weight[t.col[i]] : 1.0f;
+        bias[i] = t.have[i] && a.bias ? a.bias[t.col[i]] : 0.0f;
+        dw[i] = db[i] = 0.0f;
+    }
+    const float inv = 1.0f / p.per;
+    const bool gate = a.z != nullptr;
+    const long long NG = static_cast<long long>(a.N) * a.G;
+    for (long long n0 = blockIdx.x * static_cast<long long>(p.rows); n0 < a.N; n0 += gridDim.x * static_cast<long long>(p.rows)) {
+        const long long n = n0 + t.r;
+        const bool on = t.mine && n < a.N;
+        float x[E], z[E], dy[E];
 #pragma unroll
         for (int i = 0; i < VPT; ++i) {
-            __syncthreads();
+            const bool ok = on && t.have[i];
+            x[i] = ok ? to_f(static_cast<const T*>(a.x)[n * a.ld_x + t.col[i]]) : 0.0f;
+            z[i] = ok && gate ? to_f(static_cast<const T*>(a.z)[n * a.ld_z + t.col[i]]) : 0.0f;
+            dy[i] = ok && BWD ? to_f(static_cast<const T*>(a.dy)[n * a.ld_dy + t.col[i]]) : 0.0f;
+        }
+        if constexpr (!BWD) {
+            float s = 0.0f, q = 0.0f;
 #pragma unroll
-            for (int e = 0; e < VEC; ++e) {
-                sw[e * kThreads + threadIdx.x] = dw[i * VEC + e];
-                sb[e * kThreads + threadIdx.x] = db[i * VEC + e];
+            for (int i = 0; i < VPT; ++i) s += x[i];
+            const float mean = sum_group(s, p.lanes, warp_sums, turn) * inv;
+#pragma unroll
+            for (int i = 0; i < VPT; ++i) {
+                x[i] = t.have[i] ? x[i] - mean : 0.0f;
+                q = fmaf(x[i], x[i], q);
             }
-            __syncthreads();
-            if (r == 0 && have[i]) {
+            const float rstd = 1.0f / sqrtf(sum_group(q, p.lanes, warp_sums, turn) * inv + a.eps);
+            if (on && t.lane == 0 && a.stats) {
+                a.stats[n * a.G + t.g] = mean;
+                a.stats[NG + n * a.G + t.g] = rstd;
+            }
 #pragma unroll
-                for (int e = 0; e < VEC; ++e) {
-                    float tw = 0.0f, tb = 0.0f;
-                    for (int k = 0; k < p.rows; ++k) {
-                        tw += sw[e * kThreads + k * wide + at];
-                        tb += sb[e * kThreads + k * wide + at];
-                    }
-                    out_w[col[i] + e] = tw;
-                    out_b[col[i] + e] = tb;
+            for (int i = 0; i < VPT; ++i)
+                if (on && t.have[i]) {
+                    float y = act<T>(a.activation, fmaf(x[i] * rstd, w[i], bias[i]));
+                    if (gate) y *= z[i] * sigmoid<T>(z[i]);
+                    static_cast<T*>(a.y)[n * a.ld_y + t.col[i]] = from_f<T>(y);
                 }
-            }
+        } else {
+            const float mean = on ? a.stats[n * a.G + t.g] : 0.0f, rstd = on ? a.stats[NG + n * a.G + t.g] : 0.0f;
+            float s1 = 0.0f, s2 = 0.0f;
+#pragma unroll
+            for (int i = 0; i < VPT; ++i)
+                if (on && t.have[i]) {
+                    const float xh = (x[i] - mean) * rstd;
+                    const float dv = through<T>(a.activation, fmaf(xh, w[i], bias[i]), dy[i], gate, z[i], &z[i]);
+                    dw[i] = fmaf(dv, xh, dw[i]);
+                    db[i] += dv;
+                    x[i] = xh;
+                    dy[i] = dv * w[i];
+                    s1 += dy[i];
+                    s2 = fmaf(dy[i], xh, s2);
+                }
+            s1 = sum_group(s1, p.lanes, warp_sums, turn) * inv;
+            s2 = sum_group(s2, p.lanes, warp_sums, turn) * inv;
+#pragma unroll
+            for (int i = 0; i < VPT; ++i)
+                if (on && t.have[i]) {
+                    static_cast<T*>(a.d_x)[n * a.ld_dx + t.col[i]] = from_f<T>(rstd * (dy[i] - s1 - x[i] * s2));
+                    if (gate) static_cast<T*>(a.d_z)[n * a.ld_dz + t.col[i]] = from_f<T>(z[i]);
+                }
         }
     }
+    if constexpr (BWD) leave_sums<1, VPT>(p, t, dw, db, sums_sm);
 }
 
 // d_w and d_b from the blocks' sums: a warp's lanes hold 32 channels, its block's warps every eighth part, joined in order.
@@ -591,6 +798,174 @@ __global__ void __launch_bounds__(kThreads) spread_kernel(const Params p) {
     }
 }
 
+// The same in one kernel, where a sample's rows of a block's channels fit shared memory: every element is read once.  A thread keeps
+// its own vectors there, so that barriers are for sums alone.
+template <typename T, int VEC>
+__device__ __forceinline__ float group_sum(const Params& p, const Cover& c, float v, float* per_thread, float* per_group) {
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, vecs = p.vecs, wide = p.groups * p.vecs;
+    __syncthreads();
+    per_thread[threadIdx.x] = v;
+    __syncthreads();
+    for (int gi = warp; gi < c.groups; gi += kThreads / 32) {
+        float t = 0.0f;
+        for (int i = lane; i < c.rp * vecs; i += 32) t += per_thread[(i / vecs) * wide + gi * vecs + i % vecs];
+        t = sum_lanes(t, 32);
+        if (lane == 0) per_group[gi] = t;
+    }
+    __syncthreads();
+    return c.on ? per_group[c.gi] : 0.0f;
+}
+
+template <typename T, int VEC, bool BWD>
+__global__ void __launch_bounds__(kThreads) slab_kernel(const Params p) {
+    using V = Vec<T, VEC>;
+    extern __shared__ __align__(16) unsigned char slab[];
+    __shared__ float per_thread[kThreads], per_group[kThreads];
+    __shared__ float sw[BWD ? kThreads * VEC : 1], sb[BWD ? kThreads * VEC : 1];
+    const mamba_b200_group_norm_args& a = p.a;
+    const Cover c = cover<VEC>(p);
+    const int turns = (a.S + c.rp - 1) / c.rp;
+    V* sx = reinterpret_cast<V*>(slab) + threadIdx.x;
+    V* sd = sx + (BWD ? static_cast<size_t>(turns) * kThreads : 0);
+    V* sz = sd + static_cast<size_t>(turns) * kThreads;
+    const bool gate = a.z != nullptr;
+    const float inv = 1.0f / (static_cast<float>(p.per) * a.S);
+    const long long NG = static_cast<long long>(a.N) * a.G;
+    float w[VEC], bias[VEC], all_w[BWD ? VEC : 1], all_b[BWD ? VEC : 1];
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) {
+        w[e] = c.on && a.weight ? a.weight[c.col + e] : 1.0f;
+        bias[e] = c.on && a.bias ? a.bias[c.col + e] : 0.0f;
+        if (BWD) all_w[e] = all_b[e] = 0.0f;
+    }
+    for (int ns = blockIdx.x; ns < a.N; ns += p.side) {
+        const long long row0 = static_cast<long long>(ns) * a.S;
+        constexpr int U = 8;
+        float s1 = 0.0f, s2 = 0.0f;
+        float mean = 0.0f, rstd = 0.0f;
+        if (BWD && c.on) {
+            mean = a.stats[static_cast<long long>(ns) * a.G + c.g];
+            rstd = a.stats[NG + static_cast<long long>(ns) * a.G + c.g];
+        }
+        if (c.on) {
+            for (int s = c.r, k = 0; s < a.S; s += U * c.rp, k += U) {
+                V v[U], d[BWD ? U : 1], g[U];
+#pragma unroll
+                for (int u = 0; u < U; ++u)
+                    if (s + u * c.rp < a.S) {
+                        const long long row = row0 + s + u * c.rp;
+                        v[u] = *reinterpret_cast<const V*>(static_cast<const T*>(a.x) + row * a.ld_x + c.col);
+                        if (BWD) d[u % (BWD ? U : 1)] = *reinterpret_cast<const V*>(static_cast<const T*>(a.dy) + row * a.ld_dy + c.col);
+                        if (gate) g[u] = *reinterpret_cast<const V*>(static_cast<const T*>(a.z) + row * a.ld_z + c.col);
+                    }
+#pragma unroll
+                for (int u = 0; u < U; ++u)
+                    if (s + u * c.rp < a.S) {
+                        sx[(k + u) * kThreads] = v[u];
+                        if (BWD) sd[(k + u) * kThreads] = d[u % (BWD ? U : 1)];
+                        if (gate) sz[(k + u) * kThreads] = g[u];
+                        if (!BWD) {
+#pragma unroll
+                            for (int e = 0; e < VEC; ++e) s1 += to_f(v[u].v[e]);
+                        }
+                    }
+            }
+        }
+        if constexpr (!BWD) {
+            mean = group_sum<T, VEC>(p, c, s1, per_thread, per_group) * inv;
+            if (c.on)
+                for (int s = c.r, k = 0; s < a.S; s += c.rp, ++k) {
+                    float x[VEC];
+                    widen(sx[k * kThreads], x);
+#pragma unroll
+                    for (int e = 0; e < VEC; ++e) s2 = fmaf(x[e] - mean, x[e] - mean, s2);
+                }
+            rstd = 1.0f / sqrtf(group_sum<T, VEC>(p, c, s2, per_thread, per_group) * inv + a.eps);
+            if (c.on && a.stats && c.r == 0 && c.col == c.g * p.per) {
+                a.stats[static_cast<long long>(ns) * a.G + c.g] = mean;
+                a.stats[NG + static_cast<long long>(ns) * a.G + c.g] = rstd;
+            }
+            if (c.on)
+                for (int s = c.r, k = 0; s < a.S; s += c.rp, ++k) {
+                    float x[VEC], z[VEC];
+                    widen(sx[k * kThreads], x);
+                    if (gate) widen(sz[k * kThreads], z);
+#pragma unroll
+                    for (int e = 0; e < VEC; ++e) {
+                        x[e] = act<T>(a.activation, fmaf((x[e] - mean) * rstd, w[e], bias[e]));
+                        if (gate) x[e] *= z[e] * sigmoid<T>(z[e]);
+                    }
+                    store<T, VEC>(static_cast<T*>(a.y) + (row0 + s) * a.ld_y + c.col, x);
+                }
+        } else {
+            float dw[VEC], db[VEC];
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) dw[e] = db[e] = 0.0f;
+            if (c.on)
+                for (int s = c.r, k = 0; s < a.S; s += c.rp, ++k) {
+                    float x[VEC], z[VEC], dy[VEC], dz;
+                    widen(sx[k * kThreads], x);
+                    widen(sd[k * kThreads], dy);
+                    if (gate) widen(sz[k * kThreads], z);
+#pragma unroll
+                    for (int e = 0; e < VEC; ++e) {
+                        const float xh = (x[e] - mean) * rstd;
+                        const float dv = through<T>(a.activation, fmaf(xh, w[e], bias[e]), dy[e], gate, gate ? z[e] : 0.0f, &dz);
+                        dw[e] = fmaf(dv, xh, dw[e]);
+                        db[e] += dv;
+                    }
+                }
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) {
+                s1 = fmaf(w[e], db[e], s1);
+                s2 = fmaf(w[e], dw[e], s2);
+                all_w[e] += dw[e];
+                all_b[e] += db[e];
+            }
+            s1 = group_sum<T, VEC>(p, c, s1, per_thread, per_group) * inv;
+            s2 = group_sum<T, VEC>(p, c, s2, per_thread, per_group) * inv;
+            if (c.on)
+                for (int s = c.r, k = 0; s < a.S; s += c.rp, ++k) {
+                    float x[VEC], z[VEC], dy[VEC];
+                    widen(sx[k * kThreads], x);
+                    widen(sd[k * kThreads], dy);
+                    if (gate) widen(sz[k * kThreads], z);
+#pragma unroll
+                    for (int e = 0; e < VEC; ++e) {
+                        const float xh = (x[e] - mean) * rstd;
+                        const float dv = through<T>(a.activation, fmaf(xh, w[e], bias[e]), dy[e], gate, gate ? z[e] : 0.0f, &z[e]);
+                        x[e] = rstd * (dv * w[e] - s1 - xh * s2);
+                    }
+                    store<T, VEC>(static_cast<T*>(a.d_x) + (row0 + s) * a.ld_dx + c.col, x);
+                    if (gate) store<T, VEC>(static_cast<T*>(a.d_z) + (row0 + s) * a.ld_dz + c.col, z);
+                }
+        }
+    }
+    if constexpr (BWD) {
+        const int wide = p.groups * p.vecs;
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) {
+            sw[e * kThreads + threadIdx.x] = all_w[e];
+            sb[e * kThreads + threadIdx.x] = all_b[e];
+        }
+        __syncthreads();
+        if (c.r == 0 && c.on) {
+            float* out_w = p.sums + static_cast<long long>(blockIdx.x) * a.C + c.col;
+            float* out_b = out_w + static_cast<long long>(p.parts) * a.C;
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) {
+                float tw = all_w[e], tb = all_b[e];
+                for (int k = 1; k < c.rp; ++k) {
+                    tw += sw[e * kThreads + k * wide + threadIdx.x];
+                    tb += sb[e * kThreads + k * wide + threadIdx.x];
+                }
+                out_w[e] = tw;
+                out_b[e] = tb;
+            }
+        }
+    }
+}
+
 // ---------------------------------------------------------------------------------------------------
 // host
 // ---------------------------------------------------------------------------------------------------
@@ -636,22 +1011,58 @@ inline Room room(int N, int S, int C, int G, int backward) {
     return r;
 }
 
-template <typename T, int VEC, int VPT>
-int launch_rows(Ctx* c, Params& p, bool bwd, cudaStream_t st) {
+// One kernel for a sample: the groups of a block (into p.groups) and its shared memory, or 0 where two kernels are better.  A block's
+// piece of a row is at least 64 bytes where there are groups for it, and there have to be enough blocks for a third of the SMs.
+constexpr size_t kSlab = 192 * 1024;  // (beside 16 KB of the backward's sums)
+inline size_t slab_groups(const mamba_b200_group_norm_args& a, Params& p, size_t vec, bool bwd) {
+    const int tensors = (bwd ? 2 : 1) + (a.z ? 1 : 0);
+    int groups = static_cast<int>((64 + p.vecs * vec - 1) / (p.vecs * vec));
+    if (groups > p.groups) groups = p.groups;
+    const long long rp = kThreads / (groups * p.vecs), turns = (a.S + rp - 1) / rp, across = (a.G + groups - 1) / groups;
+    const unsigned long long bytes = static_cast<unsigned long long>(turns) * kThreads * vec * tensors;
+    if (bytes > kSlab || across > 65535 || across * a.N < 48) return 0;
+    p.groups = groups;
+    return bytes;
+}
+
+inline int join_sums(Ctx* c, const Params& p, bool bwd, cudaStream_t st) {
+    const mamba_b200_group_norm_args& a = p.a;
+    if (!bwd || (!a.d_weight && !a.d_bias)) return MAMBA_B200_OK;
+    join_kernel<<<dim3(static_cast<unsigned>((a.C + 31) / 32), 2), 256, 0, st>>>(p.sums, p.parts, a.C, a.d_weight, a.d_bias, a.accumulate);
+    MB200_CUDA_CHECK(c, cudaGetLastError());
+    return MAMBA_B200_OK;
+}
+
+template <typename T, int VEC, int VPT, bool BWD>
+const void* rows_fn(int act, bool gate) {
+    if (act == MAMBA_B200_ACT_SILU)
+        return gate ? (const void*)rows_kernel<T, VEC, VPT, BWD, MAMBA_B200_ACT_SILU, true> : (const void*)rows_kernel<T, VEC, VPT, BWD, MAMBA_B200_ACT_SILU, false>;
+    if (act == MAMBA_B200_ACT_GELU)
+        return gate ? (const void*)rows_kernel<T, VEC, VPT, BWD, MAMBA_B200_ACT_GELU, true> : (const void*)rows_kernel<T, VEC, VPT, BWD, MAMBA_B200_ACT_GELU, false>;
+    return gate ? (const void*)rows_kernel<T, VEC, VPT, BWD, MAMBA_B200_ACT_NONE, true> : (const void*)rows_kernel<T, VEC, VPT, BWD, MAMBA_B200_ACT_NONE, false>;
+}
+
+template <typename T, int VEC, int VPT, bool BWD>
+int launch_rows(Ctx* c, Params& p, cudaStream_t st) {
     const long long steps = (p.a.N + static_cast<long long>(p.rows) - 1) / p.rows;
     const int tiles = (p.a.G + p.groups - 1) / p.groups;
     if (tiles > 65535) return fail(c, MAMBA_B200_ERR_SHAPE, "group_norm: too many groups (%d)", p.a.G);
-    long long blocks = (bwd ? kBlocks : 148 * 16) / tiles;
+    // as many blocks as are resident together (registers: two or four): each goes over its share of the rows
+    long long blocks = static_cast<long long>(c->sm_count) * (BWD ? 2 : 4) / tiles;
+    if (blocks > kBlocks) blocks = kBlocks;
     if (blocks > steps) blocks = steps;
     if (blocks < 1) blocks = 1;
+    p.parts = static_cast<int>(blocks);
     const dim3 grid(static_cast<unsigned>(blocks), static_cast<unsigned>(tiles));
-    if (bwd) {
-        p.parts = static_cast<int>(blocks);
-        rows_kernel<T, VEC, VPT, true><<<grid, kThreads, 0, st>>>(p);
+    if constexpr (VEC == 1) {
+        odd_rows_kernel<T, VPT, BWD><<<grid, kThreads, 0, st>>>(p);
+        MB200_CUDA_CHECK(c, cudaGetLastError());
     } else {
-        rows_kernel<T, VEC, VPT, false><<<grid, kThreads, 0, st>>>(p);
+        const int tensors = (BWD ? 2 : 1) + (p.a.z ? 1 : 0);
+        const size_t smem = static_cast<size_t>(kRowsAhead<VPT>) * tensors * VPT * kThreads * VEC * sizeof(T);
+        void* args[] = {&p};
+        MB200_CUDA_CHECK(c, cudaLaunchKernel(rows_fn<T, VEC, VPT, BWD>(p.a.activation, p.a.z != nullptr), grid, dim3(kThreads), args, smem, st));
     }
-    MB200_CUDA_CHECK(c, cudaGetLastError());
     return MAMBA_B200_OK;
 }
 
@@ -667,18 +1078,35 @@ int launch_vec(Ctx* c, const mamba_b200_group_norm_args& a, bool bwd, cudaStream
     if (bwd) p.sums = reinterpret_cast<float*>(static_cast<char*>(a.workspace) + room.part);
     int rc = MAMBA_B200_OK;
     if (a.S == 1 && p.per <= kRowVecs) {
-        // a group stays within a warp where that takes at most four vectors a lane: no barriers
-        const int vpt = p.vecs <= 32 ? 1 : p.vecs <= 64 ? 2 : 4;
+        // a group stays within a warp where that takes at most two vectors a lane (four elements, where a vector is one): no barriers
+        constexpr int most = VEC == 1 ? 4 : 2;
+        const int vpt = p.vecs <= 32 ? 1 : p.vecs <= 64 ? 2 : most;
         p.lanes = pow2_up((p.vecs + vpt - 1) / vpt);
         p.groups = kThreads / p.lanes < a.G ? kThreads / p.lanes : a.G;
         p.rows = kThreads / (p.groups * p.lanes);
-        if (vpt == 1) rc = launch_rows<T, VEC, 1>(c, p, bwd, st);
-        else if (vpt == 2) rc = launch_rows<T, VEC, 2>(c, p, bwd, st);
-        else rc = launch_rows<T, VEC, 4>(c, p, bwd, st);
+        if (vpt == 1) rc = bwd ? launch_rows<T, VEC, 1, true>(c, p, st) : launch_rows<T, VEC, 1, false>(c, p, st);
+        else if (vpt == 2) rc = bwd ? launch_rows<T, VEC, 2, true>(c, p, st) : launch_rows<T, VEC, 2, false>(c, p, st);
+        else rc = bwd ? launch_rows<T, VEC, most, true>(c, p, st) : launch_rows<T, VEC, most, false>(c, p, st);
         if (rc) return rc;
     } else {
         p.sub = (p.vecs + kThreads - 1) / kThreads;
         p.groups = p.sub > 1 ? 1 : kThreads / p.vecs < a.G ? kThreads / p.vecs : a.G;
+        if (p.sub == 1) {
+            const size_t bytes = slab_groups(a, p, sizeof(T) * VEC, bwd);
+            if (bytes) {
+                const int across = (a.G + p.groups - 1) / p.groups;
+                p.block_rows = a.S;
+                p.blocks = 1;
+                // (no more blocks side by side than the two kernels' scratch has sums for)
+                const long long side = (2 * kBlocks + across - 1) / across;
+                p.side = p.parts = static_cast<int>(side < a.N ? side : a.N);
+                const dim3 grid(static_cast<unsigned>(p.side), static_cast<unsigned>(across));
+                if (bwd) slab_kernel<T, VEC, true><<<grid, kThreads, bytes, st>>>(p);
+                else slab_kernel<T, VEC, false><<<grid, kThreads, bytes, st>>>(p);
+                MB200_CUDA_CHECK(c, cudaGetLastError());
+                return join_sums(c, p, bwd, st);
+            }
+        }
         const long long across = p.sub > 1 ? static_cast<long long>(a.G) * p.sub : (a.G + p.groups - 1) / p.groups;
         const Cut k = cut(a.N, a.S, across);
         p.block_rows = k.block_rows;
@@ -698,11 +1126,7 @@ int launch_vec(Ctx* c, const mamba_b200_group_norm_args& a, bool bwd, cudaStream
         }
         MB200_CUDA_CHECK(c, cudaGetLastError());
     }
-    if (bwd && (a.d_weight || a.d_bias)) {
-        join_kernel<<<dim3(static_cast<unsigned>((a.C + 31) / 32), 2), 256, 0, st>>>(p.sums, p.parts, a.C, a.d_weight, a.d_bias, a.accumulate);
-        MB200_CUDA_CHECK(c, cudaGetLastError());
-    }
-    return MAMBA_B200_OK;
+    return join_sums(c, p, bwd, st);
 }
 
 template <typename T>
@@ -748,7 +1172,30 @@ int check(Ctx* c, const mamba_b200_group_norm_args* a, bool bwd) {
     return MAMBA_B200_OK;
 }
 
+template <typename T, int VEC>
+int configure(Ctx* c) {
+    if constexpr (VEC > 1) {
+        for (int act = 0; act <= MAMBA_B200_ACT_GELU; ++act)
+            for (int gate = 0; gate < 2; ++gate)
+                for (const void* f : {rows_fn<T, VEC, 1, true>(act, gate), rows_fn<T, VEC, 2, true>(act, gate)})
+                    MB200_CUDA_CHECK(c, cudaFuncSetAttribute(f, cudaFuncAttributeMaxDynamicSharedMemorySize, 48 * 1024));
+    }
+    MB200_CUDA_CHECK(c, cudaFuncSetAttribute((const void*)slab_kernel<T, VEC, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(kSlab)));
+    MB200_CUDA_CHECK(c, cudaFuncSetAttribute((const void*)slab_kernel<T, VEC, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(kSlab)));
+    return MAMBA_B200_OK;
+}
+
 }  // namespace gn
+
+int group_norm_configure(Ctx* c) {
+    int rc = gn::configure<float, 4>(c);
+    if (!rc) rc = gn::configure<float, 1>(c);
+    if (!rc) rc = gn::configure<__half, 8>(c);
+    if (!rc) rc = gn::configure<__half, 1>(c);
+    if (!rc) rc = gn::configure<__nv_bfloat16, 8>(c);
+    if (!rc) rc = gn::configure<__nv_bfloat16, 1>(c);
+    return rc;
+}
 
 
 }  // namespace mb200
