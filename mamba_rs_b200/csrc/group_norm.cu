@@ -331,7 +331,7 @@ __global__ void __launch_bounds__(kThreads, VPT > 1 ? 1 : BWD ? 2 : 4) rows_kern
                     v = add2(v, splat2(t.have[i] ? -mean : 0.0f));
                     q = fma2(v, v, q);
                 }
-            const float rstd = 1.0f / sqrtf(sum_group(q.x + q.y, p.lanes, warp_sums, turn) * inv + a.eps);
+            const float rstd = rsqrtf(fmaf(sum_group(q.x + q.y, p.lanes, warp_sums, turn), inv, a.eps));
             if (on && t.lane == 0 && a.stats) {
                 a.stats[n * a.G + t.g] = mean;
                 a.stats[NG + n * a.G + t.g] = rstd;
