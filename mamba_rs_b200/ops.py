@@ -841,25 +841,34 @@ def gated_scan_bwd(x, f, dy, chunk_states, z=None, *, d_last=None, d_h0=None, d_
 
 def _head_strides(t, name, shape, dtype):
     """Strides of batch, step and head of a [B, T, heads, width] view with contiguous columns."""
-    if t.dtype != dtype or tuple(t.shape) != shape:
+    if t.dtype != dtype or t.shape != shape:
         raise TypeError(f"{name} is {list(shape)} {dtype}, not {list(t.shape)} {t.dtype}")
-    if t.stride(3) != 1 and shape[3] > 1:
+    b, s, h, one = t.stride()
+    if one != 1 and shape[3] > 1:
         raise ValueError(f"{name}: last dimension must be contiguous")
-    return t.stride()[:3]
+    return b, s, h
 
 
 def _written(t, name):
     """Refuses an output whose elements share memory (an expanded view)."""
-    if any(s == 0 and n > 1 for s, n in zip(t.stride(), t.shape)):
+    if 0 in t.stride() and t.numel() and any(s == 0 and n > 1 for s, n in zip(t.stride(), t.shape)):
         raise ValueError(f"{name}: an expanded tensor cannot be written")
+
+
+def _heads_of(t, B, T, heads, width):
+    """A contiguous [B, T, heads, width] like t (half the host time of torch.empty)."""
+    row = heads * width
+    return torch.empty_strided((B, T, heads, width), (T * row, row, width, 1), dtype=t.dtype, device=t.device)
 
 
 def _attention_args(q, k, v, decay, scale, state):
     """LinearAttentionArgs with what forward and backward share, and the shape of a state."""
     if q.dim() != 4 or k.dim() != 4 or v.dim() != 4:
         raise ValueError("q, k, v are [B, T, heads, width]")
-    B, T, Hq, K = q.shape
-    Hk, (Hv, V) = k.shape[2], v.shape[2:]
+    dtype = q.dtype
+    B, T, Hq, K = qs = q.shape
+    Hk = k.shape[2]
+    _, _, Hv, V = v.shape
     if decay.dtype != torch.float32 or decay.dim() != 1 or not decay.is_contiguous():
         raise TypeError("decay is contiguous float32 [heads]")
     H = decay.shape[0]
@@ -868,18 +877,19 @@ def _attention_args(q, k, v, decay, scale, state):
             raise ValueError(f"{n}: {h} heads are not shared by {H} evenly")
     if not 1 <= K <= 256 or not 1 <= V <= 256:
         raise ValueError(f"K {K} and V {V} are 1 to 256")
-    a = ffi.LinearAttentionArgs(dtype_code(q.dtype), B, T, H, K, V, Hq, Hk, Hv, K ** -0.5 if scale is None else scale, decay.data_ptr(),
-                                q.data_ptr(), *_head_strides(q, "q", (B, T, Hq, K), q.dtype), k.data_ptr(),
-                                *_head_strides(k, "k", (B, T, Hk, K), q.dtype), v.data_ptr(), *_head_strides(v, "v", (B, T, Hv, V), q.dtype))
     shape = (B, H, K, V)
-    a.state = _attention_state(state, "state", shape)
+    a = ffi.LinearAttentionArgs(dtype_code(dtype), B, T, H, K, V, Hq, Hk, Hv, K ** -0.5 if scale is None else scale, decay.data_ptr(),
+                                q.data_ptr(), *_head_strides(q, "q", qs, dtype), k.data_ptr(), *_head_strides(k, "k", (B, T, Hk, K), dtype),
+                                v.data_ptr(), *_head_strides(v, "v", (B, T, Hv, V), dtype), _attention_state(state, "state", shape))
     return a, shape
 
 
 def _attention_state(t, name, shape):
-    if t is not None and (t.dtype != torch.float32 or tuple(t.shape) != shape or not t.is_contiguous()):
+    if t is None:
+        return None
+    if t.dtype != torch.float32 or t.shape != shape or not t.is_contiguous():
         raise TypeError(f"{name} is contiguous float32 {list(shape)}")
-    return _ptr(t)
+    return t.data_ptr()
 
 
 def _scratch(a, need, workspace, like):
@@ -913,10 +923,12 @@ def linear_attention_fwd(q, k, v, decay, *, scale=None, state=None, state_out=No
     B, H, _, V = shape
     T = q.shape[1]
     if o is None:
-        o = torch.empty((B, T, H, V), dtype=q.dtype, device=q.device)
+        o = _heads_of(q, B, T, H, V)
+        a.o_b, a.o_t, a.o_h = T * H * V, H * V, V
+    else:
+        a.o_b, a.o_t, a.o_h = _head_strides(o, "o", (B, T, H, V), q.dtype)
+        _written(o, "o")
     a.o = o.data_ptr()
-    a.o_b, a.o_t, a.o_h = _head_strides(o, "o", (B, T, H, V), q.dtype)
-    _written(o, "o")
     a.state_out = _attention_state(state_out, "state_out", shape)
     lib = ffi.lib()
     if T > 1:
@@ -941,7 +953,7 @@ def linear_attention_step(q, k, v, decay, state, *, scale=None, state_out=None, 
         if t is not None and (t.dtype != torch.float32 or t.shape != shape or not t.is_contiguous()):
             raise TypeError(f"{name} is contiguous float32 {list(shape)}")
     if o is None:
-        o = torch.empty((B, H, V), dtype=dtype, device=q.device)
+        o = torch.empty_strided((B, H, V), (H * V, V, 1), dtype=dtype, device=q.device)
     elif o.dtype != dtype or o.shape != (B, H, V):
         raise TypeError(f"o is {[B, H, V]} {dtype}")
     else:
@@ -969,18 +981,18 @@ def linear_attention_bwd(q, k, v, do, decay, *, scale=None, state=None, d_state_
     dev = _device_index(q, k, v, do, decay, state, d_state_out, d_q, d_k, d_v, d_state, workspace)
     a, shape = _attention_args(q, k, v, decay, scale, state)
     B, H, _, V = shape
-    new = lambda t, like: torch.empty(like.shape, dtype=like.dtype, device=like.device) if t is None else t  # noqa: E731
+    new = lambda t, like: _heads_of(like, *like.shape) if t is None else t  # noqa: E731
     d_q, d_k, d_v = new(d_q, q), new(d_k, k), new(d_v, v)
     if d_state is None and state is not None:
         d_state = torch.empty(shape, dtype=torch.float32, device=q.device)
     a.d_o = do.data_ptr()
     a.do_b, a.do_t, a.do_h = _head_strides(do, "do", (B, q.shape[1], H, V), q.dtype)
     a.d_state_out, a.d_state = _attention_state(d_state_out, "d_state_out", shape), _attention_state(d_state, "d_state", shape)
-    for n, t, like in (("q", d_q, q), ("k", d_k, k), ("v", d_v, v)):
-        setattr(a, f"d_{n}", t.data_ptr())
-        for d, s in zip("bth", _head_strides(t, f"d_{n}", tuple(like.shape), q.dtype)):
-            setattr(a, f"d{n}_{d}", s)
-        _written(t, f"d_{n}")
+    a.d_q, (a.dq_b, a.dq_t, a.dq_h) = d_q.data_ptr(), _head_strides(d_q, "d_q", q.shape, q.dtype)
+    a.d_k, (a.dk_b, a.dk_t, a.dk_h) = d_k.data_ptr(), _head_strides(d_k, "d_k", k.shape, q.dtype)
+    a.d_v, (a.dv_b, a.dv_t, a.dv_h) = d_v.data_ptr(), _head_strides(d_v, "d_v", v.shape, q.dtype)
+    for t, n in ((d_q, "d_q"), (d_k, "d_k"), (d_v, "d_v")):
+        _written(t, n)
     lib = ffi.lib()
     workspace = _scratch(a, lib.mamba_b200_linear_attention_workspace_bytes(C.byref(a), 1), workspace, q)
     _launch(lib.mamba_b200_linear_attention_bwd, dev, handle, C.byref(a))
@@ -1028,25 +1040,29 @@ def _rotary(q, k, positions, inv_freq, interleaved, scale, inverse, q_out, k_out
     dev = _device_index(q, k, positions, inv_freq, q_out, k_out)
     if q.dim() != 4 or (k is not None and k.dim() != 4):
         raise ValueError("q and k are [B, T, heads, width]")
-    B, T, Hq, D = q.shape
+    dtype = q.dtype
+    B, T, Hq, D = qs = q.shape
     if inv_freq.dtype != torch.float32 or inv_freq.dim() != 1 or not inv_freq.is_contiguous() or 2 * inv_freq.shape[0] > D:
         raise TypeError(f"inv_freq is contiguous float32 of at most {D // 2} pairs")
-    if positions.dtype != torch.int32 or not positions.is_contiguous() or tuple(positions.shape) not in ((T,), (B, T)):
+    if positions.dtype != torch.int32 or not positions.is_contiguous() or positions.shape not in ((T,), (B, T)):
         raise TypeError(f"positions are contiguous int32 [{T}] or [{B}, {T}]")
-    if q_out is None:
-        q_out = torch.empty((B, T, Hq, D), dtype=q.dtype, device=q.device)
-    a = ffi.RotaryArgs(dtype_code(q.dtype), B, T, Hq, 0, D, 2 * inv_freq.shape[0], bool(interleaved), inverse, scale, positions.data_ptr(),
-                       T if positions.dim() == 2 else 0, inv_freq.data_ptr(), q.data_ptr(), *_head_strides(q, "q", (B, T, Hq, D), q.dtype),
-                       q_out.data_ptr(), *_head_strides(q_out, "q_out", (B, T, Hq, D), q.dtype))
-    _written(q_out, "q_out")
+
+    def result(out, name, heads, shape):
+        if out is None:
+            return _heads_of(q, B, T, heads, D), (T * heads * D, heads * D, D)
+        _written(out, name)
+        return out, _head_strides(out, name, shape, dtype)
+
+    q_out, to = result(q_out, "q_out", Hq, qs)
+    ks, Hk = (), 0
     if k is not None:
-        shape = (B, T, k.shape[2], D)
-        if k_out is None:
-            k_out = torch.empty(shape, dtype=q.dtype, device=q.device)
-        a.Hk = shape[2]
-        a.k, (a.k_b, a.k_t, a.k_h) = k.data_ptr(), _head_strides(k, "k", shape, q.dtype)
-        a.k_out, (a.ko_b, a.ko_t, a.ko_h) = k_out.data_ptr(), _head_strides(k_out, "k_out", shape, q.dtype)
-        _written(k_out, "k_out")
+        shape = B, T, Hk, D = (B, T, k.shape[2], D)
+        k_in = _head_strides(k, "k", shape, dtype)
+        k_out, k_to = result(k_out, "k_out", Hk, shape)
+        ks = (k.data_ptr(), *k_in, k_out.data_ptr(), *k_to)
+    a = ffi.RotaryArgs(dtype_code(dtype), B, T, Hq, Hk, D, 2 * inv_freq.shape[0], bool(interleaved), inverse, scale, positions.data_ptr(),
+                       T if positions.dim() == 2 else 0, inv_freq.data_ptr(), q.data_ptr(), *_head_strides(q, "q", qs, dtype),
+                       q_out.data_ptr(), *to, *ks)
     _launch(ffi.lib().mamba_b200_rotary, dev, handle, C.byref(a))
     return q_out, k_out
 
@@ -1086,18 +1102,27 @@ def _norm_rows(t, name, like):
     return t.stride(1)
 
 
+def _rows_like(x):
+    """A contiguous tensor of x's shape and dtype."""
+    if x.dim() == 2:
+        return torch.empty_strided(x.shape, (x.shape[1], 1), dtype=x.dtype, device=x.device)
+    _, S, C_ = x.shape
+    return torch.empty_strided(x.shape, (S * C_, C_, 1), dtype=x.dtype, device=x.device)
+
+
 def _norm_args(x, z, weight, bias, groups, activation, eps):
     if x.dim() not in (2, 3):
         raise ValueError("x is [N, S, C] or [N, C]")
-    N, C_ = x.shape[0], x.shape[-1]
+    shape = x.shape
+    N, C_ = shape[0], shape[-1]
     if groups < 1 or C_ < 1 or C_ % groups:
         raise ValueError(f"{C_} channels are no {groups} groups")
     if activation not in ffi.ACTIVATIONS:
         raise ValueError(f"unknown activation {activation!r}")
     for t, n in ((weight, "weight"), (bias, "bias")):
-        if t is not None and (t.dtype != torch.float32 or tuple(t.shape) != (C_,) or not t.is_contiguous()):
+        if t is not None and (t.dtype != torch.float32 or t.shape != (C_,) or not t.is_contiguous()):
             raise TypeError(f"{n} is contiguous float32 [{C_}]")
-    return ffi.GroupNormArgs(dtype_code(x.dtype), N, 1 if x.dim() == 2 else x.shape[1], C_, groups, ffi.ACTIVATIONS[activation], eps,
+    return ffi.GroupNormArgs(dtype_code(x.dtype), N, 1 if len(shape) == 2 else shape[1], C_, groups, ffi.ACTIVATIONS[activation], eps,
                              x.data_ptr(), _norm_rows(x, "x", x), _ptr(z), 0 if z is None else _norm_rows(z, "z", x), _ptr(weight), _ptr(bias))
 
 
@@ -1108,14 +1133,17 @@ def group_norm_fwd(x, weight, bias, groups, *, eps=1e-5, activation=None, z=None
     Returns (y, stats): mean and rstd f32 [2,N,groups], which group_norm_bwd takes."""
     dev = _device_index(x, weight, bias, z, y, stats, workspace)
     a = _norm_args(x, z, weight, bias, groups, activation, eps)
+    N = a.N
     if y is None:
-        y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+        y, a.ld_y = _rows_like(x), a.C
+    else:
+        a.ld_y = _norm_rows(y, "y", x)
+        _written(y, "y")
     if stats is None:
-        stats = torch.empty((2, x.shape[0], groups), dtype=torch.float32, device=x.device)
-    elif stats.dtype != torch.float32 or tuple(stats.shape) != (2, x.shape[0], groups) or not stats.is_contiguous():
-        raise TypeError(f"stats is contiguous float32 {[2, x.shape[0], groups]}")
-    a.stats, a.y, a.ld_y = stats.data_ptr(), y.data_ptr(), _norm_rows(y, "y", x)
-    _written(y, "y")
+        stats = torch.empty_strided((2, N, groups), (N * groups, groups, 1), dtype=torch.float32, device=x.device)
+    elif stats.dtype != torch.float32 or stats.shape != (2, N, groups) or not stats.is_contiguous():
+        raise TypeError(f"stats is contiguous float32 {[2, N, groups]}")
+    a.stats, a.y = stats.data_ptr(), y.data_ptr()
     lib = ffi.lib()
     workspace = _scratch(a, lib.mamba_b200_group_norm_workspace_bytes(a.N, a.S, a.C, a.G, 0), workspace, x)
     _launch(lib.mamba_b200_group_norm_fwd, dev, handle, C.byref(a))
@@ -1129,17 +1157,19 @@ def group_norm_bwd(dy, x, stats, weight, bias, groups, *, activation=None, z=Non
     else made."""
     dev = _device_index(x, dy, stats, weight, bias, z, d_x, d_z, d_weight, d_bias, workspace)
     a = _norm_args(x, z, weight, bias, groups, activation, 0.0)
-    if stats.dtype != torch.float32 or tuple(stats.shape) != (2, x.shape[0], groups) or not stats.is_contiguous():
-        raise TypeError(f"stats is contiguous float32 {[2, x.shape[0], groups]}")
+    if stats.dtype != torch.float32 or stats.shape != (2, a.N, groups) or not stats.is_contiguous():
+        raise TypeError(f"stats is contiguous float32 {[2, a.N, groups]}")
     if (d_weight is None) != (d_bias is None):
         raise ValueError("d_weight and d_bias are given both or neither")
-    a.accumulate = d_weight is not None
     if d_weight is None:
-        d_weight, d_bias = torch.empty((2, a.C), dtype=torch.float32, device=x.device)
-    for t, n in ((d_weight, "d_weight"), (d_bias, "d_bias")):
-        if t.dtype != torch.float32 or tuple(t.shape) != (a.C,) or not t.is_contiguous():
-            raise TypeError(f"{n} is contiguous float32 [{a.C}]")
-    new = lambda t: torch.empty(x.shape, dtype=x.dtype, device=x.device) if t is None else t  # noqa: E731
+        d_weight = torch.empty_strided((a.C,), (1,), dtype=torch.float32, device=x.device)
+        d_bias = torch.empty_like(d_weight)
+    else:
+        a.accumulate = 1
+        for t, n in ((d_weight, "d_weight"), (d_bias, "d_bias")):
+            if t.dtype != torch.float32 or t.shape != (a.C,) or not t.is_contiguous():
+                raise TypeError(f"{n} is contiguous float32 [{a.C}]")
+    new = lambda t: _rows_like(x) if t is None else t  # noqa: E731
     d_x = new(d_x)
     a.stats, a.dy, a.ld_dy = stats.data_ptr(), dy.data_ptr(), _norm_rows(dy, "dy", x)
     a.d_x, a.ld_dx, a.d_weight, a.d_bias = d_x.data_ptr(), _norm_rows(d_x, "d_x", x), d_weight.data_ptr(), d_bias.data_ptr()
