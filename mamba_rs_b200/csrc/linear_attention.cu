@@ -97,11 +97,26 @@ __global__ void __launch_bounds__(kStepThreads) step_kernel(const mamba_b200_lin
 // With few pairs the sequence is cut into segments: STATE blocks find what each adds to a state from zero, and the full walk
 // starts from the sum of what was before.
 // ---------------------------------------------------------------------------------------------------
-constexpr int kSteps = 32, kCols = 32, kThreads = 256;
+constexpr int kCols = 32, kThreads = 256;
 
 inline size_t gen_smem(int A) { return sizeof(float) * (2 * kSteps * (A + 4) + 2 * kSteps * kCols + kSteps * (kSteps + 4) + A * kCols + 3 * kSteps); }
 
-template <typename T, bool STATE>
+// Four neighbouring elements, of which n are there (vec: they are one aligned piece).
+template <typename T>
+__device__ __forceinline__ float4 load4(const T* p, int n, bool vec) {
+    float v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+    if (vec && n >= 4) {
+        const float2 lo = ld_pair(p), hi = ld_pair(p + 2);
+        return make_float4(lo.x, lo.y, hi.x, hi.y);
+    }
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+        if (e < n) v[e] = to_f(p[e]);
+    return make_float4(v[0], v[1], v[2], v[3]);
+}
+
+// NA: blocks of 32 columns of X and Y (4 or 8).  With 4 a chunk's rows are asked for while the one before is worked on.
+template <typename T, int NA, bool STATE>
 __global__ void __launch_bounds__(kThreads) general_kernel(const Params p) {
     extern __shared__ __align__(16) float sm[];
     const Place w = place(p, blockIdx.x, STATE ? p.segments - 1 : p.segments);
@@ -118,16 +133,34 @@ __global__ void __launch_bounds__(kThreads) general_kernel(const Params p) {
     float* pw = S + Ar * kCols;  // l^i, i <= kSteps
     const float ld = p.decay[h], l2 = ld * kLog2e;
     const int t_lo = w.seg * p.seg_len, t_hi = min(p.T, t_lo + p.seg_len);
-    const T* xg = static_cast<const T*>(r.x.p) + b * r.x.sb + (h / r.x.group) * r.x.sh;
-    const T* yg = static_cast<const T*>(r.y.p) + b * r.y.sb + (h / r.y.group) * r.y.sh;
-    const T* zg = static_cast<const T*>(r.z.p) + b * r.z.sb + (h / r.z.group) * r.z.sh + c0;
+    const int i4 = tid >> 3, j8 = tid & 7, w4 = j8 * 4;
+    // this thread's pieces of a chunk: row i4, four columns at w4 of every 32
     auto row = [&](int t) { return r.backwards ? p.T - 1 - t : t; };
+    const T* xg = static_cast<const T*>(r.x.p) + b * r.x.sb + (h / r.x.group) * r.x.sh + w4;
+    const T* yg = static_cast<const T*>(r.y.p) + b * r.y.sb + (h / r.y.group) * r.y.sh + w4;
+    const T* zg = static_cast<const T*>(r.z.p) + b * r.z.sb + (h / r.z.group) * r.z.sh + c0 + w4;
+    auto whole = [](const T* q, long long st) { return ((reinterpret_cast<uintptr_t>(q) | st * sizeof(T)) & (2 * sizeof(T) - 1)) == 0; };
+    const bool vx = whole(xg, r.x.st), vy = whole(yg, r.y.st), vz = whole(zg, r.z.st);
+    float4 xr[NA], yr[NA], zr;
+    auto fetch = [&](int t0) {
+        const int t = t0 + i4;
+        const bool ok = t < t_hi;
+        const long long at = ok ? row(t) : 0;
+#pragma unroll
+        for (int m = 0; m < NA; ++m) {
+            const int n = ok ? A - w4 - 32 * m : 0;
+            if (!STATE) xr[m] = load4(xg + at * r.x.st + 32 * m, n, vx);
+            yr[m] = load4(yg + at * r.y.st + 32 * m, n, vy);
+        }
+        zr = load4(zg + at * r.z.st, ok ? nc - w4 : 0, vz);
+    };
+    fetch(t_lo);
     if (tid <= kSteps) pw[tid] = decay_at(l2, tid);
     // the state that enters this segment
     const long long slot = static_cast<long long>(A) * W;
     float* slots = r.slots ? r.slots + w.pair * p.segments * slot : nullptr;
     const bool first = w.seg == 0;
-    const Pow per_seg = decay_pow(ld, p.seg_len);
+    const Pow per_chunk = decay_pow(ld, kSteps);
     bool entered = false;
     if (first ? r.s_in != nullptr : !STATE) entered = true;
     for (int i = tid; i < Ar * kCols; i += kThreads) {
@@ -136,32 +169,27 @@ __global__ void __launch_bounds__(kThreads) general_kernel(const Params p) {
         if (a < A && c < nc && entered) {
             const long long e = static_cast<long long>(a) * W + c0 + c;
             if (first && (STATE || p.segments == 1)) s = r.s_in[w.pair * slot + static_cast<long long>(a) * r.sa + static_cast<long long>(c0 + c) * r.sw];
-            else if (first) s = slots[e];
-            else {
-                for (int k = 1; k <= w.seg; ++k) s = (k > 1 ? times(per_seg, s) : 0.0f) + slots[k * slot + e];
-            }
+            else s = slots[w.seg * slot + e];
             if (STATE && first) slots[e] = s;
         }
         S[i] = s;
     }
-    const int i4 = tid >> 3, j8 = tid & 7, w4 = j8 * 4;
     for (int t0 = t_lo; t0 < t_hi; t0 += kSteps) {
         const int n = min(kSteps, t_hi - t0);
         const int late = r.late && first && t0 == t_lo ? 1 : 0;
-        __syncthreads();  // the last chunk's readers of X, Y, Z, Zw; the state is whole
-        for (int i = tid; i < kSteps * Ar; i += kThreads) {
-            const int s = i / Ar, a = i - s * Ar;
-            const bool ok = s < n && a < A;
-            if (!STATE) X[s * LD + a] = ok ? to_f(xg[row(t0 + s) * r.x.st + a]) : 0.0f;
-            Y[s * LD + a] = ok ? to_f(yg[row(t0 + s) * r.y.st + a]) : 0.0f;
-        }
-        for (int i = tid; i < kSteps * kCols; i += kThreads) {
-            const int s = i / kCols, c = i % kCols;
-            const float z = s < n && c < nc ? to_f(zg[row(t0 + s) * r.z.st + c]) : 0.0f;
-            Z[i] = z;
-            Zw[i] = s < n ? z * pw[n - 1 - s] * r.alpha_s : 0.0f;
-        }
+        if (NA > 4 && t0 > t_lo) fetch(t0);
+        __syncthreads();  // the last chunk's readers of X, Y, Z, Zw; the state and the powers are whole
+#pragma unroll
+        for (int m = 0; m < NA; ++m)
+            if (w4 + 32 * m < Ar) {
+                if (!STATE) *reinterpret_cast<float4*>(X + i4 * LD + w4 + 32 * m) = xr[m];
+                *reinterpret_cast<float4*>(Y + i4 * LD + w4 + 32 * m) = yr[m];
+            }
+        const float f = i4 < n ? pw[n - 1 - i4] * r.alpha_s : 0.0f;
+        *reinterpret_cast<float4*>(Z + i4 * kCols + w4) = zr;
+        *reinterpret_cast<float4*>(Zw + i4 * kCols + w4) = make_float4(zr.x * f, zr.y * f, zr.z * f, zr.w * f);
         __syncthreads();
+        if (NA == 4 && t0 + kSteps < t_hi) fetch(t0 + kSteps);
         if (!STATE) {
             // P[i4][j8 + 8 m]
             float g[4] = {0.0f, 0.0f, 0.0f, 0.0f};
@@ -218,7 +246,7 @@ __global__ void __launch_bounds__(kThreads) general_kernel(const Params p) {
         }
         // S[a4 .. a4 + 3][w4 .. w4 + 3]
         if (STATE || t0 + n < t_hi || (w.seg + 1 == p.segments && r.s_out)) {
-            const Pow f = decay_pow(ld, n - late);
+            const Pow f = n - late == kSteps ? per_chunk : decay_pow(ld, n - late);
             for (int a4 = 4 * i4; a4 < Ar; a4 += 4 * (kThreads / 8)) {
                 float4 s[4];
 #pragma unroll
@@ -258,6 +286,31 @@ __global__ void __launch_bounds__(kThreads) general_kernel(const Params p) {
         }
 }
 
+// A thread has one element of a pair's state (whatever its place in a slot means) and eight segments' in flight; the blocks that
+// start from it read one slot then, not all that are before them.
+__global__ void __launch_bounds__(256) chain_kernel(const Params p) {
+    const Role& r = p.role[blockIdx.y];
+    const int size = r.A * r.W, per = (size + 255) / 256;
+    const long long pair = blockIdx.x / per;
+    const int e = (blockIdx.x - static_cast<int>(pair) * per) * 256 + threadIdx.x;
+    if (pair >= static_cast<long long>(p.B) * p.H || e >= size) return;
+    float* s = r.slots + pair * p.segments * size + e;
+    const Pow f = decay_pow(p.decay[pair % p.H], p.seg_len);
+    constexpr int U = 8;
+    float run = s[size];
+    for (int k = 2; k < p.segments; k += U) {
+        float x[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) x[u] = k + u < p.segments ? s[static_cast<long long>(k + u) * size] : 0.0f;
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+            if (k + u < p.segments) {
+                run = times(f, run) + x[u];
+                s[static_cast<long long>(k + u) * size] = run;
+            }
+    }
+}
+
 // Gradients of shared heads: the heads' f32 parts [B, T, H, D], summed in their order.
 template <typename T>
 __global__ void __launch_bounds__(256) sum_heads_kernel(const float* __restrict__ part, T* out, long long ob, long long ot, long long oh,
@@ -280,6 +333,12 @@ __global__ void __launch_bounds__(256) sum_heads_kernel(const float* __restrict_
 // ---------------------------------------------------------------------------------------------------
 inline long long up256(long long n) { return (n + 255) / 256 * 256; }
 
+// Segments of a sequence at the most: two blocks an SM, were a pair one block.
+inline long long most_segments(long long pairs) {
+    const long long n = pairs > 0 ? 2 * 148 / pairs : 1;
+    return n < 1 ? 1 : n < kMaxSegments ? n : kMaxSegments;
+}
+
 // What a call's scratch holds: the states between segments of each role, and the f32 parts of shared heads' gradients.
 struct Room {
     long long slots = 0, parts[3] = {0, 0, 0};
@@ -287,11 +346,10 @@ struct Room {
 };
 inline Room room(const mamba_b200_linear_attention_args& a, int backward) {
     Room r;
-    const long long pairs = static_cast<long long>(a.B) * a.H, chunks = (a.T + kChunk - 1) / kChunk;
-    // more than 148 blocks of the narrowest tiles are not cut, so few pairs have many segments and many have few
-    const long long seg = chunks < 2 ? 0 : kMaxSegments < chunks ? kMaxSegments : chunks;
-    const long long most = pairs > 0 ? 2 * 148 / pairs + 1 : 0;
-    const long long n = seg < most ? seg : most;
+    const long long pairs = static_cast<long long>(a.B) * a.H;
+    // (pick_segments() takes no more)
+    const long long units = (static_cast<long long>(a.T) + kSteps - 1) / kSteps, most = most_segments(pairs);
+    const long long n = units < most ? units : most;
     if (n > 1) r.slots = up256(pairs * n * a.K * a.V * 4) * (backward ? 3 : 1);
     if (backward) {
         const long long rows = static_cast<long long>(a.B) * a.T * a.H * 4;
@@ -302,15 +360,31 @@ inline Room room(const mamba_b200_linear_attention_args& a, int backward) {
     return r;
 }
 
-// Segments of a launch of `blocks` blocks an uncut sequence: as many as fill the SMs once, each of at least four chunks
-// (the states of a segment cost about half a walk of it).
-int pick_segments(int sm_count, long long blocks, int T, long long pairs) {
-    const int chunks = (T + kChunk - 1) / kChunk;
-    long long n = blocks > 0 ? sm_count / blocks : 1;
-    if (n > chunks / 4) n = chunks / 4;
-    if (n > kMaxSegments) n = kMaxSegments;
-    if (pairs > 0 && n > 2 * 148 / pairs + 1) n = 2 * 148 / pairs + 1;  // (what room() has)
-    return n < 2 ? 1 : static_cast<int>(n);
+int chain_segments(Ctx* c, const Params& p, long long pairs, cudaStream_t st) {
+    if (p.segments < 3) return MAMBA_B200_OK;
+    int most = 0;
+    for (int i = 0; i < p.roles; ++i) most = p.role[i].A * p.role[i].W > most ? p.role[i].A * p.role[i].W : most;
+    chain_kernel<<<dim3(static_cast<unsigned>(pairs * ((most + 255) / 256)), p.roles), 256, 0, st>>>(p);
+    MB200_CUDA_CHECK(c, cudaGetLastError());
+    return MAMBA_B200_OK;
+}
+
+// Segments of a sequence of `units` chunks whose uncut launch has `blocks` blocks, of which `together` run at once: the number that is
+// estimated to take least, from the times of a chunk walked in full and for its state alone and what a second kernel costs (us).
+int pick_segments(long long together, long long blocks, int units, long long pairs, double full, double state, double second) {
+    const long long most = most_segments(pairs);
+    int best = 1;
+    double best_us = 1e30;
+    for (int n = 1; n <= most && n <= units; ++n) {
+        const int per = (units + n - 1) / n;
+        const double waves = static_cast<double>((blocks * n + together - 1) / together);
+        const double us = n == 1 ? waves * per * full : second + waves * per * (full + state);
+        if (us < 0.97 * best_us) {
+            best = n;
+            best_us = us;
+        }
+    }
+    return best;
 }
 
 template <typename T>
@@ -323,17 +397,25 @@ int launch_general(Ctx* c, Params& p, bool may_cut, long long pairs, cudaStream_
         blocks += pairs * p.role[i].tiles;
         if (p.role[i].A > A) A = p.role[i].A;
     }
-    p.segments = may_cut ? pick_segments(c->sm_count, blocks, p.T, pairs) : 1;
-    const int chunks = (p.T + kChunk - 1) / kChunk, per = (chunks + p.segments - 1) / p.segments;
-    p.segments = per > 0 ? (chunks + per - 1) / per : 1;
-    p.seg_len = per * kChunk;
+    // (chunks of 32; two blocks on an SM work at their own speed)
+    const int units = (p.T + kSteps - 1) / kSteps;
+    const double width = A / 128.0 + 0.4;
+    p.segments = may_cut ? pick_segments(2 * c->sm_count, blocks, units, pairs, 4.0 * width, 1.5 * width, 6.0) : 1;
+    const int per = (units + p.segments - 1) / p.segments;
+    p.segments = (units + per - 1) / per;
+    p.seg_len = per * kSteps;
     if (blocks * p.segments > 2147483647ll) return fail(c, MAMBA_B200_ERR_SHAPE, "linear_attention: too many heads");
     const size_t smem = gen_smem((A + 3) & ~3);
-    if (p.segments > 1) {
-        general_kernel<T, true><<<static_cast<unsigned>(blocks * (p.segments - 1)), kThreads, smem, st>>>(p);
+    const unsigned grid = static_cast<unsigned>(blocks * p.segments), before = static_cast<unsigned>(blocks * (p.segments - 1));
+    if (before) {
+        if (A <= 128) general_kernel<T, 4, true><<<before, kThreads, smem, st>>>(p);
+        else general_kernel<T, 8, true><<<before, kThreads, smem, st>>>(p);
         MB200_CUDA_CHECK(c, cudaGetLastError());
+        const int rc = chain_segments(c, p, pairs, st);
+        if (rc) return rc;
     }
-    general_kernel<T, false><<<static_cast<unsigned>(blocks * p.segments), kThreads, smem, st>>>(p);
+    if (A <= 128) general_kernel<T, 4, false><<<grid, kThreads, smem, st>>>(p);
+    else general_kernel<T, 8, false><<<grid, kThreads, smem, st>>>(p);
     MB200_CUDA_CHECK(c, cudaGetLastError());
     return MAMBA_B200_OK;
 }
@@ -413,10 +495,11 @@ int dispatch(Ctx* c, const mamba_b200_linear_attention_args& a, Params& p, bool 
 
 int linear_attention_configure(Ctx* c) {
     const int most = static_cast<int>(la::gen_smem(la::kMaxDim));
-    const void* fns[] = {(const void*)la::general_kernel<float, false>,  (const void*)la::general_kernel<float, true>,
-                         (const void*)la::general_kernel<__half, false>, (const void*)la::general_kernel<__half, true>,
-                         (const void*)la::general_kernel<__nv_bfloat16, false>, (const void*)la::general_kernel<__nv_bfloat16, true>};
-    for (const void* f : fns) MB200_CUDA_CHECK(c, cudaFuncSetAttribute(f, cudaFuncAttributeMaxDynamicSharedMemorySize, most));
+#define MB200_LA(T, NA)                                                                                                                          \
+    MB200_CUDA_CHECK(c, cudaFuncSetAttribute((const void*)la::general_kernel<T, NA, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, most)); \
+    MB200_CUDA_CHECK(c, cudaFuncSetAttribute((const void*)la::general_kernel<T, NA, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, most));
+    MB200_LA(float, 4) MB200_LA(float, 8) MB200_LA(__half, 4) MB200_LA(__half, 8) MB200_LA(__nv_bfloat16, 4) MB200_LA(__nv_bfloat16, 8)
+#undef MB200_LA
     return MAMBA_B200_OK;
 }
 

@@ -18,7 +18,8 @@
 namespace mb200 {
 namespace la {
 
-constexpr int kChunk = 128;     // steps of a tensor-core tile; segments are whole chunks in both kernels
+constexpr int kChunk = 128;     // steps of a tensor-core tile
+constexpr int kSteps = 32;      // steps of a chunk of the general kernel (segments are whole chunks)
 constexpr int kMaxSegments = 64;
 constexpr int kMaxDim = 256;    // of K and V
 
@@ -42,7 +43,8 @@ struct Role {
     float alpha_p, alpha_x, alpha_s;
     int tiles;            // column tiles of W
     long long block0;     // first block of this role in a launch
-    float* slots;         // [B * H][segments][A][W]: slot 0 the entering state, slot r what segment r - 1 adds to a state
+    float* slots;         // [B * H][segments][A * W]: slot 0 the entering state, slot r what segment r - 1 leaves of it or adds to a state,
+                          // and after chain_segments() the state that enters segment r
 };
 
 struct Params {
@@ -92,6 +94,9 @@ __device__ __forceinline__ float times(const Pow& f, float s) { return fmaf(f.hi
 // l^n, n >= 0, in 32 bits (n = 0: 1 for every decay, minus infinity among them)
 __device__ __forceinline__ float decay_at(float log2_decay, int n) { return n > 0 ? exp2f(log2_decay * n) : 1.0f; }
 
+// Turns what each segment adds to a state (slots 1 ...) into what enters the next one, in place.
+int chain_segments(Ctx* c, const Params& p, long long pairs, cudaStream_t st);
+int pick_segments(long long together, long long blocks, int units, long long pairs, double full, double state, double second);
 // linear_attention_tc.cu: launches, if it takes such a call (`taken`).
 int tc_launch(Ctx* c, int dtype, Params& p, bool may_cut, long long pairs, cudaStream_t st, bool* taken);
 

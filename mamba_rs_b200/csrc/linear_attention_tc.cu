@@ -35,8 +35,8 @@ using namespace mb200::tc;
 
 constexpr int kThreads = 768, kTile = 64;
 constexpr uint32_t kSub = kSwSub;  // a [128 x 64] sub-tile
-// Tensor memory: two buffers of G, whose left half P takes and whose right half P Z; two of X S; S and, in f16, the sum of its second
-// terms.
+// Tensor memory: two buffers of G, whose left half P takes and whose right half P Z; two of X S; S and, in f16, the sum of a chunk's
+// second terms.
 constexpr uint32_t cG = 0, cY1 = 64, cY2 = 256, cS = 384, cSlo = 448, kCols = 512;
 
 struct TcParams {
@@ -314,7 +314,7 @@ __global__ void __launch_bounds__(kThreads, 1) walk_kernel(const __grid_constant
                         const bool own = F16 && t == 1;  // (the second f16 term is summed apart)
 #pragma unroll
                         for (int k = 0; k < kChunk / 16; ++k)
-                            mma(tmem + (own ? cSlo : cS), ym + at + k * mStep, wm + t * sub + k * mStep, idD, reads || k > 0 || (t > 0 && !own));
+                            mma(tmem + (own ? cSlo : cS), ym + at + k * mStep, wm + t * sub + k * mStep, idD, own ? k > 0 : reads || k > 0 || t > 0);
                     }
                     commit(&sm->d_full);
                 }
@@ -363,6 +363,7 @@ __global__ void __launch_bounds__(kThreads, 1) walk_kernel(const __grid_constant
             float rf[3];
 #pragma unroll
             for (int k = 0; k < 3; ++k) rf[k] = decay_at(l2, back ? 32 * (k + 1) - lane : lane + 32 * (k + 1) - 31) * r.alpha_p;
+            const float bound = fabsf(r.alpha_p) * fmaxf(1.0f, decay_at(l2, kChunk - 1));  // (a decay above 0 makes them grow)
             const float* diag = sm->diag + 31 + (back ? -lane : lane);
             for (int i = role == 1 ? 0 : 1; i < n; i += 2) {
                 if (!wait_warp(&sm->g_full[i & 1], (i >> 1) & 1, sm, p.status)) break;
@@ -392,16 +393,22 @@ __global__ void __launch_bounds__(kThreads, 1) walk_kernel(const __grid_constant
                 };
                 float scale = 1.0f;
                 if (F16) {
+                    // the scores themselves bound their weighted values (up to the diagonal's alpha_p), and below 2^-28 of the bound an f16 still
+                    // has all its digits
                     float m = 0.0f;
 #pragma unroll 1
                     for (int k = back ? q : 0; k <= (back ? 3 : q); ++k) {
                         float g[32];
-                        weigh(k, g);
+                        tmem_ld32(g0 + 32 * k, g);
+                        if (k == q) {
 #pragma unroll
-                        for (int u = 0; u < 32; ++u) m = fmaxf(m, fabsf(g[u]));
+                            for (int u = 0; u < 32; ++u) g[u] = (back ? u >= lane : u <= lane) ? g[u] : 0.0f;
+                        }
+#pragma unroll
+                        for (int u = 0; u < 32; u += 2) m = fmaxf(m, fmaxf(fabsf(g[u]), fabsf(g[u + 1])));
                     }
                     float undo;
-                    scale = scale_to(m, &undo);
+                    scale = scale_to(m * bound, &undo);
                     sm->row_scale[i & 1][row] = undo;
                 }
                 // (P takes the place of G's columns that have been read: from the left.  One block a turn: code unrolled over a chunk waits for
@@ -431,44 +438,49 @@ __global__ void __launch_bounds__(kThreads, 1) walk_kernel(const __grid_constant
         float* slots = r.slots ? r.slots + w.pair * p.segments * slot : nullptr;
         const bool mine = row < A;
         const int nc = min(kTile, W - c0);
+        // (states between segments lie column by column here: a warp's rows are neighbours)
         if (enters) {
-            const long long e = static_cast<long long>(row) * W + c0;
             const bool given = w.seg == 0 && (STATE || p.segments == 1);
-            const float* in = given ? r.s_in + w.pair * slot + static_cast<long long>(row) * r.sa + static_cast<long long>(c0) * r.sw : slots + e;
-            const int step = given ? r.sw : 1;
-            const Pow f = decay_pow(ld, p.seg_len);
+            const int at = mine ? row : 0;  // (rows that are none read the first one, and drop it: loads without a branch are in flight together)
+            const float* in = r.s_in + w.pair * slot + static_cast<long long>(at) * r.sa + static_cast<long long>(c0) * r.sw;
+            const bool quads = given && r.sw == 1 && nc == kTile && (reinterpret_cast<uintptr_t>(r.s_in) | (r.sa * sizeof(float))) % 16 == 0;
+            const float* between = slots + w.seg * slot + static_cast<long long>(c0) * A + at;
 #pragma unroll 1
             for (int s = 0; s < 2; ++s) {
                 float v[32];
+                const int last = max(nc - 32 * s, 1) - 1;  // columns behind the last one read that, and drop it
+                if (quads) {
 #pragma unroll
-                for (int c = 0; c < 32; ++c) {
-                    v[c] = 0.0f;
-                    if (mine && 32 * s + c < nc && w.seg == 0) v[c] = in[static_cast<long long>(32 * s + c) * step];
-                }
-#pragma unroll 1
-                for (int k = 1; k <= w.seg; ++k) {
+                    for (int c = 0; c < 32; c += 4) {
+                        const float4 x = *reinterpret_cast<const float4*>(in + 32 * s + c);
+                        v[c] = x.x; v[c + 1] = x.y; v[c + 2] = x.z; v[c + 3] = x.w;
+                    }
+                } else if (nc > 32 * s) {
+                    const float* q = given ? in + static_cast<long long>(32 * s) * r.sw : between + static_cast<long long>(32 * s) * A;
+                    const int step = given ? r.sw : A;
 #pragma unroll
-                    for (int c = 0; c < 32; ++c)
-                        if (mine && 32 * s + c < nc) v[c] = (k > 1 ? times(f, v[c]) : 0.0f) + slots[k * slot + e + 32 * s + c];
+                    for (int c = 0; c < 32; ++c) v[c] = q[min(c, last) * step];
                 }
+#pragma unroll
+                for (int c = 0; c < 32; ++c)
+                    if (!mine || 32 * s + c >= nc) v[c] = 0.0f;
                 if (STATE && mine) {
+                    float* q = slots + static_cast<long long>(c0 + 32 * s) * A + row;
 #pragma unroll
                     for (int c = 0; c < 32; ++c)
-                        if (32 * s + c < nc) slots[e + 32 * s + c] = v[c];
+                        if (32 * s + c < nc) q[c * A] = v[c];
                 }
                 tmem_st32(lanes + cS + 32 * s, v);
-                if (F16) {
-#pragma unroll
-                    for (int c = 0; c < 32; ++c) v[c] = 0.0f;
-                    tmem_st32(lanes + cSlo + 32 * s, v);
-                }
             }
         }
         const Pow whole = decay_pow(ld, kChunk);
-        // 32 columns of S
-        auto read = [&](int s, float* v, float* lo) {
+        // 32 columns of S (f16: with the sum of the last chunk's second terms)
+        auto read = [&](int s, float* v) {
             if (F16) {
+                float lo[32];
                 tmem_ld32x2(lanes + cS + 32 * s, v, lanes + cSlo + 32 * s, lo);
+#pragma unroll
+                for (int c = 0; c < 32; ++c) v[c] = fmaf(lo[c], 1.0f / 2048, v[c]);
             } else {
                 tmem_ld32(lanes + cS + 32 * s, v);
             }
@@ -491,11 +503,16 @@ __global__ void __launch_bounds__(kThreads, 1) walk_kernel(const __grid_constant
                         float m = 0.0f;
 #pragma unroll 1
                         for (int s = 0; s < 2; ++s) {
-                            float v[32], lo[32];
-                            read(s, v, lo);
+                            float v[32];
+                            if (i > 0) {
+                                read(s, v);
+                                tmem_st32(lanes + cS + 32 * s, v);
+                            } else {
+                                tmem_ld32(lanes + cS + 32 * s, v);
+                            }
                             if (mine) {
 #pragma unroll
-                                for (int c = 0; c < 32; ++c) m = fmaxf(m, fabsf(fmaf(lo[c], 1.0f / 2048, v[c])));
+                                for (int c = 0; c < 32; c += 2) m = fmaxf(m, fmaxf(fabsf(v[c]), fabsf(v[c + 1])));
                             }
                         }
                         m = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(m)));
@@ -516,8 +533,9 @@ __global__ void __launch_bounds__(kThreads, 1) walk_kernel(const __grid_constant
                 unsigned char* copy = smem + kS + (u % SB) * kSub;
 #pragma unroll 1
                 for (int s = 0; s < 2; ++s) {
-                    float v[32], lo[F16 ? 32 : 1];
-                    read(s, v, lo);
+                    float v[32];
+                    if (F16 && STATE && i > 0) read(s, v);
+                    else tmem_ld32(lanes + cS + 32 * s, v);  // (f16: joined above)
                     if (!STATE) {
 #pragma unroll
                         for (int j = 0; j < 4; ++j) {
@@ -525,8 +543,7 @@ __global__ void __launch_bounds__(kThreads, 1) walk_kernel(const __grid_constant
 #pragma unroll
                             for (int e = 0; e < 4; ++e) {
                                 const int c = 8 * j + 2 * e;
-                                if (F16) o[e] = pack2<Th>(fmaf(lo[c % (F16 ? 32 : 1)], 1.0f / 2048, v[c]) * scale, fmaf(lo[(c + 1) % (F16 ? 32 : 1)], 1.0f / 2048, v[c + 1]) * scale);
-                                else o[e] = pack2<Th>(v[c], v[c + 1]);
+                                o[e] = F16 ? pack2<Th>(v[c] * scale, v[c + 1] * scale) : pack2<Th>(v[c], v[c + 1]);
                             }
                             *reinterpret_cast<uint4*>(copy + sw_chunk(row, 4 * s + j)) = make_uint4(o[0], o[1], o[2], o[3]);
                         }
@@ -540,11 +557,6 @@ __global__ void __launch_bounds__(kThreads, 1) walk_kernel(const __grid_constant
                             v[c + 1] = x.y;
                         }
                         tmem_st32(lanes + cS + 32 * s, v);
-                        if constexpr (F16) {
-#pragma unroll
-                            for (int c = 0; c < 32; ++c) lo[c] *= f.hi;
-                            tmem_st32(lanes + cSlo + 32 * s, lo);
-                        }
                     }
                 }
                 if (!STATE) fence_proxy_async();
@@ -557,16 +569,25 @@ __global__ void __launch_bounds__(kThreads, 1) walk_kernel(const __grid_constant
             ok = wait_warp(&sm->d_full, (n - 1) & 1, sm, p.status);
             if (ok) {
                 fence_after();
-                float* out = (STATE ? slots + (w.seg + 1) * slot : r.s_out + w.pair * slot) + static_cast<long long>(row) * W + c0;
                 const Pow f = !STATE && r.last_decay ? decay_pow(ld, 1) : Pow{1.0f, 0.0f};
+                float* out = STATE ? slots + (w.seg + 1) * slot + static_cast<long long>(c0) * A + row
+                                   : r.s_out + w.pair * slot + static_cast<long long>(row) * W + c0;
+                const bool quads = !STATE && nc == kTile && (reinterpret_cast<uintptr_t>(out) | (W * sizeof(float))) % 16 == 0;
 #pragma unroll 1
                 for (int s = 0; s < 2; ++s) {
-                    float v[32], lo[32];
-                    read(s, v, lo);
-                    if (mine) {
+                    float v[32];
+                    read(s, v);
+                    const int left = mine ? nc - 32 * s : 0;
+#pragma unroll
+                    for (int c = 0; c < 32; ++c) v[c] = times(f, v[c]);
+                    if (quads) {
+#pragma unroll
+                        for (int c = 0; c < 32; c += 4)
+                            if (mine) *reinterpret_cast<float4*>(out + 32 * s + c) = make_float4(v[c], v[c + 1], v[c + 2], v[c + 3]);
+                    } else {
 #pragma unroll
                         for (int c = 0; c < 32; ++c)
-                            if (32 * s + c < nc) out[32 * s + c] = times(f, F16 ? fmaf(lo[c], 1.0f / 2048, v[c]) : v[c]);
+                            if (c < left) out[(32 * s + c) * (STATE ? A : 1)] = v[c];
                     }
                 }
             }
@@ -735,6 +756,8 @@ int launch(Ctx* c, TcParams& tp, long long pairs, cudaStream_t st) {
     if (tp.p.segments > 1) {
         walk_kernel<Th, TERMS, true><<<static_cast<unsigned>(blocks * (tp.p.segments - 1)), kThreads, smem, st>>>(tp);
         MB200_CUDA_CHECK(c, cudaGetLastError());
+        const int rc = chain_segments(c, tp.p, pairs, st);
+        if (rc) return rc;
     }
     walk_kernel<Th, TERMS, false><<<static_cast<unsigned>(blocks * tp.p.segments), kThreads, smem, st>>>(tp);
     MB200_CUDA_CHECK(c, cudaGetLastError());
@@ -742,8 +765,6 @@ int launch(Ctx* c, TcParams& tp, long long pairs, cudaStream_t st) {
 }
 
 }  // namespace tcl
-
-int pick_segments(int sm_count, long long blocks, int T, long long pairs);
 
 // Takes the call where the tensor cores' kernel can: 16-bit types, both widths up to 128, tensors that TMA can describe, and more
 // steps than the general kernel's 32 (a tile has 128 rows whatever T is).
@@ -775,8 +796,9 @@ int tc_launch(Ctx* c, int dtype, Params& p, bool may_cut, long long pairs, cudaS
         ++k;
     }
     if (blocks > 1000000000ll / kMaxSegments) return MAMBA_B200_OK;
-    p.segments = may_cut ? pick_segments(c->sm_count, blocks, p.T, pairs) : 1;
-    const int chunks = (p.T + kChunk - 1) / kChunk, per = (chunks + p.segments - 1) / p.segments;
+    const int chunks = (p.T + kChunk - 1) / kChunk;
+    p.segments = may_cut ? pick_segments(c->sm_count, blocks, chunks, pairs, 1.9, 1.3, 14.0) : 1;
+    const int per = (chunks + p.segments - 1) / p.segments;
     p.segments = (chunks + per - 1) / per;
     p.seg_len = per * kChunk;
     *taken = true;
