@@ -389,14 +389,14 @@ int pick_segments(long long together, long long blocks, int units, long long pai
 
 template <typename T>
 int launch_general(Ctx* c, Params& p, bool may_cut, long long pairs, cudaStream_t st) {
-    long long blocks = 0;
     int A = 0;
+    p.tiles = 0;
     for (int i = 0; i < p.roles; ++i) {
         p.role[i].tiles = (p.role[i].W + kCols - 1) / kCols;
-        p.role[i].block0 = blocks;
-        blocks += pairs * p.role[i].tiles;
+        p.tiles += p.role[i].tiles;
         if (p.role[i].A > A) A = p.role[i].A;
     }
+    const long long blocks = pairs * p.tiles;
     // (chunks of 32; two blocks on an SM work at their own speed)
     const int units = (p.T + kSteps - 1) / kSteps;
     const double width = A / 128.0 + 0.4;
@@ -541,7 +541,7 @@ extern "C" MAMBA_B200_API int mamba_b200_linear_attention_fwd(void* handle, void
     r.out = a.o; r.ob = a.o_b; r.ot = a.o_t; r.oh = a.o_h;
     r.s_in = a.state; r.sa = a.V; r.sw = 1;
     r.s_out = a.state_out;
-    r.alpha_p = r.alpha_x = a.scale;
+    r.alpha_p = r.alpha_x = r.alpha_z = a.scale;
     r.alpha_s = 1.0f;
     const la::Room room = la::room(a, 0);
     const bool may_cut = room.slots > 0 && a.workspace && a.workspace_bytes >= room.slots;
@@ -609,6 +609,7 @@ extern "C" MAMBA_B200_API int mamba_b200_linear_attention_bwd(void* handle, void
         r.alpha_p = a.scale;
         r.alpha_x = i == 0 ? a.scale : 1.0f;
         r.alpha_s = i == 0 ? 1.0f : a.scale;
+        r.alpha_z = i == 0 ? a.scale : 1.0f;
         if (may_cut) r.slots = reinterpret_cast<float*>(ws + room.slots / 3 * i);
     }
     rc = la::dispatch(c, a, p, may_cut, st);

@@ -41,36 +41,37 @@ struct Role {
     float* s_out;         // leaving state [A, W] (null: not wanted)
     int backwards, late, last_decay;
     float alpha_p, alpha_x, alpha_s;
+    float alpha_z;        // alpha_p / alpha_s
     int tiles;            // column tiles of W
-    long long block0;     // first block of this role in a launch
     float* slots;         // [B * H][segments][A * W]: slot 0 the entering state, slot r what segment r - 1 leaves of it or adds to a state,
                           // and after chain_segments() the state that enters segment r
 };
 
 struct Params {
     Role role[3];
-    int roles, B, T, H;
+    int roles, tiles, B, T, H;  // tiles: of all roles
     int segments, seg_len;  // seg_len: steps of a segment, whole chunks
     const float* decay;
     int* status;
 };
 
-// The role and place of a block: pair = b * H + h.
+// The role and place of a block: pair = b * H + h.  The roles and column tiles of a pair's segment are neighbours: they read the same
+// rows at about the same time, which the later ones find in L2.
 struct Place {
     int role, tile, seg;
     long long pair;
 };
 __device__ __forceinline__ Place place(const Params& p, long long block, int segments) {
     Place w;
+    const long long i = block / p.tiles;
+    w.tile = static_cast<int>(block - i * p.tiles);
     w.role = 0;
 #pragma unroll
-    for (int r = 1; r < 3; ++r)
-        if (r < p.roles && block >= p.role[r].block0 * segments) w.role = r;
-    long long i = block - p.role[w.role].block0 * segments;
-    const int tiles = p.role[w.role].tiles;
-    // the column tiles of a pair are neighbours: they read the same x and y, which the second one finds in L2
-    w.tile = static_cast<int>(i % tiles);
-    i /= tiles;
+    for (int r = 0; r < 2; ++r)
+        if (r + 1 < p.roles && w.role == r && w.tile >= p.role[r].tiles) {
+            w.tile -= p.role[r].tiles;
+            w.role = r + 1;
+        }
     w.seg = static_cast<int>(i % segments);
     w.pair = i / segments;
     return w;

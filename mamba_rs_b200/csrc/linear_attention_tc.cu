@@ -42,15 +42,16 @@ constexpr uint32_t cG = 0, cY1 = 64, cY2 = 256, cS = 384, cSlo = 448, kCols = 51
 struct TcParams {
     CUtensorMap x[3], y[3], z[3], out[3];
     Params p;
-    int na, stages, z_stages;  // sub-tiles of X (and of Y) in a stage; stages of X and Y, of Z
+    int na, stages, z_tiles;  // sub-tiles of X (and of Y) in a stage; stages of X and Y; tiles for stages of Z and terms of w o Z
     int out_map[3];  // 1: out can be described too, and rows leave in tiles of 32
 };
 
-// Copies of S and stages of Z, in the room that two stages of X and Y (of two sub-tiles) and w o Z leave.
+// Tiles beside the stages of X and Y: copies of S, and those for Z and w o Z.
 template <int TERMS>
 constexpr int kCopies = TERMS == 1 ? 2 : 1;
-template <int TERMS>
-constexpr int kMostZ = TERMS == 3 ? 2 : 3;
+constexpr int kTiles = 6;  // beside two stages of X and Y of two sub-tiles, or four of one
+// A chunk's smallest weight is above e^-kSlow where w o Z stands in for Z.
+constexpr float kSlow = 40.0f;
 
 // behind the stages, the terms of w o Z and the copies of S
 struct Small {
@@ -59,14 +60,14 @@ struct Small {
     float row_scale[2][128];
     float tile_scale[4];  // (a copy's is read until its rows are out, which is known of the chunk three before)
     float warp_max[2][4];
-    uint64_t full[4], empty[4], z_full[4], z_empty[4], g_full[2], p_full[2], y_full[2], x_full[2], y_empty[2], s_full[2], s_empty[2], w_full, d_full, max_full, drain[2];
+    uint64_t full[4], empty[4], z_full[8], z_empty[8], g_full[2], p_full[2], y_full[2], x_full[2], y_empty[2], s_full[2], s_empty[2], w_full[8], d_full, max_full, drain[2];
     uint32_t tmem;
     int dead;
 };
 
 template <int TERMS>
-uint32_t smem_bytes(int na, int stages, int z_stages) {
-    return (stages * 2 * na + z_stages + TERMS + kCopies<TERMS>) * kSub + sizeof(Small);
+uint32_t smem_bytes(int na, int stages, int z_tiles) {
+    return (stages * 2 * na + z_tiles + kCopies<TERMS>) * kSub + sizeof(Small);
 }
 
 __device__ __forceinline__ void mma_ta(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, bool accumulate) {
@@ -142,14 +143,19 @@ __global__ void __launch_bounds__(kThreads, 1) walk_kernel(const __grid_constant
     const Params& p = tp.p;
     const Place w = place(p, blockIdx.x, STATE ? p.segments - 1 : p.segments);
     const Role& r = p.role[w.role];
-    const int A = r.A, W = r.W, na = (A + 63) >> 6, c0 = w.tile * kTile, stages = tp.stages, zs = tp.z_stages;
-    const uint32_t stage = 2 * tp.na * kSub, oY = tp.na * kSub, kZ = stages * stage, kW = kZ + zs * kSub, kS = kW + TERMS * kSub;
+    const int A = r.A, W = r.W, na = (A + 63) >> 6, c0 = w.tile * kTile, stages = tp.stages;
+    const uint32_t stage = 2 * tp.na * kSub, oY = tp.na * kSub, kZ = stages * stage, kS = kZ + tp.z_tiles * kSub;
     Small* sm = reinterpret_cast<Small*>(smem + kS + SB * kSub);
     const uint32_t sbase = smem_u32(smem);
     const int b = static_cast<int>(w.pair / p.H), h = static_cast<int>(w.pair - static_cast<long long>(b) * p.H);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, role = warp >> 2, row = threadIdx.x & 127;
     const bool back = r.backwards;
     const float ld = p.decay[h], l2 = ld * kLog2e;
+    // `fold`: w o Z takes Z's place and P is G with its future cut off; what is missing, l^{row} up to a constant, is one factor a row of the
+    // result.  Not where l^{-127} leaves the numbers that 32 bits hold with room to spare, nor in f16.
+    const bool fold = !F16 && ld <= 0.0f && ld * (kChunk - 1) >= -kSlow;
+    const int zs = tp.z_tiles - TERMS + (fold ? 1 : 0);  // stages of Z
+    const uint32_t kW = kZ + zs * kSub;
     // chunks of this segment, numbered as they are walked
     const int all = (p.T + kChunk - 1) / kChunk, per = p.seg_len / kChunk;
     const int first = w.seg * per, n = min(all - first, per);
@@ -162,8 +168,11 @@ __global__ void __launch_bounds__(kThreads, 1) walk_kernel(const __grid_constant
         for (int i = 0; i < 4; ++i) {
             mbar_init(&sm->full[i], 1);
             mbar_init(&sm->empty[i], STATE ? 1 : 2);
+        }
+        for (int i = 0; i < 8; ++i) {
             mbar_init(&sm->z_full[i], 1);
             mbar_init(&sm->z_empty[i], STATE ? 1 : 4);
+            mbar_init(&sm->w_full[i], 128);
         }
         for (int i = 0; i < 2; ++i) {
             mbar_init(&sm->g_full[i], 1);
@@ -175,7 +184,6 @@ __global__ void __launch_bounds__(kThreads, 1) walk_kernel(const __grid_constant
             mbar_init(&sm->y_empty[i], 128);
             mbar_init(&sm->drain[i], 1);
         }
-        mbar_init(&sm->w_full, 128);
         mbar_init(&sm->d_full, 1);
         mbar_init(&sm->max_full, 128);
         sm->dead = 0;
@@ -262,7 +270,7 @@ __global__ void __launch_bounds__(kThreads, 1) walk_kernel(const __grid_constant
                 }
                 if (i >= 0) {
                     // P Z of chunk i
-                    ok = wait_warp(&sm->z_full[sz], turn_z & 1, sm, p.status);
+                    ok = wait_warp(fold ? &sm->w_full[sz] : &sm->z_full[sz], turn_z & 1, sm, p.status);
                     if (ok) ok = wait_warp(&sm->p_full[i & 1], (i >> 1) & 1, sm, p.status);
                     if (!ok) break;
                     fence_after();
@@ -293,9 +301,9 @@ __global__ void __launch_bounds__(kThreads, 1) walk_kernel(const __grid_constant
         // ---- Y^T (w o Z) and X S ----
         const uint32_t idY = instr_desc(fmt, 0, 1, 64), idD = instr_desc(fmt, 1, 1, 64);
         const uint64_t xk = desc_sw_k(sbase, 0), ym = desc_sw_mn(sbase + oY, 0);
-        const uint64_t wm = desc_sw_mn(sbase + kW, 0), sc = desc_sw_mn(sbase + kS, 0);
+        const uint64_t zm = desc_sw_mn(sbase + kZ, 0), wm = desc_sw_mn(sbase + kW, 0), sc = desc_sw_mn(sbase + kS, 0);
         bool ok = true;
-        int st = 0, turn = 0;
+        int st = 0, turn = 0, sz = 0, turn_z = 0;
         for (int i = 0; i < n; ++i) {
             const uint32_t at = st * per_stage;
             const bool reads = i > 0 || enters;
@@ -305,16 +313,18 @@ __global__ void __launch_bounds__(kThreads, 1) walk_kernel(const __grid_constant
             if (ok && reads) ok = wait_warp(&sm->s_full[STATE ? 0 : u % SB], (STATE ? u : u / SB) & 1, sm, p.status);
             if (!ok) break;
             if (leaves || i + 1 < n) {
-                ok = wait_warp(&sm->w_full, i & 1, sm, p.status);
+                ok = wait_warp(&sm->w_full[sz], turn_z & 1, sm, p.status);
                 if (!ok) break;
                 fence_after();
+                // first term; the others
+                const uint64_t w0 = fold ? zm + sz * sub : wm, w1 = fold ? wm - sub : wm;
                 if (elect_one()) {
 #pragma unroll
                     for (int t = 0; t < TERMS; ++t) {
                         const bool own = F16 && t == 1;  // (the second f16 term is summed apart)
 #pragma unroll
                         for (int k = 0; k < kChunk / 16; ++k)
-                            mma(tmem + (own ? cSlo : cS), ym + at + k * mStep, wm + t * sub + k * mStep, idD, own ? k > 0 : reads || k > 0 || t > 0);
+                            mma(tmem + (own ? cSlo : cS), ym + at + k * mStep, (t == 0 ? w0 : w1 + t * sub) + k * mStep, idD, own ? k > 0 : reads || k > 0 || t > 0);
                     }
                     commit(&sm->d_full);
                 }
@@ -341,12 +351,16 @@ __global__ void __launch_bounds__(kThreads, 1) walk_kernel(const __grid_constant
             }
             if (elect_one()) {
                 commit(&sm->empty[st]);
-                if (STATE) commit(&sm->z_empty[i % zs]);
+                if (STATE) commit(&sm->z_empty[sz]);
             }
             __syncwarp();
             if (++st == stages) {
                 st = 0;
                 ++turn;
+            }
+            if (++sz == zs) {
+                sz = 0;
+                ++turn_z;
             }
         }
         if (!ok) {
@@ -369,6 +383,36 @@ __global__ void __launch_bounds__(kThreads, 1) walk_kernel(const __grid_constant
                 if (!wait_warp(&sm->g_full[i & 1], (i >> 1) & 1, sm, p.status)) break;
                 fence_after();
                 const uint32_t g0 = lanes + cG + (i & 1) * 128;
+                if (fold) {
+                    // (P takes the place of G's columns that have been read: from the left.  One block a turn: code unrolled over a chunk waits for
+                    // instructions, 8000 cycles a chunk)
+#pragma unroll 1
+                    for (int k = 0; k < 4; ++k) {
+                        uint32_t o[16];
+                        if (back ? k >= q : k <= q) {
+                            float g[32];
+                            tmem_ld32(g0 + 32 * k, g);
+#pragma unroll
+                            for (int u = 0; u < 16; ++u) o[u] = pack2<Th>(g[2 * u], g[2 * u + 1]);
+                            if (k == q) {
+                                // (cut off, not multiplied by 0: what lies behind the edge may be infinite)
+#pragma unroll
+                                for (int u = 0; u < 16; ++u) {
+                                    const bool lo = back ? 2 * u >= lane : 2 * u <= lane, hi = back ? 2 * u + 1 >= lane : 2 * u + 1 <= lane;
+                                    o[u] &= (lo ? 0xffffu : 0u) | (hi ? 0xffff0000u : 0u);
+                                }
+                            }
+                        } else {
+#pragma unroll
+                            for (int u = 0; u < 16; ++u) o[u] = 0;
+                        }
+                        tmem_st16(g0 + 16 * k, o);
+                    }
+                    tmem_st_wait();
+                    fence_before();
+                    mbar_arrive(&sm->p_full[i & 1]);
+                    continue;
+                }
                 // weighted scores of block k
                 auto weigh = [&](int k, float* g) {
                     tmem_ld32(g0 + 32 * k, g);
@@ -411,8 +455,6 @@ __global__ void __launch_bounds__(kThreads, 1) walk_kernel(const __grid_constant
                     scale = scale_to(m * bound, &undo);
                     sm->row_scale[i & 1][row] = undo;
                 }
-                // (P takes the place of G's columns that have been read: from the left.  One block a turn: code unrolled over a chunk waits for
-                // instructions, 8000 cycles a chunk)
 #pragma unroll 1
                 for (int k = 0; k < 4; ++k) {
                     uint32_t o[16];
@@ -552,7 +594,7 @@ __global__ void __launch_bounds__(kThreads, 1) walk_kernel(const __grid_constant
 #pragma unroll
                         for (int c = 0; c < 32; c += 2) {
                             float2 x = make_float2(v[c], v[c + 1]);
-                            x = fma2(x, splat2(f.hi), mul2(x, splat2(f.lo)));
+                            x = TERMS == 1 ? mul2(x, splat2(f.hi)) : fma2(x, splat2(f.hi), mul2(x, splat2(f.lo)));
                             v[c] = x.x;
                             v[c + 1] = x.y;
                         }
@@ -595,6 +637,7 @@ __global__ void __launch_bounds__(kThreads, 1) walk_kernel(const __grid_constant
     } else if (role == 3 && !STATE) {
         // ---- out ----
         const float x_whole = decay_at(l2, back ? kChunk - row : row + 1) * r.alpha_x;
+        const float y_whole = fold ? decay_at(-l2, back ? row : kChunk - 1 - row) * r.alpha_z : 1.0f;
         const int nc = min(kTile, W - c0);
         const bool tiles = tp.out_map[w.role];
         for (int i = 0, sz = 0; i < n; ++i) {
@@ -604,7 +647,8 @@ __global__ void __launch_bounds__(kThreads, 1) walk_kernel(const __grid_constant
             const int t0 = start(i), rows = min(kChunk, p.T - t0);
             const bool reads = i > 0 || enters;
             const int late = i == 0 ? late0 : 0;
-            float f = x_whole, f1 = 1.0f;
+            float f = x_whole, f1 = y_whole;
+            if (fold && !back && rows != kChunk) f1 = decay_at(-l2, max(rows - 1 - row, 0)) * r.alpha_z;
             if (late || (back && rows != kChunk)) f = decay_at(l2, back ? rows - row - late : row + 1 - late) * r.alpha_x;
             if (F16) {
                 f1 = sm->row_scale[i & 1][row];
@@ -619,17 +663,15 @@ __global__ void __launch_bounds__(kThreads, 1) walk_kernel(const __grid_constant
 #pragma unroll
                     for (int c = 0; c < 32; c += 2) {
                         float2 o = make_float2(y[c], y[c + 1]);
-                        if (F16) o = mul2(o, splat2(f1));
+                        o = mul2(o, splat2(f1));
                         o = fma2(make_float2(x[c], x[c + 1]), splat2(f), o);
                         y[c] = o.x;
                         y[c + 1] = o.y;
                     }
                 } else {
                     tmem_ld32(y1 + 32 * s, y);
-                    if (F16) {
 #pragma unroll
-                        for (int c = 0; c < 32; ++c) y[c] *= f1;
-                    }
+                    for (int c = 0; c < 32; ++c) y[c] *= f1;
                 }
             };
             if (tiles) {
@@ -680,12 +722,16 @@ __global__ void __launch_bounds__(kThreads, 1) walk_kernel(const __grid_constant
     } else if (role == 4) {
         // ---- w o Z ----
         const float w_whole = decay_at(l2, back ? row : kChunk - 1 - row) * r.alpha_s;
-        for (int i = 0, st = 0, turn = 0; i < n - (leaves ? 0 : 1); ++i) {
+        // (w o Z as an operand of P's product is wanted of the last chunk too)
+        for (int i = 0, st = 0, turn = 0; i < n - (leaves || fold ? 0 : 1); ++i) {
             const int rows = min(kChunk, p.T - start(i));
             if (!wait_warp(&sm->z_full[st], turn & 1, sm, p.status)) break;
-            if (i > 0 && !wait_warp(&sm->d_full, (i - 1) & 1, sm, p.status)) break;
+            // (the terms' tiles are the last chunk's products' until they are done)
+            if ((TERMS > 1 || !fold) && i > 0 && !wait_warp(&sm->d_full, (i - 1) & 1, sm, p.status)) break;
             const float f = rows == kChunk ? w_whole : row < rows ? decay_at(l2, back ? row : rows - 1 - row) * r.alpha_s : 0.0f;
-            const unsigned char* z = smem + kZ + st * kSub;
+            unsigned char* z = smem + kZ + st * kSub;
+            unsigned char* w0 = fold ? z : smem + kW;
+            unsigned char* w1 = fold ? smem + kW - kSub : smem + kW;
 #pragma unroll 2
             for (int j = 0; j < 8; ++j) {
                 const uint4 v = *reinterpret_cast<const uint4*>(z + sw_chunk(row, j));
@@ -705,10 +751,10 @@ __global__ void __launch_bounds__(kThreads, 1) walk_kernel(const __grid_constant
                 }
 #pragma unroll
                 for (int t = 0; t < TERMS; ++t)
-                    *reinterpret_cast<uint4*>(smem + kW + t * kSub + sw_chunk(row, j)) = make_uint4(o[t][0], o[t][1], o[t][2], o[t][3]);
+                    *reinterpret_cast<uint4*>((t == 0 ? w0 : w1 + t * kSub) + sw_chunk(row, j)) = make_uint4(o[t][0], o[t][1], o[t][2], o[t][3]);
             }
             fence_proxy_async();
-            mbar_arrive(&sm->w_full);
+            mbar_arrive(&sm->w_full[st]);
             if (++st == zs) {
                 st = 0;
                 ++turn;
@@ -743,16 +789,16 @@ static bool make_map(Ctx* c, CUtensorMap* map, int dtype, const Operand& o, int 
 
 template <typename Th, int TERMS>
 int launch(Ctx* c, TcParams& tp, long long pairs, cudaStream_t st) {
-    long long blocks = 0;
     tp.na = 1;
+    tp.p.tiles = 0;
     for (int i = 0; i < tp.p.roles; ++i) {
-        tp.p.role[i].block0 = blocks;
-        blocks += pairs * tp.p.role[i].tiles;
+        tp.p.tiles += tp.p.role[i].tiles;
         if (tp.p.role[i].A > 64) tp.na = 2;
     }
-    tp.stages = tp.na == 2 ? 2 : 3;
-    tp.z_stages = tp.na == 2 ? kMostZ<TERMS> : 4;
-    const uint32_t smem = smem_bytes<TERMS>(tp.na, tp.stages, tp.z_stages);
+    const long long blocks = pairs * tp.p.tiles;
+    tp.stages = tp.na == 2 ? 2 : 4;
+    tp.z_tiles = kTiles - kCopies<TERMS>;
+    const uint32_t smem = smem_bytes<TERMS>(tp.na, tp.stages, tp.z_tiles);
     if (tp.p.segments > 1) {
         walk_kernel<Th, TERMS, true><<<static_cast<unsigned>(blocks * (tp.p.segments - 1)), kThreads, smem, st>>>(tp);
         MB200_CUDA_CHECK(c, cudaGetLastError());
@@ -778,14 +824,16 @@ int tc_launch(Ctx* c, int dtype, Params& p, bool may_cut, long long pairs, cudaS
             if (!(fabsf(p.role[i].alpha_s) <= 1.0f)) return MAMBA_B200_OK;
     for (int i = 0; i < p.roles; ++i)
         if (p.role[i].A > 128 || p.role[i].W > 128) return MAMBA_B200_OK;
-    TcParams tp[2];  // roles that leave no state, and roles that do
+    // Roles that leave a state are kept in more terms, and those of narrow X and Y have room for more stages: up to four launches.
+    TcParams tp[4];
     memset(tp, 0, sizeof(tp));
+    auto kind = [](const Role& r) { return (r.s_out ? 2 : 0) + (r.A > 64 ? 1 : 0); };
     long long blocks = 0;
-    int roles[2] = {0, 0};
+    int roles[4] = {0, 0, 0, 0};
     for (int i = 0; i < p.roles; ++i) {
         Role& r = p.role[i];
-        TcParams& to = tp[r.s_out != nullptr];
-        int& k = roles[r.s_out != nullptr];
+        TcParams& to = tp[kind(r)];
+        int& k = roles[kind(r)];
         if (!make_map(c, &to.x[k], dtype, r.x, p.H, p.T, p.B, kChunk) || !make_map(c, &to.y[k], dtype, r.y, p.H, p.T, p.B, kChunk) ||
             !make_map(c, &to.z[k], dtype, r.z, p.H, p.T, p.B, kChunk))
             return MAMBA_B200_OK;
@@ -802,15 +850,15 @@ int tc_launch(Ctx* c, int dtype, Params& p, bool may_cut, long long pairs, cudaS
     p.segments = (chunks + per - 1) / per;
     p.seg_len = per * kChunk;
     *taken = true;
-    for (int state = 0; state < 2; ++state) {
-        if (!roles[state]) continue;
-        tp[state].p = p;
-        tp[state].p.roles = 0;
+    for (int q = 0; q < 4; ++q) {
+        if (!roles[q]) continue;
+        tp[q].p = p;
+        tp[q].p.roles = 0;
         for (int i = 0; i < p.roles; ++i)
-            if ((p.role[i].s_out != nullptr) == (state == 1)) tp[state].p.role[tp[state].p.roles++] = p.role[i];
-        const int rc = dtype == MAMBA_B200_F16 ? launch<__half, 2>(c, tp[state], pairs, st)
-                       : state                 ? launch<__nv_bfloat16, 3>(c, tp[state], pairs, st)
-                                               : launch<__nv_bfloat16, 1>(c, tp[state], pairs, st);
+            if (kind(p.role[i]) == q) tp[q].p.role[tp[q].p.roles++] = p.role[i];
+        const int rc = dtype == MAMBA_B200_F16 ? launch<__half, 2>(c, tp[q], pairs, st)
+                       : q >= 2                ? launch<__nv_bfloat16, 3>(c, tp[q], pairs, st)
+                                               : launch<__nv_bfloat16, 1>(c, tp[q], pairs, st);
         if (rc) return rc;
     }
     return MAMBA_B200_OK;
@@ -822,9 +870,9 @@ int linear_attention_tc_configure(Ctx* c) {
     using namespace la::tcl;
 #define MB200_LA(Th, TERMS)                                                                                                              \
     MB200_CUDA_CHECK(c, cudaFuncSetAttribute((const void*)walk_kernel<Th, TERMS, false>, cudaFuncAttributeMaxDynamicSharedMemorySize,     \
-                                             static_cast<int>(smem_bytes<TERMS>(2, 2, kMostZ<TERMS>))));                                                \
+                                             static_cast<int>(smem_bytes<TERMS>(2, 2, kTiles - kCopies<TERMS>))));                                                \
     MB200_CUDA_CHECK(c, cudaFuncSetAttribute((const void*)walk_kernel<Th, TERMS, true>, cudaFuncAttributeMaxDynamicSharedMemorySize,      \
-                                             static_cast<int>(smem_bytes<TERMS>(2, 2, kMostZ<TERMS>))));
+                                             static_cast<int>(smem_bytes<TERMS>(2, 2, kTiles - kCopies<TERMS>))));
     MB200_LA(__half, 2)
     MB200_LA(__nv_bfloat16, 1)
     MB200_LA(__nv_bfloat16, 3)
