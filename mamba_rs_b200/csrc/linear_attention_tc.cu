@@ -5,9 +5,10 @@
 // Beside HBM, which a chunk of 128 x 64 heads of 128 x 64 keeps busy for 4100 cycles an SM, its products take 1500 cycles of the
 // tensor pipe, so one block on an SM reaches HBM's rate if nothing waits for anything else: every part has warps of its own, and the
 // state, the only thing that is carried from chunk to chunk, stays in tensor memory,
-//   warp 0      asks for the tiles, as many chunks ahead as there are stages
-//   warp 1      issues X Y^T of the next chunk and P Z of this one
-//   warp 2      issues Y^T (w o Z) and X S, the chain from chunk to chunk
+//   warp 0      asks for the tiles (X and Y, Z), as many chunks ahead as there are stages
+//   warp 1      issues X Y^T, up to two chunks ahead
+//   warp 2      issues Y^T (w o Z), the chain from chunk to chunk
+//   warp 3      issues X S and P Z
 //   warps 4-7   make P from G, of every other chunk; it goes back to tensor memory and is read there as an operand
 //   warps 8-11  leave a 16-bit copy of S for X S, and in its place what is left of it after the chunk
 //   warps 12-15 join P Z and X S and write rows
@@ -35,8 +36,8 @@ using namespace mb200::tc;
 
 constexpr int kThreads = 768, kTile = 64;
 constexpr uint32_t kSub = kSwSub;  // a [128 x 64] sub-tile
-// Tensor memory: two buffers of G, whose left half P takes and whose right half P Z; two of X S; S and, in f16, the sum of a chunk's
-// second terms.
+// Tensor memory: two buffers of G, whose left half P takes and whose right half P Z (not folded); two of X S and, folded, P Z in one sum; S
+// and, in f16, the sum of a chunk's second terms.
 constexpr uint32_t cG = 0, cY1 = 64, cY2 = 256, cS = 384, cSlo = 448, kCols = 512;
 
 struct TcParams {
@@ -60,7 +61,7 @@ struct Small {
     float row_scale[2][128];
     float tile_scale[4];  // (a copy's is read until its rows are out, which is known of the chunk three before)
     float warp_max[2][4];
-    uint64_t full[4], empty[4], z_full[8], z_empty[8], g_full[2], p_full[2], y_full[2], x_full[2], y_empty[2], s_full[2], s_empty[2], w_full[8], d_full, max_full, drain[2];
+    uint64_t full[4], empty[4], z_full[8], z_empty[8], g_full[2], p_full[2], y_full[2], y_empty[2], s_full[2], s_empty[2], w_full[8], z_read[8], d_full, max_full, drain[3];
     uint32_t tmem;
     int dead;
 };
@@ -92,6 +93,17 @@ __device__ __forceinline__ bool look(uint64_t* bar, uint32_t parity) {
     asm volatile(
         "{\n\t.reg .pred p;\n\t"
         "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(ok)
+        : "r"(smem_u32(bar)), "r"(parity)
+        : "memory");
+    return ok != 0;
+}
+__device__ __forceinline__ bool free_now(uint64_t* bar, uint32_t parity) {  // (look() may sleep for a while)
+    uint32_t ok;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
         "selp.u32 %0, 1, 0, p;\n\t}"
         : "=r"(ok)
         : "r"(smem_u32(bar)), "r"(parity)
@@ -167,23 +179,23 @@ __global__ void __launch_bounds__(kThreads, 1) walk_kernel(const __grid_constant
     if (threadIdx.x == 0) {
         for (int i = 0; i < 4; ++i) {
             mbar_init(&sm->full[i], 1);
-            mbar_init(&sm->empty[i], STATE ? 1 : 2);
+            mbar_init(&sm->empty[i], STATE ? 1 : 3);
         }
         for (int i = 0; i < 8; ++i) {
             mbar_init(&sm->z_full[i], 1);
             mbar_init(&sm->z_empty[i], STATE ? 1 : 4);
             mbar_init(&sm->w_full[i], 128);
+            mbar_init(&sm->z_read[i], 1);
         }
         for (int i = 0; i < 2; ++i) {
             mbar_init(&sm->g_full[i], 1);
             mbar_init(&sm->p_full[i], 128);
             mbar_init(&sm->s_full[i], 128);
             mbar_init(&sm->s_empty[i], 1);
-            mbar_init(&sm->x_full[i], 1);
             mbar_init(&sm->y_full[i], 1);
             mbar_init(&sm->y_empty[i], 128);
-            mbar_init(&sm->drain[i], 1);
         }
+        for (int i = 0; i < 3; ++i) mbar_init(&sm->drain[i], 1);
         mbar_init(&sm->d_full, 1);
         mbar_init(&sm->max_full, 128);
         sm->dead = 0;
@@ -208,84 +220,78 @@ __global__ void __launch_bounds__(kThreads, 1) walk_kernel(const __grid_constant
     const uint32_t per_stage = stage >> 4;  // in descriptors
     constexpr uint32_t kStep = 32 >> 4, mStep = 2048 >> 4, sub = kSub >> 4;
 
-    if (warp == 0 || warp == 3) {
+    if (warp == 0) {
         if (lane == 0) {
-            // X and Y are free when the products of S are, Z only with the rows
-            const bool z = warp == 3;
-            const int hx = h / r.x.group, hy = h / r.y.group, hz = h / r.z.group, depth = z ? zs : stages;
-            uint64_t* full = z ? sm->z_full : sm->full;
-            uint64_t* empty = z ? sm->z_empty : sm->empty;
-            int asked = 0;
-            for (int i = 0, st = 0, turn = 0; i < n; ++i) {
-                const int t0 = start(i);
-                if (turn && !wait(&empty[st], (turn - 1) & 1, sm, p.status)) break;
-                if (z) {
-                    mbar_expect_tx(&full[st], kSub);
-                    tma_load_4d(smem + kZ + st * kSub, &tp.z[w.role], &full[st], c0, hz, t0, b);
-                } else {
+            // X and Y are free when the products of S are, Z only with the rows: neither waits for the other's turn
+            const int hx = h / r.x.group, hy = h / r.y.group, hz = h / r.z.group;
+            int i = 0, st = 0, turn = 0, iz = 0, sz = 0, turn_z = 0, polls = 0;
+            while (i < n || iz < n) {
+                bool did = false;
+                if (i < n && (turn == 0 || free_now(&sm->empty[st], (turn - 1) & 1))) {
+                    const int t0 = start(i);
                     unsigned char* at = smem + st * stage;
-                    mbar_expect_tx(&full[st], (STATE ? 1 : 2) * na * kSub);
+                    mbar_expect_tx(&sm->full[st], (STATE ? 1 : 2) * na * kSub);
                     for (int s = 0; s < na; ++s) {
-                        if (!STATE) tma_load_4d(at + s * kSub, &tp.x[w.role], &full[st], 64 * s, hx, t0, b);
-                        tma_load_4d(at + oY + s * kSub, &tp.y[w.role], &full[st], 64 * s, hy, t0, b);
+                        if (!STATE) tma_load_4d(at + s * kSub, &tp.x[w.role], &sm->full[st], 64 * s, hx, t0, b);
+                        tma_load_4d(at + oY + s * kSub, &tp.y[w.role], &sm->full[st], 64 * s, hy, t0, b);
                     }
-                }
-                asked = i + 1;
-                if (++st == depth) {
-                    st = 0;
-                    ++turn;
-                }
-            }
-            // nothing may be in flight when the block ends (where all went well, it has long landed)
-            for (int i = max(0, asked - depth); i < asked; ++i) mbar_wait(&full[i % depth], (i / depth) & 1, p.status);
-        }
-    } else if (warp == 1) {
-        // ---- X Y^T and P Z ----
-        if (!STATE) {
-            const uint32_t idG = instr_desc(fmt, 0, 0, 128), idY = instr_desc(fmt, 0, 1, 64);
-            // descriptors of stage 0; a step along K is a constant more (m3_tc.cuh), a stage `per_stage`
-            const uint64_t xk = desc_sw_k(sbase, 0), yk = desc_sw_k(sbase + oY, 0), zm = desc_sw_mn(sbase + kZ, 0);
-            bool ok = true;
-            int st = 0, turn = 0, sz = 0, turn_z = 0;  // of the next G; of P Z
-            for (int i = -1; i < n; ++i) {
-                const uint32_t at = st * per_stage;
-                if (i + 1 < n) {
-                    // G of chunk i + 1; the rows of chunk i - 1 have left the buffer that it takes
-                    if (i > 0) ok = wait_warp(&sm->y_empty[(i - 1) & 1], ((i - 1) >> 1) & 1, sm, p.status);
-                    if (ok) ok = wait_warp(&sm->full[st], turn & 1, sm, p.status);
-                    if (!ok) break;
-                    fence_after();
-                    const uint32_t d = tmem + cG + ((i + 1) & 1) * 128;
-                    if (elect_one()) {
-#pragma unroll
-                        for (int k = 0; k < 4; ++k) mma(d, xk + at + k * kStep, yk + at + k * kStep, idG, k > 0);
-                        if (na == 2) {
-#pragma unroll
-                            for (int k = 0; k < 4; ++k) mma(d, xk + at + sub + k * kStep, yk + at + sub + k * kStep, idG, true);
-                        }
-                        commit(&sm->g_full[(i + 1) & 1]);
-                        commit(&sm->empty[st]);
+                    ++i;
+                    if (++st == stages) {
+                        st = 0;
+                        ++turn;
                     }
-                    __syncwarp();
+                    did = true;
                 }
-                if (i >= 0) {
-                    // P Z of chunk i
-                    ok = wait_warp(fold ? &sm->w_full[sz] : &sm->z_full[sz], turn_z & 1, sm, p.status);
-                    if (ok) ok = wait_warp(&sm->p_full[i & 1], (i >> 1) & 1, sm, p.status);
-                    if (!ok) break;
-                    fence_after();
-                    const uint32_t g = tmem + cG + (i & 1) * 128, z = sz * sub;
-                    if (elect_one()) {
-#pragma unroll
-                        for (int k = 0; k < kChunk / 16; ++k) mma_ta(g + cY1, g + k * 8, zm + z + k * mStep, idY, k > 0);
-                        commit(&sm->y_full[i & 1]);
-                    }
-                    __syncwarp();
+                if (iz < n && (turn_z == 0 || free_now(&sm->z_empty[sz], (turn_z - 1) & 1))) {
+                    mbar_expect_tx(&sm->z_full[sz], kSub);
+                    tma_load_4d(smem + kZ + sz * kSub, &tp.z[w.role], &sm->z_full[sz], c0, hz, start(iz), b);
+                    ++iz;
                     if (++sz == zs) {
                         sz = 0;
                         ++turn_z;
                     }
+                    did = true;
                 }
+                polls = did ? 0 : polls + 1;
+                if (!did) {
+                    if (polls > kMbarMaxPolls || ((polls & 15) == 15 && *reinterpret_cast<volatile int*>(&sm->dead))) {
+                        *reinterpret_cast<volatile int*>(&sm->dead) = 1;
+                        atomicCAS(p.status, kStatusOk, kStatusBarrierTimeout);
+                        break;
+                    }
+                    __nanosleep(32);
+                }
+            }
+            // nothing may be in flight when the block ends (where all went well, it has long landed)
+            for (int k = max(0, i - stages); k < i; ++k) mbar_wait(&sm->full[k % stages], (k / stages) & 1, p.status);
+            for (int k = max(0, iz - zs); k < iz; ++k) mbar_wait(&sm->z_full[k % zs], (k / zs) & 1, p.status);
+        }
+    } else if (warp == 1) {
+        // ---- X Y^T ----
+        if (!STATE) {
+            const uint32_t idG = instr_desc(fmt, 0, 0, 128);
+            // descriptors of stage 0; a step along K is a constant more (m3_tc.cuh), a stage `per_stage`
+            const uint64_t xk = desc_sw_k(sbase, 0), yk = desc_sw_k(sbase + oY, 0);
+            bool ok = true;
+            for (int i = 0, st = 0, turn = 0; i < n; ++i) {
+                const uint32_t at = st * per_stage;
+                // the buffer's P has been read (not folded: and P Z, beside it, by the rows)
+                if (i > 1) ok = wait_warp(fold ? &sm->y_full[i & 1] : &sm->y_empty[i & 1], ((i >> 1) - 1) & 1, sm, p.status);
+                if (ok) ok = wait_warp(&sm->full[st], turn & 1, sm, p.status);
+                if (!ok) break;
+                fence_after();
+                const uint32_t d = tmem + cG + (i & 1) * 128;
+                if (elect_one()) {
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) mma(d, xk + at + k * kStep, yk + at + k * kStep, idG, k > 0);
+                    if (na == 2) {
+#pragma unroll
+                        for (int k = 0; k < 4; ++k) mma(d, xk + at + sub + k * kStep, yk + at + sub + k * kStep, idG, true);
+                    }
+                    commit(&sm->g_full[i & 1]);
+                    commit(&sm->empty[st]);
+                }
+                __syncwarp();
                 if (++st == stages) {
                     st = 0;
                     ++turn;
@@ -298,60 +304,39 @@ __global__ void __launch_bounds__(kThreads, 1) walk_kernel(const __grid_constant
             }
         }
     } else if (warp == 2) {
-        // ---- Y^T (w o Z) and X S ----
-        const uint32_t idY = instr_desc(fmt, 0, 1, 64), idD = instr_desc(fmt, 1, 1, 64);
-        const uint64_t xk = desc_sw_k(sbase, 0), ym = desc_sw_mn(sbase + oY, 0);
-        const uint64_t zm = desc_sw_mn(sbase + kZ, 0), wm = desc_sw_mn(sbase + kW, 0), sc = desc_sw_mn(sbase + kS, 0);
+        // ---- Y^T (w o Z) ----
+        const uint32_t idD = instr_desc(fmt, 1, 1, 64);
+        const uint64_t ym = desc_sw_mn(sbase + oY, 0), zm = desc_sw_mn(sbase + kZ, 0), wm = desc_sw_mn(sbase + kW, 0);
         bool ok = true;
         int st = 0, turn = 0, sz = 0, turn_z = 0;
         for (int i = 0; i < n; ++i) {
             const uint32_t at = st * per_stage;
-            const bool reads = i > 0 || enters;
+            const bool reads = i > 0 || enters, adds = leaves || i + 1 < n;
             const int u = enters ? i : i - 1;  // number of the copy of S
-            ok = wait_warp(&sm->full[st], turn & 1, sm, p.status);
-            // a copy of S, and what is left of S in its place
-            if (ok && reads) ok = wait_warp(&sm->s_full[STATE ? 0 : u % SB], (STATE ? u : u / SB) & 1, sm, p.status);
-            if (!ok) break;
-            if (leaves || i + 1 < n) {
-                ok = wait_warp(&sm->w_full[sz], turn_z & 1, sm, p.status);
+            if (adds) {
+                ok = wait_warp(&sm->full[st], turn & 1, sm, p.status);
+                if (ok) ok = wait_warp(&sm->w_full[sz], turn_z & 1, sm, p.status);
+                // (with the copy of S, what is left of S is in its place)
+                if (ok && reads) ok = wait_warp(&sm->s_full[STATE ? 0 : u % SB], (STATE ? u : u / SB) & 1, sm, p.status);
                 if (!ok) break;
                 fence_after();
-                // first term; the others
-                const uint64_t w0 = fold ? zm + sz * sub : wm, w1 = fold ? wm - sub : wm;
-                if (elect_one()) {
+            }
+            // first term; the others
+            const uint64_t w0 = fold ? zm + sz * sub : wm, w1 = fold ? wm - sub : wm;
+            if (elect_one()) {
+                if (adds) {
 #pragma unroll
                     for (int t = 0; t < TERMS; ++t) {
                         const bool own = F16 && t == 1;  // (the second f16 term is summed apart)
 #pragma unroll
                         for (int k = 0; k < kChunk / 16; ++k)
-                            mma(tmem + (own ? cSlo : cS), ym + at + k * mStep, (t == 0 ? w0 : w1 + t * sub) + k * mStep, idD, own ? k > 0 : reads || k > 0 || t > 0);
+                            mma(tmem + (own ? cSlo : cS), ym + at + k * mStep, (t == 0 ? w0 : w1 + t * sub) + k * mStep, idD,
+                                own ? k > 0 : reads || k > 0 || t > 0);
                     }
                     commit(&sm->d_full);
                 }
-                __syncwarp();
-            }
-            if (!STATE) {
-                if (i > 1) ok = wait_warp(&sm->y_empty[i & 1], ((i >> 1) - 1) & 1, sm, p.status);
-                if (!ok) break;
-                fence_after();
-                const uint32_t d = tmem + cY2 + (i & 1) * 64, copy = (u % SB) * sub;
-                if (elect_one()) {
-                    if (reads) {
-#pragma unroll
-                        for (int k = 0; k < 4; ++k) mma(d, xk + at + k * kStep, sc + copy + k * mStep, idY, k > 0);
-                        if (na == 2) {
-#pragma unroll
-                            for (int k = 0; k < 4; ++k) mma(d, xk + at + sub + k * kStep, sc + copy + (4 + k) * mStep, idY, true);
-                        }
-                        commit(&sm->s_empty[u % SB]);
-                    }
-                    commit(&sm->x_full[i & 1]);
-                }
-                __syncwarp();
-            }
-            if (elect_one()) {
                 commit(&sm->empty[st]);
-                if (STATE) commit(&sm->z_empty[sz]);
+                commit(STATE ? &sm->z_empty[sz] : &sm->z_read[sz]);
             }
             __syncwarp();
             if (++st == stages) {
@@ -367,6 +352,62 @@ __global__ void __launch_bounds__(kThreads, 1) walk_kernel(const __grid_constant
             if (elect_one()) commit(&sm->drain[1]);
             __syncwarp();
             mbar_wait(&sm->drain[1], 0, p.status);
+        }
+    } else if (warp == 3) {
+        // ---- X S and P Z ----
+        if (!STATE) {
+            const uint32_t idY = instr_desc(fmt, 0, 1, 64);
+            const uint64_t xk = desc_sw_k(sbase, 0), sc = desc_sw_mn(sbase + kS, 0), zm = desc_sw_mn(sbase + kZ, 0);
+            bool ok = true;
+            int st = 0, turn = 0, sz = 0, turn_z = 0;
+            for (int i = 0; i < n; ++i) {
+                const uint32_t at = st * per_stage, d = tmem + cY2 + (i & 1) * 64;
+                const bool reads = i > 0 || enters;
+                const int u = enters ? i : i - 1;  // number of the copy of S
+                if (i > 1) ok = wait_warp(&sm->y_empty[i & 1], ((i >> 1) - 1) & 1, sm, p.status);
+                if (ok) ok = wait_warp(&sm->full[st], turn & 1, sm, p.status);
+                if (ok && reads) ok = wait_warp(&sm->s_full[u % SB], (u / SB) & 1, sm, p.status);
+                if (!ok) break;
+                fence_after();
+                if (elect_one()) {
+                    if (reads) {
+                        const uint32_t copy = (u % SB) * sub;
+#pragma unroll
+                        for (int k = 0; k < 4; ++k) mma(d, xk + at + k * kStep, sc + copy + k * mStep, idY, k > 0);
+                        if (na == 2) {
+#pragma unroll
+                            for (int k = 0; k < 4; ++k) mma(d, xk + at + sub + k * kStep, sc + copy + (4 + k) * mStep, idY, true);
+                        }
+                        commit(&sm->s_empty[u % SB]);
+                    }
+                    commit(&sm->empty[st]);
+                }
+                __syncwarp();
+                ok = wait_warp(fold ? &sm->w_full[sz] : &sm->z_full[sz], turn_z & 1, sm, p.status);
+                if (ok) ok = wait_warp(&sm->p_full[i & 1], (i >> 1) & 1, sm, p.status);
+                if (!ok) break;
+                fence_after();
+                const uint32_t g = tmem + cG + (i & 1) * 128, z = sz * sub, y = fold ? d : g + cY1;
+                if (elect_one()) {
+#pragma unroll
+                    for (int k = 0; k < kChunk / 16; ++k) mma_ta(y, g + k * 8, zm + z + k * mStep, idY, k > 0 || (fold && reads));
+                    commit(&sm->y_full[i & 1]);
+                }
+                __syncwarp();
+                if (++st == stages) {
+                    st = 0;
+                    ++turn;
+                }
+                if (++sz == zs) {
+                    sz = 0;
+                    ++turn_z;
+                }
+            }
+            if (!ok) {
+                if (elect_one()) commit(&sm->drain[2]);
+                __syncwarp();
+                mbar_wait(&sm->drain[2], 0, p.status);
+            }
         }
     } else if (role == 1 || role == 5) {
         // ---- P ----
@@ -578,6 +619,17 @@ __global__ void __launch_bounds__(kThreads, 1) walk_kernel(const __grid_constant
                     float v[32];
                     if (F16 && STATE && i > 0) read(s, v);
                     else tmem_ld32(lanes + cS + 32 * s, v);  // (f16: joined above)
+                    // (folded: rows take the factor that w o Z lacks, and with it X S is wanted of what is left of S)
+                    auto decay = [&]() {
+#pragma unroll
+                        for (int c = 0; c < 32; c += 2) {
+                            float2 x = make_float2(v[c], v[c + 1]);
+                            x = TERMS == 1 ? mul2(x, splat2(f.hi)) : fma2(x, splat2(f.hi), mul2(x, splat2(f.lo)));
+                            v[c] = x.x;
+                            v[c + 1] = x.y;
+                        }
+                    };
+                    if (fold) decay();
                     if (!STATE) {
 #pragma unroll
                         for (int j = 0; j < 4; ++j) {
@@ -590,16 +642,8 @@ __global__ void __launch_bounds__(kThreads, 1) walk_kernel(const __grid_constant
                             *reinterpret_cast<uint4*>(copy + sw_chunk(row, 4 * s + j)) = make_uint4(o[0], o[1], o[2], o[3]);
                         }
                     }
-                    if (adds) {
-#pragma unroll
-                        for (int c = 0; c < 32; c += 2) {
-                            float2 x = make_float2(v[c], v[c + 1]);
-                            x = TERMS == 1 ? mul2(x, splat2(f.hi)) : fma2(x, splat2(f.hi), mul2(x, splat2(f.lo)));
-                            v[c] = x.x;
-                            v[c + 1] = x.y;
-                        }
-                        tmem_st32(lanes + cS + 32 * s, v);
-                    }
+                    if (!fold) decay();
+                    if (adds) tmem_st32(lanes + cS + 32 * s, v);
                 }
                 if (!STATE) fence_proxy_async();
                 fence_before();
@@ -640,8 +684,9 @@ __global__ void __launch_bounds__(kThreads, 1) walk_kernel(const __grid_constant
         const float y_whole = fold ? decay_at(-l2, back ? row : kChunk - 1 - row) * r.alpha_z : 1.0f;
         const int nc = min(kTile, W - c0);
         const bool tiles = tp.out_map[w.role];
-        for (int i = 0, sz = 0; i < n; ++i) {
-            if (!wait_warp(&sm->x_full[i & 1], (i >> 1) & 1, sm, p.status)) break;
+        for (int i = 0, sz = 0, turn_z = 0; i < n; ++i) {
+            // (Z's place, where the rows go, is read by the products of S too)
+            if (!wait_warp(&sm->z_read[sz], turn_z & 1, sm, p.status)) break;
             if (!wait_warp(&sm->y_full[i & 1], (i >> 1) & 1, sm, p.status)) break;
             fence_after();
             const int t0 = start(i), rows = min(kChunk, p.T - t0);
@@ -649,21 +694,20 @@ __global__ void __launch_bounds__(kThreads, 1) walk_kernel(const __grid_constant
             const int late = i == 0 ? late0 : 0;
             float f = x_whole, f1 = y_whole;
             if (fold && !back && rows != kChunk) f1 = decay_at(-l2, max(rows - 1 - row, 0)) * r.alpha_z;
-            if (late || (back && rows != kChunk)) f = decay_at(l2, back ? rows - row - late : row + 1 - late) * r.alpha_x;
+            if (!fold && (late || (back && rows != kChunk))) f = decay_at(l2, back ? rows - row - late : row + 1 - late) * r.alpha_x;
             if (F16) {
                 f1 = sm->row_scale[i & 1][row];
                 if (reads) f *= sm->tile_scale[(enters ? i : i - 1) & 3];
             }
-            const uint32_t y1 = lanes + cG + (i & 1) * 128 + cY1, y2 = lanes + cY2 + (i & 1) * 64;
+            const uint32_t y2 = lanes + cY2 + (i & 1) * 64, y1 = fold ? y2 : lanes + cG + (i & 1) * 128 + cY1;
             // 32 columns of out
             auto read = [&](int s, float* y) {
-                float x[32];
-                if (reads) {
+                if (!fold && reads) {
+                    float x[32];
                     tmem_ld32x2(y1 + 32 * s, y, y2 + 32 * s, x);
 #pragma unroll
                     for (int c = 0; c < 32; c += 2) {
-                        float2 o = make_float2(y[c], y[c + 1]);
-                        o = mul2(o, splat2(f1));
+                        float2 o = mul2(make_float2(y[c], y[c + 1]), splat2(f1));
                         o = fma2(make_float2(x[c], x[c + 1]), splat2(f), o);
                         y[c] = o.x;
                         y[c + 1] = o.y;
@@ -671,7 +715,11 @@ __global__ void __launch_bounds__(kThreads, 1) walk_kernel(const __grid_constant
                 } else {
                     tmem_ld32(y1 + 32 * s, y);
 #pragma unroll
-                    for (int c = 0; c < 32; ++c) y[c] *= f1;
+                    for (int c = 0; c < 32; c += 2) {
+                        const float2 o = mul2(make_float2(y[c], y[c + 1]), splat2(f1));
+                        y[c] = o.x;
+                        y[c + 1] = o.y;
+                    }
                 }
             };
             if (tiles) {
@@ -717,7 +765,10 @@ __global__ void __launch_bounds__(kThreads, 1) walk_kernel(const __grid_constant
                 mbar_arrive(&sm->y_empty[i & 1]);
             }
             if (lane == 0) mbar_arrive(&sm->z_empty[sz]);
-            if (++sz == zs) sz = 0;
+            if (++sz == zs) {
+                sz = 0;
+                ++turn_z;
+            }
         }
     } else if (role == 4) {
         // ---- w o Z ----
