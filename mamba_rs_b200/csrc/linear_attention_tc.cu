@@ -745,7 +745,9 @@ __global__ void __launch_bounds__(kThreads, 1) walk_kernel(const __grid_constant
                 if (lane == 0) {
                     if (t0 + (row & ~31) < p.T) tma_store_4d(&tp.out[w.role], at + (row & ~31) * 128, c0, h, t0 + (row & ~31), b);
                     tma_commit();
-                    tma_wait_read0();
+                    // (the last chunk's rows have been read from their place meanwhile: nobody waits for this chunk's)
+                    asm volatile("cp.async.bulk.wait_group.read 1;" ::: "memory");
+                    if (i > 0) mbar_arrive(&sm->z_empty[sz == 0 ? zs - 1 : sz - 1]);
                 }
             } else {
                 const long long at = b * r.ob + static_cast<long long>(t0 + row) * r.ot + h * r.oh + c0;
@@ -764,12 +766,13 @@ __global__ void __launch_bounds__(kThreads, 1) walk_kernel(const __grid_constant
                 fence_before();
                 mbar_arrive(&sm->y_empty[i & 1]);
             }
-            if (lane == 0) mbar_arrive(&sm->z_empty[sz]);
+            if (!tiles && lane == 0) mbar_arrive(&sm->z_empty[sz]);
             if (++sz == zs) {
                 sz = 0;
                 ++turn_z;
             }
         }
+        if (tiles && lane == 0) tma_wait_read0();
     } else if (role == 4) {
         // ---- w o Z ----
         const float w_whole = decay_at(l2, back ? row : kChunk - 1 - row) * r.alpha_s;
