@@ -146,14 +146,13 @@ __device__ __forceinline__ float scale_to(float m, float* back) {
     return __uint_as_float(static_cast<uint32_t>(127 - d) << 23);
 }
 
-template <typename Th, int TERMS, bool STATE>
-__global__ void __launch_bounds__(kThreads, 1) walk_kernel(const __grid_constant__ TcParams tp) {
+// (`fold` is known to the compiler: code that is not taken lies elsewhere, and what is fits the instruction cache better)
+template <typename Th, int TERMS, bool STATE, bool fold>
+__device__ __forceinline__ void walk(const TcParams& tp, unsigned char* smem, const Place& w, const float ld) {
     constexpr bool F16 = std::is_same<Th, __half>::value;
     constexpr int SB = kCopies<TERMS>;
     constexpr uint32_t fmt = F16 ? 0u : 1u;
-    extern __shared__ __align__(1024) unsigned char smem[];
     const Params& p = tp.p;
-    const Place w = place(p, blockIdx.x, STATE ? p.segments - 1 : p.segments);
     const Role& r = p.role[w.role];
     const int A = r.A, W = r.W, na = (A + 63) >> 6, c0 = w.tile * kTile, stages = tp.stages;
     const uint32_t stage = 2 * tp.na * kSub, oY = tp.na * kSub, kZ = stages * stage, kS = kZ + tp.z_tiles * kSub;
@@ -162,10 +161,7 @@ __global__ void __launch_bounds__(kThreads, 1) walk_kernel(const __grid_constant
     const int b = static_cast<int>(w.pair / p.H), h = static_cast<int>(w.pair - static_cast<long long>(b) * p.H);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, role = warp >> 2, row = threadIdx.x & 127;
     const bool back = r.backwards;
-    const float ld = p.decay[h], l2 = ld * kLog2e;
-    // `fold`: w o Z takes Z's place and P is G with its future cut off; what is missing, l^{row} up to a constant, is one factor a row of the
-    // result.  Not where l^{-127} leaves the numbers that 32 bits hold with room to spare, nor in f16.
-    const bool fold = !F16 && ld <= 0.0f && ld * (kChunk - 1) >= -kSlow;
+    const float l2 = ld * kLog2e;
     const int zs = tp.z_tiles - TERMS + (fold ? 1 : 0);  // stages of Z
     const uint32_t kW = kZ + zs * kSub;
     // chunks of this segment, numbered as they are walked
@@ -820,6 +816,22 @@ __global__ void __launch_bounds__(kThreads, 1) walk_kernel(const __grid_constant
     fence_after();
     __syncwarp();
     if (warp == 1) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kCols) : "memory");
+}
+
+template <typename Th, int TERMS, bool STATE>
+__global__ void __launch_bounds__(kThreads, 1) walk_kernel(const __grid_constant__ TcParams tp) {
+    extern __shared__ __align__(1024) unsigned char smem[];
+    const Place w = place(tp.p, blockIdx.x, STATE ? tp.p.segments - 1 : tp.p.segments);
+    const float ld = tp.p.decay[w.pair % tp.p.H];
+    // `fold`: w o Z takes Z's place and P is G with its future cut off; what is missing, l^{row} up to a constant, is one factor a row of the
+    // result.  Not where l^{-127} leaves the numbers that 32 bits hold with room to spare, nor in f16.
+    if constexpr (!std::is_same<Th, __half>::value) {
+        if (ld <= 0.0f && ld * (kChunk - 1) >= -kSlow) {
+            walk<Th, TERMS, STATE, true>(tp, smem, w, ld);
+            return;
+        }
+    }
+    walk<Th, TERMS, STATE, false>(tp, smem, w, ld);
 }
 
 typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*,
