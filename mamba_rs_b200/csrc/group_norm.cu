@@ -46,10 +46,10 @@ __device__ __forceinline__ void store(T* p, const float* f) {
     *reinterpret_cast<Vec<T, VEC>*>(p) = v;
 }
 
-// f32 storage keeps exact forms; 16-bit results are rounded far above the fast ones' error (2^-20)
+// f32 storage keeps expf's form; 16-bit results are rounded far above the fast one's error (2^-20)
 template <typename T>
 __device__ __forceinline__ float sigmoid(float v) {
-    if (sizeof(T) == 4) return 1.0f / (1.0f + expf(-v));
+    if (sizeof(T) == 4) return rcp(1.0f + expf(-v));  // (expf to 1 ulp, the reciprocal too)
     return sigmoidf_fast(v);
 }
 // act(v), and its slope
@@ -490,7 +490,7 @@ struct Cover {
     int rows0, rows1, rp, r, gi, g, col, first, groups, blk, sub;
     bool on;
 };
-template <int VEC>
+template <int VEC, int NT = kThreads>
 __device__ __forceinline__ Cover cover(const Params& p) {
     Cover c;
     const mamba_b200_group_norm_args& a = p.a;
@@ -498,15 +498,15 @@ __device__ __forceinline__ Cover cover(const Params& p) {
     c.rows0 = c.blk * p.block_rows;
     c.rows1 = min(a.S, c.rows0 + p.block_rows);
     const int vecs = p.vecs;  // vectors of a group
-    const int wide = p.sub > 1 ? kThreads : p.groups * vecs;
-    c.rp = kThreads / wide;
+    const int wide = p.sub > 1 ? NT : p.groups * vecs;
+    c.rp = NT / wide;
     c.r = threadIdx.x / wide;
     const int at = threadIdx.x - c.r * wide;
     c.sub = p.sub > 1 ? blockIdx.y % p.sub : 0;
     c.first = p.sub > 1 ? blockIdx.y / p.sub : blockIdx.y * p.groups;
     c.groups = p.sub > 1 ? 1 : min(p.groups, a.G - c.first);
     c.gi = p.sub > 1 ? 0 : at / vecs;
-    const int k = p.sub > 1 ? c.sub * kThreads + at : at - c.gi * vecs;
+    const int k = p.sub > 1 ? c.sub * NT + at : at - c.gi * vecs;
     c.g = c.first + c.gi;
     c.col = c.g * p.per + k * VEC;
     c.on = c.r < c.rp && c.g < a.G && k < vecs;
@@ -800,13 +800,15 @@ __global__ void __launch_bounds__(kThreads) spread_kernel(const Params p) {
 
 // The same in one kernel, where a sample's rows of a block's channels fit shared memory: every element is read once.  A thread keeps
 // its own vectors there, so that barriers are for sums alone.
+constexpr int kSlabThreads = 512;
+
 template <typename T, int VEC>
 __device__ __forceinline__ float group_sum(const Params& p, const Cover& c, float v, float* per_thread, float* per_group) {
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, vecs = p.vecs, wide = p.groups * p.vecs;
     __syncthreads();
     per_thread[threadIdx.x] = v;
     __syncthreads();
-    for (int gi = warp; gi < c.groups; gi += kThreads / 32) {
+    for (int gi = warp; gi < c.groups; gi += kSlabThreads / 32) {
         float t = 0.0f;
         for (int i = lane; i < c.rp * vecs; i += 32) t += per_thread[(i / vecs) * wide + gi * vecs + i % vecs];
         t = sum_lanes(t, 32);
@@ -817,17 +819,17 @@ __device__ __forceinline__ float group_sum(const Params& p, const Cover& c, floa
 }
 
 template <typename T, int VEC, bool BWD>
-__global__ void __launch_bounds__(kThreads) slab_kernel(const Params p) {
+__global__ void __launch_bounds__(kSlabThreads) slab_kernel(const Params p) {
     using V = Vec<T, VEC>;
     extern __shared__ __align__(16) unsigned char slab[];
-    __shared__ float per_thread[kThreads], per_group[kThreads];
-    __shared__ float sw[BWD ? kThreads * VEC : 1], sb[BWD ? kThreads * VEC : 1];
+    __shared__ float per_thread[kSlabThreads], per_group[kSlabThreads];
+    __shared__ float sw[BWD ? kSlabThreads * VEC : 1], sb[BWD ? kSlabThreads * VEC : 1];
     const mamba_b200_group_norm_args& a = p.a;
-    const Cover c = cover<VEC>(p);
+    const Cover c = cover<VEC, kSlabThreads>(p);
     const int turns = (a.S + c.rp - 1) / c.rp;
     V* sx = reinterpret_cast<V*>(slab) + threadIdx.x;
-    V* sd = sx + (BWD ? static_cast<size_t>(turns) * kThreads : 0);
-    V* sz = sd + static_cast<size_t>(turns) * kThreads;
+    V* sd = sx + (BWD ? static_cast<size_t>(turns) * kSlabThreads : 0);
+    V* sz = sd + static_cast<size_t>(turns) * kSlabThreads;
     const bool gate = a.z != nullptr;
     const float inv = 1.0f / (static_cast<float>(p.per) * a.S);
     const long long NG = static_cast<long long>(a.N) * a.G;
@@ -840,7 +842,7 @@ __global__ void __launch_bounds__(kThreads) slab_kernel(const Params p) {
     }
     for (int ns = blockIdx.x; ns < a.N; ns += p.side) {
         const long long row0 = static_cast<long long>(ns) * a.S;
-        constexpr int U = 8;
+        constexpr int U = 4;
         float s1 = 0.0f, s2 = 0.0f;
         float mean = 0.0f, rstd = 0.0f;
         if (BWD && c.on) {
@@ -861,9 +863,9 @@ __global__ void __launch_bounds__(kThreads) slab_kernel(const Params p) {
 #pragma unroll
                 for (int u = 0; u < U; ++u)
                     if (s + u * c.rp < a.S) {
-                        sx[(k + u) * kThreads] = v[u];
-                        if (BWD) sd[(k + u) * kThreads] = d[u % (BWD ? U : 1)];
-                        if (gate) sz[(k + u) * kThreads] = g[u];
+                        sx[(k + u) * kSlabThreads] = v[u];
+                        if (BWD) sd[(k + u) * kSlabThreads] = d[u % (BWD ? U : 1)];
+                        if (gate) sz[(k + u) * kSlabThreads] = g[u];
                         if (!BWD) {
 #pragma unroll
                             for (int e = 0; e < VEC; ++e) s1 += to_f(v[u].v[e]);
@@ -873,14 +875,22 @@ __global__ void __launch_bounds__(kThreads) slab_kernel(const Params p) {
         }
         if constexpr (!BWD) {
             mean = group_sum<T, VEC>(p, c, s1, per_thread, per_group) * inv;
+            // deviations from that mean, and what they say it is off by: a thread's sum of values far from zero loses digits
+            s1 = 0.0f;
             if (c.on)
                 for (int s = c.r, k = 0; s < a.S; s += c.rp, ++k) {
                     float x[VEC];
-                    widen(sx[k * kThreads], x);
+                    widen(sx[k * kSlabThreads], x);
 #pragma unroll
-                    for (int e = 0; e < VEC; ++e) s2 = fmaf(x[e] - mean, x[e] - mean, s2);
+                    for (int e = 0; e < VEC; ++e) {
+                        const float d = x[e] - mean;
+                        s1 += d;
+                        s2 = fmaf(d, d, s2);
+                    }
                 }
-            rstd = 1.0f / sqrtf(group_sum<T, VEC>(p, c, s2, per_thread, per_group) * inv + a.eps);
+            const float off = group_sum<T, VEC>(p, c, s1, per_thread, per_group) * inv;
+            mean += off;
+            rstd = rsqrtf(fmaxf(fmaf(-off, off, group_sum<T, VEC>(p, c, s2, per_thread, per_group) * inv), 0.0f) + a.eps);
             if (c.on && a.stats && c.r == 0 && c.col == c.g * p.per) {
                 a.stats[static_cast<long long>(ns) * a.G + c.g] = mean;
                 a.stats[NG + static_cast<long long>(ns) * a.G + c.g] = rstd;
@@ -888,8 +898,8 @@ __global__ void __launch_bounds__(kThreads) slab_kernel(const Params p) {
             if (c.on)
                 for (int s = c.r, k = 0; s < a.S; s += c.rp, ++k) {
                     float x[VEC], z[VEC];
-                    widen(sx[k * kThreads], x);
-                    if (gate) widen(sz[k * kThreads], z);
+                    widen(sx[k * kSlabThreads], x);
+                    if (gate) widen(sz[k * kSlabThreads], z);
 #pragma unroll
                     for (int e = 0; e < VEC; ++e) {
                         x[e] = act<T>(a.activation, fmaf((x[e] - mean) * rstd, w[e], bias[e]));
@@ -904,9 +914,9 @@ __global__ void __launch_bounds__(kThreads) slab_kernel(const Params p) {
             if (c.on)
                 for (int s = c.r, k = 0; s < a.S; s += c.rp, ++k) {
                     float x[VEC], z[VEC], dy[VEC], dz;
-                    widen(sx[k * kThreads], x);
-                    widen(sd[k * kThreads], dy);
-                    if (gate) widen(sz[k * kThreads], z);
+                    widen(sx[k * kSlabThreads], x);
+                    widen(sd[k * kSlabThreads], dy);
+                    if (gate) widen(sz[k * kSlabThreads], z);
 #pragma unroll
                     for (int e = 0; e < VEC; ++e) {
                         const float xh = (x[e] - mean) * rstd;
@@ -927,9 +937,9 @@ __global__ void __launch_bounds__(kThreads) slab_kernel(const Params p) {
             if (c.on)
                 for (int s = c.r, k = 0; s < a.S; s += c.rp, ++k) {
                     float x[VEC], z[VEC], dy[VEC];
-                    widen(sx[k * kThreads], x);
-                    widen(sd[k * kThreads], dy);
-                    if (gate) widen(sz[k * kThreads], z);
+                    widen(sx[k * kSlabThreads], x);
+                    widen(sd[k * kSlabThreads], dy);
+                    if (gate) widen(sz[k * kSlabThreads], z);
 #pragma unroll
                     for (int e = 0; e < VEC; ++e) {
                         const float xh = (x[e] - mean) * rstd;
@@ -945,8 +955,8 @@ __global__ void __launch_bounds__(kThreads) slab_kernel(const Params p) {
         const int wide = p.groups * p.vecs;
 #pragma unroll
         for (int e = 0; e < VEC; ++e) {
-            sw[e * kThreads + threadIdx.x] = all_w[e];
-            sb[e * kThreads + threadIdx.x] = all_b[e];
+            sw[e * kSlabThreads + threadIdx.x] = all_w[e];
+            sb[e * kSlabThreads + threadIdx.x] = all_b[e];
         }
         __syncthreads();
         if (c.r == 0 && c.on) {
@@ -956,8 +966,8 @@ __global__ void __launch_bounds__(kThreads) slab_kernel(const Params p) {
             for (int e = 0; e < VEC; ++e) {
                 float tw = all_w[e], tb = all_b[e];
                 for (int k = 1; k < c.rp; ++k) {
-                    tw += sw[e * kThreads + k * wide + threadIdx.x];
-                    tb += sb[e * kThreads + k * wide + threadIdx.x];
+                    tw += sw[e * kSlabThreads + k * wide + threadIdx.x];
+                    tb += sb[e * kSlabThreads + k * wide + threadIdx.x];
                 }
                 out_w[e] = tw;
                 out_b[e] = tb;
@@ -1013,13 +1023,13 @@ inline Room room(int N, int S, int C, int G, int backward) {
 
 // One kernel for a sample: the groups of a block (into p.groups) and its shared memory, or 0 where two kernels are better.  A block's
 // piece of a row is at least 64 bytes where there are groups for it, and there have to be enough blocks for a third of the SMs.
-constexpr size_t kSlab = 192 * 1024;  // (beside 16 KB of the backward's sums)
+constexpr size_t kSlab = 188 * 1024;  // (beside 36 KB of the backward's sums)
 inline size_t slab_groups(const mamba_b200_group_norm_args& a, Params& p, size_t vec, bool bwd) {
     const int tensors = (bwd ? 2 : 1) + (a.z ? 1 : 0);
     int groups = static_cast<int>((64 + p.vecs * vec - 1) / (p.vecs * vec));
     if (groups > p.groups) groups = p.groups;
-    const long long rp = kThreads / (groups * p.vecs), turns = (a.S + rp - 1) / rp, across = (a.G + groups - 1) / groups;
-    const unsigned long long bytes = static_cast<unsigned long long>(turns) * kThreads * vec * tensors;
+    const long long rp = kSlabThreads / (groups * p.vecs), turns = (a.S + rp - 1) / rp, across = (a.G + groups - 1) / groups;
+    const unsigned long long bytes = static_cast<unsigned long long>(turns) * kSlabThreads * vec * tensors;
     if (bytes > kSlab || across > 65535 || across * a.N < 48) return 0;
     p.groups = groups;
     return bytes;
@@ -1101,8 +1111,8 @@ int launch_vec(Ctx* c, const mamba_b200_group_norm_args& a, bool bwd, cudaStream
                 const long long side = (2 * kBlocks + across - 1) / across;
                 p.side = p.parts = static_cast<int>(side < a.N ? side : a.N);
                 const dim3 grid(static_cast<unsigned>(p.side), static_cast<unsigned>(across));
-                if (bwd) slab_kernel<T, VEC, true><<<grid, kThreads, bytes, st>>>(p);
-                else slab_kernel<T, VEC, false><<<grid, kThreads, bytes, st>>>(p);
+                if (bwd) slab_kernel<T, VEC, true><<<grid, kSlabThreads, bytes, st>>>(p);
+                else slab_kernel<T, VEC, false><<<grid, kSlabThreads, bytes, st>>>(p);
                 MB200_CUDA_CHECK(c, cudaGetLastError());
                 return join_sums(c, p, bwd, st);
             }
