@@ -2,7 +2,7 @@
 //
 // A block has 64 columns of one pair's (sequence, head) state and walks chunks of 128 steps (roles and names: linear_attention.cuh):
 //   G = X Y^T,  P = G o l^{distance},  out = P Z + l^{row} o (X S),  S <- l^n S + Y^T (w o Z)
-// Beside HBM, which a chunk of 128 x 64 heads of 128 x 64 keeps busy for 4100 cycles an SM, its products take 1500 cycles of the
+// Beside HBM, which a chunk of 128 x 64 heads of 128 x 64 keeps busy for 4100 cycles an SM, its products take some 2000 cycles of the
 // tensor pipe, so one block on an SM reaches HBM's rate if nothing waits for anything else: every part has warps of its own, and the
 // state, the only thing that is carried from chunk to chunk, stays in tensor memory,
 //   warp 0      asks for the tiles (X and Y, Z), as many chunks ahead as there are stages
@@ -11,15 +11,23 @@
 //   warp 3      issues X S and P Z
 //   warps 4-7   make P from G, of every other chunk; it goes back to tensor memory and is read there as an operand
 //   warps 8-11  leave a 16-bit copy of S for X S, and in its place what is left of it after the chunk
-//   warps 12-15 join P Z and X S and write rows
+//   warps 12-15 join P Z and X S and write rows, by TMA from Z's place (a thread's own row in pieces of 32 bytes took 2100 cycles)
 //   warps 16-19 weigh Z
 //   warps 20-23 make P of the other chunks
 // and they meet on mbarriers alone; every wait gives up after a limit and takes the block to its end.
 //
-// Roundings to 16 bits: P (made from f32 scores) and the copy of S that is read, each once, as the result is.  The state itself is f32:
-// w o Z, which it is made of, is kept to f32 accuracy where a state is handed on: three bf16 terms of 8 bits each; where only out is
-// wanted one term is enough.  In f16 a second term of 2^-11 of the first gives 22 bits, P is scaled by a power of two a row and S by
-// one a tile, so that neither their size nor their smallness leaves the type.
+// Slow decays (`fold`, bf16): w_j = l^{n-1-j} stands in for l^{i-j} = l^{i-(n-1)} w_j too.  w o Z takes Z's place, P is G with its future cut
+// off, and l^{i-(n-1)} is one factor a row of the result, in 32 bits.  Fast ones, whose l^{-127} leaves the numbers that 32 bits hold with
+// room to spare, and f16 weigh P instead.
+//
+// Roundings to 16 bits: the scores (made in f32), the weighted values beside them where they are folded, and the copy of S that is read,
+// each once, as the result is.  The state itself is f32: w o Z, which it is made of, is kept to f32 accuracy where a state is handed on:
+// three bf16 terms of 8 bits each; where only out is wanted one term is enough.  In f16 a second term of 2^-11 of the first gives 22 bits, P
+// is scaled by a power of two a row and S by one a tile, so that neither their size nor their smallness leaves the type.
+//
+// Device time of 8 x 4096 x 32 heads of 128 x 64, bf16: 126 to 130 us, 95 % of the measured copy rate (a block alone needs 2600 cycles a
+// chunk; with 148 of them HBM has them wait); its backward 449 to 461, 50 % (2200 cycles a chunk and 64 columns, of which the products
+// and the rows' warps are busy for most).  What the steps gave is told where it matters.
 #include <math.h>
 #include <string.h>
 
@@ -146,7 +154,8 @@ __device__ __forceinline__ float scale_to(float m, float* back) {
     return __uint_as_float(static_cast<uint32_t>(127 - d) << 23);
 }
 
-// (`fold` is known to the compiler: code that is not taken lies elsewhere, and what is fits the instruction cache better)
+// (`fold` is known to the compiler: code that is not taken lies elsewhere, and what is fits the instruction cache: 137 -> 126 us, the
+// backward 559 -> 449.  `back` is not: blocks of both directions share a cache, and two more variants took 634)
 template <typename Th, int TERMS, bool STATE, bool fold>
 __device__ __forceinline__ void walk(const TcParams& tp, unsigned char* smem, const Place& w, const float ld) {
     constexpr bool F16 = std::is_same<Th, __half>::value;
@@ -309,14 +318,13 @@ __device__ __forceinline__ void walk(const TcParams& tp, unsigned char* smem, co
             const uint32_t at = st * per_stage;
             const bool reads = i > 0 || enters, adds = leaves || i + 1 < n;
             const int u = enters ? i : i - 1;  // number of the copy of S
-            if (adds) {
-                ok = wait_warp(&sm->full[st], turn & 1, sm, p.status);
-                if (ok) ok = wait_warp(&sm->w_full[sz], turn_z & 1, sm, p.status);
-                // (with the copy of S, what is left of S is in its place)
-                if (ok && reads) ok = wait_warp(&sm->s_full[STATE ? 0 : u % SB], (STATE ? u : u / SB) & 1, sm, p.status);
-                if (!ok) break;
-                fence_after();
-            }
+            // (without a product too: what this warp commits counts for the tiles of this chunk, which have to be there)
+            ok = wait_warp(&sm->full[st], turn & 1, sm, p.status);
+            if (ok) ok = wait_warp(adds ? &sm->w_full[sz] : &sm->z_full[sz], turn_z & 1, sm, p.status);
+            // (with the copy of S, what is left of S is in its place)
+            if (ok && adds && reads) ok = wait_warp(&sm->s_full[STATE ? 0 : u % SB], (STATE ? u : u / SB) & 1, sm, p.status);
+            if (!ok) break;
+            fence_after();
             // first term; the others
             const uint64_t w0 = fold ? zm + sz * sub : wm, w1 = fold ? wm - sub : wm;
             if (elect_one()) {
