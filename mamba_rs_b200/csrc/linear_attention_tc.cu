@@ -70,9 +70,13 @@ struct Small {
     float tile_scale[4];  // (a copy's is read until its rows are out, which is known of the chunk three before)
     float warp_max[2][4];
     uint64_t full[4], empty[4], z_full[8], z_empty[8], g_full[2], p_full[2], y_full[2], y_empty[2], s_full[2], s_empty[2], w_full[8], z_read[8], d_full, max_full, drain[3];
+    // Values that are not finite may change no row before their own, as 0 times them in a product would: w o Z has 0 in their place, and
+    // of their column the rows from the first of them on, counted as they are walked, are NaN (as is the state that leaves).
+    int bad[kTile], any_bad;
     uint32_t tmem;
     int dead;
 };
+constexpr int kNever = 0x7fffffff;
 
 template <int TERMS>
 uint32_t smem_bytes(int na, int stages, int z_tiles) {
@@ -154,6 +158,32 @@ __device__ __forceinline__ float scale_to(float m, float* back) {
     return __uint_as_float(static_cast<uint32_t>(127 - d) << 23);
 }
 
+// A row of w o Z (its terms' tiles lie together) and of Z, some of whose values are not finite.
+template <typename Th>
+__device__ __noinline__ void set_aside(unsigned char* w0, unsigned char* w1, int more, unsigned char* z, int row, int pos, Small* sm) {
+    constexpr unsigned inf = std::is_same<Th, __half>::value ? 0x7c00u : 0x7f80u;
+    for (int c = 0; c < kTile; ++c) {
+        const uint32_t at = sw_chunk(row, c >> 3) + 2 * (c & 7);
+        if ((*reinterpret_cast<uint16_t*>(w0 + at) & inf) != inf) continue;
+        *reinterpret_cast<uint16_t*>(w0 + at) = 0;
+        *reinterpret_cast<uint16_t*>(z + at) = 0;
+        for (int t = 0; t < more; ++t) *reinterpret_cast<uint16_t*>(w1 + t * kSub + at) = 0;
+        atomicMin(&sm->bad[c], pos);
+    }
+    *reinterpret_cast<volatile int*>(&sm->any_bad) = 1;
+}
+// ... and the rows behind them: columns c < left of a row at out, `step` elements apart, or of row `row` of a swizzled tile.
+template <typename To>
+__device__ __noinline__ void spoil(To* out, int step, int left, int pos, const Small* sm) {
+    for (int c = 0; c < left; ++c)
+        if (sm->bad[c] <= pos) out[c * step] = from_f<To>(__int_as_float(0x7fffffff));
+}
+template <typename To>
+__device__ __noinline__ void spoil_tile(unsigned char* tile, int row, int pos, const Small* sm) {
+    for (int c = 0; c < kTile; ++c)
+        if (sm->bad[c] <= pos) *reinterpret_cast<To*>(tile + sw_chunk(row, c >> 3) + 2 * (c & 7)) = from_f<To>(__int_as_float(0x7fffffff));
+}
+
 // (`fold` is known to the compiler: code that is not taken lies elsewhere, and what is fits the instruction cache: 137 -> 126 us, the
 // backward 559 -> 449.  `back` is not: blocks of both directions share a cache, and two more variants took 634)
 template <typename Th, int TERMS, bool STATE, bool fold>
@@ -204,8 +234,10 @@ __device__ __forceinline__ void walk(const TcParams& tp, unsigned char* smem, co
         mbar_init(&sm->d_full, 1);
         mbar_init(&sm->max_full, 128);
         sm->dead = 0;
+        sm->any_bad = 0;
         fence_barrier_init();
     }
+    if (threadIdx.x >= 64 && threadIdx.x < 64 + kTile) sm->bad[threadIdx.x - 64] = kNever;
     if (threadIdx.x >= 32 && threadIdx.x < 64) {
         sm->col[lane] = decay_at(l2, back ? lane : 31 - lane);
         sm->diag[lane] = 0.0f;  // (31 is written below)
@@ -320,7 +352,7 @@ __device__ __forceinline__ void walk(const TcParams& tp, unsigned char* smem, co
             const int u = enters ? i : i - 1;  // number of the copy of S
             // (without a product too: what this warp commits counts for the tiles of this chunk, which have to be there)
             ok = wait_warp(&sm->full[st], turn & 1, sm, p.status);
-            if (ok) ok = wait_warp(adds ? &sm->w_full[sz] : &sm->z_full[sz], turn_z & 1, sm, p.status);
+            if (ok) ok = wait_warp(&sm->w_full[sz], turn_z & 1, sm, p.status);
             // (with the copy of S, what is left of S is in its place)
             if (ok && adds && reads) ok = wait_warp(&sm->s_full[STATE ? 0 : u % SB], (STATE ? u : u / SB) & 1, sm, p.status);
             if (!ok) break;
@@ -387,7 +419,7 @@ __device__ __forceinline__ void walk(const TcParams& tp, unsigned char* smem, co
                     commit(&sm->empty[st]);
                 }
                 __syncwarp();
-                ok = wait_warp(fold ? &sm->w_full[sz] : &sm->z_full[sz], turn_z & 1, sm, p.status);
+                ok = wait_warp(&sm->w_full[sz], turn_z & 1, sm, p.status);
                 if (ok) ok = wait_warp(&sm->p_full[i & 1], (i >> 1) & 1, sm, p.status);
                 if (!ok) break;
                 fence_after();
@@ -602,6 +634,18 @@ __device__ __forceinline__ void walk(const TcParams& tp, unsigned char* smem, co
                                 for (int c = 0; c < 32; c += 2) m = fmaxf(m, fmaxf(fabsf(v[c]), fabsf(v[c + 1])));
                             }
                         }
+                        // (NaN are passed over, and an infinity, which only a given state brings, is: other columns keep their digits)
+                        if (__any_sync(0xffffffffu, m == INFINITY)) {
+                            tmem_st_wait();
+                            m = 0.0f;
+#pragma unroll 1
+                            for (int s = 0; s < 2; ++s) {
+                                float v[32];
+                                tmem_ld32(lanes + cS + 32 * s, v);
+                                if (mine)
+                                    for (int c = 0; c < 32; ++c) m = fmaxf(m, fabsf(v[c]) < INFINITY ? fabsf(v[c]) : 0.0f);
+                            }
+                        }
                         m = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(m)));
                         if (lane == 0) sm->warp_max[u & 1][warp & 3] = m;
                         mbar_arrive(&sm->max_full);
@@ -657,6 +701,7 @@ __device__ __forceinline__ void walk(const TcParams& tp, unsigned char* smem, co
         }
         if (ok && leaves && n > 0) {
             ok = wait_warp(&sm->d_full, (n - 1) & 1, sm, p.status);
+            if (ok) ok = wait_warp(&sm->w_full[(n - 1) % zs], ((n - 1) / zs) & 1, sm, p.status);
             if (ok) {
                 fence_after();
                 const Pow f = !STATE && r.last_decay ? decay_pow(ld, 1) : Pow{1.0f, 0.0f};
@@ -680,6 +725,7 @@ __device__ __forceinline__ void walk(const TcParams& tp, unsigned char* smem, co
                             if (c < left) out[(32 * s + c) * (STATE ? A : 1)] = v[c];
                     }
                 }
+                if (*reinterpret_cast<volatile int*>(&sm->any_bad) && mine) spoil(out, STATE ? A : 1, nc, kNever - 1, sm);
             }
         }
     } else if (role == 3 && !STATE) {
@@ -692,7 +738,10 @@ __device__ __forceinline__ void walk(const TcParams& tp, unsigned char* smem, co
             // (Z's place, where the rows go, is read by the products of S too)
             if (!wait_warp(&sm->z_read[sz], turn_z & 1, sm, p.status)) break;
             if (!wait_warp(&sm->y_full[i & 1], (i >> 1) & 1, sm, p.status)) break;
+            if (!wait_warp(&sm->w_full[sz], turn_z & 1, sm, p.status)) break;  // (long over; what it says of bad values is read here)
             fence_after();
+            const bool bad = *reinterpret_cast<volatile int*>(&sm->any_bad);
+            const int pos = i * kChunk + (back ? kChunk - 1 - row : row);
             const int t0 = start(i), rows = min(kChunk, p.T - t0);
             const bool reads = i > 0 || enters;
             const int late = i == 0 ? late0 : 0;
@@ -744,6 +793,7 @@ __device__ __forceinline__ void walk(const TcParams& tp, unsigned char* smem, co
                             make_uint4(pack2<Th>(y[8 * j], y[8 * j + 1]), pack2<Th>(y[8 * j + 2], y[8 * j + 3]),
                                        pack2<Th>(y[8 * j + 4], y[8 * j + 5]), pack2<Th>(y[8 * j + 6], y[8 * j + 7]));
                 }
+                if (bad) spoil_tile<Th>(at, row, pos, sm);
                 fence_proxy_async();
                 __syncwarp();
                 if (lane == 0) {
@@ -767,6 +817,10 @@ __device__ __forceinline__ void walk(const TcParams& tp, unsigned char* smem, co
                             else static_cast<Th*>(r.out)[at + 32 * s + c] = from_f<Th>(y[c]);
                         }
                 }
+                if (bad) {
+                    if (r.out_f32) spoil(static_cast<float*>(r.out) + at, 1, left, pos, sm);
+                    else spoil(static_cast<Th*>(r.out) + at, 1, left, pos, sm);
+                }
                 fence_before();
                 mbar_arrive(&sm->y_empty[i & 1]);
             }
@@ -780,8 +834,7 @@ __device__ __forceinline__ void walk(const TcParams& tp, unsigned char* smem, co
     } else if (role == 4) {
         // ---- w o Z ----
         const float w_whole = decay_at(l2, back ? row : kChunk - 1 - row) * r.alpha_s;
-        // (w o Z as an operand of P's product is wanted of the last chunk too)
-        for (int i = 0, st = 0, turn = 0; i < n - (leaves || fold ? 0 : 1); ++i) {
+        for (int i = 0, st = 0, turn = 0; i < n; ++i) {
             const int rows = min(kChunk, p.T - start(i));
             if (!wait_warp(&sm->z_full[st], turn & 1, sm, p.status)) break;
             // (the terms' tiles are the last chunk's products' until they are done)
@@ -790,6 +843,7 @@ __device__ __forceinline__ void walk(const TcParams& tp, unsigned char* smem, co
             unsigned char* z = smem + kZ + st * kSub;
             unsigned char* w0 = fold ? z : smem + kW;
             unsigned char* w1 = fold ? smem + kW - kSub : smem + kW;
+            float2 zero = make_float2(0.0f, 0.0f);  // NaN, if a value is not finite
 #pragma unroll 2
             for (int j = 0; j < 8; ++j) {
                 const uint4 v = *reinterpret_cast<const uint4*>(z + sw_chunk(row, j));
@@ -798,6 +852,7 @@ __device__ __forceinline__ void walk(const TcParams& tp, unsigned char* smem, co
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
                     float2 x = mul2(unpack2<Th>(in[e]), splat2(f));
+                    zero = fma2(x, splat2(0.0f), zero);
                     o[0][e] = pack2<Th>(x.x, x.y);
 #pragma unroll
                     for (int t = 1; t < TERMS; ++t) {
@@ -811,6 +866,7 @@ __device__ __forceinline__ void walk(const TcParams& tp, unsigned char* smem, co
                 for (int t = 0; t < TERMS; ++t)
                     *reinterpret_cast<uint4*>((t == 0 ? w0 : w1 + t * kSub) + sw_chunk(row, j)) = make_uint4(o[t][0], o[t][1], o[t][2], o[t][3]);
             }
+            if (!(zero.x + zero.y == 0.0f)) set_aside<Th>(w0, w1 + kSub, TERMS - 1, z, row, i * kChunk + (back ? kChunk - 1 - row : row), sm);
             fence_proxy_async();
             mbar_arrive(&sm->w_full[st]);
             if (++st == zs) {
