@@ -661,8 +661,8 @@ MAMBA_B200_API int mamba_b200_gated_scan_bwd(void* handle, void* stream, const m
  * Hv divides H, and head h reads head h / (H / Hx) of a tensor with fewer.  Strides of batch, step and head in elements, the last
  * dimension contiguous (columns of one projection, say).  decay [H] f32, log of the factor a step (0: none, minus infinity: nothing is
  * kept; above 0 the state grows as the formula says).  States [B, H, K, V] f32 contiguous.  K and V are at most 256.  T = 1 is the decode
- * step; T = 0 hands the state on.  An infinite or NaN input may show in every output of the 128 steps (from a multiple of 128 on)
- * that it lies in, the earlier ones among them, and in all that follow (T = 1: in its own alone).
+ * step; T = 0 hands the state on.  An infinite or NaN input changes no output of an earlier step, nor
+ * of another head or sequence, and a value no other column; what does depend on it may be NaN where the formula has an infinity.
  *   forward : state (NULL: zeros) enters, state_out (NULL: not written; may be state) leaves.
  *   backward: the states are made again.  d_state_out (NULL: zeros) is the gradient of the state that left, d_state (NULL: not
  *             written; not d_state_out) that of the one that entered.  d_q, d_k, d_v have the heads of q, k, v (gradients of shared
@@ -743,6 +743,7 @@ MAMBA_B200_API int mamba_b200_rotary(void* handle, void* stream, const mamba_b20
  * the C / G channels of a group (S = 1: each token by itself, a group for each head, say), in f32 around the mean.  weight, bias [C] f32
  * (NULL: 1 and 0), z NULL: no gate.  stats [2, N, G] f32: mean and rstd, which the forward writes (NULL: not kept) and the backward
  * reads.
+ * y may be x or z, d_x may be dy or x, d_z may be z (same strides); results overlap nothing else.
  *   backward: d_x and, with z, d_z are overwritten; d_weight and d_bias [C] f32 (NULL: not wanted) are added to what they hold when
  *   accumulate is not 0, else written.  Sums run in an order that the sizes alone give: the same inputs give the same bits.
  * workspace: 256-byte aligned, mamba_b200_group_norm_workspace_bytes(N, S, C, G, backward) bytes (may be 0); nothing in it is kept

@@ -917,7 +917,7 @@ def linear_attention_fwd(q, k, v, decay, *, scale=None, state=None, state_out=No
     each head's factor a token; Hq, Hk and Hv divide H (fewer heads are shared by consecutive ones); K, V <= 256; scale: K ** -0.5
     if None.  state [B,H,K,V] f32 enters (zeros if None), state_out receives what leaves (may be state).  workspace: scratch of
     linear_attention_workspace_bytes(...) bytes (made here if None).  Returns o [B,T,H,V] in q's dtype.  An infinite or NaN input
-    may show in all outputs of its block of 128 tokens, earlier ones too."""
+    changes no earlier token's output; what depends on it may be NaN where the formula has an infinity."""
     dev = _device_index(q, k, v, decay, state, state_out, o, workspace)
     a, shape = _attention_args(q, k, v, decay, scale, state)
     B, H, _, V = shape
@@ -1129,7 +1129,8 @@ def _norm_args(x, z, weight, bias, groups, activation, eps):
 def group_norm_fwd(x, weight, bias, groups, *, eps=1e-5, activation=None, z=None, y=None, stats=None, workspace=None, handle=None):
     """Group norm with channels last: y = act((x - mean) / sqrt(var + eps) * weight + bias) * SiLU(z).  x, z, y [N,S,C] in a storage dtype
     (any row stride), mean and var over a sample's S rows and the C / groups channels of a group; [N,C] is S = 1, each row by itself
-    (a group for each head, say).  weight, bias [C] f32 or None; activation None, "silu" or "gelu" (by erf); z None: no gate.
+    (a group for each head, say).  weight, bias [C] f32 or None; activation None, "silu" or "gelu" (by erf); z None: no gate.  y may be
+    x or z.
     Returns (y, stats): mean and rstd f32 [2,N,groups], which group_norm_bwd takes."""
     dev = _device_index(x, weight, bias, z, y, stats, workspace)
     a = _norm_args(x, z, weight, bias, groups, activation, eps)
