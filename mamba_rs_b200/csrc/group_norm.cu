@@ -4,11 +4,14 @@
 //   dv = dy * SiLU(z) * act'(v),     d_z = dy * act(v) * SiLU'(z),     d_w = sum dv * xh,     d_b = sum dv     (xh = (x - mean) * rstd)
 //   d_x = rstd * (dv * w - mean(dv * w) - xh * mean(dv * w * xh))
 //
-// Every element is read once or twice and written once, so HBM bounds it.  Two forms:
-//  * rows: S = 1, a group fits a block.  A thread owns the same channels of row after row; a group's sums are
-//    shuffles (and a barrier where it takes more than a warp), the variance is taken around the mean from registers, and the backward's sums over rows stay in registers until
-//    the block's end.
-//  * samples: any S.  A first kernel leaves mean and squared deviations (backward: the sums) of each block of rows and group, joined
+// Every element is read once or twice and written once, so HBM bounds it, with instructions close behind.  Three forms:
+//  * rows: S = 1, a group fits a block.  A thread owns the same channels of row after row, the next of which are on their way to
+//    shared memory; a group's sums are shuffles (and a barrier where it takes more than a warp), the variance is taken around the mean
+//    from registers, and the backward's sums over rows stay in registers until the block's end.  32768 rows of 2048 channels in 32
+//    groups, gated, bf16: 75 to 79 us, 80 % of the measured copy rate (84 with activation and gate looked up for every value, 118 without
+//    the rows on their way); backward 128, 81 %.
+//  * samples that fit shared memory: one kernel, every element read once.  3 samples of 1021 rows of 768 channels, f32: 13 us (18.5 in two kernels).
+//  * other samples: a first kernel leaves mean and squared deviations (backward: the sums) of each block of rows and group, joined
 //    pairwise around their means, and a second one joins the blocks of its groups in their order and goes over the rows again, which
 //    L2 has where they fit it.
 #include <math.h>

@@ -44,9 +44,9 @@ using namespace mb200::tc;
 
 constexpr int kThreads = 768, kTile = 64;
 constexpr uint32_t kSub = kSwSub;  // a [128 x 64] sub-tile
-// Tensor memory: two buffers of G, whose left half P takes and whose right half P Z (not folded); two of X S and, folded, P Z in one sum; S
-// and, in f16, the sum of a chunk's second terms.
-constexpr uint32_t cG = 0, cY1 = 64, cY2 = 256, cS = 384, cSlo = 448, kCols = 512;
+// Tensor memory: two buffers of G, whose left half P takes and whose right half P Z (not folded); two of X S (f16: one) and, folded, P Z in
+// one sum; S, and where it has one a chunk's sum; in f16 the sum of the second terms.
+constexpr uint32_t cG = 0, cY1 = 64, cY2 = 256, cDf = 320, cS = 384, cSlo = 448, kCols = 512;
 
 struct TcParams {
     CUtensorMap x[3], y[3], z[3], out[3];
@@ -69,7 +69,7 @@ struct Small {
     float row_scale[2][128];
     float tile_scale[4];  // (a copy's is read until its rows are out, which is known of the chunk three before)
     float warp_max[2][4];
-    uint64_t full[4], empty[4], z_full[8], z_empty[8], g_full[2], p_full[2], y_full[2], y_empty[2], s_full[2], s_empty[2], w_full[8], z_read[8], d_full, max_full, drain[3];
+    uint64_t full[4], empty[4], z_full[8], z_empty[8], g_full[2], p_full[2], y_full[2], y_empty[2], s_full[2], s_empty[2], w_full[8], z_read[8], d_full, d_read, max_full, drain[3];
     // Values that are not finite may change no row before their own, as 0 times them in a product would: w o Z has 0 in their place, and
     // of their column the rows from the first of them on, counted as they are walked, are NaN (as is the state that leaves).
     int bad[kTile], any_bad;
@@ -190,6 +190,11 @@ template <typename Th, int TERMS, bool STATE, bool fold>
 __device__ __forceinline__ void walk(const TcParams& tp, unsigned char* smem, const Place& w, const float ld) {
     constexpr bool F16 = std::is_same<Th, __half>::value;
     constexpr int SB = kCopies<TERMS>;
+    // A product adds to its accumulator by cutting off, always towards zero: with a chunk's 24 of them on top of S, a state that decays slowly
+    // lost 2^-25 of itself each time, 10^-5 over 40 chunks.  Where a state has to keep its digits a chunk's sum has an accumulator of its
+    // own, and joins S in a rounded f32 sum.  (Where only 16-bit rows are wanted, S itself: 464 us for 500 of a backward.)
+    constexpr bool FRESH = TERMS > 1;
+    constexpr uint32_t cD = !FRESH ? cS : F16 ? cDf : cSlo;
     constexpr uint32_t fmt = F16 ? 0u : 1u;
     const Params& p = tp.p;
     const Role& r = p.role[w.role];
@@ -233,6 +238,7 @@ __device__ __forceinline__ void walk(const TcParams& tp, unsigned char* smem, co
         for (int i = 0; i < 3; ++i) mbar_init(&sm->drain[i], 1);
         mbar_init(&sm->d_full, 1);
         mbar_init(&sm->max_full, 128);
+        mbar_init(&sm->d_read, 128);
         sm->dead = 0;
         sm->any_bad = 0;
         fence_barrier_init();
@@ -353,8 +359,9 @@ __device__ __forceinline__ void walk(const TcParams& tp, unsigned char* smem, co
             // (without a product too: what this warp commits counts for the tiles of this chunk, which have to be there)
             ok = wait_warp(&sm->full[st], turn & 1, sm, p.status);
             if (ok) ok = wait_warp(&sm->w_full[sz], turn_z & 1, sm, p.status);
-            // (with the copy of S, what is left of S is in its place)
-            if (ok && adds && reads) ok = wait_warp(&sm->s_full[STATE ? 0 : u % SB], (STATE ? u : u / SB) & 1, sm, p.status);
+            // the sum of the last chunk has been read; or, where it is S itself, what is left of S is in its place (with the copy of S)
+            if (FRESH && ok && adds && i > 0) ok = wait_warp(&sm->d_read, (i - 1) & 1, sm, p.status);
+            if (!FRESH && ok && adds && reads) ok = wait_warp(&sm->s_full[STATE ? 0 : u % SB], (STATE ? u : u / SB) & 1, sm, p.status);
             if (!ok) break;
             fence_after();
             // first term; the others
@@ -366,8 +373,8 @@ __device__ __forceinline__ void walk(const TcParams& tp, unsigned char* smem, co
                         const bool own = F16 && t == 1;  // (the second f16 term is summed apart)
 #pragma unroll
                         for (int k = 0; k < kChunk / 16; ++k)
-                            mma(tmem + (own ? cSlo : cS), ym + at + k * mStep, (t == 0 ? w0 : w1 + t * sub) + k * mStep, idD,
-                                own ? k > 0 : reads || k > 0 || t > 0);
+                            mma(tmem + (own ? cSlo : cD), ym + at + k * mStep, (t == 0 ? w0 : w1 + t * sub) + k * mStep, idD,
+                                own ? k > 0 : (!FRESH && reads) || k > 0 || t > 0);
                     }
                     commit(&sm->d_full);
                 }
@@ -397,10 +404,11 @@ __device__ __forceinline__ void walk(const TcParams& tp, unsigned char* smem, co
             bool ok = true;
             int st = 0, turn = 0, sz = 0, turn_z = 0;
             for (int i = 0; i < n; ++i) {
-                const uint32_t at = st * per_stage, d = tmem + cY2 + (i & 1) * 64;
+                const uint32_t at = st * per_stage, d = tmem + cY2 + (F16 ? 0 : (i & 1) * 64);
                 const bool reads = i > 0 || enters;
                 const int u = enters ? i : i - 1;  // number of the copy of S
-                if (i > 1) ok = wait_warp(&sm->y_empty[i & 1], ((i >> 1) - 1) & 1, sm, p.status);
+                const int j = F16 ? i - 1 : i - 2;  // the chunk that had this buffer before
+                if (j >= 0) ok = wait_warp(&sm->y_empty[j & 1], (j >> 1) & 1, sm, p.status);
                 if (ok) ok = wait_warp(&sm->full[st], turn & 1, sm, p.status);
                 if (ok && reads) ok = wait_warp(&sm->s_full[u % SB], (u / SB) & 1, sm, p.status);
                 if (!ok) break;
@@ -592,17 +600,33 @@ __device__ __forceinline__ void walk(const TcParams& tp, unsigned char* smem, co
                 tmem_st32(lanes + cS + 32 * s, v);
             }
         }
+        if (FRESH && !enters) {
+            const float none[32] = {};
+            tmem_st32(lanes + cS, none);
+            tmem_st32(lanes + cS + 32, none);
+        }
         const Pow whole = decay_pow(ld, kChunk);
-        // 32 columns of S (f16: with the sum of the last chunk's second terms)
+        // 32 columns of S with the last chunk's sum
         auto read = [&](int s, float* v) {
-            if (F16) {
-                float lo[32];
-                tmem_ld32x2(lanes + cS + 32 * s, v, lanes + cSlo + 32 * s, lo);
-#pragma unroll
-                for (int c = 0; c < 32; ++c) v[c] = fmaf(lo[c], 1.0f / 2048, v[c]);
-            } else {
+            if (!FRESH) {
                 tmem_ld32(lanes + cS + 32 * s, v);
+                return;
             }
+            float d[32];
+            if (F16) {
+                tmem_ld32x2(lanes + cD + 32 * s, v, lanes + cSlo + 32 * s, d);
+#pragma unroll
+                for (int c = 0; c < 32; ++c) v[c] = fmaf(d[c], 1.0f / 2048, v[c]);
+                tmem_ld32(lanes + cS + 32 * s, d);
+            } else {
+                tmem_ld32x2(lanes + cS + 32 * s, v, lanes + cD + 32 * s, d);
+            }
+#pragma unroll
+            for (int c = 0; c < 32; ++c) v[c] += d[c];
+        };
+        auto has_read = [&]() {
+            fence_before();
+            mbar_arrive(&sm->d_read);
         };
         int u = 0;  // copies of S
         bool ok = true;
@@ -634,6 +658,7 @@ __device__ __forceinline__ void walk(const TcParams& tp, unsigned char* smem, co
                                 for (int c = 0; c < 32; c += 2) m = fmaxf(m, fmaxf(fabsf(v[c]), fabsf(v[c + 1])));
                             }
                         }
+                        if (i > 0) has_read();
                         // (NaN are passed over, and an infinity, which only a given state brings, is: other columns keep their digits)
                         if (__any_sync(0xffffffffu, m == INFINITY)) {
                             tmem_st_wait();
@@ -665,8 +690,12 @@ __device__ __forceinline__ void walk(const TcParams& tp, unsigned char* smem, co
 #pragma unroll 1
                 for (int s = 0; s < 2; ++s) {
                     float v[32];
-                    if (F16 && STATE && i > 0) read(s, v);
-                    else tmem_ld32(lanes + cS + 32 * s, v);  // (f16: joined above)
+                    if (i > 0 && (!F16 || STATE)) {
+                        read(s, v);
+                        if (FRESH && s == 1) has_read();
+                    } else {
+                        tmem_ld32(lanes + cS + 32 * s, v);  // (joined above, or nothing to join)
+                    }
                     // (folded: rows take the factor that w o Z lacks, and with it X S is wanted of what is left of S)
                     auto decay = [&]() {
 #pragma unroll
@@ -695,7 +724,7 @@ __device__ __forceinline__ void walk(const TcParams& tp, unsigned char* smem, co
                 }
                 if (!STATE) fence_proxy_async();
                 fence_before();
-                mbar_arrive(&sm->s_full[STATE ? 0 : u % SB]);
+                if (!STATE || !FRESH) mbar_arrive(&sm->s_full[STATE ? 0 : u % SB]);
                 ++u;
             }
         }
@@ -752,7 +781,7 @@ __device__ __forceinline__ void walk(const TcParams& tp, unsigned char* smem, co
                 f1 = sm->row_scale[i & 1][row];
                 if (reads) f *= sm->tile_scale[(enters ? i : i - 1) & 3];
             }
-            const uint32_t y2 = lanes + cY2 + (i & 1) * 64, y1 = fold ? y2 : lanes + cG + (i & 1) * 128 + cY1;
+            const uint32_t y2 = lanes + cY2 + (F16 ? 0 : (i & 1) * 64), y1 = fold ? y2 : lanes + cG + (i & 1) * 128 + cY1;
             // 32 columns of out
             auto read = [&](int s, float* y) {
                 if (!fold && reads) {

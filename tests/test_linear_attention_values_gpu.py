@@ -184,3 +184,34 @@ def test_decays_of_every_speed_side_by_side(cuda_dev, dt):
     gmags = attention_grads(q.abs(), k.abs(), v.abs(), do.abs(), decay, K ** -0.5, state.abs(), d_last.abs())
     for g, w, m in zip(grads, wants[:3], gmags[:3]):
         close(g, w, m, dt, 64 + T, extra=2.0)
+
+
+@pytest.mark.parametrize("dt", DTS)
+@pytest.mark.parametrize("T,K,V,H", [(20000, 64, 64, 3), (6000, 128, 64, 40), (6000, 40, 72, 40)])
+def test_states_of_long_texts_keep_their_digits(cuda_dev, dt, T, K, V, H):
+    """A state that hardly decays is a sum of thousands of tokens.  The tensor cores' sums of a chunk's 24 partial products are cut off, not
+    rounded: up to 24 2^-23 of a chunk's sum, always towards zero, so up to as much of the state; its terms are kept to 2^-22; the chunks'
+    roundings, T / 128 of 2^-24 with random signs (f32: T / 32), come on top.  Nothing may grow with T faster."""
+    import torch
+    from retention_ref import DT, fro
+
+    from mamba_rs_b200 import ops
+    g = torch.Generator(cuda_dev).manual_seed(T + K)
+    rn = lambda *s: torch.randn(*s, device=cuda_dev, generator=g)  # noqa: E731
+    # (values with a mean, so that the state grows)
+    q, k = ((rn(1, T, H, K) + 0.5).to(DT[dt]) for _ in range(2))
+    v, do = ((rn(1, T, H, V) + 0.5).to(DT[dt]) for _ in range(2))
+    decay = -1e-4 * torch.arange(H, device=cuda_dev, dtype=torch.float32) / H
+    state, d_last = 10 * rn(1, H, K, V), 10 * rn(1, H, K, V)
+    tol = 24 * 2.0 ** -23 + 2.0 ** -22 + 4 * 2.0 ** -24 * math.sqrt(T / 32)
+    t = torch.arange(T, device=cuda_dev, dtype=torch.float64)[:, None]
+    whole = torch.exp(decay.double() * T)[None, :, None, None]
+    w = torch.exp(decay.double() * (T - 1 - t))
+    want = torch.stack([(k[0, :, h].double() * w[:, h, None]).T @ v[0, :, h].double() for h in range(H)])[None] + whole * state.double()
+    _, last = run(ops, q, k, v, decay, state)
+    assert fro(last, want) <= tol, fro(last, want) / tol
+    scale = K ** -0.5
+    w = torch.exp(decay.double() * (t + 1)) * scale
+    want = torch.stack([(q[0, :, h].double() * w[:, h, None]).T @ do[0, :, h].double() for h in range(H)])[None] + whole * d_last.double()
+    got = ops.linear_attention_bwd(q, k, v, do, decay, state=state, d_state_out=d_last)["d_state"]
+    assert fro(got, want) <= tol, fro(got, want) / tol
