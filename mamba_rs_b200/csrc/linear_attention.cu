@@ -94,12 +94,13 @@ __global__ void __launch_bounds__(kStepThreads) step_kernel(const mamba_b200_lin
 // Any size, type and stride: a block has 32 columns of one pair's state in shared memory and walks chunks of 32 steps,
 //   P = mask(X Y^T),  out = P Z + decayed X S,  S <- l^n S + Y^T (weights o Z),
 // all in f32 with tiles of registers.  Steps are numbered in the order they are walked, so the roles that run backwards
-// differ in what a step's address is alone.  Bound by the FP32 pipe and what feeds it from shared memory: 8 x 4096 x 32 heads of
-// 128 x 64 f32 4190 us (the same in bf16 on the tensor cores 130), 2 x 2048 x 8 heads 169.
+// differ in what a step's address is alone.  Bound by shared memory, which a load of 16 bytes a lane takes for four cycles: a thread has two
+// rows by four columns, so that six loads feed 32 products (one row, five for 16: 3710 us for 3470 at 8 x 4096 x 32 heads of 128 x 64 f32,
+// 10640 for 7310 at 4 x 4096 x 16 heads of 256 x 256 f16).  In bf16 the first of them takes 130 on the tensor cores.
 // With few pairs the sequence is cut into segments: STATE blocks find what each adds to a state from zero, and the full walk
 // starts from the sum of what was before.
 // ---------------------------------------------------------------------------------------------------
-constexpr int kCols = 32, kThreads = 256;
+constexpr int kCols = 32, kThreads = 128, kRows = 16;  // a thread has rows i and i + kRows of a chunk
 
 inline size_t gen_smem(int A) { return sizeof(float) * (2 * kSteps * (A + 4) + 2 * kSteps * kCols + kSteps * (kSteps + 4) + A * kCols + 3 * kSteps); }
 
@@ -119,7 +120,7 @@ __device__ __forceinline__ float4 load4(const T* p, int n, bool vec) {
 
 // NA: blocks of 32 columns of X and Y (4 or 8).  With 4 a chunk's rows are asked for while the one before is worked on.
 template <typename T, int NA, bool STATE>
-__global__ void __launch_bounds__(kThreads) general_kernel(const Params p) {
+__global__ void __launch_bounds__(kThreads, NA == 4 ? 3 : 2) general_kernel(const Params p) {
     extern __shared__ __align__(16) float sm[];
     const Place w = place(p, blockIdx.x, STATE ? p.segments - 1 : p.segments);
     const Role& r = p.role[w.role];
@@ -136,25 +137,28 @@ __global__ void __launch_bounds__(kThreads) general_kernel(const Params p) {
     const float ld = p.decay[h], l2 = ld * kLog2e;
     const int t_lo = w.seg * p.seg_len, t_hi = min(p.T, t_lo + p.seg_len);
     const int i4 = tid >> 3, j8 = tid & 7, w4 = j8 * 4;
-    // this thread's pieces of a chunk: row i4, four columns at w4 of every 32
+    // this thread's pieces of a chunk: rows i4 and i4 + kRows, four columns at w4 of every 32
     auto row = [&](int t) { return r.backwards ? p.T - 1 - t : t; };
     const T* xg = static_cast<const T*>(r.x.p) + b * r.x.sb + (h / r.x.group) * r.x.sh + w4;
     const T* yg = static_cast<const T*>(r.y.p) + b * r.y.sb + (h / r.y.group) * r.y.sh + w4;
     const T* zg = static_cast<const T*>(r.z.p) + b * r.z.sb + (h / r.z.group) * r.z.sh + c0 + w4;
     auto whole = [](const T* q, long long st) { return ((reinterpret_cast<uintptr_t>(q) | st * sizeof(T)) & (2 * sizeof(T) - 1)) == 0; };
     const bool vx = whole(xg, r.x.st), vy = whole(yg, r.y.st), vz = whole(zg, r.z.st);
-    float4 xr[NA], yr[NA], zr;
+    float4 xr[2][NA], yr[2][NA], zr[2];
     auto fetch = [&](int t0) {
-        const int t = t0 + i4;
-        const bool ok = t < t_hi;
-        const long long at = ok ? row(t) : 0;
 #pragma unroll
-        for (int m = 0; m < NA; ++m) {
-            const int n = ok ? A - w4 - 32 * m : 0;
-            if (!STATE) xr[m] = load4(xg + at * r.x.st + 32 * m, n, vx);
-            yr[m] = load4(yg + at * r.y.st + 32 * m, n, vy);
+        for (int e = 0; e < 2; ++e) {
+            const int t = t0 + i4 + kRows * e;
+            const bool ok = t < t_hi;
+            const long long at = ok ? row(t) : 0;
+#pragma unroll
+            for (int m = 0; m < NA; ++m) {
+                const int n = ok ? A - w4 - 32 * m : 0;
+                if (!STATE) xr[e][m] = load4(xg + at * r.x.st + 32 * m, n, vx);
+                yr[e][m] = load4(yg + at * r.y.st + 32 * m, n, vy);
+            }
+            zr[e] = load4(zg + at * r.z.st, ok ? nc - w4 : 0, vz);
         }
-        zr = load4(zg + at * r.z.st, ok ? nc - w4 : 0, vz);
     };
     fetch(t_lo);
     if (tid <= kSteps) pw[tid] = decay_at(l2, tid);
@@ -182,68 +186,90 @@ __global__ void __launch_bounds__(kThreads) general_kernel(const Params p) {
         if (NA > 4 && t0 > t_lo) fetch(t0);
         __syncthreads();  // the last chunk's readers of X, Y, Z, Zw; the state and the powers are whole
 #pragma unroll
-        for (int m = 0; m < NA; ++m)
-            if (w4 + 32 * m < Ar) {
-                if (!STATE) *reinterpret_cast<float4*>(X + i4 * LD + w4 + 32 * m) = xr[m];
-                *reinterpret_cast<float4*>(Y + i4 * LD + w4 + 32 * m) = yr[m];
-            }
-        const float f = i4 < n ? pw[n - 1 - i4] * r.alpha_s : 0.0f;
-        *reinterpret_cast<float4*>(Z + i4 * kCols + w4) = zr;
-        *reinterpret_cast<float4*>(Zw + i4 * kCols + w4) = make_float4(zr.x * f, zr.y * f, zr.z * f, zr.w * f);
+        for (int e = 0; e < 2; ++e) {
+            const int i = i4 + kRows * e;
+#pragma unroll
+            for (int m = 0; m < NA; ++m)
+                if (w4 + 32 * m < Ar) {
+                    if (!STATE) *reinterpret_cast<float4*>(X + i * LD + w4 + 32 * m) = xr[e][m];
+                    *reinterpret_cast<float4*>(Y + i * LD + w4 + 32 * m) = yr[e][m];
+                }
+            const float f = i < n ? pw[n - 1 - i] * r.alpha_s : 0.0f;
+            *reinterpret_cast<float4*>(Z + i * kCols + w4) = zr[e];
+            *reinterpret_cast<float4*>(Zw + i * kCols + w4) = make_float4(zr[e].x * f, zr[e].y * f, zr[e].z * f, zr[e].w * f);
+        }
         __syncthreads();
         if (NA == 4 && t0 + kSteps < t_hi) fetch(t0 + kSteps);
         if (!STATE) {
-            // P[i4][j8 + 8 m]
-            float g[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+            // P[i][j8 + 8 m]
+            float g[2][4] = {};
             for (int a = 0; a < Ar; a += 4) {
-                const float4 x = *reinterpret_cast<const float4*>(X + i4 * LD + a);
+                float4 x[2];
+#pragma unroll
+                for (int e = 0; e < 2; ++e) x[e] = *reinterpret_cast<const float4*>(X + (i4 + kRows * e) * LD + a);
 #pragma unroll
                 for (int m = 0; m < 4; ++m) {
                     const float4 y = *reinterpret_cast<const float4*>(Y + (j8 + 8 * m) * LD + a);
-                    g[m] = fmaf(x.x, y.x, fmaf(x.y, y.y, fmaf(x.z, y.z, fmaf(x.w, y.w, g[m]))));
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) g[e][m] = fmaf(x[e].x, y.x, fmaf(x[e].y, y.y, fmaf(x[e].z, y.z, fmaf(x[e].w, y.w, g[e][m]))));
                 }
             }
 #pragma unroll
-            for (int m = 0; m < 4; ++m) {
-                const int j = j8 + 8 * m;
-                P[i4 * (kSteps + 4) + j] = j <= i4 ? g[m] * (pw[max(i4 - j, 0)] * r.alpha_p) : 0.0f;
-            }
+            for (int e = 0; e < 2; ++e)
+#pragma unroll
+                for (int m = 0; m < 4; ++m) {
+                    const int i = i4 + kRows * e, j = j8 + 8 * m;
+                    P[i * (kSteps + 4) + j] = j <= i ? g[e][m] * (pw[max(i - j, 0)] * r.alpha_p) : 0.0f;
+                }
             __syncthreads();
-            float o[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+            float o[2][4] = {};
+            auto add = [&](int e, float q, const float4& z) {
+                o[e][0] = fmaf(q, z.x, o[e][0]);
+                o[e][1] = fmaf(q, z.y, o[e][1]);
+                o[e][2] = fmaf(q, z.z, o[e][2]);
+                o[e][3] = fmaf(q, z.w, o[e][3]);
+            };
             if (entered || t0 > t_lo) {
                 for (int a = 0; a < Ar; a += 4) {
-                    const float4 x = *reinterpret_cast<const float4*>(X + i4 * LD + a);
-                    const float xv[4] = {x.x, x.y, x.z, x.w};
+                    float xv[2][4];
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+                        const float4 x = *reinterpret_cast<const float4*>(X + (i4 + kRows * e) * LD + a);
+                        xv[e][0] = x.x; xv[e][1] = x.y; xv[e][2] = x.z; xv[e][3] = x.w;
+                    }
 #pragma unroll
                     for (int u = 0; u < 4; ++u) {
                         const float4 s = *reinterpret_cast<const float4*>(S + (a + u) * kCols + w4);
-                        o[0] = fmaf(xv[u], s.x, o[0]);
-                        o[1] = fmaf(xv[u], s.y, o[1]);
-                        o[2] = fmaf(xv[u], s.z, o[2]);
-                        o[3] = fmaf(xv[u], s.w, o[3]);
+#pragma unroll
+                        for (int e = 0; e < 2; ++e) add(e, xv[e][u], s);
                     }
                 }
-                const float f = pw[i4 + 1 - late] * r.alpha_x;
 #pragma unroll
-                for (int u = 0; u < 4; ++u) o[u] *= f;
+                for (int e = 0; e < 2; ++e) {
+                    const float f = pw[i4 + kRows * e + 1 - late] * r.alpha_x;
+#pragma unroll
+                    for (int u = 0; u < 4; ++u) o[e][u] *= f;
+                }
             }
+            // (no row meets a later one's values, which may be infinite)
             for (int j = 0; j <= i4; ++j) {
-                const float q = P[i4 * (kSteps + 4) + j];
                 const float4 z = *reinterpret_cast<const float4*>(Z + j * kCols + w4);
-                o[0] = fmaf(q, z.x, o[0]);
-                o[1] = fmaf(q, z.y, o[1]);
-                o[2] = fmaf(q, z.z, o[2]);
-                o[3] = fmaf(q, z.w, o[3]);
+                add(0, P[i4 * (kSteps + 4) + j], z);
+                add(1, P[(i4 + kRows) * (kSteps + 4) + j], z);
             }
-            if (i4 < n) {
-                const long long at = b * r.ob + row(t0 + i4) * r.ot + h * r.oh + c0 + w4;
+            for (int j = i4 + 1; j <= i4 + kRows; ++j)
+                add(1, P[(i4 + kRows) * (kSteps + 4) + j], *reinterpret_cast<const float4*>(Z + j * kCols + w4));
 #pragma unroll
-                for (int u = 0; u < 4; ++u)
-                    if (w4 + u < nc) {
-                        if (r.out_f32) static_cast<float*>(r.out)[at + u] = o[u];
-                        else static_cast<T*>(r.out)[at + u] = from_f<T>(o[u]);
-                    }
-            }
+            for (int e = 0; e < 2; ++e)
+                if (i4 + kRows * e < n) {
+                    const long long at = b * r.ob + row(t0 + i4 + kRows * e) * r.ot + h * r.oh + c0 + w4;
+#pragma unroll
+                    for (int u = 0; u < 4; ++u)
+                        if (w4 + u < nc) {
+                            if (r.out_f32) static_cast<float*>(r.out)[at + u] = o[e][u];
+                            else static_cast<T*>(r.out)[at + u] = from_f<T>(o[e][u]);
+                        }
+                }
             __syncthreads();  // every reader of S
         }
         // S[a4 .. a4 + 3][w4 .. w4 + 3]
