@@ -667,6 +667,7 @@ MAMBA_B200_API int mamba_b200_gated_scan_bwd(void* handle, void* stream, const m
  *   backward: the states are made again.  d_state_out (NULL: zeros) is the gradient of the state that left, d_state (NULL: not
  *             written; not d_state_out) that of the one that entered.  d_q, d_k, d_v have the heads of q, k, v (gradients of shared
  *             heads are summed, in f32 and in the order of the heads) and are overwritten.  The decays have no gradient here.
+ * Results overlap no input but for state_out.
  * workspace: caller-owned scratch, 256-byte aligned, or NULL, of mamba_b200_linear_attention_workspace_bytes(args, backward) bytes (may
  *   be 0; depends on the sizes alone).  A call with fewer does not cut its sequences; the backward of shared heads needs all of it.
  *   Nothing in it is kept between calls; two calls that may run at once take one each.

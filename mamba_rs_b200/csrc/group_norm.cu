@@ -1179,6 +1179,7 @@ int check(Ctx* c, const mamba_b200_group_norm_args* a, bool bwd) {
         !aligned_to(4, {a->weight, a->bias, a->stats}) || (bwd && !aligned_to(4, {a->d_weight, a->d_bias})))
         return fail(c, MAMBA_B200_ERR_ARG, "%s: misaligned pointer", what);
     if (reinterpret_cast<uintptr_t>(a->workspace) % 256) return fail(c, MAMBA_B200_ERR_ARG, "%s: misaligned workspace", what);
+    if (bwd && a->z && a->d_z == a->d_x) return fail(c, MAMBA_B200_ERR_ARG, "%s: two results are the same memory", what);
     const long long need = mamba_b200_group_norm_workspace_bytes(a->N, a->S, a->C, a->G, bwd);
     if (need && (!a->workspace || a->workspace_bytes < need))
         return fail(c, MAMBA_B200_ERR_ARG, "%s: a workspace of %lld bytes is needed (%lld given)", what, need, a->workspace ? a->workspace_bytes : 0ll);

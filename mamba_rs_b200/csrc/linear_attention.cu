@@ -497,6 +497,13 @@ int check(Ctx* c, const mamba_b200_linear_attention_args* a, bool backward) {
         !aligned_to(4, {backward ? nullptr : a->state_out, backward ? a->d_state : nullptr, backward ? a->d_state_out : nullptr}))
         return fail(c, MAMBA_B200_ERR_ARG, "%s: misaligned pointer", what);
     if (a->workspace && reinterpret_cast<uintptr_t>(a->workspace) % 256) return fail(c, MAMBA_B200_ERR_ARG, "%s: misaligned workspace", what);
+    if (backward && a->d_state && a->d_state == a->state) return fail(c, MAMBA_B200_ERR_ARG, "%s: d_state and state are the same memory", what);
+    // (blocks of one head read what others have read: nothing may be written there)
+    for (const void* in : {a->q, a->k, a->v, backward ? a->d_o : a->q})
+        for (const void* out : {backward ? a->d_q : a->o, backward ? a->d_k : a->o, backward ? a->d_v : a->o})
+            if (some && in == out) return fail(c, MAMBA_B200_ERR_ARG, "%s: a result and an input are the same memory", what);
+    if (some && backward && (a->d_q == a->d_k || a->d_q == a->d_v || a->d_k == a->d_v))
+        return fail(c, MAMBA_B200_ERR_ARG, "%s: two results are the same memory", what);
     return MAMBA_B200_OK;
 }
 

@@ -194,6 +194,8 @@ extern "C" MAMBA_B200_API int mamba_b200_rotary(void* handle, void* stream, cons
         return fail(c, MAMBA_B200_ERR_ARG, "rotary: q_out is q with other strides");
     if (a.Hk && a.k_out == a.k && ((a.B > 1 && a.ko_b != a.k_b) || (a.T > 1 && a.ko_t != a.k_t) || (a.Hk > 1 && a.ko_h != a.k_h)))
         return fail(c, MAMBA_B200_ERR_ARG, "rotary: k_out is k with other strides");
+    if (a.Hk && (a.q_out == a.k || a.k_out == a.q || a.q_out == a.k_out))
+        return fail(c, MAMBA_B200_ERR_ARG, "rotary: a result of one of q and k is the other's memory");
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     if (a.dtype == MAMBA_B200_F32) return rot::launch_typed<float>(c, a, st);
     if (a.dtype == MAMBA_B200_F16) return rot::launch_typed<__half>(c, a, st);

@@ -88,7 +88,8 @@ def test_null_and_narrow(refused):
     assert "narrower" in refused("group_norm_fwd", norm(x=p, y=p, z=p, ld_z=7))
     # a workspace that is too small or starts between lines
     q = dict(decay=p, q=p, k=p, v=p, d_o=p, d_q=p, d_k=p, d_v=p)
-    assert "workspace" in refused("linear_attention_bwd", attention(H=2, Hq=2, Hv=2, workspace=p, workspace_bytes=16, **q))
+    apart = {n: C.c_void_p(4096 * (i + 1)) for i, n in enumerate(q)}
+    assert "need a workspace" in refused("linear_attention_bwd", attention(H=2, Hq=2, Hv=2, workspace=p, workspace_bytes=16, **apart))
     assert "misaligned workspace" in refused("linear_attention_fwd", attention(decay=p, q=p, k=p, v=p, o=p, workspace=C.c_void_p(4096 + 128)))
     assert "misaligned workspace" in refused("group_norm_bwd", norm(S=1, x=p, dy=p, d_x=p, stats=p, workspace=C.c_void_p(4096 + 128)))
     big = norm(S=100000, x=p, y=p)
@@ -113,3 +114,25 @@ def test_pointers_between_elements(refused):
             base = {n: p for n in stores + tuple(n for n in w if n in ("decay", "positions", "inv_freq", "stats"))}
             for n in stores + w:
                 assert "misaligned" in refused(name, make(dtype=dtype, **{**base, n: store if n in stores else words})), (name, n)
+
+
+def test_results_in_the_place_of_what_others_read(refused):
+    """(At one step more than the decode step's, at it, and for each pair; every other pointer is a place of its own.)"""
+    def places(names):
+        return {n: C.c_void_p(4096 * (i + 1)) for i, n in enumerate(names)}
+    for T in (1, 2):
+        p = places(("decay", "q", "k", "v", "o"))
+        for n in ("q", "k", "v"):
+            assert "same memory" in refused("linear_attention_fwd", attention(T=T, **{**p, "o": p[n]})), n
+        p = places(("decay", "q", "k", "v", "d_o", "d_q", "d_k", "d_v"))
+        for out in ("d_q", "d_k", "d_v"):
+            for n in p:
+                if n not in (out, "decay"):
+                    assert "same memory" in refused("linear_attention_bwd", attention(T=T, **{**p, out: p[n]})), (out, n)
+        p = places(("decay", "q", "k", "v", "d_o", "d_q", "d_k", "d_v", "state"))
+        assert "same memory" in refused("linear_attention_bwd", attention(T=T, d_state=p["state"], **p))
+    p = places(("positions", "inv_freq", "q", "q_out", "k", "k_out"))
+    for out, n in (("q_out", "k"), ("k_out", "q"), ("q_out", "k_out")):
+        assert "memory" in refused("rotary", rotary(**{**p, out: p[n]})), out
+    p = places(("x", "dy", "stats", "z", "d_x", "d_z"))
+    assert "same memory" in refused("group_norm_bwd", norm(**{**p, "d_z": p["d_x"]}))
