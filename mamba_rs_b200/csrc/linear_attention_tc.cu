@@ -22,8 +22,9 @@
 //
 // Roundings to 16 bits: the scores (made in f32), the weighted values beside them where they are folded, and the copy of S that is read,
 // each once, as the result is.  The state itself is f32: w o Z, which it is made of, is kept to f32 accuracy where a state is handed on:
-// three bf16 terms of 8 bits each; where only out is wanted one term is enough.  In f16 a second term of 2^-11 of the first gives 22 bits, P
-// is scaled by a power of two a row and S by one a tile, so that neither their size nor their smallness leaves the type.
+// three bf16 terms of 8 bits each; where only out is wanted one term is enough.  In f16 a second term of 2^-11 of the first gives 22 bits (down
+// to 2^-26 of a tile's largest value, fewer below), P is scaled by a power of two a row, S and w o Z by one a tile, so that neither their size
+// nor their smallness leaves the type.
 //
 // Device time of 8 x 4096 x 32 heads of 128 x 64, bf16: 126 to 130 us, 95 % of the measured copy rate (a block alone needs 2600 cycles a
 // chunk; with 148 of them HBM has them wait); its backward 449 to 461, 50 % (2200 cycles a chunk and 64 columns, of which the products
@@ -69,7 +70,8 @@ struct Small {
     float row_scale[2][128];
     float tile_scale[4];  // (a copy's is read until its rows are out, which is known of the chunk three before)
     float warp_max[2][4];
-    uint64_t full[4], empty[4], z_full[8], z_empty[8], g_full[2], p_full[2], y_full[2], y_empty[2], s_full[2], s_empty[2], w_full[8], z_read[8], d_full, d_read, max_full, drain[3];
+    float z_max[2][4], z_scale[2];  // f16: magnitudes of w o Z, and what its tile's products are multiplied by
+    uint64_t full[4], empty[4], z_full[8], z_empty[8], g_full[2], p_full[2], y_full[2], y_empty[2], s_full[2], s_empty[2], w_full[8], z_read[8], d_full, d_read, max_full, z_max_full, drain[3];
     // Values that are not finite may change no row before their own, as 0 times them in a product would: w o Z has 0 in their place, and
     // of their column the rows from the first of them on, counted as they are walked, are NaN (as is the state that leaves).
     int bad[kTile], any_bad;
@@ -77,6 +79,7 @@ struct Small {
     int dead;
 };
 constexpr int kNever = 0x7fffffff;
+static_assert(14 * kSub + sizeof(Small) <= 227 * 1024, "a block's shared memory");
 
 template <int TERMS>
 uint32_t smem_bytes(int na, int stages, int z_tiles) {
@@ -153,18 +156,27 @@ __device__ __forceinline__ float scale_to(float m, float* back) {
         *back = 1.0f;
         return 1.0f;
     }
-    const int d = min(max(e - 127 - 13, -110), 110);
+    const int d = max(e - 127 - 13, -126);
     *back = __uint_as_float(static_cast<uint32_t>(127 + d) << 23);
     return __uint_as_float(static_cast<uint32_t>(127 - d) << 23);
 }
 
-// A row of w o Z (its terms' tiles lie together) and of Z, some of whose values are not finite.
+// The largest finite magnitude of a row of an f16 tile that also holds others.
+__device__ __noinline__ float finite_max(const unsigned char* z, int row) {
+    float m = 0.0f;
+    for (int c = 0; c < kTile; ++c) {
+        const float v = fabsf(__half2float(*reinterpret_cast<const __half*>(z + sw_chunk(row, c >> 3) + 2 * (c & 7))));
+        if (v < INFINITY) m = fmaxf(m, v);
+    }
+    return m;
+}
+// A row of w o Z (its terms' tiles lie together) and of Z (which may be w o Z's first term), some of whose values are not finite.
 template <typename Th>
 __device__ __noinline__ void set_aside(unsigned char* w0, unsigned char* w1, int more, unsigned char* z, int row, int pos, Small* sm) {
     constexpr unsigned inf = std::is_same<Th, __half>::value ? 0x7c00u : 0x7f80u;
     for (int c = 0; c < kTile; ++c) {
         const uint32_t at = sw_chunk(row, c >> 3) + 2 * (c & 7);
-        if ((*reinterpret_cast<uint16_t*>(w0 + at) & inf) != inf) continue;
+        if ((*reinterpret_cast<uint16_t*>(z + at) & inf) != inf) continue;
         *reinterpret_cast<uint16_t*>(w0 + at) = 0;
         *reinterpret_cast<uint16_t*>(z + at) = 0;
         for (int t = 0; t < more; ++t) *reinterpret_cast<uint16_t*>(w1 + t * kSub + at) = 0;
@@ -238,6 +250,7 @@ __device__ __forceinline__ void walk(const TcParams& tp, unsigned char* smem, co
         for (int i = 0; i < 3; ++i) mbar_init(&sm->drain[i], 1);
         mbar_init(&sm->d_full, 1);
         mbar_init(&sm->max_full, 128);
+        mbar_init(&sm->z_max_full, 4);
         mbar_init(&sm->d_read, 128);
         sm->dead = 0;
         sm->any_bad = 0;
@@ -606,6 +619,13 @@ __device__ __forceinline__ void walk(const TcParams& tp, unsigned char* smem, co
             tmem_st32(lanes + cS + 32, none);
         }
         const Pow whole = decay_pow(ld, kChunk);
+        float undo = 1.0f;  // of the last chunk's w o Z (f16)
+        auto sum_scale = [&](int i) {
+            if (!F16) return true;
+            if (!wait_warp(&sm->w_full[i % zs], (i / zs) & 1, sm, p.status)) return false;  // (long over: the products have read what it says)
+            undo = sm->z_scale[i & 1];
+            return true;
+        };
         // 32 columns of S with the last chunk's sum
         auto read = [&](int s, float* v) {
             if (!FRESH) {
@@ -622,7 +642,7 @@ __device__ __forceinline__ void walk(const TcParams& tp, unsigned char* smem, co
                 tmem_ld32x2(lanes + cS + 32 * s, v, lanes + cD + 32 * s, d);
             }
 #pragma unroll
-            for (int c = 0; c < 32; ++c) v[c] += d[c];
+            for (int c = 0; c < 32; ++c) v[c] = F16 ? fmaf(v[c], undo, d[c]) : v[c] + d[c];
         };
         auto has_read = [&]() {
             fence_before();
@@ -635,6 +655,7 @@ __device__ __forceinline__ void walk(const TcParams& tp, unsigned char* smem, co
             const bool adds = leaves || i + 1 < n;
             if (i > 0) {
                 ok = wait_warp(&sm->d_full, (i - 1) & 1, sm, p.status);
+                if (ok) ok = sum_scale(i - 1);
                 if (!ok) break;
                 fence_after();
             }
@@ -731,6 +752,7 @@ __device__ __forceinline__ void walk(const TcParams& tp, unsigned char* smem, co
         if (ok && leaves && n > 0) {
             ok = wait_warp(&sm->d_full, (n - 1) & 1, sm, p.status);
             if (ok) ok = wait_warp(&sm->w_full[(n - 1) % zs], ((n - 1) / zs) & 1, sm, p.status);
+            if (ok) ok = sum_scale(n - 1);
             if (ok) {
                 fence_after();
                 const Pow f = !STATE && r.last_decay ? decay_pow(ld, 1) : Pow{1.0f, 0.0f};
@@ -870,9 +892,36 @@ __device__ __forceinline__ void walk(const TcParams& tp, unsigned char* smem, co
         for (int i = 0, st = 0, turn = 0; i < n; ++i) {
             const int rows = min(kChunk, p.T - start(i));
             if (!wait_warp(&sm->z_full[st], turn & 1, sm, p.status)) break;
-            if (!ahead && (TERMS > 1 || !fold) && i > 0 && !wait_warp(&sm->d_full, (i - 1) & 1, sm, p.status)) break;
-            const float f = rows == kChunk ? w_whole : row < rows ? decay_at(l2, back ? row : rows - 1 - row) * r.alpha_s : 0.0f;
+            float f = rows == kChunk ? w_whole : row < rows ? decay_at(l2, back ? row : rows - 1 - row) * r.alpha_s : 0.0f;
             unsigned char* z = smem + kZ + st * kSub;
+            float undo = 1.0f;
+            bool bad = false;
+            if (F16) {
+                // a power of two takes the tile's largest magnitude to 2^13: neither small values and weights nor those that grow leave the type
+                __half2 top = __float2half2_rn(0.0f);
+#pragma unroll 2
+                for (int j = 0; j < 8; ++j) {
+                    const uint4 v = *reinterpret_cast<const uint4*>(z + sw_chunk(row, j));
+                    const uint32_t in[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) top = __hmax2_nan(top, __habs2(*reinterpret_cast<const __half2*>(in + e)));
+                }
+                float m = __low2float(__hmax2_nan(top, __lowhigh2highlow(top)));
+                bad = !(m < INFINITY);
+                if (bad) m = finite_max(z, row);
+                m = m > 0.0f ? m * fabsf(f) : 0.0f;
+                m = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(m)));
+                if (lane == 0) {
+                    sm->z_max[i & 1][warp & 3] = m;
+                    mbar_arrive(&sm->z_max_full);
+                }
+                __syncwarp();
+                if (!wait_warp(&sm->z_max_full, i & 1, sm, p.status)) break;
+                const float* zm = sm->z_max[i & 1];
+                f *= scale_to(fmaxf(fmaxf(zm[0], zm[1]), fmaxf(zm[2], zm[3])), &undo);
+            }
+            if (!ahead && (TERMS > 1 || !fold) && i > 0 && !wait_warp(&sm->d_full, (i - 1) & 1, sm, p.status)) break;
+            if (F16 && row == 0) sm->z_scale[i & 1] = undo;  // (the sum of the chunk that had this place has been read: d_full of the one between)
             unsigned char* w0 = fold ? z : smem + kW;
             unsigned char* w1 = fold ? smem + kW - kSub : smem + kW;
             float2 zero = make_float2(0.0f, 0.0f);  // NaN, if a value is not finite
@@ -885,7 +934,7 @@ __device__ __forceinline__ void walk(const TcParams& tp, unsigned char* smem, co
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
                     float2 x = mul2(unpack2<Th>(in[e]), splat2(f));
-                    zero = fma2(x, splat2(0.0f), zero);
+                    if (!F16) zero = fma2(x, splat2(0.0f), zero);
                     o[0][e] = pack2<Th>(x.x, x.y);
 #pragma unroll
                     for (int t = 1; t < TERMS; ++t) {
@@ -910,7 +959,7 @@ __device__ __forceinline__ void walk(const TcParams& tp, unsigned char* smem, co
                     for (int j = 0; j < 8; ++j)
                         *reinterpret_cast<uint4*>(w1 + t * kSub + sw_chunk(row, j)) = kept[ahead ? t - 1 : 0][ahead ? j : 0];
             }
-            if (!(zero.x + zero.y == 0.0f)) set_aside<Th>(w0, w1 + kSub, TERMS - 1, z, row, i * kChunk + (back ? kChunk - 1 - row : row), sm);
+            if (F16 ? bad : !(zero.x + zero.y == 0.0f)) set_aside<Th>(w0, w1 + kSub, TERMS - 1, z, row, i * kChunk + (back ? kChunk - 1 - row : row), sm);
             fence_proxy_async();
             mbar_arrive(&sm->w_full[st]);
             if (++st == zs) {
@@ -993,10 +1042,6 @@ int tc_launch(Ctx* c, int dtype, Params& p, bool may_cut, long long pairs, cudaS
     using namespace tcl;
     *taken = false;
     if (dtype == MAMBA_B200_F32) return MAMBA_B200_OK;
-    // (in f16 a weight above 1 could take Z out of the type)
-    if (dtype == MAMBA_B200_F16)
-        for (int i = 0; i < p.roles; ++i)
-            if (!(fabsf(p.role[i].alpha_s) <= 1.0f)) return MAMBA_B200_OK;
     for (int i = 0; i < p.roles; ++i)
         if (p.role[i].A > 128 || p.role[i].W > 128) return MAMBA_B200_OK;
     // Roles that leave a state are kept in more terms, and those of narrow X and Y have room for more stages: up to four launches.
