@@ -660,7 +660,7 @@ MAMBA_B200_API int mamba_b200_gated_scan_bwd(void* handle, void* stream, const m
  * trapezoidal update.)  q [B, T, Hq, K], k [B, T, Hk, K], v [B, T, Hv, V] in the storage dtype, o and d_o [B, T, H, V]; each of Hq, Hk,
  * Hv divides H, and head h reads head h / (H / Hx) of a tensor with fewer.  Strides of batch, step and head in elements, the last
  * dimension contiguous (columns of one projection, say).  decay [H] f32, log of the factor a step (0: none, minus infinity: nothing is
- * kept; above 0 the state grows as the formula says).  States [B, H, K, V] f32 contiguous.  K and V are at most 256.  T = 1 is the decode
+ * kept; above 0 the state grows as the formula says, as long as exp(128 decay) is a number of f32).  States [B, H, K, V] f32 contiguous.  K and V are at most 256.  T = 1 is the decode
  * step; T = 0 hands the state on.  An infinite or NaN input changes no output of an earlier step, nor
  * of another head or sequence, and a value no other column; what does depend on it may be NaN where the formula has an infinity.
  *   forward : state (NULL: zeros) enters, state_out (NULL: not written; may be state) leaves.

@@ -34,7 +34,7 @@
 
 #include <type_traits>
 
-#include "linear_attention.cuh"
+#include "linear_attention_general.cuh"
 #include "m3_tc.cuh"
 
 namespace mb200 {
@@ -975,6 +975,18 @@ __device__ __forceinline__ void walk(const TcParams& tp, unsigned char* smem, co
     if (warp == 1) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kCols) : "memory");
 }
 
+// Heads whose state grows by more than kGrows over a chunk: the first 256 threads take the block's columns in 32 bits (a f16 tile whose weights
+// lie further apart has no digits for the small ones, and they are all there is where the first keys are zeros).
+constexpr float kGrows = 5.545f;  // 2^8
+template <typename Th, bool STATE>
+__device__ __noinline__ void grown(const TcParams& tp, unsigned char* smem, Place w) {
+    const int half = threadIdx.x / gen::kThreads;
+    w.tile = 2 * w.tile + half;
+    static_assert(kTile == 2 * gen::kCols && 2 * gen::smem_bytes(128) <= 14 * kSub, "two parts of a block");
+    if (half > 1 || w.tile * gen::kCols >= tp.p.role[w.role].W) return;
+    gen::walk<Th, 4, STATE>(tp.p, w, reinterpret_cast<float*>(smem + half * gen::smem_bytes(128)), threadIdx.x % gen::kThreads, 1 + half);
+}
+
 template <typename Th, int TERMS, bool STATE>
 __global__ void __launch_bounds__(kThreads, 1) walk_kernel(const __grid_constant__ TcParams tp) {
     extern __shared__ __align__(1024) unsigned char smem[];
@@ -987,6 +999,9 @@ __global__ void __launch_bounds__(kThreads, 1) walk_kernel(const __grid_constant
             walk<Th, TERMS, STATE, true>(tp, smem, w, ld);
             return;
         }
+    } else if (ld * (kChunk - 1) > kGrows) {
+        grown<Th, STATE>(tp, smem, w);
+        return;
     }
     walk<Th, TERMS, STATE, false>(tp, smem, w, ld);
 }
