@@ -17,8 +17,8 @@
 // and they meet on mbarriers alone; every wait gives up after a limit and takes the block to its end.
 //
 // Slow decays (`fold`, bf16): w_j = l^{n-1-j} stands in for l^{i-j} = l^{i-(n-1)} w_j too.  w o Z takes Z's place, P is G with its future cut
-// off, and l^{i-(n-1)} is one factor a row of the result, in 32 bits.  Fast ones, whose l^{-127} leaves the numbers that 32 bits hold with
-// room to spare, and f16 weigh P instead.
+// off, and l^{i-(n-1)} is one factor a row of the result, in 32 bits.  Fast ones, whose l^127 takes the first rows' products far
+// below their size (kSlow), and f16 weigh P instead.
 //
 // Roundings to 16 bits: the scores (made in f32), the weighted values beside them where they are folded, and the copy of S that is read,
 // each once, as the result is.  The state itself is f32: w o Z, which it is made of, is kept to f32 accuracy where a state is handed on:
@@ -60,8 +60,10 @@ struct TcParams {
 template <int TERMS>
 constexpr int kCopies = TERMS == 1 ? 2 : 1;
 constexpr int kTiles = 6;  // beside two stages of X and Y of two sub-tiles, or four of one
-// A chunk's smallest weight is above e^-kSlow where w o Z stands in for Z.
-constexpr float kSlow = 40.0f;
+// A chunk's smallest weight is above e^-kSlow = 2^-8 where w o Z stands in for Z: the first rows' products are that much smaller than the
+// formula's, and one of 2^-126 still has 15 bits (a limit of e^-40 lost those below 3e-21.  Decays from 1 / 1.4 to 1 / 256 a step, of which this
+// limit weighs half and that one a sixth, 8 x 4096 x 32 heads of 128 x 64: 187 us for 180, backward 640 for 580).
+constexpr float kSlow = 5.545f;
 
 // behind the stages, the terms of w o Z and the copies of S
 struct Small {
@@ -993,7 +995,7 @@ __global__ void __launch_bounds__(kThreads, 1) walk_kernel(const __grid_constant
     const Place w = place(tp.p, blockIdx.x, STATE ? tp.p.segments - 1 : tp.p.segments);
     const float ld = tp.p.decay[w.pair % tp.p.H];
     // `fold`: w o Z takes Z's place and P is G with its future cut off; what is missing, l^{row} up to a constant, is one factor a row of the
-    // result.  Not where l^{-127} leaves the numbers that 32 bits hold with room to spare, nor in f16.
+    // result.  Not where l^127 is small (kSlow), nor in f16.
     if constexpr (!std::is_same<Th, __half>::value) {
         if (ld <= 0.0f && ld * (kChunk - 1) >= -kSlow) {
             walk<Th, TERMS, STATE, true>(tp, smem, w, ld);
