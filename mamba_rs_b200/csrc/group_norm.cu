@@ -1179,6 +1179,16 @@ int check(Ctx* c, const mamba_b200_group_norm_args* a, bool bwd) {
         !aligned_to(4, {a->weight, a->bias, a->stats}) || (bwd && !aligned_to(4, {a->d_weight, a->d_bias})))
         return fail(c, MAMBA_B200_ERR_ARG, "%s: misaligned pointer", what);
     if (reinterpret_cast<uintptr_t>(a->workspace) % 256) return fail(c, MAMBA_B200_ERR_ARG, "%s: misaligned workspace", what);
+    // (a thread writes where it has read: with other strides it would write where others have yet to read)
+    struct Rows {
+        const void* p;
+        long long ld;
+    };
+    if (static_cast<long long>(a->N) * a->S > 1)
+        for (const Rows& in : {Rows{a->x, a->ld_x}, Rows{a->z, a->ld_z}, bwd ? Rows{a->dy, a->ld_dy} : Rows{nullptr, 0}})
+            for (const Rows& out : {bwd ? Rows{a->d_x, a->ld_dx} : Rows{a->y, a->ld_y}, bwd && a->z ? Rows{a->d_z, a->ld_dz} : Rows{nullptr, 0}})
+                if (in.p && in.p == out.p && in.ld != out.ld)
+                    return fail(c, MAMBA_B200_ERR_ARG, "%s: a result is an input with other strides", what);
     if (bwd && a->z && a->d_z == a->d_x) return fail(c, MAMBA_B200_ERR_ARG, "%s: two results are the same memory", what);
     const long long need = mamba_b200_group_norm_workspace_bytes(a->N, a->S, a->C, a->G, bwd);
     if (need && (!a->workspace || a->workspace_bytes < need))
