@@ -893,7 +893,8 @@ __global__ void __launch_bounds__(kSlabThreads) slab_kernel(const Params p) {
                 }
             const float off = group_sum<T, VEC>(p, c, s1, per_thread, per_group) * inv;
             mean += off;
-            rstd = rsqrtf(fmaxf(fmaf(-off, off, group_sum<T, VEC>(p, c, s2, per_thread, per_group) * inv), 0.0f) + a.eps);
+            const float var = fmaf(-off, off, group_sum<T, VEC>(p, c, s2, per_thread, per_group) * inv);
+            rstd = rsqrtf((var < 0.0f ? 0.0f : var) + a.eps);  // (a NaN stays one)
             if (c.on && a.stats && c.r == 0 && c.col == c.g * p.per) {
                 a.stats[static_cast<long long>(ns) * a.G + c.g] = mean;
                 a.stats[NG + static_cast<long long>(ns) * a.G + c.g] = rstd;
