@@ -660,9 +660,14 @@ MAMBA_B200_API int mamba_b200_gated_scan_bwd(void* handle, void* stream, const m
  * trapezoidal update.)  q [B, T, Hq, K], k [B, T, Hk, K], v [B, T, Hv, V] in the storage dtype, o and d_o [B, T, H, V]; each of Hq, Hk,
  * Hv divides H, and head h reads head h / (H / Hx) of a tensor with fewer.  Strides of batch, step and head in elements, the last
  * dimension contiguous (columns of one projection, say).  decay [H] f32, log of the factor a step (0: none, minus infinity: nothing is
- * kept; above 0 the state grows as the formula says, as long as exp(128 decay) is a number of f32).  States [B, H, K, V] f32 contiguous.  K and V are at most 256.  T = 1 is the decode
- * step; T = 0 hands the state on.  An infinite or NaN input changes no output of an earlier step, nor
- * of another head or sequence, and a value no other column; what does depend on it may be NaN where the formula has an infinity.
+ * kept; above 0 the state grows as the formula says, as long as exp(128 decay) is a number of f32).  States [B, H, K, V] f32
+ * contiguous.  K and V are at most 256.  T = 1 is the decode step; T = 0 hands the state on.  An infinite or NaN input changes no output
+ * of an earlier step, nor of another head or sequence, and a value no other column; what does depend on it may be NaN where the formula
+ * has an infinity.
+ * Sums and states are f32.  Whole texts of 16-bit types with K, V <= 128 round to that type, once each: the scores, the copy of a state that
+ * is read, and, where no state leaves, the weighted values that it is made of (so the last bits of o and d_v depend on whether state_out
+ * and d_state are asked for).  What a step adds to a state that leaves is kept to 2^-22 of itself, in f16 at most to 2^-48 of the largest
+ * weighted value among its 128 steps, and an f16 score to 2^-39 of the largest in its row of them.
  *   forward : state (NULL: zeros) enters, state_out (NULL: not written; may be state) leaves.
  *   backward: the states are made again.  d_state_out (NULL: zeros) is the gradient of the state that left, d_state (NULL: not
  *             written; not d_state_out) that of the one that entered.  d_q, d_k, d_v have the heads of q, k, v (gradients of shared

@@ -8,12 +8,14 @@
 //  * rows: S = 1, a group fits a block.  A thread owns the same channels of row after row, the next of which are on their way to
 //    shared memory; a group's sums are shuffles (and a barrier where it takes more than a warp), the variance is taken around the mean
 //    from registers, and the backward's sums over rows stay in registers until the block's end.  32768 rows of 2048 channels in 32
-//    groups, gated, bf16: 75 to 79 us, 80 % of the measured copy rate (84 with activation and gate looked up for every value, 118 without
-//    the rows on their way); backward 128, 81 %.
-//  * samples that fit shared memory: one kernel, every element read once.  3 samples of 1021 rows of 768 channels, f32: 13 us (18.5 in two kernels).
+//    groups, gated, bf16: 75 to 84 us, 75 to 84 % of the measured copy rate (where it was 79: 84 with activation and gate looked up for every
+//    value, 118 without the rows on their way); backward 128 to 134, 78 to 81 %.  Calls one after another: 80 to 86 and 134 to 139.
+//  * samples that fit shared memory: one kernel, every element read once.  3 samples of 1021 rows of 768 channels, f32: 13 to 14 us
+//    (18.5 in two kernels), backward 31 to 33.
 //  * other samples: a first kernel leaves mean and squared deviations (backward: the sums) of each block of rows and group, joined
 //    pairwise around their means, and a second one joins the blocks of its groups in their order and goes over the rows again, which
-//    L2 has where they fit it.
+//    L2 has where they fit it.  8 samples of 16384 rows of 512 channels, SiLU, bf16: 212 us, 19 % of the copy rate by the bytes of one
+//    pass; backward 309.
 #include <math.h>
 #include <string.h>
 

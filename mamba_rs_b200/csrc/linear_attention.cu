@@ -11,8 +11,8 @@ namespace la {
 // ---------------------------------------------------------------------------------------------------
 // One token for each sequence.  S is read and written once (K * V * 8 bytes a head, beside which nothing counts), so a thread has
 // four columns of it (one, where V is no multiple of four) and every row of its row group in flight; the groups' parts of o
-// are joined through shared memory in their order.  64 sequences x 32 heads of 128 x 64 bf16 take 23.0 us, 90 % of
-// the measured copy rate; 32 heads of one sequence 2.8.
+// are joined through shared memory in their order.  64 sequences x 32 heads of 128 x 64 bf16 take 21.2 to 23.0 us, 90 % of
+// the measured copy rate and more (the last states are still in L2 when it ends); 32 heads of one sequence 3.2.
 // ---------------------------------------------------------------------------------------------------
 constexpr int kStepThreads = 256;
 

@@ -26,9 +26,11 @@
 // to 2^-26 of a tile's largest value, fewer below), P is scaled by a power of two a row, S and w o Z by one a tile, so that neither their size
 // nor their smallness leaves the type.
 //
-// Device time of 8 x 4096 x 32 heads of 128 x 64, bf16: 126 to 130 us, 95 % of the measured copy rate (a block alone needs 2600 cycles a
-// chunk; with 148 of them HBM has them wait); its backward 449 to 461, 50 % (2200 cycles a chunk and 64 columns, of which the products
-// and the rows' warps are busy for most).  What the steps gave is told where it matters.
+// Device time of 8 x 4096 x 32 heads of 128 x 64, bf16: 127 to 134 us, 92 to 97 % of the measured copy rate (a block alone needs 2600 cycles a
+// chunk; with 148 of them HBM has them wait); its backward 458 to 482, 47 to 49 % (2200 cycles a chunk and 64 columns, of which the products
+// and the rows' warps are busy for most).  Calls one after another, each on inputs of its own, take 142 to 152 and 532 to 563.  f16: 265 to 275, its
+// backward 1125 to 1165 (weights, scores and states are looked over once more for their magnitudes, and nothing is folded).
+// What the steps gave is told where it matters.
 #include <math.h>
 #include <string.h>
 
@@ -1053,8 +1055,8 @@ int launch(Ctx* c, TcParams& tp, long long pairs, cudaStream_t st) {
 }  // namespace tcl
 
 // Takes the call where the tensor cores' kernel can: 16-bit types, both widths up to 128, tensors that TMA can describe.  A tile has 128 rows
-// whatever T is, and still a few steps take less than in the general kernel's chunks of 32: 2 of 32 heads of 128 x 64 5.7 us (8.0 there), with
-// states 9.1 (14.3), 64 sequences of 32 steps with states 131 (372).
+// whatever T is, and still a few steps take less than in the general kernel's chunks of 32: 2 of 32 heads of 128 x 64 5.8 us (8.0 there), with
+// states 8.8 (14.3), 64 sequences of 32 steps with states 123 (372).
 int tc_launch(Ctx* c, int dtype, Params& p, bool may_cut, long long pairs, cudaStream_t st, bool* taken) {
     using namespace tcl;
     *taken = false;

@@ -5,8 +5,8 @@
 // One read and one write of every element, so HBM bounds it if instructions do not.  A thread owns one place in the head (16 bytes of
 // pairs, or of columns that are handed on) of one token, makes that place's sines and cosines once, and goes through heads of q and k with
 // them, four in flight, by pointers that go on by a head.  A block has places of pairs first and places to be handed on behind them, so that
-// warps do one or the other.  The angle is reduced to turns in 64 bits: at position 10^6 its 32-bit product is off by 2^-5 of a turn, in
-// 64 bits by 2^-33.  8 x 4096 tokens, 2 x 32 heads of 128 columns, bf16, 64 of them turned: 174 us,
+// warps do one or the other.  The angle is reduced to turns in 64 bits: at position 10^6 its 32-bit product is off by 2^-5 of a radian, in
+// 64 bits by 2^-34.  8 x 4096 tokens, 2 x 32 heads of 128 columns, bf16, 64 of them turned: 174 us,
 // 6.2 TB/s (250 with places of both kinds in a warp and addresses made for every head).
 #include <math.h>
 #include <string.h>

@@ -917,7 +917,8 @@ def linear_attention_fwd(q, k, v, decay, *, scale=None, state=None, state_out=No
     each head's factor a token; Hq, Hk and Hv divide H (fewer heads are shared by consecutive ones); K, V <= 256; scale: K ** -0.5
     if None.  state [B,H,K,V] f32 enters (zeros if None), state_out receives what leaves (may be state).  workspace: scratch of
     linear_attention_workspace_bytes(...) bytes (made here if None).  Returns o [B,T,H,V] in q's dtype.  An infinite or NaN input
-    changes no earlier token's output; what depends on it may be NaN where the formula has an infinity."""
+    changes no earlier token's output; what depends on it may be NaN where the formula has an infinity.  16-bit types keep a state that
+    leaves in more digits than one that does not, so the last bits of o depend on whether state_out is asked for."""
     dev = _device_index(q, k, v, decay, state, state_out, o, workspace)
     a, shape = _attention_args(q, k, v, decay, scale, state)
     B, H, _, V = shape
