@@ -667,7 +667,7 @@ MAMBA_B200_API int mamba_b200_gated_scan_bwd(void* handle, void* stream, const m
  * Sums and states are f32.  Whole texts of 16-bit types with K, V <= 128 round to that type, once each: the scores, the copy of a state that
  * is read, and, where no state leaves, the weighted values that it is made of (so the last bits of o and d_v depend on whether state_out
  * and d_state are asked for).  What a step adds to a state that leaves is kept to 2^-22 of itself, in f16 at most to 2^-48 of the largest
- * weighted value among its 128 steps, and an f16 score to 2^-39 of the largest in its row of them.
+ * weighted value among its 128 steps, and an f16 score to 2^-38 of the largest in its row of them (2^-30 where the state grows).
  *   forward : state (NULL: zeros) enters, state_out (NULL: not written; may be state) leaves.
  *   backward: the states are made again.  d_state_out (NULL: zeros) is the gradient of the state that left, d_state (NULL: not
  *             written; not d_state_out) that of the one that entered.  d_q, d_k, d_v have the heads of q, k, v (gradients of shared
